@@ -331,6 +331,112 @@ int llmx_lm_head_argmax_device(const int16_t *hidden, uint32_t rows, uint32_t hi
                                void *stream);
 
 /* ---------------------------------------------------------------------------
+ * A projection shared by many requests, with each row's own low-rank adapter
+ * beside it (no counterpart in the reference, which serves one model's weights
+ * to one sequence).  For rows x (Q8.8) and the shared weight W (Q4.12):
+ *
+ *   t[i][j] = sat16(rnd24(scale_a * sum_k down_a[j][k] x[i][k]))     Q8.8
+ *   y[i][n] = sum_k W[n][k] x[i][k] + sum_j up_a[n][j] t[i][j]       exact, Q20
+ *
+ * with a = slot[i]; down_a, up_a and scale_a are Q4.12, rndk(v) =
+ * floor(v / 2^k + 1/2).  y is rounded once, as every projection here is
+ * (golden_projection host:3105-3142): sat16(rnd8(sat32(rnd4(y)))) as Q8.8, or
+ * only sat32(rnd4(y)) as Q16.16 (an LM head's logits).  The results are exact
+ * integers: they do not depend on the number of rows, their order or the grid.
+ * ------------------------------------------------------------------------- */
+typedef struct llmx_adapters llmx_adapters;
+#define LLMX_OUT_Q8_8 0   /* int16 rows */
+#define LLMX_OUT_Q16_16 1 /* int32 rows */
+/* Lays out a shared weight (device, dense [out_dim][in_dim] int16, 16-byte
+ * aligned) for the kernels and allocates room for `slots` adapters of rank <=
+ * max_rank (none set yet) and for calls of up to max_rows rows.  The layout is
+ * made in stream order: keep `weight` until the stream has passed this call;
+ * it is not used afterwards.  in_dim: a multiple of 8 up to 32768; out_dim: 1
+ * to 2^22; slots: 0 to 65536; max_rank: 1 to 128 (any value when slots is 0);
+ * max_rows: 1 to 65536. */
+int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_dim, const int16_t *weight,
+                         uint32_t slots, uint32_t max_rank, uint32_t max_rows, void *stream,
+                         llmx_adapters **out);
+int llmx_adapters_destroy(llmx_adapters *a);
+/* Puts an adapter into a slot in stream order: down [rank][in_dim] (16-byte
+ * aligned), up [out_dim][rank], device, dense.  rank 0 empties the slot (down and up may
+ * then be NULL). */
+int llmx_adapters_set(llmx_adapters *a, uint32_t slot, uint32_t rank, int16_t scale,
+                      const int16_t *down, const int16_t *up, void *stream);
+/* One call on `rows` rows (0 to max_rows), stream-ordered; allocates nothing
+ * and may be captured into a graph.
+ *   x     device, int16 rows ld_x elements apart (0 = in_dim; a multiple of 8
+ *         otherwise), 16-byte aligned
+ *   slot  device, int32 per row, or NULL: no adapters.  A row whose slot is
+ *         empty or outside [0, slots) has no adapter
+ *   out   device, rows ld_out elements apart (0 = out_dim), format LLMX_OUT_*
+ * The handle's workspace is shared by its calls: order calls that use one
+ * handle on one stream or with events.  A bounded wait that expired in a
+ * kernel is reported by llmx_adapters_error. */
+int llmx_adapters_project(llmx_adapters *a, const int16_t *x, uint32_t rows, size_t ld_x,
+                          const int32_t *slot, void *out, int out_format, size_t ld_out, void *stream);
+/* Waits for the stream and returns LLMX_ERR_TIMEOUT if a kernel of this handle
+ * gave up a wait since the last such call (its results are void), else LLMX_OK. */
+int llmx_adapters_error(llmx_adapters *a, void *stream);
+/* Bytes of device memory the handle holds. */
+uint64_t llmx_adapters_device_bytes(const llmx_adapters *a);
+
+/* ---------------------------------------------------------------------------
+ * Verification of drafted tokens: rejection sampling from the target's
+ * probabilities with random numbers that the caller gives (no counterpart in
+ * the reference, which decodes greedily).  One call serves `requests` requests;
+ * request b has k_b = offsets[b+1] - offsets[b] drafts (0 = it only samples).
+ *
+ * A row of Q16.16 logits z at temperature T becomes whole-number weights
+ *   e[v] = (max - z[v]) * (log2(e) / 2^16 / T), capped at 100    (32-bit steps)
+ *   w[v] = floor(2^31 * 2^-e[v])
+ * where 2^x = 2^round(x) (1 + f (c0 + f (c1 + f (c2 + f (c3 + f c4))))), every
+ * step rounded to binary32 (relative error below 2e-7), and Q0.40
+ * probabilities
+ *   P[v] = (w[v] * floor(2^62 / (S >> h))) >> (22 + h),  S = sum w,
+ * h such that 2^31 <= S >> h < 2^32.  A logit of INT32_MIN excludes its token
+ * (w = 0); T <= 1e-6 (or NaN) is greedy: w = 2^31 at the first maximum, else 0.
+ * Draft j (token x_j) is accepted while U_j * Q[x_j] < 2^32 * P[x_j], Q from the
+ * draft model's row (2^40 at x_j where there is none).  After the first
+ * rejection one token of max(0, P - Q) follows (of P if that is all zero), after k_b
+ * acceptances one of the last row's P: the first v whose running sum exceeds
+ * floor(V * total / 2^32).  U and V are uniform 32-bit numbers.  A row that
+ * excludes every token yields the token 0xffffffff.  Sums are exact, so the
+ * tokens depend on no order of summation.
+ * ------------------------------------------------------------------------- */
+/* Bytes of workspace for a call of these sizes. */
+size_t llmx_verify_workspace_bytes(uint32_t requests, uint32_t drafts, uint32_t vocab);
+/*   target        device, int32 rows ld_target elements apart (0 = vocab): request b's
+ *                 k_b + 1 rows start at row offsets[b] + b
+ *   draft         device, int32 rows ld_draft elements apart (0 = vocab): request b's
+ *                 k_b rows start at row offsets[b]; NULL = the drafts have no
+ *                 distribution (copied from a prompt, say)
+ *   vocab         1 to 2^22
+ *   draft_tokens  device, [drafts] (NULL when drafts is 0); one outside the vocabulary
+ *                 is rejected
+ *   offsets       device, [requests + 1], offsets[0] = 0, offsets[requests] = drafts; a request
+ *                 whose pair of offsets is out of order, outside [0, drafts] or more than
+ *                 max_drafts apart gets accepted = 0xffffffff and no tokens
+ *   requests      1 to 65535, drafts: their sum of k_b, max_drafts: the largest k_b (0 to 1023)
+ *   temperature   device, float per request
+ *   accept_u      device, [drafts] (NULL when drafts is 0); sample_u device, [requests]
+ *   tokens        device, [requests][max_drafts + 1]: the accepted drafts, the drawn
+ *                 token, then 0xffffffff
+ *   accepted      device, [requests]: accepted drafts of each request
+ *   probs         device, [drafts][2]: P and Q of each drafted token (Q0.40), or NULL
+ *   workspace     device, 256-byte aligned, llmx_verify_workspace_bytes of the
+ *                 same sizes (or larger ones); one call at a time may use it
+ * Rows whose length or stride is not a multiple of 4, or whose base is not 16-byte
+ * aligned, are served with narrower loads.  Stream-ordered, allocates nothing,
+ * may be captured into a graph. */
+int llmx_verify_drafts(const int32_t *target, size_t ld_target, const int32_t *draft, size_t ld_draft,
+                       uint32_t vocab, const uint32_t *draft_tokens, const uint32_t *offsets,
+                       uint32_t requests, uint32_t drafts, uint32_t max_drafts,
+                       const float *temperature, const uint32_t *accept_u, const uint32_t *sample_u,
+                       uint32_t *tokens, uint32_t *accepted, uint64_t *probs, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/* ---------------------------------------------------------------------------
  * Host runtime: qwen_executor_t host:7607-8161
  * ------------------------------------------------------------------------- */
 /* run_prompt_block host:7840-7918: embedding rows of 1..8 tokens at

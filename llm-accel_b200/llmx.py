@@ -35,6 +35,7 @@ OP_DECODER_LAYER, OP_ATTN_PREFILL_BLOCK = 16, 17
 FEATURE_OPS = tuple(range(1, 11))
 AR_NONE, AR_NCCL, AR_PEER = 0, 1, 2
 MAX_ROWS = 8
+OUT_Q8_8, OUT_Q16_16 = 0, 1
 KERNEL_QKV, KERNEL_ATTN, KERNEL_O, KERNEL_GATE_UP, KERNEL_DOWN, KERNEL_FINAL_NORM = range(6)
 
 
@@ -138,6 +139,16 @@ def lib():
             "llmx_run_prompt_block": (C.c_int, [vp, vp, u32p, C.c_uint32, C.c_uint32, C.c_int, i16p]),
             "llmx_run_token": (C.c_int, [vp, vp, C.c_uint32, C.c_uint32, i16p]),
             "llmx_lm_head_argmax_device": (C.c_int, [vp, C.c_uint32, C.c_uint32, vp, C.c_uint32, vp, vp]),
+            "llmx_adapters_create": (C.c_int, [C.c_int, C.c_uint32, C.c_uint32, vp, C.c_uint32, C.c_uint32,
+                                               C.c_uint32, vp, C.POINTER(vp)]),
+            "llmx_adapters_destroy": (C.c_int, [vp]),
+            "llmx_adapters_set": (C.c_int, [vp, C.c_uint32, C.c_uint32, C.c_int16, vp, vp, vp]),
+            "llmx_adapters_project": (C.c_int, [vp, vp, C.c_uint32, C.c_size_t, vp, vp, C.c_int, C.c_size_t, vp]),
+            "llmx_adapters_error": (C.c_int, [vp, vp]),
+            "llmx_adapters_device_bytes": (C.c_uint64, [vp]),
+            "llmx_verify_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
+            "llmx_verify_drafts": (C.c_int, [vp, C.c_size_t, vp, C.c_size_t, C.c_uint32, vp, vp, C.c_uint32,
+                                             C.c_uint32, C.c_uint32, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
             "llmx_upload_vocab": (C.c_int, [vp, vp]),
             "llmx_allreduce_kind": (C.c_int, [vp]),
             "llmx_decode_fuses_o": (C.c_int, [vp]),
@@ -286,6 +297,58 @@ def lm_head_argmax_device(hidden_ptr, rows, hidden_size, lm_head_ptr, vocab, tok
     Returns the status code without raising."""
     return lib().llmx_lm_head_argmax_device(hidden_ptr, rows, hidden_size, lm_head_ptr, vocab, tokens_ptr,
                                             stream)
+
+
+class Adapters:
+    """llmx_adapters: a projection shared by many requests, with each row's own
+    low-rank adapter beside it.  Pointers are device pointers (ints)."""
+
+    def __init__(self, in_dim, out_dim, weight_ptr, slots, max_rank, max_rows, device=0, stream=None):
+        self.h = C.c_void_p()
+        check(lib().llmx_adapters_create(device, in_dim, out_dim, weight_ptr, slots, max_rank, max_rows, stream,
+                                         C.byref(self.h)), "adapters_create")
+
+    def close(self):
+        if self.h:
+            lib().llmx_adapters_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def set(self, slot, rank, scale=4096, down_ptr=None, up_ptr=None, stream=None):
+        """Puts an adapter (down [rank][in_dim], up [out_dim][rank], scale Q4.12)
+        into a slot; rank 0 empties it."""
+        check(lib().llmx_adapters_set(self.h, slot, rank, scale, down_ptr, up_ptr, stream), "adapters_set")
+
+    def project(self, x_ptr, rows, slot_ptr, out_ptr, out_format=OUT_Q8_8, ld_x=0, ld_out=0, stream=None):
+        check(lib().llmx_adapters_project(self.h, x_ptr, rows, ld_x, slot_ptr, out_ptr, out_format, ld_out, stream),
+              "adapters_project")
+
+    def error(self, stream=None):
+        """Waits for the stream; raises when a kernel of this handle gave up a wait."""
+        check(lib().llmx_adapters_error(self.h, stream), "adapters_error")
+
+    @property
+    def device_bytes(self):
+        return lib().llmx_adapters_device_bytes(self.h)
+
+
+def verify_workspace_bytes(requests, drafts, vocab):
+    return lib().llmx_verify_workspace_bytes(requests, drafts, vocab)
+
+
+def verify_drafts(target_ptr, draft_ptr, vocab, draft_tokens_ptr, offsets_ptr, requests, drafts, max_drafts,
+                  temperature_ptr, accept_u_ptr, sample_u_ptr, tokens_ptr, accepted_ptr, probs_ptr, workspace_ptr,
+                  workspace_bytes, ld_target=0, ld_draft=0, stream=None):
+    """llmx_verify_drafts on device pointers (ints); allocates nothing."""
+    check(lib().llmx_verify_drafts(target_ptr, ld_target, draft_ptr, ld_draft, vocab, draft_tokens_ptr, offsets_ptr,
+                                   requests, drafts, max_drafts, temperature_ptr, accept_u_ptr, sample_u_ptr,
+                                   tokens_ptr, accepted_ptr, probs_ptr, workspace_ptr, workspace_bytes, stream),
+          "verify_drafts")
 
 
 def tp_unique_id() -> bytes:
