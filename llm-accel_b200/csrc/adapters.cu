@@ -66,11 +66,12 @@ constexpr uint32_t kMaxIn = 32768, kMaxOut = 1u << 22, kMaxSlots = 65536, kMaxRa
 constexpr int kOutTile = 128;             // outputs per tile (TMEM lanes) and inputs per item
 constexpr int kRowTile = 128;          // most rows per tile: 4 sums x 128 rows = all 512 TMEM columns
 constexpr int kPiece = 2 * kOutTile * 16; // bytes of a weight piece: two planes of 128 x 16
-constexpr int kItem = 8 * kPiece;
-constexpr int kProjectThreads = 6 * 32;
-constexpr int kHeader = 3072;          // barriers, flags, row-tile table at the start of shared memory
-constexpr int kMaxRing = 8;
-static_assert(192 + (kMaxCallRows / kRowTile + 1) * 4 <= kHeader, "the row-tile table lies in the header");
+constexpr int kProjectSmem = 221 * 1024;
+constexpr int kProjectThreads = 10 * 32; // TMEM + products, loads, 8 warps of results
+constexpr int kHeader = 16 * 16 + 96;  // barriers and flags at the start of shared memory, then the row-tile tables
+constexpr int kMaxRing = 16;
+constexpr int kResultThreads = 256;
+constexpr int kMoreTiles = 3;          // row tiles beyond the fewest that a call may take
 constexpr int kGroup = 8;              // rows of one adapter that share a pass over its down matrix
 
 // What the kernels need of a handle and a call.
@@ -82,24 +83,29 @@ struct Call {
     size_t ld_out;
     uint32_t rows;
     int wide;
-    int K, C, T, N;       // inputs, chunks of 128, tiles of 128 outputs, outputs
+    int K, P, T, N;       // inputs, pieces of 16 (a multiple of 8), tiles of 128 outputs, outputs
+    int D, C;             // pieces per ring stage, stages of a tile's weight
     int NT, RT;           // rows per row tile (a multiple of 16), row tiles
     int slots, Q;         // pieces reserved per adapter
-    int max_pieces;       // adapter pieces of one row tile at most (even)
+    int max_pieces;       // adapter pieces of one row tile at most
+    int span, ranks, ksplit; // k_prepare: rows and ranks per block of t, blocks of a cluster that share k
     int down_words;       // 32-bit words of one down row
-    const uint8_t *weight; // items [T][C]
+    const uint8_t *weight; // pieces [T][P]
     const int32_t *wsum;   // [T * 128] sums of the weights of an output
     const uint8_t *up;     // pieces [slots][T][Q]
     const uint32_t *down;  // [slots][16 Q][K / 2] words {lo(w0), lo(w1), hi(w0), hi(w1)}
     const int32_t *rank, *scale;
-    uint8_t *xp;           // row pieces [RT][C][8]
-    uint8_t *tp;           // t pieces [RT][max_pieces]
-    int32_t *list;         // [RT][max_pieces] slot * Q + piece
+    uint8_t *xp;           // row pieces [RT][P]
+    uint8_t *tp;           // t pieces [RT][NT first rows][Q]
+    const uint8_t *zero;   // a piece of zeros
+    int2 *list;            // [RT][max_pieces] {slot * Q + piece, first row * Q + piece}
     int32_t *count;        // [RT] pieces
     int64_t *acc;          // [grid][NT][128] sums of tiles cut between CTAs, zero between calls
     int32_t *arrived;      // [grid]
     int *error;
     int ring, buffers;     // ring stages, accumulator sets
+    int shared_tiles;      // tiles whose stages are shared by several CTAs
+    int sharers;           // CTAs that share them
 };
 
 static __device__ __forceinline__ int slot_of(const Call &c, uint32_t row) {
@@ -109,33 +115,68 @@ static __device__ __forceinline__ int slot_of(const Call &c, uint32_t row) {
 }
 static __device__ __forceinline__ int pieces_of(const Call &c, int a) { return a >= 0 ? (c.rank[a] + 15) >> 4 : 0; }
 
-// The adapters of one row tile.  Thread t < 128 stands for row t of the tile:
-// its slot, its place among the rows of that slot, and where that adapter's
-// pieces start in the tile's list (adapters in the order of their first rows).
+// The rows of tile rt that have slot a, as a bit per row, in every lane of a warp.
+struct RowMask {
+    uint32_t w[kRowTile / 32];
+    __device__ __forceinline__ int first() const {
+        for (int k = 0; k < kRowTile / 32; k++)
+            if (w[k]) return k * 32 + __ffs((int)w[k]) - 1;
+        return -1;
+    }
+    __device__ __forceinline__ int before(int at) const {  // rows of the mask below row at
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < kRowTile / 32; k++) {
+            const int top = at - k * 32;
+            n += __popc(top >= 32 ? w[k] : top > 0 ? w[k] & ((1u << top) - 1) : 0u);
+        }
+        return n;
+    }
+};
+static __device__ __forceinline__ RowMask rows_of_slot(const Call &c, int rt, int a) {
+    const int lane = threadIdx.x & 31;
+    int32_t v[kRowTile / 32];
+#pragma unroll
+    for (int k = 0; k < kRowTile / 32; k++) {
+        const uint32_t row = (uint32_t)rt * c.NT + k * 32 + lane;
+        v[k] = k * 32 + lane < c.NT && row < c.rows ? c.slot[row] : -1;
+    }
+    RowMask m;
+#pragma unroll
+    for (int k = 0; k < kRowTile / 32; k++) m.w[k] = __ballot_sync(~0u, v[k] == a);
+    return m;
+}
+
+// The adapters of one row tile, by a block of at least 128 threads.  Thread t <
+// 128 stands for row t: whether it is the first row of its adapter, and where
+// that adapter's pieces start in the tile's list.  total: pieces of the tile.
 struct TileSlots {
-    int32_t slot[kRowTile], base[kRowTile];
+    int4 slot[kRowTile / 4];
     int32_t warp_sum[4];
 };
 struct RowSlot {
-    int slot, order, base, total;
+    int slot, base, total;
+    bool first;
 };
 static __device__ RowSlot tile_slots(const Call &c, int rt, TileSlots &s) {
     const int t = threadIdx.x, lane = t & 31;
-    RowSlot r{-1, 0, 0, 0};
+    RowSlot r{-1, 0, 0, false};
+    int own = 0, scan = 0;
     if (t < kRowTile) {
         r.slot = t < c.NT ? slot_of(c, (uint32_t)rt * c.NT + t) : -1;
-        s.slot[t] = r.slot;
+        reinterpret_cast<int32_t *>(s.slot)[t] = r.slot;
+        own = pieces_of(c, r.slot);
     }
     __syncthreads();
-    int leader = t, scan = 0, own = 0;
     if (t < kRowTile) {
-        if (r.slot >= 0)
-            for (int u = 0; u < t; u++)
-                if (s.slot[u] == r.slot) {
-                    if (r.order == 0) leader = u;
-                    r.order++;
-                }
-        own = r.order == 0 ? pieces_of(c, r.slot) : 0;
+        bool seen = r.slot < 0;
+        for (int u = 0; u < c.NT; u += 4) {
+            const int4 v = s.slot[u >> 2];
+            seen |= (v.x == r.slot && u < t) | (v.y == r.slot && u + 1 < t) | (v.z == r.slot && u + 2 < t) |
+                    (v.w == r.slot && u + 3 < t);
+        }
+        r.first = !seen;
+        if (seen) own = 0;
         scan = own;
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(~0u, scan, o);
@@ -145,12 +186,9 @@ static __device__ RowSlot tile_slots(const Call &c, int rt, TileSlots &s) {
     }
     __syncthreads();
     if (t < kRowTile) {
-        int before = 0;
-        for (int w = 0; w < (t >> 5); w++) before += s.warp_sum[w];
-        s.base[t] = before + scan - own;
+        for (int w = 0; w < (t >> 5); w++) r.base += s.warp_sum[w];
+        r.base += scan - own;
     }
-    __syncthreads();
-    if (t < kRowTile) r.base = s.base[leader];
     r.total = s.warp_sum[0] + s.warp_sum[1] + s.warp_sum[2] + s.warp_sum[3];
     return r;
 }
@@ -159,7 +197,7 @@ static __device__ RowSlot tile_slots(const Call &c, int rt, TileSlots &s) {
 // rows -> byte planes, t -> byte planes, the lists of adapter pieces
 // ---------------------------------------------------------------------------
 static __device__ void split_item(const Call &c, int item) {
-    const int rt = item / c.C, chunk = item - rt * c.C;
+    const int chunks = c.P >> 3, rt = item / chunks, chunk = item - rt * chunks;
     uint8_t *dst = c.xp + (size_t)item * 8 * c.NT * 32;
     for (int u = threadIdx.x; u < c.NT * 8; u += blockDim.x) {
         const int kc = u / c.NT, r = u - kc * c.NT;
@@ -186,169 +224,250 @@ static __device__ void split_item(const Call &c, int item) {
     }
 }
 
-constexpr int kPrepareThreads = 256;
+constexpr int kPrepareThreads = 256, kMaxSplit = 4;
 
-// t of up to 8 rows of one adapter for 16 of its ranks, and the zeros of the
-// tile's other rows (by the adapter's first group).
-static __device__ void form_t(const Call &c, uint32_t row, int q, TileSlots &ts) {
-    __shared__ int32_t member_s[kGroup];
-    __shared__ int32_t me_s[2];  // order and base of this block's row
-    __shared__ int16_t t_s[kGroup][16];
-    const int a = slot_of(c, row);
-    if (a < 0 || q >= pieces_of(c, a)) return;
-    const int rt = row / c.NT, at = row - rt * c.NT;
-    const int rank = c.rank[a], scale = c.scale[a];
-    const RowSlot r = tile_slots(c, rt, ts);
-    if (threadIdx.x < kGroup) member_s[threadIdx.x] = -1;
-    if ((int)threadIdx.x == at) {
-        me_s[0] = r.order;
-        me_s[1] = r.base;
-    }
-    __syncthreads();
-    const int order = me_s[0], base = me_s[1] + q;
-    if (order % kGroup != 0) return;
-    if (r.slot == a && r.order >= order && r.order < order + kGroup) member_s[r.order - order] = threadIdx.x;
-    __syncthreads();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int j0 = q * 16 + warp * 2;  // two ranks per warp
-    const int16_t *xr[kGroup];
+// Adds a value to the first block of the cluster's shared memory at p's place (the
+// blocks write different words).
+static __device__ __forceinline__ void store_first(int64_t *p, int64_t v) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
+    asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Products of two down rows (d, d + ld) with M rows over vectors [va, vb): sum[2 g + rank].
+// U vectors of every row are in flight per lane; int32 partials are flushed
+// after at most 16 vectors of 8 products: |lo| <= 128 * 255 * 2^15 < 2^30.
+template <int M, int U>
+static __device__ __forceinline__ void down_dots(const uint4 *d, int ld, const uint4 *const (&xr)[kGroup], int va, int vb,
+                                                 int lane, int64_t (&sum)[2 * kGroup]) {
+    const uint4 none = make_uint4(0, 0, 0, 0);
+    for (int v0 = va; v0 < vb; v0 += 32 * 16) {
+        int lo[2 * M], hi[2 * M];
 #pragma unroll
-    for (int g = 0; g < kGroup; g++)  // absent members repeat the first: loaded, not stored
-        xr[g] = c.x + ((size_t)rt * c.NT + (member_s[g] >= 0 ? member_s[g] : at)) * c.ld_x;
-    const uint32_t *d0 = c.down + ((size_t)a * c.Q * 16 + j0) * c.down_words, *d1 = d0 + c.down_words;
-    const int members = 1 + (member_s[1] >= 0) + (member_s[2] >= 0) + (member_s[3] >= 0) + (member_s[4] >= 0) +
-                        (member_s[5] >= 0) + (member_s[6] >= 0) + (member_s[7] >= 0);
-    int64_t sum[2 * kGroup];
+        for (int g = 0; g < 2 * M; g++) lo[g] = hi[g] = 0;
+        for (int k = 0; k < 16 && v0 + k * 32 < vb; k += U) {
+            uint4 w[2][U], x[M][U];
 #pragma unroll
-    for (int g = 0; g < 2 * kGroup; g++) sum[g] = 0;
-    const int vectors = c.K >> 3;
-    for (int v0 = 0; v0 < vectors; v0 += 32 * 16) {
-        // 16 vectors of 8 products per lane between flushes: |lo| <= 128 * 255 * 2^15 < 2^30
-        int lo[2 * kGroup], hi[2 * kGroup];
+            for (int u = 0; u < U; u++) {
+                const int v = v0 + (k + u) * 32 + lane;
+                const bool in = v < vb;
+                w[0][u] = in ? __ldg(d + v) : none;
+                w[1][u] = in ? __ldg(d + ld + v) : none;
 #pragma unroll
-        for (int g = 0; g < 2 * kGroup; g++) lo[g] = hi[g] = 0;
-#pragma unroll 2
-        for (int k = 0; k < 16; k++) {
-            const int v = v0 + k * 32 + lane;
-            if (v >= vectors) break;
-            const uint4 w0 = __ldg(reinterpret_cast<const uint4 *>(d0) + v), w1 = __ldg(reinterpret_cast<const uint4 *>(d1) + v);
-#pragma unroll
-            for (int g = 0; g < kGroup; g++) {
-                if (g >= members) break;
-                const uint4 x = __ldg(reinterpret_cast<const uint4 *>(xr[g]) + v);
-                lo[2 * g] = dp2a_lo_su(x.x, w0.x, lo[2 * g]);
-                hi[2 * g] = dp2a_hi_ss(x.x, w0.x, hi[2 * g]);
-                lo[2 * g] = dp2a_lo_su(x.y, w0.y, lo[2 * g]);
-                hi[2 * g] = dp2a_hi_ss(x.y, w0.y, hi[2 * g]);
-                lo[2 * g] = dp2a_lo_su(x.z, w0.z, lo[2 * g]);
-                hi[2 * g] = dp2a_hi_ss(x.z, w0.z, hi[2 * g]);
-                lo[2 * g] = dp2a_lo_su(x.w, w0.w, lo[2 * g]);
-                hi[2 * g] = dp2a_hi_ss(x.w, w0.w, hi[2 * g]);
-                lo[2 * g + 1] = dp2a_lo_su(x.x, w1.x, lo[2 * g + 1]);
-                hi[2 * g + 1] = dp2a_hi_ss(x.x, w1.x, hi[2 * g + 1]);
-                lo[2 * g + 1] = dp2a_lo_su(x.y, w1.y, lo[2 * g + 1]);
-                hi[2 * g + 1] = dp2a_hi_ss(x.y, w1.y, hi[2 * g + 1]);
-                lo[2 * g + 1] = dp2a_lo_su(x.z, w1.z, lo[2 * g + 1]);
-                hi[2 * g + 1] = dp2a_hi_ss(x.z, w1.z, hi[2 * g + 1]);
-                lo[2 * g + 1] = dp2a_lo_su(x.w, w1.w, lo[2 * g + 1]);
-                hi[2 * g + 1] = dp2a_hi_ss(x.w, w1.w, hi[2 * g + 1]);
+                for (int g = 0; g < M; g++) x[g][u] = in ? __ldg(xr[g] + v) : none;
             }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int g = 0; g < M; g++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        const int i = 2 * g + r;
+                        lo[i] = dp2a_lo_su(x[g][u].x, w[r][u].x, lo[i]);
+                        hi[i] = dp2a_hi_ss(x[g][u].x, w[r][u].x, hi[i]);
+                        lo[i] = dp2a_lo_su(x[g][u].y, w[r][u].y, lo[i]);
+                        hi[i] = dp2a_hi_ss(x[g][u].y, w[r][u].y, hi[i]);
+                        lo[i] = dp2a_lo_su(x[g][u].z, w[r][u].z, lo[i]);
+                        hi[i] = dp2a_hi_ss(x[g][u].z, w[r][u].z, hi[i]);
+                        lo[i] = dp2a_lo_su(x[g][u].w, w[r][u].w, lo[i]);
+                        hi[i] = dp2a_hi_ss(x[g][u].w, w[r][u].w, hi[i]);
+                    }
         }
 #pragma unroll
-        for (int g = 0; g < 2 * kGroup; g++) sum[g] += (int64_t)hi[g] * 256 + lo[g];
-    }
-    int idx;
-    const int64_t s = warp_reduce_n<2 * kGroup>(sum, lane, idx);
-    if ((lane & 1) == 0) {  // two lanes hold each sum
-        const int j = j0 + (idx & 1);
-        t_s[idx >> 1][warp * 2 + (idx & 1)] = j < rank ? (int16_t)sat16(rnd(s * scale, 24)) : (int16_t)0;
-    }
-    __syncthreads();
-    uint8_t *dst = c.tp + ((size_t)rt * c.max_pieces + base) * c.NT * 32;
-    if (threadIdx.x < kGroup && member_s[threadIdx.x] >= 0) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t *p = reinterpret_cast<const uint32_t *>(&t_s[threadIdx.x][4 * k]);
-            hi[k] = __byte_perm(p[0], p[1], 0x7531);
-            lo[k] = __byte_perm(p[0], p[1], 0x6420);
-        }
-        uint8_t *p = dst + member_s[threadIdx.x] * 16;
-        *reinterpret_cast<uint4 *>(p) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(p + c.NT * 16) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    }
-    if (order == 0 && (int)threadIdx.x < c.NT && r.slot != a) {
-        *reinterpret_cast<uint4 *>(dst + threadIdx.x * 16) = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4 *>(dst + c.NT * 16 + threadIdx.x * 16) = make_uint4(0, 0, 0, 0);
+        for (int g = 0; g < 2 * M; g++) sum[g] += (int64_t)hi[g] * 256 + lo[g];
     }
 }
 
-__global__ void __launch_bounds__(kPrepareThreads) k_prepare(const Call c) {
+// t of rows [row0, row0 + span) for `ranks` (16 or 4) ranks of their adapters from 16
+// q + sub * ranks on, a pass per group of up to 8 rows of one adapter (the group that
+// starts at a row of the span).  A warp takes two ranks and a share of k: with 4
+// ranks a block has four shares, times the blocks of its cluster.  Every thread
+// of the cluster takes the same path: it depends on the row, q and the slots alone.
+static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int share) {
+    constexpr int kWarps = kPrepareThreads / 32, kShares = 4 * kMaxSplit;
+    __shared__ int64_t sum_s[kShares * kGroup * 16 / 4];  // [share][row][rank]: 16 ranks x 8 shares or 4 x 32
+    __shared__ int16_t t_s[kGroup][16];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int R = c.ranks, pairs = R >> 1, parts = kWarps / pairs;  // warps that share k
+    const int vectors = c.K >> 3, all = parts * c.ksplit, part = share * parts + warp / pairs;
+    const int va = (int)((int64_t)vectors * part / all), vb = (int)((int64_t)vectors * (part + 1) / all);
+    const int pair = warp % pairs, j0 = q * 16 + sub * R + pair * 2;
+    for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
+        const int rt = row / c.NT, at = row - rt * c.NT;
+        const int a = slot_of(c, row);
+        if (a < 0) continue;
+        const RowMask mask = rows_of_slot(c, rt, a);
+        const int order = mask.before(at);
+        if (order % kGroup != 0 || q >= pieces_of(c, a)) continue;
+        if (c.ksplit > 1) cluster_arrive();  // the sums' memory is free here
+        const int rank = c.rank[a], scale = c.scale[a];
+        // members: the next 8 rows of the mask from this one on
+        int member[kGroup], members = 0;
+        {
+            int from = at;
+#pragma unroll
+            for (int g = 0; g < kGroup; g++) {
+                member[g] = at;  // absent members repeat the first: never stored
+                int k = from >> 5;
+                uint32_t w = k < kRowTile / 32 ? mask.w[k] & (~0u << (from & 31)) : 0u;
+                while (w == 0 && ++k < kRowTile / 32) w = mask.w[k];
+                if (k < kRowTile / 32 && w) {
+                    member[g] = k * 32 + __ffs((int)w) - 1;
+                    members = g + 1;
+                    from = member[g] + 1;
+                } else {
+                    from = kRowTile;
+                }
+            }
+        }
+        const uint4 *xr[kGroup];
+#pragma unroll
+        for (int g = 0; g < kGroup; g++)
+            xr[g] = reinterpret_cast<const uint4 *>(c.x + ((size_t)rt * c.NT + member[g]) * c.ld_x);
+        const uint4 *d0 = reinterpret_cast<const uint4 *>(c.down + ((size_t)a * c.Q * 16 + j0) * c.down_words);
+        int64_t sum[2 * kGroup];
+#pragma unroll
+        for (int g = 0; g < 2 * kGroup; g++) sum[g] = 0;
+        if (members == 1) down_dots<1, 4>(d0, c.down_words / 4, xr, va, vb, lane, sum);
+        else if (members == 2) down_dots<2, 2>(d0, c.down_words / 4, xr, va, vb, lane, sum);
+        else if (members <= 4) down_dots<4, 2>(d0, c.down_words / 4, xr, va, vb, lane, sum);
+        else down_dots<8, 1>(d0, c.down_words / 4, xr, va, vb, lane, sum);
+        int idx;
+        const int64_t mine = warp_reduce_n<2 * kGroup>(sum, lane, idx);
+        int64_t *place = sum_s + (part * kGroup + (idx >> 1)) * R + pair * 2 + (idx & 1);
+        if (c.ksplit > 1) {
+            cluster_wait();
+            if ((lane & 1) == 0) store_first(place, mine);  // two lanes hold each sum
+            cluster_arrive();
+            cluster_wait();
+        } else {
+            if ((lane & 1) == 0) *place = mine;
+            __syncthreads();
+        }
+        if (share == 0) {
+            if (threadIdx.x < kGroup * R) {
+                const int g = threadIdx.x / R, j = threadIdx.x % R;
+                int64_t v = 0;
+                for (int p = 0; p < all; p++) v += sum_s[p * kGroup * R + threadIdx.x];
+                t_s[g][j] = q * 16 + sub * R + j < rank ? (int16_t)sat16(rnd(v * scale, 24)) : (int16_t)0;
+            }
+            __syncthreads();
+            uint8_t *dst = c.tp + (((size_t)rt * c.NT + mask.first()) * c.Q + q) * c.NT * 32 + sub * R;
+            const int words = R / 4, g = threadIdx.x / words, w4 = threadIdx.x % words;  // 4 ranks per thread
+            if (g < members) {
+                int row_of = member[0];
+#pragma unroll
+                for (int u = 1; u < kGroup; u++)  // member[] stays in registers
+                    if (g == u) row_of = member[u];
+                const uint32_t *v = reinterpret_cast<const uint32_t *>(&t_s[g][4 * w4]);
+                uint8_t *p = dst + row_of * 16 + 4 * w4;
+                *reinterpret_cast<uint32_t *>(p) = __byte_perm(v[0], v[1], 0x7531);
+                *reinterpret_cast<uint32_t *>(p + c.NT * 16) = __byte_perm(v[0], v[1], 0x6420);
+            }
+            // zeros of the tile's other rows, by the adapter's first group
+            if (order == 0)
+                for (int u = threadIdx.x; u < c.NT * words; u += kPrepareThreads) {
+                    const int t = u / words, w = u % words;
+                    if ((mask.w[t >> 5] >> (t & 31)) & 1u) continue;
+                    *reinterpret_cast<uint32_t *>(dst + t * 16 + 4 * w) = 0;
+                    *reinterpret_cast<uint32_t *>(dst + c.NT * 16 + t * 16 + 4 * w) = 0;
+                }
+        }
+        if (c.ksplit == 1) __syncthreads();  // the sums are read before the next group's
+    }
+}
+
+// Blocks (x, share): per x first the rows' items and lists, then t.
+__global__ void __launch_bounds__(kPrepareThreads, 2) k_prepare(const Call c) {
     __shared__ TileSlots ts;
     pdl_wait();     // the caller's rows, and the last call's reads of the workspace
     pdl_trigger();
-    const int splits = c.RT * c.C;
+    const int share = blockIdx.y;
     int b = blockIdx.x;
+    const int per_row = c.Q * (16 / c.ranks), forms = c.slot ? (int)((c.rows + c.span - 1) / c.span) * per_row : 0;
+    if (b < forms) {
+        const int e = b % per_row;
+        form_t(c, (uint32_t)(b / per_row) * c.span, e / (16 / c.ranks), e % (16 / c.ranks), share);
+        return;
+    }
+    b -= forms;
+    const int items = c.RT * (c.P >> 3), splits = (items + c.ksplit - 1) / c.ksplit;
     if (b < splits) {
-        split_item(c, b);
+        if (b * c.ksplit + share < items) split_item(c, b * c.ksplit + share);
         return;
     }
     b -= splits;
-    if (b < c.RT) {  // the list of the row tile's adapter pieces
-        const RowSlot r = tile_slots(c, b, ts);
-        if (r.slot >= 0 && r.order == 0)
-            for (int q = 0; q < pieces_of(c, r.slot); q++) c.list[(size_t)b * c.max_pieces + r.base + q] = r.slot * c.Q + q;
-        if (threadIdx.x == 0) c.count[b] = r.total;
-        if (r.total & 1) {  // the second half of the last MMA step: zeros
-            uint4 *z = reinterpret_cast<uint4 *>(c.tp + ((size_t)b * c.max_pieces + r.total) * c.NT * 32);
-            for (int u = threadIdx.x; u < c.NT * 2; u += blockDim.x) z[u] = make_uint4(0, 0, 0, 0);
-        }
-        return;
-    }
-    b -= c.RT;
-    form_t(c, (uint32_t)(b / c.Q), b % c.Q, ts);
+    if (share != 0) return;
+    const RowSlot r = tile_slots(c, b, ts);  // the list of the row tile's adapter pieces
+    if (r.first)
+        for (int q = 0; q < pieces_of(c, r.slot); q++)
+            c.list[(size_t)b * c.max_pieces + r.base + q] = make_int2(r.slot * c.Q + q, (int)threadIdx.x * c.Q + q);
+    if (threadIdx.x == 0) c.count[b] = r.total;
 }
 
 // ---------------------------------------------------------------------------
 // the projection
 // ---------------------------------------------------------------------------
-static __device__ __forceinline__ int64_t range_begin(int b, int64_t items, int grid) { return items * b / grid; }
-static __device__ __forceinline__ int cta_of(int64_t i, int64_t items, int grid) {
-    int b = (int)(i * grid / items);
-    while (b + 1 < grid && range_begin(b + 1, items, grid) <= i) b++;
-    while (b > 0 && range_begin(b, items, grid) > i) b--;
+static __host__ __device__ __forceinline__ int header_bytes(int RT) { return (kHeader + (2 * RT + 1) * 4 + 127) / 128 * 128; }
+static __device__ __forceinline__ int64_t range_begin(int b, int64_t stages, int grid) { return stages * b / grid; }
+static __device__ __forceinline__ int cta_of(int64_t i, int64_t stages, int grid) {
+    int b = (int)(i * grid / stages);
+    while (b + 1 < grid && range_begin(b + 1, stages, grid) <= i) b++;
+    while (b > 0 && range_begin(b, stages, grid) > i) b--;
     return b;
 }
-
-// A place in the line of items: outputs tile ft, row tile rt, item i of the
-// `len` of that tile (C chunks of the weight, then stages of 8 adapter pieces).
-struct Cursor {
-    int ft, rt, i, len;
-    int64_t tile0;  // line position of the tile's first item
-};
-static __device__ __forceinline__ Cursor cursor_at(int64_t w, const int32_t *pre, int RT) {
-    Cursor k;
-    const int per = pre[RT];
-    k.ft = (int)(w / per);
-    const int rem = (int)(w - (int64_t)k.ft * per);
-    k.rt = 0;
-    while (k.rt + 1 < RT && pre[k.rt + 1] <= rem) k.rt++;
-    k.i = rem - pre[k.rt];
-    k.len = pre[k.rt + 1] - pre[k.rt];
-    k.tile0 = w - k.i;
-    return k;
+// Stages before tile t in the line of all tiles (row tiles of the same outputs
+// are neighbours); pre[rt]: stages of the row tiles before rt.
+static __device__ __forceinline__ int64_t line_at(int t, const int32_t *pre, int RT) {
+    return (int64_t)(t / RT) * pre[RT] + pre[t % RT];
 }
-static __device__ __forceinline__ void next_tile(Cursor &k, const int32_t *pre, int RT) {
-    k.tile0 += k.len;
-    k.i = 0;
-    if (++k.rt == RT) {
-        k.rt = 0;
-        k.ft++;
+
+// A CTA's way through the tiles: its run of the stages of the first `shared`
+// tiles, then every grid-th of the tiles after them, whole.  A step is the run of
+// a tile's stages [begin, end) that the CTA takes: of the weight's (below C), then
+// of the adapters'.
+struct Walk {
+    int tile, ft, rt;     // tile, its outputs and its row tile
+    int begin, end, len;  // stages of this step, stages of the tile
+    int left;             // stages left in the shared run, this step's included
+
+    __device__ __forceinline__ void set(const Call &c, const int32_t *pre, int t, int stage) {
+        tile = t;
+        ft = t / c.RT;
+        rt = t - ft * c.RT;
+        len = pre[rt + 1] - pre[rt];
+        begin = stage;
+        end = left > 0 ? min(len, begin + left) : len;
     }
-    k.len = pre[k.rt + 1] - pre[k.rt];
-}
+    __device__ __forceinline__ void start(const Call &c, const int32_t *pre, int64_t w0, int64_t w1) {
+        left = (int)(w1 - w0);
+        if (left == 0) {
+            set(c, pre, c.shared_tiles + blockIdx.x, 0);
+            return;
+        }
+        const int per = pre[c.RT];
+        const int f = (int)(w0 / per), rem = (int)(w0 - (int64_t)f * per);
+        int r = 0;
+        while (r + 1 < c.RT && pre[r + 1] <= rem) r++;
+        set(c, pre, f * c.RT + r, rem - pre[r]);
+    }
+    __device__ __forceinline__ bool more(const Call &c) const { return left > 0 || tile < c.T * c.RT; }
+    __device__ __forceinline__ void next(const Call &c, const int32_t *pre) {
+        if (left > 0) {
+            left -= end - begin;
+            set(c, pre, left > 0 ? tile + 1 : c.shared_tiles + blockIdx.x, 0);
+        } else {
+            set(c, pre, tile + gridDim.x, 0);
+        }
+    }
+};
 
-__global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
+// At most 96 registers a thread and kProjectSmem bytes of shared memory: a block of
+// k_prepare then fits beside it, so that neither waits for the other's SM.
+template <int D>
+__global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem);  // [kMaxRing] stage loaded
     uint64_t *empty = full + kMaxRing;                    // [kMaxRing] stage consumed
@@ -357,11 +476,13 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
     uint64_t *done = tempty + 2;                          // every MMA of the CTA complete
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     int *last_s = reinterpret_cast<int *>(tmem_slot + 1);
-    int *fail_s = last_s + 1;                             // [4] wait outcome of each epilogue warp
-    int32_t *pre = fail_s + 4;                            // [RT + 1] items before each row tile
-    uint8_t *ring = smem + kHeader;
+    int *fail_s = last_s + 1;                             // [8] wait outcome of each result warp
+    int32_t *pre = fail_s + 8;                            // [RT + 1] stages before each row tile
+    int32_t *pieces = pre + c.RT + 1;                     // [RT] adapter pieces of each row tile
+    uint8_t *ring = smem + header_bytes(c.RT);
     const int NT = c.NT, C = c.C, S = c.ring;
-    const int x_bytes = NT * 256, stage = kItem + x_bytes;
+    
+    const int w_bytes = D * kPiece, x_bytes = D * NT * 32, stage = w_bytes + x_bytes;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint32_t columns = 32;
     while (columns < (uint32_t)(4 * NT * c.buffers)) columns <<= 1;
@@ -373,7 +494,7 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(tfull + b, 1);
-            mbar_init(tempty + b, 128);
+            mbar_init(tempty + b, kResultThreads);
         }
         mbar_init(done, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -384,7 +505,7 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // Items of each row tile.  With one row tile its adapters are counted here,
+    // Stages of each row tile.  With one row tile its adapters are counted here,
     // from the slots themselves (k_prepare passed its wait before this kernel
     // could start, so they are final), and the weights can be fetched before
     // k_prepare ends; with more, k_prepare's counts are waited for.
@@ -392,18 +513,21 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
         TileSlots &ts = *reinterpret_cast<TileSlots *>(ring);
         const RowSlot r = tile_slots(c, 0, ts);
         if (threadIdx.x == 0) {
+            pieces[0] = r.total;
             pre[0] = 0;
-            pre[1] = C + (r.total + 7) / 8;
+            pre[1] = C + (r.total + D - 1) / D;
         }
         // the ring takes this memory over for bulk copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     } else {
         if (c.slot) pdl_wait();
+        for (int rt = threadIdx.x; rt < c.RT; rt += blockDim.x) pieces[rt] = c.slot ? __ldcg(c.count + rt) : 0;
+        __syncthreads();
         if (threadIdx.x == 0) {
             int n = 0;
             for (int rt = 0; rt < c.RT; rt++) {
                 pre[rt] = n;
-                n += C + (c.slot ? (__ldcg(c.count + rt) + 7) / 8 : 0);
+                n += C + (pieces[rt] + D - 1) / D;
             }
             pre[c.RT] = n;
         }
@@ -412,151 +536,198 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int64_t items = (int64_t)c.T * pre[c.RT];
-    const int64_t w0 = range_begin(blockIdx.x, items, gridDim.x), w1 = range_begin(blockIdx.x + 1, items, gridDim.x);
-    const int n = (int)(w1 - w0);
-    const Cursor start = cursor_at(n > 0 ? w0 : 0, pre, c.RT);
+    const int64_t line = line_at(c.shared_tiles, pre, c.RT);  // stages that are shared out one by one
+    const int me = min((int)blockIdx.x, c.sharers);
+    Walk k;
+    k.start(c, pre, line ? range_begin(me, line, c.sharers) : 0,
+            line && me < c.sharers ? range_begin(me + 1, line, c.sharers) : line ? range_begin(me, line, c.sharers) : 0);
 
     if (warp == 1) {  // ---- loads ---------------------------------------------------
-        if (lane == 0) {
-            const uint64_t policy = evict_first_policy();
-            auto load_weight = [&](const Cursor &k, int s) {  // announces the whole stage
-                uint8_t *dst = ring + (size_t)s * stage;
-                if (k.i < C) {
-                    mbar_expect_tx(full + s, kItem + x_bytes);
-                    const uint8_t *src = c.weight + ((size_t)k.ft * C + k.i) * kItem;
-                    if (c.RT == 1) bulk_g2s_hint(dst, src, kItem, full + s, policy);  // read once
-                    else bulk_g2s(dst, src, kItem, full + s);
-                } else {
-                    const int p0 = (k.i - C) * 8, np = min(8, __ldcg(c.count + k.rt) - p0);
-                    mbar_expect_tx(full + s, np * kPiece + ((np + 1) & ~1) * NT * 32);
-                    for (int p = 0; p < np; p++) {
-                        const int e = __ldcg(c.list + (size_t)k.rt * c.max_pieces + p0 + p), a = e / c.Q, q = e - a * c.Q;
-                        bulk_g2s(dst + p * kPiece, c.up + (((size_t)a * c.T + k.ft) * c.Q + q) * kPiece, kPiece, full + s);
-                    }
-                }
-            };
-            auto load_rows = [&](const Cursor &k, int s) {
-                uint8_t *dst = ring + (size_t)s * stage + kItem;
-                if (k.i < C) {
-                    bulk_g2s(dst, c.xp + ((size_t)k.rt * C + k.i) * x_bytes, x_bytes, full + s);
-                } else {
-                    const int p0 = (k.i - C) * 8, np = min(8, __ldcg(c.count + k.rt) - p0);
-                    bulk_g2s(dst, c.tp + ((size_t)k.rt * c.max_pieces + p0) * NT * 32, ((np + 1) & ~1) * NT * 32, full + s);
-                }
-            };
-            // weights of the first stages before k_prepare has finished; adapter
-            // stages wait for its lists
-            Cursor k = start, kr = start;
-            int early = 0;
-            while (early < n && early < S && k.i < C) {
-                load_weight(k, early);
-                early++;
-                if (++k.i == k.len) next_tile(k, pre, c.RT);
-            }
-            pdl_wait();
-            asm volatile("fence.proxy.async.global;" ::: "memory");  // k_prepare's stores before the bulk reads
-            for (int j = 0; j < early; j++) {
-                load_rows(kr, j);
-                if (++kr.i == kr.len) next_tile(kr, pre, c.RT);
-            }
-            bool ok = true;
-            int issued = early;
-            for (int j = early; j < n; j++) {
-                const int s = j % S;
-                if (j >= S && !mbar_wait(empty + s, ((j / S) - 1) & 1)) {
-                    ok = false;
+        // Lane 0 loads the weight's stages: few instructions per stage, since one
+        // thread's latency is all that paces them.  In an adapter stage lanes 0-7 load
+        // its pieces and lanes 8-15 their t.
+        const uint64_t policy = evict_first_policy();
+        auto load_weight = [&](const uint8_t *src, int s) {  // announces the whole stage
+            mbar_expect_tx(full + s, stage);
+            if (c.RT == 1) bulk_g2s_hint(ring + s * stage, src, w_bytes, full + s, policy);  // read once
+            else bulk_g2s(ring + s * stage, src, w_bytes, full + s);
+        };
+        auto weight_of = [&](const Walk &w, int i) { return c.weight + ((size_t)w.ft * c.P + (size_t)i * D) * kPiece; };
+        auto rows_of = [&](const Walk &w, int i) { return c.xp + ((size_t)w.rt * c.P + (size_t)i * D) * NT * 32; };
+        // weights of the first stages before k_prepare has finished, up to the
+        // first adapter stage, whose list it writes
+        Walk w = k;
+        int early = 0;
+        for (bool go = true; go && early < S && w.more(c); w.next(c, pre)) {
+            for (int i = w.begin; i < w.end && early < S; i++) {
+                if (i >= C) {
+                    go = false;
                     break;
                 }
-                load_weight(k, s);
-                load_rows(k, s);
-                issued = j + 1;
-                if (++k.i == k.len) next_tile(k, pre, c.RT);
+                if (lane == 0) load_weight(weight_of(w, i), early);
+                early++;
             }
-            if (!ok) {
-                atomicExch(c.error, 1);
-                for (int s = 0; s < S && s < issued; s++) {  // the copies in flight land before the CTA ends
-                    const int last = s + ((issued - 1 - s) / S) * S;
-                    (void)mbar_wait(full + s, (last / S) & 1);
+        }
+        pdl_wait();
+        asm volatile("fence.proxy.async.global;" ::: "memory");  // k_prepare's stores before the bulk reads
+        bool ok = true;
+        int s = 0, phase = 1, issued = 0;  // phase: of the last use of stage s
+        for (; ok && k.more(c); k.next(c, pre)) {
+            const int bound = min(k.end, C), first = k.begin;
+            if (lane == 0 && first < bound) {
+                const uint8_t *src = weight_of(k, first), *rows = rows_of(k, first);
+                for (int i = first; i < bound; i++) {
+                    if (issued >= S && !mbar_wait(empty + s, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    if (issued >= early) load_weight(src, s);
+                    bulk_g2s(ring + s * stage + w_bytes, rows, x_bytes, full + s);
+                    src += w_bytes;
+                    rows += x_bytes;
+                    issued++;
+                    if (++s == S) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
+            }
+            ok = __shfl_sync(~0u, ok, 0);
+            s = __shfl_sync(~0u, s, 0);
+            phase = __shfl_sync(~0u, phase, 0);
+            issued = __shfl_sync(~0u, issued, 0);
+            for (int i = max(first, C); ok && i < k.end; i++) {
+                const int p0 = (i - C) * D, np = min(D, pieces[k.rt] - p0);
+                const int2 mine = (lane & 7) < np ? __ldcg(c.list + (size_t)k.rt * c.max_pieces + p0 + (lane & 7)) : make_int2(0, 0);
+                if (issued >= S) {
+                    ok = mbar_wait(empty + s, phase);
+                    ok = __all_sync(~0u, ok);
+                    if (!ok) break;
+                }
+                uint8_t *dst = ring + s * stage;
+                if (lane == 0) mbar_expect_tx(full + s, np * kPiece + ((np + 1) & ~1) * NT * 32);
+                __syncwarp();
+                if (lane < np) {
+                    const int a = mine.x / c.Q, q = mine.x - a * c.Q;
+                    bulk_g2s(dst + lane * kPiece, c.up + (((size_t)a * c.T + k.ft) * c.Q + q) * kPiece, kPiece, full + s);
+                }
+                const int p = lane - 8;  // an odd last piece is paired with one of zeros
+                if (p >= 0 && p < ((np + 1) & ~1))
+                    bulk_g2s(dst + w_bytes + p * NT * 32,
+                             p < np ? c.tp + ((size_t)k.rt * NT * c.Q + mine.y) * NT * 32 : c.zero, NT * 32, full + s);
+                issued++;
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        if (!ok && lane == 0) {
+            atomicExch(c.error, 1);
+            issued = max(issued, early);
+            for (int q = 0; q < S && q < issued; q++) {  // the copies in flight land before the CTA ends
+                const int last = q + ((issued - 1 - q) / S) * S;
+                (void)mbar_wait(full + q, (last / S) & 1);
             }
         }
         __syncwarp();
     } else if (warp == 0) {  // ---- products ---------------------------------------
+        // One lane issues.  Descriptors are a stage's first one plus constants: their
+        // arithmetic is what limits narrow row tiles (a step of 32 columns takes
+        // the tensor cores 41 cycles).
         if (lane == 0) {
-            // [xh | xs] of NT rows each: signed; t's planes one by one, the low one unsigned
-            const uint32_t ss2 = umma_idesc_i8(1, 1, 2 * NT), us2 = umma_idesc_i8(0, 1, 2 * NT);
+            const uint32_t ss2 = umma_idesc_i8(1, 1, 2 * NT), us2 = umma_idesc_i8(0, 1, 2 * NT);  // [xh | xs] of NT rows each
             const uint32_t ss = umma_idesc_i8(1, 1, NT), su = umma_idesc_i8(1, 0, NT), us = umma_idesc_i8(0, 1, NT),
-                           uu = umma_idesc_i8(0, 0, NT);
-            const uint32_t lbo = NT * 32;
-            pdl_wait();  // k_prepare's counts
-            Cursor k = start;
-            int tiles = 0;
+                           uu = umma_idesc_i8(0, 0, NT);  // t's planes one by one, the low one unsigned
+            const uint64_t wd0 = umma_desc(smem_u32(ring), kPiece, 128), xd0 = umma_desc(smem_u32(ring) + w_bytes, NT * 32, 128);
+            const uint32_t step = (uint32_t)(2 * NT * 32) >> 4;  // two row pieces, in descriptor units
+            constexpr uint32_t kStep = 2 * kPiece >> 4, kLow = kPiece / 2 >> 4;
+            int tiles = 0, s = 0, phase = 0;
+            uint64_t wd = wd0, xd = xd0;
             bool ok = true;
-            for (int j = 0; j < n; j++) {
-                const bool first = j == 0 || k.i == 0, last = j == n - 1 || k.i == k.len - 1;
+            auto advance = [&] {
+                umma_commit(empty + s);
+                wd += (uint32_t)stage >> 4;
+                xd += (uint32_t)stage >> 4;
+                if (++s == S) {
+                    s = 0;
+                    phase ^= 1;
+                    wd = wd0;
+                    xd = xd0;
+                }
+            };
+            for (; k.more(c); k.next(c, pre), tiles++) {
                 const int b = c.buffers == 2 ? tiles & 1 : 0, use = c.buffers == 2 ? tiles >> 1 : tiles;
-                if (first && use > 0 && !mbar_wait(tempty + b, (use - 1) & 1)) ok = false;
-                if (ok && !mbar_wait(full + j % S, (j / S) & 1)) ok = false;
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t wa = smem_u32(ring + (size_t)(j % S) * stage), xa = wa + kItem;
+                if (use > 0 && !mbar_wait(tempty + b, (use - 1) & 1)) ok = false;
                 const uint32_t dh = tmem + (uint32_t)(b * 4 * NT), dl = dh + 2 * NT;
-                if (k.i < C) {
+                const int bound = min(k.end, C);
+                uint32_t more = 0;  // the first product of the step overwrites
+                for (int i = k.begin; ok && i < bound; i++) {
+                    if (!mbar_wait(full + s, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    umma_i8(dh, wd, xd, ss2, more);
+                    umma_i8(dl, wd + kLow, xd, us2, more);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {  // 32-deep steps: two pieces
-                        const uint32_t acc = (first && q == 0) ? 0u : 1u;
-                        const uint64_t wh = umma_desc(wa + q * 2 * kPiece, kPiece, 128);
-                        const uint64_t wl = umma_desc(wa + q * 2 * kPiece + kPiece / 2, kPiece, 128);
-                        const uint64_t x2 = umma_desc(xa + q * 2 * lbo, lbo, 128);
-                        umma_i8(dh, wh, x2, ss2, acc);
-                        umma_i8(dl, wl, x2, us2, acc);
+                    for (int q = 1; q < D / 2; q++) {  // 32-deep steps: two pieces
+                        umma_i8(dh, wd + q * kStep, xd + q * step, ss2, 1u);
+                        umma_i8(dl, wd + q * kStep + kLow, xd + q * step, us2, 1u);
                     }
-                } else {
-                    const int np = min(8, __ldcg(c.count + k.rt) - (k.i - C) * 8);
+                    more = 1;
+                    advance();
+                }
+                for (int i = max(k.begin, C); ok && i < k.end; i++) {
+                    if (!mbar_wait(full + s, phase)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const int np = min(D, pieces[k.rt] - (i - C) * D);
+                    const uint32_t low = (uint32_t)(NT * 16) >> 4;
                     for (int q = 0; 2 * q < np; q++) {
-                        const uint32_t acc = (first && q == 0) ? 0u : 1u;
-                        const uint64_t wh = umma_desc(wa + q * 2 * kPiece, kPiece, 128);
-                        const uint64_t wl = umma_desc(wa + q * 2 * kPiece + kPiece / 2, kPiece, 128);
-                        const uint64_t th = umma_desc(xa + q * 2 * lbo, lbo, 128);
-                        const uint64_t tl = umma_desc(xa + q * 2 * lbo + NT * 16, lbo, 128);
-                        umma_i8(dh, wh, th, ss, acc);
-                        umma_i8(dh + NT, wh, tl, su, acc);
-                        umma_i8(dl, wl, th, us, acc);
-                        umma_i8(dl + NT, wl, tl, uu, acc);
+                        const uint64_t wh = wd + q * kStep, th = xd + q * step;
+                        umma_i8(dh, wh, th, ss, more);
+                        umma_i8(dh + NT, wh, th + low, su, more);
+                        umma_i8(dl, wh + kLow, th, us, more);
+                        umma_i8(dl + NT, wh + kLow, th + low, uu, more);
+                        more = 1;
                     }
+                    advance();
                 }
-                umma_commit(empty + j % S);
-                if (last) {
-                    umma_commit(tfull + b);
-                    tiles++;
-                }
-                if (++k.i == k.len) next_tile(k, pre, c.RT);
+                if (!ok) break;
+                umma_commit(tfull + b);
             }
             if (!ok) atomicExch(c.error, 2);
             umma_commit(done);  // the accumulators are released only after every MMA
             if (!mbar_wait(done, 0)) atomicExch(c.error, 2);
         }
         __syncwarp();
-    } else {  // ---- results: warps 2-5, thread m = output m of the tile ---------------------
-        const int q4 = warp & 3, m = q4 * 32 + lane;
-        Cursor k = start;
-        int64_t w = w0;
-        for (int tiles = 0; w < w1; tiles++) {
+    } else {  // ---- results: warps 2-9, a thread per output of the tile and half of its rows ----
+        const int q4 = warp & 3, m = q4 * 32 + lane;   // TMEM lanes of this warp, output of this thread
+        const int half = (warp - 2) >> 2;              // rows 16 i + 8 half .. + 7
+        for (int tiles = 0; k.more(c); tiles++, k.next(c, pre)) {
             const int b = c.buffers == 2 ? tiles & 1 : 0, use = c.buffers == 2 ? tiles >> 1 : tiles;
-            const int64_t seg1 = min(w1, k.tile0 + k.len);
-            const bool whole = w == k.tile0 && seg1 == k.tile0 + k.len;
+            const bool whole = k.begin == 0 && k.end == k.len;
             const int o = k.ft * kOutTile + m;
             const bool live = o < c.N;
-            const int64_t corr = w == k.tile0 ? 128 * (int64_t)c.wsum[o] : 0;
+            const int64_t corr = k.begin == 0 ? 128 * (int64_t)c.wsum[o] : 0;
             const int rows = min(NT, (int)c.rows - k.rt * NT);
+            int b_lo = 0, b_hi = 0;
+            if (!whole) {
+                const int64_t at = line_at(k.tile, pre, c.RT);
+                b_lo = cta_of(at, line, c.sharers);
+                b_hi = cta_of(at + k.len - 1, line, c.sharers);
+            }
+            unsigned long long *acc = reinterpret_cast<unsigned long long *>(c.acc) + (size_t)b_lo * NT * kOutTile + m;
             const bool okw = mbar_wait_err(tfull + b, use & 1, c.error);
-            if (lane == 0) fail_s[q4] = okw ? 0 : 1;
-            named_sync(3, 128);
-            const int failed = fail_s[0] | fail_s[1] | fail_s[2] | fail_s[3];
-            named_sync(3, 128);  // read by all before the next tile writes it
+            if (lane == 0) fail_s[warp - 2] = okw ? 0 : 1;
+            named_sync(3, kResultThreads);
+            const int failed = fail_s[0] | fail_s[1] | fail_s[2] | fail_s[3] | fail_s[4] | fail_s[5] | fail_s[6] | fail_s[7];
+            named_sync(3, kResultThreads);  // read by all before the next tile writes it
             if (failed) {
-                if (m == 0) atomicCAS(c.error, 0, 3);
+                if (threadIdx.x == 64) atomicCAS(c.error, 0, 3);
                 break;
             }
             tc_fence_after();
@@ -567,14 +738,7 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
                 if (c.wide) static_cast<int32_t *>(c.out)[at] = v;
                 else static_cast<int16_t *>(c.out)[at] = (int16_t)sat16(rnd(v, 8));
             };
-            int b_lo = 0, b_hi = 0;
-            unsigned long long *acc = nullptr;
-            if (!whole) {
-                b_lo = cta_of(k.tile0, items, gridDim.x);
-                b_hi = cta_of(k.tile0 + k.len - 1, items, gridDim.x);
-                acc = reinterpret_cast<unsigned long long *>(c.acc) + (size_t)b_lo * NT * kOutTile + m;
-            }
-            for (int r0 = 0; r0 < rows; r0 += 8) {
+            for (int r0 = 8 * half; r0 < rows; r0 += 16) {
                 uint32_t v[32];
                 tmem_ld4x8(t0 + r0, t0 + NT + r0, t0 + 2 * NT + r0, t0 + 3 * NT + r0, v);
 #pragma unroll
@@ -590,8 +754,8 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
             tc_fence_before();
             mbar_arrive(tempty + b);
             if (!whole) {
-                named_sync(3, 128);  // every thread's additions before thread 0's release
-                if (m == 0) {
+                named_sync(3, kResultThreads);  // every thread's additions before the release below
+                if (threadIdx.x == 64) {
                     int old;
                     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;"
                                  : "=r"(old)
@@ -599,26 +763,26 @@ __global__ void __launch_bounds__(kProjectThreads, 1) k_project(const Call c) {
                                  : "memory");
                     *last_s = old == b_hi - b_lo;
                 }
-                named_sync(3, 128);
-                const int finish = *last_s;
-                if (finish) {
-                    for (int r0 = 0; r0 < rows; r0 += 8) {
-                        int64_t s[8];
+                named_sync(3, kResultThreads);
+                if (*last_s) {
+                    for (int r0 = 8 * half; r0 < rows; r0 += 32) {  // 16 rows' sums in flight
+                        int64_t s[16];
 #pragma unroll
-                        for (int r = 0; r < 8; r++)
-                            s[r] = r0 + r < rows ? (int64_t)__ldcg(acc + (size_t)(r0 + r) * kOutTile) : 0;
+                        for (int r = 0; r < 16; r++) {
+                            const int row = r0 + (r & 7) + (r >> 3) * 16;
+                            s[r] = row < rows ? (int64_t)__ldcg(acc + (size_t)row * kOutTile) : 0;
+                        }
 #pragma unroll
-                        for (int r = 0; r < 8; r++) {
-                            if (r0 + r >= rows) break;
-                            acc[(size_t)(r0 + r) * kOutTile] = 0;  // ready for the next call
-                            if (live) put(r0 + r, s[r]);
+                        for (int r = 0; r < 16; r++) {
+                            const int row = r0 + (r & 7) + (r >> 3) * 16;
+                            if (row >= rows) continue;
+                            acc[(size_t)row * kOutTile] = 0;  // ready for the next call
+                            if (live) put(row, s[r]);
                         }
                     }
-                    if (m == 0) c.arrived[b_lo] = 0;
+                    if (threadIdx.x == 64) c.arrived[b_lo] = 0;
                 }
             }
-            w = seg1;
-            next_tile(k, pre, c.RT);
         }
     }
     __syncthreads();
@@ -675,36 +839,40 @@ __global__ void k_set_slot(int32_t *ranks, int32_t *scales, uint32_t slot, int32
     scales[slot] = scale;
 }
 
-// Rows per row tile of a call: as few row tiles as 128 rows each allow, evenly
-// filled, in steps of 16 (the MMA's column granularity).
+// Rows per tile when a call's rows are spread over rt row tiles, in steps of 16
+// (the MMA's column granularity).
+int rows_per_tile(uint32_t rows, int rt) { return (int)(((rows + rt - 1) / rt + 15) / 16 * 16); }
 int row_tiles(uint32_t rows) { return (int)((rows + kRowTile - 1) / kRowTile); }
-int rows_per_tile(uint32_t rows) {
-    const uint32_t rt = (uint32_t)row_tiles(rows);
-    return (int)(((rows + rt - 1) / rt + 15) / 16 * 16);
+
+// Tiles whose stages are shared out one by one: all when there are fewer tiles
+// than CTAs, else what is left after whole tiles for every CTA -- unless that is
+// nearly another one for each, which then costs less than adding up shared tiles.
+int shared_tiles(int64_t tiles, int ctas) {
+    if (tiles < ctas) return (int)tiles;
+    const int rest = (int)(tiles % ctas);
+    return 4 * rest >= 3 * ctas ? 0 : rest;
 }
 
 }  // namespace
 
 struct llmx_adapters {
-    int dev = 0, sms = 0, smem = 0;
+    int dev = 0, sms = 0;
     uint32_t in_dim = 0, out_dim = 0, slots = 0, max_rank = 0, max_rows = 0;
-    int C = 0, T = 0, Q = 0, row_cap = 0;  // row_cap: most rows per row tile of any call
-    uint8_t *weight = nullptr;   // items [T][C]
+    int P = 0, T = 0, Q = 0, row_cap = 0;  // row_cap: most rows per row tile of any call
+    uint8_t *weight = nullptr;   // pieces [T][P]
     int32_t *wsum = nullptr;     // [T * 128]
     uint32_t *down = nullptr;    // [slots][16 Q][in_dim / 2]
     uint8_t *up = nullptr;       // pieces [slots][T][Q]
     int32_t *rank = nullptr, *scale = nullptr;  // [slots]
-    uint8_t *xp = nullptr, *tp = nullptr;       // row and t pieces of a call
-    int32_t *list = nullptr, *count = nullptr;  // adapter pieces of its row tiles
+    uint8_t *xp = nullptr, *tp = nullptr, *zero = nullptr;  // row and t pieces of a call, a piece of zeros
+    int2 *list = nullptr;                       // adapter pieces of its row tiles
+    int32_t *count = nullptr;
     int64_t *acc = nullptr;
     int32_t *arrived = nullptr;
     int *error = nullptr;
     uint64_t bytes = 0;
 
-    size_t max_pieces(int nt) const {  // of one row tile, even
-        const size_t n = std::min<size_t>((size_t)nt, slots) * Q;
-        return (n + 1) / 2 * 2;
-    }
+    size_t max_pieces(int nt) const { return std::min<size_t>((size_t)nt, slots) * Q; }  // of one row tile
     size_t acc_bytes() const { return (size_t)sms * row_cap * kOutTile * 8; }
 };
 
@@ -734,25 +902,29 @@ struct DeviceScope {
 
 void release(llmx_adapters *h) {
     for (void *p : {(void *)h->weight, (void *)h->wsum, (void *)h->down, (void *)h->up, (void *)h->rank, (void *)h->scale,
-                    (void *)h->xp, (void *)h->tp, (void *)h->list, (void *)h->count, (void *)h->acc, (void *)h->arrived,
+                    (void *)h->xp, (void *)h->tp, (void *)h->zero, (void *)h->list, (void *)h->count, (void *)h->acc, (void *)h->arrived,
                     (void *)h->error})
         cudaFree(p);
     delete h;
 }
 
-cudaError_t launch(const void *fn, int grid, int threads, size_t smem, const Call &c, cudaStream_t s) {
+cudaError_t launch(const void *fn, dim3 grid, int cluster_y, int threads, size_t smem, const Call &c, cudaStream_t s) {
     Call copy = c;
     void *args[] = {&copy};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 1;
+    attr[1].val.clusterDim.y = (unsigned)cluster_y;
+    attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster_y > 1 ? 2 : 1;
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
@@ -783,29 +955,34 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
     h->slots = slots;
     h->max_rank = slots ? max_rank : 0;
     h->max_rows = max_rows;
-    h->C = (int)((in_dim + kOutTile - 1) / kOutTile);
+    h->P = (int)((in_dim + 127) / 128 * 8);
     h->T = (int)((out_dim + kOutTile - 1) / kOutTile);
     h->Q = (int)((h->max_rank + 15) / 16);
-    h->row_cap = max_rows > kRowTile ? kRowTile : rows_per_tile(max_rows);
+    h->row_cap = max_rows > kRowTile ? kRowTile : rows_per_tile(max_rows, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     auto get = [&](auto **p, size_t n) {
         n = std::max<size_t>(n, 16);
         h->bytes += n;
         return cudaMalloc(reinterpret_cast<void **>(p), n);
     };
-    const size_t rt = (size_t)row_tiles(max_rows), up_bytes = (size_t)slots * h->T * h->Q * kPiece;
+    const size_t rt = (size_t)row_tiles(max_rows) + (max_rows > kRowTile ? kMoreTiles : 0);
+    const size_t xt = rt == 1 ? (size_t)h->row_cap : max_rows + 16 * rt;  // rows of all row tiles
+    const size_t up_bytes = (size_t)slots * h->T * h->Q * kPiece;
     const size_t pieces = h->max_pieces(h->row_cap);
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
-        (e = cudaDeviceGetAttribute(&h->smem, cudaDevAttrMaxSharedMemoryPerBlockOptin, device)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(k_project, cudaFuncAttributeMaxDynamicSharedMemorySize, h->smem)) != cudaSuccess ||
-        (e = get(&h->weight, (size_t)h->T * h->C * kItem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(k_project<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(k_project<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
+        (e = get(&h->weight, (size_t)h->T * h->P * kPiece)) != cudaSuccess ||
         (e = get(&h->wsum, (size_t)h->T * kOutTile * 4)) != cudaSuccess ||
         (e = get(&h->down, (size_t)slots * h->Q * 16 * in_dim * 2)) != cudaSuccess ||
         (e = get(&h->up, up_bytes)) != cudaSuccess || (e = get(&h->rank, (size_t)slots * 4)) != cudaSuccess ||
         (e = get(&h->scale, (size_t)slots * 4)) != cudaSuccess ||
-        (e = get(&h->xp, rt * h->C * h->row_cap * 256)) != cudaSuccess ||
-        (e = get(&h->tp, rt * pieces * h->row_cap * 32)) != cudaSuccess || (e = get(&h->list, rt * pieces * 4)) != cudaSuccess ||
+        (e = get(&h->xp, xt * h->P * 32)) != cudaSuccess ||
+        (e = get(&h->tp, xt * h->Q * h->row_cap * 32)) != cudaSuccess ||
+        (e = get(&h->zero, (size_t)h->row_cap * 32)) != cudaSuccess ||
+        (e = cudaMemsetAsync(h->zero, 0, (size_t)h->row_cap * 32, s)) != cudaSuccess ||
+        (e = get(&h->list, rt * pieces * 8)) != cudaSuccess ||
         (e = get(&h->count, rt * 4)) != cudaSuccess || (e = get(&h->acc, h->acc_bytes())) != cudaSuccess ||
         (e = get(&h->arrived, (size_t)h->sms * 4)) != cudaSuccess || (e = get(&h->error, 4)) != cudaSuccess ||
         (e = cudaMemsetAsync(h->rank, 0, (size_t)slots * 4, s)) != cudaSuccess ||
@@ -817,7 +994,7 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
         release(h);
         return cuda_fail("create", e);
     }
-    k_pack_pieces<<<h->sms * 8, 256, 0, s>>>(weight, out_dim, in_dim, in_dim, h->C * 8, h->C * 8, h->T, h->weight);
+    k_pack_pieces<<<h->sms * 8, 256, 0, s>>>(weight, out_dim, in_dim, in_dim, h->P, h->P, h->T, h->weight);
     k_weight_sums<<<h->T * (kOutTile / 8), 256, 0, s>>>(weight, out_dim, in_dim, h->T * kOutTile, h->wsum);
     if ((e = cudaGetLastError()) != cudaSuccess) {
         release(h);
@@ -887,11 +1064,22 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     c.rows = rows;
     c.wide = wide;
     c.K = (int)h->in_dim;
-    c.C = h->C;
+    c.P = h->P;
     c.T = h->T;
     c.N = (int)h->out_dim;
-    c.RT = row_tiles(rows);
-    c.NT = rows_per_tile(rows);
+    // Row tiles: the fewest, or a few more where narrower tiles fill the CTAs' turns better.
+    // A stage's time goes as its bytes, 128 outputs and NT rows wide.
+    double best = 0;
+    for (int rt = row_tiles(rows); rt <= row_tiles(rows) + (rows > kRowTile ? kMoreTiles : 0); rt++) {
+        const int nt = rows_per_tile(rows, rt), shared = shared_tiles((int64_t)h->T * rt, h->sms);
+        const double turns = (double)(((int64_t)h->T * rt - shared + h->sms - 1) / h->sms) + (double)shared / h->sms;
+        if (c.RT == 0 || turns * (kOutTile + nt) < best) {
+            best = turns * (kOutTile + nt);
+            c.RT = rt;
+            c.NT = nt;
+            c.shared_tiles = shared;
+        }
+    }
     c.slots = (int)h->slots;
     c.Q = h->Q;
     c.max_pieces = (int)h->max_pieces(c.NT);
@@ -904,19 +1092,37 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     c.scale = h->scale;
     c.xp = h->xp;
     c.tp = h->tp;
+    c.zero = h->zero;
     c.list = h->list;
     c.count = h->count;
     c.acc = h->acc;
     c.arrived = h->arrived;
     c.error = h->error;
     c.buffers = c.NT <= 64 ? 2 : 1;  // 4 sums x NT columns each, 512 in all
-    const int stage = kItem + c.NT * 256;
-    c.ring = std::min(kMaxRing, (h->smem - kHeader) / stage);
+    c.D = c.NT < 96 ? 8 : 4;
+    c.C = c.P / c.D;
+    const int stage = c.D * (kPiece + c.NT * 32), header = header_bytes(c.RT);
+    c.ring = std::min(kMaxRing, (kProjectSmem - header) / stage);
     const int grid = (int)std::min<int64_t>(h->sms, (int64_t)c.T * c.RT * c.C);
-    const int64_t blocks = (int64_t)c.RT * c.C + (c.slot ? c.RT + (int64_t)rows * c.Q : 0);
-    cudaError_t e = launch((const void *)k_prepare, (int)blocks, kPrepareThreads, 0, c, s);
+    // A shared tile is cut into equal parts where that leaves at most a quarter of the CTAs
+    // without one (every part then belongs to one tile only), else the line of all
+    // their stages is cut evenly.
+    const int parts = c.shared_tiles ? grid / c.shared_tiles : 0;
+    c.sharers = 4 * parts * c.shared_tiles >= 3 * grid ? parts * c.shared_tiles : grid;
+    // t: a block per row and 4 ranks while that is few blocks (most end at once: the
+    // first row of 8 of an adapter does the work), else per 8 rows and 16 ranks; k is
+    // cut so that a warp has about 512 inputs, over up to 8 blocks of a cluster
+    const bool few = c.slot && (int64_t)rows * c.Q * 4 <= 4 * h->sms;
+    c.span = few || rows <= kRowTile ? 1 : kGroup;
+    c.ranks = few ? 4 : 16;
+    const int forms = c.slot ? (int)((rows + c.span - 1) / c.span) * c.Q * (16 / c.ranks) : 0;
+    c.ksplit = 1;
+    while (few && c.ksplit < kMaxSplit && c.K > 4 * 512 * c.ksplit) c.ksplit *= 2;
+    const dim3 blocks((unsigned)(forms + (c.RT * (c.P / 8) + c.ksplit - 1) / c.ksplit + (c.slot ? c.RT : 0)), (unsigned)c.ksplit);
+    cudaError_t e = launch((const void *)k_prepare, blocks, c.ksplit, kPrepareThreads, 0, c, s);
     if (e == cudaSuccess)
-        e = launch((const void *)k_project, grid, kProjectThreads, kHeader + (size_t)c.ring * stage, c, s);
+        e = launch(c.D == 8 ? (const void *)k_project<8> : (const void *)k_project<4>, dim3((unsigned)grid), 1, kProjectThreads,
+                   header + (size_t)c.ring * stage, c, s);
     return e == cudaSuccess ? LLMX_OK : cuda_fail("project", e);
 }
 
