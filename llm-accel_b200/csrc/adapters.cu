@@ -732,25 +732,54 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
             }
             tc_fence_after();
             const uint32_t t0 = tmem + ((uint32_t)(q4 * 32) << 16) + (uint32_t)(b * 4 * NT);
-            auto put = [&](int r, int64_t s) {
-                const int32_t v = sat32(rnd(s, 4));
-                const size_t at = ((size_t)k.rt * NT + r) * c.ld_out + o;
-                if (c.wide) static_cast<int32_t *>(c.out)[at] = v;
-                else static_cast<int16_t *>(c.out)[at] = (int16_t)sat16(rnd(v, 8));
-            };
-            for (int r0 = 8 * half; r0 < rows; r0 += 16) {
-                uint32_t v[32];
-                tmem_ld4x8(t0 + r0, t0 + NT + r0, t0 + 2 * NT + r0, t0 + 3 * NT + r0, v);
+            // 8 rows at a time: sums from the accumulators, or (a shared tile's last CTA) from
+            // memory, into the results or added to memory.  One body for all three
+            // keeps the code small: it runs once or twice per CTA, mostly uncached.
+            auto rows8 = [&](bool summed, bool add) {
+#pragma unroll 1
+                for (int r0 = 8 * half; r0 < rows; r0 += 16) {
+                    int64_t sum[8];
+                    unsigned long long *at = acc + (size_t)r0 * kOutTile;
+                    const int n = min(8, rows - r0);
+                    if (summed) {
 #pragma unroll
-                for (int r = 0; r < 8; r++) {
-                    if (r0 + r >= rows) break;
-                    const int64_t s = (int64_t)(int32_t)v[r] * 65536 +
-                                      ((int64_t)(int32_t)v[8 + r] + (int64_t)(int32_t)v[16 + r]) * 256 +
-                                      (int64_t)(int32_t)v[24 + r] + corr;
-                    if (!whole) atomicAdd(acc + (size_t)(r0 + r) * kOutTile, (unsigned long long)s);
-                    else if (live) put(r0 + r, s);
+                        for (int r = 0; r < 8; r++) sum[r] = r < n ? (int64_t)__ldcg(at + r * kOutTile) : 0;
+                    } else {
+                        uint32_t v[32];
+                        tmem_ld4x8(t0 + r0, t0 + NT + r0, t0 + 2 * NT + r0, t0 + 3 * NT + r0, v);
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            sum[r] = (int64_t)(int32_t)v[r] * 65536 +
+                                     ((int64_t)(int32_t)v[8 + r] + (int64_t)(int32_t)v[16 + r]) * 256 +
+                                     (int64_t)(int32_t)v[24 + r] + corr;
+                    }
+                    if (add) {
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (r < n) atomicAdd(at + r * kOutTile, (unsigned long long)sum[r]);
+                        continue;
+                    }
+                    if (summed) {
+#pragma unroll
+                        for (int r = 0; r < 8; r++)
+                            if (r < n) at[r * kOutTile] = 0;  // ready for the next call
+                    }
+                    if (!live) continue;
+                    const size_t first = ((size_t)k.rt * NT + r0) * c.ld_out + o;
+                    if (c.wide) {
+                        int32_t *out = static_cast<int32_t *>(c.out) + first;
+#pragma unroll
+                        for (int r = 0; r < 8; r++, out += c.ld_out)
+                            if (r < n) *out = sat32(rnd(sum[r], 4));
+                    } else {
+                        int16_t *out = static_cast<int16_t *>(c.out) + first;
+#pragma unroll
+                        for (int r = 0; r < 8; r++, out += c.ld_out)
+                            if (r < n) *out = (int16_t)sat16(rnd(sat32(rnd(sum[r], 4)), 8));
+                    }
                 }
-            }
+            };
+            rows8(false, !whole);
             tc_fence_before();
             mbar_arrive(tempty + b);
             if (!whole) {
@@ -765,21 +794,7 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
                 }
                 named_sync(3, kResultThreads);
                 if (*last_s) {
-                    for (int r0 = 8 * half; r0 < rows; r0 += 32) {  // 16 rows' sums in flight
-                        int64_t s[16];
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int row = r0 + (r & 7) + (r >> 3) * 16;
-                            s[r] = row < rows ? (int64_t)__ldcg(acc + (size_t)row * kOutTile) : 0;
-                        }
-#pragma unroll
-                        for (int r = 0; r < 16; r++) {
-                            const int row = r0 + (r & 7) + (r >> 3) * 16;
-                            if (row >= rows) continue;
-                            acc[(size_t)row * kOutTile] = 0;  // ready for the next call
-                            if (live) put(row, s[r]);
-                        }
-                    }
+                    rows8(true, false);
                     if (threadIdx.x == 64) c.arrived[b_lo] = 0;
                 }
             }
