@@ -416,7 +416,8 @@ size_t llmx_verify_workspace_bytes(uint32_t requests, uint32_t drafts, uint32_t 
  *                 is rejected
  *   offsets       device, [requests + 1], offsets[0] = 0, offsets[requests] = drafts; a request
  *                 whose pair of offsets is out of order, outside [0, drafts] or more than
- *                 max_drafts apart gets accepted = 0xffffffff and no tokens
+ *                 max_drafts apart gets accepted = 0xffffffff and no tokens (where
+ *                 others then claim the same row, theirs are unspecified)
  *   requests      1 to 65535, drafts: their sum of k_b, max_drafts: the largest k_b (0 to 1023)
  *   temperature   device, float per request
  *   accept_u      device, [drafts] (NULL when drafts is 0); sample_u device, [requests]
