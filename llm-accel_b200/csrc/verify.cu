@@ -10,10 +10,13 @@
 //
 // Two launches.  k_mass reduces every row of logits to its maximum and its
 // sum of weights.  A weight depends on the row's maximum, so a row is read
-// twice; to read it from memory once, a cluster of CTAs holds it in shared
-// memory between the two passes, exchanges the maxima there, and the pieces
-// of its next row arrive while this one is being summed.  k_draw tests the
-// drafts of a request and draws its last token, a cluster per request.
+// twice, by a cluster of CTAs that exchange their maxima through shared memory.
+// The sums are bound by instructions (some 20 per logit), not by memory.  With
+// few rows, for latency, a cluster is so large that it holds a row in
+// shared memory between the passes.  With many it is small, and takes the next row's
+// first pass chunk by chunk beside this row's second, whose chunks come
+// again, from L2: the loads are even, and no exchange is waited for.  k_draw tests
+// the drafts of a request and draws its last token, a cluster per request.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -47,8 +50,7 @@ constexpr int kMaxCluster = 16;
 
 // What a row of logits is reduced to, as k_mass leaves it: every CTA of the
 // row's cluster writes its part, the sum of its weights or (greedy) the first
-// position of the maximum in its share.
-constexpr unsigned long long kNoPart = ~0ull;   // greedy: not here
+// position of the maximum in its share (kNoToken: not there).
 constexpr unsigned long long kGaveUp = ~1ull;   // a wait of the CTA ran out
 struct RowPart {
     int32_t top;
@@ -70,7 +72,7 @@ struct Args {
     uint32_t total;  // rows
     int split;       // CTAs per row (k_mass), and of a cluster there
     int ring;        // chunks of shared memory per CTA
-    int resident;    // a CTA's share of a row fits the ring
+    int resident;    // the ring holds a CTA's share of a row: it is loaded once
     unsigned long long minus_zero;  // two -0.0f (mul2)
 };
 
@@ -110,41 +112,74 @@ static __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// floor(2^31 * 2^-e), e = (top - z) * scale capped at 100, of two logits.  Every
-// float step is rounded on its own (no contraction), so that the weight is the
-// same integer wherever it is computed.  2^x = 2^round(x) 2^f and 2^f on
-// [-1/2, 1/2] is 1 + f q(f), q of degree 4 fitted to the relative error at
-// Chebyshev points: below 2e-7 with the rounding of its steps.  x = -e; adding
-// 1.5 * 2^23 rounds it to the nearest whole number (even at ties) and leaves that number in the
-// low bits, from where one shifted addition puts it into the exponent.  The
-// cap keeps the exponent in range; beyond e = 32 the weight is 0 anyway.  The
-// coefficients carry the 2^31.  Packed pairs halve the float instructions, which
-// are what a row's second pass spends its time on.
-static __device__ __forceinline__ void soft_weight2(int32_t z0, int32_t z1, int32_t top, f32x2 minus_scale, f32x2 mz, uint32_t &w0,
-                                                    uint32_t &w1) {
-    const f32x2 magic = pack2(12582912.0f, 12582912.0f), minus_magic = pack2(-12582912.0f, -12582912.0f);
-    float x0 = __uint2float_rn((uint32_t)top - (uint32_t)z0), x1 = __uint2float_rn((uint32_t)top - (uint32_t)z1);
-    unpack2(mul2(pack2(x0, x1), minus_scale, mz), x0, x1);
-    const f32x2 x = pack2(fmaxf(x0, -100.0f), fmaxf(x1, -100.0f));
-    const f32x2 m = add2(x, magic), r = add2(m, minus_magic);
-    float r0, r1, m0, m1, p0, p1;
-    unpack2(r, r0, r1);
-    const f32x2 f = add2(x, pack2(-r0, -r1));
-    f32x2 p = add2(mul2(f, pack2(0x1.5bba12p21f, 0x1.5bba12p21f), mz), pack2(0x1.3cea88p24f, 0x1.3cea88p24f));
-    p = add2(mul2(p, f, mz), pack2(0x1.c6b752p26f, 0x1.c6b752p26f));
-    p = add2(mul2(p, f, mz), pack2(0x1.ebf9bcp28f, 0x1.ebf9bcp28f));
-    p = add2(mul2(p, f, mz), pack2(0x1.62e42ap30f, 0x1.62e42ap30f));
-    p = add2(mul2(p, f, mz), pack2(0x1p31f, 0x1p31f));
-    unpack2(m, m0, m1);
-    unpack2(p, p0, p1);
-    w0 = __float2uint_rz(__int_as_float(__float_as_int(p0) + (__float_as_int(m0) << 23)));
-    w1 = __float2uint_rz(__int_as_float(__float_as_int(p1) + (__float_as_int(m1) << 23)));
+static __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
 }
-// Whether an excluded logit needs a test of its own: not when its difference to the
-// maximum is 40 octaves or more, where the weight is 0 by the formula.
-static __device__ __forceinline__ bool must_test_excluded(int32_t top, float scale) {
-    return !(__fmul_rn(__uint2float_rn((uint32_t)top - (uint32_t)kExcluded), scale) >= 40.0f);
-}
+
+// floor(2^31 * 2^-e), e = (top - z) * scale capped at 100, of the logits of one
+// row.  Every float step of the definition is rounded on its own, so that the
+// weight is the same integer wherever it is computed.
+//   2^x = 2^round(x) 2^f, and 2^f on [-1/2, 1/2] is 1 + f q(f), q of degree 4 fitted
+// to the relative error at Chebyshev points: below 2e-7 with the rounding of its
+// steps.  Here x = -e; adding 1.5 * 2^23 rounds it to the nearest whole number
+// (even at ties) and leaves that number in the low bits, from where one shifted
+// addition puts it into the exponent.  The coefficients carry the 2^31.  Packed
+// pairs halve the float instructions, which a row's second pass spends most of its time on.
+//   The usual row (fast) needs no conversion to float: with d = top - z below
+// 2^23, the bits of 2^23 + d are 0x4b000000 + d, and (2^23 + d) (-scale) + 2^23 scale in one
+// fused step is d (-scale) rounded once (2^23 scale is exact).  A d of 32 / scale
+// or more has a weight of 0, as has any larger one, so d is cut there in
+// whole numbers; that needs 32 / scale < 2^23 (T below 5.7) and a maximum so low
+// that 0x4b000000 + d cannot pass 2^32.  The other rows convert and cap as defined.
+struct RowWeight {
+    int32_t top;
+    float scale;
+    bool greedy, fast, test;  // test: an excluded logit is not far enough below the maximum to vanish by itself
+    uint32_t base, most;      // fast: 0x4b000000 + top, 0x4b000000 + the largest d
+    f32x2 minus_scale, shift, mz;
+
+    __device__ __forceinline__ void set(int32_t t, float s, f32x2 minus_zero) {
+        top = t;
+        scale = s;
+        greedy = s < 0.0f;
+        test = !(__fmul_rn(__uint2float_rn((uint32_t)t - (uint32_t)kExcluded), s) >= 33.0f);
+        const float limit = __fdiv_rn(32.0f, s);
+        fast = !greedy && !test && limit < 8388000.0f && t < 889192448;
+        base = 0x4b000000u + (uint32_t)t;
+        most = 0x4b000000u + (fast ? __float2uint_ru(limit) : 0u);
+        minus_scale = pack2(-s, -s);
+        shift = pack2(8388608.0f * s, 8388608.0f * s);
+        mz = minus_zero;
+    }
+    // the second half, from x = -e
+    __device__ __forceinline__ void finish(f32x2 x, uint32_t &w0, uint32_t &w1) const {
+        const f32x2 magic = pack2(12582912.0f, 12582912.0f), minus_magic = pack2(-12582912.0f, -12582912.0f);
+        const f32x2 m = add2(x, magic), f = fma2(add2(m, minus_magic), pack2(-1.0f, -1.0f), x);
+        f32x2 p = add2(mul2(f, pack2(0x1.5bba12p21f, 0x1.5bba12p21f), mz), pack2(0x1.3cea88p24f, 0x1.3cea88p24f));
+        p = add2(mul2(p, f, mz), pack2(0x1.c6b752p26f, 0x1.c6b752p26f));
+        p = add2(mul2(p, f, mz), pack2(0x1.ebf9bcp28f, 0x1.ebf9bcp28f));
+        p = add2(mul2(p, f, mz), pack2(0x1.62e42ap30f, 0x1.62e42ap30f));
+        p = add2(mul2(p, f, mz), pack2(0x1p31f, 0x1p31f));
+        float m0, m1, p0, p1;
+        unpack2(m, m0, m1);
+        unpack2(p, p0, p1);
+        w0 = __float2uint_rz(__int_as_float(__float_as_int(p0) + (__float_as_int(m0) << 23)));
+        w1 = __float2uint_rz(__int_as_float(__float_as_int(p1) + (__float_as_int(m1) << 23)));
+    }
+    __device__ __forceinline__ void fast2(int32_t z0, int32_t z1, uint32_t &w0, uint32_t &w1) const {
+        const uint32_t d0 = min(base - (uint32_t)z0, most), d1 = min(base - (uint32_t)z1, most);
+        finish(fma2(pack2(__uint_as_float(d0), __uint_as_float(d1)), minus_scale, shift), w0, w1);
+    }
+    __device__ __forceinline__ void slow2(int32_t z0, int32_t z1, uint32_t &w0, uint32_t &w1) const {
+        float x0 = __uint2float_rn((uint32_t)top - (uint32_t)z0), x1 = __uint2float_rn((uint32_t)top - (uint32_t)z1);
+        unpack2(mul2(pack2(x0, x1), minus_scale, mz), x0, x1);
+        finish(pack2(fmaxf(x0, -100.0f), fmaxf(x1, -100.0f)), w0, w1);
+        w0 = z0 == kExcluded ? 0u : w0;
+        w1 = z1 == kExcluded ? 0u : w1;
+    }
+};
 
 // A row's numbers as k_draw uses them.
 struct RowMass {
@@ -153,42 +188,52 @@ struct RowMass {
     uint32_t first;    // greedy: the maximum's first position
     uint32_t inverse;  // floor(2^62 / (S >> h)), 0 when nothing is left
     int32_t shift;     // 22 + h
-    bool ok;
+    int ok;
 };
+// From the parts of a row, by half a warp: its lanes hold a part each.
 static __device__ RowMass load_row(const RowPart *rows, uint32_t row, int split) {
+    const int i = threadIdx.x & (kMaxCluster - 1);
     const RowPart *p = rows + row;
     RowMass r;
+    unsigned long long v = i < split ? p->part[i] : 0;
     r.top = p->top;
     r.scale = p->scale;
-    r.first = kNoToken;
-    r.ok = true;
-    unsigned long long sum = 0;
-    for (int i = 0; i < split; i++) {
-        const unsigned long long v = p->part[i];
-        if (v == kGaveUp) r.ok = false;
-        else if (r.scale < 0.0f) r.first = min(r.first, (uint32_t)v);
-        else sum += v;
+    const bool greedy = r.scale < 0.0f;
+    r.ok = !(i < split && v == kGaveUp);
+    uint32_t first = greedy && i < split ? (uint32_t)v : kNoToken;
+    if (greedy) v = 0;
+    for (int o = kMaxCluster / 2; o; o >>= 1) {
+        v += __shfl_xor_sync(~0u, v, o);
+        first = min(first, __shfl_xor_sync(~0u, first, o));
+        r.ok &= __shfl_xor_sync(~0u, r.ok, o);
     }
-    if (r.scale < 0.0f) sum = r.top != kExcluded && r.first != kNoToken ? 1ull << 31 : 0;
+    r.first = first;
+    const unsigned long long sum = greedy ? (r.top != kExcluded && first != kNoToken ? 1ull << 31 : 0) : v;
     int h = 32 - __clzll((long long)sum);  // sum has 64 - clz bits; 32 remain
     h = h < 0 ? 0 : h;
     r.inverse = sum ? (uint32_t)((1ull << 62) / (sum >> h)) : 0u;
     r.shift = 22 + h;
     return r;
 }
-static __device__ __forceinline__ void row_weight2(const RowMass &r, f32x2 mz, int32_t z0, int32_t z1, uint32_t v0,
+static __device__ __forceinline__ void row_weight2(const RowWeight &w, uint32_t first, int32_t z0, int32_t z1, uint32_t v0,
                                                    uint32_t v1, uint32_t &w0, uint32_t &w1) {
-    if (r.scale < 0.0f) {
-        w0 = v0 == r.first ? 0x80000000u : 0u;
-        w1 = v1 == r.first ? 0x80000000u : 0u;
+    if (w.fast) {
+        w.fast2(z0, z1, w0, w1);
+    } else if (w.greedy) {
+        w0 = v0 == first && z0 != kExcluded ? 0x80000000u : 0u;
+        w1 = v1 == first && z1 != kExcluded ? 0x80000000u : 0u;
     } else {
-        soft_weight2(z0, z1, r.top, pack2(-r.scale, -r.scale), mz, w0, w1);
+        w.slow2(z0, z1, w0, w1);
     }
-    if (z0 == kExcluded) w0 = 0;
-    if (z1 == kExcluded) w1 = 0;
 }
 static __device__ __forceinline__ uint64_t row_share(uint32_t w, const RowMass &r) {
     return ((uint64_t)w * r.inverse) >> r.shift;
+}
+// The same for shifts below 32 (a sum of weights below 2^42: the usual row).
+static __device__ __forceinline__ uint64_t row_share_small(uint32_t w, const RowMass &r) {
+    const uint64_t v = (uint64_t)w * r.inverse;
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    return ((uint64_t)(hi >> r.shift) << 32) | __funnelshift_r(lo, hi, r.shift);
 }
 // floor(a * u / 2^32)
 static __device__ __forceinline__ uint64_t mul_frac(uint64_t a, uint32_t u) { return __umul64hi(a, (uint64_t)u << 32); }
@@ -223,10 +268,11 @@ static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t
 // ---------------------------------------------------------------------------
 // rows -> maxima and sums
 // ---------------------------------------------------------------------------
-constexpr int kMassWarps = 16, kMassThreads = (kMassWarps + 2) * 32;  // sums, loads, the rows' requests
-constexpr int kChunk = 4096;                                          // logits per chunk: two 16-byte vectors per thread
+constexpr int kMassWarps = 16, kMassThreads = (kMassWarps + 3) * 32;  // sums, loads (two), the rows' requests
+constexpr int kChunk = 4096;                                          // logits per chunk
 constexpr int kChunkBytes = kChunk * 4;
-constexpr int kMaxRing = 13;
+constexpr int kMaxRing = 12, kFirstRing = 8;  // chunks in shared memory; of these a row's first pass has, where it has its own
+constexpr int kTops = 4;                      // rows whose exchange may be under way: see k_mass
 
 // A row's logits: a head of at most 3 up to a 16-byte boundary, vectors of 4, a
 // tail of at most 3.  CTA `rank` of `split` takes an even share of the
@@ -239,8 +285,8 @@ struct Row {
         z = row < targets ? a.target + row * a.ld_target : a.draft + (row - targets) * a.ld_draft;
         head = min(a.vocab, (uint32_t)((16 - ((uintptr_t)z & 15)) & 15) >> 2);
         vectors = (a.vocab - head) >> 2;
-        v0 = (uint32_t)((uint64_t)vectors * rank / a.split);
-        v1 = (uint32_t)((uint64_t)vectors * (rank + 1) / a.split);
+        v0 = vectors * rank / a.split;  // below 2^20 * 16
+        v1 = vectors * (rank + 1) / a.split;
     }
 };
 
@@ -276,29 +322,59 @@ static __device__ uint32_t owner_of(const Args &a, uint32_t row) {
     return kNoToken;
 }
 
+// A CTA's part in a row, and what a thread knows of it between the passes.
+struct Held {
+    Row r;
+    int chunks;
+    uint32_t edge_at;  // this thread's logit of the head or tail, if any
+    int32_t edge;
+    __device__ __forceinline__ Held(const Args &a, uint32_t row, int rank, bool there) : r(a, there ? row : 0, rank) {
+        chunks = there ? (int)((r.v1 - r.v0 + kChunk / 4 - 1) / (kChunk / 4)) : 0;
+        edge_at = kNoToken;
+        edge = kExcluded;
+        const uint32_t tail = r.head + r.vectors * 4;
+        if (threadIdx.x < 3 && rank == 0 && threadIdx.x < r.head) edge_at = threadIdx.x;
+        if (threadIdx.x >= 4 && threadIdx.x < 7 && rank == a.split - 1 && tail + threadIdx.x - 4 < a.vocab)
+            edge_at = tail + threadIdx.x - 4;
+        if (edge_at != kNoToken) edge = r.z[edge_at];
+    }
+};
+
+// No barrier over the CTA: the last warp to add its maximum (or sum) passes
+// the CTA's on.  A CTA's own buffers alternate between rows; the maxima of the cluster
+// arrive in one of four places: a CTA sends row i + 4's after its second pass of i + 2,
+// so after every CTA has sent i + 2's, and a warp adds to those after it has read i's.
+//
+// A chunk is one group's of GW warps.  kTwice: rows are loaded twice, each pass
+// through a ring of its own (slots [0, kFirstRing) and the rest), and the first pass
+// of the next row goes beside the second of this one; else through one ring,
+// in which a row stays until it is summed.
+template <bool kTwice, int GW>
 __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
+    constexpr int kGroups = kMassWarps / GW, kVectors = kChunk / 4 / (GW * 32);  // 16-byte vectors per thread and chunk
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t full[kMaxRing], empty[kMaxRing];
     __shared__ uint64_t info_full[2], info_empty[2];  // a row's temperature
-    __shared__ uint64_t top_full[2];                  // every CTA's maximum of the row
+    __shared__ uint64_t top_full[kTops];              // every CTA's maximum of the row
     __shared__ float scale_s[2];
-    __shared__ int32_t tops[2][kMaxCluster];
-    __shared__ int32_t warp_top[kMassWarps];
+    __shared__ int32_t tops[kTops][kMaxCluster];
+    __shared__ int32_t warp_top[2][kMassWarps];
     __shared__ unsigned long long warp_part[2][kMassWarps];
+    __shared__ int top_count[2], part_count[2];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = a.split, rank = S > 1 ? (int)cluster_rank() : 0;
     const uint32_t group = blockIdx.x / S, groups = gridDim.x / S;
-    const int passes = a.resident ? 1 : 2;  // times that a row is loaded
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.ring; i++) {
             mbar_init(full + i, 1);
-            mbar_init(empty + i, kMassWarps);
+            mbar_init(empty + i, GW);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(info_full + i, 1);
             mbar_init(info_empty + i, kMassWarps);
-            mbar_init(top_full + i, S);
+            top_count[i] = part_count[i] = 0;
         }
+        for (int i = 0; i < kTops; i++) mbar_init(top_full + i, S);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (S > 1) cluster_sync();
@@ -306,34 +382,38 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
     pdl_wait();
     pdl_trigger();
 
-    if (warp == kMassWarps) {  // ---- loads ------------------------------------------
-        if (lane == 0) {
+    if (warp == kMassWarps || warp == kMassWarps + 1) {  // ---- loads, of the first pass and of the second -----
+        if (lane == 0 && (kTwice || warp == kMassWarps)) {
+            const int base = warp == kMassWarps ? 0 : kFirstRing;
+            const int ring = !kTwice ? a.ring : warp == kMassWarps ? kFirstRing : a.ring - kFirstRing;
             int s = 0, phase = 1, issued = 0;
             bool ok = true;
             for (uint32_t row = group; ok && row < a.total; row += groups) {
                 const Row r(a, row, rank);
-                for (int pass = 0; ok && pass < passes; pass++)
-                    for (uint32_t v = r.v0; v < r.v1; v += kChunk / 4) {
-                        if (issued >= a.ring && !mbar_wait(empty + s, phase)) {
-                            ok = false;
-                            break;
-                        }
-                        const uint32_t bytes = min(r.v1 - v, (uint32_t)kChunk / 4) * 16;
-                        mbar_expect_tx(full + s, bytes);
-                        bulk_g2s(smem + s * kChunkBytes, r.z + r.head + (size_t)v * 4, bytes, full + s);
-                        issued++;
-                        if (++s == a.ring) {
-                            s = 0;
-                            phase ^= 1;
-                        }
+                for (uint32_t v = r.v0; v < r.v1; v += kChunk / 4) {
+                    const int at = base + s;
+                    if (issued >= ring && !mbar_wait(empty + at, phase)) {
+                        ok = false;
+                        break;
                     }
+                    const uint32_t bytes = min(r.v1 - v, (uint32_t)kChunk / 4) * 16;
+                    mbar_expect_tx(full + at, bytes);
+                    bulk_g2s(smem + at * kChunkBytes, r.z + r.head + (size_t)v * 4, bytes, full + at);
+                    issued++;
+                    if (++s == ring) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
             }
-            for (int q = 0; !ok && q < a.ring && q < issued; q++) {  // the copies in flight land before the CTA ends
-                const int last = q + ((issued - 1 - q) / a.ring) * a.ring;
-                (void)mbar_wait(full + q, (last / a.ring) & 1);
+            for (int q = 0; !ok && q < ring && q < issued; q++) {  // the copies in flight land before the CTA ends
+                const int last = q + ((issued - 1 - q) / ring) * ring;
+                (void)mbar_wait(full + base + q, (last / ring) & 1);
             }
         }
-    } else if (warp == kMassWarps + 1) {  // ---- the rows' temperatures --------------------
+        return;
+    }
+    if (warp == kMassWarps + 2) {  // ---- the rows' temperatures --------------------------
         uint32_t i = 0;
         for (uint32_t row = group; row < a.total; row += groups, i++) {
             const uint32_t b = owner_of(a, row);
@@ -345,148 +425,231 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
             }
             __syncwarp();
         }
-    } else {  // ---- maxima and sums ----------------------------------------------------
-        int s = 0, phase = 0;
-        uint32_t i = 0;
-        bool ok = true;
-        for (uint32_t row = group; row < a.total; row += groups, i++) {
-            if (!ok) {  // a wait ran out: this row and the rest have no sums
-                if (threadIdx.x == 0) a.rows[row].part[rank] = kGaveUp;
-                continue;
+        return;
+    }
+
+    // ---- maxima and sums ---------------------------------------------------------------
+    const int mine = warp / GW, gt = (warp % GW) * 32 + lane;
+    bool ok = true;
+    // A place in a ring of n slots from slot `base` on, moved by chunks.  Slot s is always
+    // group s mod kGroups's (n is a multiple of kGroups): a warp then meets every phase of the
+    // barriers that it waits on, and cannot take an older phase for the one it needs.
+    struct Place {
+        int at, phase, base, n;
+        __device__ __forceinline__ void move(int by) {
+            at += by;
+            while (at >= n) {
+                at -= n;
+                phase ^= 1;
             }
-            const Row r(a, row, rank);
-            const int b = i & 1;
-            // the head and the tail, one logit of a thread
-            int32_t edge = kExcluded;
-            uint32_t edge_at = kNoToken;
-            if (threadIdx.x < 3 && rank == 0 && threadIdx.x < r.head) edge_at = threadIdx.x;
-            const uint32_t tail = r.head + r.vectors * 4;
-            if (threadIdx.x >= 4 && threadIdx.x < 7 && rank == S - 1 && tail + threadIdx.x - 4 < a.vocab)
-                edge_at = tail + threadIdx.x - 4;
-            if (edge_at != kNoToken) edge = r.z[edge_at];
-            int32_t top = edge;
-            const int s0 = s, phase0 = phase;
-            for (uint32_t v = r.v0; ok && v < r.v1; v += kChunk / 4) {
-                ok = mbar_wait(full + s, phase);
-                const int4 *p = reinterpret_cast<const int4 *>(smem + s * kChunkBytes);
-                const int n = min(r.v1 - v, (uint32_t)kChunk / 4);
+        }
+        __device__ __forceinline__ int slot() const { return base + at; }
+        // moves to the group's first chunk from here on, and says how far that is
+        __device__ __forceinline__ int own(int group) {
+            const int by = (group + kGroups - at % kGroups) % kGroups;
+            move(by);
+            return by;
+        }
+    };
+    static_assert(kFirstRing % kGroups == 0 && kMaxRing % kGroups == 0, "a slot is one group's");
+    // whether this warp, whose lane 0 has just written its word, is the last of the CTA to
+    // come here; it then sees the others' words
+    auto last_of = [&](int *count) {
+        int old = 0;
+        if (lane == 0) {
+            asm volatile("atom.acq_rel.cta.shared::cta.add.s32 %0, [%1], 1;" : "=r"(old) : "r"(smem_u32(count)) : "memory");
+            if (old == kMassWarps - 1) *count = 0;
+        }
+        return __shfl_sync(~0u, old, 0) == kMassWarps - 1;
+    };
+    // this thread's vectors of a chunk: the first, and how far the chunk goes from there
+    auto vectors_of = [&](const Row &r, int at, int c, const int4 *&p) {
+        p = reinterpret_cast<const int4 *>(smem + at * kChunkBytes) + gt;
+        return (int)min(r.v1 - r.v0 - c * (kChunk / 4), (uint32_t)kChunk / 4) - gt;
+    };
+    constexpr int kStride = GW * 32;
+    int32_t top = kExcluded;  // of the row in its first pass
+    auto first_chunk = [&](const Row &r, int at, int c) {
+        const int4 *p;
+        const int n = vectors_of(r, at, c, p);
+        int4 q[kVectors];
 #pragma unroll
-                for (int u = 0; u < kChunk / 4; u += kMassWarps * 32) {
-                    const int at = u + threadIdx.x;
-                    if (at < n) {
-                        const int4 q = p[at];
-                        top = max(max(top, q.x), max(max(q.y, q.z), q.w));
-                    }
-                }
-                if (!a.resident) {
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(empty + s);
-                }
-                if (++s == a.ring) {
-                    s = 0;
-                    phase ^= 1;
-                }
-            }
-            top = __reduce_max_sync(~0u, top);
-            if (lane == 0) warp_top[warp] = top;
-            asm volatile("bar.sync 1, %0;" ::"n"(kMassWarps * 32) : "memory");
-            top = __reduce_max_sync(~0u, warp_top[lane & (kMassWarps - 1)]);
-            if (S > 1) {  // push it to every CTA of the cluster, wait for theirs
-                if (warp == 0 && lane < S) {
-                    asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote(&tops[b][rank], lane)), "r"(top) : "memory");
-                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(top_full + b, lane))
-                                 : "memory");
-                }
-                ok = mbar_wait_cluster(top_full + b, (i >> 1) & 1) && ok;
-                top = __reduce_max_sync(~0u, lane < S ? tops[b][lane] : kExcluded);
-            }
-            ok = mbar_wait(info_full + b, (i >> 1) & 1) && ok;
-            const float scale = scale_s[b];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(info_empty + b);
-            unsigned long long sum = 0;
-            const bool greedy = scale < 0.0f, test = must_test_excluded(top, scale);
-            const f32x2 minus_scale = pack2(-scale, -scale);
-            uint32_t first = kNoToken;
-            if (edge_at != kNoToken) {
-                uint32_t w, none;
-                soft_weight2(edge, edge, top, minus_scale, a.minus_zero, w, none);
-                sum = edge == kExcluded ? 0 : w;
-                if (edge == top) first = edge_at;
-            }
-            if (a.resident) {
-                s = s0;
-                phase = phase0;
-            }
-            for (uint32_t v = r.v0; ok && v < r.v1; v += kChunk / 4) {
-                if (!a.resident) ok = mbar_wait(full + s, phase);
-                const int4 *p = reinterpret_cast<const int4 *>(smem + s * kChunkBytes);
-                const int n = min(r.v1 - v, (uint32_t)kChunk / 4);
+        for (int u = 0; u < kVectors; u++)
+            q[u] = u * kStride < n ? p[u * kStride] : make_int4(kExcluded, kExcluded, kExcluded, kExcluded);
 #pragma unroll
-                for (int u = 0; u < kChunk / 4; u += kMassWarps * 32) {
-                    const int at = u + threadIdx.x;
-                    if (at < n) {
-                        const int4 q = p[at];
-                        if (!greedy) {
-                            uint32_t w0, w1, w2, w3;
-                            soft_weight2(q.x, q.y, top, minus_scale, a.minus_zero, w0, w1);
-                            soft_weight2(q.z, q.w, top, minus_scale, a.minus_zero, w2, w3);
-                            if (test) {
-                                w0 = q.x == kExcluded ? 0u : w0;
-                                w1 = q.y == kExcluded ? 0u : w1;
-                                w2 = q.z == kExcluded ? 0u : w2;
-                                w3 = q.w == kExcluded ? 0u : w3;
-                            }
-                            sum += (unsigned long long)w0 + w1;
-                            sum += (unsigned long long)w2 + w3;
-                        } else {
-                            const uint32_t e = r.head + (v + at) * 4;
-                            if (q.w == top) first = min(first, e + 3);
-                            if (q.z == top) first = min(first, e + 2);
-                            if (q.y == top) first = min(first, e + 1);
-                            if (q.x == top) first = min(first, e);
-                        }
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(empty + s);
-                if (++s == a.ring) {
-                    s = 0;
-                    phase ^= 1;
-                }
+        for (int u = 0; u < kVectors; u++) top = max(max(top, q[u].x), max(max(q[u].y, q[u].z), q[u].w));
+    };
+    // row number i's maximum, sent to every CTA of the cluster
+    auto send_top = [&](uint32_t i, int32_t edge) {
+        top = __reduce_max_sync(~0u, max(top, edge));
+        if (lane == 0) warp_top[i & 1][warp] = top;
+        if (last_of(&top_count[i & 1])) {
+            top = __reduce_max_sync(~0u, lane < kMassWarps ? warp_top[i & 1][lane] : kExcluded);
+            if (lane < S) {
+                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote(&tops[i % kTops][rank], lane)), "r"(top) : "memory");
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(top_full + i % kTops, lane))
+                             : "memory");
             }
-            if (greedy) {
-                first = __reduce_min_sync(~0u, first);
-                sum = first == kNoToken ? kNoPart : first;
+        }
+        top = kExcluded;
+        __syncwarp();
+    };
+    RowWeight rw;  // of the row in its second pass
+    unsigned long long sum = 0;
+    uint32_t first = kNoToken;
+    auto begin_second = [&](const Held &h, uint32_t i) {
+        ok = ok && mbar_wait(info_full + (i & 1), (i >> 1) & 1);
+        const float scale = scale_s[i & 1];
+        __syncwarp();
+        if (lane == 0) mbar_arrive(info_empty + (i & 1));
+        ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1);
+        rw.set(__reduce_max_sync(~0u, lane < S ? tops[i % kTops][lane] : kExcluded), scale, a.minus_zero);
+        sum = 0;
+        first = kNoToken;
+        if (h.edge_at != kNoToken) {
+            uint32_t w, none;
+            rw.slow2(h.edge, h.edge, w, none);
+            sum = w;
+            if (h.edge == rw.top) first = h.edge_at;
+        }
+    };
+    auto second_chunk = [&](const Row &r, int at, int c) {
+        const int4 *p;
+        const int n = vectors_of(r, at, c, p);
+        if (rw.fast) {
+            auto add = [&](const int4 &q) {
+                uint32_t w0, w1, w2, w3;
+                rw.fast2(q.x, q.y, w0, w1);
+                rw.fast2(q.z, q.w, w2, w3);
+                sum += (unsigned long long)w0 + w1;
+                sum += (unsigned long long)w2 + w3;
+            };
+            if ((kVectors - 1) * kStride < n) {
+#pragma unroll
+                for (int u = 0; u < kVectors; u++) add(p[u * kStride]);
             } else {
-                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+#pragma unroll 1
+                for (int u = 0; u * kStride < n; u++) add(p[u * kStride]);
             }
-            // read by thread 0 below before the next but one row's are written
-            if (lane == 0) warp_part[b][warp] = sum;
-            int fine;
-            asm volatile("{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.red.and.pred q, 1, %2, p;\n selp.b32 %0, 1, 0, q;\n}"
-                         : "=r"(fine)
-                         : "r"((int)ok), "n"(kMassWarps * 32)
-                         : "memory");
-            ok = fine != 0;  // all warps go on, or none
-            if (threadIdx.x == 0) {
-                unsigned long long part = greedy ? kNoPart : 0;
-                for (int q = 0; q < kMassWarps; q++) part = greedy ? min(part, warp_part[b][q]) : part + warp_part[b][q];
+            return;
+        }
+#pragma unroll 1
+        for (int u = 0; u * kStride < n; u++) {
+            const int4 q = p[u * kStride];
+            if (rw.greedy) {
+                const uint32_t e = r.head + (r.v0 + c * (kChunk / 4) + gt + u * kStride) * 4;
+                if (q.w == rw.top) first = min(first, e + 3);
+                if (q.z == rw.top) first = min(first, e + 2);
+                if (q.y == rw.top) first = min(first, e + 1);
+                if (q.x == rw.top) first = min(first, e);
+            } else {
+                uint32_t w0, w1, w2, w3;
+                rw.slow2(q.x, q.y, w0, w1);
+                rw.slow2(q.z, q.w, w2, w3);
+                sum += (unsigned long long)w0 + w1;
+                sum += (unsigned long long)w2 + w3;
+            }
+        }
+    };
+    auto end_second = [&](uint32_t row, uint32_t i) {
+        // sums (greedy: the smallest first position) of the warp, then of the CTA
+        auto whole = [&](unsigned long long v) {
+            if (rw.greedy) return (unsigned long long)__reduce_min_sync(~0u, (uint32_t)v);
+            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+            return v;
+        };
+        sum = whole(rw.greedy ? first : sum);
+        if (lane == 0) warp_part[i & 1][warp] = sum;
+        if (last_of(&part_count[i & 1])) {
+            const unsigned long long part =
+                whole(lane < kMassWarps ? warp_part[i & 1][lane] : rw.greedy ? (unsigned long long)kNoToken : 0);
+            if (lane == 0) {
                 RowPart *out = a.rows + row;
-                out->part[rank] = ok ? part : kGaveUp;
+                out->part[rank] = part;
                 if (rank == 0) {
-                    out->top = top;
-                    out->scale = scale;
+                    out->top = rw.top;
+                    out->scale = rw.scale;
                 }
             }
         }
+        __syncwarp();
+    };
+    auto release = [&](int at) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty + at);
+    };
+    uint32_t i = 0;
+    if (!kTwice) {
+        Place place{0, 0, 0, a.ring};
+        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
+            const Held h(a, row, rank, true);
+            Place p = place, q = place;
+            for (int c = p.own(mine); c < h.chunks; c += kGroups, p.move(kGroups)) {
+                ok = ok && mbar_wait(full + p.slot(), p.phase);
+                first_chunk(h.r, p.slot(), c);
+            }
+            send_top(i, h.edge);
+            begin_second(h, i);
+            for (int c = q.own(mine); c < h.chunks; c += kGroups, q.move(kGroups)) {
+                second_chunk(h.r, q.slot(), c);
+                release(q.slot());
+            }
+            end_second(row, i);
+            place.move(h.chunks);
+        }
+    } else {
+        Place first_place{0, 0, 0, kFirstRing}, second_place{0, 0, kFirstRing, a.ring - kFirstRing};
+        auto take_first = [&](const Row &r, Place &p, int c) {
+            ok = ok && mbar_wait(full + p.slot(), p.phase);
+            first_chunk(r, p.slot(), c);
+            release(p.slot());
+            p.move(kGroups);
+        };
+        Held now(a, group, rank, true);
+        Place p = first_place;
+        for (int c = p.own(mine); c < now.chunks; c += kGroups) take_first(now.r, p, c);
+        first_place.move(now.chunks);
+        send_top(0, now.edge);
+        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
+            const bool there = row + groups < a.total;
+            const Held next(a, row + groups, rank, there);
+            Place q = second_place;
+            p = first_place;
+            int c1 = p.own(mine);
+            if (c1 < next.chunks) {  // a chunk ahead, behind which the exchange of this row's maxima passes
+                take_first(next.r, p, c1);
+                c1 += kGroups;
+            }
+            begin_second(now, i);
+            for (int c = q.own(mine); c < now.chunks; c += kGroups, q.move(kGroups)) {
+                if (c1 < next.chunks) {
+                    take_first(next.r, p, c1);
+                    c1 += kGroups;
+                }
+                ok = ok && mbar_wait(full + q.slot(), q.phase);
+                second_chunk(now.r, q.slot(), c);
+                release(q.slot());
+            }
+            for (; c1 < next.chunks; c1 += kGroups) take_first(next.r, p, c1);
+            first_place.move(next.chunks);
+            second_place.move(now.chunks);
+            if (there) send_top(i + 1, next.edge);
+            end_second(row, i);
+            now = next;
+        }
     }
+    // a wait ran out: rows of this cluster may lack sums, and none of them is to be used
+    ok = __all_sync(~0u, ok);
+    if (!ok && lane == 0)
+        for (uint32_t row = group; row < a.total; row += groups) a.rows[row].part[rank] = kGaveUp;
 }
 
 // ---------------------------------------------------------------------------
 // accept tests and the drawn token, a cluster per request
 // ---------------------------------------------------------------------------
 constexpr int kDrawWarps = 16, kDrawThreads = kDrawWarps * 32;
+constexpr int kRuns = 32;
+constexpr uint32_t kKeep = 32;  // rows of a request whose numbers stay in shared memory
 struct DrawArgs {
     Args a;
     int split;  // CTAs per request
@@ -495,12 +658,14 @@ struct DrawArgs {
 __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
     const Args &a = d.a;
     __shared__ uint32_t first_s, bad_s;
-    __shared__ RowMass mt_s, md_s;
+    __shared__ RowMass mass_s[kKeep][2], last_s[2];
     __shared__ unsigned long long warp_sum[kDrawWarps], cta_sum[2][kMaxCluster];
+    __shared__ unsigned long long run_sum[kDrawWarps][kRuns];  // of up to kRuns runs of a warp's steps
     const int S = d.split, rank = S > 1 ? (int)cluster_rank() : 0;
     const uint32_t b = blockIdx.x / S;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
+    if (S > 1) cluster_sync();  // every CTA of the cluster runs before one stores into another
     pdl_wait();
     pdl_trigger();
     uint32_t begin, count;
@@ -511,66 +676,106 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
         bad_s = valid ? 0u : 1u;
     }
     __syncthreads();
-    for (uint32_t j = threadIdx.x; j < count; j += kDrawThreads) {
-        const uint32_t e = begin + j, x = a.draft_tokens[e];
-        uint64_t pq[2] = {0, a.draft ? 0 : 1ull << 40};
-        for (int side = 0; side < (a.draft ? 2 : 1); side++) {
-            const RowMass m = load_row(a.rows, side ? a.drafts + a.requests + e : e + b, a.split);
-            if (!m.ok) bad_s = 1;
-            if (x < a.vocab) {
-                const int32_t z = side ? a.draft[e * a.ld_draft + x] : a.target[(e + b) * a.ld_target + x];
-                uint32_t w, none;
-                row_weight2(m, a.minus_zero, z, z, x, x, w, none);
-                pq[side] = row_share(w, m);
+    const uint32_t targets = a.drafts + a.requests;
+    // a warp per row: its lower half has the target's, its upper half the draft's;
+    // j = count is the row after the last draft
+    for (uint32_t j = warp; valid && j <= count; j += kDrawWarps) {
+        const uint32_t e = begin + j;
+        const bool is_draft = lane >= 16, has = j < count, there = is_draft ? has && a.draft : true;
+        const RowMass m = load_row(a.rows, there && is_draft ? targets + e : e + b, a.split);
+        if (!m.ok && (lane & 15) == 0) bad_s = 1;
+        if ((lane & 15) == 0 && j < kKeep) mass_s[j][lane >> 4] = m;
+        const uint32_t x = has ? a.draft_tokens[e] : kNoToken;
+        uint64_t share = 0;
+        if (x < a.vocab && there) {
+            const int32_t z = is_draft ? a.draft[e * a.ld_draft + x] : a.target[(e + b) * a.ld_target + x];
+            RowWeight rw;
+            rw.set(m.top, m.scale, a.minus_zero);
+            uint32_t w, none;
+            row_weight2(rw, m.first, z, z, x, x, w, none);
+            share = row_share(w, m);
+        }
+        if (is_draft && !a.draft) share = 1ull << 40;
+        const uint64_t p = __shfl_sync(~0u, share, 0), q = __shfl_sync(~0u, share, 16);
+        if (has && lane == 0) {
+            if (a.probs && rank == 0) {
+                a.probs[2 * (size_t)e] = p;
+                a.probs[2 * (size_t)e + 1] = q;
             }
+            if (mul_frac(q, a.accept_u[e]) >= p) atomicMin(&first_s, j);
         }
-        if (a.probs && rank == 0) {
-            a.probs[2 * (size_t)e] = pq[0];
-            a.probs[2 * (size_t)e + 1] = pq[1];
-        }
-        if (mul_frac(pq[1], a.accept_u[e]) >= pq[0]) atomicMin(&first_s, j);
     }
     __syncthreads();
     const uint32_t n = first_s;
     const bool rejected = n < count, both = rejected && a.draft != nullptr;
     const uint32_t trow = begin + b + n, drow = begin + n;
-    if (threadIdx.x == 0) {
-        mt_s = load_row(a.rows, min(trow, a.drafts + a.requests - 1), a.split);
-        if (!mt_s.ok) bad_s = 1;
+    if (n >= kKeep && warp == 0) {
+        const RowMass m = load_row(a.rows, lane >= 16 && both ? targets + drow : trow, a.split);
+        if ((lane & 15) == 0) last_s[lane >> 4] = m;
     }
-    if (threadIdx.x == 32 && both) md_s = load_row(a.rows, a.drafts + a.requests + drow, a.split);
-    __syncthreads();
+    if (n >= kKeep) __syncthreads();
+    const RowMass mt = n < kKeep ? mass_s[n][0] : last_s[0], md = n < kKeep ? mass_s[n][1] : last_s[1];
     // one path for the whole cluster from here: all of it depends on the request alone
     uint32_t drawn = kNoToken;
     const bool bad = bad_s != 0;
     if (!bad) {
-        const RowMass mt = mt_s, md = md_s;
+        RowWeight wt, wd;
+        wt.set(mt.top, mt.scale, a.minus_zero);
+        wd.set(md.top, md.scale, a.minus_zero);
         const int32_t *zt = a.target + trow * a.ld_target, *zd = both ? a.draft + drow * a.ld_draft : zt;
         const uint32_t x = rejected ? a.draft_tokens[drow] : kNoToken;
         // a CTA has a run of the vocabulary, a warp a run of that, in steps of 128
         const uint32_t steps = (a.vocab + 127) / 128, parts = S * kDrawWarps, part = rank * kDrawWarps + warp;
         const uint32_t v0 = (uint32_t)((uint64_t)steps * part / parts) * 128,
                        v1 = min(a.vocab, (uint32_t)((uint64_t)steps * (part + 1) / parts) * 128);
-        // what is drawn from, of logits v + lane + 32 u; rest: p less q
-        auto four = [&](uint32_t v, bool rest, uint64_t (&m)[4]) {
+        const uint32_t run = ((v1 - v0 + 127) / 128 + kRuns - 1) / kRuns * 128;  // logits per run
+        // logits v + lane + 32 u of both rows, and what is drawn from there (rest: p less q)
+        struct Four {
             int32_t t[4], q[4];
+        };
+        auto fetch = [&](uint32_t v, bool rest, Four &z) {
+            const int32_t *pt = zt + v + lane, *pq = zd + v + lane;
+            if (v + 128 <= v1) {
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const uint32_t at = v + lane + 32 * u;
-                t[u] = at < v1 ? zt[at] : kExcluded;
-                q[u] = both && rest && at < v1 ? zd[at] : kExcluded;
+                for (int u = 0; u < 4; u++) {
+                    z.t[u] = pt[32 * u];
+                    if (both && rest) z.q[u] = pq[32 * u];
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const bool in = v + lane + 32 * u < v1;
+                    z.t[u] = in ? pt[32 * u] : kExcluded;
+                    z.q[u] = both && rest && in ? pq[32 * u] : kExcluded;
+                }
+            }
+        };
+        const bool usual = wt.fast && both && wd.fast && mt.shift < 32 && md.shift < 32;
+        auto four = [&](uint32_t v, bool rest, const Four &z, uint64_t (&m)[4]) {
+            if (usual && rest) {
+#pragma unroll
+                for (int u = 0; u < 4; u += 2) {
+                    uint32_t t0, t1, q0, q1;
+                    wt.fast2(z.t[u], z.t[u + 1], t0, t1);
+                    wd.fast2(z.q[u], z.q[u + 1], q0, q1);
+                    const int64_t d0 = (int64_t)(row_share_small(t0, mt) - row_share_small(q0, md));
+                    const int64_t d1 = (int64_t)(row_share_small(t1, mt) - row_share_small(q1, md));
+                    m[u] = d0 > 0 ? d0 : 0;
+                    m[u + 1] = d1 > 0 ? d1 : 0;
+                }
+                return;
             }
 #pragma unroll
             for (int u = 0; u < 4; u += 2) {
                 const uint32_t at = v + lane + 32 * u;
                 uint32_t w0, w1;
-                row_weight2(mt, a.minus_zero, t[u], t[u + 1], at, at + 32, w0, w1);
+                row_weight2(wt, mt.first, z.t[u], z.t[u + 1], at, at + 32, w0, w1);
                 m[u] = row_share(w0, mt);
                 m[u + 1] = row_share(w1, mt);
                 if (!rest) continue;
                 uint64_t q0 = at == x ? 1ull << 40 : 0, q1 = at + 32 == x ? 1ull << 40 : 0;
                 if (both) {
-                    row_weight2(md, a.minus_zero, q[u], q[u + 1], at, at + 32, w0, w1);
+                    row_weight2(wd, md.first, z.q[u], z.q[u + 1], at, at + 32, w0, w1);
                     q0 = row_share(w0, md);
                     q1 = row_share(w1, md);
                 }
@@ -583,10 +788,28 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
         unsigned long long total = 0, mine = 0, below = 0;
         for (int round = 0; round < 2; round++, rest = false) {
             mine = 0;
-            for (uint32_t v = v0; v < v1; v += 128) {
-                uint64_t m[4];
-                four(v, rest, m);
-                mine += (m[0] + m[1]) + (m[2] + m[3]);
+            Four next;
+            if (v0 < v1) fetch(v0, rest, next);
+            uint32_t in_run = 0, at_run = 0;
+            for (uint32_t v = v0; v < v1; v += 128) {  // the next step's logits under way while this one's are summed
+                const Four z = next;
+                if (v + 128 < v1) fetch(v + 128, rest, next);
+                // nothing where p is nothing: below the likely tokens that is most of a row
+                const uint32_t d = min(min(wt.base - (uint32_t)z.t[0], wt.base - (uint32_t)z.t[1]),
+                                       min(wt.base - (uint32_t)z.t[2], wt.base - (uint32_t)z.t[3]));
+                if (!wt.fast || __any_sync(~0u, d < wt.most)) {
+                    uint64_t m[4];
+                    four(v, rest, z, m);
+                    mine += (m[0] + m[1]) + (m[2] + m[3]);
+                }
+                in_run += 128;
+                if (v + 128 >= v1 || in_run == run) {
+                    unsigned long long t = mine;
+                    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
+                    if (lane == 0) run_sum[warp][at_run] = t;  // of all runs so far
+                    at_run++;
+                    in_run = 0;
+                }
             }
             for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
             if (lane == 0) warp_sum[warp] = mine;
@@ -615,9 +838,17 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
         }
         const uint64_t point = mul_frac(total, a.sample_u[b]);
         if (total != 0 && point >= below && point - below < mine) {  // one warp of the cluster holds the point
-            for (uint32_t v = v0; v < v1; v += 128) {
+            __syncwarp();
+            // the run that holds it: the first whose running sum passes the point
+            const int runs = (int)((v1 - v0 + run - 1) / run);
+            const unsigned passed = __ballot_sync(~0u, lane < runs && below + run_sum[warp][lane < runs ? lane : 0] > point);
+            const int hit_run = __ffs((int)passed) - 1;
+            if (hit_run > 0) below += run_sum[warp][hit_run - 1];
+            for (uint32_t v = v0 + hit_run * run; v < v1; v += 128) {
+                Four z;
                 uint64_t m[4];
-                four(v, rest, m);
+                fetch(v, rest, z);
+                four(v, rest, z, m);
                 for (int u = 0; u < 4; u++) {
                     unsigned long long sum = m[u];
                     for (int o = 1; o < 32; o <<= 1) {
@@ -644,6 +875,11 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
     }
 }
 
+// CTAs per row that are considered: 9 and 6 fill a group of 18 SMs that cannot hold
+// a cluster together with its neighbours.
+constexpr int kSplits[] = {1, 2, 3, 4, 6, 8, 9, 12, 16};
+// Loaded once (a cluster's shares fit), loaded twice.
+void (*const kMass[2])(Args) = {k_mass<false, 8>, k_mass<true, 4>};
 // Per device: how many clusters of k_mass run at once, by their size.
 struct DeviceSetup {
     bool ready = false;
@@ -682,16 +918,19 @@ cudaError_t device_setup(DeviceSetup &out) {
     if (!d.ready) {
         if ((e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, dev)) != cudaSuccess) return e;
         const int smem = kMaxRing * kChunkBytes;
-        if ((e = cudaFuncSetAttribute(k_mass, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
-        if ((e = cudaFuncSetAttribute(k_mass, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        for (auto fn : kMass) {
+            if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+            if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        }
         if ((e = cudaFuncSetAttribute(k_draw, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         d.clusters[1] = d.sms;
-        for (int c = 2; c <= kMaxCluster; c *= 2) {
+        for (int c : kSplits) {
+            if (c == 1) continue;
             cudaLaunchConfig_t cfg;
             cudaLaunchAttribute attr[2];
             configure(cfg, attr, dim3((unsigned)c), kMassThreads, smem, c, nullptr);
             int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, k_mass, &cfg) != cudaSuccess) {
+            if (cudaOccupancyMaxActiveClusters(&n, kMass[0], &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
                 n = 0;
             }
@@ -766,30 +1005,33 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     DeviceSetup dev;
     cudaError_t e = device_setup(dev);
     if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("device set-up: ") + cudaGetErrorString(e));
-    // CTAs per row: the split with the least work for the busiest CTA, counting a
-    // row's exchange of maxima as a chunk and a half; a row's share has to fit the ring with some
-    // chunks to spare, else it is loaded twice.
+    // CTAs per row: the split with the least time for the busiest cluster, in
+    // microseconds as measured on one SM: a chunk's first pass alone 0.4 and its second 0.5,
+    // both beside one another 0.62; a row's exchange and its ends 2, or 0.6 where they are hidden.
     const int chunks = (int)((vocab + kChunk - 1) / kChunk);
     double best = 0;
-    for (int split = 1; split <= kMaxCluster; split *= 2) {
+    for (int split : kSplits) {
         if (dev.clusters[split] == 0 || (split > 1 && chunks < split)) continue;
         const int share = (chunks + split - 1) / split;
-        const bool fits = share <= kMaxRing;
         const uint32_t rounds = (a.total + dev.clusters[split] - 1) / dev.clusters[split];
-        const double cost = rounds * ((double)chunks / split * (fits ? 1 : 2) + 1.5) + (share + 3 > kMaxRing ? 0.3 * rounds * share : 0);
-        if (a.split == 0 || cost < best) {
-            best = cost;
-            a.split = split;
-            a.resident = fits;
+        for (int resident = 0; resident < 2; resident++) {
+            if (resident && share > kMaxRing) continue;
+            const double per = (double)chunks / split;
+            const double cost = resident ? rounds * (per * 0.9 + 2.0) : rounds * (per * 0.62 + 0.6) + per * 0.4 + 2.0;
+            if (a.split == 0 || cost < best) {
+                best = cost;
+                a.split = split;
+                a.resident = resident;
+                // (even: a slot is one of two groups')
+                a.ring = resident ? std::min(kMaxRing, rounds > 1 ? 2 * share : (share + 1) / 2 * 2) : kMaxRing;
+            }
         }
     }
-    a.ring = std::min(kMaxRing, std::max(2, 2 * ((chunks + a.split - 1) / a.split) + 1));
-    if (!a.resident) a.ring = kMaxRing;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
     const uint32_t groups = std::min<uint32_t>(a.total, (uint32_t)dev.clusters[a.split]);
     configure(cfg, attr, dim3(groups * a.split), kMassThreads, (size_t)a.ring * kChunkBytes, a.split, s);
-    e = cudaLaunchKernelEx(&cfg, k_mass, a);
+    e = cudaLaunchKernelEx(&cfg, kMass[a.resident ? 0 : 1], a);
     if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("k_mass: ") + cudaGetErrorString(e));
     DrawArgs d{a, 1};
     while (d.split < kMaxCluster && requests * d.split * 2 <= (uint32_t)dev.sms * 2 && vocab >= 2048u * d.split) d.split *= 2;

@@ -148,6 +148,23 @@ def test_many_requests(llmx, torch, seed):
 
 
 @gpu
+@pytest.mark.parametrize("requests,k,vocab", [(60, 2, 30001), (200, 1, 9000), (20, 2, 151936), (90, 0, 100003), (500, 0, 5000),
+                                              (3, 0, 400000), (2, 1, 900001)])
+def test_many_long_rows(llmx, torch, requests, k, vocab):
+    """More rows than run at once, rows held by clusters of every size, and rows that pass
+    through shared memory twice; rows of every alignment."""
+    rng = np.random.default_rng(requests + vocab)
+    c = make(rng, [k - (r % 3 == 2 and k > 0) for r in range(requests)], vocab, temperature=rng.random(requests) + 0.4)
+    c["temperature"][::5] = 0.0
+    d = Device(llmx, torch, c)
+    d.call()
+    d.check()
+    for _ in range(5):  # the same again, back to back
+        d.call()
+    d.check()
+
+
+@gpu
 @pytest.mark.parametrize("ld,skip", [(1001, 0), (1004, 0), (1004, 1), (1003, 3), (2048, 2), (0, 1)])
 @pytest.mark.parametrize("vocab", [999, 1000])
 def test_strides(llmx, torch, vocab, ld, skip):
