@@ -24,6 +24,7 @@
 #include <cstdint>
 #include <mutex>
 #include <string>
+#include <type_traits>
 
 #include "llmx.h"
 #include "device_util.cuh"
@@ -268,11 +269,13 @@ static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t
 // ---------------------------------------------------------------------------
 // rows -> maxima and sums
 // ---------------------------------------------------------------------------
-constexpr int kMassWarps = 16, kMassThreads = (kMassWarps + 3) * 32;  // sums, loads (two), the rows' requests
-constexpr int kChunk = 4096;                                          // logits per chunk
+constexpr int kMassWarps = 16;              // that sum
+constexpr int kChunk = 4096;                // logits per chunk
 constexpr int kChunkBytes = kChunk * 4;
-constexpr int kMaxRing = 12, kFirstRing = 8;  // chunks in shared memory; of these a row's first pass has, where it has its own
-constexpr int kTops = 4;                      // rows whose exchange may be under way: see k_mass
+constexpr int kMaxRing = 12, kFirstRing = 4;  // chunks in shared memory; of these the first pass's, where it has its own
+constexpr int kFirstWarps = 4;              // of a first pass of its own
+constexpr int kTops = 2;                    // rows whose maxima may be under way
+static __host__ __device__ constexpr int mass_threads(bool twice) { return (kMassWarps + (twice ? kFirstWarps : 0) + 3) * 32; }
 
 // A row's logits: a head of at most 3 up to a 16-byte boundary, vectors of 4, a
 // tail of at most 3.  CTA `rank` of `split` takes an even share of the
@@ -322,40 +325,41 @@ static __device__ uint32_t owner_of(const Args &a, uint32_t row) {
     return kNoToken;
 }
 
-// A CTA's part in a row, and what a thread knows of it between the passes.
+// A CTA's part in a row, and a thread's logit of its head or tail, if any.
 struct Held {
     Row r;
     int chunks;
-    uint32_t edge_at;  // this thread's logit of the head or tail, if any
+    uint32_t edge_at;
     int32_t edge;
-    __device__ __forceinline__ Held(const Args &a, uint32_t row, int rank, bool there) : r(a, there ? row : 0, rank) {
-        chunks = there ? (int)((r.v1 - r.v0 + kChunk / 4 - 1) / (kChunk / 4)) : 0;
+    __device__ __forceinline__ Held(const Args &a, uint32_t row, int rank, int t) : r(a, row, rank) {
+        chunks = (int)((r.v1 - r.v0 + kChunk / 4 - 1) / (kChunk / 4));
         edge_at = kNoToken;
         edge = kExcluded;
         const uint32_t tail = r.head + r.vectors * 4;
-        if (threadIdx.x < 3 && rank == 0 && threadIdx.x < r.head) edge_at = threadIdx.x;
-        if (threadIdx.x >= 4 && threadIdx.x < 7 && rank == a.split - 1 && tail + threadIdx.x - 4 < a.vocab)
-            edge_at = tail + threadIdx.x - 4;
+        if (t < 3 && rank == 0 && t < (int)r.head) edge_at = t;
+        if (t >= 4 && t < 7 && rank == a.split - 1 && tail + t - 4 < a.vocab) edge_at = tail + t - 4;
         if (edge_at != kNoToken) edge = r.z[edge_at];
     }
 };
 
+// Warps of a CTA: the first kMassWarps sum; kTwice: kFirstWarps more take the
+// maxima, through a ring of their own (slots [0, kFirstRing)), else the summing
+// warps do, and a row stays in the one ring until it is summed; then two that load
+// and one that finds the rows' temperatures.
 // No barrier over the CTA: the last warp to add its maximum (or sum) passes
-// the CTA's on.  A CTA's own buffers alternate between rows; the maxima of the cluster
-// arrive in one of four places: a CTA sends row i + 4's after its second pass of i + 2,
-// so after every CTA has sent i + 2's, and a warp adds to those after it has read i's.
-//
-// A chunk is one group's of GW warps.  kTwice: rows are loaded twice, each pass
-// through a ring of its own (slots [0, kFirstRing) and the rest), and the first pass
-// of the next row goes beside the second of this one; else through one ring,
-// in which a row stays until it is summed.
+// the CTA's on.  The maxima of the cluster arrive in one of kTops places; a CTA
+// sends row i + kTops's once every CTA of the cluster has summed row i (top_done),
+// which also keeps the words that its warps share apart: they alternate between rows.
+// A chunk is one group's of GW summing warps.
 template <bool kTwice, int GW>
-__global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
-    constexpr int kGroups = kMassWarps / GW, kVectors = kChunk / 4 / (GW * 32);  // 16-byte vectors per thread and chunk
+__global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) {
+    constexpr int kGroups = kMassWarps / GW;
+    constexpr int kMaxWarps = kTwice ? kFirstWarps : kMassWarps;  // that take maxima
+    constexpr int kLoad = kMassWarps + (kTwice ? kFirstWarps : 0);
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t full[kMaxRing], empty[kMaxRing];
-    __shared__ uint64_t info_full[2], info_empty[2];  // a row's temperature
-    __shared__ uint64_t top_full[kTops];              // every CTA's maximum of the row
+    __shared__ uint64_t info_full[2], info_empty[2];      // a row's temperature
+    __shared__ uint64_t top_full[kTops], top_done[kTops]; // of every CTA: its maximum of the row is there, its sum done
     __shared__ float scale_s[2];
     __shared__ int32_t tops[kTops][kMaxCluster];
     __shared__ int32_t warp_top[2][kMassWarps];
@@ -367,14 +371,17 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
     if (threadIdx.x == 0) {
         for (int i = 0; i < a.ring; i++) {
             mbar_init(full + i, 1);
-            mbar_init(empty + i, GW);
+            mbar_init(empty + i, kTwice && i < kFirstRing ? kFirstWarps : GW);
         }
         for (int i = 0; i < 2; i++) {
             mbar_init(info_full + i, 1);
             mbar_init(info_empty + i, kMassWarps);
             top_count[i] = part_count[i] = 0;
         }
-        for (int i = 0; i < kTops; i++) mbar_init(top_full + i, S);
+        for (int i = 0; i < kTops; i++) {
+            mbar_init(top_full + i, S);
+            mbar_init(top_done + i, S);
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (S > 1) cluster_sync();
@@ -382,10 +389,10 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
     pdl_wait();
     pdl_trigger();
 
-    if (warp == kMassWarps || warp == kMassWarps + 1) {  // ---- loads, of the first pass and of the second -----
-        if (lane == 0 && (kTwice || warp == kMassWarps)) {
-            const int base = warp == kMassWarps ? 0 : kFirstRing;
-            const int ring = !kTwice ? a.ring : warp == kMassWarps ? kFirstRing : a.ring - kFirstRing;
+    if (warp >= kLoad && warp < kLoad + 2) {  // ---- loads, of the first pass and of the second -----
+        if (lane == 0 && (kTwice || warp == kLoad)) {
+            const int base = warp == kLoad ? 0 : kFirstRing;
+            const int ring = !kTwice ? a.ring : warp == kLoad ? kFirstRing : a.ring - kFirstRing;
             int s = 0, phase = 1, issued = 0;
             bool ok = true;
             for (uint32_t row = group; ok && row < a.total; row += groups) {
@@ -413,7 +420,7 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
         }
         return;
     }
-    if (warp == kMassWarps + 2) {  // ---- the rows' temperatures --------------------------
+    if (warp == kLoad + 2) {  // ---- the rows' temperatures --------------------------
         uint32_t i = 0;
         for (uint32_t row = group; row < a.total; row += groups, i++) {
             const uint32_t b = owner_of(a, row);
@@ -429,7 +436,6 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
     }
 
     // ---- maxima and sums ---------------------------------------------------------------
-    const int mine = warp / GW, gt = (warp % GW) * 32 + lane;
     bool ok = true;
     // A place in a ring of n slots from slot `base` on, moved by chunks.  Slot s is always
     // group s mod kGroups's (n is a multiple of kGroups): a warp then meets every phase of the
@@ -451,191 +457,176 @@ __global__ void __launch_bounds__(kMassThreads, 1) k_mass(const Args a) {
             return by;
         }
     };
-    static_assert(kFirstRing % kGroups == 0 && kMaxRing % kGroups == 0, "a slot is one group's");
-    // whether this warp, whose lane 0 has just written its word, is the last of the CTA to
+    static_assert((kMaxRing - kFirstRing) % kGroups == 0 && kMaxRing % kGroups == 0, "a slot is one group's");
+    // whether this warp, whose lane 0 has just written its word, is the last of n to
     // come here; it then sees the others' words
-    auto last_of = [&](int *count) {
+    auto last_of = [&](int *count, int n) {
         int old = 0;
         if (lane == 0) {
             asm volatile("atom.acq_rel.cta.shared::cta.add.s32 %0, [%1], 1;" : "=r"(old) : "r"(smem_u32(count)) : "memory");
-            if (old == kMassWarps - 1) *count = 0;
+            if (old == n - 1) *count = 0;
         }
-        return __shfl_sync(~0u, old, 0) == kMassWarps - 1;
+        return __shfl_sync(~0u, old, 0) == n - 1;
     };
-    // this thread's vectors of a chunk: the first, and how far the chunk goes from there
-    auto vectors_of = [&](const Row &r, int at, int c, const int4 *&p) {
-        p = reinterpret_cast<const int4 *>(smem + at * kChunkBytes) + gt;
-        return (int)min(r.v1 - r.v0 - c * (kChunk / 4), (uint32_t)kChunk / 4) - gt;
-    };
-    constexpr int kStride = GW * 32;
-    int32_t top = kExcluded;  // of the row in its first pass
-    auto first_chunk = [&](const Row &r, int at, int c) {
-        const int4 *p;
-        const int n = vectors_of(r, at, c, p);
-        int4 q[kVectors];
-#pragma unroll
-        for (int u = 0; u < kVectors; u++)
-            q[u] = u * kStride < n ? p[u * kStride] : make_int4(kExcluded, kExcluded, kExcluded, kExcluded);
-#pragma unroll
-        for (int u = 0; u < kVectors; u++) top = max(max(top, q[u].x), max(max(q[u].y, q[u].z), q[u].w));
-    };
-    // row number i's maximum, sent to every CTA of the cluster
-    auto send_top = [&](uint32_t i, int32_t edge) {
-        top = __reduce_max_sync(~0u, max(top, edge));
-        if (lane == 0) warp_top[i & 1][warp] = top;
-        if (last_of(&top_count[i & 1])) {
-            top = __reduce_max_sync(~0u, lane < kMassWarps ? warp_top[i & 1][lane] : kExcluded);
-            if (lane < S) {
-                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote(&tops[i % kTops][rank], lane)), "r"(top) : "memory");
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(top_full + i % kTops, lane))
-                             : "memory");
-            }
-        }
-        top = kExcluded;
-        __syncwarp();
-    };
-    RowWeight rw;  // of the row in its second pass
-    unsigned long long sum = 0;
-    uint32_t first = kNoToken;
-    auto begin_second = [&](const Held &h, uint32_t i) {
-        ok = ok && mbar_wait(info_full + (i & 1), (i >> 1) & 1);
-        const float scale = scale_s[i & 1];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(info_empty + (i & 1));
-        ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1);
-        rw.set(__reduce_max_sync(~0u, lane < S ? tops[i % kTops][lane] : kExcluded), scale, a.minus_zero);
-        sum = 0;
-        first = kNoToken;
-        if (h.edge_at != kNoToken) {
-            uint32_t w, none;
-            rw.slow2(h.edge, h.edge, w, none);
-            sum = w;
-            if (h.edge == rw.top) first = h.edge_at;
-        }
-    };
-    auto second_chunk = [&](const Row &r, int at, int c) {
-        const int4 *p;
-        const int n = vectors_of(r, at, c, p);
-        if (rw.fast) {
-            auto add = [&](const int4 &q) {
-                uint32_t w0, w1, w2, w3;
-                rw.fast2(q.x, q.y, w0, w1);
-                rw.fast2(q.z, q.w, w2, w3);
-                sum += (unsigned long long)w0 + w1;
-                sum += (unsigned long long)w2 + w3;
-            };
-            if ((kVectors - 1) * kStride < n) {
-#pragma unroll
-                for (int u = 0; u < kVectors; u++) add(p[u * kStride]);
-            } else {
-#pragma unroll 1
-                for (int u = 0; u * kStride < n; u++) add(p[u * kStride]);
-            }
-            return;
-        }
-#pragma unroll 1
-        for (int u = 0; u * kStride < n; u++) {
-            const int4 q = p[u * kStride];
-            if (rw.greedy) {
-                const uint32_t e = r.head + (r.v0 + c * (kChunk / 4) + gt + u * kStride) * 4;
-                if (q.w == rw.top) first = min(first, e + 3);
-                if (q.z == rw.top) first = min(first, e + 2);
-                if (q.y == rw.top) first = min(first, e + 1);
-                if (q.x == rw.top) first = min(first, e);
-            } else {
-                uint32_t w0, w1, w2, w3;
-                rw.slow2(q.x, q.y, w0, w1);
-                rw.slow2(q.z, q.w, w2, w3);
-                sum += (unsigned long long)w0 + w1;
-                sum += (unsigned long long)w2 + w3;
-            }
-        }
-    };
-    auto end_second = [&](uint32_t row, uint32_t i) {
-        // sums (greedy: the smallest first position) of the warp, then of the CTA
-        auto whole = [&](unsigned long long v) {
-            if (rw.greedy) return (unsigned long long)__reduce_min_sync(~0u, (uint32_t)v);
-            for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-            return v;
-        };
-        sum = whole(rw.greedy ? first : sum);
-        if (lane == 0) warp_part[i & 1][warp] = sum;
-        if (last_of(&part_count[i & 1])) {
-            const unsigned long long part =
-                whole(lane < kMassWarps ? warp_part[i & 1][lane] : rw.greedy ? (unsigned long long)kNoToken : 0);
-            if (lane == 0) {
-                RowPart *out = a.rows + row;
-                out->part[rank] = part;
-                if (rank == 0) {
-                    out->top = rw.top;
-                    out->scale = rw.scale;
-                }
-            }
-        }
-        __syncwarp();
+    auto arrive_all = [&](uint64_t *bar) {  // on this barrier of every CTA of the cluster
+        if (lane < S)
+            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(bar, lane)) : "memory");
     };
     auto release = [&](int at) {
         __syncwarp();
         if (lane == 0) mbar_arrive(empty + at);
     };
-    uint32_t i = 0;
-    if (!kTwice) {
-        Place place{0, 0, 0, a.ring};
+    int32_t top = kExcluded;  // of the row in its first pass
+    // thread t of `stride` takes its vectors of a chunk
+    auto first_chunk = [&](const Row &r, int at, int c, int t, auto stride) {
+        constexpr int kStride = decltype(stride)::value, kVectors = kChunk / 4 / kStride;
+        const int4 *p = reinterpret_cast<const int4 *>(smem + at * kChunkBytes) + t;
+        const int n = (int)min(r.v1 - r.v0 - c * (kChunk / 4), (uint32_t)kChunk / 4) - t;
+        auto most = [&](const int4 &q) { top = max(max(top, q.x), max(max(q.y, q.z), q.w)); };
+        if ((kVectors - 1) * kStride < n) {
+#pragma unroll
+            for (int u = 0; u < kVectors; u++) most(p[u * kStride]);
+        } else {
+            for (int u = 0; u * kStride < n; u++) most(p[u * kStride]);
+        }
+    };
+    // row number i's maximum, sent to every CTA of the cluster
+    auto send_top = [&](uint32_t i, int32_t edge, int w) {
+        top = __reduce_max_sync(~0u, max(top, edge));
+        // every warp waits, not the last alone: else one could go on two rows and be counted
+        // in a row that others have not reached
+        if (i >= kTops) ok = ok && mbar_wait_cluster(top_done + i % kTops, (i / kTops - 1) & 1);
+        if (lane == 0) warp_top[i & 1][w] = top;
+        if (last_of(&top_count[i & 1], kMaxWarps)) {
+            top = __reduce_max_sync(~0u, lane < kMaxWarps ? warp_top[i & 1][lane] : kExcluded);
+            if (lane < S)
+                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote(&tops[i % kTops][rank], lane)), "r"(top) : "memory");
+            arrive_all(top_full + i % kTops);
+        }
+        top = kExcluded;
+        __syncwarp();
+    };
+    if (kTwice && warp >= kMassWarps) {  // ---- first passes of their own ---------------------
+        const int w = warp - kMassWarps, t = w * 32 + lane;
+        Place p{0, 0, 0, kFirstRing};
+        uint32_t i = 0;
         for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
-            const Held h(a, row, rank, true);
-            Place p = place, q = place;
-            for (int c = p.own(mine); c < h.chunks; c += kGroups, p.move(kGroups)) {
+            const Held h(a, row, rank, t);
+            for (int c = 0; c < h.chunks; c++, p.move(1)) {
                 ok = ok && mbar_wait(full + p.slot(), p.phase);
-                first_chunk(h.r, p.slot(), c);
+                first_chunk(h.r, p.slot(), c, t, std::integral_constant<int, kFirstWarps * 32>());
+                release(p.slot());
             }
-            send_top(i, h.edge);
+            send_top(i, h.edge, w);
+        }
+    } else {
+        const int mine = warp / GW, gt = (warp % GW) * 32 + lane;
+        const uint32_t count = group < a.total ? (a.total - group + groups - 1) / groups : 0;  // rows
+        constexpr int kStride = GW * 32, kVectors = kChunk / 4 / kStride;
+        RowWeight rw;
+        unsigned long long sum = 0;
+        uint32_t first = kNoToken;
+        auto begin_second = [&](const Held &h, uint32_t i) {
+            ok = ok && mbar_wait(info_full + (i & 1), (i >> 1) & 1);
+            const float scale = scale_s[i & 1];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(info_empty + (i & 1));
+            ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1);
+            const int32_t t = __reduce_max_sync(~0u, lane < S ? tops[i % kTops][lane] : kExcluded);
+            rw.set(t, scale, a.minus_zero);
+            sum = 0;
+            first = kNoToken;
+            if (h.edge_at != kNoToken) {
+                uint32_t w, none;
+                rw.slow2(h.edge, h.edge, w, none);
+                sum = w;
+                if (h.edge == rw.top) first = h.edge_at;
+            }
+        };
+        auto second_chunk = [&](const Row &r, int at, int c) {
+            const int4 *p = reinterpret_cast<const int4 *>(smem + at * kChunkBytes) + gt;
+            const int n = (int)min(r.v1 - r.v0 - c * (kChunk / 4), (uint32_t)kChunk / 4) - gt;
+            if (rw.fast) {
+                auto add = [&](const int4 &q) {
+                    uint32_t w0, w1, w2, w3;
+                    rw.fast2(q.x, q.y, w0, w1);
+                    rw.fast2(q.z, q.w, w2, w3);
+                    sum += (unsigned long long)w0 + w1;
+                    sum += (unsigned long long)w2 + w3;
+                };
+                if ((kVectors - 1) * kStride < n) {
+#pragma unroll
+                    for (int u = 0; u < kVectors; u++) add(p[u * kStride]);
+                } else {
+#pragma unroll 1
+                    for (int u = 0; u * kStride < n; u++) add(p[u * kStride]);
+                }
+                return;
+            }
+#pragma unroll 1
+            for (int u = 0; u * kStride < n; u++) {
+                const int4 q = p[u * kStride];
+                if (rw.greedy) {
+                    const uint32_t e = r.head + (r.v0 + c * (kChunk / 4) + gt + u * kStride) * 4;
+                    if (q.w == rw.top) first = min(first, e + 3);
+                    if (q.z == rw.top) first = min(first, e + 2);
+                    if (q.y == rw.top) first = min(first, e + 1);
+                    if (q.x == rw.top) first = min(first, e);
+                } else {
+                    uint32_t w0, w1, w2, w3;
+                    rw.slow2(q.x, q.y, w0, w1);
+                    rw.slow2(q.z, q.w, w2, w3);
+                    sum += (unsigned long long)w0 + w1;
+                    sum += (unsigned long long)w2 + w3;
+                }
+            }
+        };
+        auto end_second = [&](uint32_t row, uint32_t i) {
+            // sums (greedy: the smallest first position) of the warp, then of the CTA
+            auto whole = [&](unsigned long long v) {
+                if (rw.greedy) return (unsigned long long)__reduce_min_sync(~0u, (uint32_t)v);
+                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
+                return v;
+            };
+            sum = whole(rw.greedy ? first : sum);
+            if (lane == 0) warp_part[i & 1][warp] = sum;
+            if (last_of(&part_count[i & 1], kMassWarps)) {
+                const unsigned long long part =
+                    whole(lane < kMassWarps ? warp_part[i & 1][lane] : rw.greedy ? (unsigned long long)kNoToken : 0);
+                if (lane == 0) {
+                    RowPart *out = a.rows + row;
+                    out->part[rank] = part;
+                    if (rank == 0) {
+                        out->top = rw.top;
+                        out->scale = rw.scale;
+                    }
+                }
+                // (nobody waits for the last rows', and their CTAs may be gone)
+                if (i + kTops < count) arrive_all(top_done + i % kTops);
+            }
+            __syncwarp();
+        };
+        Place place{0, 0, kTwice ? kFirstRing : 0, kTwice ? a.ring - kFirstRing : a.ring};
+        uint32_t i = 0;
+        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
+            const Held h(a, row, rank, (int)threadIdx.x);
+            if (!kTwice) {
+                Place p = place;
+                for (int c = p.own(mine); c < h.chunks; c += kGroups, p.move(kGroups)) {
+                    ok = ok && mbar_wait(full + p.slot(), p.phase);
+                    first_chunk(h.r, p.slot(), c, gt, std::integral_constant<int, kStride>());
+                }
+                send_top(i, h.edge, warp);
+            }
             begin_second(h, i);
+            Place q = place;
             for (int c = q.own(mine); c < h.chunks; c += kGroups, q.move(kGroups)) {
+                if (kTwice) ok = ok && mbar_wait(full + q.slot(), q.phase);
                 second_chunk(h.r, q.slot(), c);
                 release(q.slot());
             }
             end_second(row, i);
             place.move(h.chunks);
-        }
-    } else {
-        Place first_place{0, 0, 0, kFirstRing}, second_place{0, 0, kFirstRing, a.ring - kFirstRing};
-        auto take_first = [&](const Row &r, Place &p, int c) {
-            ok = ok && mbar_wait(full + p.slot(), p.phase);
-            first_chunk(r, p.slot(), c);
-            release(p.slot());
-            p.move(kGroups);
-        };
-        Held now(a, group, rank, true);
-        Place p = first_place;
-        for (int c = p.own(mine); c < now.chunks; c += kGroups) take_first(now.r, p, c);
-        first_place.move(now.chunks);
-        send_top(0, now.edge);
-        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
-            const bool there = row + groups < a.total;
-            const Held next(a, row + groups, rank, there);
-            Place q = second_place;
-            p = first_place;
-            int c1 = p.own(mine);
-            if (c1 < next.chunks) {  // a chunk ahead, behind which the exchange of this row's maxima passes
-                take_first(next.r, p, c1);
-                c1 += kGroups;
-            }
-            begin_second(now, i);
-            for (int c = q.own(mine); c < now.chunks; c += kGroups, q.move(kGroups)) {
-                if (c1 < next.chunks) {
-                    take_first(next.r, p, c1);
-                    c1 += kGroups;
-                }
-                ok = ok && mbar_wait(full + q.slot(), q.phase);
-                second_chunk(now.r, q.slot(), c);
-                release(q.slot());
-            }
-            for (; c1 < next.chunks; c1 += kGroups) take_first(next.r, p, c1);
-            first_place.move(next.chunks);
-            second_place.move(now.chunks);
-            if (there) send_top(i + 1, next.edge);
-            end_second(row, i);
-            now = next;
         }
     }
     // a wait ran out: rows of this cluster may lack sums, and none of them is to be used
@@ -750,9 +741,19 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
                 }
             }
         };
-        const bool usual = wt.fast && both && wd.fast && mt.shift < 32 && md.shift < 32;
+        const bool usual = wt.fast && mt.shift < 32, usual_both = usual && both && wd.fast && md.shift < 32;
         auto four = [&](uint32_t v, bool rest, const Four &z, uint64_t (&m)[4]) {
-            if (usual && rest) {
+            if (usual && !rest) {
+#pragma unroll
+                for (int u = 0; u < 4; u += 2) {
+                    uint32_t w0, w1;
+                    wt.fast2(z.t[u], z.t[u + 1], w0, w1);
+                    m[u] = row_share_small(w0, mt);
+                    m[u + 1] = row_share_small(w1, mt);
+                }
+                return;
+            }
+            if (usual_both && rest) {
 #pragma unroll
                 for (int u = 0; u < 4; u += 2) {
                     uint32_t t0, t1, q0, q1;
@@ -928,9 +929,9 @@ cudaError_t device_setup(DeviceSetup &out) {
             if (c == 1) continue;
             cudaLaunchConfig_t cfg;
             cudaLaunchAttribute attr[2];
-            configure(cfg, attr, dim3((unsigned)c), kMassThreads, smem, c, nullptr);
+            configure(cfg, attr, dim3((unsigned)c), mass_threads(true), smem, c, nullptr);
             int n = 0;
-            if (cudaOccupancyMaxActiveClusters(&n, kMass[0], &cfg) != cudaSuccess) {
+            if (cudaOccupancyMaxActiveClusters(&n, kMass[1], &cfg) != cudaSuccess) {
                 (void)cudaGetLastError();
                 n = 0;
             }
@@ -1030,7 +1031,7 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[2];
     const uint32_t groups = std::min<uint32_t>(a.total, (uint32_t)dev.clusters[a.split]);
-    configure(cfg, attr, dim3(groups * a.split), kMassThreads, (size_t)a.ring * kChunkBytes, a.split, s);
+    configure(cfg, attr, dim3(groups * a.split), mass_threads(!a.resident), (size_t)a.ring * kChunkBytes, a.split, s);
     e = cudaLaunchKernelEx(&cfg, kMass[a.resident ? 0 : 1], a);
     if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("k_mass: ") + cudaGetErrorString(e));
     DrawArgs d{a, 1};
