@@ -537,10 +537,10 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     const int64_t line = line_at(c.shared_tiles, pre, c.RT);  // stages that are shared out one by one
-    const int me = min((int)blockIdx.x, c.sharers);
+    // no more sharers than stages: every CTA between a tile's first and last takes a part in it
+    const int sharers = (int)min((int64_t)c.sharers, max(line, (int64_t)1)), me = min((int)blockIdx.x, sharers);
     Walk k;
-    k.start(c, pre, line ? range_begin(me, line, c.sharers) : 0,
-            line && me < c.sharers ? range_begin(me + 1, line, c.sharers) : line ? range_begin(me, line, c.sharers) : 0);
+    k.start(c, pre, range_begin(me, line, sharers), range_begin(min(me + 1, sharers), line, sharers));
 
     if (warp == 1) {  // ---- loads ---------------------------------------------------
         // Lane 0 loads the weight's stages: few instructions per stage, since one
@@ -717,8 +717,8 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
             int b_lo = 0, b_hi = 0;
             if (!whole) {
                 const int64_t at = line_at(k.tile, pre, c.RT);
-                b_lo = cta_of(at, line, c.sharers);
-                b_hi = cta_of(at + k.len - 1, line, c.sharers);
+                b_lo = cta_of(at, line, sharers);
+                b_hi = cta_of(at + k.len - 1, line, sharers);
             }
             unsigned long long *acc = reinterpret_cast<unsigned long long *>(c.acc) + (size_t)b_lo * NT * kOutTile + m;
             const bool okw = mbar_wait_err(tfull + b, use & 1, c.error);

@@ -387,7 +387,8 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
     if (S > 1) cluster_sync();
     else __syncthreads();
     pdl_wait();
-    pdl_trigger();
+    // with many rows the draw's CTAs would only take room from the last of this kernel's
+    if (!kTwice) pdl_trigger();
 
     if (warp >= kLoad && warp < kLoad + 2) {  // ---- loads, of the first pass and of the second -----
         if (lane == 0 && (kTwice || warp == kLoad)) {

@@ -133,6 +133,21 @@ def test_many_adapters(llmx, torch):
 
 
 @gpu
+@pytest.mark.parametrize("rows", [5, 40, 200, 300])
+@pytest.mark.parametrize("more", [0, 1, 3, 60, 147])
+def test_tiles_beyond_the_processors(llmx, torch, rows, more):
+    """More tiles than processors, with a few, many and no tiles left over to share; an
+    accumulator that a call leaves behind would show in the next."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    n = (sms + more) * 128 - 5
+    for k in (64, 640):
+        c = Case(llmx, torch, k, n, [9, 20, 33], rows, seed=more)
+        for _ in range(2):
+            x = whole(c.rng, (rows, k), 700)
+            c.check(x, c.rng.integers(-1, 3, rows), wide=True)
+
+
+@gpu
 @pytest.mark.parametrize("k", [128, 32768])
 @pytest.mark.parametrize("rows", [3, 40, 130])
 def test_extremes(llmx, torch, k, rows):
