@@ -50,6 +50,7 @@
 #include <cstdint>
 #include <new>
 #include <string>
+#include <type_traits>
 
 #include "llmx.h"
 #include "device_util.cuh"
@@ -811,26 +812,49 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
 // layouts
 // ---------------------------------------------------------------------------
 // Pieces of a dense [rows][ld] matrix: tile t, piece p (columns 16 p .. 16 p + 15) at
-// dst + (t * pieces + p) * kPiece as [plane][row][16 bytes], zeros past the matrix.
-__global__ void k_pack_pieces(const int16_t *__restrict__ src, uint32_t rows, uint32_t cols, uint32_t ld, uint32_t pieces,
-                              uint32_t stride_pieces, uint32_t tiles, uint8_t *__restrict__ dst) {
+// dst + (t * stride_pieces + p) * kPiece as [plane][row][16 bytes], zeros past the matrix.
+// kWide: rows of 16-byte aligned vectors of 8 (the weight); else one by one (up matrices).
+template <bool kWide>
+__global__ void __launch_bounds__(256) k_pack_pieces(const int16_t *__restrict__ src, uint32_t rows, uint32_t cols, uint32_t pieces,
+                                                     uint32_t stride_pieces, uint32_t tiles, uint8_t *__restrict__ dst) {
     const uint64_t total = (uint64_t)tiles * pieces * kOutTile;
     for (uint64_t g = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; g < total; g += (uint64_t)gridDim.x * blockDim.x) {
-        const uint32_t m = (uint32_t)(g % kOutTile);
-        const uint64_t rest = g / kOutTile;
-        const uint32_t p = (uint32_t)(rest % pieces), t = (uint32_t)(rest / pieces), row = t * kOutTile + m;
-        uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
-        if (row < rows)
+        // 8 rows x 4 pieces per warp: whole sectors are read, core matrices written
+        const uint32_t in = (uint32_t)(g % (kOutTile * 4)), m = (in >> 5) * 8 + (in & 7), quad = (in >> 3) & 3;
+        const uint64_t rest = g / (kOutTile * 4);
+        const uint32_t quads = pieces / 4;
+        uint32_t p, t;
+        if (kWide) {
+            t = (uint32_t)(rest / quads);
+            p = (uint32_t)(rest % quads) * 4 + quad;
+        } else {
+            const uint64_t lin = g / kOutTile;
+            t = (uint32_t)(lin / pieces);
+            p = (uint32_t)(lin % pieces);
+        }
+        const uint32_t mm = kWide ? m : (uint32_t)(g % kOutTile), row = t * kOutTile + mm;
+        uint4 v[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+        if (row < rows) {
+            if (kWide) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const uint32_t col = p * 16 + e;
-                const uint32_t v = col < cols ? (uint16_t)src[(size_t)row * ld + col] : 0u;
-                hi[e >> 2] |= (v >> 8) << (8 * (e & 3));
-                lo[e >> 2] |= (v & 255u) << (8 * (e & 3));
+                for (int h = 0; h < 2; h++)
+                    if (p * 16 + h * 8 < cols)
+                        v[h] = *reinterpret_cast<const uint4 *>(src + (size_t)row * cols + p * 16 + h * 8);
+            } else {
+                uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (p * 16 + e < cols) w[e >> 1] |= (uint32_t)(uint16_t)src[(size_t)row * cols + p * 16 + e] << (16 * (e & 1));
+                v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+                v[1] = make_uint4(w[4], w[5], w[6], w[7]);
             }
-        uint8_t *d = dst + ((size_t)t * stride_pieces + p) * kPiece + m * 16;
-        *reinterpret_cast<uint4 *>(d) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        *reinterpret_cast<uint4 *>(d + kPiece / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        }
+        uint8_t *d = dst + ((size_t)t * stride_pieces + p) * kPiece + mm * 16;
+        *reinterpret_cast<uint4 *>(d) = make_uint4(__byte_perm(v[0].x, v[0].y, 0x7531), __byte_perm(v[0].z, v[0].w, 0x7531),
+                                                   __byte_perm(v[1].x, v[1].y, 0x7531), __byte_perm(v[1].z, v[1].w, 0x7531));
+        *reinterpret_cast<uint4 *>(d + kPiece / 2) =
+            make_uint4(__byte_perm(v[0].x, v[0].y, 0x6420), __byte_perm(v[0].z, v[0].w, 0x6420),
+                       __byte_perm(v[1].x, v[1].y, 0x6420), __byte_perm(v[1].z, v[1].w, 0x6420));
     }
 }
 // Sum of every output's weights (|sum| <= 2^15 * 32768: 32 bits hold it), 0 past the last output.
@@ -839,8 +863,13 @@ __global__ void __launch_bounds__(256) k_weight_sums(const int16_t *__restrict__
     const uint32_t row = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
     if (row >= padded) return;
     int32_t s = 0;
-    if (row < rows)
-        for (uint32_t k = lane; k < cols; k += 32) s += src[(size_t)row * cols + k];
+    if (row < rows) {
+        const uint4 *p = reinterpret_cast<const uint4 *>(src + (size_t)row * cols);
+        for (uint32_t k = lane; k < cols / 8; k += 32) {
+            const uint4 v = p[k];
+            s += lo16(v.x) + hi16(v.x) + lo16(v.y) + hi16(v.y) + lo16(v.z) + hi16(v.z) + lo16(v.w) + hi16(v.w);
+        }
+    }
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane == 0) sums[row] = s;
 }
@@ -874,6 +903,7 @@ struct llmx_adapters {
     int dev = 0, sms = 0;
     uint32_t in_dim = 0, out_dim = 0, slots = 0, max_rank = 0, max_rows = 0;
     int P = 0, T = 0, Q = 0, row_cap = 0;  // row_cap: most rows per row tile of any call
+    uint8_t *memory = nullptr;   // the one allocation
     uint8_t *weight = nullptr;   // pieces [T][P]
     int32_t *wsum = nullptr;     // [T * 128]
     uint32_t *down = nullptr;    // [slots][16 Q][in_dim / 2]
@@ -916,10 +946,7 @@ struct DeviceScope {
 };
 
 void release(llmx_adapters *h) {
-    for (void *p : {(void *)h->weight, (void *)h->wsum, (void *)h->down, (void *)h->up, (void *)h->rank, (void *)h->scale,
-                    (void *)h->xp, (void *)h->tp, (void *)h->zero, (void *)h->list, (void *)h->count, (void *)h->acc, (void *)h->arrived,
-                    (void *)h->error})
-        cudaFree(p);
+    cudaFree(h->memory);
     delete h;
 }
 
@@ -975,41 +1002,52 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
     h->Q = (int)((h->max_rank + 15) / 16);
     h->row_cap = max_rows > kRowTile ? kRowTile : rows_per_tile(max_rows, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    auto get = [&](auto **p, size_t n) {
-        n = std::max<size_t>(n, 16);
-        h->bytes += n;
-        return cudaMalloc(reinterpret_cast<void **>(p), n);
-    };
     const size_t rt = (size_t)row_tiles(max_rows) + (max_rows > kRowTile ? kMoreTiles : 0);
     const size_t xt = rt == 1 ? (size_t)h->row_cap : max_rows + 16 * rt;  // rows of all row tiles
-    const size_t up_bytes = (size_t)slots * h->T * h->Q * kPiece;
     const size_t pieces = h->max_pieces(h->row_cap);
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
         (e = cudaFuncSetAttribute(k_project<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(k_project<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
-        (e = get(&h->weight, (size_t)h->T * h->P * kPiece)) != cudaSuccess ||
-        (e = get(&h->wsum, (size_t)h->T * kOutTile * 4)) != cudaSuccess ||
-        (e = get(&h->down, (size_t)slots * h->Q * 16 * in_dim * 2)) != cudaSuccess ||
-        (e = get(&h->up, up_bytes)) != cudaSuccess || (e = get(&h->rank, (size_t)slots * 4)) != cudaSuccess ||
-        (e = get(&h->scale, (size_t)slots * 4)) != cudaSuccess ||
-        (e = get(&h->xp, xt * h->P * 32)) != cudaSuccess ||
-        (e = get(&h->tp, xt * h->Q * h->row_cap * 32)) != cudaSuccess ||
-        (e = get(&h->zero, (size_t)h->row_cap * 32)) != cudaSuccess ||
-        (e = cudaMemsetAsync(h->zero, 0, (size_t)h->row_cap * 32, s)) != cudaSuccess ||
-        (e = get(&h->list, rt * pieces * 8)) != cudaSuccess ||
-        (e = get(&h->count, rt * 4)) != cudaSuccess || (e = get(&h->acc, h->acc_bytes())) != cudaSuccess ||
-        (e = get(&h->arrived, (size_t)h->sms * 4)) != cudaSuccess || (e = get(&h->error, 4)) != cudaSuccess ||
-        (e = cudaMemsetAsync(h->rank, 0, (size_t)slots * 4, s)) != cudaSuccess ||
-        // the last ranks of a slot that no adapter fills are multiplied by nothing, but read
-        (e = cudaMemsetAsync(h->down, 0, (size_t)slots * h->Q * 16 * in_dim * 2, s)) != cudaSuccess ||
-        (e = cudaMemsetAsync(h->acc, 0, h->acc_bytes(), s)) != cudaSuccess ||
-        (e = cudaMemsetAsync(h->arrived, 0, (size_t)h->sms * 4, s)) != cudaSuccess ||
-        (e = cudaMemsetAsync(h->error, 0, 4, s)) != cudaSuccess) {
+        (e = cudaFuncSetAttribute(k_project<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess) {
         release(h);
         return cuda_fail("create", e);
     }
-    k_pack_pieces<<<h->sms * 8, 256, 0, s>>>(weight, out_dim, in_dim, in_dim, h->P, h->P, h->T, h->weight);
+    // one allocation; what has to start as zeros lies at its front
+    size_t at = 0;
+    auto place = [&](size_t n) {
+        const size_t was = at;
+        at += (n + 255) / 256 * 256;
+        return was;
+    };
+    const size_t rank_at = place((size_t)slots * 4), zero_at = place((size_t)h->row_cap * 32), acc_at = place(h->acc_bytes()),
+                 arrived_at = place((size_t)h->sms * 4), error_at = place(4),
+                 // ranks of a slot that no adapter fills are multiplied by nothing, but read
+                 down_at = place((size_t)slots * h->Q * 16 * in_dim * 2), zeros = at, scale_at = place((size_t)slots * 4),
+                 wsum_at = place((size_t)h->T * kOutTile * 4), xp_at = place(xt * h->P * 32),
+                 tp_at = place(xt * h->Q * h->row_cap * 32), list_at = place(rt * pieces * 8), count_at = place(rt * 4),
+                 up_at = place((size_t)slots * h->T * h->Q * kPiece), weight_at = place((size_t)h->T * h->P * kPiece);
+    h->bytes = at;
+    if ((e = cudaMalloc(reinterpret_cast<void **>(&h->memory), at)) != cudaSuccess ||
+        (e = cudaMemsetAsync(h->memory, 0, zeros, s)) != cudaSuccess) {
+        release(h);
+        return cuda_fail("create", e);
+    }
+    auto as = [&](auto *&p, size_t where) { p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(h->memory + where); };
+    as(h->rank, rank_at);
+    as(h->zero, zero_at);
+    as(h->acc, acc_at);
+    as(h->arrived, arrived_at);
+    as(h->error, error_at);
+    as(h->down, down_at);
+    as(h->scale, scale_at);
+    as(h->wsum, wsum_at);
+    as(h->xp, xp_at);
+    as(h->tp, tp_at);
+    as(h->list, list_at);
+    as(h->count, count_at);
+    as(h->up, up_at);
+    as(h->weight, weight_at);
+    k_pack_pieces<true><<<h->sms * 8, 256, 0, s>>>(weight, out_dim, in_dim, h->P, h->P, h->T, h->weight);
     k_weight_sums<<<h->T * (kOutTile / 8), 256, 0, s>>>(weight, out_dim, in_dim, h->T * kOutTile, h->wsum);
     if ((e = cudaGetLastError()) != cudaSuccess) {
         release(h);
@@ -1043,8 +1081,8 @@ extern "C" int llmx_adapters_set(llmx_adapters *h, uint32_t slot, uint32_t rank,
         const uint32_t words = rank * h->in_dim / 2, used = (rank + 15) / 16;
         k_pack_down<<<256, 256, 0, s>>>(reinterpret_cast<const uint32_t *>(down), words,
                                         h->down + (size_t)slot * h->Q * 16 * (h->in_dim / 2));
-        k_pack_pieces<<<h->sms * 4, 256, 0, s>>>(up, h->out_dim, rank, rank, used, h->Q, h->T,
-                                                 h->up + (size_t)slot * h->T * h->Q * kPiece);
+        k_pack_pieces<false><<<h->sms * 4, 256, 0, s>>>(up, h->out_dim, rank, used, h->Q, h->T,
+                                                        h->up + (size_t)slot * h->T * h->Q * kPiece);
     }
     k_set_slot<<<1, 1, 0, s>>>(h->rank, h->scale, slot, (int32_t)rank, scale);
     const cudaError_t e = cudaGetLastError();

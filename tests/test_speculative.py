@@ -1,0 +1,59 @@
+"""The serving loop of speculative.py: adapters, blocks and verification together."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def server(spec, model, drafts, ranks=(8, 3)):
+    s = model.shape
+    out = spec.Server(model, 3, len(ranks), max(ranks), drafts)
+    rng = np.random.default_rng(2)
+    for slot, rank in enumerate(ranks):
+        out.set_adapter(slot, 4096, rng.integers(-400, 400, (rank, s.hidden)), rng.integers(-400, 400, (s.vocab, rank)))
+    return out
+
+
+PROMPTS = [[3, 9, 4, 3, 9], [5, 5, 5, 5], [1, 2, 3, 1, 2, 3, 1]]
+
+
+def test_drafts_change_nothing_but_the_steps(llmx):
+    """Greedy: the tokens with drafts are those without, and some drafts are accepted;
+    a request without an adapter gets the tokens of the host's greedy loop."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    s = llmx.shape("small")
+    model = llmx.Model(s).init_reference_random(7)
+    results = []
+    for drafts in (0, 1, 4, 7):
+        sv = server(spec, model, drafts)
+        out, (drafted, taken) = sv.generate(PROMPTS, [0, -1, 1], 14)
+        sv.close()
+        assert [len(o) for o in out] == [14, 14, 14]
+        results.append(out)
+        assert (drafted == 0) == (drafts == 0)
+    assert all(r == results[0] for r in results)
+    acc = llmx.Accelerator(s)
+    acc.upload_model(model)
+    ex = llmx.Executor(acc, model)
+    text = list(PROMPTS[1])
+    hidden = ex.run_prompt_block(text, 0)[-1]
+    for _ in range(14):
+        text.append(model.lm_head_argmax(hidden))
+        hidden = ex.run_token(text[-1], len(text) - 1)[0]
+    assert text[len(PROMPTS[1]):] == results[0][1]
+
+
+def test_drawn_with_a_temperature(llmx):
+    """The same seed gives the same tokens; a request's tokens do not depend on the others' adapters."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    model = llmx.Model(llmx.shape("small")).init_reference_random(7)
+    sv = server(spec, model, 3)
+    a, _ = sv.generate(PROMPTS, [0, -1, 1], 20, temperature=1.0, seed=5)
+    b, _ = sv.generate(PROMPTS, [0, -1, 1], 20, temperature=1.0, seed=5)
+    c, _ = sv.generate(PROMPTS, [-1, -1, -1], 20, temperature=0.0)
+    d, _ = sv.generate(PROMPTS, [0, -1, 1], 20, temperature=0.0)
+    sv.close()
+    assert a == b
+    assert c[1] == d[1]
