@@ -67,11 +67,13 @@ constexpr uint32_t kMaxIn = 32768, kMaxOut = 1u << 22, kMaxSlots = 65536, kMaxRa
 constexpr int kOutTile = 128;             // outputs per tile (TMEM lanes) and inputs per item
 constexpr int kRowTile = 128;          // most rows per tile: 4 sums x 128 rows = all 512 TMEM columns
 constexpr int kPiece = 2 * kOutTile * 16; // bytes of a weight piece: two planes of 128 x 16
-constexpr int kProjectSmem = 221 * 1024;
-constexpr int kProjectThreads = 10 * 32; // TMEM + products, loads, 8 warps of results
-constexpr int kHeader = 16 * 16 + 96;  // barriers and flags at the start of shared memory, then the row-tile tables
+constexpr int kProjectSmem = 221 * 1024, kBesideSmem = 190 * 1024;  // alone on an SM, beside a block of k_prepare
+// TMEM + products, loads, and warps of results: 8, or 16 for wide row tiles, whose
+// accumulators fill the tensor memory, so that the next tile waits for the results
+__host__ __device__ constexpr int result_threads(int depth) { return depth == 4 ? 512 : 256; }
+__host__ __device__ constexpr int project_threads(int depth) { return 64 + result_threads(depth); }
+constexpr int kHeader = 16 * 16 + 32 + 16 + 64 + 16;  // barriers and flags at the start of shared memory, then the row-tile tables
 constexpr int kMaxRing = 16;
-constexpr int kResultThreads = 256;
 constexpr int kMoreTiles = 3;          // row tiles beyond the fewest that a call may take
 constexpr int kGroup = 8;              // rows of one adapter that share a pass over its down matrix
 
@@ -297,13 +299,15 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int 
     const int pair = warp % pairs, j0 = q * 16 + sub * R + pair * 2;
     for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
         const int rt = row / c.NT, at = row - rt * c.NT;
-        const int a = slot_of(c, row);
-        if (a < 0) continue;
+        const int a = c.slot[row];
+        if (a < 0 || a >= c.slots) continue;
+        const int rank = c.rank[a], scale = c.scale[a];
         const RowMask mask = rows_of_slot(c, rt, a);
         const int order = mask.before(at);
-        if (order % kGroup != 0 || q >= pieces_of(c, a)) continue;
+        if (order % kGroup != 0) continue;
+        // (the first piece does not wait for the rank: an empty slot's t is formed and never read)
+        if (q > 0 && q * 16 >= rank) continue;
         if (c.ksplit > 1) cluster_arrive();  // the sums' memory is free here
-        const int rank = c.rank[a], scale = c.scale[a];
         // members: the next 8 rows of the mask from this one on
         int member[kGroup], members = 0;
         {
@@ -465,10 +469,12 @@ struct Walk {
     }
 };
 
-// At most 96 registers a thread and kProjectSmem bytes of shared memory: a block of
-// k_prepare then fits beside it, so that neither waits for the other's SM.
+// D: pieces per ring stage.  With 8 (narrow row tiles) at most 96 registers a thread
+// and kBesideSmem bytes of shared memory: a block of k_prepare then fits beside it, so
+// that neither waits for the other's SM.
 template <int D>
-__global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
+__global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(const Call c) {
+    constexpr int kResultThreads = result_threads(D), kResultWarps = kResultThreads / 32;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint64_t *full = reinterpret_cast<uint64_t *>(smem);  // [kMaxRing] stage loaded
     uint64_t *empty = full + kMaxRing;                    // [kMaxRing] stage consumed
@@ -477,8 +483,8 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
     uint64_t *done = tempty + 2;                          // every MMA of the CTA complete
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(done + 1);
     int *last_s = reinterpret_cast<int *>(tmem_slot + 1);
-    int *fail_s = last_s + 1;                             // [8] wait outcome of each result warp
-    int32_t *pre = fail_s + 8;                            // [RT + 1] stages before each row tile
+    int *fail_s = last_s + 1;                             // [16] wait outcome of each result warp
+    int32_t *pre = fail_s + 16;                           // [RT + 1] stages before each row tile
     int32_t *pieces = pre + c.RT + 1;                     // [RT] adapter pieces of each row tile
     uint8_t *ring = smem + header_bytes(c.RT);
     const int NT = c.NT, C = c.C, S = c.ring;
@@ -705,9 +711,9 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
             if (!mbar_wait(done, 0)) atomicExch(c.error, 2);
         }
         __syncwarp();
-    } else {  // ---- results: warps 2-9, a thread per output of the tile and half of its rows ----
+    } else {  // ---- results: a thread per output of the tile and a half or a quarter of its rows ----
         const int q4 = warp & 3, m = q4 * 32 + lane;   // TMEM lanes of this warp, output of this thread
-        const int half = (warp - 2) >> 2;              // rows 16 i + 8 half .. + 7
+        const int part = (warp - 2) >> 2;              // rows 8 (i kResultWarps / 4 + part) .. + 7
         for (int tiles = 0; k.more(c); tiles++, k.next(c, pre)) {
             const int b = c.buffers == 2 ? tiles & 1 : 0, use = c.buffers == 2 ? tiles >> 1 : tiles;
             const bool whole = k.begin == 0 && k.end == k.len;
@@ -725,7 +731,9 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
             const bool okw = mbar_wait_err(tfull + b, use & 1, c.error);
             if (lane == 0) fail_s[warp - 2] = okw ? 0 : 1;
             named_sync(3, kResultThreads);
-            const int failed = fail_s[0] | fail_s[1] | fail_s[2] | fail_s[3] | fail_s[4] | fail_s[5] | fail_s[6] | fail_s[7];
+            int failed = 0;
+#pragma unroll
+            for (int w = 0; w < kResultWarps; w++) failed |= fail_s[w];
             named_sync(3, kResultThreads);  // read by all before the next tile writes it
             if (failed) {
                 if (threadIdx.x == 64) atomicCAS(c.error, 0, 3);
@@ -738,7 +746,7 @@ __global__ void __launch_bounds__(kProjectThreads, 2) k_project(const Call c) {
             // keeps the code small: it runs once or twice per CTA, mostly uncached.
             auto rows8 = [&](bool summed, bool add) {
 #pragma unroll 1
-                for (int r0 = 8 * half; r0 < rows; r0 += 16) {
+                for (int r0 = 8 * part; r0 < rows; r0 += 2 * kResultWarps) {
                     int64_t sum[8];
                     unsigned long long *at = acc + (size_t)r0 * kOutTile;
                     const int n = min(8, rows - r0);
@@ -1008,7 +1016,11 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
         (e = cudaFuncSetAttribute(k_project<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(k_project<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess) {
+        (e = cudaFuncSetAttribute(k_project<4>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
+        // an SM changes its division into L1 and shared memory only when it is empty: with
+        // k_prepare's default one k_project would wait for its blocks to end
+        (e = cudaFuncSetAttribute(k_prepare, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared)) !=
+            cudaSuccess) {
         release(h);
         return cuda_fail("create", e);
     }
@@ -1155,13 +1167,19 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     c.D = c.NT < 96 ? 8 : 4;
     c.C = c.P / c.D;
     const int stage = c.D * (kPiece + c.NT * 32), header = header_bytes(c.RT);
-    c.ring = std::min(kMaxRing, (kProjectSmem - header) / stage);
+    c.ring = std::min(kMaxRing, ((c.NT <= 64 ? kBesideSmem : kProjectSmem) - header) / stage);
     const int grid = (int)std::min<int64_t>(h->sms, (int64_t)c.T * c.RT * c.C);
     // A shared tile is cut into equal parts where that leaves at most a quarter of the CTAs
     // without one (every part then belongs to one tile only), else the line of all
-    // their stages is cut evenly.
+    // their stages is cut evenly.  Fewer tiles than CTAs stay whole where their stages
+    // (measured 0.45 us for 128 inputs) take no longer than a part's and adding the
+    // parts up (2 us and 0.085 a row: 77 rows x 1096 -> 4999 23 us cut in three).
     const int parts = c.shared_tiles ? grid / c.shared_tiles : 0;
     c.sharers = 4 * parts * c.shared_tiles >= 3 * grid ? parts * c.shared_tiles : grid;
+    if ((int64_t)c.T * c.RT < grid) {
+        const double depth = 0.45 * c.P / 8, share = depth * c.shared_tiles / c.sharers;
+        if (depth <= share + 2.0 + 0.085 * std::min<uint32_t>(rows, (uint32_t)c.NT)) c.shared_tiles = 0;
+    }
     // t: a block per row and 4 ranks while that is few blocks (most end at once: the
     // first row of 8 of an adapter does the work), else per 8 rows and 16 ranks; k is
     // cut so that a warp has about 512 inputs, over up to 8 blocks of a cluster
@@ -1174,7 +1192,7 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     const dim3 blocks((unsigned)(forms + (c.RT * (c.P / 8) + c.ksplit - 1) / c.ksplit + (c.slot ? c.RT : 0)), (unsigned)c.ksplit);
     cudaError_t e = launch((const void *)k_prepare, blocks, c.ksplit, kPrepareThreads, 0, c, s);
     if (e == cudaSuccess)
-        e = launch(c.D == 8 ? (const void *)k_project<8> : (const void *)k_project<4>, dim3((unsigned)grid), 1, kProjectThreads,
+        e = launch(c.D == 8 ? (const void *)k_project<8> : (const void *)k_project<4>, dim3((unsigned)grid), 1, project_threads(c.D),
                    header + (size_t)c.ring * stage, c, s);
     return e == cudaSuccess ? LLMX_OK : cuda_fail("project", e);
 }
