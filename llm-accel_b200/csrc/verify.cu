@@ -34,6 +34,7 @@
 namespace {
 
 using llmx::bulk_g2s;
+using llmx::bulk_g2s_hint;
 using llmx::mbar_arrive;
 using llmx::mbar_expect_tx;
 using llmx::mbar_init;
@@ -394,6 +395,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         if (lane == 0 && (kTwice || warp == kLoad)) {
             const int base = warp == kLoad ? 0 : kFirstRing;
             const int ring = !kTwice ? a.ring : warp == kLoad ? kFirstRing : a.ring - kFirstRing;
+            const uint64_t policy = llmx::evict_first_policy();
             int s = 0, phase = 1, issued = 0;
             bool ok = true;
             for (uint32_t row = group; ok && row < a.total; row += groups) {
@@ -406,7 +408,9 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                     }
                     const uint32_t bytes = min(r.v1 - v, (uint32_t)kChunk / 4) * 16;
                     mbar_expect_tx(full + at, bytes);
-                    bulk_g2s(smem + at * kChunkBytes, r.z + r.head + (size_t)v * 4, bytes, full + at);
+                    const int32_t *src = r.z + r.head + (size_t)v * 4;
+                    if (base == 0) bulk_g2s(smem + at * kChunkBytes, src, bytes, full + at);
+                    else bulk_g2s_hint(smem + at * kChunkBytes, src, bytes, full + at, policy);  // not needed again
                     issued++;
                     if (++s == ring) {
                         s = 0;
@@ -640,7 +644,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
 // accept tests and the drawn token, a cluster per request
 // ---------------------------------------------------------------------------
 constexpr int kDrawWarps = 16, kDrawThreads = kDrawWarps * 32;
-constexpr int kRuns = 32;
+constexpr int kRuns = 8;
 constexpr uint32_t kKeep = 32;  // rows of a request whose numbers stay in shared memory
 struct DrawArgs {
     Args a;
@@ -792,25 +796,23 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
             mine = 0;
             Four next;
             if (v0 < v1) fetch(v0, rest, next);
-            uint32_t in_run = 0, at_run = 0;
+            uint32_t next_run = v0 + run, at_run = 0;
             for (uint32_t v = v0; v < v1; v += 128) {  // the next step's logits under way while this one's are summed
                 const Four z = next;
                 if (v + 128 < v1) fetch(v + 128, rest, next);
-                // nothing where p is nothing: below the likely tokens that is most of a row
-                const uint32_t d = min(min(wt.base - (uint32_t)z.t[0], wt.base - (uint32_t)z.t[1]),
-                                       min(wt.base - (uint32_t)z.t[2], wt.base - (uint32_t)z.t[3]));
-                if (!wt.fast || __any_sync(~0u, d < wt.most)) {
+                // nothing where p is nothing
+                const int32_t most = max(max(z.t[0], z.t[1]), max(z.t[2], z.t[3]));
+                if (!wt.fast || !__all_sync(~0u, wt.base - (uint32_t)most >= wt.most)) {
                     uint64_t m[4];
                     four(v, rest, z, m);
                     mine += (m[0] + m[1]) + (m[2] + m[3]);
                 }
-                in_run += 128;
-                if (v + 128 >= v1 || in_run == run) {
+                if (v + 128 >= v1 || v + 128 == next_run) {
                     unsigned long long t = mine;
                     for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
                     if (lane == 0) run_sum[warp][at_run] = t;  // of all runs so far
                     at_run++;
-                    in_run = 0;
+                    next_run += run;
                 }
             }
             for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
