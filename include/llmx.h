@@ -427,9 +427,11 @@ size_t llmx_verify_workspace_bytes(uint32_t requests, uint32_t drafts, uint32_t 
  *   probs         device, [drafts][2]: P and Q of each drafted token (Q0.40), or NULL
  *   workspace     device, 256-byte aligned, llmx_verify_workspace_bytes of the
  *                 same sizes (or larger ones); one call at a time may use it
- * Rows whose length or stride is not a multiple of 4, or whose base is not 16-byte
- * aligned, are served with narrower loads.  Stream-ordered, allocates nothing,
- * may be captured into a graph. */
+ * Rows of any alignment and length are served alike.  Runs on the current device,
+ * stream-ordered; allocates nothing and may be captured into a graph (after a
+ * first call on the device, which looks up how many clusters fit it).  A request
+ * one of whose rows a kernel gave up (a bounded wait that ran out) gets accepted =
+ * 0xffffffff as well; probs of the drafts of requests without tokens are not written. */
 int llmx_verify_drafts(const int32_t *target, size_t ld_target, const int32_t *draft, size_t ld_draft,
                        uint32_t vocab, const uint32_t *draft_tokens, const uint32_t *offsets,
                        uint32_t requests, uint32_t drafts, uint32_t max_drafts,

@@ -29,20 +29,26 @@
 //
 // Layouts.  k is cut into pieces of 16 (one 16-byte core-matrix column): a
 // weight piece is [high | low][128 outputs][16 bytes] = 4 KiB, a row piece
-// [high | low][row tile][16 bytes].  Eight weight pieces in a row are an item of 128 outputs x
-// 128 inputs; an adapter of rank r has ceil(r / 16) pieces per 128 outputs, so
-// pieces of different adapters fill one 32-deep MMA step together and a rank of 16
-// wastes nothing.  All of it lands in shared memory by 1-D bulk copies.
+// [high | low][row tile][16 bytes].  A stage of the ring is 8 pieces (4 for wide row
+// tiles) of 128 outputs; an adapter of rank r has ceil(r / 16) pieces per 128
+// outputs, so pieces of different adapters fill one 32-deep MMA step together and a
+// rank of 16 wastes nothing.  All of it lands in shared memory by 1-D bulk copies.
 //
-// Two launches per call.  k_prepare splits the rows into pieces and forms t (a
-// block per 16 ranks and up to 8 rows of one adapter in one row tile, so that
-// an adapter's down matrix is read once for 8 rows).  k_project streams the
-// items: tiles of 128 outputs x up to 128 rows, the items of all tiles in one
-// line cut evenly over one CTA per SM (a tile cut between CTAs is summed in
-// int64 atomics, which no order changes, and finished by the last to arrive);
-// row tiles of the same outputs are neighbours in that line, so a weight item
-// comes from HBM once.  k_project starts under k_prepare (dependent launch): its
-// ring of weight items fills while the rows are still being split.
+// Two launches per call.  k_prepare splits the rows into pieces and forms t;
+// k_project streams the stages of tiles of 128 outputs x up to 128 rows through one
+// CTA per SM, and starts under k_prepare (dependent launch): its ring of weight
+// stages fills while the rows are still being split.  Row tiles of the same outputs
+// are neighbours, so a weight stage comes from HBM once.
+//
+// What bounds it (B200, in a graph of calls; bytes at 6.47 TB/s, exact products at
+// a quarter of the int8 rate, which a loop of such MMAs measured as 4.5 P/s).  Up to
+// about 64 rows the weight stream: LM head 151936 x 2048, 40 rows of 8 adapters, 105 us =
+// 0.97 of the floor of 102; Gate/Up 22016 x 2048, 16 rows of 16 adapters, 27.5 us
+// against 16.9, of which 7 pass before k_prepare's t is there and the tail takes 2.
+// 512 rows x 11008 x 2048 with rank 64: 69 us against 20.8 of products; per tile of 112
+// rows the stages take 10.8 us (shared memory: 44 KB read by the MMAs and 30 KB
+// written per 64 inputs, at 128 bytes a cycle) and the results 2, three tiles each,
+// after 16 us of k_prepare.  One row x 2560 x 2048: 9.9 us, the two kernels' latencies.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -227,7 +233,7 @@ static __device__ void split_item(const Call &c, int item) {
     }
 }
 
-constexpr int kPrepareThreads = 256, kMaxSplit = 4;
+constexpr int kPrepareThreads = 256, kMaxSplit = 8;
 
 // Adds a value to the first block of the cluster's shared memory at p's place (the
 // blocks write different words).
@@ -384,7 +390,12 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int 
     }
 }
 
-// Blocks (x, share): per x first the rows' items and lists, then t.
+// Blocks (x, share): per x first t, then the rows' pieces and the lists of the row tiles'
+// adapters.  Bound by latency: slots, then ranks, then products, 1.2 us each at one
+// row (4 KiB of a row, 64 KiB of a rank-16 down matrix), and by the dp2a pipe with
+// hundreds of rows (512 rows of rank 64: 9 us of products).  Blocks of 4 ranks with
+// k cut over their warps (and over a cluster's blocks) halved the first: 8 rows
+// x 11008 25 -> 9 us against blocks of 16 ranks over all of k.
 __global__ void __launch_bounds__(kPrepareThreads, 2) k_prepare(const Call c) {
     __shared__ TileSlots ts;
     pdl_wait();     // the caller's rows, and the last call's reads of the workspace
@@ -469,6 +480,12 @@ struct Walk {
     }
 };
 
+// Warp roles: 0 tensor memory and products, 1 loads, the others results.  The issuing
+// lanes' instructions pace a stage (an MMA of 32 columns takes 41 cycles, one whose
+// descriptors are computed anew 190), so each loop over stages has little more
+// than its wait, its issue and its commit: LM head 40 rows 132 -> 111 us.  Result code is
+// small for the same reason (it runs a few times per CTA, from a cold instruction
+// cache): one body instead of two took 77 rows x 1096 -> 4999 from 31 to 23 us.
 // D: pieces per ring stage.  With 8 (narrow row tiles) at most 96 registers a thread
 // and kBesideSmem bytes of shared memory: a block of k_prepare then fits beside it, so
 // that neither waits for the other's SM.
