@@ -245,17 +245,21 @@ static __device__ __forceinline__ void store_first(int64_t *p, int64_t v) {
 static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Products of two down rows (d, d + ld) with M rows over vectors [va, vb): sum[2 g + rank].
-// U vectors of every row are in flight per lane; int32 partials are flushed
-// after at most 16 vectors of 8 products: |lo| <= 128 * 255 * 2^15 < 2^30.
+// Sums over vectors [va, vb) of the products of two down rows (d, d + ld) with M rows,
+// over the lanes too: a lane ends with the sum of number idx (2 * row + down row), as
+// 16 / M lanes do.  U vectors of every row are in flight per lane; int32 partials join
+// the sum every 4096 inputs: |lo| <= 16 * 8 * 255 * 2^15 < 2^30.
 template <int M, int U>
-static __device__ __forceinline__ void down_dots(const uint4 *d, int ld, const uint4 *const (&xr)[kGroup], int va, int vb,
-                                                 int lane, int64_t (&sum)[2 * kGroup]) {
+static __device__ __forceinline__ int64_t down_dots(const uint4 *d, int ld, const uint4 *const (&xr)[kGroup], int va, int vb,
+                                                    int lane, int &idx) {
     const uint4 none = make_uint4(0, 0, 0, 0);
-    for (int v0 = va; v0 < vb; v0 += 32 * 16) {
+    int64_t mine = 0;
+    int v0 = va;
+    do {  // (once at least: idx is the reduction's)
         int lo[2 * M], hi[2 * M];
 #pragma unroll
         for (int g = 0; g < 2 * M; g++) lo[g] = hi[g] = 0;
+#pragma unroll 1
         for (int k = 0; k < 16 && v0 + k * 32 < vb; k += U) {
             uint4 w[2][U], x[M][U];
 #pragma unroll
@@ -284,9 +288,13 @@ static __device__ __forceinline__ void down_dots(const uint4 *d, int ld, const u
                         hi[i] = dp2a_hi_ss(x[g][u].w, w[r][u].w, hi[i]);
                     }
         }
+        int64_t sum[2 * M];
 #pragma unroll
-        for (int g = 0; g < 2 * M; g++) sum[g] += (int64_t)hi[g] * 256 + lo[g];
-    }
+        for (int g = 0; g < 2 * M; g++) sum[g] = (int64_t)hi[g] * 256 + lo[g];
+        mine += warp_reduce_n<2 * M>(sum, lane, idx);
+        v0 += 32 * 16;
+    } while (v0 < vb);
+    return mine;
 }
 
 // t of rows [row0, row0 + span) for `ranks` (16 or 4) ranks of their adapters from 16
@@ -338,23 +346,20 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int 
         for (int g = 0; g < kGroup; g++)
             xr[g] = reinterpret_cast<const uint4 *>(c.x + ((size_t)rt * c.NT + member[g]) * c.ld_x);
         const uint4 *d0 = reinterpret_cast<const uint4 *>(c.down + ((size_t)a * c.Q * 16 + j0) * c.down_words);
-        int64_t sum[2 * kGroup];
-#pragma unroll
-        for (int g = 0; g < 2 * kGroup; g++) sum[g] = 0;
-        if (members == 1) down_dots<1, 4>(d0, c.down_words / 4, xr, va, vb, lane, sum);
-        else if (members == 2) down_dots<2, 2>(d0, c.down_words / 4, xr, va, vb, lane, sum);
-        else if (members <= 4) down_dots<4, 2>(d0, c.down_words / 4, xr, va, vb, lane, sum);
-        else down_dots<8, 1>(d0, c.down_words / 4, xr, va, vb, lane, sum);
-        int idx;
-        const int64_t mine = warp_reduce_n<2 * kGroup>(sum, lane, idx);
+        int idx, same;  // lanes that hold one sum
+        int64_t mine;
+        if (members == 1) mine = down_dots<1, 4>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 16;
+        else if (members <= 4) mine = down_dots<4, 2>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 4;
+        else mine = down_dots<8, 1>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 2;
+        const bool holds = lane % same == 0 && (idx >> 1) < members;
         int64_t *place = sum_s + (part * kGroup + (idx >> 1)) * R + pair * 2 + (idx & 1);
         if (c.ksplit > 1) {
             cluster_wait();
-            if ((lane & 1) == 0) store_first(place, mine);  // two lanes hold each sum
+            if (holds) store_first(place, mine);
             cluster_arrive();
             cluster_wait();
         } else {
-            if ((lane & 1) == 0) *place = mine;
+            if (holds) *place = mine;
             __syncthreads();
         }
         if (share == 0) {
@@ -427,17 +432,18 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_prepare(const Call c) {
 // the projection
 // ---------------------------------------------------------------------------
 static __host__ __device__ __forceinline__ int header_bytes(int RT) { return (kHeader + (2 * RT + 1) * 4 + 127) / 128 * 128; }
-static __device__ __forceinline__ int64_t range_begin(int b, int64_t stages, int grid) { return stages * b / grid; }
-static __device__ __forceinline__ int cta_of(int64_t i, int64_t stages, int grid) {
-    int b = (int)(i * grid / stages);
+// Shared stages are those of fewer tiles than there are SMs: 32 bits hold them times the CTAs.
+static __device__ __forceinline__ int range_begin(int b, int stages, int grid) { return stages * b / grid; }
+static __device__ __forceinline__ int cta_of(int i, int stages, int grid) {
+    int b = i * grid / stages;
     while (b + 1 < grid && range_begin(b + 1, stages, grid) <= i) b++;
     while (b > 0 && range_begin(b, stages, grid) > i) b--;
     return b;
 }
-// Stages before tile t in the line of all tiles (row tiles of the same outputs
+// Stages before shared tile t in the line of all of them (row tiles of the same outputs
 // are neighbours); pre[rt]: stages of the row tiles before rt.
-static __device__ __forceinline__ int64_t line_at(int t, const int32_t *pre, int RT) {
-    return (int64_t)(t / RT) * pre[RT] + pre[t % RT];
+static __device__ __forceinline__ int line_at(int t, const int32_t *pre, int RT) {
+    return RT == 1 ? t * pre[1] : t / RT * pre[RT] + pre[t % RT];
 }
 
 // A CTA's way through the tiles: its run of the stages of the first `shared`
@@ -451,20 +457,20 @@ struct Walk {
 
     __device__ __forceinline__ void set(const Call &c, const int32_t *pre, int t, int stage) {
         tile = t;
-        ft = t / c.RT;
+        ft = c.RT == 1 ? t : t / c.RT;
         rt = t - ft * c.RT;
         len = pre[rt + 1] - pre[rt];
         begin = stage;
         end = left > 0 ? min(len, begin + left) : len;
     }
-    __device__ __forceinline__ void start(const Call &c, const int32_t *pre, int64_t w0, int64_t w1) {
-        left = (int)(w1 - w0);
+    __device__ __forceinline__ void start(const Call &c, const int32_t *pre, int w0, int w1) {
+        left = w1 - w0;
         if (left == 0) {
             set(c, pre, c.shared_tiles + blockIdx.x, 0);
             return;
         }
         const int per = pre[c.RT];
-        const int f = (int)(w0 / per), rem = (int)(w0 - (int64_t)f * per);
+        const int f = w0 / per, rem = w0 - f * per;
         int r = 0;
         while (r + 1 < c.RT && pre[r + 1] <= rem) r++;
         set(c, pre, f * c.RT + r, rem - pre[r]);
@@ -560,9 +566,9 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int64_t line = line_at(c.shared_tiles, pre, c.RT);  // stages that are shared out one by one
+    const int line = line_at(c.shared_tiles, pre, c.RT);  // stages that are shared out one by one
     // no more sharers than stages: every CTA between a tile's first and last takes a part in it
-    const int sharers = (int)min((int64_t)c.sharers, max(line, (int64_t)1)), me = min((int)blockIdx.x, sharers);
+    const int sharers = min(c.sharers, max(line, 1)), me = min((int)blockIdx.x, sharers);
     Walk k;
     k.start(c, pre, range_begin(me, line, sharers), range_begin(min(me + 1, sharers), line, sharers));
 
@@ -740,7 +746,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
             const int rows = min(NT, (int)c.rows - k.rt * NT);
             int b_lo = 0, b_hi = 0;
             if (!whole) {
-                const int64_t at = line_at(k.tile, pre, c.RT);
+                const int at = line_at(k.tile, pre, c.RT);
                 b_lo = cta_of(at, line, sharers);
                 b_hi = cta_of(at + k.len - 1, line, sharers);
             }
