@@ -117,6 +117,25 @@ struct Call {
     int sharers;           // CTAs that share them
 };
 
+// Results are many and their arithmetic is all that the result warps do, so it is kept
+// short: sums by 64-bit multiply-adds, each rounding in the width that holds it.
+static __device__ __forceinline__ int64_t mad_wide(int32_t a, int32_t b, int64_t c) {
+    int64_t r;
+    asm("mad.wide.s32 %0, %1, %2, %3;" : "=l"(r) : "r"(a), "r"(b), "l"(c));
+    return r;
+}
+// sat32(rnd4(s - 8)): the 8 of the rounding is in the sum already.
+static __device__ __forceinline__ int32_t to_q16(int64_t s) {
+    const uint32_t lo = (uint32_t)s;
+    const int32_t hi = (int32_t)(s >> 32), v = (int32_t)__funnelshift_r(lo, (uint32_t)hi, 4);
+    return (hi >> 4) == (v >> 31) ? v : (hi >> 31) ^ 0x7fffffff;
+}
+// sat16(rnd8(v)), without the carry out of 32 bits.
+static __device__ __forceinline__ int32_t to_q8(int32_t v) {
+    v = (v >> 8) + ((v >> 7) & 1);
+    return min(max(v, -32768), 32767);
+}
+
 static __device__ __forceinline__ int slot_of(const Call &c, uint32_t row) {
     if (!c.slot || row >= c.rows) return -1;
     const int a = c.slot[row];
@@ -742,7 +761,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
             const bool whole = k.begin == 0 && k.end == k.len;
             const int o = k.ft * kOutTile + m;
             const bool live = o < c.N;
-            const int64_t corr = k.begin == 0 ? 128 * (int64_t)c.wsum[o] : 0;
+            const int64_t corr = k.begin == 0 ? 128 * (int64_t)c.wsum[o] + 8 : 0;  // and half of a Q16.16 step, for the rounding
             const int rows = min(NT, (int)c.rows - k.rt * NT);
             int b_lo = 0, b_hi = 0;
             if (!whole) {
@@ -781,9 +800,9 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                         tmem_ld4x8(t0 + r0, t0 + NT + r0, t0 + 2 * NT + r0, t0 + 3 * NT + r0, v);
 #pragma unroll
                         for (int r = 0; r < 8; r++)
-                            sum[r] = (int64_t)(int32_t)v[r] * 65536 +
-                                     ((int64_t)(int32_t)v[8 + r] + (int64_t)(int32_t)v[16 + r]) * 256 +
-                                     (int64_t)(int32_t)v[24 + r] + corr;
+                            // hs + lh <= 2^15 * (2^14 + 255 * 2^7) < 2^31
+                            sum[r] = mad_wide((int32_t)v[r], 65536,
+                                              mad_wide((int32_t)(v[8 + r] + v[16 + r]), 256, mad_wide((int32_t)v[24 + r], 1, corr)));
                     }
                     if (add) {
 #pragma unroll
@@ -802,12 +821,12 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                         int32_t *out = static_cast<int32_t *>(c.out) + first;
 #pragma unroll
                         for (int r = 0; r < 8; r++, out += c.ld_out)
-                            if (r < n) *out = sat32(rnd(sum[r], 4));
+                            if (r < n) *out = to_q16(sum[r]);
                     } else {
                         int16_t *out = static_cast<int16_t *>(c.out) + first;
 #pragma unroll
                         for (int r = 0; r < 8; r++, out += c.ld_out)
-                            if (r < n) *out = (int16_t)sat16(rnd(sat32(rnd(sum[r], 4)), 8));
+                            if (r < n) *out = (int16_t)to_q8(to_q16(sum[r]));
                     }
                 }
             };
