@@ -660,7 +660,9 @@ struct DrawArgs {
     int split;  // CTAs per request
 };
 
-__global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
+// kModel: drafts have a distribution of their own.
+template <bool kModel>
+__global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const Args &a = d.a;
     __shared__ uint32_t first_s, bad_s;
     __shared__ RowMass mass_s[kKeep][2], last_s[2];
@@ -686,7 +688,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
     // j = count is the row after the last draft
     for (uint32_t j = warp; valid && j <= count; j += kDrawWarps) {
         const uint32_t e = begin + j;
-        const bool is_draft = lane >= 16, has = j < count, there = is_draft ? has && a.draft : true;
+        const bool is_draft = lane >= 16, has = j < count, there = is_draft ? has && kModel : true;
         const RowMass m = load_row(a.rows, there && is_draft ? targets + e : e + b, a.split);
         if (!m.ok && (lane & 15) == 0) bad_s = 1;
         if ((lane & 15) == 0 && j < kKeep) mass_s[j][lane >> 4] = m;
@@ -700,7 +702,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
             row_weight2(rw, m.first, z, z, x, x, w, none);
             share = row_share(w, m);
         }
-        if (is_draft && !a.draft) share = 1ull << 40;
+        if (is_draft && !kModel) share = 1ull << 40;
         const uint64_t p = __shfl_sync(~0u, share, 0), q = __shfl_sync(~0u, share, 16);
         if (has && lane == 0) {
             if (a.probs && rank == 0) {
@@ -712,7 +714,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
     }
     __syncthreads();
     const uint32_t n = first_s;
-    const bool rejected = n < count, both = rejected && a.draft != nullptr;
+    const bool rejected = n < count, both = kModel && rejected;
     const uint32_t trow = begin + b + n, drow = begin + n;
     if (n >= kKeep && warp == 0) {
         const RowMass m = load_row(a.rows, lane >= 16 && both ? targets + drow : trow, a.split);
@@ -726,7 +728,7 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
     if (!bad) {
         RowWeight wt, wd;
         wt.set(mt.top, mt.scale, a.minus_zero);
-        wd.set(md.top, md.scale, a.minus_zero);
+        if (kModel) wd.set(md.top, md.scale, a.minus_zero);
         const int32_t *zt = a.target + trow * a.ld_target, *zd = both ? a.draft + drow * a.ld_draft : zt;
         const uint32_t x = rejected ? a.draft_tokens[drow] : kNoToken;
         // a CTA has a run of the vocabulary, a warp a run of that, in steps of 128
@@ -734,68 +736,59 @@ __global__ void __launch_bounds__(kDrawThreads) k_draw(const DrawArgs d) {
         const uint32_t v0 = (uint32_t)((uint64_t)steps * part / parts) * 128,
                        v1 = min(a.vocab, (uint32_t)((uint64_t)steps * (part + 1) / parts) * 128);
         const uint32_t run = ((v1 - v0 + 127) / 128 + kRuns - 1) / kRuns * 128;  // logits per run
-        // logits v + lane + 32 u of both rows, and what is drawn from there (rest: p less q)
+        // logits v + lane + 32 u of both rows, and what is drawn from there
         struct Four {
-            int32_t t[4], q[4];
+            int32_t t[4], q[kModel ? 4 : 1];
         };
         auto fetch = [&](uint32_t v, bool rest, Four &z) {
             const int32_t *pt = zt + v + lane, *pq = zd + v + lane;
             if (v + 128 <= v1) {
 #pragma unroll
-                for (int u = 0; u < 4; u++) {
-                    z.t[u] = pt[32 * u];
-                    if (both && rest) z.q[u] = pq[32 * u];
-                }
+                for (int u = 0; u < 4; u++) z.t[u] = pt[32 * u];
+                if (kModel && both && rest)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) z.q[kModel ? u : 0] = pq[32 * u];
             } else {
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const bool in = v + lane + 32 * u < v1;
                     z.t[u] = in ? pt[32 * u] : kExcluded;
-                    z.q[u] = both && rest && in ? pq[32 * u] : kExcluded;
+                    if (kModel) z.q[kModel ? u : 0] = both && rest && in ? pq[32 * u] : kExcluded;
                 }
             }
         };
-        const bool usual = wt.fast && mt.shift < 32, usual_both = usual && both && wd.fast && md.shift < 32;
+        // Q0.40 probabilities of four logits of a row
+        auto shares = [&](const RowWeight &w, const RowMass &row, bool usual, uint32_t v, const int32_t *z, uint64_t (&m)[4]) {
+            uint32_t x0, x1, x2, x3;
+            if (usual) {
+                w.fast2(z[0], z[1], x0, x1);
+                w.fast2(z[2], z[3], x2, x3);
+                m[0] = row_share_small(x0, row);
+                m[1] = row_share_small(x1, row);
+                m[2] = row_share_small(x2, row);
+                m[3] = row_share_small(x3, row);
+            } else {
+                const uint32_t at = v + lane;
+                row_weight2(w, row.first, z[0], z[1], at, at + 32, x0, x1);
+                row_weight2(w, row.first, z[2], z[3], at + 64, at + 96, x2, x3);
+                m[0] = row_share(x0, row);
+                m[1] = row_share(x1, row);
+                m[2] = row_share(x2, row);
+                m[3] = row_share(x3, row);
+            }
+        };
+        const bool usual_t = wt.fast && mt.shift < 32, usual_q = kModel && wd.fast && md.shift < 32;
         auto four = [&](uint32_t v, bool rest, const Four &z, uint64_t (&m)[4]) {
-            if (usual && !rest) {
+            shares(wt, mt, usual_t, v, z.t, m);
+            if (!rest) return;
+            if (kModel) {
+                uint64_t q[4];
+                shares(wd, md, usual_q, v, z.q, q);
 #pragma unroll
-                for (int u = 0; u < 4; u += 2) {
-                    uint32_t w0, w1;
-                    wt.fast2(z.t[u], z.t[u + 1], w0, w1);
-                    m[u] = row_share_small(w0, mt);
-                    m[u + 1] = row_share_small(w1, mt);
-                }
-                return;
-            }
-            if (usual_both && rest) {
+                for (int u = 0; u < 4; u++) m[u] = m[u] > q[u] ? m[u] - q[u] : 0;
+            } else {  // q is all at x, and p at most that
 #pragma unroll
-                for (int u = 0; u < 4; u += 2) {
-                    uint32_t t0, t1, q0, q1;
-                    wt.fast2(z.t[u], z.t[u + 1], t0, t1);
-                    wd.fast2(z.q[u], z.q[u + 1], q0, q1);
-                    const int64_t d0 = (int64_t)(row_share_small(t0, mt) - row_share_small(q0, md));
-                    const int64_t d1 = (int64_t)(row_share_small(t1, mt) - row_share_small(q1, md));
-                    m[u] = d0 > 0 ? d0 : 0;
-                    m[u + 1] = d1 > 0 ? d1 : 0;
-                }
-                return;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; u += 2) {
-                const uint32_t at = v + lane + 32 * u;
-                uint32_t w0, w1;
-                row_weight2(wt, mt.first, z.t[u], z.t[u + 1], at, at + 32, w0, w1);
-                m[u] = row_share(w0, mt);
-                m[u + 1] = row_share(w1, mt);
-                if (!rest) continue;
-                uint64_t q0 = at == x ? 1ull << 40 : 0, q1 = at + 32 == x ? 1ull << 40 : 0;
-                if (both) {
-                    row_weight2(wd, md.first, z.q[u], z.q[u + 1], at, at + 32, w0, w1);
-                    q0 = row_share(w0, md);
-                    q1 = row_share(w1, md);
-                }
-                m[u] = m[u] > q0 ? m[u] - q0 : 0;
-                m[u + 1] = m[u + 1] > q1 ? m[u + 1] - q1 : 0;
+                for (int u = 0; u < 4; u++) m[u] = v + lane + 32 * u == x ? 0 : m[u];
             }
         };
         // p less q after a rejection; should that be nothing at all, p
@@ -935,7 +928,8 @@ cudaError_t device_setup(DeviceSetup &out) {
             if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
             if ((e = cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         }
-        if ((e = cudaFuncSetAttribute(k_draw, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(k_draw<false>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+        if ((e = cudaFuncSetAttribute(k_draw<true>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
         d.clusters[1] = d.sms;
         for (int c : kSplits) {
             if (c == 1) continue;
@@ -1049,7 +1043,7 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     DrawArgs d{a, 1};
     while (d.split < kMaxCluster && requests * d.split * 2 <= (uint32_t)dev.sms * 2 && vocab >= 2048u * d.split) d.split *= 2;
     configure(cfg, attr, dim3(requests * d.split), kDrawThreads, 0, d.split, s);
-    e = cudaLaunchKernelEx(&cfg, k_draw, d);
+    e = cudaLaunchKernelEx(&cfg, a.draft ? k_draw<true> : k_draw<false>, d);
     if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("k_draw: ") + cudaGetErrorString(e));
     return LLMX_OK;
 }
