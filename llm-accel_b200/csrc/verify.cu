@@ -84,7 +84,6 @@ struct Args {
     int split;       // CTAs per row (k_mass), and of a cluster there
     int ring;        // chunks of shared memory per CTA
     int resident;    // the ring holds a CTA's share of a row: it is loaded once
-    unsigned long long minus_zero;  // two -0.0f (mul2)
 };
 
 // ---- arithmetic -------------------------------------------------------------------
@@ -109,14 +108,15 @@ static __device__ __forceinline__ f32x2 pack2(float a, float b) {
 static __device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) {
     asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
 }
-// a * b, rounded on its own: a fused operation with -0, which the compiler must not
-// see through (it fuses a packed product, mul.rn or with a constant -0, with the
-// addition that follows it, and the weights would differ in their last bits).
-// So the -0 is a kernel argument.
-static __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b, f32x2 minus_zero) {
-    f32x2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(minus_zero));
-    return r;
+// Products of pairs one by one: a packed mul.rn is fused by the compiler with the packed
+// addition that follows it, and the weights would differ in their last bits; a scalar
+// product and a packed sum it cannot fuse. (A packed fma with a -0 that the compiler
+// cannot see through is as exact: 64 requests x 7 drafts 162 us against 155.)
+static __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    float a0, a1, b0, b1;
+    unpack2(a, a0, a1);
+    unpack2(b, b0, b1);
+    return pack2(__fmul_rn(a0, b0), __fmul_rn(a1, b1));
 }
 static __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     f32x2 r;
@@ -137,7 +137,7 @@ static __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
 // steps.  Here x = -e; adding 1.5 * 2^23 rounds it to the nearest whole number
 // (even at ties) and leaves that number in the low bits, from where one shifted
 // addition puts it into the exponent.  The coefficients carry the 2^31.  Packed
-// pairs halve the float instructions, which a row's second pass spends most of its time on.
+// pairs halve the sums' instructions; a row's second pass spends most of its time on these steps.
 //   The usual row (fast) needs no conversion to float: with d = top - z below
 // 2^23, the bits of 2^23 + d are 0x4b000000 + d, and (2^23 + d) (-scale) + 2^23 scale in one
 // fused step is d (-scale) rounded once (2^23 scale is exact).  A d of 32 / scale
@@ -149,9 +149,9 @@ struct RowWeight {
     float scale;
     bool greedy, fast, test;  // test: an excluded logit is not far enough below the maximum to vanish by itself
     uint32_t base, most;      // fast: 0x4b000000 + top, 0x4b000000 + the largest d
-    f32x2 minus_scale, shift, mz;
+    f32x2 minus_scale, shift;
 
-    __device__ __forceinline__ void set(int32_t t, float s, f32x2 minus_zero) {
+    __device__ __forceinline__ void set(int32_t t, float s) {
         top = t;
         scale = s;
         greedy = s < 0.0f;
@@ -162,17 +162,16 @@ struct RowWeight {
         most = 0x4b000000u + (fast ? __float2uint_ru(limit) : 0u);
         minus_scale = pack2(-s, -s);
         shift = pack2(8388608.0f * s, 8388608.0f * s);
-        mz = minus_zero;
     }
     // the second half, from x = -e
     __device__ __forceinline__ void finish(f32x2 x, uint32_t &w0, uint32_t &w1) const {
         const f32x2 magic = pack2(12582912.0f, 12582912.0f), minus_magic = pack2(-12582912.0f, -12582912.0f);
         const f32x2 m = add2(x, magic), f = fma2(add2(m, minus_magic), pack2(-1.0f, -1.0f), x);
-        f32x2 p = add2(mul2(f, pack2(0x1.5bba12p21f, 0x1.5bba12p21f), mz), pack2(0x1.3cea88p24f, 0x1.3cea88p24f));
-        p = add2(mul2(p, f, mz), pack2(0x1.c6b752p26f, 0x1.c6b752p26f));
-        p = add2(mul2(p, f, mz), pack2(0x1.ebf9bcp28f, 0x1.ebf9bcp28f));
-        p = add2(mul2(p, f, mz), pack2(0x1.62e42ap30f, 0x1.62e42ap30f));
-        p = add2(mul2(p, f, mz), pack2(0x1p31f, 0x1p31f));
+        f32x2 p = add2(mul2(f, pack2(0x1.5bba12p21f, 0x1.5bba12p21f)), pack2(0x1.3cea88p24f, 0x1.3cea88p24f));
+        p = add2(mul2(p, f), pack2(0x1.c6b752p26f, 0x1.c6b752p26f));
+        p = add2(mul2(p, f), pack2(0x1.ebf9bcp28f, 0x1.ebf9bcp28f));
+        p = add2(mul2(p, f), pack2(0x1.62e42ap30f, 0x1.62e42ap30f));
+        p = add2(mul2(p, f), pack2(0x1p31f, 0x1p31f));
         float m0, m1, p0, p1;
         unpack2(m, m0, m1);
         unpack2(p, p0, p1);
@@ -185,7 +184,7 @@ struct RowWeight {
     }
     __device__ __forceinline__ void slow2(int32_t z0, int32_t z1, uint32_t &w0, uint32_t &w1) const {
         float x0 = __uint2float_rn((uint32_t)top - (uint32_t)z0), x1 = __uint2float_rn((uint32_t)top - (uint32_t)z1);
-        unpack2(mul2(pack2(x0, x1), minus_scale, mz), x0, x1);
+        unpack2(mul2(pack2(x0, x1), minus_scale), x0, x1);
         finish(pack2(fmaxf(x0, -100.0f), fmaxf(x1, -100.0f)), w0, w1);
         w0 = z0 == kExcluded ? 0u : w0;
         w1 = z1 == kExcluded ? 0u : w1;
@@ -547,7 +546,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             if (lane == 0) mbar_arrive(info_empty + (i & 1));
             ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1);
             const int32_t t = __reduce_max_sync(~0u, lane < S ? tops[i % kTops][lane] : kExcluded);
-            rw.set(t, scale, a.minus_zero);
+            rw.set(t, scale);
             sum = 0;
             first = kNoToken;
             if (h.edge_at != kNoToken) {
@@ -697,7 +696,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
         if (x < a.vocab && there) {
             const int32_t z = is_draft ? a.draft[e * a.ld_draft + x] : a.target[(e + b) * a.ld_target + x];
             RowWeight rw;
-            rw.set(m.top, m.scale, a.minus_zero);
+            rw.set(m.top, m.scale);
             uint32_t w, none;
             row_weight2(rw, m.first, z, z, x, x, w, none);
             share = row_share(w, m);
@@ -727,8 +726,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const bool bad = bad_s != 0;
     if (!bad) {
         RowWeight wt, wd;
-        wt.set(mt.top, mt.scale, a.minus_zero);
-        if (kModel) wd.set(md.top, md.scale, a.minus_zero);
+        wt.set(mt.top, mt.scale);
+        if (kModel) wd.set(md.top, md.scale);
         const int32_t *zt = a.target + trow * a.ld_target, *zd = both ? a.draft + drow * a.ld_draft : zt;
         const uint32_t x = rejected ? a.draft_tokens[drow] : kNoToken;
         // a CTA has a run of the vocabulary, a warp a run of that, in steps of 128
@@ -1005,7 +1004,6 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     a.tokens = tokens;
     a.accepted = accepted;
     a.probs = probs;
-    a.minus_zero = 0x8000000080000000ull;
     a.rows = static_cast<RowPart *>(workspace);
     a.total = drafts + requests + (a.draft ? drafts : 0);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
