@@ -97,7 +97,7 @@ struct Call {
     int NT, RT;           // rows per row tile (a multiple of 16), row tiles
     int slots, Q;         // pieces reserved per adapter
     int max_pieces;       // adapter pieces of one row tile at most
-    int span, ranks, ksplit; // k_prepare: rows and ranks per block of t, blocks of a cluster that share k
+    int span, ksplit;     // k_prepare: rows per block of t, blocks of a cluster that share k
     int down_words;       // 32-bit words of one down row
     const uint8_t *weight; // pieces [T][P]
     const int32_t *wsum;   // [T * 128] sums of the weights of an output
@@ -252,7 +252,7 @@ static __device__ void split_item(const Call &c, int item) {
     }
 }
 
-constexpr int kPrepareThreads = 256, kMaxSplit = 8;
+constexpr int kPrepareThreads = 256, kMaxSplit = 8, kSplitInputs = 2048;
 
 // Adds a value to the first block of the cluster's shared memory at p's place (the
 // blocks write different words).
@@ -264,72 +264,71 @@ static __device__ __forceinline__ void store_first(int64_t *p, int64_t v) {
 static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Sums over vectors [va, vb) of the products of two down rows (d, d + ld) with M rows,
-// over the lanes too: a lane ends with the sum of number idx (2 * row + down row), as
-// 16 / M lanes do.  U vectors of every row are in flight per lane; int32 partials join
-// the sum every 4096 inputs: |lo| <= 16 * 8 * 255 * 2^15 < 2^30.
-template <int M, int U>
-static __device__ __forceinline__ int64_t down_dots(const uint4 *d, int ld, const uint4 *const (&xr)[kGroup], int va, int vb,
-                                                    int lane, int &idx) {
+// d += 16 ranks x 8 rows over 32 inputs; each side's bytes signed or not.
+#define LLMX_MMA_BYTES(name, at, bt)                                                                                    \
+    static __device__ __forceinline__ void name(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {        \
+        asm("mma.sync.aligned.m16n8k32.row.col.s32." at "." bt ".s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "    \
+            "{%0, %1, %2, %3};"                                                                                         \
+            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                            \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));                                            \
+    }
+LLMX_MMA_BYTES(mma_ss, "s8", "s8")
+LLMX_MMA_BYTES(mma_su, "s8", "u8")
+LLMX_MMA_BYTES(mma_us, "u8", "s8")
+LLMX_MMA_BYTES(mma_uu, "u8", "u8")
+#undef LLMX_MMA_BYTES
+
+// Sums over steps [from, to) of 32 inputs of the products of 16 down rows (d, d + ld, ...)
+// with 8 rows: v[0..3] are those of down rows lane / 4 (v[0], v[1]) and lane / 4 + 8
+// with rows 2 (lane % 4) and the next.  d8: down row lane / 4 + 8, d0: lane / 4,
+// x: row lane / 4.  A lane takes 8 inputs of each, whatever places they have among
+// the 32: both sides of a product agree.  int32 holds every sum: 2^16 * 2 * 4128 inputs.
+static __device__ __forceinline__ void down_products(const uint4 *d0, const uint4 *d8, const uint4 *x, int from, int to,
+                                                     int vectors, int lane, int64_t (&v)[4]) {
+    constexpr int U = 4;  // steps in flight
     const uint4 none = make_uint4(0, 0, 0, 0);
-    int64_t mine = 0;
-    int v0 = va;
-    do {  // (once at least: idx is the reduction's)
-        int lo[2 * M], hi[2 * M];
-#pragma unroll
-        for (int g = 0; g < 2 * M; g++) lo[g] = hi[g] = 0;
+    int hh[4] = {}, mid[4] = {}, ll[4] = {};
 #pragma unroll 1
-        for (int k = 0; k < 16 && v0 + k * 32 < vb; k += U) {
-            uint4 w[2][U], x[M][U];
+    for (int s = from; s < to; s += U) {
+        uint4 w[U], w8[U], r[U];
 #pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int v = v0 + (k + u) * 32 + lane;
-                const bool in = v < vb;
-                w[0][u] = in ? __ldg(d + v) : none;
-                w[1][u] = in ? __ldg(d + ld + v) : none;
-#pragma unroll
-                for (int g = 0; g < M; g++) x[g][u] = in ? __ldg(xr[g] + v) : none;
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++)
-#pragma unroll
-                for (int g = 0; g < M; g++)
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const int i = 2 * g + r;
-                        lo[i] = dp2a_lo_su(x[g][u].x, w[r][u].x, lo[i]);
-                        hi[i] = dp2a_hi_ss(x[g][u].x, w[r][u].x, hi[i]);
-                        lo[i] = dp2a_lo_su(x[g][u].y, w[r][u].y, lo[i]);
-                        hi[i] = dp2a_hi_ss(x[g][u].y, w[r][u].y, hi[i]);
-                        lo[i] = dp2a_lo_su(x[g][u].z, w[r][u].z, lo[i]);
-                        hi[i] = dp2a_hi_ss(x[g][u].z, w[r][u].z, hi[i]);
-                        lo[i] = dp2a_lo_su(x[g][u].w, w[r][u].w, lo[i]);
-                        hi[i] = dp2a_hi_ss(x[g][u].w, w[r][u].w, hi[i]);
-                    }
+        for (int u = 0; u < U; u++) {
+            const int at = (s + u) * 4 + (lane & 3);
+            const bool in = s + u < to && at < vectors;
+            w[u] = in ? __ldg(d0 + at) : none;
+            w8[u] = in ? __ldg(d8 + at) : none;
+            r[u] = in ? __ldg(x + at) : none;
         }
-        int64_t sum[2 * M];
 #pragma unroll
-        for (int g = 0; g < 2 * M; g++) sum[g] = (int64_t)hi[g] * 256 + lo[g];
-        mine += warp_reduce_n<2 * M>(sum, lane, idx);
-        v0 += 32 * 16;
-    } while (v0 < vb);
-    return mine;
+        for (int u = 0; u < U; u++) {
+            const uint32_t low[4] = {__byte_perm(w[u].x, w[u].y, 0x5410), __byte_perm(w8[u].x, w8[u].y, 0x5410),
+                                     __byte_perm(w[u].z, w[u].w, 0x5410), __byte_perm(w8[u].z, w8[u].w, 0x5410)};
+            const uint32_t high[4] = {__byte_perm(w[u].x, w[u].y, 0x7632), __byte_perm(w8[u].x, w8[u].y, 0x7632),
+                                      __byte_perm(w[u].z, w[u].w, 0x7632), __byte_perm(w8[u].z, w8[u].w, 0x7632)};
+            const uint32_t xl0 = __byte_perm(r[u].x, r[u].y, 0x6420), xl1 = __byte_perm(r[u].z, r[u].w, 0x6420);
+            const uint32_t xh0 = __byte_perm(r[u].x, r[u].y, 0x7531), xh1 = __byte_perm(r[u].z, r[u].w, 0x7531);
+            mma_ss(hh, high, xh0, xh1);
+            mma_uu(ll, low, xl0, xl1);
+            mma_su(mid, high, xl0, xl1);
+            mma_us(mid, low, xh0, xh1);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = ((int64_t)hh[i] << 16) + ((int64_t)mid[i] << 8) + ll[i];
 }
 
-// t of rows [row0, row0 + span) for `ranks` (16 or 4) ranks of their adapters from 16
-// q + sub * ranks on, a pass per group of up to 8 rows of one adapter (the group that
-// starts at a row of the span).  A warp takes two ranks and a share of k: with 4
-// ranks a block has four shares, times the blocks of its cluster.  Every thread
-// of the cluster takes the same path: it depends on the row, q and the slots alone.
-static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int share) {
-    constexpr int kWarps = kPrepareThreads / 32, kShares = 4 * kMaxSplit;
-    __shared__ int64_t sum_s[kShares * kGroup * 16 / 4];  // [share][row][rank]: 16 ranks x 8 shares or 4 x 32
+// t of rows [row0, row0 + span) for ranks 16 q to 16 q + 15 of their adapters, a pass per
+// group of up to 8 rows of one adapter (the group that starts at a row of the span).
+// The warps of a block, times the blocks of its cluster, share k.  Every thread of
+// the cluster takes the same path: it depends on the row, q and the slots alone.
+static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
+    constexpr int kWarps = kPrepareThreads / 32, kSums = 16 * kGroup;
+    __shared__ __align__(16) int64_t sum_s[kWarps][kSums];  // [rank][row] of each warp
+    __shared__ int64_t part_s[kMaxSplit][kSums];            // of each block, in the cluster's first
     __shared__ int16_t t_s[kGroup][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int R = c.ranks, pairs = R >> 1, parts = kWarps / pairs;  // warps that share k
-    const int vectors = c.K >> 3, all = parts * c.ksplit, part = share * parts + warp / pairs;
-    const int va = (int)((int64_t)vectors * part / all), vb = (int)((int64_t)vectors * (part + 1) / all);
-    const int pair = warp % pairs, j0 = q * 16 + sub * R + pair * 2;
+    const int vectors = c.K >> 3, steps = (vectors + 3) >> 2, all = kWarps * c.ksplit, part = share * kWarps + warp;
+    const int from = steps * part / all, to = steps * (part + 1) / all;
     for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
         const int rt = row / c.NT, at = row - rt * c.NT;
         const int a = c.slot[row];
@@ -344,73 +343,72 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int sub, int 
         // members: the next 8 rows of the mask from this one on
         int member[kGroup], members = 0;
         {
-            int from = at;
+            int next = at;
 #pragma unroll
             for (int g = 0; g < kGroup; g++) {
                 member[g] = at;  // absent members repeat the first: never stored
-                int k = from >> 5;
-                uint32_t w = k < kRowTile / 32 ? mask.w[k] & (~0u << (from & 31)) : 0u;
+                int k = next >> 5;
+                uint32_t w = k < kRowTile / 32 ? mask.w[k] & (~0u << (next & 31)) : 0u;
                 while (w == 0 && ++k < kRowTile / 32) w = mask.w[k];
                 if (k < kRowTile / 32 && w) {
                     member[g] = k * 32 + __ffs((int)w) - 1;
                     members = g + 1;
-                    from = member[g] + 1;
+                    next = member[g] + 1;
                 } else {
-                    from = kRowTile;
+                    next = kRowTile;
                 }
             }
         }
-        const uint4 *xr[kGroup];
+        auto row_of = [&](int g) {  // member[] stays in registers
+            int r = member[0];
 #pragma unroll
-        for (int g = 0; g < kGroup; g++)
-            xr[g] = reinterpret_cast<const uint4 *>(c.x + ((size_t)rt * c.NT + member[g]) * c.ld_x);
-        const uint4 *d0 = reinterpret_cast<const uint4 *>(c.down + ((size_t)a * c.Q * 16 + j0) * c.down_words);
-        int idx, same;  // lanes that hold one sum
-        int64_t mine;
-        if (members == 1) mine = down_dots<1, 4>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 16;
-        else if (members <= 4) mine = down_dots<4, 2>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 4;
-        else mine = down_dots<8, 1>(d0, c.down_words / 4, xr, va, vb, lane, idx), same = 2;
-        const bool holds = lane % same == 0 && (idx >> 1) < members;
-        int64_t *place = sum_s + (part * kGroup + (idx >> 1)) * R + pair * 2 + (idx & 1);
+            for (int u = 1; u < kGroup; u++)
+                if (g == u) r = member[u];
+            return r;
+        };
+        const uint32_t *d = c.down + ((size_t)a * c.Q * 16 + q * 16 + (lane >> 2)) * c.down_words;
+        const int16_t *x = c.x + ((size_t)rt * c.NT + row_of(lane >> 2)) * c.ld_x;
+        int64_t v[4];
+        down_products(reinterpret_cast<const uint4 *>(d), reinterpret_cast<const uint4 *>(d + 8 * (size_t)c.down_words),
+                      reinterpret_cast<const uint4 *>(x), from, to, vectors, lane, v);
+        *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane]) = make_longlong2(v[0], v[1]);
+        *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane + 8 * kGroup]) = make_longlong2(v[2], v[3]);
+        __syncthreads();
+        int64_t sum = 0;
+        if (threadIdx.x < kSums)
+#pragma unroll
+            for (int w = 0; w < kWarps; w++) sum += sum_s[w][threadIdx.x];
         if (c.ksplit > 1) {
             cluster_wait();
-            if (holds) store_first(place, mine);
+            if (threadIdx.x < kSums) store_first(&part_s[share][threadIdx.x], sum);
             cluster_arrive();
             cluster_wait();
-        } else {
-            if (holds) *place = mine;
-            __syncthreads();
+            if (share != 0) continue;
+            sum = 0;
+            if (threadIdx.x < kSums)
+                for (int p = 0; p < c.ksplit; p++) sum += part_s[p][threadIdx.x];
         }
-        if (share == 0) {
-            if (threadIdx.x < kGroup * R) {
-                const int g = threadIdx.x / R, j = threadIdx.x % R;
-                int64_t v = 0;
-                for (int p = 0; p < all; p++) v += sum_s[p * kGroup * R + threadIdx.x];
-                t_s[g][j] = q * 16 + sub * R + j < rank ? (int16_t)sat16(rnd(v * scale, 24)) : (int16_t)0;
-            }
-            __syncthreads();
-            uint8_t *dst = c.tp + (((size_t)rt * c.NT + mask.first()) * c.Q + q) * c.NT * 32 + sub * R;
-            const int words = R / 4, g = threadIdx.x / words, w4 = threadIdx.x % words;  // 4 ranks per thread
-            if (g < members) {
-                int row_of = member[0];
-#pragma unroll
-                for (int u = 1; u < kGroup; u++)  // member[] stays in registers
-                    if (g == u) row_of = member[u];
-                const uint32_t *v = reinterpret_cast<const uint32_t *>(&t_s[g][4 * w4]);
-                uint8_t *p = dst + row_of * 16 + 4 * w4;
-                *reinterpret_cast<uint32_t *>(p) = __byte_perm(v[0], v[1], 0x7531);
-                *reinterpret_cast<uint32_t *>(p + c.NT * 16) = __byte_perm(v[0], v[1], 0x6420);
-            }
-            // zeros of the tile's other rows, by the adapter's first group
-            if (order == 0)
-                for (int u = threadIdx.x; u < c.NT * words; u += kPrepareThreads) {
-                    const int t = u / words, w = u % words;
-                    if ((mask.w[t >> 5] >> (t & 31)) & 1u) continue;
-                    *reinterpret_cast<uint32_t *>(dst + t * 16 + 4 * w) = 0;
-                    *reinterpret_cast<uint32_t *>(dst + c.NT * 16 + t * 16 + 4 * w) = 0;
-                }
+        if (threadIdx.x < kSums) {
+            const int j = threadIdx.x / kGroup, g = threadIdx.x % kGroup;
+            t_s[g][j] = q * 16 + j < rank ? (int16_t)sat16(rnd(sum * scale, 24)) : (int16_t)0;
         }
-        if (c.ksplit == 1) __syncthreads();  // the sums are read before the next group's
+        __syncthreads();
+        uint8_t *dst = c.tp + (((size_t)rt * c.NT + mask.first()) * c.Q + q) * c.NT * 32;
+        const int g = threadIdx.x / 4, w4 = threadIdx.x % 4;  // 4 ranks per thread
+        if (g < members) {
+            const uint32_t *t = reinterpret_cast<const uint32_t *>(&t_s[g][4 * w4]);
+            uint8_t *p = dst + row_of(g) * 16 + 4 * w4;
+            *reinterpret_cast<uint32_t *>(p) = __byte_perm(t[0], t[1], 0x7531);
+            *reinterpret_cast<uint32_t *>(p + c.NT * 16) = __byte_perm(t[0], t[1], 0x6420);
+        }
+        // zeros of the tile's other rows, by the adapter's first group
+        if (order == 0)
+            for (int u = threadIdx.x; u < c.NT * 4; u += kPrepareThreads) {
+                const int r = u / 4, w = u % 4;
+                if ((mask.w[r >> 5] >> (r & 31)) & 1u) continue;
+                *reinterpret_cast<uint32_t *>(dst + r * 16 + 4 * w) = 0;
+                *reinterpret_cast<uint32_t *>(dst + c.NT * 16 + r * 16 + 4 * w) = 0;
+            }
     }
 }
 
@@ -426,10 +424,9 @@ __global__ void __launch_bounds__(kPrepareThreads, 2) k_prepare(const Call c) {
     pdl_trigger();
     const int share = blockIdx.y;
     int b = blockIdx.x;
-    const int per_row = c.Q * (16 / c.ranks), forms = c.slot ? (int)((c.rows + c.span - 1) / c.span) * per_row : 0;
+    const int forms = c.slot ? (int)((c.rows + c.span - 1) / c.span) * c.Q : 0;
     if (b < forms) {
-        const int e = b % per_row;
-        form_t(c, (uint32_t)(b / per_row) * c.span, e / (16 / c.ranks), e % (16 / c.ranks), share);
+        form_t(c, (uint32_t)(b / c.Q) * c.span, b % c.Q, share);
         return;
     }
     b -= forms;
@@ -923,7 +920,7 @@ __global__ void __launch_bounds__(256) k_weight_sums(const int16_t *__restrict__
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane == 0) sums[row] = s;
 }
-// down [rank][K] -> words {lo(w0), lo(w1), hi(w0), hi(w1)} for the dp2a products
+// down [rank][K] -> words {lo(w0), lo(w1), hi(w0), hi(w1)}
 __global__ void k_pack_down(const uint32_t *__restrict__ src, uint32_t words, uint32_t *__restrict__ dst) {
     for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += gridDim.x * blockDim.x)
         dst[i] = __byte_perm(src[i], 0, 0x3120);
@@ -1225,12 +1222,11 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     // t: a block per row and 4 ranks while that is few blocks (most end at once: the
     // first row of 8 of an adapter does the work), else per 8 rows and 16 ranks; k is
     // cut so that a warp has about 512 inputs, over up to 8 blocks of a cluster
-    const bool few = c.slot && (int64_t)rows * c.Q * 4 <= 4 * h->sms;
+    const bool few = c.slot && (int64_t)rows * c.Q <= h->sms;
     c.span = few || rows <= kRowTile ? 1 : kGroup;
-    c.ranks = few ? 4 : 16;
-    const int forms = c.slot ? (int)((rows + c.span - 1) / c.span) * c.Q * (16 / c.ranks) : 0;
+    const int forms = c.slot ? (int)((rows + c.span - 1) / c.span) * c.Q : 0;
     c.ksplit = 1;
-    while (few && c.ksplit < kMaxSplit && c.K > 4 * 512 * c.ksplit) c.ksplit *= 2;
+    while (few && c.ksplit < kMaxSplit && c.K > kSplitInputs * c.ksplit) c.ksplit *= 2;
     const dim3 blocks((unsigned)(forms + (c.RT * (c.P / 8) + c.ksplit - 1) / c.ksplit + (c.slot ? c.RT : 0)), (unsigned)c.ksplit);
     cudaError_t e = launch((const void *)k_prepare, blocks, c.ksplit, kPrepareThreads, 0, c, s);
     if (e == cudaSuccess)
