@@ -98,11 +98,11 @@ struct Call {
     int slots, Q;         // pieces reserved per adapter
     int max_pieces;       // adapter pieces of one row tile at most
     int span, ksplit;     // k_prepare: rows per block of t, blocks of a cluster that share k
-    int down_words;       // 32-bit words of one down row
+    int steps;            // of 32 inputs
     const uint8_t *weight; // pieces [T][P]
     const int32_t *wsum;   // [T * 128] sums of the weights of an output
     const uint8_t *up;     // pieces [slots][T][Q]
-    const uint32_t *down;  // [slots][16 Q][K / 2] words {lo(w0), lo(w1), hi(w0), hi(w1)}
+    const uint4 *down;     // [slots][Q][steps][2][32] operands of t's products: see k_pack_down
     const int32_t *rank, *scale;
     uint8_t *xp;           // row pieces [RT][P]
     uint8_t *tp;           // t pieces [RT][NT first rows][Q]
@@ -278,13 +278,13 @@ LLMX_MMA_BYTES(mma_us, "u8", "s8")
 LLMX_MMA_BYTES(mma_uu, "u8", "u8")
 #undef LLMX_MMA_BYTES
 
-// Sums over steps [from, to) of 32 inputs of the products of 16 down rows (d, d + ld, ...)
-// with 8 rows: v[0..3] are those of down rows lane / 4 (v[0], v[1]) and lane / 4 + 8
-// with rows 2 (lane % 4) and the next.  d8: down row lane / 4 + 8, d0: lane / 4,
-// x: row lane / 4.  A lane takes 8 inputs of each, whatever places they have among
-// the 32: both sides of a product agree.  int32 holds every sum: 2^16 * 2 * 4128 inputs.
-static __device__ __forceinline__ void down_products(const uint4 *d0, const uint4 *d8, const uint4 *x, int from, int to,
-                                                     int vectors, int lane, int64_t (&v)[4]) {
+// Sums over steps [from, to) of 32 inputs of the products of 16 down rows with 8 rows:
+// v[0..3] are those of down rows lane / 4 (v[0], v[1]) and lane / 4 + 8 with rows
+// 2 (lane % 4) and the next.  x: row lane / 4.  A lane takes 8 inputs of each, whatever
+// places they have among the 32: both sides of a product agree.  int32 holds every
+// sum: 2 * 2^16 * 4128 inputs.
+static __device__ __forceinline__ void down_products(const uint4 *d, const uint4 *x, int from, int to, int vectors, int lane,
+                                                     int64_t (&v)[4]) {
     constexpr int U = 4;  // steps in flight
     const uint4 none = make_uint4(0, 0, 0, 0);
     int hh[4] = {}, mid[4] = {}, ll[4] = {};
@@ -294,17 +294,14 @@ static __device__ __forceinline__ void down_products(const uint4 *d0, const uint
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = (s + u) * 4 + (lane & 3);
-            const bool in = s + u < to && at < vectors;
-            w[u] = in ? __ldg(d0 + at) : none;
-            w8[u] = in ? __ldg(d8 + at) : none;
-            r[u] = in ? __ldg(x + at) : none;
+            const bool in = s + u < to;
+            w[u] = in ? __ldg(d + (s + u) * 64 + lane) : none;
+            w8[u] = in ? __ldg(d + (s + u) * 64 + 32 + lane) : none;
+            r[u] = in && at < vectors ? __ldg(x + at) : none;
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
-            const uint32_t low[4] = {__byte_perm(w[u].x, w[u].y, 0x5410), __byte_perm(w8[u].x, w8[u].y, 0x5410),
-                                     __byte_perm(w[u].z, w[u].w, 0x5410), __byte_perm(w8[u].z, w8[u].w, 0x5410)};
-            const uint32_t high[4] = {__byte_perm(w[u].x, w[u].y, 0x7632), __byte_perm(w8[u].x, w8[u].y, 0x7632),
-                                      __byte_perm(w[u].z, w[u].w, 0x7632), __byte_perm(w8[u].z, w8[u].w, 0x7632)};
+            const uint32_t low[4] = {w[u].x, w8[u].x, w[u].y, w8[u].y}, high[4] = {w[u].z, w8[u].z, w[u].w, w8[u].w};
             const uint32_t xl0 = __byte_perm(r[u].x, r[u].y, 0x6420), xl1 = __byte_perm(r[u].z, r[u].w, 0x6420);
             const uint32_t xh0 = __byte_perm(r[u].x, r[u].y, 0x7531), xh1 = __byte_perm(r[u].z, r[u].w, 0x7531);
             mma_ss(hh, high, xh0, xh1);
@@ -327,8 +324,8 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
     __shared__ int64_t part_s[kMaxSplit][kSums];            // of each block, in the cluster's first
     __shared__ int16_t t_s[kGroup][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int vectors = c.K >> 3, steps = (vectors + 3) >> 2, all = kWarps * c.ksplit, part = share * kWarps + warp;
-    const int from = steps * part / all, to = steps * (part + 1) / all;
+    const int vectors = c.K >> 3, all = kWarps * c.ksplit, part = share * kWarps + warp;
+    const int from = c.steps * part / all, to = c.steps * (part + 1) / all;
     for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
         const int rt = row / c.NT, at = row - rt * c.NT;
         const int a = c.slot[row];
@@ -366,11 +363,10 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
                 if (g == u) r = member[u];
             return r;
         };
-        const uint32_t *d = c.down + ((size_t)a * c.Q * 16 + q * 16 + (lane >> 2)) * c.down_words;
         const int16_t *x = c.x + ((size_t)rt * c.NT + row_of(lane >> 2)) * c.ld_x;
         int64_t v[4];
-        down_products(reinterpret_cast<const uint4 *>(d), reinterpret_cast<const uint4 *>(d + 8 * (size_t)c.down_words),
-                      reinterpret_cast<const uint4 *>(x), from, to, vectors, lane, v);
+        down_products(c.down + ((size_t)a * c.Q + q) * c.steps * 64, reinterpret_cast<const uint4 *>(x), from, to, vectors, lane,
+                      v);
         *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane]) = make_longlong2(v[0], v[1]);
         *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane + 8 * kGroup]) = make_longlong2(v[2], v[3]);
         __syncthreads();
@@ -920,10 +916,20 @@ __global__ void __launch_bounds__(256) k_weight_sums(const int16_t *__restrict__
     for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(~0u, s, o);
     if (lane == 0) sums[row] = s;
 }
-// down [rank][K] -> words {lo(w0), lo(w1), hi(w0), hi(w1)}
-__global__ void k_pack_down(const uint32_t *__restrict__ src, uint32_t words, uint32_t *__restrict__ dst) {
-    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < words; i += gridDim.x * blockDim.x)
-        dst[i] = __byte_perm(src[i], 0, 0x3120);
+// down [rank][K] -> [rank / 16][step of 32 inputs][half][lane]: the operands of t's products
+// as their lanes take them, 8 inputs of a rank's row as {low bytes, high bytes}, so that
+// a warp reads 512 bytes in a row; zeros past the last rank and input
+__global__ void k_pack_down(const int16_t *__restrict__ src, uint32_t rank, uint32_t cols, uint32_t steps,
+                            uint4 *__restrict__ dst) {
+    const uint32_t n = (rank + 15) / 16 * steps * 64;
+    for (uint32_t i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
+        const uint32_t lane = i & 31, step = i / 64 % steps, row = i / 64 / steps * 16 + (i >> 5 & 1) * 8 + lane / 4;
+        const uint32_t col = (step * 4 + lane % 4) * 8;
+        const uint4 v = row < rank && col < cols ? *reinterpret_cast<const uint4 *>(src + (size_t)row * cols + col)
+                                                 : make_uint4(0, 0, 0, 0);
+        dst[i] = make_uint4(__byte_perm(v.x, v.y, 0x6420), __byte_perm(v.z, v.w, 0x6420), __byte_perm(v.x, v.y, 0x7531),
+                            __byte_perm(v.z, v.w, 0x7531));
+    }
 }
 __global__ void k_set_slot(int32_t *ranks, int32_t *scales, uint32_t slot, int32_t rank, int32_t scale) {
     ranks[slot] = rank;
@@ -953,7 +959,7 @@ struct llmx_adapters {
     uint8_t *memory = nullptr;   // the one allocation
     uint8_t *weight = nullptr;   // pieces [T][P]
     int32_t *wsum = nullptr;     // [T * 128]
-    uint32_t *down = nullptr;    // [slots][16 Q][in_dim / 2]
+    uint4 *down = nullptr;    // [slots][Q][steps of 32 inputs][2][32]
     uint8_t *up = nullptr;       // pieces [slots][T][Q]
     int32_t *rank = nullptr, *scale = nullptr;  // [slots]
     uint8_t *xp = nullptr, *tp = nullptr, *zero = nullptr;  // row and t pieces of a call, a piece of zeros
@@ -1073,7 +1079,7 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
     const size_t rank_at = place((size_t)slots * 4), zero_at = place((size_t)h->row_cap * 32), acc_at = place(h->acc_bytes()),
                  arrived_at = place((size_t)h->sms * 4), error_at = place(4),
                  // ranks of a slot that no adapter fills are multiplied by nothing, but read
-                 down_at = place((size_t)slots * h->Q * 16 * in_dim * 2), zeros = at, scale_at = place((size_t)slots * 4),
+                 down_at = place((size_t)slots * h->Q * ((in_dim + 31) / 32) * 64 * sizeof(uint4)), zeros = at, scale_at = place((size_t)slots * 4),
                  wsum_at = place((size_t)h->T * kOutTile * 4), xp_at = place(xt * h->P * 32),
                  tp_at = place(xt * h->Q * h->row_cap * 32), list_at = place(rt * pieces * 8), count_at = place(rt * 4),
                  up_at = place((size_t)slots * h->T * h->Q * kPiece), weight_at = place((size_t)h->T * h->P * kPiece);
@@ -1129,9 +1135,8 @@ extern "C" int llmx_adapters_set(llmx_adapters *h, uint32_t slot, uint32_t rank,
     if (scope.err != cudaSuccess) return cuda_fail("cudaSetDevice", scope.err);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (rank) {
-        const uint32_t words = rank * h->in_dim / 2, used = (rank + 15) / 16;
-        k_pack_down<<<256, 256, 0, s>>>(reinterpret_cast<const uint32_t *>(down), words,
-                                        h->down + (size_t)slot * h->Q * 16 * (h->in_dim / 2));
+        const uint32_t used = (rank + 15) / 16, steps = (h->in_dim + 31) / 32;
+        k_pack_down<<<256, 256, 0, s>>>(down, rank, h->in_dim, steps, h->down + (size_t)slot * h->Q * steps * 64);
         k_pack_pieces<false><<<h->sms * 4, 256, 0, s>>>(up, h->out_dim, rank, used, h->Q, h->T,
                                                         h->up + (size_t)slot * h->T * h->Q * kPiece);
     }
@@ -1187,7 +1192,7 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     c.slots = (int)h->slots;
     c.Q = h->Q;
     c.max_pieces = (int)h->max_pieces(c.NT);
-    c.down_words = (int)(h->in_dim / 2);
+    c.steps = (int)((h->in_dim + 31) / 32);
     c.weight = h->weight;
     c.wsum = h->wsum;
     c.up = h->up;
