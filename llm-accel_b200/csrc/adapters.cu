@@ -61,6 +61,7 @@
 #include "llmx.h"
 #include "device_util.cuh"
 #include "fixed.cuh"
+#include "cluster.cuh"
 #include "gemv_common.cuh"
 #include "kernels.cuh"
 #include "tcgen05.cuh"
@@ -254,16 +255,6 @@ static __device__ void split_item(const Call &c, int item) {
 
 constexpr int kPrepareThreads = 256, kMaxSplit = 8, kSplitInputs = 2048;
 
-// Adds a value to the first block of the cluster's shared memory at p's place (the
-// blocks write different words).
-static __device__ __forceinline__ void store_first(int64_t *p, int64_t v) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(p)));
-    asm volatile("st.shared::cluster.s64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
-}
-static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-
 // d += 16 ranks x 8 rows over 32 inputs; each side's bytes signed or not.
 #define LLMX_MMA_BYTES(name, at, bt)                                                                                    \
     static __device__ __forceinline__ void name(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {        \
@@ -322,6 +313,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
     constexpr int kWarps = kPrepareThreads / 32, kSums = 16 * kGroup;
     __shared__ __align__(16) int64_t sum_s[kWarps][kSums];  // [rank][row] of each warp
     __shared__ int64_t part_s[kMaxSplit][kSums];            // of each block, in the cluster's first
+    __shared__ uint64_t part_bar;
     __shared__ int16_t t_s[kGroup][16];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vectors = c.K >> 3, all = kWarps * c.ksplit, part = share * kWarps + warp;
@@ -336,7 +328,14 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
         if (order % kGroup != 0) continue;
         // (the first piece does not wait for the rank: an empty slot's t is formed and never read)
         if (q > 0 && q * 16 >= rank) continue;
-        if (c.ksplit > 1) cluster_arrive();  // the sums' memory is free here
+        if (c.ksplit > 1) {  // (a block then has one row, so one group at most)
+            if (threadIdx.x == 0) {
+                mbar_init(&part_bar, 1);
+                asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+                mbar_expect_tx(&part_bar, c.ksplit * kSums * 8);
+            }
+            cluster_arrive();
+        }
         // members: the next 8 rows of the mask from this one on
         int member[kGroup], members = 0;
         {
@@ -376,10 +375,10 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
             for (int w = 0; w < kWarps; w++) sum += sum_s[w][threadIdx.x];
         if (c.ksplit > 1) {
             cluster_wait();
-            if (threadIdx.x < kSums) store_first(&part_s[share][threadIdx.x], sum);
-            cluster_arrive();
-            cluster_wait();
+            if (threadIdx.x < kSums)
+                st_async(remote(&part_s[share][threadIdx.x], 0), (uint64_t)sum, remote(&part_bar, 0));
             if (share != 0) continue;
+            if (!mbar_wait_cluster(&part_bar, 0)) atomicExch(c.error, 3);
             sum = 0;
             if (threadIdx.x < kSums)
                 for (int p = 0; p < c.ksplit; p++) sum += part_s[p][threadIdx.x];

@@ -37,6 +37,7 @@
 
 #include "llmx.h"
 #include "device_util.cuh"
+#include "cluster.cuh"
 #include "gemv_common.cuh"
 #include "kernels.cuh"
 
@@ -44,13 +45,19 @@ namespace {
 
 using llmx::bulk_g2s;
 using llmx::bulk_g2s_hint;
+using llmx::cluster_arrive;
+using llmx::cluster_rank;
+using llmx::cluster_wait;
 using llmx::mbar_arrive;
 using llmx::mbar_expect_tx;
 using llmx::mbar_init;
 using llmx::mbar_wait;
+using llmx::mbar_wait_cluster;
 using llmx::pdl_trigger;
 using llmx::pdl_wait;
+using llmx::remote;
 using llmx::smem_u32;
+using llmx::st_async;
 
 constexpr int kExcluded = INT_MIN;
 constexpr uint32_t kNoToken = 0xffffffffu;
@@ -248,33 +255,6 @@ static __device__ __forceinline__ uint64_t row_share_small(uint32_t w, const Row
 // floor(a * u / 2^32)
 static __device__ __forceinline__ uint64_t mul_frac(uint64_t a, uint32_t u) { return __umul64hi(a, (uint64_t)u << 32); }
 
-// ---- clusters -------------------------------------------------------------------
-static __device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
-static __device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) {
-    uint32_t a;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-    return a;
-}
-static __device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
-    for (uint32_t i = 0; i < llmx::kSpinLimit; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-            : "=r"(ok)
-            : "r"(smem_u32(bar)), "r"(parity)
-            : "memory");
-        if (ok) return true;
-    }
-    return false;
-}
-
 // ---------------------------------------------------------------------------
 // rows -> maxima and sums
 // ---------------------------------------------------------------------------
@@ -388,13 +368,17 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             top_count[i] = part_count[i] = 0;
         }
         for (int i = 0; i < kTops; i++) {
-            mbar_init(top_full + i, S);
+            mbar_init(top_full + i, 1);
             mbar_init(top_done + i, S);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (S > 1) cluster_sync();
-    else __syncthreads();
+    if (S > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
     pdl_wait();
     // with many rows the draw's CTAs would only take room from the last of this kernel's
     if (!kTwice) pdl_trigger();
@@ -512,9 +496,16 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         if (lane == 0) warp_top[i & 1][w] = top;
         if (last_of(&top_count[i & 1], kMaxWarps)) {
             top = __reduce_max_sync(~0u, lane < kMaxWarps ? warp_top[i & 1][lane] : kExcluded);
-            if (lane < S)
-                asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(remote(&tops[i % kTops][rank], lane)), "r"(top) : "memory");
-            arrive_all(top_full + i % kTops);
+            // (without a cluster there is no asynchronous store, not even to the CTA itself)
+            if (S == 1) {
+                if (lane == 0) {
+                    tops[i % kTops][0] = top;
+                    mbar_arrive(top_full + i % kTops);
+                }
+            } else if (lane == 0) {
+                mbar_expect_tx(top_full + i % kTops, S * 4);
+            }
+            if (S > 1 && lane < S) st_async(remote(&tops[i % kTops][rank], lane), top, remote(top_full + i % kTops, lane));
         }
         top = kExcluded;
         __syncwarp();
@@ -667,11 +658,20 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     __shared__ RowMass mass_s[kKeep][2], last_s[2];
     __shared__ unsigned long long warp_sum[kDrawWarps], cta_sum[2][kMaxCluster];
     __shared__ unsigned long long run_sum[kDrawWarps][kRuns];  // of up to kRuns runs of a warp's steps
+    __shared__ uint64_t sums_full[2];                          // every CTA's sum of the round is there
     const int S = d.split, rank = S > 1 ? (int)cluster_rank() : 0;
     const uint32_t b = blockIdx.x / S;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
-    if (S > 1) cluster_sync();  // every CTA of the cluster runs before one stores into another
+    if (S > 1) {
+        if (threadIdx.x == 0) {
+            for (int i = 0; i < 2; i++) mbar_init(sums_full + i, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            for (int i = 0; i < 2; i++) mbar_expect_tx(sums_full + i, S * 8);
+        }
+        __syncwarp();
+        cluster_arrive();  // waited for before the first sums are sent
+    }
     pdl_wait();
     pdl_trigger();
     uint32_t begin, count;
@@ -723,7 +723,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const RowMass mt = n < kKeep ? mass_s[n][0] : last_s[0], md = n < kKeep ? mass_s[n][1] : last_s[1];
     // one path for the whole cluster from here: all of it depends on the request alone
     uint32_t drawn = kNoToken;
-    const bool bad = bad_s != 0;
+    bool bad = bad_s != 0;
+    if (S > 1) cluster_wait();
     if (!bad) {
         RowWeight wt, wd;
         wt.set(mt.top, mt.scale);
@@ -817,6 +818,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 }
             }
             for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
+            if (round > 0) __syncthreads();  // the last round's sums have been read
             if (lane == 0) warp_sum[warp] = mine;
             __syncthreads();
             unsigned long long cta = 0;
@@ -827,17 +829,18 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
             }
             if (S > 1) {
                 if ((int)threadIdx.x < S)
-                    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(remote(&cta_sum[round][rank], threadIdx.x)), "l"(cta)
-                                 : "memory");
-                cluster_sync();
+                    st_async(remote(&cta_sum[round][rank], threadIdx.x), (uint64_t)cta, remote(&sums_full[round], threadIdx.x));
                 total = 0;
+                if (!mbar_wait_cluster(&sums_full[round], 0)) {
+                    bad = true;
+                    break;
+                }
                 for (int q = 0; q < S; q++) {
                     if (q < rank) below += cta_sum[round][q];
                     total += cta_sum[round][q];
                 }
             } else {
                 total = cta;
-                __syncthreads();  // the warps' sums are read before the next round's
             }
             if (total != 0 || !rest) break;
         }
