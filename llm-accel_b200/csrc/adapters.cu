@@ -318,7 +318,9 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vectors = c.K >> 3, all = kWarps * c.ksplit, part = share * kWarps + warp;
     const int from = c.steps * part / all, to = c.steps * (part + 1) / all;
+    uint32_t taken = 0;  // rows of the span that are members of a group of it (a group's first row aside)
     for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
+        if ((taken >> (row - row0)) & 1u) continue;
         const int rt = row / c.NT, at = row - rt * c.NT;
         const int a = c.slot[row];
         if (a < 0 || a >= c.slots) continue;
@@ -350,6 +352,8 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
                     member[g] = k * 32 + __ffs((int)w) - 1;
                     members = g + 1;
                     next = member[g] + 1;
+                    const uint32_t of_span = row + member[g] - at - row0;
+                    if (of_span < 32) taken |= 1u << of_span;
                 } else {
                     next = kRowTile;
                 }
