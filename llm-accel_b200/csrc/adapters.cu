@@ -82,6 +82,12 @@ __host__ __device__ constexpr int project_threads(int depth) { return 64 + resul
 constexpr int kHeader = 16 * 16 + 32 + 16 + 64 + 16;  // barriers and flags at the start of shared memory, then the row-tile tables
 constexpr int kMaxRing = 16;
 constexpr int kMoreTiles = 3;          // row tiles beyond the fewest that a call may take
+// Measured, in us: a stage of 128 inputs at least and per row of its tile, adding a cut tile
+// up and per row, and the later start that it has where there are several row tiles,
+// the results per row.  77 rows x 1096 -> 4999: cut in three 23, whole 15.6, whole in
+// three row tiles 13.1; 40 rows x 2048 -> 2560: cut in seven 13.6, whole in three row
+// tiles 14.9; 100 rows x 2048 -> 2560: whole 20.1, in four row tiles 15.7.
+constexpr double kStageUs = 0.5, kStageRowUs = 0.0056, kAddUs = 2.0, kAddRowUs = 0.085, kLateUs = 1.5, kResultRowUs = 0.03;
 constexpr int kGroup = 8;              // rows of one adapter that share a pass over its down matrix
 
 // What the kernels need of a handle and a call.
@@ -550,17 +556,17 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // Stages of each row tile.  With one row tile its adapters are counted here,
-    // from the slots themselves (k_prepare passed its wait before this kernel
-    // could start, so they are final), and the weights can be fetched before
+    // Stages of each row tile.  Where the CTA meets one row tile only, its adapters are
+    // counted here, from the slots themselves (k_prepare passed its wait before this
+    // kernel could start, so they are final), and the weights can be fetched before
     // k_prepare ends; with more, k_prepare's counts are waited for.
-    if (c.slot && c.RT == 1) {
+    if (c.slot && (c.RT == 1 || (c.shared_tiles == 0 && c.T * c.RT <= (int)gridDim.x))) {
         TileSlots &ts = *reinterpret_cast<TileSlots *>(ring);
-        const RowSlot r = tile_slots(c, 0, ts);
+        const int own = blockIdx.x % c.RT;
+        const RowSlot r = tile_slots(c, own, ts);
         if (threadIdx.x == 0) {
-            pieces[0] = r.total;
-            pre[0] = 0;
-            pre[1] = C + (r.total + D - 1) / D;
+            pieces[own] = r.total;
+            for (int rt = 0; rt <= c.RT; rt++) pre[rt] = rt <= own ? 0 : C + (r.total + D - 1) / D;
         }
         // the ring takes this memory over for bulk copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1058,9 +1064,6 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
     h->Q = (int)((h->max_rank + 15) / 16);
     h->row_cap = max_rows > kRowTile ? kRowTile : rows_per_tile(max_rows, 1);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const size_t rt = (size_t)row_tiles(max_rows) + (max_rows > kRowTile ? kMoreTiles : 0);
-    const size_t xt = rt == 1 ? (size_t)h->row_cap : max_rows + 16 * rt;  // rows of all row tiles
-    const size_t pieces = h->max_pieces(h->row_cap);
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&h->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
         (e = cudaFuncSetAttribute(k_project<8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kProjectSmem)) != cudaSuccess ||
@@ -1072,6 +1075,9 @@ extern "C" int llmx_adapters_create(int device, uint32_t in_dim, uint32_t out_di
         release(h);
         return cuda_fail("create", e);
     }
+    const size_t rt = (size_t)row_tiles(max_rows) + (max_rows > kRowTile || 2 * (int64_t)h->T <= h->sms ? kMoreTiles : 0);
+    const size_t xt = rt == 1 ? (size_t)h->row_cap : max_rows + 16 * rt;  // rows of all row tiles
+    const size_t pieces = h->max_pieces(h->row_cap);
     // one allocation; what has to start as zeros lies at its front
     size_t at = 0;
     auto place = [&](size_t n) {
@@ -1192,6 +1198,24 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
             c.shared_tiles = shared;
         }
     }
+    // Fewer tiles than CTAs: a tile's stages of 128 inputs, one after another or shared
+    // out and then added up, and its results.  More row tiles make both shorter.
+    auto tile_us = [&](int rt, int nt, bool cut) {
+        const double depth = std::max(kStageUs, kStageRowUs * nt) * (h->P / 8);
+        const double adding = kAddUs + kAddRowUs * std::min<int>((int)rows, nt) + (rt > 1 ? kLateUs : 0);
+        return (cut ? depth * ((double)h->T * rt / h->sms) + adding : depth) + kResultRowUs * nt;
+    };
+    const int fewest = row_tiles(rows);
+    for (int rt = fewest; rt <= fewest + kMoreTiles && (int64_t)h->T * rt <= h->sms; rt++) {
+        const int nt = rows_per_tile(rows, rt);
+        const bool cut = tile_us(rt, nt, true) < tile_us(rt, nt, false);
+        const double us = tile_us(rt, nt, cut);
+        if (rt > fewest && ((uint32_t)((rt - 1) * nt) >= rows || us >= best)) continue;
+        best = us;
+        c.RT = rt;
+        c.NT = nt;
+        c.shared_tiles = cut ? h->T * rt : 0;
+    }
     c.slots = (int)h->slots;
     c.Q = h->Q;
     c.max_pieces = (int)h->max_pieces(c.NT);
@@ -1218,18 +1242,13 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     const int grid = (int)std::min<int64_t>(h->sms, (int64_t)c.T * c.RT * c.C);
     // A shared tile is cut into equal parts where that leaves at most a quarter of the CTAs
     // without one (every part then belongs to one tile only), else the line of all
-    // their stages is cut evenly.  Fewer tiles than CTAs stay whole where their stages
-    // (measured 0.45 us for 128 inputs) take no longer than a part's and adding the
-    // parts up (2 us and 0.085 a row: 77 rows x 1096 -> 4999 23 us cut in three).
+    // their stages is cut evenly.
     const int parts = c.shared_tiles ? grid / c.shared_tiles : 0;
     c.sharers = 4 * parts * c.shared_tiles >= 3 * grid ? parts * c.shared_tiles : grid;
-    if ((int64_t)c.T * c.RT < grid) {
-        const double depth = 0.45 * c.P / 8, share = depth * c.shared_tiles / c.sharers;
-        if (depth <= share + 2.0 + 0.085 * std::min<uint32_t>(rows, (uint32_t)c.NT)) c.shared_tiles = 0;
-    }
-    // t: a block per row and 4 ranks while that is few blocks (most end at once: the
-    // first row of 8 of an adapter does the work), else per 8 rows and 16 ranks; k is
-    // cut so that a warp has about 512 inputs, over up to 8 blocks of a cluster
+    // t: a block per row and 16 ranks while that is few blocks or few rows (most end at once:
+    // the first row of 8 of an adapter does the work), else per 8 rows.  Few blocks cut k
+    // beyond their warps, over up to 8 of a cluster, in runs of more than 2048 inputs: the
+    // exchange costs 1 to 2 us (16 rows x 2048 cut in two 26.2 -> 28.6).
     const bool few = c.slot && (int64_t)rows * c.Q <= h->sms;
     c.span = few || rows <= kRowTile ? 1 : kGroup;
     const int forms = c.slot ? (int)((rows + c.span - 1) / c.span) * c.Q : 0;

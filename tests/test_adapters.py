@@ -148,6 +148,19 @@ def test_tiles_beyond_the_processors(llmx, torch, rows, more):
 
 
 @gpu
+@pytest.mark.parametrize("n", [100, 4999, 9000, 18900])
+@pytest.mark.parametrize("k", [64, 1096, 11008])
+def test_fewer_tiles_than_processors(llmx, torch, n, k):
+    """Rows over one or several row tiles, tiles whole or cut, of one handle in turn; row
+    tiles whose rows have no adapter, the last one's rows fewer."""
+    c = Case(llmx, torch, k, n, [9, 20, 33, 16], 150, seed=n)
+    for rows in (128, 1, 17, 33, 150, 77, 49, 97, 113):
+        x = whole(c.rng, (rows, k), 700)
+        c.check(x, c.rng.integers(-1, 4, rows), wide=True)
+        c.check(x, np.where(np.arange(rows) < rows // 2, -1, 2), wide=False)
+
+
+@gpu
 @pytest.mark.parametrize("k", [128, 32768])
 @pytest.mark.parametrize("rows", [3, 40, 130])
 def test_extremes(llmx, torch, k, rows):
