@@ -40,15 +40,18 @@
 // stages fills while the rows are still being split.  Row tiles of the same outputs
 // are neighbours, so a weight stage comes from HBM once.
 //
-// What bounds it (B200, in a graph of calls; bytes at 6.47 TB/s, exact products at
-// a quarter of the int8 rate, which a loop of such MMAs measured as 4.5 P/s).  Up to
-// about 64 rows the weight stream: LM head 151936 x 2048, 40 rows of 8 adapters, 105 us =
-// 0.97 of the floor of 102; Gate/Up 22016 x 2048, 16 rows of 16 adapters, 27.5 us
-// against 16.9, of which 7 pass before k_prepare's t is there and the tail takes 2.
-// 512 rows x 11008 x 2048 with rank 64: 69 us against 20.8 of products; per tile of 112
-// rows the stages take 10.8 us (shared memory: 44 KB read by the MMAs and 30 KB
-// written per 64 inputs, at 128 bytes a cycle) and the results 2, three tiles each,
-// after 16 us of k_prepare.  One row x 2560 x 2048: 9.9 us, the two kernels' latencies.
+// What bounds it (B200, in graphs of calls over three sets of weights, which thus come
+// from HBM; bytes at 6.47 TB/s, exact products at a quarter of the int8 rate, which a
+// loop of such MMAs measured as 4.5 P/s).  Up to about 64 rows the weight stream: LM
+// head 151936 x 2048, 40 rows of 8 adapters, 110 us = 0.93 of the floor of 102 (adapters
+// of rank 8 are stored as pieces of 16: 20 MB more); Gate/Up 22016 x 2048, 16 rows of
+// 16 adapters, 26.2 us against 16.9, of which 5 pass before k_prepare's t is there and
+// the tail takes 2; 8 rows x 11008 -> 2048 15.4 against 7.1: 5 until t, 5 of stages,
+// 2.5 of adding parts up.  512 rows x 11008 x 2048 with rank 64: 57 us against 20.8 of
+// products: k_prepare 6, its end to the first product 5, then two whole tiles of 128
+// rows and a part of one: stages 0.72 us per 128 inputs (shared memory: 48 KB read by
+// the MMAs and 32 KB written per 64 inputs, at 128 bytes a cycle) and the results 3.5 a
+// tile.  One row x 2560 x 2048: 9.3 us, the two kernels' latencies.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -418,11 +421,12 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
 }
 
 // Blocks (x, share): per x first t, then the rows' pieces and the lists of the row tiles'
-// adapters.  Bound by latency: slots, then ranks, then products, 1.2 us each at one
-// row (4 KiB of a row, 64 KiB of a rank-16 down matrix), and by the dp2a pipe with
-// hundreds of rows (512 rows of rank 64: 9 us of products).  Blocks of 4 ranks with
-// k cut over their warps (and over a cluster's blocks) halved the first: 8 rows
-// x 11008 25 -> 9 us against blocks of 16 ranks over all of k.
+// adapters.  Bound by latency: slots 0.7 us, then ranks and the rows of the adapter,
+// then products 2 us (one row: 4 KiB of a row, 64 KiB of a rank-16 down matrix) and their
+// sums 0.4, or 0.75 across a cluster.  t on the legacy matrix instructions, whose 16 x 8
+// tile is 16 ranks of 8 rows, took 512 rows of rank 64 from 65 to 59.5 us against
+// dp2a products, whose pipe took 9 us of that; tcgen05 would need the operands in shared
+// memory and 128 ranks or rows a tile.
 __global__ void __launch_bounds__(kPrepareThreads, 2) k_prepare(const Call c) {
     __shared__ TileSlots ts;
     pdl_wait();     // the caller's rows, and the last call's reads of the workspace

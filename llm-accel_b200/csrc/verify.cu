@@ -18,13 +18,13 @@
 // the other's loads.  k_draw tests the drafts of a request and draws its last
 // token, a cluster per request.
 //
-// What bounds it (B200, vocabulary of 151936, in a graph of calls).  64 requests x 7
-// drafts with draft rows, 960 rows, 583 MB: 163 us against 90 for the bytes; k_mass
-// 121 (5 TB/s; half of the second loads miss the L2, 0.86 GB are read; without its
-// arithmetic 107), k_draw 42 (78 MB and 30 to 50 instructions a logit pair: the ALU and
-// the packed-float pipes at a third each, 0.6 instructions a cycle).  One request with 4
-// copied drafts: 15 us, latency: 7.5 in k_mass (loads 1.1, exchange 1, sums 1.3,
-// launch), 7.5 in k_draw (accept tests 1.5, sums 3.9, cluster totals 1.9, the token 1.4).
+// What bounds it (B200, vocabulary of 151936, in graphs of calls over three sets of
+// inputs).  64 requests x 7 drafts with draft rows, 960 rows, 583 MB: 158 us against 90
+// for the bytes; k_mass 118 (0.64 GB read: second loads leave the L2 first; 19
+// instructions a logit of both passes, 0.69 a cycle and scheduler), k_draw 39 (78 MB,
+// 0.61 instructions a cycle).  One request with 4 copied drafts: 12.1 us, latency, about
+// half in each kernel: loads 1.1, exchange 0.6, sums 1.3; accept tests 1.5, sums 3.9,
+// cluster totals 1.3, the token 1.4.
 // Simple kernels, a block per row and per request, took 862 and 194 us.
 #include <cuda_runtime.h>
 
@@ -208,6 +208,12 @@ struct RowMass {
     int ok;
 };
 // From the parts of a row, by half a warp: its lanes hold a part each.
+// Sum over the warp, below 2^59: two 32-bit reductions take less than five rounds of
+// 64-bit shuffles.
+static __device__ __forceinline__ unsigned long long sum_lanes(unsigned long long v) {
+    const uint32_t lo = __reduce_add_sync(~0u, (uint32_t)v & 0x7ffffffu), hi = __reduce_add_sync(~0u, (uint32_t)(v >> 27));
+    return ((unsigned long long)hi << 27) + lo;
+}
 static __device__ RowMass load_row(const RowPart *rows, uint32_t row, int split) {
     const int i = threadIdx.x & (kMaxCluster - 1);
     const RowPart *p = rows + row;
@@ -589,8 +595,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             // sums (greedy: the smallest first position) of the warp, then of the CTA
             auto whole = [&](unsigned long long v) {
                 if (rw.greedy) return (unsigned long long)__reduce_min_sync(~0u, (uint32_t)v);
-                for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-                return v;
+                return sum_lanes(v);
             };
             sum = whole(rw.greedy ? first : sum);
             if (lane == 0) warp_part[i & 1][warp] = sum;
@@ -799,6 +804,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
             Four next;
             if (v0 < v1) fetch(v0, rest, next);
             uint32_t next_run = v0 + run, at_run = 0;
+            unsigned long long lanes = 0;
             for (uint32_t v = v0; v < v1; v += 128) {  // the next step's logits under way while this one's are summed
                 const Four z = next;
                 if (v + 128 < v1) fetch(v + 128, rest, next);
@@ -807,26 +813,20 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 if (!wt.fast || !__all_sync(~0u, wt.base - (uint32_t)most >= wt.most)) {
                     uint64_t m[4];
                     four(v, rest, z, m);
-                    mine += (m[0] + m[1]) + (m[2] + m[3]);
+                    lanes += (m[0] + m[1]) + (m[2] + m[3]);
                 }
                 if (v + 128 >= v1 || v + 128 == next_run) {
-                    unsigned long long t = mine;
-                    for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(~0u, t, o);
-                    if (lane == 0) run_sum[warp][at_run] = t;  // of all runs so far
+                    mine = sum_lanes(lanes);
+                    if (lane == 0) run_sum[warp][at_run] = mine;  // of all runs so far
                     at_run++;
                     next_run += run;
                 }
             }
-            for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
             if (round > 0) __syncthreads();  // the last round's sums have been read
             if (lane == 0) warp_sum[warp] = mine;
             __syncthreads();
-            unsigned long long cta = 0;
-            below = 0;
-            for (int q = 0; q < kDrawWarps; q++) {
-                if (q < warp) below += warp_sum[q];
-                cta += warp_sum[q];
-            }
+            const unsigned long long of_warp = lane < kDrawWarps ? warp_sum[lane] : 0, cta = sum_lanes(of_warp);
+            below = sum_lanes(lane < warp ? of_warp : 0);
             if (S > 1) {
                 if ((int)threadIdx.x < S)
                     st_async(remote(&cta_sum[round][rank], threadIdx.x), (uint64_t)cta, remote(&sums_full[round], threadIdx.x));
@@ -835,10 +835,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                     bad = true;
                     break;
                 }
-                for (int q = 0; q < S; q++) {
-                    if (q < rank) below += cta_sum[round][q];
-                    total += cta_sum[round][q];
-                }
+                const unsigned long long of_cta = lane < S ? cta_sum[round][lane] : 0;
+                total = sum_lanes(of_cta);
+                below += sum_lanes(lane < rank ? of_cta : 0);
             } else {
                 total = cta;
             }
@@ -857,17 +856,23 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 uint64_t m[4];
                 fetch(v, rest, z);
                 four(v, rest, z, m);
-                for (int u = 0; u < 4; u++) {
-                    unsigned long long sum = m[u];
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const unsigned long long t = __shfl_up_sync(~0u, sum, o);
-                        if (lane >= o) sum += t;
+                unsigned long long sum[4], hit = 0;
+                int at = -1;
+#pragma unroll
+                for (int u = 0; u < 4; u++) sum[u] = sum_lanes(m[u]);
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (at < 0) {
+                        if (below + sum[u] > point) at = u, hit = m[u];
+                        else below += sum[u];
                     }
-                    const unsigned hit = __ballot_sync(~0u, below + sum > point);
-                    if (hit && drawn == kNoToken) drawn = v + 32 * u + (uint32_t)__ffs((int)hit) - 1;
-                    below += __shfl_sync(~0u, sum, 31);
+                if (at < 0) continue;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned long long t = __shfl_up_sync(~0u, hit, o);
+                    if (lane >= o) hit += t;
                 }
-                if (drawn != kNoToken) break;
+                drawn = v + 32 * at + (uint32_t)__ffs((int)__ballot_sync(~0u, below + hit > point)) - 1;
+                break;
             }
             if (lane == 0) out[n] = drawn;
         } else if (total == 0 && rank == 0 && threadIdx.x == 0) {
