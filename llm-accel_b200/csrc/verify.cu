@@ -19,12 +19,11 @@
 // token, a cluster per request.
 //
 // What bounds it (B200, vocabulary of 151936, in graphs of calls over three sets of
-// inputs).  64 requests x 7 drafts with draft rows, 960 rows, 583 MB: 158 us against 90
-// for the bytes; k_mass 118 (0.64 GB read: second loads leave the L2 first; 19
-// instructions a logit of both passes, 0.69 a cycle and scheduler), k_draw 39 (78 MB,
-// 0.61 instructions a cycle).  One request with 4 copied drafts: 12.1 us, latency, about
-// half in each kernel: loads 1.1, exchange 0.6, sums 1.3; accept tests 1.5, sums 3.9,
-// cluster totals 1.3, the token 1.4.
+// inputs).  64 requests x 7 drafts with draft rows, 960 rows, 583 MB: 156 us against 90
+// for the bytes; k_mass 120 (0.64 GB read: second loads leave the L2 first; 19
+// instructions a logit of both passes, 0.69 a cycle and scheduler), k_draw 32 to 40 (78
+// MB, 0.61 instructions a cycle).  One request with 4 copied drafts: 10.9 us, latency: 4.6
+// in k_mass, then accept tests 1.5, sums 2.9, cluster totals 0.6, the token 1.0.
 // Simple kernels, a block per row and per request, took 862 and 194 us.
 #include <cuda_runtime.h>
 
