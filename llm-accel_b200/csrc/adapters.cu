@@ -564,7 +564,8 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
     // counted here, from the slots themselves (k_prepare passed its wait before this
     // kernel could start, so they are final), and the weights can be fetched before
     // k_prepare ends; with more, k_prepare's counts are waited for.
-    if (c.slot && (c.RT == 1 || (c.shared_tiles == 0 && c.T * c.RT <= (int)gridDim.x))) {
+    const bool waits = c.slot && c.RT > 1 && (c.shared_tiles != 0 || c.T * c.RT > (int)gridDim.x);
+    if (c.slot && !waits) {
         TileSlots &ts = *reinterpret_cast<TileSlots *>(ring);
         const int own = blockIdx.x % c.RT;
         const RowSlot r = tile_slots(c, own, ts);
@@ -575,7 +576,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
         // the ring takes this memory over for bulk copies
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     } else {
-        if (c.slot) pdl_wait();
+        if (waits) pdl_wait();
         for (int rt = threadIdx.x; rt < c.RT; rt += blockDim.x) pieces[rt] = c.slot ? __ldcg(c.count + rt) : 0;
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -609,11 +610,11 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
         };
         auto weight_of = [&](const Walk &w, int i) { return c.weight + ((size_t)w.ft * c.P + (size_t)i * D) * kPiece; };
         auto rows_of = [&](const Walk &w, int i) { return c.xp + ((size_t)w.rt * c.P + (size_t)i * D) * NT * 32; };
-        // weights of the first stages before k_prepare has finished, up to the
-        // first adapter stage, whose list it writes
+        // weights of the first stages before k_prepare has finished (unless that has
+        // been waited for), up to the first adapter stage, whose list it writes
         Walk w = k;
         int early = 0;
-        for (bool go = true; go && early < S && w.more(c); w.next(c, pre)) {
+        for (bool go = !waits; go && early < S && w.more(c); w.next(c, pre)) {
             for (int i = w.begin; i < w.end && early < S; i++) {
                 if (i >= C) {
                     go = false;
