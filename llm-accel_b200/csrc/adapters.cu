@@ -994,7 +994,10 @@ int fail(int code, const std::string &msg) {
     set_last_error("adapters: " + msg);
     return code;
 }
+// The runtime keeps a failed call's code for the thread's next check of a launch, of any
+// operator: it is reported here, and only here.
 int cuda_fail(const char *what, cudaError_t e) {
+    (void)cudaGetLastError();
     return fail(e == cudaErrorMemoryAllocation ? LLMX_ERR_NOMEM : LLMX_ERR_CUDA,
                 std::string(what) + ": " + cudaGetErrorString(e));
 }

@@ -959,6 +959,12 @@ int fail(int code, const std::string &msg) {
     llmx::set_last_error("verify_drafts: " + msg);
     return code;
 }
+// Reports a failed runtime call, whose code would else be found by the thread's next
+// check of a launch.
+int cuda_fail(const char *what, cudaError_t e) {
+    (void)cudaGetLastError();
+    return fail(LLMX_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
 
 }  // namespace
 
@@ -1016,7 +1022,7 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DeviceSetup dev;
     cudaError_t e = device_setup(dev);
-    if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("device set-up: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_fail("device set-up", e);
     // CTAs per row: the split with the least time for the busiest cluster, in
     // microseconds as measured on one SM: a chunk's first pass alone 0.4 and its second 0.5,
     // both beside one another 0.62; a row's exchange and its ends 2, or 0.6 where they are hidden.
@@ -1044,11 +1050,11 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     const uint32_t groups = std::min<uint32_t>(a.total, (uint32_t)dev.clusters[a.split]);
     configure(cfg, attr, dim3(groups * a.split), mass_threads(!a.resident), (size_t)a.ring * kChunkBytes, a.split, s);
     e = cudaLaunchKernelEx(&cfg, kMass[a.resident ? 0 : 1], a);
-    if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("k_mass: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_fail("k_mass", e);
     DrawArgs d{a, 1};
     while (d.split < kMaxCluster && requests * d.split * 2 <= (uint32_t)dev.sms * 2 && vocab >= 2048u * d.split) d.split *= 2;
     configure(cfg, attr, dim3(requests * d.split), kDrawThreads, 0, d.split, s);
     e = cudaLaunchKernelEx(&cfg, a.draft ? k_draw<true> : k_draw<false>, d);
-    if (e != cudaSuccess) return fail(LLMX_ERR_CUDA, std::string("k_draw: ") + cudaGetErrorString(e));
+    if (e != cudaSuccess) return cuda_fail("k_draw", e);
     return LLMX_OK;
 }

@@ -339,3 +339,31 @@ def test_call_refusals(llmx, torch):
             c.h.set(*args)
         assert e.value.code == llmx.ERR_ARG
     c.check(whole(c.rng, (8, 128), 700), np.zeros(8), wide=True)  # the handle still serves
+
+
+@gpu
+def test_refusals_leave_no_error_behind(llmx, torch):
+    """A handle that the device cannot hold (2^22 x 32768 weights, 275 GB) or whose device does
+    not exist is refused; the calls after that, of this handle, of a new one and of another operator, succeed."""
+    c = Case(llmx, torch, 128, 64, [4], 8)
+    x = whole(c.rng, (8, 128), 700)
+    few = torch.zeros(64 * 128, dtype=torch.int16, device="cuda")
+    tokens = torch.zeros(8, dtype=torch.int32, device="cuda")
+
+    def refuse(what):
+        with pytest.raises(llmx.LlmxError) as e:
+            if what == "memory":
+                llmx.Adapters(32768, 1 << 22, few.data_ptr(), 0, 0, 1, stream=c.stream())
+            else:
+                llmx.Adapters(128, 64, few.data_ptr(), 0, 0, 1, device=9999, stream=c.stream())
+        assert e.value.code == (llmx.ERR_NOMEM if what == "memory" else llmx.ERR_CUDA)
+
+    for what in ("memory", "device"):
+        refuse(what)
+        c.put(0, 3)
+        refuse(what)
+        h = llmx.Adapters(128, 64, few.data_ptr(), 0, 0, 8, stream=c.stream())
+        h.close()
+        refuse(what)
+        assert llmx.lm_head_argmax_device(few.data_ptr(), 8, 128, few.data_ptr(), 64, tokens.data_ptr(), c.stream()) == llmx.OK
+        c.check(x, np.zeros(8), wide=True)
