@@ -167,6 +167,9 @@ size_t llmx_layer_weight_elems(const llmx_shape *shape);
 int16_t *llmx_model_layer(llmx_model *m, uint32_t layer);
 int16_t *llmx_model_norms(llmx_model *m);        /* [2L+1][hidden] */
 int16_t *llmx_model_embedding(llmx_model *m);    /* [vocab][hidden] or NULL */
+/* The table that scores tokens, [vocab][hidden]: the untied LM head, else the token
+ * embedding (a synthetic model's is materialised first).  NULL when the model has neither. */
+const int16_t *llmx_model_lm_head(llmx_model *m);
 /* model_data_t::embedding host:871-884 (rows of token ids -> Q8.8 rows). */
 int llmx_model_embed(const llmx_model *m, const uint32_t *tokens, uint32_t n,
                      int16_t *out_rows);

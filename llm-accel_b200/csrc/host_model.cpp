@@ -333,6 +333,13 @@ int16_t *llmx_model_norms(llmx_model *m) { return m && !m->norms.empty() ? m->no
 int16_t *llmx_model_embedding(llmx_model *m) {
     return m && !m->embedding.empty() ? m->embedding.data() : nullptr;
 }
+const int16_t *llmx_model_lm_head(llmx_model *m) {
+    try {
+        return m ? model_lm_head_table(m) : nullptr;
+    } catch (const std::bad_alloc &) {
+        return nullptr;
+    }
+}
 
 int llmx_model_embed(const llmx_model *m, const uint32_t *tokens, uint32_t n, int16_t *out) {
     if (!m || (!tokens && n) || (!out && n)) return LLMX_ERR_ARG;

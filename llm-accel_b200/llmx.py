@@ -111,6 +111,7 @@ def lib():
             "llmx_model_layer": (C.POINTER(C.c_int16), [vp, C.c_uint32]),
             "llmx_model_norms": (C.POINTER(C.c_int16), [vp]),
             "llmx_model_embedding": (C.POINTER(C.c_int16), [vp]),
+            "llmx_model_lm_head": (C.POINTER(C.c_int16), [vp]),
             "llmx_model_embed": (C.c_int, [vp, u32p, C.c_uint32, i16p]),
             "llmx_model_lm_head_argmax": (C.c_int, [vp, i16p, C.c_int, C.POINTER(C.c_uint32)]),
             "llmx_tp_unique_id": (C.c_int, [vp]),
@@ -284,6 +285,14 @@ class Model:
         out = np.zeros((len(t), self.shape.hidden), np.int16)
         check(lib().llmx_model_embed(self.h, t, len(t), out), "embed")
         return out
+
+    def lm_head(self) -> np.ndarray:
+        """The table that scores tokens: the untied LM head, else the embedding."""
+        s = self.shape
+        p = lib().llmx_model_lm_head(self.h)
+        if not p:
+            raise LlmxError(ERR_STATE, "no LM head: the model holds no weights")
+        return np.ctypeslib.as_array(p, shape=(s.vocab, s.hidden))
 
     def lm_head_argmax(self, hidden_row, threads=0) -> int:
         tok = C.c_uint32()

@@ -39,8 +39,8 @@ class Server:
         self.contexts = [llmx.Accelerator(self.s, device) for _ in range(requests)]
         for c in self.contexts:
             c.upload_model(model)
-        # the LM head is the embedding table (tied); the handle keeps its own layout of it
-        table = torch.from_numpy(model.embed(np.arange(self.s.vocab))).to(self.dev)
+        # the handle keeps its own layout of the LM head
+        table = torch.from_numpy(model.lm_head()).to(self.dev)
         self.rows = requests * (drafts + 1)
         self.head = llmx.Adapters(self.s.hidden, self.s.vocab, table.data_ptr(), slots, max_rank, self.rows, device,
                                   stream=self.stream())

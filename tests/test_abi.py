@@ -198,3 +198,19 @@ def test_create_without_gpu_fails_loudly(llmx):
     with pytest.raises(llmx.LlmxError) as e:
         llmx.Accelerator(llmx.shape("small"))
     assert e.value.code in (llmx.ERR_CUDA, llmx.ERR_NOMEM)
+
+
+def test_lm_head_table(llmx):
+    """llmx_model_lm_head: the untied head, else the embedding; none without weights."""
+    s = llmx.shape("small")
+    with pytest.raises(llmx.LlmxError):
+        llmx.Model(s).lm_head()
+    untied = llmx.Model(s).init_gaussian(3, lm_head=True)
+    tied = llmx.Model(s).init_gaussian(3)
+    rows = tied.embed(np.arange(s.vocab))
+    assert np.array_equal(tied.lm_head(), rows)
+    assert untied.lm_head().shape == rows.shape and not np.array_equal(untied.lm_head(), rows)
+    h = np.arange(s.hidden, dtype=np.int16) - 30
+    for m in (tied, untied):
+        assert m.lm_head_argmax(h) == int(np.argmax(m.lm_head().astype(np.int64) @ h.astype(np.int64)))
+    assert not llmx.lib().llmx_model_lm_head(None)

@@ -57,3 +57,31 @@ def test_drawn_with_a_temperature(llmx):
     sv.close()
     assert a == b
     assert c[1] == d[1]
+
+
+def host_greedy(llmx, model, prompt, count):
+    """The host's greedy loop: exact scores, the first maximum."""
+    acc = llmx.Accelerator(model.shape)
+    acc.upload_model(model)
+    ex = llmx.Executor(acc, model)
+    text = list(prompt)
+    for at in range(0, len(text), llmx.MAX_ROWS):
+        hidden = ex.run_prompt_block(text[at:at + llmx.MAX_ROWS], at)[-1]
+    for _ in range(count):
+        text.append(model.lm_head_argmax(hidden))
+        hidden = ex.run_token(text[-1], len(text) - 1)[0]
+    acc.close()
+    return text[len(prompt):]
+
+
+@pytest.mark.parametrize("untied", [True, False])
+def test_scores_come_from_the_lm_head(llmx, untied):
+    """Requests without adapters get the host's greedy tokens, with an LM head of its own as
+    with a tied one."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    model = llmx.Model(llmx.shape("small")).init_gaussian(11, lm_head=untied)
+    sv = spec.Server(model, 3, 1, 8, 2)
+    out, _ = sv.generate(PROMPTS, [-1, -1, -1], 8)
+    sv.close()
+    assert out == [host_greedy(llmx, model, p, 8) for p in PROMPTS]
