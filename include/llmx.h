@@ -170,6 +170,8 @@ int16_t *llmx_model_embedding(llmx_model *m);    /* [vocab][hidden] or NULL */
 /* The table that scores tokens, [vocab][hidden]: the untied LM head, else the token
  * embedding (a synthetic model's is materialised first).  NULL when the model has neither. */
 const int16_t *llmx_model_lm_head(llmx_model *m);
+/* 1 when that table is the embedding, whose values are Q8.8; an LM head's are Q4.12. */
+int llmx_model_tied(const llmx_model *m);
 /* model_data_t::embedding host:871-884 (rows of token ids -> Q8.8 rows). */
 int llmx_model_embed(const llmx_model *m, const uint32_t *tokens, uint32_t n,
                      int16_t *out_rows);

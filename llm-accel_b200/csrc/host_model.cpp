@@ -340,6 +340,7 @@ const int16_t *llmx_model_lm_head(llmx_model *m) {
         return nullptr;
     }
 }
+int llmx_model_tied(const llmx_model *m) { return m && m->tied ? 1 : 0; }
 
 int llmx_model_embed(const llmx_model *m, const uint32_t *tokens, uint32_t n, int16_t *out) {
     if (!m || (!tokens && n) || (!out && n)) return LLMX_ERR_ARG;

@@ -111,6 +111,7 @@ def lib():
             "llmx_model_layer": (C.POINTER(C.c_int16), [vp, C.c_uint32]),
             "llmx_model_norms": (C.POINTER(C.c_int16), [vp]),
             "llmx_model_embedding": (C.POINTER(C.c_int16), [vp]),
+            "llmx_model_tied": (C.c_int, [vp]),
             "llmx_model_lm_head": (C.POINTER(C.c_int16), [vp]),
             "llmx_model_embed": (C.c_int, [vp, u32p, C.c_uint32, i16p]),
             "llmx_model_lm_head_argmax": (C.c_int, [vp, i16p, C.c_int, C.POINTER(C.c_uint32)]),
@@ -293,6 +294,11 @@ class Model:
         if not p:
             raise LlmxError(ERR_STATE, "no LM head: the model holds no weights")
         return np.ctypeslib.as_array(p, shape=(s.vocab, s.hidden))
+
+    @property
+    def tied(self) -> bool:
+        """Whether the embedding (Q8.8) stands in for an LM head (Q4.12)."""
+        return bool(lib().llmx_model_tied(self.h))
 
     def lm_head_argmax(self, hidden_row, threads=0) -> int:
         tok = C.c_uint32()

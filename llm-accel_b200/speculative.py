@@ -39,8 +39,10 @@ class Server:
         self.contexts = [llmx.Accelerator(self.s, device) for _ in range(requests)]
         for c in self.contexts:
             c.upload_model(model)
-        # the handle keeps its own layout of the LM head
+        # the handle keeps its own layout of the LM head.  An LM head is Q4.12; an embedding that
+        # stands in for it is Q8.8, so that what the handle writes as Q16.16 is 1/16 of the logits
         table = torch.from_numpy(model.lm_head()).to(self.dev)
+        self.logit_step = 16.0 if model.tied else 1.0
         self.rows = requests * (drafts + 1)
         self.head = llmx.Adapters(self.s.hidden, self.s.vocab, table.data_ptr(), slots, max_rank, self.rows, device,
                                   stream=self.stream())
@@ -61,7 +63,8 @@ class Server:
         return self.torch.cuda.current_stream(self.dev).cuda_stream
 
     def set_adapter(self, slot, scale, down, up):
-        """down [rank][hidden], up [vocab][rank], scale: Q4.12."""
+        """down [rank][hidden] and scale: Q4.12; up [vocab][rank]: in the LM head's format
+        (Q4.12, or Q8.8 where the embedding stands in for it)."""
         d, u = (self.torch.from_numpy(np.ascontiguousarray(a, np.int16)).to(self.dev) for a in (down, up))
         self.head.set(slot, d.shape[0], scale, d.data_ptr(), u.data_ptr(), stream=self.stream())
         self.torch.cuda.current_stream(self.dev).synchronize()
@@ -88,7 +91,7 @@ class Server:
                 self.contexts[r].stack(self.model.embed(block), position=at, include_final_norm=False, materialize=False)
         goal = [len(p) + max_new for p in prompts]
         dev = lambda a: t.from_numpy(np.ascontiguousarray(a).view(np.int32)).to(self.dev)  # noqa: E731
-        temperatures = t.full((count,), float(temperature), device=self.dev)
+        temperatures = t.full((count,), float(temperature) / self.logit_step, device=self.dev)
         drafted = taken = 0
         while any(len(x) < g for x, g in zip(texts, goal)):
             guesses, offsets, row, owners = [], [0], 0, []

@@ -214,3 +214,4 @@ def test_lm_head_table(llmx):
     for m in (tied, untied):
         assert m.lm_head_argmax(h) == int(np.argmax(m.lm_head().astype(np.int64) @ h.astype(np.int64)))
     assert not llmx.lib().llmx_model_lm_head(None)
+    assert tied.tied and not untied.tied

@@ -85,3 +85,37 @@ def test_scores_come_from_the_lm_head(llmx, untied):
     out, _ = sv.generate(PROMPTS, [-1, -1, -1], 8)
     sv.close()
     assert out == [host_greedy(llmx, model, p, 8) for p in PROMPTS]
+
+
+@pytest.mark.parametrize("untied", [True, False])
+def test_temperature_is_that_of_the_logits(llmx, untied):
+    """One drawn token at temperature T lies where the cumulative softmax of the model's logits
+    over T passes the random number.  The logits are rounded once, to 2^-12 (tied) or
+    2^-16: half a step moves a logit over T by at most 2^-13 / T, a cumulative probability by at
+    most twice that; the whole-number weights and shares add less than 1e-6 (2e-7 each, and 64
+    tokens' roundings of 2^-31 and 2^-40)."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    model = llmx.Model(llmx.shape("small")).init_gaussian(11, lm_head=untied)
+    acc = llmx.Accelerator(model.shape)
+    acc.upload_model(model)
+    ex = llmx.Executor(acc, model)
+    unit = 2.0 ** (16 if untied else 12)  # of a logit, in the products' last places over 2^4
+    sv = spec.Server(model, 1, 1, 8, 0)
+    drawn = set()
+    for prompt in ([3], [9, 4], [5, 5, 7], [1, 2, 3, 1]):
+        hidden = ex.run_prompt_block(prompt, 0)[-1].astype(np.int64)
+        z = (model.lm_head().astype(np.int64) @ hidden) / (16 * unit)
+        for t in (0.5, 1.0, 4.0):
+            p = np.exp((z - z.max()) / t)
+            p /= p.sum()
+            mass = np.concatenate([[0], np.cumsum(p)])
+            for seed in range(8):
+                u = int(np.random.default_rng(seed).integers(0, 2**32, 1, dtype=np.uint64)[0]) / 2**32
+                (out,), _ = sv.generate([prompt], [-1], 1, temperature=t, seed=seed)
+                off = 2 * 2.0**-13 / t + 1e-6
+                assert mass[out[0]] - off <= u <= mass[out[0] + 1] + off, (prompt, t, seed)
+                drawn.add(out[0])
+    assert len(drawn) > 4
+    sv.close()
+    acc.close()
