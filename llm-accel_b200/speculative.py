@@ -19,6 +19,8 @@ import numpy as np
 
 import llmx
 
+NO_TOKEN = 0xFFFFFFFF
+
 
 def copied_drafts(tokens, most):
     """What followed the last earlier occurrence of the last two tokens, at most `most` tokens."""
@@ -26,6 +28,26 @@ def copied_drafts(tokens, most):
         if tokens[at:at + 2] == tokens[-2:]:
             return tokens[at + 2:at + 2 + most]
     return []
+
+
+def append_tokens(texts, goal, tokens, accepted):
+    """Appends a step's tokens [requests][most + 1] to the texts that are short of their goal, and says
+    how many drafts were accepted for them; raises, with the texts as they were, where the verification
+    has no tokens for a request (accepted = 0xffffffff) or no token could be drawn."""
+    words = lambda a: np.ascontiguousarray(a).view(np.uint32)  # noqa: E731
+    tokens, accepted = words(tokens), words(accepted)
+    new = {}
+    for r, text in enumerate(texts):
+        if len(text) >= goal[r]:
+            continue
+        if accepted[r] >= tokens.shape[1]:
+            raise llmx.LlmxError(llmx.ERR_TIMEOUT, f"request {r}: the verification gave up")
+        new[r] = tokens[r, :accepted[r] + 1].tolist()
+        if NO_TOKEN in new[r]:
+            raise llmx.LlmxError(llmx.ERR_RANGE, f"request {r}: its row excludes every token")
+    for r, more in new.items():
+        texts[r] += more
+    return sum(len(more) - 1 for more in new.values())
 
 
 class Server:
@@ -83,6 +105,10 @@ class Server:
         t, count = self.torch, len(prompts)
         if count != len(self.contexts):
             raise ValueError(f"{count} prompts for {len(self.contexts)} requests")
+        if len(slots) != count:
+            raise ValueError(f"{len(slots)} slots for {count} requests")
+        if any(len(p) == 0 for p in prompts):
+            raise ValueError("a prompt has at least one token")
         rng = np.random.default_rng(seed)
         texts = [list(map(int, p)) for p in prompts]
         for r, text in enumerate(texts):  # all but the last prompt token
@@ -111,13 +137,12 @@ class Server:
             llmx.verify_drafts(self.logits.data_ptr(), None, self.s.vocab, p(d_guess), p(d_offsets), count, len(guesses), self.drafts,
                                p(temperatures), p(d_accept), p(d_sample), p(self.tokens), p(self.accepted), None, p(self.work),
                                self.work.numel(), stream=self.stream())
-            tokens, accepted = self.tokens.cpu().numpy(), self.accepted.cpu().numpy()
-            for r, text in enumerate(texts):
-                if len(text) < goal[r]:
-                    text += tokens[r, :accepted[r] + 1].tolist()
-                    drafted += offsets[r + 1] - offsets[r]
-                    taken += int(accepted[r])
-        self.head.error(self.stream())
+            # nothing is made of rows or logits that a kernel gave up
+            self.head.error(self.stream())
+            for c in self.contexts:
+                c.synchronize()
+            drafted += sum(offsets[r + 1] - offsets[r] for r, text in enumerate(texts) if len(text) < goal[r])
+            taken += append_tokens(texts, goal, self.tokens.cpu().numpy(), self.accepted.cpu().numpy())
         return [text[len(q):] for text, q in zip(texts, prompts)], (drafted, taken)
 
 
