@@ -87,6 +87,12 @@ class Server:
     def set_adapter(self, slot, scale, down, up):
         """down [rank][hidden] and scale: Q4.12; up [vocab][rank]: in the LM head's format
         (Q4.12, or Q8.8 where the embedding stands in for it)."""
+        down, up = np.asarray(down), np.asarray(up)
+        if down.ndim != 2 or up.shape != (self.s.vocab, len(down)) or down.shape[1] != self.s.hidden:
+            raise ValueError(f"down {down.shape} and up {up.shape} are not [rank][{self.s.hidden}] and [{self.s.vocab}][rank]")
+        for what, a in (("down", down), ("up", up), ("scale", np.asarray(scale))):
+            if a.dtype.kind not in "iu" or (a.size and (a.min() < -32768 or a.max() > 32767)):
+                raise ValueError(f"{what} is not whole numbers of 16 bits")
         d, u = (self.torch.from_numpy(np.ascontiguousarray(a, np.int16)).to(self.dev) for a in (down, up))
         self.head.set(slot, d.shape[0], scale, d.data_ptr(), u.data_ptr(), stream=self.stream())
         self.torch.cuda.current_stream(self.dev).synchronize()

@@ -97,3 +97,17 @@ def test_refusals(monkeypatch):
     for kw in (dict(prompts=((), (3,))), dict(slots=(0,)), dict(prompts=((1,),))):
         with pytest.raises(ValueError):
             Loop(monkeypatch, fine).run(**kw)
+
+
+def test_adapters_of_other_sizes_are_refused(monkeypatch):
+    """The device kernels read [rank][hidden] and [vocab][rank] of what they are given."""
+    sv = Loop(monkeypatch, fine).server
+    put = []
+    sv.head.set = lambda *a, **k: put.append(a)
+    good = dict(slot=0, scale=4096, down=np.zeros((4, 64), np.int64), up=np.zeros((64, 4), np.int64))
+    for bad in (dict(up=np.zeros((64, 3), np.int64)), dict(up=np.zeros((63, 4), np.int64)), dict(down=np.zeros((4, 56), np.int64)),
+                dict(down=np.zeros((64,), np.int64)), dict(down=np.full((4, 64), 32768)), dict(up=np.full((64, 4), -32769)),
+                dict(up=np.zeros((64, 4))), dict(scale=32768), dict(scale=0.5)):
+        with pytest.raises(ValueError):
+            sv.set_adapter(**{**good, **bad})
+    assert not put
