@@ -122,6 +122,7 @@ struct Call {
     int64_t *acc;          // [grid][NT][128] sums of tiles cut between CTAs, zero between calls
     int32_t *arrived;      // [grid]
     int *error;
+    uint32_t polls;        // of a wait, except for what has to land before a CTA ends
     int ring, buffers;     // ring stages, accumulator sets
     int shared_tiles;      // tiles whose stages are shared by several CTAs
     int sharers;           // CTAs that share them
@@ -391,7 +392,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
             if (threadIdx.x < kSums)
                 st_async(remote(&part_s[share][threadIdx.x], 0), (uint64_t)sum, remote(&part_bar, 0));
             if (share != 0) continue;
-            if (!mbar_wait_cluster(&part_bar, 0)) atomicExch(c.error, 3);
+            if (!mbar_wait_cluster(&part_bar, 0, c.polls)) atomicExch(c.error, 3);
             sum = 0;
             if (threadIdx.x < kSums)
                 for (int p = 0; p < c.ksplit; p++) sum += part_s[p][threadIdx.x];
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
             if (lane == 0 && first < bound) {
                 const uint8_t *src = weight_of(k, first), *rows = rows_of(k, first);
                 for (int i = first; i < bound; i++) {
-                    if (issued >= S && !mbar_wait(empty + s, phase)) {
+                    if (issued >= S && !mbar_wait(empty + s, phase, c.polls)) {
                         ok = false;
                         break;
                     }
@@ -656,7 +657,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                 const int p0 = (i - C) * D, np = min(D, pieces[k.rt] - p0);
                 const int2 mine = (lane & 7) < np ? __ldcg(c.list + (size_t)k.rt * c.max_pieces + p0 + (lane & 7)) : make_int2(0, 0);
                 if (issued >= S) {
-                    ok = mbar_wait(empty + s, phase);
+                    ok = mbar_wait(empty + s, phase, c.polls);
                     ok = __all_sync(~0u, ok);
                     if (!ok) break;
                 }
@@ -678,13 +679,12 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                 }
             }
         }
-        if (!ok && lane == 0) {
-            atomicExch(c.error, 1);
-            issued = max(issued, early);
-            for (int q = 0; q < S && q < issued; q++) {  // the copies in flight land before the CTA ends
-                const int last = q + ((issued - 1 - q) / S) * S;
-                (void)mbar_wait(full + q, (last / S) & 1);
-            }
+        if (!ok && lane == 0) atomicExch(c.error, 1);
+        // The copies in flight land before the CTA ends, also where the warp that waits for them
+        // has given up.  (Every announced stage was issued whole: the first S need no wait.)
+        for (int q = 0; lane == 0 && q < S && q < issued; q++) {
+            const int last = q + ((issued - 1 - q) / S) * S;
+            (void)mbar_wait(full + q, (last / S) & 1);
         }
         __syncwarp();
     } else if (warp == 0) {  // ---- products ---------------------------------------
@@ -714,12 +714,12 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
             };
             for (; k.more(c); k.next(c, pre), tiles++) {
                 const int b = c.buffers == 2 ? tiles & 1 : 0, use = c.buffers == 2 ? tiles >> 1 : tiles;
-                if (use > 0 && !mbar_wait(tempty + b, (use - 1) & 1)) ok = false;
+                if (use > 0 && !mbar_wait(tempty + b, (use - 1) & 1, c.polls)) ok = false;
                 const uint32_t dh = tmem + (uint32_t)(b * 4 * NT), dl = dh + 2 * NT;
                 const int bound = min(k.end, C);
                 uint32_t more = 0;  // the first product of the step overwrites
                 for (int i = k.begin; ok && i < bound; i++) {
-                    if (!mbar_wait(full + s, phase)) {
+                    if (!mbar_wait(full + s, phase, c.polls)) {
                         ok = false;
                         break;
                     }
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                     advance();
                 }
                 for (int i = max(k.begin, C); ok && i < k.end; i++) {
-                    if (!mbar_wait(full + s, phase)) {
+                    if (!mbar_wait(full + s, phase, c.polls)) {
                         ok = false;
                         break;
                     }
@@ -777,7 +777,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                 b_hi = cta_of(at + k.len - 1, line, sharers);
             }
             unsigned long long *acc = reinterpret_cast<unsigned long long *>(c.acc) + (size_t)b_lo * NT * kOutTile + m;
-            const bool okw = mbar_wait_err(tfull + b, use & 1, c.error);
+            const bool okw = mbar_wait_err(tfull + b, use & 1, c.error, c.polls);
             if (lane == 0) fail_s[warp - 2] = okw ? 0 : 1;
             named_sync(3, kResultThreads);
             int failed = 0;
@@ -1242,6 +1242,7 @@ extern "C" int llmx_adapters_project(llmx_adapters *h, const int16_t *x, uint32_
     c.acc = h->acc;
     c.arrived = h->arrived;
     c.error = h->error;
+    c.polls = serving_wait_polls();
     c.buffers = c.NT <= 64 ? 2 : 1;  // 4 sums x NT columns each, 512 in all
     c.D = c.NT < 96 ? 8 : 4;
     c.C = c.P / c.D;

@@ -34,8 +34,8 @@ static __device__ __forceinline__ void st_async(uint32_t to, int32_t v, uint32_t
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.s32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar)
                  : "memory");
 }
-static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpinLimit; i++) {
+static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, uint32_t polls = kSpinLimit) {
+    for (uint32_t i = 0; i < polls; i++) {
         uint32_t ok;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"

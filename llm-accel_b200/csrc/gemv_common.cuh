@@ -11,7 +11,6 @@
 namespace llmx {
 
 constexpr int kMaxStages = 32;
-constexpr uint32_t kSpinLimit = 1u << 26;           // bounded mbarrier waits (seconds of polling)
 
 // ---- mbarrier / bulk-copy primitives ---------------------------------------
 static __device__ __forceinline__ uint32_t smem_u32(const void *p) {
@@ -37,14 +36,15 @@ static __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t par
     return ok != 0;
 }
 // Bounded wait: false when the limit expired (the caller records an error).
-static __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
-    for (uint32_t i = 0; i < kSpinLimit; i++)
+static __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32_t polls = kSpinLimit) {
+    for (uint32_t i = 0; i < polls; i++)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
 // Bounded wait that also gives up as soon as any CTA has recorded an error.
-static __device__ __forceinline__ bool mbar_wait_err(uint64_t *bar, uint32_t parity, const int *err) {
-    for (uint32_t i = 0; i < kSpinLimit; i++) {
+static __device__ __forceinline__ bool mbar_wait_err(uint64_t *bar, uint32_t parity, const int *err,
+                                                     uint32_t polls = kSpinLimit) {
+    for (uint32_t i = 0; i < polls; i++) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 255u && *reinterpret_cast<const volatile int *>(err) != 0) return false;
     }

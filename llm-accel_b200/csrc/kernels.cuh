@@ -319,6 +319,9 @@ cudaError_t launch_embed_rows(const int16_t *table, const uint32_t *tokens, int 
                               int16_t *out, int *err, cudaStream_t s);
 
 // Message returned by llmx_last_error() on this thread.
+constexpr uint32_t kSpinLimit = 1u << 26;  // polls of a bounded mbarrier wait (about a microsecond each)
 void set_last_error(const std::string &msg);
+// Polls of a wait in the kernels that serve several requests (llmx_selftest_serving_waits).
+uint32_t serving_wait_polls();
 
 }  // namespace llmx

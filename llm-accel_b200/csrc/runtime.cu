@@ -6,6 +6,7 @@
 #include <nccl.h>
 
 #include <algorithm>
+#include <atomic>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
@@ -60,6 +61,8 @@ int rows_template(uint32_t rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <
 }  // namespace
 
 void llmx::set_last_error(const std::string &msg) { g_last_error = msg; }
+static std::atomic<uint32_t> g_serving_wait_polls{kSpinLimit};
+uint32_t llmx::serving_wait_polls() { return g_serving_wait_polls.load(std::memory_order_relaxed); }
 
 // Geometry of one projection in the tensor-core item layout.
 struct MmaGeom {
@@ -1546,6 +1549,11 @@ int llmx_selftest_ar_timeout(llmx_ctx *c, uint32_t poll_limit) {
     ArFinishArgs f{a, 0, c->hid[1], c->hid[0], c->step, c->err};
     CK(launch_ar_finish(f, c->stream));
     return finish(c);
+}
+
+int llmx_selftest_serving_waits(uint32_t polls) {
+    g_serving_wait_polls.store(std::min(polls, kSpinLimit), std::memory_order_relaxed);
+    return LLMX_OK;
 }
 
 int llmx_decode_fuses_o(const llmx_ctx *c) { return c && use_fuse_o(c, 1) ? 1 : 0; }

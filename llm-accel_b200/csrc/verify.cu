@@ -90,6 +90,7 @@ struct Args {
     int split;       // CTAs per row (k_mass), and of a cluster there
     int ring;        // chunks of shared memory per CTA
     int resident;    // the ring holds a CTA's share of a row: it is loaded once
+    uint32_t polls;  // of a wait, except for what has to land before a CTA ends
 };
 
 // ---- arithmetic -------------------------------------------------------------------
@@ -399,7 +400,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                 const Row r(a, row, rank);
                 for (uint32_t v = r.v0; v < r.v1; v += kChunk / 4) {
                     const int at = base + s;
-                    if (issued >= ring && !mbar_wait(empty + at, phase)) {
+                    if (issued >= ring && !mbar_wait(empty + at, phase, a.polls)) {
                         ok = false;
                         break;
                     }
@@ -415,7 +416,8 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                     }
                 }
             }
-            for (int q = 0; !ok && q < ring && q < issued; q++) {  // the copies in flight land before the CTA ends
+            // the copies in flight land before the CTA ends, also where a warp that waits for them has given up
+            for (int q = 0; q < ring && q < issued; q++) {
                 const int last = q + ((issued - 1 - q) / ring) * ring;
                 (void)mbar_wait(full + base + q, (last / ring) & 1);
             }
@@ -427,7 +429,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         for (uint32_t row = group; row < a.total; row += groups, i++) {
             const uint32_t b = owner_of(a, row);
             const float scale = b == kNoToken ? -1.0f : row_scale(a.temperature[b]);
-            if (i >= 2 && !__all_sync(~0u, mbar_wait(info_empty + (i & 1), ((i >> 1) - 1) & 1))) break;
+            if (i >= 2 && !__all_sync(~0u, mbar_wait(info_empty + (i & 1), ((i >> 1) - 1) & 1, a.polls))) break;
             if (lane == 0) {
                 scale_s[i & 1] = scale;
                 mbar_arrive(info_full + (i & 1));
@@ -474,9 +476,10 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         if (lane < S)
             asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(bar, lane)) : "memory");
     };
+    // (a slot whose chunk was not waited for to the end stays this warp's: it may still be filled)
     auto release = [&](int at) {
         __syncwarp();
-        if (lane == 0) mbar_arrive(empty + at);
+        if (lane == 0 && ok) mbar_arrive(empty + at);
     };
     int32_t top = kExcluded;  // of the row in its first pass
     // thread t of `stride` takes its vectors of a chunk
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         top = __reduce_max_sync(~0u, max(top, edge));
         // every warp waits, not the last alone: else one could go on two rows and be counted
         // in a row that others have not reached
-        if (i >= kTops) ok = ok && mbar_wait_cluster(top_done + i % kTops, (i / kTops - 1) & 1);
+        if (i >= kTops) ok = ok && mbar_wait_cluster(top_done + i % kTops, (i / kTops - 1) & 1, a.polls);
         if (lane == 0) warp_top[i & 1][w] = top;
         if (last_of(&top_count[i & 1], kMaxWarps)) {
             top = __reduce_max_sync(~0u, lane < kMaxWarps ? warp_top[i & 1][lane] : kExcluded);
@@ -522,7 +525,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
             const Held h(a, row, rank, t);
             for (int c = 0; c < h.chunks; c++, p.move(1)) {
-                ok = ok && mbar_wait(full + p.slot(), p.phase);
+                ok = ok && mbar_wait(full + p.slot(), p.phase, a.polls);
                 first_chunk(h.r, p.slot(), c, t, std::integral_constant<int, kFirstWarps * 32>());
                 release(p.slot());
             }
@@ -536,11 +539,11 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         unsigned long long sum = 0;
         uint32_t first = kNoToken;
         auto begin_second = [&](const Held &h, uint32_t i) {
-            ok = ok && mbar_wait(info_full + (i & 1), (i >> 1) & 1);
+            ok = ok && mbar_wait(info_full + (i & 1), (i >> 1) & 1, a.polls);
             const float scale = scale_s[i & 1];
             __syncwarp();
-            if (lane == 0) mbar_arrive(info_empty + (i & 1));
-            ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1);
+            if (lane == 0 && ok) mbar_arrive(info_empty + (i & 1));
+            ok = ok && mbar_wait_cluster(top_full + i % kTops, (i / kTops) & 1, a.polls);
             const int32_t t = __reduce_max_sync(~0u, lane < S ? tops[i % kTops][lane] : kExcluded);
             rw.set(t, scale);
             sum = 0;
@@ -621,7 +624,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             if (!kTwice) {
                 Place p = place;
                 for (int c = p.own(mine); c < h.chunks; c += kGroups, p.move(kGroups)) {
-                    ok = ok && mbar_wait(full + p.slot(), p.phase);
+                    ok = ok && mbar_wait(full + p.slot(), p.phase, a.polls);
                     first_chunk(h.r, p.slot(), c, gt, std::integral_constant<int, kStride>());
                 }
                 send_top(i, h.edge, warp);
@@ -629,7 +632,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             begin_second(h, i);
             Place q = place;
             for (int c = q.own(mine); c < h.chunks; c += kGroups, q.move(kGroups)) {
-                if (kTwice) ok = ok && mbar_wait(full + q.slot(), q.phase);
+                if (kTwice) ok = ok && mbar_wait(full + q.slot(), q.phase, a.polls);
                 second_chunk(h.r, q.slot(), c);
                 release(q.slot());
             }
@@ -830,7 +833,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 if ((int)threadIdx.x < S)
                     st_async(remote(&cta_sum[round][rank], threadIdx.x), (uint64_t)cta, remote(&sums_full[round], threadIdx.x));
                 total = 0;
-                if (!mbar_wait_cluster(&sums_full[round], 0)) {
+                if (!mbar_wait_cluster(&sums_full[round], 0, a.polls)) {
                     bad = true;
                     break;
                 }
@@ -1018,6 +1021,7 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     a.accepted = accepted;
     a.probs = probs;
     a.rows = static_cast<RowPart *>(workspace);
+    a.polls = llmx::serving_wait_polls();
     a.total = drafts + requests + (a.draft ? drafts : 0);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     DeviceSetup dev;

@@ -1,0 +1,65 @@
+"""Waits that run out in the kernels that serve several requests.
+
+Their bound is set so low (llmx_selftest_serving_waits) that warps give up while copies and other
+warps are still under way.  The kernels have to end, report what they gave up, and serve the next
+call exactly.
+"""
+import numpy as np
+import pytest
+
+import serving_oracle as S
+from test_adapters import Case, whole
+from test_verify import Device, make
+
+pytestmark = pytest.mark.gpu
+POLLS = [0, 1, 2, 3, 4, 6, 9]
+
+
+@pytest.fixture(scope="module")
+def torch():
+    return pytest.importorskip("torch")
+
+
+@pytest.fixture
+def short(llmx):
+    """Sets the bound; the default is back after the test."""
+    yield llmx.selftest_serving_waits
+    llmx.selftest_serving_waits()
+
+
+def project(llmx, torch, short, k, n, ranks, rows):
+    c = Case(llmx, torch, k, n, ranks, rows, seed=k)
+    x = whole(c.rng, (rows, k), 700)
+    slot = c.rng.integers(-1, len(ranks), rows)
+    outcomes = []
+    for polls in POLLS:
+        short(polls)
+        for _ in range(3):
+            try:
+                c.check(x, slot, wide=True)  # exact, or reported
+                outcomes.append(llmx.OK)
+            except llmx.LlmxError as e:
+                outcomes.append(e.code)
+        short()
+        c.check(x, slot, wide=True)
+    assert set(outcomes) <= {llmx.OK, llmx.ERR_TIMEOUT} and outcomes[:3] == [llmx.ERR_TIMEOUT] * 3
+
+
+@pytest.mark.parametrize("k,n,ranks,rows", [(64, 100, [9], 1), (2048, 2560, [16, 4], 1), (1096, 4999, [13] * 20, 77),
+                                            (2048, 22016, [32] * 16, 16), (2048, 3000, [64] * 4, 300)])
+def test_projection(llmx, torch, short, k, n, ranks, rows):
+    project(llmx, torch, short, k, n, ranks, rows)
+
+
+@pytest.mark.parametrize("counts,vocab", [([3, 0, 2], 997), ([1] * 300, 500), ([0] * 500, 2000)])
+def test_verification(llmx, torch, short, counts, vocab):
+    """Rows and requests of one CTA each."""
+    d = Device(llmx, torch, make(np.random.default_rng(vocab), counts, vocab))
+    for polls in POLLS:
+        short(polls)
+        for _ in range(3):
+            d.call()
+        torch.cuda.synchronize()
+        short()
+        d.call()
+        d.check()
