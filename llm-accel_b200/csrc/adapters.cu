@@ -328,6 +328,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vectors = c.K >> 3, all = kWarps * c.ksplit, part = share * kWarps + warp;
     const int from = c.steps * part / all, to = c.steps * (part + 1) / all;
+    bool came = true;    // the other blocks' sums
     uint32_t taken = 0;  // rows of the span that are members of a group of it (a group's first row aside)
     for (uint32_t row = row0; row < min(row0 + c.span, c.rows); row++) {
         if ((taken >> (row - row0)) & 1u) continue;
@@ -391,8 +392,14 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
             cluster_wait();
             if (threadIdx.x < kSums)
                 st_async(remote(&part_s[share][threadIdx.x], 0), (uint64_t)sum, remote(&part_bar, 0));
-            if (share != 0) continue;
-            if (!mbar_wait_cluster(&part_bar, 0, c.polls)) atomicExch(c.error, 3);
+            __syncwarp();
+            cluster_arrive();  // nothing more is sent
+            if (share != 0) {
+                cluster_leave(true);
+                return;
+            }
+            came = mbar_wait_cluster(&part_bar, 0, c.polls);
+            if (!came) atomicExch(c.error, 3);
             sum = 0;
             if (threadIdx.x < kSums)
                 for (int p = 0; p < c.ksplit; p++) sum += part_s[p][threadIdx.x];
@@ -418,6 +425,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
                 *reinterpret_cast<uint32_t *>(dst + r * 16 + 4 * w) = 0;
                 *reinterpret_cast<uint32_t *>(dst + c.NT * 16 + r * 16 + 4 * w) = 0;
             }
+        if (c.ksplit > 1) cluster_leave(came);
     }
 }
 

@@ -51,6 +51,12 @@ def test_projection(llmx, torch, short, k, n, ranks, rows):
     project(llmx, torch, short, k, n, ranks, rows)
 
 
+@pytest.mark.parametrize("k,n,ranks,rows", [(11008, 2048, [16, 5], 8), (32768, 200, [128], 2), (4096, 4000, [16] * 3, 40)])
+def test_projection_of_many_inputs(llmx, torch, short, k, n, ranks, rows):
+    """Adapters' products cut over the blocks of a cluster."""
+    project(llmx, torch, short, k, n, ranks, rows)
+
+
 @pytest.mark.parametrize("counts,vocab", [([3, 0, 2], 997), ([1] * 300, 500), ([0] * 500, 2000)])
 def test_verification(llmx, torch, short, counts, vocab):
     """Rows and requests of one CTA each."""
