@@ -45,6 +45,7 @@ namespace {
 using llmx::bulk_g2s;
 using llmx::bulk_g2s_hint;
 using llmx::cluster_arrive;
+using llmx::cluster_leave;
 using llmx::cluster_rank;
 using llmx::cluster_wait;
 using llmx::mbar_arrive;
@@ -661,7 +662,7 @@ struct DrawArgs {
 template <bool kModel>
 __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const Args &a = d.a;
-    __shared__ uint32_t first_s, bad_s;
+    __shared__ uint32_t first_s, bad_s, lost_s;  // lost: the other CTAs' sums did not come
     __shared__ RowMass mass_s[kKeep][2], last_s[2];
     __shared__ unsigned long long warp_sum[kDrawWarps], cta_sum[2][kMaxCluster];
     __shared__ unsigned long long run_sum[kDrawWarps][kRuns];  // of up to kRuns runs of a warp's steps
@@ -687,6 +688,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     if (threadIdx.x == 0) {
         first_s = count;
         bad_s = valid ? 0u : 1u;
+        lost_s = 0;
     }
     __syncthreads();
     const uint32_t targets = a.drafts + a.requests;
@@ -833,7 +835,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 if ((int)threadIdx.x < S)
                     st_async(remote(&cta_sum[round][rank], threadIdx.x), (uint64_t)cta, remote(&sums_full[round], threadIdx.x));
                 total = 0;
-                if (!mbar_wait_cluster(&sums_full[round], 0, a.polls)) {
+                if (__syncthreads_or(!mbar_wait_cluster(&sums_full[round], 0, a.polls))) {
+                    lost_s = 1;  // the CTA's threads go on, or give up, as one
                     bad = true;
                     break;
                 }
@@ -844,6 +847,10 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 total = cta;
             }
             if (total != 0 || !rest) break;
+        }
+        if (S > 1) {
+            __syncwarp();
+            cluster_arrive();  // nothing more is sent
         }
         const uint64_t point = mul_frac(total, a.sample_u[b]);
         if (total != 0 && point >= below && point - below < mine) {  // one warp of the cluster holds the point
@@ -880,6 +887,8 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
         } else if (total == 0 && rank == 0 && threadIdx.x == 0) {
             out[n] = kNoToken;
         }
+    } else if (S > 1) {
+        cluster_arrive();
     }
     if (rank == 0) {
         for (uint32_t j = threadIdx.x; j <= a.max_drafts; j += kDrawThreads) {
@@ -888,6 +897,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
         }
         if (threadIdx.x == 0) a.accepted[b] = bad ? kNoToken : n;
     }
+    if (S > 1) cluster_leave(lost_s == 0);
 }
 
 // CTAs per row that are considered: 9 and 6 fill a group of 18 SMs that cannot hold
