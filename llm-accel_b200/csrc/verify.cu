@@ -390,6 +390,13 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
     // with many rows the draw's CTAs would only take room from the last of this kernel's
     if (!kTwice) pdl_trigger();
 
+    // every warp's end
+    auto leave = [&](bool came) {
+        if (S == 1) return;
+        __syncwarp();
+        cluster_arrive();
+        cluster_leave(came);
+    };
     if (warp >= kLoad && warp < kLoad + 2) {  // ---- loads, of the first pass and of the second -----
         if (lane == 0 && (kTwice || warp == kLoad)) {
             const int base = warp == kLoad ? 0 : kFirstRing;
@@ -423,6 +430,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                 (void)mbar_wait(full + base + q, (last / ring) & 1);
             }
         }
+        leave(true);
         return;
     }
     if (warp == kLoad + 2) {  // ---- the rows' temperatures --------------------------
@@ -437,6 +445,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             }
             __syncwarp();
         }
+        leave(true);
         return;
     }
 
@@ -645,6 +654,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
     ok = __all_sync(~0u, ok);
     if (!ok && lane == 0)
         for (uint32_t row = group; row < a.total; row += groups) a.rows[row].part[rank] = kGaveUp;
+    leave(ok);
 }
 
 // ---------------------------------------------------------------------------

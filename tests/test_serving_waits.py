@@ -59,7 +59,9 @@ def test_projection_of_many_inputs(llmx, torch, short, k, n, ranks, rows):
 
 @pytest.mark.parametrize("counts,vocab", [([3, 0, 2], 997), ([1] * 300, 500), ([0] * 500, 2000),
                                           # requests of two CTAs each
-                                          ([3, 0, 2], 4000), ([1] * 60, 4000), ([0], 4000)])
+                                          ([3, 0, 2], 4000), ([1] * 60, 4000), ([0], 4000),
+                                          # rows and requests of several CTAs
+                                          ([3, 0, 2], 50001), ([4], 151936), ([0] * 100, 30001), ([2] * 60, 60002)])
 def test_verification(llmx, torch, short, counts, vocab):
     d = Device(llmx, torch, make(np.random.default_rng(vocab), counts, vocab))
     for polls in POLLS:
