@@ -451,6 +451,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
 
     // ---- maxima and sums ---------------------------------------------------------------
     bool ok = true;
+    uint32_t row = group;
     // A place in a ring of n slots from slot `base` on, moved by chunks.  Slot s is always
     // group s mod kGroups's (n is a multiple of kGroups): a warp then meets every phase of the
     // barriers that it waits on, and cannot take an older phase for the one it needs.
@@ -511,6 +512,10 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         // every warp waits, not the last alone: else one could go on two rows and be counted
         // in a row that others have not reached
         if (i >= kTops) ok = ok && mbar_wait_cluster(top_done + i % kTops, (i / kTops - 1) & 1, a.polls);
+        // a warp that gave up counts in nothing any more: what it has no part in is never sent, and
+        // all that need it give up too
+        ok = __all_sync(~0u, ok);
+        if (!ok) return;
         if (lane == 0) warp_top[i & 1][w] = top;
         if (last_of(&top_count[i & 1], kMaxWarps)) {
             top = __reduce_max_sync(~0u, lane < kMaxWarps ? warp_top[i & 1][lane] : kExcluded);
@@ -532,7 +537,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         const int w = warp - kMassWarps, t = w * 32 + lane;
         Place p{0, 0, 0, kFirstRing};
         uint32_t i = 0;
-        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
+        for (; ok && row < a.total; row += groups, i++) {
             const Held h(a, row, rank, t);
             for (int c = 0; c < h.chunks; c++, p.move(1)) {
                 ok = ok && mbar_wait(full + p.slot(), p.phase, a.polls);
@@ -540,6 +545,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                 release(p.slot());
             }
             send_top(i, h.edge, w);
+            if (!ok) break;
         }
     } else {
         const int mine = warp / GW, gt = (warp % GW) * 32 + lane;
@@ -604,7 +610,10 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
             }
         };
         auto end_second = [&](uint32_t row, uint32_t i) {
-            // sums (greedy: the smallest first position) of the warp, then of the CTA
+            // sums (greedy: the smallest first position) of the warp, then of the CTA; nothing is
+            // written for a row that a warp of the CTA gave up
+            ok = __all_sync(~0u, ok);
+            if (!ok) return;
             auto whole = [&](unsigned long long v) {
                 if (rw.greedy) return (unsigned long long)__reduce_min_sync(~0u, (uint32_t)v);
                 return sum_lanes(v);
@@ -629,7 +638,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         };
         Place place{0, 0, kTwice ? kFirstRing : 0, kTwice ? a.ring - kFirstRing : a.ring};
         uint32_t i = 0;
-        for (uint32_t row = group; ok && row < a.total; row += groups, i++) {
+        for (; ok && row < a.total; row += groups, i++) {
             const Held h(a, row, rank, (int)threadIdx.x);
             if (!kTwice) {
                 Place p = place;
@@ -638,6 +647,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                     first_chunk(h.r, p.slot(), c, gt, std::integral_constant<int, kStride>());
                 }
                 send_top(i, h.edge, warp);
+                if (!ok) break;
             }
             begin_second(h, i);
             Place q = place;
@@ -647,13 +657,14 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                 release(q.slot());
             }
             end_second(row, i);
+            if (!ok) break;
             place.move(h.chunks);
         }
     }
-    // a wait ran out: rows of this cluster may lack sums, and none of them is to be used
-    ok = __all_sync(~0u, ok);
+    // A wait ran out: from this row on the CTA has no parts, since none is written without every
+    // warp, and the mark stays.
     if (!ok && lane == 0)
-        for (uint32_t row = group; row < a.total; row += groups) a.rows[row].part[rank] = kGaveUp;
+        for (; row < a.total; row += groups) a.rows[row].part[rank] = kGaveUp;
     leave(ok);
 }
 

@@ -72,3 +72,31 @@ def test_verification(llmx, torch, short, counts, vocab):
         short()
         d.call()
         d.check()
+
+
+def exact_or_given_up(torch, d):
+    """Every request has its tokens, or accepted = 0xffffffff; how many have the latter."""
+    torch.cuda.synchronize()
+    c = d.c
+    want = d.want
+    n = d.b * (c["most"] + 1)
+    accepted = d.accepted.cpu().numpy()[:d.b].view(np.uint32)
+    out = d.out.cpu().numpy()[:n].view(np.uint32).reshape(d.b, -1)
+    gone = accepted == S.NO_TOKEN
+    assert np.array_equal(accepted[~gone], want[1][~gone]) and np.array_equal(out[~gone], want[0][~gone])
+    return int(gone.sum())
+
+
+@pytest.mark.parametrize("counts,vocab", [([3, 0, 2], 997), ([1] * 300, 500), ([0] * 150, 20000), ([1] * 100, 40001), ([0] * 80, 150001)])
+def test_sums_given_up_are_marked(llmx, torch, short, counts, vocab):
+    """A row of which any warp gave up has no sum, whatever the other warps did after that."""
+    d = Device(llmx, torch, make(np.random.default_rng(vocab), counts, vocab))
+    d.call()
+    d.want = d.check()
+    for polls in POLLS:
+        short(polls)
+        for _ in range(30):
+            d.accepted.fill_(777)
+            d.call()
+            gone = exact_or_given_up(torch, d)
+            assert polls > 0 or gone == d.b
