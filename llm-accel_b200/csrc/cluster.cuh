@@ -26,15 +26,17 @@ static __device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) 
 static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 // For the exchange's end, after a cluster_arrive by every thread of the cluster once it sends
-// nothing more: no CTA's shared memory goes while another may still address it.  came: this
+// nothing more (and once every thread of its CTA has passed the cluster_wait before): no CTA's shared memory goes while another may still address it.  came: this
 // thread got all that it waited for.  If not, something may have been sent just now that nobody
 // waits for any more; it is given time to land (some 100 us, hundreds of times what it takes).
+static __device__ __forceinline__ void let_land() {
+    for (const long long t = clock64(); clock64() - t < 200000;) {
+    }
+}
 static __device__ __forceinline__ void cluster_leave(bool came) {
     __syncwarp();
     cluster_wait();
-    if (!came)
-        for (const long long t = clock64(); clock64() - t < 200000;) {
-        }
+    if (!came) let_land();
 }
 // The receiver's barrier expects the bytes of all values (mbar_expect_tx).
 static __device__ __forceinline__ void st_async(uint32_t to, uint64_t v, uint32_t bar) {
@@ -44,6 +46,20 @@ static __device__ __forceinline__ void st_async(uint32_t to, uint64_t v, uint32_
 static __device__ __forceinline__ void st_async(uint32_t to, int32_t v, uint32_t bar) {
     asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.s32 [%0], %1, [%2];" ::"r"(to), "r"(v), "r"(bar)
                  : "memory");
+}
+// An arrival on another CTA's barrier, once everything this thread did before is seen there.
+static __device__ __forceinline__ void arrive_remote(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Whether the phase is complete now; try_wait would stay for a microsecond where it is not.
+static __device__ __forceinline__ bool mbar_test_cluster(uint64_t *bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, uint32_t polls = kSpinLimit) {
     for (uint32_t i = 0; i < polls; i++) {

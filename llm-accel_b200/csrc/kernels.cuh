@@ -321,7 +321,9 @@ cudaError_t launch_embed_rows(const int16_t *table, const uint32_t *tokens, int 
 // Message returned by llmx_last_error() on this thread.
 constexpr uint32_t kSpinLimit = 1u << 26;  // polls of a bounded mbarrier wait (about a microsecond each)
 void set_last_error(const std::string &msg);
-// Polls of a wait in the kernels that serve several requests (llmx_selftest_serving_waits).
+// Of llmx_selftest_serving_waits: polls of a wait in the kernels that serve several requests, and
+// the CTAs of a request's draw, by rank in their cluster, that give up at once.
 uint32_t serving_wait_polls();
+uint32_t serving_lost_draws();
 
 }  // namespace llmx

@@ -61,8 +61,9 @@ int rows_template(uint32_t rows) { return rows <= 1 ? 1 : rows <= 2 ? 2 : rows <
 }  // namespace
 
 void llmx::set_last_error(const std::string &msg) { g_last_error = msg; }
-static std::atomic<uint32_t> g_serving_wait_polls{kSpinLimit};
+static std::atomic<uint32_t> g_serving_wait_polls{kSpinLimit}, g_serving_lost_draws{0};
 uint32_t llmx::serving_wait_polls() { return g_serving_wait_polls.load(std::memory_order_relaxed); }
+uint32_t llmx::serving_lost_draws() { return g_serving_lost_draws.load(std::memory_order_relaxed); }
 
 // Geometry of one projection in the tensor-core item layout.
 struct MmaGeom {
@@ -1551,7 +1552,8 @@ int llmx_selftest_ar_timeout(llmx_ctx *c, uint32_t poll_limit) {
     return finish(c);
 }
 
-int llmx_selftest_serving_waits(uint32_t polls) {
+int llmx_selftest_serving_waits(uint32_t polls, uint32_t draw_ranks) {
+    g_serving_lost_draws.store(draw_ranks, std::memory_order_relaxed);
     g_serving_wait_polls.store(std::min(polls, kSpinLimit), std::memory_order_relaxed);
     return LLMX_OK;
 }

@@ -42,15 +42,18 @@
 
 namespace {
 
+using llmx::arrive_remote;
 using llmx::bulk_g2s;
 using llmx::bulk_g2s_hint;
 using llmx::cluster_arrive;
 using llmx::cluster_leave;
 using llmx::cluster_rank;
 using llmx::cluster_wait;
+using llmx::let_land;
 using llmx::mbar_arrive;
 using llmx::mbar_expect_tx;
 using llmx::mbar_init;
+using llmx::mbar_test_cluster;
 using llmx::mbar_wait;
 using llmx::mbar_wait_cluster;
 using llmx::pdl_trigger;
@@ -676,25 +679,27 @@ constexpr int kRuns = 8;
 constexpr uint32_t kKeep = 32;  // rows of a request whose numbers stay in shared memory
 struct DrawArgs {
     Args a;
-    int split;  // CTAs per request
+    int split;      // CTAs per request
+    uint32_t lose;  // by rank in the cluster: CTAs that give the others' sums up at once
 };
 
 // kModel: drafts have a distribution of their own.
 template <bool kModel>
 __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const Args &a = d.a;
-    __shared__ uint32_t first_s, bad_s, lost_s;  // lost: the other CTAs' sums did not come
+    __shared__ uint32_t first_s, bad_s, begin_s;
     __shared__ RowMass mass_s[kKeep][2], last_s[2];
     __shared__ unsigned long long warp_sum[kDrawWarps], cta_sum[2][kMaxCluster];
     __shared__ unsigned long long run_sum[kDrawWarps][kRuns];  // of up to kRuns runs of a warp's steps
     __shared__ uint64_t sums_full[2];                          // every CTA's sum of the round is there
+    __shared__ uint64_t lost[kMaxCluster];                     // a CTA of the cluster, by rank, did not get them
     const int S = d.split, rank = S > 1 ? (int)cluster_rank() : 0;
     const uint32_t b = blockIdx.x / S;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
     if (S > 1) {
         if (threadIdx.x == 0) {
             for (int i = 0; i < 2; i++) mbar_init(sums_full + i, 1);
+            for (int i = 0; i < S; i++) mbar_init(lost + i, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             for (int i = 0; i < 2; i++) mbar_expect_tx(sums_full + i, S * 8);
         }
@@ -709,7 +714,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     if (threadIdx.x == 0) {
         first_s = count;
         bad_s = valid ? 0u : 1u;
-        lost_s = 0;
+        begin_s = begin;
     }
     __syncthreads();
     const uint32_t targets = a.drafts + a.requests;
@@ -753,7 +758,7 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
     const RowMass mt = n < kKeep ? mass_s[n][0] : last_s[0], md = n < kKeep ? mass_s[n][1] : last_s[1];
     // one path for the whole cluster from here: all of it depends on the request alone
     uint32_t drawn = kNoToken;
-    bool bad = bad_s != 0;
+    bool bad = bad_s != 0, none = false;  // none: no token can be drawn
     if (S > 1) cluster_wait();
     if (!bad) {
         RowWeight wt, wd;
@@ -856,10 +861,9 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 if ((int)threadIdx.x < S)
                     st_async(remote(&cta_sum[round][rank], threadIdx.x), (uint64_t)cta, remote(&sums_full[round], threadIdx.x));
                 total = 0;
-                if (__syncthreads_or(!mbar_wait_cluster(&sums_full[round], 0, a.polls))) {
-                    lost_s = 1;  // the CTA's threads go on, or give up, as one
-                    bad = true;
-                    break;
+                if (__syncthreads_or(!mbar_wait_cluster(&sums_full[round], 0, d.lose >> rank & 1 ? 0 : a.polls))) {
+                    if ((int)threadIdx.x < S) arrive_remote(remote(lost + rank, threadIdx.x));
+                    break;  // the CTA's threads go on, or give up, as one
                 }
                 const unsigned long long of_cta = lane < S ? cta_sum[round][lane] : 0;
                 total = sum_lanes(of_cta);
@@ -904,21 +908,31 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
                 drawn = v + 32 * at + (uint32_t)__ffs((int)__ballot_sync(~0u, below + hit > point)) - 1;
                 break;
             }
-            if (lane == 0) out[n] = drawn;
-        } else if (total == 0 && rank == 0 && threadIdx.x == 0) {
-            out[n] = kNoToken;
         }
+        none = total == 0;
     } else if (S > 1) {
+        __syncthreads();  // (the others' part of this lies in the sums) no thread arrives before all have passed the last wait
         cluster_arrive();
     }
+    // no token is written before every CTA has said whether it got the sums: all of them write, or none
+    if (S > 1) {
+        __syncwarp();
+        cluster_wait();
+        if (__any_sync(~0u, lane < S && mbar_test_cluster(lost + lane, 0))) {
+            bad = true;
+            let_land();
+        }
+    }
+    uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
+    if (drawn != kNoToken && !bad && lane == 0) out[n] = drawn;
     if (rank == 0) {
+        const uint32_t from = *(const volatile uint32_t *)&begin_s;  // (begin would take a register until here)
         for (uint32_t j = threadIdx.x; j <= a.max_drafts; j += kDrawThreads) {
-            if (bad) out[j] = kNoToken;
-            else if (j != n) out[j] = j < n ? a.draft_tokens[begin + j] : kNoToken;
+            if (bad || (none && j == n)) out[j] = kNoToken;
+            else if (j != n) out[j] = j < n ? a.draft_tokens[from + j] : kNoToken;
         }
         if (threadIdx.x == 0) a.accepted[b] = bad ? kNoToken : n;
     }
-    if (S > 1) cluster_leave(lost_s == 0);
 }
 
 // CTAs per row that are considered: 9 and 6 fill a group of 18 SMs that cannot hold
@@ -1086,7 +1100,7 @@ extern "C" int llmx_verify_drafts(const int32_t *target, size_t ld_target, const
     configure(cfg, attr, dim3(groups * a.split), mass_threads(!a.resident), (size_t)a.ring * kChunkBytes, a.split, s);
     e = cudaLaunchKernelEx(&cfg, kMass[a.resident ? 0 : 1], a);
     if (e != cudaSuccess) return cuda_fail("k_mass", e);
-    DrawArgs d{a, 1};
+    DrawArgs d{a, 1, llmx::serving_lost_draws()};
     while (d.split < kMaxCluster && requests * d.split * 2 <= (uint32_t)dev.sms * 2 && vocab >= 2048u * d.split) d.split *= 2;
     configure(cfg, attr, dim3(requests * d.split), kDrawThreads, 0, d.split, s);
     e = cudaLaunchKernelEx(&cfg, a.draft ? k_draw<true> : k_draw<false>, d);

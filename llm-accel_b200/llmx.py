@@ -155,7 +155,7 @@ def lib():
             "llmx_allreduce_kind": (C.c_int, [vp]),
             "llmx_decode_fuses_o": (C.c_int, [vp]),
             "llmx_selftest_ar_timeout": (C.c_int, [vp, C.c_uint32]),
-            "llmx_selftest_serving_waits": (C.c_int, [C.c_uint32]),
+            "llmx_selftest_serving_waits": (C.c_int, [C.c_uint32, C.c_uint32]),
             "llmx_generate": (C.c_int, [vp, u32p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, vp, vp]),
         }
         if TIMELINE:
@@ -315,9 +315,10 @@ def lm_head_argmax_device(hidden_ptr, rows, hidden_size, lm_head_ptr, vocab, tok
                                             stream)
 
 
-def selftest_serving_waits(polls=None):
-    """Polls after which kernels of Adapters.project and verify_drafts give a wait up (None: the default)."""
-    check(lib().llmx_selftest_serving_waits(0xFFFFFFFF if polls is None else polls), "selftest_serving_waits")
+def selftest_serving_waits(polls=None, draw_ranks=0):
+    """Polls after which kernels of Adapters.project and verify_drafts give a wait up (None: the default),
+    and the CTAs of a request's draw, a bit each, that give up at once."""
+    check(lib().llmx_selftest_serving_waits(0xFFFFFFFF if polls is None else polls, draw_ranks), "selftest_serving_waits")
 
 
 class Adapters:

@@ -100,3 +100,29 @@ def test_sums_given_up_are_marked(llmx, torch, short, counts, vocab):
             d.call()
             gone = exact_or_given_up(torch, d)
             assert polls > 0 or gone == d.b
+
+
+@pytest.mark.parametrize("counts,vocab,ctas", [([3, 0, 2], 4000, 2), ([1] * 60, 4000, 2), ([0], 40000, 16), ([4], 151936, 16),
+                                               ([3, 0, 2], 50001, 16), ([0] * 30, 20000, 8), ([2] * 60, 60002, 4)])
+@pytest.mark.parametrize("model", [True, False])
+def test_draws_given_up_are_marked(llmx, torch, short, counts, vocab, ctas, model):
+    """A request of which any CTA lacks the others' sums has no tokens: neither a count without
+    its token nor one CTA's token beside another's mark."""
+    d = Device(llmx, torch, make(np.random.default_rng(vocab), counts, vocab, model=model))
+    for lost in (0, 1, 2, 3, 1 << (ctas - 1), (1 << ctas) - 1, (1 << ctas) - 2, 0x5555, 0xaaaa):
+        lost &= (1 << ctas) - 1
+        short(None, lost)
+        for _ in range(5):
+            d.accepted.fill_(777)
+            d.out.fill_(777)
+            d.call()
+            torch.cuda.synchronize()
+            if lost:
+                assert (d.accepted[:d.b] == -1).all() and (d.accepted[d.b:] == 777).all()
+                n = d.b * (d.c["most"] + 1)
+                assert (d.out[:n] == -1).all() and (d.out[n:] == 777).all()
+            else:
+                d.check()
+    short()
+    d.call()
+    d.check()
