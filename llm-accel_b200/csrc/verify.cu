@@ -393,20 +393,25 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
     // with many rows the draw's CTAs would only take room from the last of this kernel's
     if (!kTwice) pdl_trigger();
 
-    // every warp's end
+    // Every warp's end; true where a warp of the CTA gave up.  Where none did, all that was on its way
+    // to the CTA has been waited for.
     auto leave = [&](bool came) {
-        if (S == 1) return;
         __syncwarp();
-        cluster_arrive();
-        cluster_leave(came);
+        const bool lost = __syncthreads_or(!came);
+        if (S > 1) {
+            cluster_arrive();
+            cluster_leave(!lost);
+        }
+        return lost;
     };
     if (warp >= kLoad && warp < kLoad + 2) {  // ---- loads, of the first pass and of the second -----
+        int base = 0, ring = 1, issued = 0;
+        bool ok = true;
         if (lane == 0 && (kTwice || warp == kLoad)) {
-            const int base = warp == kLoad ? 0 : kFirstRing;
-            const int ring = !kTwice ? a.ring : warp == kLoad ? kFirstRing : a.ring - kFirstRing;
+            base = warp == kLoad ? 0 : kFirstRing;
+            ring = !kTwice ? a.ring : warp == kLoad ? kFirstRing : a.ring - kFirstRing;
             const uint64_t policy = llmx::evict_first_policy();
-            int s = 0, phase = 1, issued = 0;
-            bool ok = true;
+            int s = 0, phase = 1;
             for (uint32_t row = group; ok && row < a.total; row += groups) {
                 const Row r(a, row, rank);
                 for (uint32_t v = r.v0; v < r.v1; v += kChunk / 4) {
@@ -427,13 +432,12 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
                     }
                 }
             }
-            // the copies in flight land before the CTA ends, also where a warp that waits for them has given up
+        }
+        if (leave(ok))  // the copies in flight land before the CTA ends, which warp of it gave up ever
             for (int q = 0; q < ring && q < issued; q++) {
                 const int last = q + ((issued - 1 - q) / ring) * ring;
                 (void)mbar_wait(full + base + q, (last / ring) & 1);
             }
-        }
-        leave(true);
         return;
     }
     if (warp == kLoad + 2) {  // ---- the rows' temperatures --------------------------
@@ -487,8 +491,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         return __shfl_sync(~0u, old, 0) == n - 1;
     };
     auto arrive_all = [&](uint64_t *bar) {  // on this barrier of every CTA of the cluster
-        if (lane < S)
-            asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(bar, lane)) : "memory");
+        if (lane < S) arrive_remote(remote(bar, lane));
     };
     // (a slot whose chunk was not waited for to the end stays this warp's: it may still be filled)
     auto release = [&](int at) {
