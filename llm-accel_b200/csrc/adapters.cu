@@ -324,7 +324,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
     __shared__ __align__(16) int64_t sum_s[kWarps][kSums];  // [rank][row] of each warp
     __shared__ int64_t part_s[kMaxSplit][kSums];            // of each block, in the cluster's first
     __shared__ uint64_t part_bar;
-    __shared__ int16_t t_s[kGroup][16];
+    __shared__ __align__(16) int16_t t_s[kGroup][16];       // read as 32-bit words
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int vectors = c.K >> 3, all = kWarps * c.ksplit, part = share * kWarps + warp;
     const int from = c.steps * part / all, to = c.steps * (part + 1) / all;
