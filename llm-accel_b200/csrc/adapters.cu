@@ -347,6 +347,7 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
                 asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
                 mbar_expect_tx(&part_bar, c.ksplit * kSums * 8);
             }
+            __syncwarp();
             cluster_arrive();
         }
         // members: the next 8 rows of the mask from this one on
@@ -383,13 +384,16 @@ static __device__ void form_t(const Call &c, uint32_t row0, int q, int share) {
                       v);
         *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane]) = make_longlong2(v[0], v[1]);
         *reinterpret_cast<longlong2 *>(&sum_s[warp][2 * lane + 8 * kGroup]) = make_longlong2(v[2], v[3]);
-        __syncthreads();
+        if (c.ksplit > 1) {
+            __syncwarp();
+            cluster_wait();
+        }
+        __syncthreads();  // (also between this wait and the next arrival)
         int64_t sum = 0;
         if (threadIdx.x < kSums)
 #pragma unroll
             for (int w = 0; w < kWarps; w++) sum += sum_s[w][threadIdx.x];
         if (c.ksplit > 1) {
-            cluster_wait();
             if (threadIdx.x < kSums)
                 st_async(remote(&part_s[share][threadIdx.x], 0), (uint64_t)sum, remote(&part_bar, 0));
             __syncwarp();
@@ -830,9 +834,9 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                         for (int r = 0; r < 8; r++)
                             if (r < n) at[r * kOutTile] = 0;  // ready for the next call
                     }
-                    if (!live) continue;
                     const size_t first = ((size_t)k.rt * NT + r0) * c.ld_out + o;
-                    if (c.wide) {
+                    if (!live) {
+                    } else if (c.wide) {
                         int32_t *out = static_cast<int32_t *>(c.out) + first;
 #pragma unroll
                         for (int r = 0; r < 8; r++, out += c.ld_out)
@@ -843,6 +847,7 @@ __global__ void __launch_bounds__(project_threads(D), D == 8 ? 2 : 1) k_project(
                         for (int r = 0; r < 8; r++, out += c.ld_out)
                             if (r < n) *out = (int16_t)to_q8(to_q16(sum[r]));
                     }
+                    __syncwarp();  // the next loads from tensor memory are the whole warp's
                 }
             };
             rows8(false, !whole);

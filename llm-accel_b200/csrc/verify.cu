@@ -211,13 +211,13 @@ struct RowMass {
     int32_t shift;     // 22 + h
     int ok;
 };
-// From the parts of a row, by half a warp: its lanes hold a part each.
 // Sum over the warp, below 2^59: two 32-bit reductions take less than five rounds of
 // 64-bit shuffles.
 static __device__ __forceinline__ unsigned long long sum_lanes(unsigned long long v) {
     const uint32_t lo = __reduce_add_sync(~0u, (uint32_t)v & 0x7ffffffu), hi = __reduce_add_sync(~0u, (uint32_t)(v >> 27));
     return ((unsigned long long)hi << 27) + lo;
 }
+// From the parts of a row, by half a warp: its lanes hold a part each.
 static __device__ RowMass load_row(const RowPart *rows, uint32_t row, int split) {
     const int i = threadIdx.x & (kMaxCluster - 1);
     const RowPart *p = rows + row;
@@ -384,6 +384,7 @@ __global__ void __launch_bounds__(mass_threads(kTwice), 1) k_mass(const Args a) 
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (S > 1) {
+        __syncwarp();
         cluster_arrive();
         cluster_wait();
     } else {
