@@ -292,8 +292,8 @@ int llmx_decode_fuses_o(const llmx_ctx *ctx);
 int llmx_selftest_ar_timeout(llmx_ctx *ctx, uint32_t poll_limit);
 /* The same for the operators that serve several requests (llmx_adapters_project,
  * llmx_verify_drafts): calls of this process made from now on give a wait of their kernels up
- * after `polls` polls of about a microsecond (0: at once; UINT32_MAX: the default), except the
- * waits by which a kernel lets its own copies land before it ends.  draw_ranks: bit i makes CTA i of
+ * after `polls` polls of about a microsecond (0: some after one poll, and at once where results or
+ * a row's maximum are waited for, so that nothing succeeds; UINT32_MAX: the default), except the waits by which a kernel lets its own copies land before it ends.  draw_ranks: bit i makes CTA i of
  * a request's cluster give up at once when it waits for the other CTAs' sums of probabilities (0:
  * the default). */
 int llmx_selftest_serving_waits(uint32_t polls, uint32_t draw_ranks);

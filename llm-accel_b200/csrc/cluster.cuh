@@ -61,7 +61,8 @@ static __device__ __forceinline__ bool mbar_test_cluster(uint64_t *bar, uint32_t
         : "memory");
     return ok != 0;
 }
-static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, uint32_t polls = kSpinLimit) {
+static __device__ __forceinline__ bool mbar_wait_cluster(uint64_t *bar, uint32_t parity, uint32_t polls) {
+#pragma unroll 1
     for (uint32_t i = 0; i < polls; i++) {
         uint32_t ok;
         asm volatile(

@@ -36,14 +36,31 @@ static __device__ __forceinline__ bool mbar_try_wait(uint64_t *bar, uint32_t par
     return ok != 0;
 }
 // Bounded wait: false when the limit expired (the caller records an error).
-static __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32_t polls = kSpinLimit) {
-    for (uint32_t i = 0; i < polls; i++)
+static __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity) {
+    for (uint32_t i = 0; i < kSpinLimit; i++)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+// The same with a bound of its own, one poll at least.  The first look is not counted: with a
+// count before it, which is not a constant, 512 rows of the shared projection took 61.6 us, not 59.5.
+static __device__ __forceinline__ bool mbar_wait(uint64_t *bar, uint32_t parity, uint32_t polls) {
+    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (uint32_t i = 1; i < polls; i++)
         if (mbar_try_wait(bar, parity)) return true;
     return false;
 }
 // Bounded wait that also gives up as soon as any CTA has recorded an error.
-static __device__ __forceinline__ bool mbar_wait_err(uint64_t *bar, uint32_t parity, const int *err,
-                                                     uint32_t polls = kSpinLimit) {
+static __device__ __forceinline__ bool mbar_wait_err(uint64_t *bar, uint32_t parity, const int *err) {
+    for (uint32_t i = 0; i < kSpinLimit; i++) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if ((i & 255u) == 255u && *reinterpret_cast<const volatile int *>(err) != 0) return false;
+    }
+    return false;
+}
+// The same with a bound of its own.
+static __device__ __forceinline__ bool mbar_wait_err(uint64_t *bar, uint32_t parity, const int *err, uint32_t polls) {
+#pragma unroll 1
     for (uint32_t i = 0; i < polls; i++) {
         if (mbar_try_wait(bar, parity)) return true;
         if ((i & 255u) == 255u && *reinterpret_cast<const volatile int *>(err) != 0) return false;
