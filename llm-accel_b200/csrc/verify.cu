@@ -918,24 +918,28 @@ __global__ void __launch_bounds__(kDrawThreads, 2) k_draw(const DrawArgs d) {
         __syncthreads();  // (the others' part of this lies in the sums) no thread arrives before all have passed the last wait
         cluster_arrive();
     }
-    // no token is written before every CTA has said whether it got the sums: all of them write, or none
+    uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
+    if (rank == 0) {
+        const uint32_t from = *(const volatile uint32_t *)&begin_s;  // (begin would take a register until here)
+        for (uint32_t j = threadIdx.x; j <= a.max_drafts; j += kDrawThreads)
+            if (bad || j > n) out[j] = kNoToken;
+            else if (j < n) out[j] = a.draft_tokens[from + j];
+    }
+    // no count and no drawn token is written before every CTA has said whether it got the sums
     if (S > 1) {
         __syncwarp();
         cluster_wait();
         if (__any_sync(~0u, lane < S && mbar_test_cluster(lost + lane, 0))) {
+            if (rank == 0)
+                for (uint32_t j = threadIdx.x; j <= a.max_drafts; j += kDrawThreads) out[j] = kNoToken;
             bad = true;
             let_land();
         }
     }
-    uint32_t *out = a.tokens + (size_t)b * (a.max_drafts + 1);
     if (drawn != kNoToken && !bad && lane == 0) out[n] = drawn;
-    if (rank == 0) {
-        const uint32_t from = *(const volatile uint32_t *)&begin_s;  // (begin would take a register until here)
-        for (uint32_t j = threadIdx.x; j <= a.max_drafts; j += kDrawThreads) {
-            if (bad || (none && j == n)) out[j] = kNoToken;
-            else if (j != n) out[j] = j < n ? a.draft_tokens[from + j] : kNoToken;
-        }
-        if (threadIdx.x == 0) a.accepted[b] = bad ? kNoToken : n;
+    if (rank == 0 && threadIdx.x == 0) {
+        if (none && !bad) out[n] = kNoToken;
+        a.accepted[b] = bad ? kNoToken : n;
     }
 }
 
