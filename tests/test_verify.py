@@ -357,3 +357,53 @@ def test_refusals(llmx, kw, text):
 def test_workspace_grows_with_the_call(llmx):
     f = llmx.verify_workspace_bytes
     assert 0 < f(1, 0, 10) <= f(1, 7, 10) <= f(64, 448, 151936)
+
+
+@gpu
+@pytest.mark.parametrize("model", [True, False])
+@pytest.mark.parametrize("vocab", [501, 5000])
+def test_many_drafts_accepted(llmx, torch, vocab, model):
+    """More drafts accepted than the rows whose numbers stay in shared memory (32): all of them, then
+    a rejection at 31, 32, 33 and 39, sampled and greedy."""
+    rng = np.random.default_rng(12)
+    counts = [40] * 6 + [0, 33]
+    c = make(rng, counts, vocab, model, temperature=[0.8, 0.8, 0.8, 0.0, 0.0, 1.2, 1.0, 0.9])
+    off = [int(o) for o in c["offsets"]]
+    rows = [off[r] + r + j for r in range(len(counts)) for j in range(counts[r])]
+    c["tokens"] = np.argmax(c["target"][rows], 1).astype(np.uint32)
+    if model:
+        c["draft"] = c["target"][rows].copy()
+        c["accept_u"][:] = 2**32 - 1  # p = q is accepted whatever the number
+    else:
+        c["accept_u"][:] = 0
+    stop = {1: 31, 2: 32, 4: 33, 5: 39}
+    for r, j in stop.items():
+        c["target"][off[r] + r + j, c["tokens"][off[r] + j]] = NONE  # and so rejected
+    want = check(llmx, torch, c)
+    assert want[1].tolist() == [40, 31, 32, 40, 33, 39, 0, 33]
+
+
+@gpu
+def test_offsets_out_of_order_leave_the_others(llmx, torch):
+    """Beside requests with unusable offsets, those whose rows nobody else claims get their exact
+    tokens and probabilities."""
+    rng = np.random.default_rng(13)
+    c = make(rng, [2, 2, 2, 2], 300)
+    # offsets and the requests with usable ones that share no row
+    for bad, alone in (([0, 2, 1, 6, 8], [0, 3]), ([0, 2, 4, 99, 8], [0, 1]), ([0, 2**32 - 1, 4, 6, 8], [2, 3]), ([0, 8, 8, 8, 8], [1, 2, 3]),
+                       ([0, 2, 99, 6, 8], [0, 3])):
+        c["offsets"] = np.array(bad, np.uint32)
+        d = Device(llmx, torch, c)
+        d.call()
+        torch.cuda.synchronize()
+        want = S.verify(c["target"], c["draft"], c["tokens"], c["offsets"], c["most"], c["temperature"], c["accept_u"], c["sample_u"])
+        out, accepted = d.out.cpu().numpy()[:12].view(np.uint32).reshape(4, 3), d.accepted.cpu().numpy()[:4].view(np.uint32)
+        probs = d.probs.cpu().numpy()
+        for r in range(4):
+            if want[1][r] == S.NO_TOKEN:
+                assert accepted[r] == S.NO_TOKEN and (out[r] == S.NO_TOKEN).all()
+            elif r in alone:
+                assert accepted[r] == want[1][r] and np.array_equal(out[r], want[0][r])
+                for j in range(bad[r], bad[r + 1]):
+                    assert tuple(probs[j]) == want[2][j]
+        assert all(want[1][r] != S.NO_TOKEN for r in alone)
