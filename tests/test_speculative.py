@@ -119,3 +119,49 @@ def test_temperature_is_that_of_the_logits(llmx, untied):
     assert len(drawn) > 4
     sv.close()
     acc.close()
+
+
+def test_each_request_gets_its_own_adapter(llmx):
+    """Adapters that favour tokens of their own: each request's text is that of its slot's adapter,
+    with drafts (some accepted) as without, whichever request has which slot."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    model = llmx.Model(llmx.shape("small")).init_gaussian(11, lm_head=True)
+    s = model.shape
+
+    def adapter(token):
+        """Rank 1: t is some tens, of either sign, and lifts `token` or the next one far above the others."""
+        up = np.zeros((s.vocab, 1), np.int64)
+        up[token], up[token + 1] = 32767, -32767
+        return np.random.default_rng(token).integers(-2000, 2000, (1, s.hidden)), up
+
+    def expect(prompt, token, count):
+        """Greedy tokens of a request whose adapter is `token`'s (None: no adapter)."""
+        acc = llmx.Accelerator(s)
+        acc.upload_model(model)
+        ex = llmx.Executor(acc, model)
+        text = list(prompt)
+        hidden = ex.run_prompt_block(text, 0)[-1].astype(np.int64)
+        for _ in range(count):
+            y = model.lm_head().astype(np.int64) @ hidden
+            if token is not None:
+                down, up = adapter(token)
+                y = y + up @ np.clip((down @ hidden * 32767 + (1 << 23)) >> 24, -32768, 32767)
+            text.append(int(np.argmax(np.clip((y + 8) >> 4, -2**31, 2**31 - 1))))
+            hidden = ex.run_token(text[-1], len(text) - 1)[0].astype(np.int64)
+        acc.close()
+        return text[len(prompt):]
+
+    tokens = [7, 23]
+    plain = [expect(p, None, 14) for p in PROMPTS]
+    for drafts in (0, 4):
+        sv = spec.Server(model, 3, 2, 1, drafts)
+        for slot, token in enumerate(tokens):
+            sv.set_adapter(slot, 32767, *adapter(token))
+        for slots in ([0, -1, 1], [1, 0, -1], [-1, 1, 0]):
+            want = [expect(p, None if a < 0 else tokens[a], 14) for p, a in zip(PROMPTS, slots)]
+            assert all((w != q) == (a >= 0) for w, q, a in zip(want, plain, slots))  # an adapter changes the text
+            out, (drafted, taken) = sv.generate(PROMPTS, slots, 14)
+            assert out == want
+            assert (taken > 0) == (drafts > 0)
+        sv.close()
