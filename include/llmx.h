@@ -355,6 +355,8 @@ int llmx_lm_head_argmax_device(const int16_t *hidden, uint32_t rows, uint32_t hi
  * (golden_projection host:3105-3142): sat16(rnd8(sat32(rnd4(y)))) as Q8.8, or
  * only sat32(rnd4(y)) as Q16.16 (an LM head's logits).  The results are exact
  * integers: they do not depend on the number of rows, their order or the grid.
+ * t is a Q8.8 activation: against unrounded t, y is off by up to 2^-9 sum_j |up_a[n][j]|, t
+ * saturates at +-128, and an adapter with |scale_a down_a x| below 2^-9 adds nothing.
  * ------------------------------------------------------------------------- */
 typedef struct llmx_adapters llmx_adapters;
 #define LLMX_OUT_Q8_8 0   /* int16 rows */

@@ -11,9 +11,11 @@
 //
 // t is kept in the Q8.8 of every activation between two projections of the
 // path: with up_a in Q4.12 its product has the scale of W x, so the adapter is a
-// longer sum over k and nothing is rounded in between.  A row of rank 16 with
-// up values of 0.05 then differs by about 16^(1/2) * 0.05 * 2^-9 = 4e-4 from
-// one with unrounded t, a tenth of the Q8.8 result's own step.
+// longer sum over k and nothing is rounded in between.  Each t is off by up to 2^-9, so
+// a result by up to 2^-9 sum |up|, in the root mean square 2^-8 / 12^(1/2) (rank)^(1/2) |up|:
+// at rank 16 with up values of 0.05, 2e-4.  That is a twentieth of a Q8.8 result's step, but 15
+// of a Q16.16 one's: an adapter's part in logits is good to t's step, not to the format's.  t
+// saturates at +-128, and an adapter whose scaled down x stays below 2^-9 adds nothing.
 //
 // Tensor cores.  Both factors are split into bytes, as in mma_proj.cu: w = 256 wh
 // + wl (wl unsigned), x = 256 xh + xs + 128 with xs = (x & 255) - 128, so that

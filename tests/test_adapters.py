@@ -367,3 +367,26 @@ def test_refusals_leave_no_error_behind(llmx, torch):
         refuse(what)
         assert llmx.lm_head_argmax_device(few.data_ptr(), 8, 128, few.data_ptr(), 64, tokens.data_ptr(), c.stream()) == llmx.OK
         c.check(x, np.zeros(8), wide=True)
+
+
+def test_definition_is_the_adapter_in_real_numbers():
+    """Against W x + s B (A x) in 64 bits.  t is rounded to Q8.8, half a step of 2^-9 for each rank,
+    which up multiplies, and y to the format's step; that is the whole difference while t stays
+    within +-128.  A scaled A x below 2^-9 is a t of zero: the adapter then adds nothing."""
+    rng = np.random.default_rng(21)
+    k, n, rows, rank = 512, 60, 9, 16
+    x, w = whole(rng, (rows, k), 256), whole(rng, (n, k), 82)
+    down, up, scale = whole(rng, (rank, k), 82), whole(rng, (n, rank), 400), 5000
+    real = lambda a, bits: a.astype(np.float64) / 2.0**bits  # noqa: E731
+    t = real(x, 8) @ real(down, 12).T * (scale / 4096)
+    assert np.abs(t).max() < 128
+    y = real(x, 8) @ real(w, 12).T + t @ real(up, 12).T
+    off = 2.0**-9 * np.abs(real(up, 12)).sum(1)
+    for wide, bits in ((True, 16), (False, 8)):
+        got = S.project(x, w, np.zeros(rows, int), {0: (scale, down, up)}, wide).astype(np.float64) / 2.0**bits
+        # Q8.8 is rounded by way of Q16.16: half a step of each
+        step = 2.0**-(bits + 1) + (0 if wide else 2.0**-17)
+        assert (np.abs(got - y) <= off + step + 1e-9).all()
+    small = {0: (1, down, up)}  # s = 2^-12: |t| below 2^-9
+    assert np.abs(real(x, 8) @ real(down, 12).T / 4096).max() < 2.0**-9
+    assert np.array_equal(S.project(x, w, np.zeros(rows, int), small, True), S.project(x, w, None, {}, True))
