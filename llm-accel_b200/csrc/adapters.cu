@@ -45,15 +45,17 @@
 // What bounds it (B200, in graphs of calls over three sets of weights, which thus come
 // from HBM; bytes at 6.47 TB/s, exact products at a quarter of the int8 rate, which a
 // loop of such MMAs measured as 4.5 P/s).  Up to about 64 rows the weight stream: LM
-// head 151936 x 2048, 40 rows of 8 adapters, 110 us = 0.93 of the floor of 102 (adapters
-// of rank 8 are stored as pieces of 16: 20 MB more); Gate/Up 22016 x 2048, 16 rows of
-// 16 adapters, 26.2 us against 16.9, of which 5 pass before k_prepare's t is there and
-// the tail takes 2; 8 rows x 11008 -> 2048 15.4 against 7.1: 5 until t, 5 of stages,
-// 2.5 of adding parts up.  512 rows x 11008 x 2048 with rank 64: 57 us against 20.8 of
-// products: k_prepare 6, its end to the first product 5, then two whole tiles of 128
-// rows and a part of one: stages 0.72 us per 128 inputs (shared memory: 48 KB read by
-// the MMAs and 32 KB written per 64 inputs, at 128 bytes a cycle) and the results 3.5 a
-// tile.  One row x 2560 x 2048: 9.3 us, the two kernels' latencies.
+// head 151936 x 2048, 40 rows of 8 adapters, 110 to 116 us by machine (119 outside a graph, 0.86
+// of the floor of 102; adapters of rank 8 are stored as pieces of 16: 20 MB more); Gate/Up
+// 22016 x 2048, 16 rows of 16 adapters, 26.7 us against 16.9 (19.0 without adapters), of which
+// 5 pass before k_prepare's t is there and the tail takes 2; 8 rows x 11008 -> 2048 15.3
+// against 7.1 (13.6 without adapters): 5 until t, 5 of stages, 2.5 of adding parts up.
+// 512 rows x 11008 x 2048 with rank 64: 57 us against 20.8 of products (47 without adapters):
+// k_prepare 6, its end to the first product 5, then two whole tiles of 128 rows and a part of
+// one: stages 0.72 us per 128 inputs (by calculation shared memory: 48 KB read by the MMAs and 32 KB
+// written per 64 inputs, at 128 bytes a cycle; the tensor pipe is active half the time) and
+// the results 3.5 a tile.  One row x 2560 x 2048: 9.2 us, the two kernels' latencies (8.0
+// without an adapter).
 #include <cuda_runtime.h>
 
 #include <algorithm>

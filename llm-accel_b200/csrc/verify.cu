@@ -19,12 +19,19 @@
 // token, a cluster per request.
 //
 // What bounds it (B200, vocabulary of 151936, in graphs of calls over three sets of
-// inputs).  64 requests x 7 drafts with draft rows, 960 rows, 583 MB: 156 us against 90
-// for the bytes; k_mass 120 (0.64 GB read: second loads leave the L2 first; 19
-// instructions a logit of both passes, 0.69 a cycle and scheduler), k_draw 32 to 40 (78
-// MB, 0.61 instructions a cycle).  One request with 4 copied drafts: 10.9 us, latency: 4.6
-// in k_mass, then accept tests 1.5, sums 2.9, cluster totals 0.6, the token 1.0.
-// Simple kernels, a block per row and per request, took 862 and 194 us.
+// inputs; 156 to 164 us for the first by machine).  64 requests x 7 drafts with draft rows, 960 rows,
+// 583 MB: 156 us against 90 for the bytes; k_mass 120 (0.6 GB read: second loads leave the L2
+// first; 19 instructions a logit of both passes, 0.68 a cycle and scheduler), k_draw 32 to 40 (70
+// MB, 0.60 instructions a cycle).  64 requests without drafts: 36.8 us against 6, three passes over
+// a row, none of them at a limit of the machine (under ncu 20.5 in k_mass and 24.5 in
+// k_draw, 0.48 and 0.57 instructions a cycle, DRAM at a fifth).  One request with 4 copied
+// drafts: 11.6 us, latency: 4.8 in k_mass, then accept tests 1.5, sums 2.9, cluster totals
+// 0.6, the token 1.0, the cluster's end 0.3.  Simple kernels, a block per row and per request, took 862 and 194 us.
+//
+// Waits are bounded.  A warp that gives one up takes part in nothing after it: no maximum, sum or
+// slot is passed on from it, so whatever needs them gives up as well, and a row or
+// request is either exact or marked.  CTAs end when their copies have landed and their cluster
+// sends nothing more (0.3 to 0.9 us of a call).
 #include <cuda_runtime.h>
 
 #include <algorithm>
