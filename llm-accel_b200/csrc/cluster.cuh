@@ -25,14 +25,15 @@ static __device__ __forceinline__ uint32_t remote(const void *p, uint32_t rank) 
 // fence.mbarrier_init), nothing is sent before cluster_wait.
 static __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
 static __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// For the exchange's end, after a cluster_arrive by every thread of the cluster once it sends
-// nothing more (and once every thread of its CTA has passed the cluster_wait before): no CTA's shared memory goes while another may still address it.  came: this
-// thread got all that it waited for.  If not, something may have been sent just now that nobody
-// waits for any more; it is given time to land (some 100 us, hundreds of times what it takes).
+// Time for what nobody waits for any more to land: some 100 us, hundreds of times what it takes.
 static __device__ __forceinline__ void let_land() {
     for (const long long t = clock64(); clock64() - t < 200000;) {
     }
 }
+// The exchange's end, after a cluster_arrive by every thread of the cluster once it sends nothing
+// more and every thread of its CTA has passed the cluster_wait before: no CTA's shared memory
+// goes while another may still address it.  came: this thread got all that it waited for; if
+// not, something may have been sent just now.
 static __device__ __forceinline__ void cluster_leave(bool came) {
     __syncwarp();
     cluster_wait();

@@ -390,3 +390,13 @@ def test_definition_is_the_adapter_in_real_numbers():
     small = {0: (1, down, up)}  # s = 2^-12: |t| below 2^-9
     assert np.abs(real(x, 8) @ real(down, 12).T / 4096).max() < 2.0**-9
     assert np.array_equal(S.project(x, w, np.zeros(rows, int), small, True), S.project(x, w, None, {}, True))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [1000, 4097, 65536])
+def test_hundreds_of_row_tiles(llmx, torch, rows):
+    c = Case(llmx, torch, 64, 130, [16, 5, 20], rows)
+    x = whole(c.rng, (rows, 64), 900)
+    c.check(x, c.rng.integers(-1, 3, rows), wide=True)
+    c.check(x, None, wide=False)
+    c.check(x[:17], np.arange(17) % 3, wide=True)
