@@ -454,6 +454,104 @@ int llmx_verify_drafts(const int32_t *target, size_t ld_target, const int32_t *d
                        size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------
+ * Log probabilities of given tokens, their rank, the rows' entropy and the most likely tokens (no
+ * counterpart in the reference, which takes the maximum only).  For a row z of Q16.16 logits
+ * at temperature T, with d_v = (max z - z_v) / (2^16 T) and rest = the sum of exp(-d_v) over all
+ * tokens but one maximum:
+ *   logprob(v) = -d_v - log1p(rest)
+ *   entropy    = log1p(rest) + sum of d_v exp(-d_v) / (1 + rest)            nats
+ *   rank(v)    = the number of tokens ahead of v in the order (logit down, index up)
+ * INT32_MIN excludes a token; T <= 1e-6 (or NaN) leaves the first maximum alone (its log probability
+ * is 0, all others' -infinity, the entropy 0).  Terms are binary32 with whole-number
+ * differences, added in a fixed order (16 at a time, a lane's and a warp's sums in binary32, those
+ * of a row in binary64), the formulas binary64: results are within 4e-7 of the
+ * entropy and max(1, |logprob|), and do not depend on the rows beside them in more than that.
+ * ------------------------------------------------------------------------- */
+/* Bytes of workspace for a call of these sizes. */
+size_t llmx_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top);
+/*   logits        device, int32 rows ld elements apart (0 = vocab), of any alignment
+ *   vocab         1 to 2^22; rows: 0 to 2^20; top: 0 to 32
+ *   tokens        device, a token per row, or NULL; one that is excluded or outside the vocabulary has
+ *                 log probability -infinity and rank 0xffffffff
+ *   temperature   device, float per row, or NULL = 1
+ *   logprob, rank device, [rows] (not used without tokens); entropy device, [rows]
+ *   top_tokens, top_logprobs  device, [rows][top]: the most likely tokens in order, then
+ *                 0xffffffff and -infinity where fewer are not excluded (not used when top is 0)
+ *   workspace     device, 256-byte aligned, llmx_logprobs_workspace_bytes of the same sizes (or
+ *                 larger ones); one call at a time may use it
+ * Runs on the current device, stream-ordered; allocates nothing and may be captured into a graph. */
+int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vocab, uint32_t rows, const uint32_t *tokens,
+                        const float *temperature, uint32_t top, float *logprob, uint32_t *rank, float *entropy,
+                        uint32_t *top_tokens, float *top_logprobs, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* ---------------------------------------------------------------------------
+ * A key-value cache in pages, shared by many requests (no counterpart in the
+ * reference, whose cache is one sequence's).  The caller owns the pages, one pair of
+ * arrays per layer:
+ *   k, v    device, int16 [pages][kv_heads][page_len][head_dim], Q8.8, 16-byte aligned
+ *   table   device, int32 [requests][ld_table]: entry i of a request's row names the page of
+ *           its positions i * page_len and on; entries that no position uses may hold anything.
+ *           Requests may share pages that nothing is appended to
+ * and describes a step by the same two arrays for both operators:
+ *   offsets device, uint32 [requests + 1], ascending: request b's n_b rows are rows offsets[b]
+ *           to offsets[b+1] - 1
+ *   lengths device, uint32 [requests]: positions of request b with this step's rows, so
+ *           that its row j is at position lengths[b] - n_b + j (in front of the sequence if negative)
+ * Rows of no request (before offsets[0], behind offsets[requests]) are left as they are.
+ * Results are the resident path's (Task 18), bit for bit, whatever the pages and other requests.
+ * ------------------------------------------------------------------------- */
+typedef struct llmx_paged llmx_paged;
+/* Reserves the workspace of attention calls: heads (1 to 1024, a multiple of kv_heads), head_dim
+ * (a multiple of 16 up to 128), page_len (a multiple of 8 up to 65536); at most max_requests
+ * (1 to 1024) requests of max_block (1 to 8) rows, max_length (1 to 2^20) positions each
+ * and max_positions together.  heads / kv_heads * max_block is at most 128.  One handle
+ * serves every layer of these sizes. */
+int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_len,
+                      uint32_t max_requests, uint32_t max_block, uint32_t max_length, uint64_t max_positions,
+                      void *stream, llmx_paged **out);
+int llmx_paged_destroy(llmx_paged *p);
+/* Rotates the queries and keys of rows [heads queries | kv_heads keys | kv_heads values] by their
+ * positions (rotate_fix16_pair_with_quantized_rope host:4765-4788) and puts keys and
+ * values into the pages.  Any number of rows per request; stream-ordered, allocates nothing,
+ * may be captured into a graph.
+ *   qkv   device, int16 rows ld_qkv elements apart (0 = (heads + 2 kv_heads) * head_dim, else a
+ *         multiple of 8), 16-byte aligned: what a projection by [Q; K; V] gives
+ *   rope  device, int16 [positions][head_dim]: cos half | sin half, Q8.8 (llmx_rope_table),
+ *         16-byte aligned
+ *   q     device, the rotated queries, rows ld_q elements apart (0 = heads * head_dim, else a
+ *         multiple of 8), 16-byte aligned; may be qkv itself with the same stride
+ * A row in front of its sequence is left out.  A row whose position has no table entry or rope
+ * row, or whose page number is outside [0, pages), is left out and reported by
+ * llmx_paged_error.  Two rows of a call must not have the same place in the pages. */
+int llmx_paged_append(llmx_paged *p, const int16_t *qkv, uint32_t rows, size_t ld_qkv, const uint32_t *offsets,
+                      const uint32_t *lengths, uint32_t requests, const int16_t *rope, uint32_t positions,
+                      const int32_t *table, size_t ld_table, int16_t *k, int16_t *v, uint32_t pages, int16_t *q,
+                      size_t ld_q, void *stream);
+/* Attention of the requests' rows over their pages: the tile-exact Q2.14 online softmax of Task
+ * 18 (golden_tiled_flash_attention_q2_14_impl host:3610-3739).  A row sees the positions up to its
+ * own; one in front of its sequence sees none and gives zeros.  Stream-ordered, allocates
+ * nothing, may be captured into a graph.
+ *   q, out   device, int16 rows [heads][head_dim], ld_q and ld_out elements apart (0 = heads *
+ *            head_dim, else a multiple of 8), 16-byte aligned
+ *   longest  no request is longer (0 = max_length); ld_table has to hold that many positions
+ * A request whose offsets are out of order, outside [0, rows] or more than max_block
+ * apart, or that is longer than `longest`, is left out and reported by llmx_paged_error (rows that
+ * others claim as well are unspecified); so is the whole call when the lengths add up to more than max_positions allows (each rounded
+ * up to 64).  A page number outside [0, pages) makes its request's rows void and is reported.
+ * The handle's workspace is shared by its calls: order attention calls that use one handle on
+ * one stream or with events (captured graphs too). */
+int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t rows, size_t ld_q, const uint32_t *offsets,
+                         const uint32_t *lengths, uint32_t requests, uint32_t longest, const int32_t *table,
+                         size_t ld_table, const int16_t *k, const int16_t *v, uint32_t pages, int16_t *out,
+                         size_t ld_out, void *stream);
+/* Waits for the stream and returns LLMX_ERR_RANGE if a call of this handle met something out of
+ * range since the last such call, else LLMX_OK. */
+int llmx_paged_error(llmx_paged *p, void *stream);
+/* Bytes of device memory the handle holds. */
+uint64_t llmx_paged_device_bytes(const llmx_paged *p);
+
+/* ---------------------------------------------------------------------------
  * Host runtime: qwen_executor_t host:7607-8161
  * ------------------------------------------------------------------------- */
 /* run_prompt_block host:7840-7918: embedding rows of 1..8 tokens at

@@ -1,0 +1,470 @@
+// Log probabilities of given tokens, with their rank, the rows' entropy and the most
+// likely tokens, from Q16.16 logits.
+//
+// No counterpart in the LLM-ACCEL tree: its host takes the maximum only (lm_head_argmax,
+// host/host_qwen_8x64.cpp:937-977).  For a row z at temperature T, with m its maximum
+// and d_v = (m - z_v) / (2^16 T):
+//   rest = sum of exp(-d_v) over all tokens but one maximum
+//   logprob(v) = -d_v - log1p(rest)
+//   entropy    = log1p(rest) + sum of d_v exp(-d_v) / (1 + rest)
+// so that nothing cancels where one token has nearly all the probability.
+//
+// Two launches.  k_rows reads the logits once.  All rows are one line of chunks of 512 logits, cut
+// into equal runs, a run per warp; for every row that its run touches a warp leaves a
+// part: the maximum, both sums relative to it (binary32, of 16 terms at a time), the tokens
+// ahead of the given one and its best tokens in order.  k_rows_join adds up a row's parts, in
+// binary64 and in order, so a result depends on no timing.
+//
+// The best tokens: a warp holds them in order, one a lane, as 64-bit keys (logit, then the
+// lower index), and passes over chunks whose maximum does not exceed the least of them.
+// Others' logits above that go to a buffer in shared memory; 32 of them are sorted over the lanes and
+// merged at a time, so that even rising logits cost a few instructions each.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "llmx.h"
+#include "device_util.cuh"
+#include "kernels.cuh"
+
+namespace {
+
+using llmx::pdl_trigger;
+using llmx::pdl_wait;
+
+constexpr int kExcluded = INT_MIN;
+constexpr uint32_t kNone = 0xffffffffu;
+constexpr uint32_t kMaxVocab = 1u << 22, kMaxRows = 1u << 20, kMaxTop = 32;
+constexpr float kMinTemperature = 1e-6f;  // at or below: the first maximum alone
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kChunk = 512;               // logits: four 16-byte loads a lane
+constexpr uint32_t kMaxCtas = 592;        // of k_rows: four on each of 148 SMs
+
+// What a warp leaves of a row; its best tokens follow.
+struct Part {
+    int32_t top;      // maximum; kExcluded: nothing but excluded tokens
+    uint32_t ahead;   // tokens ahead of the given one
+    float rest, sum;  // of exp(-d) and of log2(e) d exp(-d), without one maximum
+};
+
+struct Call {
+    const int32_t *logits;
+    size_t ld;
+    uint32_t vocab, rows, top;
+    const uint32_t *tokens;
+    const float *temperature;
+    float *logprob;
+    uint32_t *rank;
+    float *entropy;
+    uint32_t *top_tokens;
+    float *top_logprobs;
+    unsigned char *parts;  // [slots] of part_bytes
+    uint32_t part_bytes;
+    uint32_t chunks;       // of a row
+    uint32_t per;          // chunks a warp
+};
+
+// Parts of a warp's rows lie one after another, and those of a row's warps too: warp w's part
+// of row r is slot w + r, and on the way from one to the next either w or r grows by one.
+static __device__ __forceinline__ unsigned char *part_at(const Call &c, unsigned long long slot) { return c.parts + slot * c.part_bytes; }
+
+static __device__ __forceinline__ bool is_greedy(float t) { return !(t > kMinTemperature); }
+
+static __device__ __forceinline__ unsigned long long key_of(int z, uint32_t token) {
+    return (unsigned long long)((uint32_t)z ^ 0x80000000u) << 32 | (kNone - token);
+}
+static __device__ __forceinline__ int logit_of(unsigned long long key) { return (int)((uint32_t)(key >> 32) ^ 0x80000000u); }
+
+static __device__ __forceinline__ unsigned long long shfl64(unsigned long long v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+
+// One step of a sorting network: lanes whose index has `bit` clear keep the larger of the two
+// (down) or the smaller.
+static __device__ __forceinline__ unsigned long long step64(unsigned long long v, int bit, bool down) {
+    const unsigned long long o = shfl64(v, bit);
+    const bool first = (threadIdx.x & bit) == 0;
+    return (first == down) == (o > v) ? o : v;
+}
+// 32 keys over the lanes, sorted from the largest.
+static __device__ __forceinline__ unsigned long long sort64(unsigned long long v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
+        for (int bit = size / 2; bit; bit /= 2) v = step64(v, bit, (lane & size) == 0 || size == 32);
+    return v;
+}
+// The 32 largest of two sorted lists, sorted.
+static __device__ __forceinline__ unsigned long long merge64(unsigned long long a, unsigned long long b) {
+    const unsigned long long r = __shfl_sync(0xffffffffu, b, 31 - (threadIdx.x & 31));
+    unsigned long long v = a > r ? a : r;
+#pragma unroll
+    for (int bit = 16; bit; bit /= 2) v = step64(v, bit, true);
+    return v;
+}
+
+// The best keys that a warp has met.
+struct Best {
+    unsigned long long list;  // sorted over the lanes; 0: none
+    unsigned long long *buf;  // [64] in shared memory, the warp's own
+    int count;                // in it
+    uint32_t top;
+
+    __device__ void start(unsigned long long *buffer, uint32_t n) {
+        list = 0;
+        buf = buffer;
+        count = 0;
+        top = n;
+    }
+    // The least key of the list: what does not exceed it stays out.
+    __device__ unsigned long long least() const { return __shfl_sync(0xffffffffu, list, (int)top - 1); }
+    __device__ void flush() {
+        const int lane = threadIdx.x & 31;
+        __syncwarp();
+        const unsigned long long k = lane < count ? buf[lane] : 0;
+        const unsigned long long rest = lane + 32 < count ? buf[lane + 32] : 0;
+        __syncwarp();
+        if (lane + 32 < count) buf[lane] = rest;
+        count = max(count - 32, 0);
+        list = merge64(list, sort64(k));
+    }
+    // By all lanes; `in`: this lane's key belongs in.
+    __device__ void push(bool in, unsigned long long key) {
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (!who) return;
+        if (in) buf[count + __popc(who & ((1u << (threadIdx.x & 31)) - 1))] = key;
+        count += __popc(who);
+        if (count >= 32) flush();
+    }
+    __device__ void finish() {
+        while (count > 0) flush();
+    }
+};
+
+// Logits i0 + 128 j + 4 lane .. + 3 of a row, excluded ones in place of those that are not there;
+// wide: the row's elements with an index that is 0 mod 4 are 16-byte aligned.
+static __device__ __forceinline__ void load(const int32_t *row, uint32_t vocab, uint32_t i0, bool wide, int (&z)[16]) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t i = i0 + 128 * j + 4 * (threadIdx.x & 31);
+        if (wide && i + 3 < vocab) {
+            asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
+                         : "=r"(z[4 * j]), "=r"(z[4 * j + 1]), "=r"(z[4 * j + 2]), "=r"(z[4 * j + 3])
+                         : "l"(row + i)
+                         : "memory");
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                z[4 * j + k] = kExcluded;
+                if (i + k < vocab) z[4 * j + k] = __ldcg(row + i + k);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
+    __shared__ unsigned long long buffers[kWarps][64];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_trigger();
+    const unsigned long long w = (unsigned long long)blockIdx.x * kWarps + warp;
+    const unsigned long long all = (unsigned long long)c.chunks * c.rows;
+    const unsigned long long begin = w * c.per, end = min(begin + c.per, all);
+    if (begin >= all) return;
+    Best best;
+    uint32_t r = (uint32_t)(begin / c.chunks), chunk = (uint32_t)(begin - (unsigned long long)r * c.chunks);
+    int next[16];
+    auto fetch = [&](uint32_t row, uint32_t at) {
+        const int32_t *p = c.logits + (size_t)row * c.ld;
+        load(p, c.vocab, at * kChunk, ((uintptr_t)p & 15u) == 0, next);
+    };
+    fetch(r, chunk);
+    for (unsigned long long at = begin; at < end;) {
+        // one row's share of the run
+        const uint32_t share = (uint32_t)min((unsigned long long)(c.chunks - chunk), end - at);
+        const float temperature = c.temperature ? c.temperature[r] : 1.0f;
+        const bool greedy = is_greedy(temperature);
+        // log2(e) / 2^16 / T in two parts: a rounded one alone would turn all terms the same way
+        const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
+        const float s_hi = (float)scale, s_lo = (float)(scale - (double)s_hi);
+        const uint32_t token = c.tokens ? c.tokens[r] : kNone;
+        const int mine = token < c.vocab ? __ldcg(c.logits + (size_t)r * c.ld + token) : kExcluded;
+        int m = kExcluded;  // of the warp
+        int least = kExcluded;
+        float rest = 0, sum = 0;
+        uint32_t ahead = 0;
+        best.start(buffers[warp], c.top);
+        for (uint32_t n = 0; n < share; n++, at++) {
+            int z[16];
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[i] = next[i];
+            const uint32_t i0 = chunk * kChunk + 4 * lane;
+            if (++chunk == c.chunks) {
+                chunk = 0;
+                r++;
+            }
+            if (at + 1 < end) fetch(r, chunk);
+            int most = z[0];
+#pragma unroll
+            for (int i = 1; i < 16; i++) most = max(most, z[i]);
+            const int top = __reduce_max_sync(0xffffffffu, most);
+            if (top == kExcluded) continue;
+            int skip = -1;  // the maximum that is left out of the sums
+            if (top > m) {
+                if (!greedy && m != kExcluded) {  // the old maximum becomes an ordinary token
+                    const float d = (float)((uint32_t)top - (uint32_t)m);
+                    const float e = fmaf(d, s_hi, d * s_lo);
+                    const float f = exp2f(-e);
+                    if (lane == 0) rest += 1.0f;  // (it is 0 away from itself)
+                    sum = f * fmaf(rest, e, sum);
+                    rest *= f;
+                }
+                m = top;
+                const uint32_t who = __ballot_sync(0xffffffffu, most == top);
+                if (lane == __ffs(who) - 1) {
+#pragma unroll
+                    for (int i = 15; i >= 0; i--)
+                        if (z[i] == top) skip = i;
+                }
+            }
+            if (!greedy) {
+                float r16 = 0, s16 = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float d = (float)((uint32_t)m - (uint32_t)z[i]);
+                    const float e = fmaf(d, s_hi, d * s_lo);
+                    float x;
+                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(-e));
+                    if (z[i] == kExcluded || i == skip) x = 0;
+                    r16 += x;
+                    s16 = fmaf(x, e, s16);
+                }
+                rest += r16;
+                sum += s16;
+            }
+            if (mine != kExcluded && top >= mine) {
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const uint32_t v = i0 + 128 * (i / 4) + i % 4;
+                    ahead += z[i] > mine || (z[i] == mine && v < token);
+                }
+            }
+            if (c.top && top > least) {
+                int bound = least;
+                if (least == kExcluded) {  // the first chunk: the top-th of the lanes' maxima bounds from below
+                    const unsigned long long k = sort64(key_of(most, 0));
+                    const int t = logit_of(__shfl_sync(0xffffffffu, k, (int)c.top - 1));
+                    bound = t == kExcluded ? t : t - 1;
+                }
+#pragma unroll
+                for (int i = 0; i < 16; i++) best.push(z[i] > bound, key_of(z[i], i0 + 128 * (i / 4) + i % 4));
+                best.finish();
+                const unsigned long long k = best.least();
+                least = k ? logit_of(k) : kExcluded;
+            }
+        }
+        ahead = __reduce_add_sync(0xffffffffu, ahead);
+#pragma unroll
+        for (int o = 16; o; o /= 2) {
+            rest += __shfl_xor_sync(0xffffffffu, rest, o);
+            sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        const uint32_t row = chunk == 0 ? r - 1 : r;
+        unsigned char *part = part_at(c, w + row);
+        if (lane == 0) *reinterpret_cast<Part *>(part) = Part{m, ahead, rest, sum};
+        if (lane < (int)c.top) reinterpret_cast<unsigned long long *>(part + sizeof(Part))[lane] = best.list;
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
+    __shared__ unsigned long long buffers[kWarps][64];
+    __shared__ unsigned long long lists[kWarps][32];
+    __shared__ int tops[kWarps], holders[kWarps];
+    __shared__ double rests[kWarps], sums[kWarps];
+    __shared__ uint32_t aheads[kWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait();
+    pdl_trigger();
+    const uint32_t r = blockIdx.x;
+    // the warps of k_rows that had a share of this row
+    const unsigned long long first = (unsigned long long)r * c.chunks / c.per, last = ((unsigned long long)(r + 1) * c.chunks - 1) / c.per;
+    const int parts = (int)(last - first + 1);
+    const float temperature = c.temperature ? c.temperature[r] : 1.0f;
+    const bool greedy = is_greedy(temperature);
+    const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
+
+    int m = kExcluded;
+    for (int i = threadIdx.x; i < parts; i += kThreads) m = max(m, reinterpret_cast<const Part *>(part_at(c, first + i + r))->top);
+    m = __reduce_max_sync(0xffffffffu, m);
+    if (lane == 0) tops[warp] = m;
+    __syncthreads();
+    for (int i = 0; i < kWarps; i++) m = max(m, tops[i]);
+    // one maximum stays out of the sums: that of the first part which holds it
+    int holder = INT_MAX;
+    for (int i = threadIdx.x; i < parts && holder == INT_MAX; i += kThreads)
+        if (reinterpret_cast<const Part *>(part_at(c, first + i + r))->top == m) holder = i;
+    holder = __reduce_min_sync(0xffffffffu, holder);
+    if (lane == 0) holders[warp] = holder;
+    __syncthreads();
+    for (int i = 0; i < kWarps; i++) holder = min(holder, holders[i]);
+    double rest = 0, sum = 0;
+    uint32_t ahead = 0;
+    for (int i = threadIdx.x; i < parts; i += kThreads) {
+        const Part p = *reinterpret_cast<const Part *>(part_at(c, first + i + r));
+        ahead += p.ahead;
+        if (p.top == kExcluded || greedy) continue;
+        if (i == holder) {
+            rest += (double)p.rest;
+            sum += (double)p.sum;
+        } else {
+            const double e = (double)((uint32_t)m - (uint32_t)p.top) * scale, f = exp2(-e), with = (double)p.rest + 1.0;
+            rest += f * with;
+            sum += f * ((double)p.sum + with * e);
+        }
+    }
+    Best best;
+    best.start(buffers[warp], c.top);
+    if (c.top) {
+        // this warp's parts: warp, warp + kWarps, ...; their best tokens bound the list from below
+        unsigned long long k = 0;
+        if (warp + kWarps * lane < parts)
+            k = reinterpret_cast<const unsigned long long *>(part_at(c, first + warp + kWarps * lane + r) + sizeof(Part))[0];
+        k = __shfl_sync(0xffffffffu, sort64(k), (int)c.top - 1);
+        unsigned long long bound = k ? k - 1 : 0;
+        for (int i = warp; i < parts; i += kWarps) {
+            const unsigned long long *list = reinterpret_cast<const unsigned long long *>(part_at(c, first + i + r) + sizeof(Part));
+            const unsigned long long key = lane < (int)c.top ? list[lane] : 0;
+            best.push(key > bound, key);
+            bound = max(bound, best.least());
+        }
+        best.finish();
+    }
+#pragma unroll
+    for (int o = 16; o; o /= 2) {
+        rest += __shfl_xor_sync(0xffffffffu, rest, o);
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    lists[warp][lane] = best.list;
+    if (lane == 0) {
+        rests[warp] = rest;
+        sums[warp] = sum;
+        aheads[warp] = ahead;
+    }
+    __syncthreads();
+    if (warp != 0) return;
+    rest = sum = 0;
+    ahead = 0;
+    for (int i = 0; i < kWarps; i++) {
+        rest += rests[i];
+        sum += sums[i];
+        ahead += aheads[i];
+    }
+    unsigned long long list = best.list;
+    if (c.top)
+        for (int i = 1; i < kWarps; i++) list = merge64(list, lists[i][lane]);
+    const double log_sum = log1p(rest), step = greedy ? 0.0 : 1.0 / (65536.0 * (double)temperature);
+    // of a token that is not excluded
+    auto logprob = [&](int z, bool ahead_of_all) -> float {
+        if (greedy) return ahead_of_all ? 0.0f : -INFINITY;
+        return (float)(-(double)((uint32_t)m - (uint32_t)z) * step - log_sum);
+    };
+    if (lane == 0) {
+        if (c.tokens) {
+            const uint32_t token = c.tokens[r];
+            const int z = token < c.vocab ? __ldcg(c.logits + (size_t)r * c.ld + token) : kExcluded;
+            c.logprob[r] = z == kExcluded ? -INFINITY : logprob(z, ahead == 0);
+            c.rank[r] = z == kExcluded ? kNone : ahead;
+        }
+        c.entropy[r] = greedy || m == kExcluded ? 0.0f : (float)(log_sum + 0.6931471805599453 * sum / (1.0 + rest));
+    }
+    if (lane < (int)c.top) {
+        c.top_tokens[(size_t)r * c.top + lane] = list ? kNone - (uint32_t)list : kNone;
+        c.top_logprobs[(size_t)r * c.top + lane] = list ? logprob(logit_of(list), lane == 0) : -INFINITY;
+    }
+}
+
+uint32_t part_bytes(uint32_t top) { return (uint32_t)sizeof(Part) + 8 * ((top + 1) / 2 * 2); }
+uint64_t chunks_of(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + kChunk - 1) / kChunk); }
+
+int fail(int code, const std::string &msg) {
+    llmx::set_last_error("token_logprobs: " + msg);
+    return code;
+}
+int cuda_fail(const char *what, cudaError_t e) {
+    (void)cudaGetLastError();
+    return fail(LLMX_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
+}
+
+cudaError_t launch(const void *fn, unsigned grid, const Call &call, cudaStream_t s) {
+    Call copy = call;
+    void *args[] = {&copy};
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelExC(&cfg, fn, args);
+}
+
+}  // namespace
+
+extern "C" size_t llmx_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top) {
+    const uint64_t warps = std::min<uint64_t>(chunks_of(rows, vocab), (uint64_t)kMaxCtas * kWarps);
+    return ((warps + rows) * part_bytes(std::min(top, kMaxTop)) + 255) / 256 * 256;
+}
+
+extern "C" int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vocab, uint32_t rows, const uint32_t *tokens,
+                                   const float *temperature, uint32_t top, float *logprob, uint32_t *rank, float *entropy,
+                                   uint32_t *top_tokens, float *top_logprobs, void *workspace, size_t workspace_bytes,
+                                   void *stream) {
+    if (vocab == 0 || vocab > kMaxVocab) return fail(LLMX_ERR_ARG, "vocab must be 1..2^22, got " + std::to_string(vocab));
+    if (rows > kMaxRows) return fail(LLMX_ERR_ARG, "rows must be at most 2^20, got " + std::to_string(rows));
+    if (top > kMaxTop) return fail(LLMX_ERR_ARG, "top must be at most 32, got " + std::to_string(top));
+    if (ld == 0) ld = vocab;
+    if (ld < vocab) return fail(LLMX_ERR_ARG, "the row stride is smaller than vocab");
+    if (rows == 0) return LLMX_OK;
+    if (!logits || !entropy || !workspace) return fail(LLMX_ERR_ARG, "null pointer");
+    if (tokens && (!logprob || !rank)) return fail(LLMX_ERR_ARG, "null pointer with tokens");
+    if (top && (!top_tokens || !top_logprobs)) return fail(LLMX_ERR_ARG, "null pointer with top > 0");
+    if (((uintptr_t)logits | (uintptr_t)tokens | (uintptr_t)temperature | (uintptr_t)logprob | (uintptr_t)rank | (uintptr_t)entropy |
+         (uintptr_t)top_tokens | (uintptr_t)top_logprobs) & 3u)
+        return fail(LLMX_ERR_ARG, "a pointer is not aligned to its element");
+    if ((uintptr_t)workspace & 255u) return fail(LLMX_ERR_ARG, "workspace must be 256-byte aligned");
+    if (workspace_bytes < llmx_logprobs_workspace_bytes(rows, vocab, top))
+        return fail(LLMX_ERR_ARG, "workspace too small: " + std::to_string(workspace_bytes) + " bytes");
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e != cudaSuccess) return cuda_fail("device", e);
+    Call c{};
+    c.logits = logits;
+    c.ld = ld;
+    c.vocab = vocab;
+    c.rows = rows;
+    c.top = top;
+    c.tokens = tokens;
+    c.temperature = temperature;
+    c.logprob = logprob;
+    c.rank = rank;
+    c.entropy = entropy;
+    c.top_tokens = top_tokens;
+    c.top_logprobs = top_logprobs;
+    c.parts = static_cast<unsigned char *>(workspace);
+    c.part_bytes = part_bytes(top);
+    c.chunks = (vocab + kChunk - 1) / kChunk;
+    const uint64_t all = chunks_of(rows, vocab), most = std::min<uint64_t>((uint64_t)sms * 3, kMaxCtas) * kWarps;
+    c.per = (uint32_t)((all + most - 1) / most);
+    const uint64_t warps = (all + c.per - 1) / c.per;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    e = launch((const void *)k_rows, (unsigned)((warps + kWarps - 1) / kWarps), c, s);
+    if (e == cudaSuccess) e = launch((const void *)k_rows_join, rows, c, s);
+    return e == cudaSuccess ? LLMX_OK : cuda_fail("launch", e);
+}

@@ -151,6 +151,17 @@ def lib():
             "llmx_verify_workspace_bytes": (C.c_size_t, [C.c_uint32, C.c_uint32, C.c_uint32]),
             "llmx_verify_drafts": (C.c_int, [vp, C.c_size_t, vp, C.c_size_t, C.c_uint32, vp, vp, C.c_uint32,
                                              C.c_uint32, C.c_uint32, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]),
+            "llmx_logprobs_workspace_bytes": (C.c_size_t, [C.c_uint32] * 3),
+            "llmx_token_logprobs": (C.c_int, [vp, C.c_size_t, C.c_uint32, C.c_uint32, vp, vp, C.c_uint32, vp, vp, vp, vp, vp, vp,
+                                              C.c_size_t, vp]),
+            "llmx_paged_create": (C.c_int, [C.c_int] + [C.c_uint32] * 7 + [C.c_uint64, vp, C.POINTER(vp)]),
+            "llmx_paged_destroy": (C.c_int, [vp]),
+            "llmx_paged_append": (C.c_int, [vp, vp, C.c_uint32, C.c_size_t, vp, vp, C.c_uint32, vp, C.c_uint32, vp, C.c_size_t,
+                                            vp, vp, C.c_uint32, vp, C.c_size_t, vp]),
+            "llmx_paged_attention": (C.c_int, [vp, vp, C.c_uint32, C.c_size_t, vp, vp, C.c_uint32, C.c_uint32, vp,
+                                               C.c_size_t, vp, vp, C.c_uint32, vp, C.c_size_t, vp]),
+            "llmx_paged_error": (C.c_int, [vp, vp]),
+            "llmx_paged_device_bytes": (C.c_uint64, [vp]),
             "llmx_upload_vocab": (C.c_int, [vp, vp]),
             "llmx_allreduce_kind": (C.c_int, [vp]),
             "llmx_decode_fuses_o": (C.c_int, [vp]),
@@ -359,6 +370,48 @@ class Adapters:
         return lib().llmx_adapters_device_bytes(self.h)
 
 
+class Paged:
+    """llmx_paged: append and attention over a key-value cache in pages, for many
+    requests.  Pointers are device pointers (ints); the pages are the caller's."""
+
+    def __init__(self, heads, kv_heads, head_dim, page_len, max_requests, max_block, max_length, max_positions, device=0,
+                 stream=None):
+        self.h = C.c_void_p()
+        check(lib().llmx_paged_create(device, heads, kv_heads, head_dim, page_len, max_requests, max_block, max_length,
+                                      max_positions, stream, C.byref(self.h)), "paged_create")
+
+    def close(self):
+        if self.h:
+            lib().llmx_paged_destroy(self.h)
+            self.h = C.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def append(self, qkv_ptr, rows, offsets_ptr, lengths_ptr, requests, rope_ptr, positions, table_ptr, ld_table, k_ptr,
+               v_ptr, pages, q_ptr, ld_qkv=0, ld_q=0, stream=None):
+        """Rotates queries and keys of rows [q | k | v] and puts keys and values into the pages."""
+        check(lib().llmx_paged_append(self.h, qkv_ptr, rows, ld_qkv, offsets_ptr, lengths_ptr, requests, rope_ptr, positions,
+                                      table_ptr, ld_table, k_ptr, v_ptr, pages, q_ptr, ld_q, stream), "paged_append")
+
+    def attention(self, q_ptr, rows, offsets_ptr, lengths_ptr, requests, table_ptr, ld_table, k_ptr, v_ptr, pages, out_ptr,
+                  longest=0, ld_q=0, ld_out=0, stream=None):
+        """Attention of every request's rows over its pages (Task 18's arithmetic)."""
+        check(lib().llmx_paged_attention(self.h, q_ptr, rows, ld_q, offsets_ptr, lengths_ptr, requests, longest, table_ptr,
+                                         ld_table, k_ptr, v_ptr, pages, out_ptr, ld_out, stream), "paged_attention")
+
+    def error(self, stream=None):
+        """Waits for the stream; raises when a call met something out of range."""
+        check(lib().llmx_paged_error(self.h, stream), "paged_error")
+
+    @property
+    def device_bytes(self):
+        return lib().llmx_paged_device_bytes(self.h)
+
+
 def verify_workspace_bytes(requests, drafts, vocab):
     return lib().llmx_verify_workspace_bytes(requests, drafts, vocab)
 
@@ -371,6 +424,18 @@ def verify_drafts(target_ptr, draft_ptr, vocab, draft_tokens_ptr, offsets_ptr, r
                                    requests, drafts, max_drafts, temperature_ptr, accept_u_ptr, sample_u_ptr,
                                    tokens_ptr, accepted_ptr, probs_ptr, workspace_ptr, workspace_bytes, stream),
           "verify_drafts")
+
+
+def logprobs_workspace_bytes(rows, vocab, top):
+    return lib().llmx_logprobs_workspace_bytes(rows, vocab, top)
+
+
+def token_logprobs(logits_ptr, rows, vocab, tokens_ptr, temperature_ptr, top, logprob_ptr, rank_ptr, entropy_ptr,
+                   top_tokens_ptr, top_logprobs_ptr, workspace_ptr, workspace_bytes, ld=0, stream=None):
+    """llmx_token_logprobs on device pointers (ints); allocates nothing."""
+    check(lib().llmx_token_logprobs(logits_ptr, ld, vocab, rows, tokens_ptr, temperature_ptr, top, logprob_ptr, rank_ptr,
+                                    entropy_ptr, top_tokens_ptr, top_logprobs_ptr, workspace_ptr, workspace_bytes, stream),
+          "token_logprobs")
 
 
 def tp_unique_id() -> bytes:
