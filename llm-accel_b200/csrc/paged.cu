@@ -51,6 +51,7 @@ using llmx::sat32;
 constexpr uint32_t kMaxRequests = 1024, kMaxHeads = 1024, kMaxLength = 1u << 20, kMaxColumns = 128, kMaxPageLen = 65536;
 constexpr uint32_t kMaxAppendRows = 1u << 20;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kMaxSmem = 160 * 1024;  // what any call of k_scores, k_values or k_join asks for
 constexpr int kErrRequest = 1;    // offsets or length of a request out of range
 constexpr int kErrPage = 2;       // a page number out of range
 constexpr int kErrBudget = 4;     // more positions than the handle has room for
@@ -74,6 +75,7 @@ struct Call {
     const uint32_t *offsets, *lengths;
     uint32_t rows, requests, longest, pages;
     int heads, kv, group, dim, page_len, max_block;
+    int groups;                   // of k_join's threads
     uint32_t page8, page8_magic;  // page_len / 8, and for dividing by it
     int scale8;                   // fm(1/sqrt(dim)), Q8.8
     long long capacity;           // (key head, tile) items
@@ -82,8 +84,7 @@ struct Call {
     int16_t *score;      // [slot][8 columns][64 positions]
     int16_t *top;        // [slot][8] maxima
     int16_t *tv;         // [slot][8][dim]
-    int32_t *psum;       // [slot][4 blocks of 16 positions][8] sums of P
-    int32_t *factor;     // [slot][8] P(m_before - m)
+    int2 *fsum;          // [slot][8]: P(m_before - m), the sum of P
     const int16_t *exps; // [2049]
     int *error;
 };
@@ -106,11 +107,6 @@ static __device__ __forceinline__ const int16_t *rows_at(const Call &c, const in
 static __device__ __forceinline__ uint4 ld16(const void *p) {
     uint4 v;
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
-    return v;
-}
-static __device__ __forceinline__ uint2 ld8(const void *p) {
-    uint2 v;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
     return v;
 }
 static __device__ __forceinline__ uint32_t min16x2(uint32_t a, uint32_t b) { return __vmins2(a, b); }
@@ -136,7 +132,6 @@ static __device__ __forceinline__ uint32_t high4(uint32_t a, uint32_t b) { retur
             : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                             \
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                                     \
     }
-LLMX_MMA(mma_ss, "s8", "s8")
 LLMX_MMA(mma_su, "s8", "u8")
 LLMX_MMA(mma_us, "u8", "s8")
 LLMX_MMA(mma_uu, "u8", "u8")
@@ -149,9 +144,16 @@ static __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
     return r;
 }
 
+// Two 32-bit values saturated to 16 bits each, the first in the low half.
+static __device__ __forceinline__ uint32_t pack_sat16(int lo, int hi) {
+    uint32_t r;
+    asm("cvt.pack.sat.s16.s32 %0, %1, %2;" : "=r"(r) : "r"(hi), "r"(lo));
+    return r;
+}
+// A score before its saturation to 16 bits: rnd8 of rnd8 of a total times fm(1/sqrt(d)) (the
+// first never saturates: the factor is below 1), with both roundings' halves added at once.
 static __device__ __forceinline__ int score_of(int total, int scale8) {
-    const int v = (int)(((long long)total * scale8 + 128) >> 8);
-    return sat16((v + 128) >> 8);
+    return (int)(((long long)total * scale8 + (128 + (128 << 8))) >> 16);
 }
 // A score with its four saturating banks.
 static __device__ __noinline__ int score_exact(const int16_t *q, const int16_t *k, int dim, int scale8) {
@@ -228,15 +230,20 @@ static __device__ int plan(const Call &c, Meta *meta) {
 
 // One (request, key head, tile) after another.
 struct Cursor {
-    int b, h, t;      // request, key head, tile
-    Meta m;
-    int length;
+    int b, h, t;  // request, key head, tile
+    int tiles, rows, length, blocks;
+    int slot0;    // of tile 0 in the first column block of this key head
     const int32_t *table;
 
-    __device__ void enter(const Call &c, const Meta *meta, int request) {
+    __device__ void enter(const Call &c, const Meta *meta, int request, int head) {
         b = request;
-        m = meta[b];
+        h = head;
+        const Meta m = meta[b];
+        tiles = m.tiles;
+        rows = m.rows;
         length = (int)c.lengths[b];
+        blocks = (rows * c.group + 7) >> 3;
+        slot0 = m.slot + h * blocks * tiles;
         table = c.table + (size_t)b * c.ld_table;
     }
     // item: below the number of items
@@ -247,30 +254,26 @@ struct Cursor {
             if (meta[mid].item <= item) lo = mid;
             else hi = mid - 1;
         }
-        enter(c, meta, lo);
-        h = (item - m.item) / m.tiles;
-        t = item - m.item - h * m.tiles;
+        const Meta m = meta[lo];
+        const int head = (item - m.item) / m.tiles;
+        enter(c, meta, lo, head);
+        t = item - m.item - head * m.tiles;
     }
     // The next item, which there is.  Returns whether it is of another request or key head.
     __device__ bool next(const Call &c, const Meta *meta) {
-        if (++t < m.tiles) return false;
+        if (++t < tiles) return false;
         t = 0;
-        if (++h == c.kv) {
-            h = 0;
-            int r = b + 1;
-            while (meta[r].tiles == 0) r++;
-            enter(c, meta, r);
+        int r = b, head = h + 1;
+        if (head == c.kv) {
+            head = 0;
+            do r++;
+            while (meta[r].tiles == 0);
         }
+        enter(c, meta, r, head);
         return true;
     }
-    __device__ int columns(const Call &c) const { return m.rows * c.group; }
     // Slot of this tile in column block nb.
-    __device__ size_t slot(const Call &c, int nb) const {
-        const int blocks = (columns(c) + 7) / 8;
-        return (size_t)m.slot + (size_t)(h * blocks + nb) * m.tiles + t;
-    }
-    // Positions that column col sees.
-    __device__ int seen(const Call &c, int col) const { return length - m.rows + 1 + col / c.group; }
+    __device__ int slot(int nb) const { return slot0 + nb * tiles + t; }
 };
 
 static __device__ __forceinline__ void range_of(int items, int &first, int &end) {
@@ -280,13 +283,29 @@ static __device__ __forceinline__ void range_of(int items, int &first, int &end)
 }
 
 // ---- scores -------------------------------------------------------------------------
+// What k_scores keeps of a column (a query row) of the (request, key head) at hand.
+struct __align__(16) Column {
+    int seen;  // positions that it sees
+    int bias;  // 2048 times its sum
+    int wide;  // a bank may saturate
+    int pad;
+};
+
 // A warp scores 16 positions against 8 columns (query rows) at a time: the positions are
 // the rows of A, and a lane's 16-byte load of a key row's 8 dimensions is, split into
-// bytes, its share of A for both byte planes; no shared memory is passed through.
+// bytes, its share of A for both byte planes; no shared memory is passed through.  The
+// queries' shares of B, with those of (8 - q) >> 4, wait in shared memory.  Keys are limited by two
+// instructions a pair: min(k, 2048), then max(k + 2048, 0), so both planes are
+// unsigned and 2048 times the sum of q is taken off again.
 template <int KS>  // steps of 32 dimensions
 __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
-    extern __shared__ Meta meta[];
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ int tops[2][kMaxColumns];
+    __shared__ Column column[kMaxColumns];
+    const int most = (c.max_block * c.group + 7) / 8;  // column blocks
+    uint4 *queries = reinterpret_cast<uint4 *>(dynamic);  // [most][KS][32 lanes] {low, low, high, high}
+    uint4 *rests = queries + most * KS * 32;              // the same of (8 - q) >> 4
+    Meta *meta = reinterpret_cast<Meta *>(rests + most * KS * 32);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     for (int i = threadIdx.x; i < 2 * (int)kMaxColumns; i += kThreads) tops[i / kMaxColumns][i % kMaxColumns] = -32768;
     pdl_wait();
@@ -304,125 +323,116 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             const int p = p0 + 8 * r;
-            const bool any = p < u.length;
-            const int16_t *row = any ? rows_at(c, c.k, u.table, (uint32_t)p >> 3, u.h) + (size_t)g * c.dim : nullptr;
+            const int16_t *row = p < u.length ? rows_at(c, c.k, u.table, (uint32_t)p >> 3, u.h) + g * c.dim + 8 * t4 : nullptr;
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const int e = 32 * s + 8 * t4;
-                raw[r][s] = p + g < u.length && e < c.dim ? ld16(row + e) : make_uint4(0, 0, 0, 0);
-            }
+            for (int s = 0; s < KS; s++)
+                raw[r][s] = p + g < u.length && 32 * s + 8 * t4 < c.dim ? ld16(row + 32 * s) : make_uint4(0, 0, 0, 0);
         }
     };
     load(cur);
-    uint32_t qh[KS][2], ql[KS][2];  // this lane's share of B: column g
-    bool held = false;              // the registers hold the only column block of (b, h)
-    uint32_t wide = 0;
+    bool moved = true;
     for (int item = first; item < end; item++) {
-        const int buf = item & 1;
-        const int p0 = cur.t * kTile + warp * 16;
-        const bool live = p0 < cur.length;
-        // byte planes of the keys
-        uint32_t kh[KS][4], kl[KS][4];
-        uint32_t out = 0;
+        const Cursor now = cur;
+        if (moved) {
+            __syncthreads();  // the last key head's columns are done with
+            const int columns = now.rows * c.group;
+            const uint32_t row0 = c.offsets[now.b];
+            for (int nb = warp; nb < now.blocks; nb += kWarps) {
+                const int col = nb * 8 + g, j = col / c.group;
+                const int16_t *q = c.q + (size_t)(row0 + j) * c.ld_q + (size_t)(now.h * c.group + col - j * c.group) * c.dim + 8 * t4;
+                uint32_t big = 0;
+                int sum = 0;
+#pragma unroll
+                for (int s = 0; s < KS; s++) {
+                    const uint4 w = col < columns && 32 * s + 8 * t4 < c.dim ? *reinterpret_cast<const uint4 *>(q + 32 * s) : make_uint4(0, 0, 0, 0);
+                    // above 8192: the top three of 16 bits differ
+                    big |= (w.x ^ (w.x << 1)) | (w.x ^ (w.x << 2)) | (w.y ^ (w.y << 1)) | (w.y ^ (w.y << 2)) | (w.z ^ (w.z << 1)) |
+                           (w.z ^ (w.z << 2)) | (w.w ^ (w.w << 1)) | (w.w ^ (w.w << 2));
+                    // (a total reaches 2^31 only where every q is -8192, the first one too)
+                    if (s == 0 && t4 == 0 && (w.x & 0xffffu) == 0xe000u) big |= 0x8000u;
+                    sum += llmx::lo16(w.x) + llmx::hi16(w.x) + llmx::lo16(w.y) + llmx::hi16(w.y) + llmx::lo16(w.z) + llmx::hi16(w.z) +
+                           llmx::lo16(w.w) + llmx::hi16(w.w);
+                    queries[(nb * KS + s) * 32 + lane] = make_uint4(low4(w.x, w.y), low4(w.z, w.w), high4(w.x, w.y), high4(w.z, w.w));
+                    const uint4 r = make_uint4(rest2(w.x), rest2(w.y), rest2(w.z), rest2(w.w));
+                    rests[(nb * KS + s) * 32 + lane] = make_uint4(low4(r.x, r.y), low4(r.z, r.w), high4(r.x, r.y), high4(r.z, r.w));
+                }
+                big |= __shfl_xor_sync(0xffffffffu, big, 1);
+                big |= __shfl_xor_sync(0xffffffffu, big, 2);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                if (t4 == 0) column[col] = Column{col < columns ? now.length - now.rows + 1 + j : 0, 2048 * sum, (int)(big & 0x80008000u), 0};
+            }
+            __syncthreads();
+        }
+        const int p0 = now.t * kTile + warp * 16;
+        // byte planes of the keys, from 0 to 4096
+        uint32_t kh[KS][4], kl[KS][4], limit = 0;
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
             for (int r = 0; r < 2; r++) {
-                kl[s][r] = low4(raw[r][s].x, raw[r][s].y);
-                kl[s][r + 2] = low4(raw[r][s].z, raw[r][s].w);
-                kh[s][r] = high4(raw[r][s].x, raw[r][s].y);
-                kh[s][r + 2] = high4(raw[r][s].z, raw[r][s].w);
-                out |= beyond(kh[s][r]) | beyond(kh[s][r + 2]);
+                auto shift = [](uint32_t w) { return __viaddmax_s16x2(min16x2(w, 0x08000800u), 0x08000800u, 0u); };
+                const uint4 w = make_uint4(shift(raw[r][s].x), shift(raw[r][s].y), shift(raw[r][s].z), shift(raw[r][s].w));
+                kl[s][r] = low4(w.x, w.y);
+                kl[s][r + 2] = low4(w.z, w.w);
+                kh[s][r] = high4(w.x, w.y);
+                kh[s][r + 2] = high4(w.z, w.w);
+                limit |= kh[s][r] | kh[s][r + 2];
             }
-        const bool limit = __any_sync(0xffffffffu, out != 0);
-        if (limit) {
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const uint4 w = make_uint4(limit2(raw[r][s].x), limit2(raw[r][s].y), limit2(raw[r][s].z), limit2(raw[r][s].w));
-                    kl[s][r] = low4(w.x, w.y);
-                    kl[s][r + 2] = low4(w.z, w.w);
-                    kh[s][r] = high4(w.x, w.y);
-                    kh[s][r + 2] = high4(w.z, w.w);
-                }
-        }
+        // some high byte is 16: the value 4096, at the upper limit
+        const bool some = __any_sync(0xffffffffu, (limit & 0x10101010u) != 0);
         // the next item's keys are on their way while this one's are used
-        Cursor now = cur;
-        const bool more = item + 1 < end;
-        bool moved = false;
-        if (more) {
+        if (item + 1 < end) {
             moved = cur.next(c, meta);
             load(cur);
         }
-        const int columns = now.columns(c), blocks = (columns + 7) / 8;
-        for (int nb = 0; live && nb < blocks; nb++) {
-            const int col = nb * 8 + g;
-            const int head = now.h * c.group + col % c.group;
-            const int16_t *qrow = c.q + (size_t)(c.offsets[now.b] + col / c.group) * c.ld_q + (size_t)head * c.dim;
-            if (!held) {
-                uint32_t most = 0;
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const int e = 32 * s + 8 * t4;
-                    const uint4 w = col < columns && e < c.dim ? *reinterpret_cast<const uint4 *>(qrow + e) : make_uint4(0, 0, 0, 0);
-                    ql[s][0] = low4(w.x, w.y);
-                    ql[s][1] = low4(w.z, w.w);
-                    qh[s][0] = high4(w.x, w.y);
-                    qh[s][1] = high4(w.z, w.w);
-                    // |q| above 8192: the top three bits of a high byte differ
-                    most |= (qh[s][0] ^ (qh[s][0] << 1)) | (qh[s][1] ^ (qh[s][1] << 1)) | (qh[s][0] ^ (qh[s][0] << 2)) | (qh[s][1] ^ (qh[s][1] << 2));
-                }
-                // (the sum reaches 2^31 only where every q is -8192, the first one too)
-                const bool lowest = t4 == 0 && (qh[0][0] & 0xffu) == 0xe0u && (ql[0][0] & 0xffu) == 0;
-                wide = __ballot_sync(0xffffffffu, (most & 0x80808080u) != 0 || lowest);
-            }
-            held = blocks == 1;
+        for (int nb = 0; p0 < now.length && nb < now.blocks; nb++) {
             int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int s = 0; s < KS; s++) {
-                mma_ss(hh, kh[s][0], kh[s][1], kh[s][2], kh[s][3], qh[s][0], qh[s][1]);
-                mma_su(mid, kh[s][0], kh[s][1], kh[s][2], kh[s][3], ql[s][0], ql[s][1]);
-                mma_uu(ll, kl[s][0], kl[s][1], kl[s][2], kl[s][3], ql[s][0], ql[s][1]);
-                mma_us(mid, kl[s][0], kl[s][1], kl[s][2], kl[s][3], qh[s][0], qh[s][1]);
+                const uint4 q = queries[(nb * KS + s) * 32 + lane];
+                mma_us(hh, kh[s][0], kh[s][1], kh[s][2], kh[s][3], q.z, q.w);
+                mma_uu(mid, kh[s][0], kh[s][1], kh[s][2], kh[s][3], q.x, q.y);
+                mma_uu(ll, kl[s][0], kl[s][1], kl[s][2], kl[s][3], q.x, q.y);
+                mma_us(mid, kl[s][0], kl[s][1], kl[s][2], kl[s][3], q.z, q.w);
             }
-            if (limit) {
+            if (some) {
 #pragma unroll
                 for (int s = 0; s < KS; s++) {
-                    uint32_t m[4], r[4];
+                    const uint4 r = rests[(nb * KS + s) * 32 + lane];
+                    uint32_t m[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) m[i] = at_limit(kh[s][i]);
-#pragma unroll
-                    for (int i = 0; i < 2; i++) {  // (8 - q) >> 4, from the bytes of q
-                        r[2 * i] = rest2(__byte_perm(ql[s][i], qh[s][i], 0x5140));
-                        r[2 * i + 1] = rest2(__byte_perm(ql[s][i], qh[s][i], 0x7362));
-                    }
-                    mma_us(mid, m[0], m[1], m[2], m[3], high4(r[0], r[1]), high4(r[2], r[3]));
-                    mma_uu(ll, m[0], m[1], m[2], m[3], low4(r[0], r[1]), low4(r[2], r[3]));
+                    for (int i = 0; i < 4; i++) m[i] = kh[s][i] >> 4 & 0x01010101u;
+                    mma_us(mid, m[0], m[1], m[2], m[3], r.z, r.w);
+                    mma_uu(ll, m[0], m[1], m[2], m[3], r.x, r.y);
                 }
             }
+            const Column ca = column[nb * 8 + 2 * t4], cb = column[nb * 8 + 2 * t4 + 1];
             int sc[4];
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                sc[i] = score_of((int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]), c.scale8);
-            if (wide) {
+                sc[i] = score_of((int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i] - (uint32_t)(i & 1 ? cb.bias : ca.bias)),
+                                 c.scale8);
+            if (__any_sync(0xffffffffu, (ca.wide | cb.wide) != 0)) {
 #pragma unroll 1
                 for (int i = 0; i < 4; i++) {
-                    const int col1 = 2 * t4 + (i & 1), p = p0 + g + (i >> 1) * 8;
-                    if ((wide >> (4 * col1) & 15u) == 0 || p >= now.length || nb * 8 + col1 >= columns) continue;
-                    const int cc = nb * 8 + col1;
-                    const int16_t *q1 = c.q + (size_t)(c.offsets[now.b] + cc / c.group) * c.ld_q + (size_t)(now.h * c.group + cc % c.group) * c.dim;
-                    sc[i] = score_exact(q1, rows_at(c, c.k, now.table, (uint32_t)p >> 3, now.h) + (size_t)(p & 7) * c.dim, c.dim, c.scale8);
+                    const int col = nb * 8 + 2 * t4 + (i & 1), p = p0 + g + (i >> 1) * 8;
+                    if (!column[col].wide || p >= now.length) continue;
+                    const int j = col / c.group;
+                    const int16_t *q = c.q + (size_t)(c.offsets[now.b] + j) * c.ld_q + (size_t)(now.h * c.group + col - j * c.group) * c.dim;
+                    const int y = score_exact(q, rows_at(c, c.k, now.table, (uint32_t)p >> 3, now.h) + (p & 7) * c.dim, c.dim, c.scale8);
+                    if (i == 0) sc[0] = y;
+                    else if (i == 1) sc[1] = y;
+                    else if (i == 2) sc[2] = y;
+                    else sc[3] = y;
                 }
             }
             // column g, positions 2 t4, 2 t4 + 1 (and + 8) after the transposition
-            const uint32_t w0 = transpose8((uint32_t)(sc[0] & 0xffff) | ((uint32_t)sc[1] << 16));
-            const uint32_t w1 = transpose8((uint32_t)(sc[2] & 0xffff) | ((uint32_t)sc[3] << 16));
-            const size_t slot = now.slot(c, nb);
-            uint32_t *dst = reinterpret_cast<uint32_t *>(c.score + (slot * 8 + g) * kTile + warp * 16 + 2 * t4);
+            const uint32_t w0 = transpose8(pack_sat16(sc[0], sc[1])), w1 = transpose8(pack_sat16(sc[2], sc[3]));
+            uint32_t *dst = reinterpret_cast<uint32_t *>(c.score + ((size_t)now.slot(nb) * 8 + g) * kTile + warp * 16 + 2 * t4);
             dst[0] = w0;
             dst[4] = w1;
-            const int seen = now.seen(c, col) - (p0 + 2 * t4);
+            const int seen = column[nb * 8 + g].seen - (p0 + 2 * t4);
             int top = -32768;
             if (seen > 0) top = llmx::lo16(w0);
             if (seen > 1) top = max(top, llmx::hi16(w0));
@@ -430,39 +440,56 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
             if (seen > 9) top = max(top, llmx::hi16(w1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (t4 == 0) atomicMax(&tops[buf][col], top);
+            if (t4 == 0) atomicMax(&tops[item & 1][nb * 8 + g], top);
         }
-        if (moved) held = false;
         __syncthreads();
         // (the other buffer is in use until every thread is here again)
-        for (int col = threadIdx.x; col < blocks * 8; col += kThreads) {
-            c.top[now.slot(c, col >> 3) * 8 + (col & 7)] = (int16_t)tops[buf][col];
-            tops[buf][col] = -32768;
+        for (int col = threadIdx.x; col < now.blocks * 8; col += kThreads) {
+            c.top[(size_t)now.slot(col >> 3) * 8 + (col & 7)] = (int16_t)tops[item & 1][col];
+            tops[item & 1][col] = -32768;
         }
     }
 }
 
 // ---- values -------------------------------------------------------------------------
 constexpr int kExpWords = 1028;  // 2049 entries of 16 bits, rounded up to 16 bytes
+constexpr int kRowBytes = 256;   // of a value row in shared memory
+constexpr int kValueBytes = kTile * kRowBytes;
+
+// A stage of k_values' ring: a tile's value rows, then per column block the scores (1 KB) and maxima
+// (16 bytes).
+static __host__ __device__ int stage_bytes(int blocks) { return kValueBytes + blocks * (8 * kTile * 2 + 16); }
+static __host__ __device__ int stages_of(int blocks) { return blocks <= 2 ? 3 : 2; }
+
+static __device__ __forceinline__ void copy16(void *dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0)
+                 : "memory");
+}
 
 // A warp forms 32 of a tile's elements: the elements are the rows of A, so that a lane needs
 // the bytes of four positions in a word, a 4 x 4 transposition of bytes in its
-// registers.  A tile's probabilities are formed once, by all warps, and pass
-// through shared memory in the order of B.
+// registers.  Value rows come through shared memory, whole lines at a time: 16 bytes go to
+// unit u ^ 2 (row / 8 mod 4) of their row, so that the four rows that a quarter of a warp
+// reads lie in different banks.  A tile's probabilities are formed once, by all
+// warps, and pass through shared memory in the order of B.
 __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const int warps = blockDim.x >> 5;
     const int most = (c.max_block * c.group + 7) / 8;  // column blocks
-    uint32_t *exps_w = reinterpret_cast<uint32_t *>(dynamic);
-    const int16_t *exps = reinterpret_cast<const int16_t *>(dynamic) + 2048;  // of differences <= 0
-    uint4 *prob = reinterpret_cast<uint4 *>(dynamic + kExpWords * 4);         // [2][most][2 steps][32 lanes]
-    int *before = reinterpret_cast<int *>(prob + 2 * most * 64) + warp * most * 8;  // this warp's running maxima
-    Meta *meta = reinterpret_cast<Meta *>(reinterpret_cast<int *>(prob + 2 * most * 64) + kWarps * most * 8);
-    for (int i = threadIdx.x; i < kExpWords; i += blockDim.x) exps_w[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
+    const int stages = stages_of(most), stage_size = stage_bytes(most);
+    unsigned char *ring = dynamic;
+    uint4 *prob = reinterpret_cast<uint4 *>(ring + stages * stage_size);  // [most][2 steps][32 lanes] {low, low, high, high}
+    uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + most * 64);
+    const int16_t *exps = reinterpret_cast<const int16_t *>(exps_w) + 2048;  // of differences <= 0
+    int *seen = reinterpret_cast<int *>(exps_w + kExpWords);  // [most * 8] positions that a column sees
+    int *psum = seen + most * 8;                              // [4][most * 8] sums of P over 16 positions
+    int *factor = psum + 4 * most * 8;                        // [most * 8]
+    int *before = factor + most * 8 + warp * most * 8;        // [most * 8] the warp's own running maxima
+    Meta *meta = reinterpret_cast<Meta *>(factor + (1 + kWarps) * most * 8);
+    for (int i = threadIdx.x; i < kExpWords; i += kThreads) exps_w[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
     pdl_wait();
     pdl_trigger();
-    for (uint32_t b = threadIdx.x; b < c.requests; b += blockDim.x) meta[b] = c.meta[b];
+    for (uint32_t b = threadIdx.x; b < c.requests; b += kThreads) meta[b] = c.meta[b];
     __syncthreads();
     const Meta last = meta[c.requests - 1];
     // void requests have no items but their place in the order
@@ -470,37 +497,71 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     int first, end;
     range_of(items, first, end);
     if (first >= end) return;
-    const int e0 = warp * 32 + g * 4;  // this lane's elements: e0 .. e0 + 3
+
+    // the elements are shared out over `parts` warps; with fewer than four, the others take other column blocks
+    const int parts = (c.dim + 31) >> 5, turns = 4 / parts, part = warp % parts, turn = warp / parts;
+    const int e0 = part * 32 + g * 4;  // this lane's elements: e0 .. e0 + 3
     const bool mine = e0 < c.dim;
 
-    Cursor cur;
-    cur.start(c, meta, first);
-    uint2 raw[2][8];  // positions 32 s + 8 t4 + i, elements e0 .. e0 + 3
-    auto load = [&](const Cursor &u) {
+    auto fetch = [&](const Cursor &u, int stage) {
+        unsigned char *dst = ring + stage * stage_size;
+        const int unit = threadIdx.x & 15, r8 = threadIdx.x >> 4;
+        const int left = u.length - u.t * kTile;
+        if (unit * 8 < c.dim) {
+            const uint32_t p8 = (uint32_t)u.t * 8;
+            uint32_t at = div_page(c, p8), inside = p8 - at * c.page8;
+            const int16_t *rows = nullptr;
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            const int p = u.t * kTile + 32 * s + 8 * t4;
-            const bool any = p < u.length;
-            const int16_t *row = any ? rows_at(c, c.v, u.table, (uint32_t)p >> 3, u.h) + e0 : nullptr;
-#pragma unroll
-            for (int i = 0; i < 8; i++) raw[s][i] = mine && p + i < u.length ? ld8(row + (size_t)i * c.dim) : make_uint2(0, 0);
+            for (int j = 0; j < 8; j++) {
+                if (8 * j < left && (j == 0 || inside == c.page8)) {  // the next page
+                    if (j) {
+                        at++;
+                        inside = 0;
+                    }
+                    uint32_t page = (uint32_t)u.table[at];
+                    if (page >= c.pages) {
+                        atomicOr(c.error, kErrPage);
+                        page = 0;
+                    }
+                    rows = c.v + (((size_t)page * c.kv + u.h) * c.page_len + inside * 8 + r8) * c.dim + unit * 8;
+                }
+                const bool there = 8 * j + r8 < left;
+                copy16(dst + (8 * j + r8) * kRowBytes + (unit ^ (2 * (j & 3))) * 16, there ? rows : c.v, there);
+                rows += 8 * c.dim;
+                inside++;
+            }
         }
+        unsigned char *score = dst + kValueBytes, *top = score + most * (8 * kTile * 2);
+        for (int i = threadIdx.x; i < u.blocks * 64; i += kThreads) {  // (columns' rows of 8 units, turned by 2 (column mod 4))
+            const int col = i >> 3 & 7, w = i & 7;
+            copy16(score + (i - w + (w ^ (2 * (col & 3)))) * 16, c.score + ((size_t)u.slot(i >> 6) * 64 + (i & 63)) * 8, true);
+        }
+        if (threadIdx.x < u.blocks) copy16(top + threadIdx.x * 16, c.top + (size_t)u.slot(threadIdx.x) * 8, true);
     };
-    load(cur);
+    Cursor cur, ahead;
+    cur.start(c, meta, first);
+    ahead = cur;
+    int fetched = first;
+    for (int i = 0; i < stages - 1; i++) {
+        if (fetched < end) {
+            if (fetched > first) ahead.next(c, meta);
+            fetch(ahead, i);
+            fetched++;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    int stage = 0;
     bool moved = true;
     for (int item = first; item < end; item++) {
-        const int columns = cur.columns(c), blocks = (columns + 7) / 8;
-        uint4 *pb = prob + (item & 1) * most * 64;
-        if (moved) {  // the maxima of the tiles before
+        const int blocks = cur.blocks;
+        if (moved) {
+            // the maxima of the tiles before, by every warp for itself
             for (int nb = 0; nb < blocks; nb++) {
-                const uint4 *tops = reinterpret_cast<const uint4 *>(c.top + (cur.slot(c, nb) - cur.t) * 8);
+                const uint4 *tops = reinterpret_cast<const uint4 *>(c.top) + cur.slot(nb) - cur.t;
                 uint4 m = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
                 for (int i = lane; i < cur.t; i += 32) {
                     const uint4 w = tops[i];
-                    m.x = max16x2(m.x, w.x);
-                    m.y = max16x2(m.y, w.y);
-                    m.z = max16x2(m.z, w.z);
-                    m.w = max16x2(m.w, w.w);
+                    m = make_uint4(max16x2(m.x, w.x), max16x2(m.y, w.y), max16x2(m.z, w.z), max16x2(m.w, w.w));
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) {
@@ -512,117 +573,125 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
                 const uint32_t w = g < 4 ? (g < 2 ? m.x : m.y) : (g < 6 ? m.z : m.w);
                 if (t4 == 0) before[nb * 8 + g] = g & 1 ? llmx::hi16(w) : llmx::lo16(w);
             }
-            __syncwarp();
+            __syncthreads();  // (the last key head's columns are done with)
+            for (int col = threadIdx.x; col < blocks * 8; col += kThreads)
+                seen[col] = col < cur.rows * c.group ? cur.length - cur.rows + 1 + col / c.group : 0;
         }
-        // probabilities: 16 positions a warp at a time, lane: column g, 4 positions
+        if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncthreads();
+        const unsigned char *here = ring + stage * stage_size;
+        if (fetched < end) {  // into the stage of the item before, which is free
+            ahead.next(c, meta);
+            fetch(ahead, stage == 0 ? stages - 1 : stage - 1);
+            fetched++;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        // probabilities: 16 positions a warp, lane: column g, 4 positions
         for (int nb = 0; nb < blocks; nb++) {
-            const size_t slot = cur.slot(c, nb);
-            const int col = nb * 8 + g;
-            const int was = before[col];
-            const int m = max(was, (int)c.top[slot * 8 + g]);
-            for (int blk = warp; blk < 4; blk += warps) {
-                const uint2 w = *reinterpret_cast<const uint2 *>(c.score + (slot * 8 + g) * kTile + blk * 16 + 4 * t4);
-                const int seen = col < columns ? cur.seen(c, col) - (cur.t * kTile + blk * 16 + 4 * t4) : 0;
-                const int s[4] = {llmx::lo16(w.x), llmx::hi16(w.x), llmx::lo16(w.y), llmx::hi16(w.y)};
-                int p[4], sum = 0;
+            const int col = nb * 8 + g, was = before[col];
+            const int16_t *top = reinterpret_cast<const int16_t *>(here + kValueBytes + most * (8 * kTile * 2)) + col;
+            const int m = max(was, (int)*top);
+            const uint2 w = *reinterpret_cast<const uint2 *>(here + kValueBytes + (col * 8 + ((2 * warp + (t4 >> 1)) ^ (2 * (g & 3)))) * 16 + (t4 & 1) * 8);
+            const int left = seen[col] - (cur.t * kTile + warp * 16 + 4 * t4);
+            const int s[4] = {llmx::lo16(w.x), llmx::hi16(w.x), llmx::lo16(w.y), llmx::hi16(w.y)};
+            int p[4], sum = 0;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    // (what lies behind the last position that is seen may hold anything)
-                    p[i] = i < seen ? exps[min(max(s[i] - m, -2048), 0)] : 0;
-                    sum += p[i];
-                }
-                const uint32_t w0 = (uint32_t)p[0] | (uint32_t)p[1] << 16, w1 = (uint32_t)p[2] | (uint32_t)p[3] << 16;
-                uint32_t *dst = reinterpret_cast<uint32_t *>(pb + nb * 64 + (blk >> 1) * 32 + g * 4 + 2 * (blk & 1) + (t4 >> 1));
-                dst[t4 & 1] = low4(w0, w1);
-                dst[2 + (t4 & 1)] = high4(w0, w1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t4 == 0) {
-                    c.psum[(slot * 4 + blk) * 8 + g] = sum;
-                    if (blk == 0) c.factor[slot * 8 + g] = exps[max(was - m, -2048)];
-                }
+            for (int i = 0; i < 4; i++) {
+                // (what lies behind the last position that is seen may hold anything)
+                p[i] = i < left ? exps[min(max(s[i] - m, -2048), 0)] : 0;
+                sum += p[i];
             }
-            __syncwarp();
-            if (t4 == 0) before[col] = m;
-            __syncwarp();
-        }
-        // byte planes of the values: [step][element pair][row or row + 8, positions 0-3 or 4-7]
-        uint32_t vh[2][2][4], vl[2][2][4];
-        uint32_t out = 0;
-        auto planes = [&]() {
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int mb = 0; mb < 2; mb++)
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = mb ? raw[s][4 * half + i].y : raw[s][4 * half + i].x;
-                        const uint32_t a = __byte_perm(w[0], w[1], 0x5140), b = __byte_perm(w[2], w[3], 0x5140);
-                        const uint32_t d = __byte_perm(w[0], w[1], 0x7362), e = __byte_perm(w[2], w[3], 0x7362);
-                        vl[s][mb][2 * half] = __byte_perm(a, b, 0x5410);
-                        vh[s][mb][2 * half] = __byte_perm(a, b, 0x7632);
-                        vl[s][mb][2 * half + 1] = __byte_perm(d, e, 0x5410);
-                        vh[s][mb][2 * half + 1] = __byte_perm(d, e, 0x7632);
-                        out |= beyond(vh[s][mb][2 * half]) | beyond(vh[s][mb][2 * half + 1]);
-                    }
-        };
-        planes();
-        const bool limit = __any_sync(0xffffffffu, out != 0);
-        if (limit) {
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) raw[s][i] = make_uint2(limit2(raw[s][i].x), limit2(raw[s][i].y));
-            planes();
-        }
-        const Cursor now = cur;
-        if (item + 1 < end) {
-            moved = cur.next(c, meta);
-            load(cur);
+            const uint32_t w0 = (uint32_t)p[0] | (uint32_t)p[1] << 16, w1 = (uint32_t)p[2] | (uint32_t)p[3] << 16;
+            uint32_t *dst = reinterpret_cast<uint32_t *>(prob + nb * 64 + (warp >> 1) * 32 + g * 4 + 2 * (warp & 1) + (t4 >> 1)) + (t4 & 1);
+            dst[0] = low4(w0, w1);
+            dst[2] = high4(w0, w1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t4 == 0) {
+                psum[warp * most * 8 + col] = sum;
+                before[col] = m;
+                if (warp == 0) factor[col] = exps[max(was - m, -2048)];
+            }
         }
         __syncthreads();
-        for (int nb = 0; nb < blocks; nb++) {
-            const uint4 b0 = pb[nb * 64 + lane], b1 = pb[nb * 64 + 32 + lane];  // {low, low, high, high}
-            uint32_t tv[2][2];  // [column 2 t4 + j][elements e0, e0 + 1 and e0 + 2, e0 + 3]
+        for (int col = threadIdx.x; col < blocks * 8; col += kThreads) {
+            const int *ps = psum + col;
+            c.fsum[(size_t)cur.slot(col >> 3) * 8 + (col & 7)] = make_int2(factor[col], ps[0] + ps[most * 8] + ps[2 * most * 8] + ps[3 * most * 8]);
+        }
+        if (turn < turns && turn < blocks) {
+            // byte planes of the values: [step][element pair][row or row + 8, positions 0-3 or 4-7]
+            uint32_t vh[2][2][4], vl[2][2][4], out = 0;
+            const unsigned char *v = here + 8 * t4 * kRowBytes + ((part * 4 + (g >> 1)) ^ (2 * t4)) * 16 + (g & 1) * 8;
+            auto planes = [&](bool limited) {
 #pragma unroll
-            for (int mb = 0; mb < 2; mb++) {
-                int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+                for (int s = 0; s < 2; s++)
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    const uint4 b = s ? b1 : b0;
-                    const uint32_t(&h)[4] = vh[s][mb], (&l)[4] = vl[s][mb];
-                    mma_su(hh, h[0], h[1], h[2], h[3], b.z, b.w);
-                    mma_su(mid, h[0], h[1], h[2], h[3], b.x, b.y);
-                    mma_uu(ll, l[0], l[1], l[2], l[3], b.x, b.y);
-                    mma_uu(mid, l[0], l[1], l[2], l[3], b.z, b.w);
-                    if (limit) {
-                        const uint32_t r0 = rest2(__byte_perm(b.x, b.z, 0x5140)), r1 = rest2(__byte_perm(b.x, b.z, 0x7362));
-                        const uint32_t r2 = rest2(__byte_perm(b.y, b.w, 0x5140)), r3 = rest2(__byte_perm(b.y, b.w, 0x7362));
-                        uint32_t m[4];
+                    for (int half = 0; half < 2; half++) {
+                        uint2 w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) m[i] = at_limit(h[i]);
-                        mma_us(mid, m[0], m[1], m[2], m[3], high4(r0, r1), high4(r2, r3));
-                        mma_uu(ll, m[0], m[1], m[2], m[3], low4(r0, r1), low4(r2, r3));
+                        for (int i = 0; i < 4; i++) {
+                            w[i] = *reinterpret_cast<const uint2 *>(v + (32 * s + 4 * half + i) * kRowBytes);
+                            if (limited) w[i] = make_uint2(limit2(w[i].x), limit2(w[i].y));
+                        }
+#pragma unroll
+                        for (int mb = 0; mb < 2; mb++) {
+                            const uint32_t w0 = mb ? w[0].y : w[0].x, w1 = mb ? w[1].y : w[1].x, w2 = mb ? w[2].y : w[2].x, w3 = mb ? w[3].y : w[3].x;
+                            const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
+                            const uint32_t d = __byte_perm(w0, w1, 0x7362), e = __byte_perm(w2, w3, 0x7362);
+                            vl[s][mb][2 * half] = __byte_perm(a, b, 0x5410);
+                            vh[s][mb][2 * half] = __byte_perm(a, b, 0x7632);
+                            vl[s][mb][2 * half + 1] = __byte_perm(d, e, 0x5410);
+                            vh[s][mb][2 * half + 1] = __byte_perm(d, e, 0x7632);
+                            if (!limited) out |= beyond(vh[s][mb][2 * half]) | beyond(vh[s][mb][2 * half + 1]);
+                        }
                     }
-                }
-                int y[4];
+            };
+            planes(false);
+            const bool limit = __any_sync(0xffffffffu, mine && out != 0);
+            if (limit) planes(true);
+            for (int nb = turn; nb < blocks; nb += turns) {
+                const uint4 b0 = prob[nb * 64 + lane], b1 = prob[nb * 64 + 32 + lane];
+                uint32_t tv[2][2];  // [column 2 t4 + j][elements e0, e0 + 1 and e0 + 2, e0 + 3]
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int ts = (int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]);
-                    const int r6 = ((ts >> 5) + 1) >> 1;  // rnd6, in 32 bits
-                    y[i] = sat16((r6 + 128) >> 8);
+                for (int mb = 0; mb < 2; mb++) {
+                    int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < 2; s++) {
+                        const uint4 b = s ? b1 : b0;
+                        const uint32_t(&h)[4] = vh[s][mb], (&l)[4] = vl[s][mb];
+                        mma_su(hh, h[0], h[1], h[2], h[3], b.z, b.w);
+                        mma_su(mid, h[0], h[1], h[2], h[3], b.x, b.y);
+                        mma_uu(ll, l[0], l[1], l[2], l[3], b.x, b.y);
+                        mma_uu(mid, l[0], l[1], l[2], l[3], b.z, b.w);
+                        if (limit) {
+                            const uint32_t r0 = rest2(__byte_perm(b.x, b.z, 0x5140)), r1 = rest2(__byte_perm(b.x, b.z, 0x7362));
+                            const uint32_t r2 = rest2(__byte_perm(b.y, b.w, 0x5140)), r3 = rest2(__byte_perm(b.y, b.w, 0x7362));
+                            uint32_t m[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) m[i] = at_limit(h[i]);
+                            mma_us(mid, m[0], m[1], m[2], m[3], high4(r0, r1), high4(r2, r3));
+                            mma_uu(ll, m[0], m[1], m[2], m[3], low4(r0, r1), low4(r2, r3));
+                        }
+                    }
+                    int y[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int ts = (int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]);
+                        y[i] = ((ts >> 5) + 257) >> 9;  // rnd8 of rnd6: (ts + 2^5 + 2^13) / 2^14, within 32 bits
+                    }
+                    tv[0][mb] = pack_sat16(y[0], y[2]);
+                    tv[1][mb] = pack_sat16(y[1], y[3]);
                 }
-                tv[0][mb] = (uint32_t)(y[0] & 0xffff) | (uint32_t)y[2] << 16;
-                tv[1][mb] = (uint32_t)(y[1] & 0xffff) | (uint32_t)y[3] << 16;
-            }
-            if (mine) {
-                int16_t *dst = c.tv + (now.slot(c, nb) * 8 + 2 * t4) * c.dim + e0;
-                *reinterpret_cast<uint2 *>(dst) = make_uint2(tv[0][0], tv[0][1]);
-                *reinterpret_cast<uint2 *>(dst + c.dim) = make_uint2(tv[1][0], tv[1][1]);
+                if (mine) {
+                    int16_t *dst = c.tv + ((size_t)cur.slot(nb) * 8 + 2 * t4) * c.dim + e0;
+                    *reinterpret_cast<uint2 *>(dst) = make_uint2(tv[0][0], tv[0][1]);
+                    *reinterpret_cast<uint2 *>(dst + c.dim) = make_uint2(tv[1][0], tv[1][1]);
+                }
             }
         }
+        stage = stage + 1 == stages ? 0 : stage + 1;
+        moved = item + 1 < end && cur.next(c, meta);
     }
 }
 
@@ -640,64 +709,190 @@ static __device__ __forceinline__ uint32_t request_of(const uint32_t *offsets, u
     return before ? block + 31 - __clz(before) : block;
 }
 
-// A thread carries two elements of one query head's row through its tiles in order.
-__global__ void __launch_bounds__(kThreads) k_join(const Call c) {
-    const int pairs = c.dim >> 1;  // threads of a head
+// What a stretch of tiles makes of a value x that comes in: x + s, limited to [lo, hi] (sums that
+// saturate at every step combine to that).  Without kLong no sum can reach the limits.
+template <bool kLong>
+struct Stretch;
+template <>
+struct Stretch<false> {
+    int s;
+    __device__ void start() { s = 0; }
+    __device__ void add(int v) { s += v; }
+    __device__ int of(int x) const { return x + s; }
+};
+template <>
+struct Stretch<true> {
+    long long s;
+    int lo, hi;
+    __device__ void start() {
+        s = 0;
+        lo = INT_MIN;
+        hi = INT_MAX;
+    }
+    __device__ void add(int v) {
+        s += v;
+        lo = llmx::add_sat(lo, v);
+        hi = llmx::add_sat(hi, v);
+    }
+    __device__ int of(int x) const { return (int)min(max(x + s, (long long)lo), (long long)hi); }
+};
+
+constexpr int kShortTiles = 255;  // tiles whose sums stay below 2^31: of values 2^23 each, of probabilities 2^22
+constexpr int kMaxStretches = 3;  // per group of threads
+constexpr int kAhead = 8;         // tiles loaded at once
+constexpr int kMaxGroups = 16;
+
+// x times a factor f < 1 (Q2.14), rounded
+static __device__ __forceinline__ int times(int x, int f) { return (int)(((long long)x * (4 * f) + 32768) >> 16); }
+
+// One query head's row per CTA, dim / 2 threads times `groups`; a thread has two elements, a group an equal
+// part of the tiles.  Between tiles that raise the maximum (whose factor is not 1: few in a
+// long text) the recurrence only adds, so a group gives what its tiles do to any value that
+// comes in as a few stretches (a factor, then a sum), and the first group, which starts from 0,
+// puts them together; tiles beyond a group's kMaxStretches it goes through itself.
+template <bool kLong>
+__global__ void __launch_bounds__(1024) k_join(const Call c) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    struct Pair {
+        Stretch<kLong> a, b;
+    };
+    __shared__ Stretch<kLong> norms[kMaxGroups][kMaxStretches];
+    __shared__ int factors[kMaxGroups][kMaxStretches], counts[kMaxGroups], rest[kMaxGroups];
+    const int pairs = c.dim >> 1, groups = c.groups;  // (whole warps: the last threads may have no group)
+    const int group = (int)threadIdx.x / pairs, e2 = (int)threadIdx.x - group * pairs;
+    Pair *stretches = reinterpret_cast<Pair *>(dynamic);  // [groups - 1][kMaxStretches][pairs]
     pdl_wait();
     pdl_trigger();
-    const long long id = (long long)blockIdx.x * kThreads + threadIdx.x;
-    const long long unit = id / pairs;  // (row, head)
-    const uint32_t row = (uint32_t)min(unit / c.heads, (long long)c.rows - 1);
-    // a warp may hold threads of two rows (pairs need not divide 32)
-    const uint32_t row0 = __shfl_sync(0xffffffffu, row, 0), row1 = __shfl_sync(0xffffffffu, row, 31);
-    uint32_t b = request_of(c.offsets, c.requests, row0);
-    if (row1 != row0)
-        for (uint32_t r = row0 + 1; r <= row1; r++) {
-            const uint32_t n = request_of(c.offsets, c.requests, r);
-            if (row == r) b = n;
-        }
-    if (unit / c.heads >= c.rows) return;
-    const uint32_t first = c.offsets[b], last = c.offsets[b + 1];
+    const uint32_t row = blockIdx.x / c.heads;
+    const int head = (int)(blockIdx.x - row * c.heads);
+    const uint32_t b = request_of(c.offsets, c.requests, row);
+    const uint32_t begin = c.offsets[b], behind = c.offsets[b + 1];
     const Meta m = c.meta[b];
-    if (row < first || row >= last || m.rows < 0) return;  // of no request, or of a void one
-    const int head = (int)(unit % c.heads), e = 2 * (int)(id % pairs);
-    const int h = head / c.group, col = (int)(row - first) * c.group + head % c.group;
+    if (row < begin || row >= behind || m.rows < 0) return;  // of no request, or of a void one
+    const int h = head / c.group, col = (int)(row - begin) * c.group + head - h * c.group;
     const int blocks = (m.rows * c.group + 7) / 8;
-    const size_t slot = (size_t)m.slot + (size_t)(h * blocks + (col >> 3)) * m.tiles;
-    const int lane8 = col & 7;
-    const int16_t *tv = c.tv + (slot * 8 + lane8) * c.dim + e;
-    const int32_t *psum = c.psum + slot * 32 + lane8, *factor = c.factor + slot * 8 + lane8;
-    int sum = 0, a0 = 0, a1 = 0;
-    constexpr int kAhead = 8;
-    for (int t0 = 0; t0 < m.tiles; t0 += kAhead) {
-        uint32_t v[kAhead];
-        int f[kAhead], s[kAhead];
+    const size_t at = ((size_t)m.slot + (size_t)(h * blocks + (col >> 3)) * m.tiles) * 8 + (col & 7);
+    const uint32_t *tv = reinterpret_cast<const uint32_t *>(c.tv + at * c.dim) + e2;
+    const int2 *fsum = c.fsum + at;
+    const size_t step = (size_t)8 * pairs;  // words from a tile to the next
+    const int first = (int)((long long)m.tiles * group / groups), end = (int)((long long)m.tiles * (group + 1) / groups);
+
+    int sum = 0, a = 0, d = 0;
+    // tiles t0 .. t1 - 1 on top of (sum, a, d)
+    auto replay = [&](int t0, int t1) {
+        for (; t0 < t1; t0 += kAhead) {
+            uint32_t v[kAhead];
+            int2 f[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            const int t = min(t0 + i, m.tiles - 1);
-            v[i] = *reinterpret_cast<const uint32_t *>(tv + (size_t)t * 8 * c.dim);
-            f[i] = factor[(size_t)t * 8];
-            const int32_t *p = psum + (size_t)t * 32;
-            s[i] = p[0] + p[8] + p[16] + p[24];
+            for (int i = 0; i < kAhead; i++)
+                if (t0 + i < t1) {
+                    v[i] = tv[(t0 + i) * step];
+                    f[i] = fsum[(size_t)(t0 + i) * 8];
+                }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (t0 + i < t1) {
+                    if (f[i].x != 16384) {  // a factor of 1 leaves everything as it is
+                        sum = times(sum, f[i].x);
+                        a = times(a, f[i].x);
+                        d = times(d, f[i].x);
+                    }
+                    if constexpr (kLong) {
+                        sum = llmx::add_sat(sum, 4 * f[i].y);
+                        a = llmx::add_sat(a, llmx::lo16(v[i]) * 256);
+                        d = llmx::add_sat(d, llmx::hi16(v[i]) * 256);
+                    } else {
+                        sum += 4 * f[i].y;
+                        a += llmx::lo16(v[i]) * 256;
+                        d += llmx::hi16(v[i]) * 256;
+                    }
+                }
         }
+    };
+    if (group == 0) {
+        replay(first, end);
+    } else if (group < groups) {
+        Stretch<kLong> n;
+        Pair p;
+        n.start();
+        p.a.start();
+        p.b.start();
+        int f0 = 16384, count = 0, left = end;
+        Pair *mine = stretches + (size_t)(group - 1) * kMaxStretches * pairs + e2;
+        for (int t0 = first; t0 < end && left == end; t0 += kAhead) {
+            uint32_t v[kAhead];
+            int2 f[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            if (t0 + i >= m.tiles) break;
-            if (f[i] != 16384) {  // a factor of 1 leaves everything as it is
-                const long long o = (long long)f[i] * 4;  // Q2.14 -> Q16.16
-                sum = (int)rnd((long long)sum * o, 16);   // o < 2^16: no saturation
-                a0 = (int)rnd((long long)a0 * o, 16);
-                a1 = (int)rnd((long long)a1 * o, 16);
+            for (int i = 0; i < kAhead; i++)
+                if (t0 + i < end) {
+                    v[i] = tv[(t0 + i) * step];
+                    f[i] = fsum[(size_t)(t0 + i) * 8];
+                }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++)
+                if (t0 + i < end && left == end) {
+                    bool full = false;
+                    if (f[i].x != 16384) {
+                        if (t0 + i > first) {  // the stretch ends here
+                            if (count + 1 == kMaxStretches) {
+                                left = t0 + i;
+                                full = true;
+                            } else {
+                                mine[count * pairs] = p;
+                                if (e2 == 0) {
+                                    norms[group][count] = n;
+                                    factors[group][count] = f0;
+                                }
+                                count++;
+                                n.start();
+                                p.a.start();
+                                p.b.start();
+                            }
+                        }
+                        if (!full) f0 = f[i].x;
+                    }
+                    if (!full) {
+                        n.add(4 * f[i].y);
+                        p.a.add(llmx::lo16(v[i]) * 256);
+                        p.b.add(llmx::hi16(v[i]) * 256);
+                    }
+                }
+        }
+        if (first < end) {
+            mine[count * pairs] = p;
+            if (e2 == 0) {
+                norms[group][count] = n;
+                factors[group][count] = f0;
             }
-            sum = llmx::add_sat(sum, 4 * s[i]);
-            a0 = llmx::add_sat(a0, llmx::lo16(v[i]) * 256);
-            a1 = llmx::add_sat(a1, llmx::hi16(v[i]) * 256);
+            count++;
+        }
+        if (e2 == 0) {
+            counts[group] = count;
+            rest[group] = left;
+        }
+    }
+    if (groups > 1) __syncthreads();
+    if (group != 0) return;
+    if (groups > 1) {
+        for (int i = 1; i < groups; i++) {
+            for (int k = 0; k < counts[i]; k++) {
+                const int f = factors[i][k];
+                if (f != 16384) {
+                    sum = times(sum, f);
+                    a = times(a, f);
+                    d = times(d, f);
+                }
+                const Pair p = stretches[((size_t)(i - 1) * kMaxStretches + k) * pairs + e2];
+                sum = norms[i][k].of(sum);
+                a = p.a.of(a);
+                d = p.b.of(d);
+            }
+            replay(rest[i], (int)((long long)m.tiles * (i + 1) / groups));
         }
     }
     const long long inv = sat16(rnd((long long)llmx::recip_q16(sum < 16 ? 16 : sum), 8));
-    const int y0 = sat16(rnd((long long)a0 * inv, 16)), y1 = sat16(rnd((long long)a1 * inv, 16));
-    *reinterpret_cast<uint32_t *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + e) =
-        (uint32_t)(y0 & 0xffff) | (uint32_t)y1 << 16;
+    const int y0 = sat16(rnd((long long)a * inv, 16)), y1 = sat16(rnd((long long)d * inv, 16));
+    *reinterpret_cast<uint32_t *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 2 * e2) = (uint32_t)(y0 & 0xffff) | (uint32_t)y1 << 16;
 }
 
 // ---- append -------------------------------------------------------------------------
@@ -781,11 +976,11 @@ struct llmx_paged {
     int heads = 0, kv = 0, dim = 0, page_len = 0;
     uint32_t max_requests = 0, max_block = 0, max_length = 0;
     long long capacity = 0;  // (key head, tile) items of a call
-    size_t values_smem = 0;
+    size_t scores_smem = 0, values_smem = 0;
     unsigned char *memory = nullptr;
     Meta *meta = nullptr;
     int16_t *score = nullptr, *top = nullptr, *tv = nullptr, *exps = nullptr;
-    int32_t *psum = nullptr, *factor = nullptr;
+    int2 *fsum = nullptr;
     int *error = nullptr;
     uint64_t bytes = 0;
 };
@@ -915,15 +1110,19 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     };
     const size_t error_at = place(4), exps_at = place(kExpWords * 4), meta_at = place(max_requests * sizeof(Meta)),
                  score_at = place(slots * 8 * kTile * 2), top_at = place(slots * 16), tv_at = place(slots * 8 * head_dim * 2),
-                 psum_at = place(slots * 128), factor_at = place(slots * 32);
+                 fsum_at = place(slots * 64);
     p->bytes = at;
-    p->values_smem = kExpWords * 4 + blocks * 2 * 64 * 16 + kWarps * blocks * 8 * 4 + (size_t)max_requests * sizeof(Meta);
+    p->scores_smem = 2 * blocks * ((head_dim + 31) / 32) * 512 + (size_t)max_requests * sizeof(Meta);
+    p->values_smem = (size_t)stages_of((int)blocks) * stage_bytes((int)blocks) + blocks * 1024 + kExpWords * 4 +
+                     (6 + kWarps) * blocks * 32 + (size_t)max_requests * sizeof(Meta);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int16_t e16[2049], host[kExpWords * 2] = {};
     llmx::build_exp_tables(e16, host);
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute((const void *)k_values, cudaFuncAttributeMaxDynamicSharedMemorySize, 96 * 1024)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(scores_kernel(p->dim), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute((const void *)k_values, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute((const void *)k_join<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaMalloc(reinterpret_cast<void **>(&p->memory), at)) != cudaSuccess ||
         (e = cudaMemsetAsync(p->memory + error_at, 0, 4, s)) != cudaSuccess ||
         (e = cudaMemcpyAsync(p->memory + exps_at, host, sizeof(host), cudaMemcpyHostToDevice, s)) != cudaSuccess ||
@@ -938,8 +1137,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     as(p->score, score_at);
     as(p->top, top_at);
     as(p->tv, tv_at);
-    as(p->psum, psum_at);
-    as(p->factor, factor_at);
+    as(p->fsum, fsum_at);
     *out = p;
     return LLMX_OK;
 }
@@ -1045,18 +1243,20 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.score = p->score;
     c.top = p->top;
     c.tv = p->tv;
-    c.psum = p->psum;
-    c.factor = p->factor;
+    c.fsum = p->fsum;
     c.exps = p->exps;
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint64_t items = (uint64_t)requests * p->kv * ((longest + kTile - 1) / kTile);
     const unsigned grid = (unsigned)std::min<uint64_t>(items, (uint64_t)p->sms * 4);
-    cudaError_t e = launch(scores_kernel(p->dim), grid, kThreads, requests * sizeof(Meta), c, s);
-    if (e == cudaSuccess) e = launch((const void *)k_values, grid, (p->dim + 31) / 32 * 32, p->values_smem, c, s);
+    cudaError_t e = launch(scores_kernel(p->dim), grid, kThreads, p->scores_smem, c, s);
+    if (e == cudaSuccess) e = launch((const void *)k_values, grid, kThreads, p->values_smem, c, s);
     if (e == cudaSuccess) {
-        const uint64_t threads = (uint64_t)rows * p->heads * (p->dim / 2);
-        e = launch((const void *)k_join, (unsigned)((threads + kThreads - 1) / kThreads), kThreads, 0, c, s);
+        const int tiles = (int)((longest + kTile - 1) / kTile), pairs = p->dim / 2;
+        c.groups = std::min(kMaxGroups, (tiles + kAhead - 1) / kAhead);
+        const bool far = tiles > kShortTiles;
+        const size_t smem = (size_t)(c.groups - 1) * kMaxStretches * pairs * (far ? 2 * sizeof(Stretch<true>) : 2 * sizeof(Stretch<false>));
+        e = launch(far ? (const void *)k_join<true> : (const void *)k_join<false>, rows * (unsigned)p->heads, (pairs * c.groups + 31) / 32 * 32, smem, c, s);
     }
     return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
 }
