@@ -503,7 +503,7 @@ int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vocab, uint32
  * ------------------------------------------------------------------------- */
 typedef struct llmx_paged llmx_paged;
 /* Reserves the workspace of attention calls: heads (1 to 1024, a multiple of kv_heads), head_dim
- * (a multiple of 16 up to 128), page_len (a multiple of 8 up to 65536); at most max_requests
+ * (a multiple of 16 up to 128), page_len (a multiple of 8 up to 65536, fewer than 2^31 values a page); at most max_requests
  * (1 to 1024) requests of max_block (1 to 8) rows, max_length (1 to 2^20) positions each
  * and max_positions together.  heads / kv_heads * max_block is at most 128.  One handle
  * serves every layer of these sizes. */

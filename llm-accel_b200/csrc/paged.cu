@@ -75,8 +75,8 @@ struct Call {
     const uint32_t *offsets, *lengths;
     uint32_t rows, requests, longest, pages;
     int heads, kv, group, dim, page_len, max_block;
-    int groups;                   // of k_join's threads
     uint32_t page8, page8_magic;  // page_len / 8, and for dividing by it
+    uint32_t page_bytes, row_bytes;
     int scale8;                   // fm(1/sqrt(dim)), Q8.8
     long long capacity;           // (key head, tile) items
     // workspace
@@ -93,15 +93,19 @@ struct Call {
 static __device__ __forceinline__ uint32_t div_page(const Call &c, uint32_t p8) {
     return c.page8 == 1 ? p8 : __umulhi(p8, c.page8_magic);
 }
-// First row of 8 positions 8 p8 .. 8 p8 + 7 of key head h (page lengths are multiples of 8).
-static __device__ __forceinline__ const int16_t *rows_at(const Call &c, const int16_t *cache, const int32_t *table, uint32_t p8, int h) {
-    const uint32_t at = div_page(c, p8);
+// First row of positions 8 inside .. of key head h in the page that entry `at` of a table names.
+static __device__ __forceinline__ const char *page_rows(const Call &c, const int16_t *cache, const int32_t *table, uint32_t at, uint32_t inside, int h) {
     uint32_t page = (uint32_t)table[at];
     if (page >= c.pages) {
         atomicOr(c.error, kErrPage);
         page = 0;
     }
-    return cache + (((size_t)page * c.kv + h) * c.page_len + (size_t)(p8 - at * c.page8) * 8) * c.dim;
+    return reinterpret_cast<const char *>(cache) + (unsigned long long)page * c.page_bytes + ((uint32_t)h * c.page_len + inside * 8) * c.row_bytes;
+}
+// First row of positions 8 p8 .. 8 p8 + 7 (page lengths are multiples of 8).
+static __device__ __forceinline__ const char *rows_at(const Call &c, const int16_t *cache, const int32_t *table, uint32_t p8, int h) {
+    const uint32_t at = div_page(c, p8);
+    return page_rows(c, cache, table, at, p8 - at * c.page8, h);
 }
 // (not .nc: the launch before may still be writing the cache when this one starts)
 static __device__ __forceinline__ uint4 ld16(const void *p) {
@@ -112,8 +116,6 @@ static __device__ __forceinline__ uint4 ld16(const void *p) {
 static __device__ __forceinline__ uint32_t min16x2(uint32_t a, uint32_t b) { return __vmins2(a, b); }
 static __device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) { return __vmaxs2(a, b); }
 static __device__ __forceinline__ uint32_t limit2(uint32_t v) { return max16x2(min16x2(v, 0x08000800u), 0xf800f800u); }
-// Of four high bytes: 0xff.. where one is not in [-8, 7] (bits 3 to 7 differ).
-static __device__ __forceinline__ uint32_t beyond(uint32_t h) { return (h ^ (h << 1)) & 0xf0f0f0f0u; }
 // Of four high bytes of limited values: 1 where the byte is 8 (the value 2048).
 static __device__ __forceinline__ uint32_t at_limit(uint32_t h) { return (h >> 3) & ~(h >> 4) & 0x01010101u; }
 // (8 - x) >> 4 of two 16-bit values, as 16 bits each
@@ -298,16 +300,15 @@ struct __align__(16) Column {
 // instructions a pair: min(k, 2048), then max(k + 2048, 0), so both planes are
 // unsigned and 2048 times the sum of q is taken off again.
 template <int KS>  // steps of 32 dimensions
-__global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
+__global__ void __launch_bounds__(kThreads, 5) k_scores(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ int tops[2][kMaxColumns];
+    __shared__ int tops[2][kWarps][kMaxColumns];
     __shared__ Column column[kMaxColumns];
     const int most = (c.max_block * c.group + 7) / 8;  // column blocks
     uint4 *queries = reinterpret_cast<uint4 *>(dynamic);  // [most][KS][32 lanes] {low, low, high, high}
     uint4 *rests = queries + most * KS * 32;              // the same of (8 - q) >> 4
     Meta *meta = reinterpret_cast<Meta *>(rests + most * KS * 32);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    for (int i = threadIdx.x; i < 2 * (int)kMaxColumns; i += kThreads) tops[i / kMaxColumns][i % kMaxColumns] = -32768;
     pdl_wait();
     pdl_trigger();
     const int items = plan(c, meta);
@@ -320,13 +321,24 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
     uint4 raw[2][KS];  // key rows g and g + 8 of the warp's 16 positions
     auto load = [&](const Cursor &u) {
         const int p0 = u.t * kTile + warp * 16;
+        if (p0 + 16 <= u.length && c.dim == 32 * KS) {
+            const uint32_t p8 = (uint32_t)p0 >> 3, at = div_page(c, p8), inside = p8 - at * c.page8;
+            const char *row = page_rows(c, c.k, u.table, at, inside, u.h) + g * (64 * KS) + 16 * t4;
+#pragma unroll
+            for (int s = 0; s < KS; s++) raw[0][s] = ld16(row + 64 * s);
+            // 8 positions on: in the same page, or at the next one's start
+            row = inside + 1 < c.page8 ? row + 8 * 64 * KS : page_rows(c, c.k, u.table, at + 1, 0, u.h) + g * (64 * KS) + 16 * t4;
+#pragma unroll
+            for (int s = 0; s < KS; s++) raw[1][s] = ld16(row + 64 * s);
+            return;
+        }
 #pragma unroll
         for (int r = 0; r < 2; r++) {
             const int p = p0 + 8 * r;
-            const int16_t *row = p < u.length ? rows_at(c, c.k, u.table, (uint32_t)p >> 3, u.h) + g * c.dim + 8 * t4 : nullptr;
+            const char *row = p < u.length ? rows_at(c, c.k, u.table, (uint32_t)p >> 3, u.h) + g * c.row_bytes + 16 * t4 : nullptr;
 #pragma unroll
             for (int s = 0; s < KS; s++)
-                raw[r][s] = p + g < u.length && 32 * s + 8 * t4 < c.dim ? ld16(row + 32 * s) : make_uint4(0, 0, 0, 0);
+                raw[r][s] = p + g < u.length && 32 * s + 8 * t4 < c.dim ? ld16(row + 64 * s) : make_uint4(0, 0, 0, 0);
         }
     };
     load(cur);
@@ -386,6 +398,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
             moved = cur.next(c, meta);
             load(cur);
         }
+        int(&top_of)[kMaxColumns] = tops[item & 1][warp];
+        if (p0 >= now.length)
+            for (int col = lane; col < now.blocks * 8; col += 32) top_of[col] = -32768;
+        const bool whole = p0 + 16 <= now.length - now.rows + 1;  // every column sees all 16 positions
         for (int nb = 0; p0 < now.length && nb < now.blocks; nb++) {
             int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
 #pragma unroll
@@ -420,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
                     if (!column[col].wide || p >= now.length) continue;
                     const int j = col / c.group;
                     const int16_t *q = c.q + (size_t)(c.offsets[now.b] + j) * c.ld_q + (size_t)(now.h * c.group + col - j * c.group) * c.dim;
-                    const int y = score_exact(q, rows_at(c, c.k, now.table, (uint32_t)p >> 3, now.h) + (p & 7) * c.dim, c.dim, c.scale8);
+                    const int y = score_exact(q, reinterpret_cast<const int16_t *>(rows_at(c, c.k, now.table, (uint32_t)p >> 3, now.h) + (p & 7) * c.row_bytes), c.dim, c.scale8);
                     if (i == 0) sc[0] = y;
                     else if (i == 1) sc[1] = y;
                     else if (i == 2) sc[2] = y;
@@ -432,21 +448,23 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
             uint32_t *dst = reinterpret_cast<uint32_t *>(c.score + ((size_t)now.slot(nb) * 8 + g) * kTile + warp * 16 + 2 * t4);
             dst[0] = w0;
             dst[4] = w1;
-            const int seen = column[nb * 8 + g].seen - (p0 + 2 * t4);
-            int top = -32768;
-            if (seen > 0) top = llmx::lo16(w0);
-            if (seen > 1) top = max(top, llmx::hi16(w0));
-            if (seen > 8) top = max(top, llmx::lo16(w1));
-            if (seen > 9) top = max(top, llmx::hi16(w1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (t4 == 0) atomicMax(&tops[item & 1][nb * 8 + g], top);
+            uint32_t top = max16x2(w0, w1);
+            if (!whole) {
+                const int seen = column[nb * 8 + g].seen - (p0 + 2 * t4);
+                auto masked = [](uint32_t w, int n) { return n >= 2 ? w : n == 1 ? (w & 0xffffu) | 0x80000000u : 0x80008000u; };
+                top = max16x2(masked(w0, seen), masked(w1, seen - 8));
+            }
+            top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            if (t4 == 0) top_of[nb * 8 + g] = max(llmx::lo16(top), llmx::hi16(top));
         }
         __syncthreads();
         // (the other buffer is in use until every thread is here again)
         for (int col = threadIdx.x; col < now.blocks * 8; col += kThreads) {
-            c.top[(size_t)now.slot(col >> 3) * 8 + (col & 7)] = (int16_t)tops[item & 1][col];
-            tops[item & 1][col] = -32768;
+            int top = tops[item & 1][0][col];
+#pragma unroll
+            for (int w = 1; w < kWarps; w++) top = max(top, tops[item & 1][w][col]);
+            c.top[(size_t)now.slot(col >> 3) * 8 + (col & 7)] = (int16_t)top;
         }
     }
 }
@@ -459,8 +477,11 @@ constexpr int kValueBytes = kTile * kRowBytes;
 // A stage of k_values' ring: a tile's value rows, then per column block the scores (1 KB) and maxima
 // (16 bytes).
 static __host__ __device__ int stage_bytes(int blocks) { return kValueBytes + blocks * (8 * kTile * 2 + 16); }
-static __host__ __device__ int stages_of(int blocks) { return blocks <= 2 ? 3 : 2; }
+constexpr int kStages = 2;
 
+static __device__ __forceinline__ void copy16(void *dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
 static __device__ __forceinline__ void copy16(void *dst, const void *src, bool there) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0)
                  : "memory");
@@ -472,11 +493,12 @@ static __device__ __forceinline__ void copy16(void *dst, const void *src, bool t
 // unit u ^ 2 (row / 8 mod 4) of their row, so that the four rows that a quarter of a warp
 // reads lie in different banks.  A tile's probabilities are formed once, by all
 // warps, and pass through shared memory in the order of B.
-__global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
+__global__ void __launch_bounds__(kThreads, 5) k_values(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int most = (c.max_block * c.group + 7) / 8;  // column blocks
-    const int stages = stages_of(most), stage_size = stage_bytes(most);
+    constexpr int stages = kStages;
+    const int stage_size = stage_bytes(most);
     unsigned char *ring = dynamic;
     uint4 *prob = reinterpret_cast<uint4 *>(ring + stages * stage_size);  // [most][2 steps][32 lanes] {low, low, high, high}
     uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + most * 64);
@@ -510,33 +532,36 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
         if (unit * 8 < c.dim) {
             const uint32_t p8 = (uint32_t)u.t * 8;
             uint32_t at = div_page(c, p8), inside = p8 - at * c.page8;
-            const int16_t *rows = nullptr;
+            unsigned char *to = dst + r8 * kRowBytes;
+            const char *rows = nullptr;
+            const uint32_t mine = r8 * c.row_bytes + unit * 16;
+            if (left >= kTile && inside + 8 <= c.page8) {  // whole, in one page
+                rows = page_rows(c, c.v, u.table, at, inside, u.h) + mine;
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (8 * j < left && (j == 0 || inside == c.page8)) {  // the next page
-                    if (j) {
-                        at++;
-                        inside = 0;
+                for (int j = 0; j < 8; j++) copy16(to + 8 * j * kRowBytes + (unit ^ (2 * (j & 3))) * 16, rows + j * 8 * c.row_bytes);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (8 * j < left && (j == 0 || inside == c.page8)) {  // the next page
+                        if (j) {
+                            at++;
+                            inside = 0;
+                        }
+                        rows = page_rows(c, c.v, u.table, at, inside, u.h) + mine;
                     }
-                    uint32_t page = (uint32_t)u.table[at];
-                    if (page >= c.pages) {
-                        atomicOr(c.error, kErrPage);
-                        page = 0;
-                    }
-                    rows = c.v + (((size_t)page * c.kv + u.h) * c.page_len + inside * 8 + r8) * c.dim + unit * 8;
+                    const bool there = 8 * j + r8 < left;
+                    copy16(to + 8 * j * kRowBytes + (unit ^ (2 * (j & 3))) * 16, there ? (const void *)rows : (const void *)c.v, there);
+                    rows += 8 * c.row_bytes;
+                    inside++;
                 }
-                const bool there = 8 * j + r8 < left;
-                copy16(dst + (8 * j + r8) * kRowBytes + (unit ^ (2 * (j & 3))) * 16, there ? rows : c.v, there);
-                rows += 8 * c.dim;
-                inside++;
             }
         }
         unsigned char *score = dst + kValueBytes, *top = score + most * (8 * kTile * 2);
         for (int i = threadIdx.x; i < u.blocks * 64; i += kThreads) {  // (columns' rows of 8 units, turned by 2 (column mod 4))
             const int col = i >> 3 & 7, w = i & 7;
-            copy16(score + (i - w + (w ^ (2 * (col & 3)))) * 16, c.score + ((size_t)u.slot(i >> 6) * 64 + (i & 63)) * 8, true);
+            copy16(score + (i - w + (w ^ (2 * (col & 3)))) * 16, c.score + ((size_t)u.slot(i >> 6) * 64 + (i & 63)) * 8);
         }
-        if (threadIdx.x < u.blocks) copy16(top + threadIdx.x * 16, c.top + (size_t)u.slot(threadIdx.x) * 8, true);
+        if (threadIdx.x < u.blocks) copy16(top + threadIdx.x * 16, c.top + (size_t)u.slot(threadIdx.x) * 8);
     };
     Cursor cur, ahead;
     cur.start(c, meta, first);
@@ -577,10 +602,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
             for (int col = threadIdx.x; col < blocks * 8; col += kThreads)
                 seen[col] = col < cur.rows * c.group ? cur.length - cur.rows + 1 + col / c.group : 0;
         }
-        if (stages == 3) asm volatile("cp.async.wait_group 1;" ::: "memory");
-        else asm volatile("cp.async.wait_group 0;" ::: "memory");
+        asm volatile("cp.async.wait_group %0;" ::"n"(stages - 2) : "memory");
         __syncthreads();
-        const unsigned char *here = ring + stage * stage_size;
+        unsigned char *here = ring + stage * stage_size;
         if (fetched < end) {  // into the stage of the item before, which is free
             ahead.next(c, meta);
             fetch(ahead, stage == 0 ? stages - 1 : stage - 1);
@@ -621,19 +645,19 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
         }
         if (turn < turns && turn < blocks) {
             // byte planes of the values: [step][element pair][row or row + 8, positions 0-3 or 4-7]
-            uint32_t vh[2][2][4], vl[2][2][4], out = 0;
-            const unsigned char *v = here + 8 * t4 * kRowBytes + ((part * 4 + (g >> 1)) ^ (2 * t4)) * 16 + (g & 1) * 8;
-            auto planes = [&](bool limited) {
+            uint32_t vh[2][2][4], vl[2][2][4];
+            unsigned char *v = here + 8 * t4 * kRowBytes + ((part * 4 + (g >> 1)) ^ (2 * t4)) * 16 + (g & 1) * 8;
+            bool limit = false;
+#pragma unroll 1
+            for (;;) {
+                uint32_t out = 0;
 #pragma unroll
                 for (int s = 0; s < 2; s++)
 #pragma unroll
                     for (int half = 0; half < 2; half++) {
                         uint2 w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            w[i] = *reinterpret_cast<const uint2 *>(v + (32 * s + 4 * half + i) * kRowBytes);
-                            if (limited) w[i] = make_uint2(limit2(w[i].x), limit2(w[i].y));
-                        }
+                        for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint2 *>(v + (32 * s + 4 * half + i) * kRowBytes);
 #pragma unroll
                         for (int mb = 0; mb < 2; mb++) {
                             const uint32_t w0 = mb ? w[0].y : w[0].x, w1 = mb ? w[1].y : w[1].x, w2 = mb ? w[2].y : w[2].x, w3 = mb ? w[3].y : w[3].x;
@@ -643,13 +667,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
                             vh[s][mb][2 * half] = __byte_perm(a, b, 0x7632);
                             vl[s][mb][2 * half + 1] = __byte_perm(d, e, 0x5410);
                             vh[s][mb][2 * half + 1] = __byte_perm(d, e, 0x7632);
-                            if (!limited) out |= beyond(vh[s][mb][2 * half]) | beyond(vh[s][mb][2 * half + 1]);
+                            out |= (vh[s][mb][2 * half] ^ (vh[s][mb][2 * half] << 1)) | (vh[s][mb][2 * half + 1] ^ (vh[s][mb][2 * half + 1] << 1));
                         }
                     }
-            };
-            planes(false);
-            const bool limit = __any_sync(0xffffffffu, mine && out != 0);
-            if (limit) planes(true);
+                // some high byte is not in [-8, 7] (its bits 3 to 7 differ): limited where they lie, and once more
+                if (limit || !__any_sync(0xffffffffu, mine && (out & 0xf0f0f0f0u) != 0)) break;
+                limit = true;
+#pragma unroll 1
+                for (int i = 0; i < 16; i++) {
+                    uint2 *w = reinterpret_cast<uint2 *>(v + ((i & 8) * 4 + (i & 7)) * kRowBytes);
+                    *w = make_uint2(limit2(w->x), limit2(w->y));
+                }
+            }
             for (int nb = turn; nb < blocks; nb += turns) {
                 const uint4 b0 = prob[nb * 64 + lane], b1 = prob[nb * 64 + 32 + lane];
                 uint32_t tv[2][2];  // [column 2 t4 + j][elements e0, e0 + 1 and e0 + 2, e0 + 3]
@@ -738,29 +767,40 @@ struct Stretch<true> {
 };
 
 constexpr int kShortTiles = 255;  // tiles whose sums stay below 2^31: of values 2^23 each, of probabilities 2^22
-constexpr int kMaxStretches = 3;  // per group of threads
+constexpr int kMaxStretches = 3;  // per warp
 constexpr int kAhead = 8;         // tiles loaded at once
-constexpr int kMaxGroups = 16;
+constexpr int kMaxJoinWarps = 16;
 
 // x times a factor f < 1 (Q2.14), rounded
 static __device__ __forceinline__ int times(int x, int f) { return (int)(((long long)x * (4 * f) + 32768) >> 16); }
+// Sum of a word's low or high half and x
+static __device__ __forceinline__ int add_low(uint32_t w, int x) {
+    int r;
+    asm("dp2a.lo.s32.s32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x0001), "r"(x));
+    return r;
+}
+static __device__ __forceinline__ int add_high(uint32_t w, int x) {
+    int r;
+    asm("dp2a.lo.s32.s32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x0100), "r"(x));
+    return r;
+}
 
-// One query head's row per CTA, dim / 2 threads times `groups`; a thread has two elements, a group an equal
-// part of the tiles.  Between tiles that raise the maximum (whose factor is not 1: few in a
-// long text) the recurrence only adds, so a group gives what its tiles do to any value that
-// comes in as a few stretches (a factor, then a sum), and the first group, which starts from 0,
-// puts them together; tiles beyond a group's kMaxStretches it goes through itself.
+// One query head's row per CTA.  A lane has four elements, a warp an equal part of the tiles.  Between
+// tiles that raise the maximum (whose factor is not 1: few in a long text) the recurrence only adds,
+// so a warp gives what its tiles do to any value that comes in as a few stretches (a factor, then a
+// sum), and the first warp, which starts from 0, puts them together; tiles beyond a warp's
+// kMaxStretches it goes through itself.
 template <bool kLong>
-__global__ void __launch_bounds__(1024) k_join(const Call c) {
+__global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    struct Pair {
-        Stretch<kLong> a, b;
+    struct Four {
+        Stretch<kLong> e[4];
     };
-    __shared__ Stretch<kLong> norms[kMaxGroups][kMaxStretches];
-    __shared__ int factors[kMaxGroups][kMaxStretches], counts[kMaxGroups], rest[kMaxGroups];
-    const int pairs = c.dim >> 1, groups = c.groups;  // (whole warps: the last threads may have no group)
-    const int group = (int)threadIdx.x / pairs, e2 = (int)threadIdx.x - group * pairs;
-    Pair *stretches = reinterpret_cast<Pair *>(dynamic);  // [groups - 1][kMaxStretches][pairs]
+    __shared__ Stretch<kLong> norms[kMaxJoinWarps][kMaxStretches];
+    __shared__ int factors[kMaxJoinWarps][kMaxStretches], counts[kMaxJoinWarps], rest[kMaxJoinWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
+    const int quads = c.dim >> 2;
+    Four *stretches = reinterpret_cast<Four *>(dynamic);  // [warps - 1][kMaxStretches][quads]
     pdl_wait();
     pdl_trigger();
     const uint32_t row = blockIdx.x / c.heads;
@@ -772,127 +812,162 @@ __global__ void __launch_bounds__(1024) k_join(const Call c) {
     const int h = head / c.group, col = (int)(row - begin) * c.group + head - h * c.group;
     const int blocks = (m.rows * c.group + 7) / 8;
     const size_t at = ((size_t)m.slot + (size_t)(h * blocks + (col >> 3)) * m.tiles) * 8 + (col & 7);
-    const uint32_t *tv = reinterpret_cast<const uint32_t *>(c.tv + at * c.dim) + e2;
+    const uint2 *tv = reinterpret_cast<const uint2 *>(c.tv + at * c.dim) + min(lane, quads - 1);
     const int2 *fsum = c.fsum + at;
-    const size_t step = (size_t)8 * pairs;  // words from a tile to the next
-    const int first = (int)((long long)m.tiles * group / groups), end = (int)((long long)m.tiles * (group + 1) / groups);
+    const int step = 8 * quads;  // from a tile to the next
+    const int first = (int)((long long)m.tiles * warp / warps), end = (int)((long long)m.tiles * (warp + 1) / warps);
 
-    int sum = 0, a = 0, d = 0;
-    // tiles t0 .. t1 - 1 on top of (sum, a, d)
-    auto replay = [&](int t0, int t1) {
-        for (; t0 < t1; t0 += kAhead) {
-            uint32_t v[kAhead];
-            int2 f[kAhead];
+    int sum = 0, x[4] = {0, 0, 0, 0};
+    uint2 v[kAhead];
+    int2 f[kAhead];
+    auto load = [&](int t0, int t1) {  // what lies behind t1 changes nothing
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (t0 + i < t1) {
-                    v[i] = tv[(t0 + i) * step];
-                    f[i] = fsum[(size_t)(t0 + i) * 8];
-                }
-#pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (t0 + i < t1) {
-                    if (f[i].x != 16384) {  // a factor of 1 leaves everything as it is
-                        sum = times(sum, f[i].x);
-                        a = times(a, f[i].x);
-                        d = times(d, f[i].x);
-                    }
-                    if constexpr (kLong) {
-                        sum = llmx::add_sat(sum, 4 * f[i].y);
-                        a = llmx::add_sat(a, llmx::lo16(v[i]) * 256);
-                        d = llmx::add_sat(d, llmx::hi16(v[i]) * 256);
-                    } else {
-                        sum += 4 * f[i].y;
-                        a += llmx::lo16(v[i]) * 256;
-                        d += llmx::hi16(v[i]) * 256;
-                    }
-                }
+        for (int i = 0; i < kAhead; i++) {
+            v[i] = make_uint2(0, 0);
+            f[i] = make_int2(16384, 0);
+            if (t0 + i < t1) {
+                v[i] = tv[(size_t)(t0 + i) * step];
+                f[i] = fsum[(size_t)(t0 + i) * 8];
+            }
         }
     };
-    if (group == 0) {
-        replay(first, end);
-    } else if (group < groups) {
-        Stretch<kLong> n;
-        Pair p;
-        n.start();
-        p.a.start();
-        p.b.start();
-        int f0 = 16384, count = 0, left = end;
-        Pair *mine = stretches + (size_t)(group - 1) * kMaxStretches * pairs + e2;
-        for (int t0 = first; t0 < end && left == end; t0 += kAhead) {
-            uint32_t v[kAhead];
-            int2 f[kAhead];
+    // (one of a warp's lanes' factors stands for all of them)
+    auto plain = [&]() {
+        int all = 16384;
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (t0 + i < end) {
-                    v[i] = tv[(t0 + i) * step];
-                    f[i] = fsum[(size_t)(t0 + i) * 8];
-                }
+        for (int i = 0; i < kAhead; i++) all &= f[i].x;  // at most 16384: a factor below it has no bit 14
+        return __any_sync(0xffffffffu, all == 16384) != 0;
+    };
+    auto add_all = [&](Stretch<kLong> &n, Four &p) {
+        if constexpr (kLong) {
 #pragma unroll
-            for (int i = 0; i < kAhead; i++)
-                if (t0 + i < end && left == end) {
-                    bool full = false;
-                    if (f[i].x != 16384) {
-                        if (t0 + i > first) {  // the stretch ends here
-                            if (count + 1 == kMaxStretches) {
-                                left = t0 + i;
-                                full = true;
-                            } else {
-                                mine[count * pairs] = p;
-                                if (e2 == 0) {
-                                    norms[group][count] = n;
-                                    factors[group][count] = f0;
-                                }
-                                count++;
-                                n.start();
-                                p.a.start();
-                                p.b.start();
-                            }
-                        }
-                        if (!full) f0 = f[i].x;
-                    }
-                    if (!full) {
-                        n.add(4 * f[i].y);
-                        p.a.add(llmx::lo16(v[i]) * 256);
-                        p.b.add(llmx::hi16(v[i]) * 256);
-                    }
-                }
+            for (int i = 0; i < kAhead; i++) {
+                n.add(4 * f[i].y);
+                p.e[0].add(add_low(v[i].x, 0) * 256);
+                p.e[1].add(add_high(v[i].x, 0) * 256);
+                p.e[2].add(add_low(v[i].y, 0) * 256);
+                p.e[3].add(add_high(v[i].y, 0) * 256);
+            }
+        } else {
+            int s = 0, y[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                s += f[i].y;
+                y[0] = add_low(v[i].x, y[0]);
+                y[1] = add_high(v[i].x, y[1]);
+                y[2] = add_low(v[i].y, y[2]);
+                y[3] = add_high(v[i].y, y[3]);
+            }
+            n.add(4 * s);
+#pragma unroll
+            for (int k = 0; k < 4; k++) p.e[k].add(256 * y[k]);
         }
-        if (first < end) {
-            mine[count * pairs] = p;
-            if (e2 == 0) {
-                norms[group][count] = n;
-                factors[group][count] = f0;
+    };
+    auto add_one = [&](Stretch<kLong> &n, Four &p, uint2 w, int s) {
+        n.add(4 * s);
+        p.e[0].add(llmx::lo16(w.x) * 256);
+        p.e[1].add(llmx::hi16(w.x) * 256);
+        p.e[2].add(llmx::lo16(w.y) * 256);
+        p.e[3].add(llmx::hi16(w.y) * 256);
+    };
+    auto factor = [&](int by) {  // a factor of 1 leaves everything as it is
+        if (by == 16384) return;
+        sum = times(sum, by);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = times(x[k], by);
+    };
+    auto apply = [&](const Stretch<kLong> &n, const Four &p) {
+        sum = n.of(sum);
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = p.e[k].of(x[k]);
+    };
+    auto clear = [&](Stretch<kLong> &n, Four &p) {
+        n.start();
+#pragma unroll
+        for (int k = 0; k < 4; k++) p.e[k].start();
+    };
+    // tiles t0 .. t1 - 1 on top of (sum, x)
+    auto replay = [&](int t0, int t1) {
+        for (; t0 < t1; t0 += kAhead) {
+            load(t0, t1);
+            Stretch<kLong> n;
+            Four p;
+            clear(n, p);
+            if (plain()) {
+                add_all(n, p);
+                apply(n, p);
+                continue;
+            }
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                factor(f[i].x);
+                clear(n, p);
+                add_one(n, p, v[i], f[i].y);
+                apply(n, p);
+            }
+        }
+    };
+    if (warp == 0) {
+        replay(first, end);
+    } else {
+        Stretch<kLong> n;
+        Four p;
+        clear(n, p);
+        int f0 = 16384, count = 0, left = end;
+        Four *mine = stretches + (size_t)(warp - 1) * kMaxStretches * quads + lane;
+        auto close = [&]() {
+            if (lane < quads) mine[count * quads] = p;
+            if (lane == 0) {
+                norms[warp][count] = n;
+                factors[warp][count] = f0;
             }
             count++;
-        }
-        if (e2 == 0) {
-            counts[group] = count;
-            rest[group] = left;
-        }
-    }
-    if (groups > 1) __syncthreads();
-    if (group != 0) return;
-    if (groups > 1) {
-        for (int i = 1; i < groups; i++) {
-            for (int k = 0; k < counts[i]; k++) {
-                const int f = factors[i][k];
-                if (f != 16384) {
-                    sum = times(sum, f);
-                    a = times(a, f);
-                    d = times(d, f);
-                }
-                const Pair p = stretches[((size_t)(i - 1) * kMaxStretches + k) * pairs + e2];
-                sum = norms[i][k].of(sum);
-                a = p.a.of(a);
-                d = p.b.of(d);
+        };
+        for (int t0 = first; t0 < end && left == end; t0 += kAhead) {
+            load(t0, end);
+            if (plain()) {
+                add_all(n, p);
+                continue;
             }
-            replay(rest[i], (int)((long long)m.tiles * (i + 1) / groups));
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                if (left != end) continue;
+                if (f[i].x != 16384) {
+                    if (t0 + i > first) {  // the stretch ends here
+                        if (count + 1 == kMaxStretches) {
+                            left = t0 + i;
+                            continue;
+                        }
+                        close();
+                        clear(n, p);
+                    }
+                    f0 = f[i].x;
+                }
+                add_one(n, p, v[i], f[i].y);
+            }
+        }
+        if (first < end) close();
+        if (lane == 0) {
+            counts[warp] = count;
+            rest[warp] = left;
         }
     }
+    if (warps > 1) {
+        __syncthreads();
+        if (warp != 0) return;
+        for (int w = 1; w < warps; w++) {
+            for (int k = 0; k < counts[w]; k++) {
+                factor(factors[w][k]);
+                apply(norms[w][k], stretches[((size_t)(w - 1) * kMaxStretches + k) * quads + min(lane, quads - 1)]);
+            }
+            replay(rest[w], (int)((long long)m.tiles * (w + 1) / warps));
+        }
+    }
+    if (lane >= quads) return;
     const long long inv = sat16(rnd((long long)llmx::recip_q16(sum < 16 ? 16 : sum), 8));
-    const int y0 = sat16(rnd((long long)a * inv, 16)), y1 = sat16(rnd((long long)d * inv, 16));
-    *reinterpret_cast<uint32_t *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 2 * e2) = (uint32_t)(y0 & 0xffff) | (uint32_t)y1 << 16;
+    auto last = [&](int y) { return (int)(((long long)y * inv + 32768) >> 16); };
+    *reinterpret_cast<uint2 *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 4 * lane) =
+        make_uint2(pack_sat16(last(x[0]), last(x[1])), pack_sat16(last(x[2]), last(x[3])));
 }
 
 // ---- append -------------------------------------------------------------------------
@@ -977,6 +1052,7 @@ struct llmx_paged {
     uint32_t max_requests = 0, max_block = 0, max_length = 0;
     long long capacity = 0;  // (key head, tile) items of a call
     size_t scores_smem = 0, values_smem = 0;
+    int scores_ctas = 0, values_ctas = 0;  // that are on the device at once
     unsigned char *memory = nullptr;
     Meta *meta = nullptr;
     int16_t *score = nullptr, *top = nullptr, *tv = nullptr, *exps = nullptr;
@@ -1074,6 +1150,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
         return fail(LLMX_ERR_ARG, "head_dim must be a multiple of 16 up to 128, got " + std::to_string(head_dim));
     if (page_len == 0 || page_len % 8 != 0 || page_len > kMaxPageLen)
         return fail(LLMX_ERR_ARG, "page_len must be a multiple of 8 up to 65536, got " + std::to_string(page_len));
+    if ((uint64_t)kv_heads * page_len * head_dim >= 1ull << 31) return fail(LLMX_ERR_ARG, "a page must hold fewer than 2^31 values");
     if (max_requests == 0 || max_requests > kMaxRequests)
         return fail(LLMX_ERR_ARG, "max_requests must be 1..1024, got " + std::to_string(max_requests));
     if (max_block == 0 || max_block > (uint32_t)llmx::kMaxRows)
@@ -1113,7 +1190,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
                  fsum_at = place(slots * 64);
     p->bytes = at;
     p->scores_smem = 2 * blocks * ((head_dim + 31) / 32) * 512 + (size_t)max_requests * sizeof(Meta);
-    p->values_smem = (size_t)stages_of((int)blocks) * stage_bytes((int)blocks) + blocks * 1024 + kExpWords * 4 +
+    p->values_smem = (size_t)kStages * stage_bytes((int)blocks) + blocks * 1024 + kExpWords * 4 +
                      (6 + kWarps) * blocks * 32 + (size_t)max_requests * sizeof(Meta);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int16_t e16[2049], host[kExpWords * 2] = {};
@@ -1130,6 +1207,14 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
         release(p);
         return cuda_fail("create", e);
     }
+    int per_sm[2] = {0, 0};
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[0], scores_kernel(p->dim), kThreads, p->scores_smem)) != cudaSuccess ||
+        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[1], (const void *)k_values, kThreads, p->values_smem)) != cudaSuccess) {
+        release(p);
+        return cuda_fail("create", e);
+    }
+    p->scores_ctas = p->sms * std::max(per_sm[0], 1);
+    p->values_ctas = p->sms * std::max(per_sm[1], 1);
     auto as = [&](auto *&ptr, size_t where) { ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(p->memory + where); };
     as(p->error, error_at);
     as(p->exps, exps_at);
@@ -1237,6 +1322,8 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.page8 = (uint32_t)p->page_len / 8;
     // p8 < 2^17 + 8 and page8 <= 2^13: (2^32 + page8 - 1) / page8 divides exactly
     c.page8_magic = (uint32_t)(((1ull << 32) + c.page8 - 1) / c.page8);
+    c.row_bytes = (uint32_t)p->dim * 2;
+    c.page_bytes = (uint32_t)p->kv * (uint32_t)p->page_len * c.row_bytes;
     c.scale8 = llmx::qk_scale_q1616(p->dim) >> 8;
     c.capacity = p->capacity;
     c.meta = p->meta;
@@ -1248,15 +1335,17 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const uint64_t items = (uint64_t)requests * p->kv * ((longest + kTile - 1) / kTile);
-    const unsigned grid = (unsigned)std::min<uint64_t>(items, (uint64_t)p->sms * 4);
-    cudaError_t e = launch(scores_kernel(p->dim), grid, kThreads, p->scores_smem, c, s);
-    if (e == cudaSuccess) e = launch((const void *)k_values, grid, kThreads, p->values_smem, c, s);
+    auto grid = [&](int ctas) { return (unsigned)std::min<uint64_t>(items, (uint64_t)ctas); };
+    cudaError_t e = launch(scores_kernel(p->dim), grid(p->scores_ctas), kThreads, p->scores_smem, c, s);
+    if (e == cudaSuccess) e = launch((const void *)k_values, grid(p->values_ctas), kThreads, p->values_smem, c, s);
     if (e == cudaSuccess) {
-        const int tiles = (int)((longest + kTile - 1) / kTile), pairs = p->dim / 2;
-        c.groups = std::min(kMaxGroups, (tiles + kAhead - 1) / kAhead);
+        const int tiles = (int)((longest + kTile - 1) / kTile);
+        // few columns: a warp per kAhead tiles, for latency; many: no more warps than fill the SMs
+        const uint64_t columns = (uint64_t)rows * p->heads;
+        const int warps = (int)std::max<uint64_t>(1, std::min<uint64_t>({kMaxJoinWarps, (uint64_t)(tiles + kAhead - 1) / kAhead, (uint64_t)p->sms * 32 / columns}));
         const bool far = tiles > kShortTiles;
-        const size_t smem = (size_t)(c.groups - 1) * kMaxStretches * pairs * (far ? 2 * sizeof(Stretch<true>) : 2 * sizeof(Stretch<false>));
-        e = launch(far ? (const void *)k_join<true> : (const void *)k_join<false>, rows * (unsigned)p->heads, (pairs * c.groups + 31) / 32 * 32, smem, c, s);
+        const size_t smem = (size_t)(warps - 1) * kMaxStretches * p->dim * (far ? sizeof(Stretch<true>) : sizeof(Stretch<false>));
+        e = launch(far ? (const void *)k_join<true> : (const void *)k_join<false>, rows * (unsigned)p->heads, 32 * warps, smem, c, s);
     }
     return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
 }
