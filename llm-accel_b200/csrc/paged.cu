@@ -28,12 +28,14 @@
 
 #include <algorithm>
 #include <climits>
+#include <cstdlib>
 #include <cstdint>
 #include <new>
 #include <string>
 #include <type_traits>
 
 #include "llmx.h"
+#include "cluster.cuh"
 #include "device_util.cuh"
 #include "fixed.cuh"
 #include "host_model.h"
@@ -81,31 +83,33 @@ struct Call {
     long long capacity;           // (key head, tile) items
     // workspace
     Meta *meta;          // [requests]
-    int16_t *score;      // [slot][8 columns][64 positions]
-    int16_t *top;        // [slot][8] maxima
+    uint32_t *score;     // [slot][64 positions][4 column pairs], biased
+    uint4 *top;          // [slot][4 blocks of 16 positions]: the maxima of 4 column pairs, biased
     int16_t *tv;         // [slot][8][dim]
     int2 *fsum;          // [slot][8]: P(m_before - m), the sum of P
-    const int16_t *exps; // [2049]
+    const int16_t *exps; // [2049] of differences 0, -1, ... -2048
     int *error;
+    int tiles, cluster_log;  // k_attend: of a CTA at most; CTAs of a (request, key head): up to 8, a power of 2
 };
 
 // ---- small pieces -------------------------------------------------------------------
 static __device__ __forceinline__ uint32_t div_page(const Call &c, uint32_t p8) {
     return c.page8 == 1 ? p8 : __umulhi(p8, c.page8_magic);
 }
-// First row of positions 8 inside .. of key head h in the page that entry `at` of a table names.
-static __device__ __forceinline__ const char *page_rows(const Call &c, const int16_t *cache, const int32_t *table, uint32_t at, uint32_t inside, int h) {
-    uint32_t page = (uint32_t)table[at];
-    if (page >= c.pages) {
-        atomicOr(c.error, kErrPage);
-        page = 0;
-    }
-    return reinterpret_cast<const char *>(cache) + (unsigned long long)page * c.page_bytes + ((uint32_t)h * c.page_len + inside * 8) * c.row_bytes;
+// The page of positions 8 p8 .. 8 p8 + 7 (page lengths are multiples of 8).  worst: the largest number met, which
+// is reported at the kernel's end; one out of range is read as the last page.
+static __device__ __forceinline__ uint32_t page_of(const Call &c, const int32_t *table, uint32_t p8, uint32_t &worst) {
+    const uint32_t page = (uint32_t)table[div_page(c, p8)];
+    worst = max(worst, page);
+    return min(page, c.pages - 1);
 }
-// First row of positions 8 p8 .. 8 p8 + 7 (page lengths are multiples of 8).
-static __device__ __forceinline__ const char *rows_at(const Call &c, const int16_t *cache, const int32_t *table, uint32_t p8, int h) {
-    const uint32_t at = div_page(c, p8);
-    return page_rows(c, cache, table, at, p8 - at * c.page8, h);
+// First of their rows of key head h.
+static __device__ __forceinline__ const char *rows_of(const Call &c, const int16_t *cache, uint32_t page, uint32_t p8, int h) {
+    const uint32_t inside = p8 - div_page(c, p8) * c.page8;
+    return reinterpret_cast<const char *>(cache) + ((unsigned long long)page * c.page_bytes + ((uint32_t)h * c.page_len + inside * 8) * c.row_bytes);
+}
+static __device__ __forceinline__ void report(const Call &c, uint32_t worst) {
+    if (worst >= c.pages) atomicOr(c.error, kErrPage);
 }
 // (not .nc: the launch before may still be writing the cache when this one starts)
 static __device__ __forceinline__ uint4 ld16(const void *p) {
@@ -113,9 +117,7 @@ static __device__ __forceinline__ uint4 ld16(const void *p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
     return v;
 }
-static __device__ __forceinline__ uint32_t min16x2(uint32_t a, uint32_t b) { return __vmins2(a, b); }
-static __device__ __forceinline__ uint32_t max16x2(uint32_t a, uint32_t b) { return __vmaxs2(a, b); }
-static __device__ __forceinline__ uint32_t limit2(uint32_t v) { return max16x2(min16x2(v, 0x08000800u), 0xf800f800u); }
+static __device__ __forceinline__ uint32_t limit2(uint32_t v) { return __vmaxs2(__vmins2(v, 0x08000800u), 0xf800f800u); }
 // Of four high bytes of limited values: 1 where the byte is 8 (the value 2048).
 static __device__ __forceinline__ uint32_t at_limit(uint32_t h) { return (h >> 3) & ~(h >> 4) & 0x01010101u; }
 // (8 - x) >> 4 of two 16-bit values, as 16 bits each
@@ -126,13 +128,12 @@ static __device__ __forceinline__ uint32_t rest2(uint32_t x) {
 static __device__ __forceinline__ uint32_t low4(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x6420); }
 static __device__ __forceinline__ uint32_t high4(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7531); }
 
-// D += A B, A 16 x 32 and B 32 x 8 bytes; S and U: signed and unsigned.
-#define LLMX_MMA(name, ta, tb)                                                                                           \
-    static __device__ __forceinline__ void name(int(&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, \
-                                                uint32_t b1) {                                                           \
-        asm("mma.sync.aligned.m16n8k32.row.col.s32." ta "." tb ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};" \
-            : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])                                                             \
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                                     \
+// D = A B + C, A 16 x 32 and B 32 x 8 bytes; s and u: signed and unsigned.
+#define LLMX_MMA(name, ta, tb)                                                                                                  \
+    static __device__ __forceinline__ void name(int(&d)[4], const uint32_t(&a)[4], uint32_t b0, uint32_t b1, const int(&c)[4]) { \
+        asm("mma.sync.aligned.m16n8k32.row.col.s32." ta "." tb ".s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"  \
+            : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])                                                                     \
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(c[0]), "r"(c[1]), "r"(c[2]), "r"(c[3]));          \
     }
 LLMX_MMA(mma_su, "s8", "u8")
 LLMX_MMA(mma_us, "u8", "s8")
@@ -166,6 +167,14 @@ static __device__ __noinline__ int score_exact(const int16_t *q, const int16_t *
     return score_of(sat32(t), scale8);
 }
 
+// Rows and tiles of request b; false where it is void.
+static __device__ __forceinline__ bool request(const Call &c, uint32_t b, int &rows, int &tiles) {
+    const uint32_t o0 = c.offsets[b], o1 = c.offsets[b + 1], length = c.lengths[b];
+    rows = (int)(o1 - o0);
+    tiles = rows ? (int)((length + kTile - 1) / kTile) : 0;
+    return o0 <= o1 && o1 <= c.rows && o1 - o0 <= (uint32_t)c.max_block && length <= c.longest;
+}
+
 // The requests' first slots and items, into shared memory (and by CTA 0 into the
 // workspace); returns the number of items, 0 when the call needs more than the handle has.
 static __device__ int plan(const Call &c, Meta *meta) {
@@ -177,10 +186,10 @@ static __device__ int plan(const Call &c, Meta *meta) {
         Meta m{0, 0, 0, -1};
         long long s = 0, i = 0;
         if (b < c.requests) {
-            const uint32_t o0 = c.offsets[b], o1 = c.offsets[b + 1], length = c.lengths[b];
-            if (o0 <= o1 && o1 <= c.rows && o1 - o0 <= (uint32_t)c.max_block && length <= c.longest) {
-                m.rows = (int)(o1 - o0);
-                m.tiles = m.rows ? (int)((length + kTile - 1) / kTile) : 0;
+            int rows, tiles;
+            if (request(c, b, rows, tiles)) {
+                m.rows = rows;
+                m.tiles = tiles;
                 i = (long long)c.kv * m.tiles;
                 s = i * ((m.rows * c.group + 7) / 8);
             } else if (blockIdx.x == 0) {
@@ -230,10 +239,17 @@ static __device__ int plan(const Call &c, Meta *meta) {
     return fits ? (int)items : 0;
 }
 
+// A (request, key head) at hand.
+struct Strip {
+    const int32_t *table;
+    int h, rows, length, blocks;
+    uint32_t row0;
+};
 // One (request, key head, tile) after another.
 struct Cursor {
     int b, h, t;  // request, key head, tile
     int tiles, rows, length, blocks;
+    uint32_t row0;
     int slot0;    // of tile 0 in the first column block of this key head
     const int32_t *table;
 
@@ -244,6 +260,7 @@ struct Cursor {
         tiles = m.tiles;
         rows = m.rows;
         length = (int)c.lengths[b];
+        row0 = c.offsets[b];
         blocks = (rows * c.group + 7) >> 3;
         slot0 = m.slot + h * blocks * tiles;
         table = c.table + (size_t)b * c.ld_table;
@@ -276,6 +293,7 @@ struct Cursor {
     }
     // Slot of this tile in column block nb.
     __device__ int slot(int nb) const { return slot0 + nb * tiles + t; }
+    __device__ Strip strip() const { return Strip{table, h, rows, length, blocks, row0}; }
 };
 
 static __device__ __forceinline__ void range_of(int items, int &first, int &end) {
@@ -285,229 +303,391 @@ static __device__ __forceinline__ void range_of(int items, int &first, int &end)
 }
 
 // ---- scores -------------------------------------------------------------------------
-// What k_scores keeps of a column (a query row) of the (request, key head) at hand.
-struct __align__(16) Column {
-    int seen;  // positions that it sees
-    int bias;  // 2048 times its sum
-    int wide;  // a bank may saturate
-    int pad;
-};
+// Scores are kept biased (with the sign bit turned), so that unsigned minima, maxima and
+// differences of packed pairs do.
+constexpr uint32_t kBias2 = 0x80008000u;
 
-// A warp scores 16 positions against 8 columns (query rows) at a time: the positions are
-// the rows of A, and a lane's 16-byte load of a key row's 8 dimensions is, split into
-// bytes, its share of A for both byte planes; no shared memory is passed through.  The
-// queries' shares of B, with those of (8 - q) >> 4, wait in shared memory.  Keys are limited by two
-// instructions a pair: min(k, 2048), then max(k + 2048, 0), so both planes are
-// unsigned and 2048 times the sum of q is taken off again.
-template <int KS>  // steps of 32 dimensions
-__global__ void __launch_bounds__(kThreads, 5) k_scores(const Call c) {
+// What a CTA keeps of a column (a query row) of the (request, key head) at hand.
+struct Column {
+    int bias[kMaxColumns];  // 2048 times its sum
+    int seen[kMaxColumns];  // positions that it sees
+    int wide[kMaxColumns];  // a bank may saturate
+};
+// Queries as the lanes' shares of B, [block][KS][32 lanes] {low, low, high, high}, and the same of
+// (8 - q) >> 4; by `warps` warps.
+template <int KS>
+static __device__ __forceinline__ void stage_queries(const Call &c, const Strip &z, int warp, int warps, uint4 *queries, uint4 *rests, Column &column) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int columns = z.rows * c.group;
+    for (int nb = warp; nb < z.blocks; nb += warps) {
+        const int col = nb * 8 + g, j = col / c.group;
+        const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + col - j * c.group) * c.dim + 8 * t4;
+        uint32_t big = 0;
+        int sum = 0;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const uint4 w = col < columns && 32 * s + 8 * t4 < c.dim ? *reinterpret_cast<const uint4 *>(q + 32 * s) : make_uint4(0, 0, 0, 0);
+            // above 8192: the top three of 16 bits differ
+            big |= (w.x ^ (w.x << 1)) | (w.x ^ (w.x << 2)) | (w.y ^ (w.y << 1)) | (w.y ^ (w.y << 2)) | (w.z ^ (w.z << 1)) | (w.z ^ (w.z << 2)) |
+                   (w.w ^ (w.w << 1)) | (w.w ^ (w.w << 2));
+            // (a total reaches 2^31 only where every q is -8192, the first one too)
+            if (s == 0 && t4 == 0 && (w.x & 0xffffu) == 0xe000u) big |= 0x8000u;
+            sum += llmx::lo16(w.x) + llmx::hi16(w.x) + llmx::lo16(w.y) + llmx::hi16(w.y) + llmx::lo16(w.z) + llmx::hi16(w.z) + llmx::lo16(w.w) +
+                   llmx::hi16(w.w);
+            queries[(nb * KS + s) * 32 + lane] = make_uint4(low4(w.x, w.y), low4(w.z, w.w), high4(w.x, w.y), high4(w.z, w.w));
+            const uint4 r = make_uint4(rest2(w.x), rest2(w.y), rest2(w.z), rest2(w.w));
+            rests[(nb * KS + s) * 32 + lane] = make_uint4(low4(r.x, r.y), low4(r.z, r.w), high4(r.x, r.y), high4(r.z, r.w));
+        }
+        big |= __shfl_xor_sync(0xffffffffu, big, 1);
+        big |= __shfl_xor_sync(0xffffffffu, big, 2);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        if (t4 == 0) {
+            column.bias[col] = 2048 * sum;
+            column.seen[col] = col < columns ? z.length - z.rows + 1 + j : 0;
+            column.wide[col] = (int)(big & 0x80008000u);
+        }
+    }
+}
+
+// The pages of 16 positions' keys, and this lane's share of them: rows g and g + 8, dimensions 32 s + 8 t4
+// .. + 7; zeros for what is not there.
+struct KeyPages {
+    uint32_t page[2];
+    __device__ __forceinline__ void load(const Call &c, const Strip &z, int p0, uint32_t &worst) {
+#pragma unroll
+        for (int r = 0; r < 2; r++) page[r] = p0 + 8 * r < z.length ? page_of(c, z.table, (uint32_t)(p0 >> 3) + r, worst) : 0;
+    }
+};
+template <int KS>
+static __device__ __forceinline__ void load_keys(const Call &c, const Strip &z, const KeyPages &pages, int p0, uint4 (&raw)[2][KS]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const char *row[2];
+#pragma unroll
+    for (int r = 0; r < 2; r++) row[r] = rows_of(c, c.k, pages.page[r], (uint32_t)(p0 >> 3) + r, z.h) + (g * c.row_bytes + 16 * t4);
+    if (p0 + 16 <= z.length && c.dim == 32 * KS) {
+#pragma unroll
+        for (int r = 0; r < 2; r++)
+#pragma unroll
+            for (int s = 0; s < KS; s++) raw[r][s] = ld16(row[r] + 64 * s);
+        return;
+    }
+#pragma unroll
+    for (int r = 0; r < 2; r++)
+#pragma unroll
+        for (int s = 0; s < KS; s++) raw[r][s] = p0 + 8 * r + g < z.length && 32 * s + 8 * t4 < c.dim ? ld16(row[r] + 64 * s) : make_uint4(0, 0, 0, 0);
+}
+// Their byte planes, limited and from 0 to 4096: min(k, 2048), then max(k + 2048, 0).  Returns whether some
+// value of the warp's is at the upper limit (its high byte is 16).
+template <int KS>
+static __device__ __forceinline__ bool key_planes(const uint4 (&raw)[2][KS], uint32_t (&kl)[KS][4], uint32_t (&kh)[KS][4]) {
+    uint32_t limit = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            auto shift = [](uint32_t w) { return __viaddmax_s16x2(__vmins2(w, 0x08000800u), 0x08000800u, 0u); };
+            const uint4 w = make_uint4(shift(raw[r][s].x), shift(raw[r][s].y), shift(raw[r][s].z), shift(raw[r][s].w));
+            kl[s][r] = low4(w.x, w.y);
+            kl[s][r + 2] = low4(w.z, w.w);
+            kh[s][r] = high4(w.x, w.y);
+            kh[s][r + 2] = high4(w.z, w.w);
+            limit |= kh[s][r] | kh[s][r + 2];
+        }
+    return __any_sync(0xffffffffu, (limit & 0x10101010u) != 0);
+}
+
+// A warp scores 16 positions (the rows of A, a lane's 16-byte loads of key rows split into bytes)
+// against the 8 columns (query rows) of block nb: w[0] position p0 + g, w[1] p0 + 8 + g, columns
+// 2 t4 and 2 t4 + 1, biased.  Returns their columns' maxima over the positions that they see, in
+// lanes 0 to 3 (of column pair t4).
+template <int KS>
+static __device__ __forceinline__ uint32_t score_block(const Call &c, const Strip &z, const uint32_t (&kl)[KS][4], const uint32_t (&kh)[KS][4], bool some,
+                                                       int nb, int p0, const uint4 *queries, const uint4 *rests, const Column &column, uint32_t (&w)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+    const int2 bias = *reinterpret_cast<const int2 *>(&column.bias[nb * 8 + 2 * t4]);
+    int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {-bias.x, -bias.y, -bias.x, -bias.y};
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        const uint4 q = queries[(nb * KS + s) * 32 + lane];
+        mma_us(hh, kh[s], q.z, q.w, hh);
+        mma_uu(mid, kh[s], q.x, q.y, mid);
+        mma_uu(ll, kl[s], q.x, q.y, ll);
+        mma_us(mid, kl[s], q.z, q.w, mid);
+    }
+    if (some) {
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const uint4 r = rests[(nb * KS + s) * 32 + lane];
+            uint32_t m[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) m[i] = kh[s][i] >> 4 & 0x01010101u;
+            mma_us(mid, m, r.z, r.w, mid);
+            mma_uu(ll, m, r.x, r.y, ll);
+        }
+    }
+    int sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) sc[i] = score_of((int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]), c.scale8);
+    const int2 wide = *reinterpret_cast<const int2 *>(&column.wide[nb * 8 + 2 * t4]);
+    if (__any_sync(0xffffffffu, (wide.x | wide.y) != 0)) {
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+            const int col = nb * 8 + 2 * t4 + (i & 1), p = p0 + g + (i >> 1) * 8;
+            if (!column.wide[col] || p >= z.length) continue;
+            uint32_t none = 0;
+            const int j = col / c.group;
+            const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + col - j * c.group) * c.dim;
+            const int16_t *k = reinterpret_cast<const int16_t *>(rows_of(c, c.k, page_of(c, z.table, (uint32_t)p >> 3, none), (uint32_t)p >> 3, z.h) + (p & 7) * c.row_bytes);
+            const int y = score_exact(q, k, c.dim, c.scale8);
+            if (i == 0) sc[0] = y;
+            else if (i == 1) sc[1] = y;
+            else if (i == 2) sc[2] = y;
+            else sc[3] = y;
+        }
+    }
+    w[0] = pack_sat16(sc[0], sc[1]) ^ kBias2;
+    w[1] = pack_sat16(sc[2], sc[3]) ^ kBias2;
+    uint32_t top = __vmaxu2(w[0], w[1]);
+    if (p0 + 16 > z.length - z.rows + 1) {  // some column does not see all 16 positions
+        const int2 n = *reinterpret_cast<const int2 *>(&column.seen[nb * 8 + 2 * t4]);
+        auto seen = [&](int p) { return (p < n.x ? 0xffffu : 0u) | (p < n.y ? 0xffff0000u : 0u); };
+        top = __vmaxu2(w[0] & seen(p0 + g), w[1] & seen(p0 + 8 + g));
+    }
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, o));
+    return top;
+}
+
+// One CTA's run of tiles, a warp per 16 positions.
+template <int KS, bool kOne>  // steps of 32 dimensions; one column block
+__global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ int tops[2][kWarps][kMaxColumns];
-    __shared__ Column column[kMaxColumns];
-    const int most = (c.max_block * c.group + 7) / 8;  // column blocks
-    uint4 *queries = reinterpret_cast<uint4 *>(dynamic);  // [most][KS][32 lanes] {low, low, high, high}
-    uint4 *rests = queries + most * KS * 32;              // the same of (8 - q) >> 4
+    __shared__ __align__(16) Column column;
+    const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;  // column blocks
+    uint4 *queries = reinterpret_cast<uint4 *>(dynamic);          // [most][KS][32]
+    uint4 *rests = queries + most * KS * 32;
     Meta *meta = reinterpret_cast<Meta *>(rests + most * KS * 32);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     pdl_trigger();
     const int items = plan(c, meta);
     int first, end;
     range_of(items, first, end);
     if (first >= end) return;
-
+    uint32_t worst = 0;
     Cursor cur;
     cur.start(c, meta, first);
-    uint4 raw[2][KS];  // key rows g and g + 8 of the warp's 16 positions
-    auto load = [&](const Cursor &u) {
-        const int p0 = u.t * kTile + warp * 16;
-        if (p0 + 16 <= u.length && c.dim == 32 * KS) {
-            const uint32_t p8 = (uint32_t)p0 >> 3, at = div_page(c, p8), inside = p8 - at * c.page8;
-            const char *row = page_rows(c, c.k, u.table, at, inside, u.h) + g * (64 * KS) + 16 * t4;
-#pragma unroll
-            for (int s = 0; s < KS; s++) raw[0][s] = ld16(row + 64 * s);
-            // 8 positions on: in the same page, or at the next one's start
-            row = inside + 1 < c.page8 ? row + 8 * 64 * KS : page_rows(c, c.k, u.table, at + 1, 0, u.h) + g * (64 * KS) + 16 * t4;
-#pragma unroll
-            for (int s = 0; s < KS; s++) raw[1][s] = ld16(row + 64 * s);
-            return;
-        }
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            const int p = p0 + 8 * r;
-            const char *row = p < u.length ? rows_at(c, c.k, u.table, (uint32_t)p >> 3, u.h) + g * c.row_bytes + 16 * t4 : nullptr;
-#pragma unroll
-            for (int s = 0; s < KS; s++)
-                raw[r][s] = p + g < u.length && 32 * s + 8 * t4 < c.dim ? ld16(row + 64 * s) : make_uint4(0, 0, 0, 0);
-        }
-    };
-    load(cur);
-    bool moved = true;
-    for (int item = first; item < end; item++) {
-        const Cursor now = cur;
-        if (moved) {
-            __syncthreads();  // the last key head's columns are done with
-            const int columns = now.rows * c.group;
-            const uint32_t row0 = c.offsets[now.b];
-            for (int nb = warp; nb < now.blocks; nb += kWarps) {
-                const int col = nb * 8 + g, j = col / c.group;
-                const int16_t *q = c.q + (size_t)(row0 + j) * c.ld_q + (size_t)(now.h * c.group + col - j * c.group) * c.dim + 8 * t4;
-                uint32_t big = 0;
-                int sum = 0;
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const uint4 w = col < columns && 32 * s + 8 * t4 < c.dim ? *reinterpret_cast<const uint4 *>(q + 32 * s) : make_uint4(0, 0, 0, 0);
-                    // above 8192: the top three of 16 bits differ
-                    big |= (w.x ^ (w.x << 1)) | (w.x ^ (w.x << 2)) | (w.y ^ (w.y << 1)) | (w.y ^ (w.y << 2)) | (w.z ^ (w.z << 1)) |
-                           (w.z ^ (w.z << 2)) | (w.w ^ (w.w << 1)) | (w.w ^ (w.w << 2));
-                    // (a total reaches 2^31 only where every q is -8192, the first one too)
-                    if (s == 0 && t4 == 0 && (w.x & 0xffffu) == 0xe000u) big |= 0x8000u;
-                    sum += llmx::lo16(w.x) + llmx::hi16(w.x) + llmx::lo16(w.y) + llmx::hi16(w.y) + llmx::lo16(w.z) + llmx::hi16(w.z) +
-                           llmx::lo16(w.w) + llmx::hi16(w.w);
-                    queries[(nb * KS + s) * 32 + lane] = make_uint4(low4(w.x, w.y), low4(w.z, w.w), high4(w.x, w.y), high4(w.z, w.w));
-                    const uint4 r = make_uint4(rest2(w.x), rest2(w.y), rest2(w.z), rest2(w.w));
-                    rests[(nb * KS + s) * 32 + lane] = make_uint4(low4(r.x, r.y), low4(r.z, r.w), high4(r.x, r.y), high4(r.z, r.w));
-                }
-                big |= __shfl_xor_sync(0xffffffffu, big, 1);
-                big |= __shfl_xor_sync(0xffffffffu, big, 2);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-                if (t4 == 0) column[col] = Column{col < columns ? now.length - now.rows + 1 + j : 0, 2048 * sum, (int)(big & 0x80008000u), 0};
-            }
-            __syncthreads();
-        }
-        const int p0 = now.t * kTile + warp * 16;
-        // byte planes of the keys, from 0 to 4096
-        uint32_t kh[KS][4], kl[KS][4], limit = 0;
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                auto shift = [](uint32_t w) { return __viaddmax_s16x2(min16x2(w, 0x08000800u), 0x08000800u, 0u); };
-                const uint4 w = make_uint4(shift(raw[r][s].x), shift(raw[r][s].y), shift(raw[r][s].z), shift(raw[r][s].w));
-                kl[s][r] = low4(w.x, w.y);
-                kl[s][r + 2] = low4(w.z, w.w);
-                kh[s][r] = high4(w.x, w.y);
-                kh[s][r + 2] = high4(w.z, w.w);
-                limit |= kh[s][r] | kh[s][r + 2];
-            }
-        // some high byte is 16: the value 4096, at the upper limit
-        const bool some = __any_sync(0xffffffffu, (limit & 0x10101010u) != 0);
-        // the next item's keys are on their way while this one's are used
-        if (item + 1 < end) {
-            moved = cur.next(c, meta);
-            load(cur);
-        }
-        int(&top_of)[kMaxColumns] = tops[item & 1][warp];
-        if (p0 >= now.length)
-            for (int col = lane; col < now.blocks * 8; col += 32) top_of[col] = -32768;
-        const bool whole = p0 + 16 <= now.length - now.rows + 1;  // every column sees all 16 positions
-        for (int nb = 0; p0 < now.length && nb < now.blocks; nb++) {
-            int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int s = 0; s < KS; s++) {
-                const uint4 q = queries[(nb * KS + s) * 32 + lane];
-                mma_us(hh, kh[s][0], kh[s][1], kh[s][2], kh[s][3], q.z, q.w);
-                mma_uu(mid, kh[s][0], kh[s][1], kh[s][2], kh[s][3], q.x, q.y);
-                mma_uu(ll, kl[s][0], kl[s][1], kl[s][2], kl[s][3], q.x, q.y);
-                mma_us(mid, kl[s][0], kl[s][1], kl[s][2], kl[s][3], q.z, q.w);
-            }
-            if (some) {
-#pragma unroll
-                for (int s = 0; s < KS; s++) {
-                    const uint4 r = rests[(nb * KS + s) * 32 + lane];
-                    uint32_t m[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) m[i] = kh[s][i] >> 4 & 0x01010101u;
-                    mma_us(mid, m[0], m[1], m[2], m[3], r.z, r.w);
-                    mma_uu(ll, m[0], m[1], m[2], m[3], r.x, r.y);
-                }
-            }
-            const Column ca = column[nb * 8 + 2 * t4], cb = column[nb * 8 + 2 * t4 + 1];
-            int sc[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                sc[i] = score_of((int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i] - (uint32_t)(i & 1 ? cb.bias : ca.bias)),
-                                 c.scale8);
-            if (__any_sync(0xffffffffu, (ca.wide | cb.wide) != 0)) {
-#pragma unroll 1
-                for (int i = 0; i < 4; i++) {
-                    const int col = nb * 8 + 2 * t4 + (i & 1), p = p0 + g + (i >> 1) * 8;
-                    if (!column[col].wide || p >= now.length) continue;
-                    const int j = col / c.group;
-                    const int16_t *q = c.q + (size_t)(c.offsets[now.b] + j) * c.ld_q + (size_t)(now.h * c.group + col - j * c.group) * c.dim;
-                    const int y = score_exact(q, reinterpret_cast<const int16_t *>(rows_at(c, c.k, now.table, (uint32_t)p >> 3, now.h) + (p & 7) * c.row_bytes), c.dim, c.scale8);
-                    if (i == 0) sc[0] = y;
-                    else if (i == 1) sc[1] = y;
-                    else if (i == 2) sc[2] = y;
-                    else sc[3] = y;
-                }
-            }
-            // column g, positions 2 t4, 2 t4 + 1 (and + 8) after the transposition
-            const uint32_t w0 = transpose8(pack_sat16(sc[0], sc[1])), w1 = transpose8(pack_sat16(sc[2], sc[3]));
-            uint32_t *dst = reinterpret_cast<uint32_t *>(c.score + ((size_t)now.slot(nb) * 8 + g) * kTile + warp * 16 + 2 * t4);
-            dst[0] = w0;
-            dst[4] = w1;
-            uint32_t top = max16x2(w0, w1);
-            if (!whole) {
-                const int seen = column[nb * 8 + g].seen - (p0 + 2 * t4);
-                auto masked = [](uint32_t w, int n) { return n >= 2 ? w : n == 1 ? (w & 0xffffu) | 0x80000000u : 0x80008000u; };
-                top = max16x2(masked(w0, seen), masked(w1, seen - 8));
-            }
-            top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = max16x2(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            if (t4 == 0) top_of[nb * 8 + g] = max(llmx::lo16(top), llmx::hi16(top));
-        }
+    Strip z = cur.strip();
+    uint4 raw[2][KS];
+    KeyPages pages;
+    pages.load(c, z, cur.t * kTile + warp * 16, worst);
+    load_keys<KS>(c, z, pages, cur.t * kTile + warp * 16, raw);
+    if (cur.t + 1 < cur.tiles) pages.load(c, z, (cur.t + 1) * kTile + warp * 16, worst);
+    for (int item = first; item < end;) {  // a (request, key head)
+        __syncthreads();                   // the last one's columns are done with
+        stage_queries<KS>(c, z, warp, kWarps, queries, rests, column);
         __syncthreads();
-        // (the other buffer is in use until every thread is here again)
-        for (int col = threadIdx.x; col < now.blocks * 8; col += kThreads) {
-            int top = tops[item & 1][0][col];
-#pragma unroll
-            for (int w = 1; w < kWarps; w++) top = max(top, tops[item & 1][w][col]);
-            c.top[(size_t)now.slot(col >> 3) * 8 + (col & 7)] = (int16_t)top;
+        const int n = min(cur.tiles - cur.t, end - item);
+        size_t at = (size_t)cur.slot(0) * 4 + warp;  // the block of 16 positions in the first column block
+        const size_t step = (size_t)cur.tiles * 4;
+        int p0 = cur.t * kTile + warp * 16;
+        const Strip here = z;
+        for (int k = 0; k < n; k++, p0 += kTile, at += 4) {
+            uint32_t kh[KS][4], kl[KS][4];
+            const bool some = key_planes<KS>(raw, kl, kh);
+            // the next tile's keys are on their way while this one's are used, the next one's page numbers too
+            if (k + 1 < n) {
+                load_keys<KS>(c, z, pages, p0 + kTile, raw);
+                if (k + 2 < n) pages.load(c, z, p0 + 2 * kTile, worst);
+            } else if (item + n < end) {
+                cur.t += n - 1;
+                cur.next(c, meta);
+                z = cur.strip();
+                pages.load(c, z, warp * 16, worst);
+                load_keys<KS>(c, z, pages, warp * 16, raw);
+                if (cur.tiles > 1) pages.load(c, z, kTile + warp * 16, worst);
+            }
+            for (int nb = 0; nb < (kOne ? 1 : here.blocks); nb++) {
+                const size_t block = at + nb * step;
+                uint32_t top = 0;  // (-32768)
+                if (p0 < here.length) {
+                    uint32_t w[2];
+                    top = score_block<KS>(c, here, kl, kh, some, nb, p0, queries, rests, column, w);
+                    c.score[block * 64 + lane] = w[0];
+                    c.score[block * 64 + 32 + lane] = w[1];
+                }
+                if (lane < 4) reinterpret_cast<uint32_t *>(c.top)[block * 4 + lane] = top;
+            }
         }
+        item += n;
     }
+    report(c, worst);
 }
 
 // ---- values -------------------------------------------------------------------------
-constexpr int kExpWords = 1028;  // 2049 entries of 16 bits, rounded up to 16 bytes
-constexpr int kRowBytes = 256;   // of a value row in shared memory
-constexpr int kValueBytes = kTile * kRowBytes;
+constexpr int kExpWords = 1028;                 // 2049 entries of 16 bits, rounded up to 16 bytes
+constexpr int kDepth = 2;                       // tiles of a warp's ring
+constexpr int kSlice = kTile * 64;              // bytes of a tile's share: 64 positions, 32 elements
+constexpr int kRing = kWarps * kDepth * kSlice;
 
-// A stage of k_values' ring: a tile's value rows, then per column block the scores (1 KB) and maxima
-// (16 bytes).
-static __host__ __device__ int stage_bytes(int blocks) { return kValueBytes + blocks * (8 * kTile * 2 + 16); }
-constexpr int kStages = 2;
-
-static __device__ __forceinline__ void copy16(void *dst, const void *src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
-}
-static __device__ __forceinline__ void copy16(void *dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0)
-                 : "memory");
+static __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-// A warp forms 32 of a tile's elements: the elements are the rows of A, so that a lane needs
-// the bytes of four positions in a word, a 4 x 4 transposition of bytes in its
-// registers.  Value rows come through shared memory, whole lines at a time: 16 bytes go to
-// unit u ^ 2 (row / 8 mod 4) of their row, so that the four rows that a quarter of a warp
-// reads lie in different banks.  A tile's probabilities are formed once, by all
-// warps, and pass through shared memory in the order of B.
-__global__ void __launch_bounds__(kThreads, 5) k_values(const Call c) {
+// A tile's values of 32 elements into a warp's ring: a position's 64 bytes in a row, its 16-byte units
+// turned by row / 2 mod 4, so that the 8 rows that a matrix load takes, and those that a copy writes, lie in
+// different banks.  A lane copies one unit of 8 positions, from one page.
+static __device__ __forceinline__ void fetch_values(const Call &c, const Strip &z, int t, int part, unsigned char *ring, uint32_t &worst) {
+    const int lane = threadIdx.x & 31, unit = lane & 3, j = lane >> 2;
+    const int left = z.length - t * kTile - 8 * j;  // positions from this lane's first on
+    const uint32_t p8 = (uint32_t)(t * 8 + j);
+    // (what is not there may hold anything: the probabilities there are 0)
+    if (left <= 0 || part * 32 + unit * 8 >= c.dim) return;
+    const char *rows = rows_of(c, c.v, page_of(c, z.table, p8, worst), p8, z.h) + (part * 64 + unit * 16);
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring) + j * 512;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const uint32_t r = (i + j) & 7;  // (rows in another order for each lane: in different banks)
+        copy16(dst + r * 64 + ((unit ^ (r >> 1)) & 3) * 16, rows + r * c.row_bytes, (int)r < left);
+    }
+}
+static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// The four registers of an octet of elements: the words of positions 8 j + 2 t4, + 1, element g.
+static __device__ __forceinline__ void load_octet(uint32_t at, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+// Byte planes of a tile's 32 elements as A: [step of 32 positions][16 elements].  A lane's bytes of positions
+// are those of 8 j + 2 t4 and the next, j = 0, 1 (first words) and j = 2, 3.  Returns whether values were limited.
+static __device__ __forceinline__ bool value_planes(const unsigned char *ring, uint32_t (&vl)[2][2][4], uint32_t (&vh)[2][2][4]) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t row = (uint32_t)__cvta_generic_to_shared(ring) + lane * 64;
+    const int turn = lane >> 1 & 3;
+    bool limit = false;
+#pragma unroll 1
+    for (;;) {
+        uint32_t out = 0;
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int o = 0; o < 4; o++) {
+                uint32_t r[4];
+                load_octet(row + s * 2048 + ((o ^ turn) * 16), r);
+                if (limit)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) r[i] = limit2(r[i]);
+                vl[s][o >> 1][o & 1] = low4(r[0], r[1]);
+                vl[s][o >> 1][2 + (o & 1)] = low4(r[2], r[3]);
+                vh[s][o >> 1][o & 1] = high4(r[0], r[1]);
+                vh[s][o >> 1][2 + (o & 1)] = high4(r[2], r[3]);
+#pragma unroll
+                for (int i = 0; i < 2; i++) out |= vh[s][o >> 1][2 * i + (o & 1)] ^ (vh[s][o >> 1][2 * i + (o & 1)] << 1);
+            }
+        // some high byte is not in [-8, 7] (its bits 3 to 7 differ): limited, once more
+        if (limit || !__any_sync(0xffffffffu, (out & 0xf0f0f0f0u) != 0)) return limit;
+        limit = true;
+    }
+}
+
+// Probabilities of 16 positions (block blk of a tile) against 8 columns, as bytes in the order of B.
+// Lane: column pair lane & 3, positions 8 r + 2 t and the next; s: their scores, biased; m: the pair's
+// maxima; prob: [2 steps][32 lanes] {low, low, high, high}.
+static __device__ __forceinline__ void probabilities(const int16_t *exps, uint32_t s0, uint32_t s1, uint32_t m, bool whole, int p, int seen0, int seen1, int blk,
+                                                     uint4 *prob) {
+    const int lane = threadIdx.x & 31, cp = lane & 3, t = lane >> 2 & 3, r = lane >> 4;
+    const uint32_t floor = __vmaxu2(m, 0x08000800u) - 0x08000800u;
+    // differences to the maximum, 0 to 2048 (what is not seen may hold anything)
+    const uint32_t d0 = m - __vminu2(__vmaxu2(s0, floor), m), d1 = m - __vminu2(__vmaxu2(s1, floor), m);
+    uint32_t a0 = (uint16_t)exps[d0 & 0xffffu], b0 = (uint16_t)exps[d0 >> 16], a1 = (uint16_t)exps[d1 & 0xffffu], b1 = (uint16_t)exps[d1 >> 16];
+    if (!whole) {
+        if (p >= seen0) a0 = 0;
+        if (p >= seen1) b0 = 0;
+        if (p + 1 >= seen0) a1 = 0;
+        if (p + 1 >= seen1) b1 = 0;
+    }
+    const uint32_t a = __byte_perm(a0, a1, 0x5140), b = __byte_perm(b0, b1, 0x5140);  // {low, low, high, high}
+    uint16_t *dst = reinterpret_cast<uint16_t *>(prob + (blk >> 1) * 32 + cp * 8 + t) + 2 * (blk & 1) + r;
+    dst[0] = (uint16_t)a;
+    dst[4] = (uint16_t)(a >> 16);
+    dst[32] = (uint16_t)b;
+    dst[36] = (uint16_t)(b >> 16);
+}
+
+// A tile's values against 8 columns: y[o] is the word of column g, elements 8 o + 2 t4 and the next, of
+// the part's 32.  sum: lanes 0 to 3 get the columns' sums of P (2 t4 and 2 t4 + 1).
+static __device__ __forceinline__ void weigh(const uint32_t (&vl)[2][2][4], const uint32_t (&vh)[2][2][4], bool limit, const uint4 *prob, uint32_t (&y)[4],
+                                             bool with_sum, int (&sum)[2]) {
+    const int lane = threadIdx.x & 31;
+    const uint4 b[2] = {prob[lane], prob[32 + lane]};
+#pragma unroll
+    for (int mb = 0; mb < 2; mb++) {
+        // rnd8 of rnd6 of the sum is (sum + 2^5 + 2^13) >> 14; the sum is below 2^31 - 2^16
+        int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {8224, 8224, 8224, 8224};
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            mma_su(hh, vh[s][mb], b[s].z, b[s].w, hh);
+            mma_su(mid, vh[s][mb], b[s].x, b[s].y, mid);
+            mma_uu(ll, vl[s][mb], b[s].x, b[s].y, ll);
+            mma_uu(mid, vl[s][mb], b[s].z, b[s].w, mid);
+            if (limit) {
+                const uint32_t r0 = rest2(__byte_perm(b[s].x, b[s].z, 0x5140)), r1 = rest2(__byte_perm(b[s].x, b[s].z, 0x7362));
+                const uint32_t r2 = rest2(__byte_perm(b[s].y, b[s].w, 0x5140)), r3 = rest2(__byte_perm(b[s].y, b[s].w, 0x7362));
+                uint32_t m[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) m[i] = at_limit(vh[s][mb][i]);
+                mma_us(mid, m, high4(r0, r1), high4(r2, r3), mid);
+                mma_uu(ll, m, low4(r0, r1), low4(r2, r3), ll);
+            }
+        }
+        int v[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = (int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]) >> 14;
+        y[2 * mb] = transpose8(pack_sat16(v[0], v[1]));
+        y[2 * mb + 1] = transpose8(pack_sat16(v[2], v[3]));
+    }
+    if (with_sum) {
+        const uint32_t one[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+        int low[4] = {0, 0, 0, 0}, high[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            mma_uu(low, one, b[s].x, b[s].y, low);
+            mma_uu(high, one, b[s].z, b[s].w, high);
+        }
+        sum[0] = low[0] + 256 * high[0];
+        sum[1] = low[1] + 256 * high[1];
+    }
+}
+
+constexpr int kChunk = 4;  // tiles of a (request, key head) whose probabilities k_values forms at once
+
+// The warps' shares of a tile's elements: `part` of 32, and with fewer parts than warps every `step`-th tile.
+struct Share {
+    int part, first, step;
+    __device__ __forceinline__ Share(int dim, int warp) {
+        const int log = dim > 64 ? 2 : dim > 32 ? 1 : 0;  // 4, 2 or 1 (of three parts the fourth warp has none)
+        part = warp & ((1 << log) - 1);
+        first = part * 32 < dim ? warp >> log : INT_MAX;
+        step = kWarps >> log;
+    }
+};
+
+// One CTA's run of tiles, in chunks of up to kChunk: their probabilities, by all warps, through shared
+// memory; then every warp weighs its 32 elements of every tile, for itself.
+template <bool kOne>
+__global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const int most = (c.max_block * c.group + 7) / 8;  // column blocks
-    constexpr int stages = kStages;
-    const int stage_size = stage_bytes(most);
-    unsigned char *ring = dynamic;
-    uint4 *prob = reinterpret_cast<uint4 *>(ring + stages * stage_size);  // [most][2 steps][32 lanes] {low, low, high, high}
-    uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + most * 64);
-    const int16_t *exps = reinterpret_cast<const int16_t *>(exps_w) + 2048;  // of differences <= 0
-    int *seen = reinterpret_cast<int *>(exps_w + kExpWords);  // [most * 8] positions that a column sees
-    int *psum = seen + most * 8;                              // [4][most * 8] sums of P over 16 positions
-    int *factor = psum + 4 * most * 8;                        // [most * 8]
-    int *before = factor + most * 8 + warp * most * 8;        // [most * 8] the warp's own running maxima
-    Meta *meta = reinterpret_cast<Meta *>(factor + (1 + kWarps) * most * 8);
+    const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;  // column blocks
+    const int chunk = kOne ? kChunk : max(1, kChunk / most);
+    unsigned char *ring = dynamic + warp * kDepth * kSlice;
+    uint4 *prob = reinterpret_cast<uint4 *>(dynamic + kRing);                    // [chunk][most][64]
+    uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + chunk * most * 64);
+    const int16_t *exps = reinterpret_cast<const int16_t *>(exps_w);
+    uint32_t *runs = exps_w + kExpWords;         // [chunk + 1][most * 4] maxima of column pairs up to a tile
+    uint32_t *parts_top = runs + (chunk + 1) * most * 4;  // [kWarps][most * 4]
+    int *seen = reinterpret_cast<int *>(parts_top + kWarps * most * 4);  // [most * 8]
+    Meta *meta = reinterpret_cast<Meta *>(seen + most * 8);
     for (int i = threadIdx.x; i < kExpWords; i += kThreads) exps_w[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
     pdl_wait();
     pdl_trigger();
@@ -519,209 +699,125 @@ __global__ void __launch_bounds__(kThreads, 5) k_values(const Call c) {
     int first, end;
     range_of(items, first, end);
     if (first >= end) return;
-
-    // the elements are shared out over `parts` warps; with fewer than four, the others take other column blocks
-    const int parts = (c.dim + 31) >> 5, turns = 4 / parts, part = warp % parts, turn = warp / parts;
-    const int e0 = part * 32 + g * 4;  // this lane's elements: e0 .. e0 + 3
-    const bool mine = e0 < c.dim;
-
-    auto fetch = [&](const Cursor &u, int stage) {
-        unsigned char *dst = ring + stage * stage_size;
-        const int unit = threadIdx.x & 15, r8 = threadIdx.x >> 4;
-        const int left = u.length - u.t * kTile;
-        if (unit * 8 < c.dim) {
-            const uint32_t p8 = (uint32_t)u.t * 8;
-            uint32_t at = div_page(c, p8), inside = p8 - at * c.page8;
-            unsigned char *to = dst + r8 * kRowBytes;
-            const char *rows = nullptr;
-            const uint32_t mine = r8 * c.row_bytes + unit * 16;
-            if (left >= kTile && inside + 8 <= c.page8) {  // whole, in one page
-                rows = page_rows(c, c.v, u.table, at, inside, u.h) + mine;
-#pragma unroll
-                for (int j = 0; j < 8; j++) copy16(to + 8 * j * kRowBytes + (unit ^ (2 * (j & 3))) * 16, rows + j * 8 * c.row_bytes);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if (8 * j < left && (j == 0 || inside == c.page8)) {  // the next page
-                        if (j) {
-                            at++;
-                            inside = 0;
-                        }
-                        rows = page_rows(c, c.v, u.table, at, inside, u.h) + mine;
-                    }
-                    const bool there = 8 * j + r8 < left;
-                    copy16(to + 8 * j * kRowBytes + (unit ^ (2 * (j & 3))) * 16, there ? (const void *)rows : (const void *)c.v, there);
-                    rows += 8 * c.row_bytes;
-                    inside++;
-                }
-            }
-        }
-        unsigned char *score = dst + kValueBytes, *top = score + most * (8 * kTile * 2);
-        for (int i = threadIdx.x; i < u.blocks * 64; i += kThreads) {  // (columns' rows of 8 units, turned by 2 (column mod 4))
-            const int col = i >> 3 & 7, w = i & 7;
-            copy16(score + (i - w + (w ^ (2 * (col & 3)))) * 16, c.score + ((size_t)u.slot(i >> 6) * 64 + (i & 63)) * 8);
-        }
-        if (threadIdx.x < u.blocks) copy16(top + threadIdx.x * 16, c.top + (size_t)u.slot(threadIdx.x) * 8);
-    };
-    Cursor cur, ahead;
+    uint32_t worst = 0;
+    const Share share(c.dim, warp);
+    Cursor cur;
     cur.start(c, meta, first);
-    ahead = cur;
-    int fetched = first;
-    for (int i = 0; i < stages - 1; i++) {
-        if (fetched < end) {
-            if (fetched > first) ahead.next(c, meta);
-            fetch(ahead, i);
-            fetched++;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-    int stage = 0;
     bool moved = true;
-    for (int item = first; item < end; item++) {
-        const int blocks = cur.blocks;
-        if (moved) {
-            // the maxima of the tiles before, by every warp for itself
-            for (int nb = 0; nb < blocks; nb++) {
-                const uint4 *tops = reinterpret_cast<const uint4 *>(c.top) + cur.slot(nb) - cur.t;
-                uint4 m = make_uint4(0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u);
-                for (int i = lane; i < cur.t; i += 32) {
+    for (int item = first; item < end;) {
+        const Strip z = cur.strip();
+        const int n = min(min(chunk, cur.tiles - cur.t), end - item);  // tiles of this chunk
+        const int pairs = z.blocks * 4;
+        int fetched = share.first;
+        auto fetch = [&](int slot) {
+            if (fetched < n) {
+                fetch_values(c, z, cur.t + fetched, share.part, ring + slot * kSlice, worst);
+                fetched += share.step;
+            }
+            commit();
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) fetch(i);
+        __syncthreads();  // the last chunk is done with
+        if (moved) {      // the maxima of the tiles before
+            for (int nb = 0; nb < z.blocks; nb++) {
+                const uint4 *tops = c.top + (size_t)(cur.slot(nb) - cur.t) * 4;
+                uint4 m = make_uint4(0, 0, 0, 0);
+                for (int i = threadIdx.x; i < cur.t * 4; i += kThreads) {
                     const uint4 w = tops[i];
-                    m = make_uint4(max16x2(m.x, w.x), max16x2(m.y, w.y), max16x2(m.z, w.z), max16x2(m.w, w.w));
+                    m = make_uint4(__vmaxu2(m.x, w.x), __vmaxu2(m.y, w.y), __vmaxu2(m.z, w.z), __vmaxu2(m.w, w.w));
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) {
-                    m.x = max16x2(m.x, __shfl_xor_sync(0xffffffffu, m.x, o));
-                    m.y = max16x2(m.y, __shfl_xor_sync(0xffffffffu, m.y, o));
-                    m.z = max16x2(m.z, __shfl_xor_sync(0xffffffffu, m.z, o));
-                    m.w = max16x2(m.w, __shfl_xor_sync(0xffffffffu, m.w, o));
+                    m.x = __vmaxu2(m.x, __shfl_xor_sync(0xffffffffu, m.x, o));
+                    m.y = __vmaxu2(m.y, __shfl_xor_sync(0xffffffffu, m.y, o));
+                    m.z = __vmaxu2(m.z, __shfl_xor_sync(0xffffffffu, m.z, o));
+                    m.w = __vmaxu2(m.w, __shfl_xor_sync(0xffffffffu, m.w, o));
                 }
-                const uint32_t w = g < 4 ? (g < 2 ? m.x : m.y) : (g < 6 ? m.z : m.w);
-                if (t4 == 0) before[nb * 8 + g] = g & 1 ? llmx::hi16(w) : llmx::lo16(w);
+                if (lane == 0) *reinterpret_cast<uint4 *>(parts_top + (warp * most + nb) * 4) = m;
             }
-            __syncthreads();  // (the last key head's columns are done with)
-            for (int col = threadIdx.x; col < blocks * 8; col += kThreads)
-                seen[col] = col < cur.rows * c.group ? cur.length - cur.rows + 1 + col / c.group : 0;
+            for (int col = threadIdx.x; col < z.blocks * 8; col += kThreads)
+                seen[col] = col < z.rows * c.group ? z.length - z.rows + 1 + col / c.group : 0;
+            __syncthreads();
         }
-        asm volatile("cp.async.wait_group %0;" ::"n"(stages - 2) : "memory");
-        __syncthreads();
-        unsigned char *here = ring + stage * stage_size;
-        if (fetched < end) {  // into the stage of the item before, which is free
-            ahead.next(c, meta);
-            fetch(ahead, stage == 0 ? stages - 1 : stage - 1);
-            fetched++;
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        // probabilities: 16 positions a warp, lane: column g, 4 positions
-        for (int nb = 0; nb < blocks; nb++) {
-            const int col = nb * 8 + g, was = before[col];
-            const int16_t *top = reinterpret_cast<const int16_t *>(here + kValueBytes + most * (8 * kTile * 2)) + col;
-            const int m = max(was, (int)*top);
-            const uint2 w = *reinterpret_cast<const uint2 *>(here + kValueBytes + (col * 8 + ((2 * warp + (t4 >> 1)) ^ (2 * (g & 3)))) * 16 + (t4 & 1) * 8);
-            const int left = seen[col] - (cur.t * kTile + warp * 16 + 4 * t4);
-            const int s[4] = {llmx::lo16(w.x), llmx::hi16(w.x), llmx::lo16(w.y), llmx::hi16(w.y)};
-            int p[4], sum = 0;
+        for (int i = threadIdx.x; i < pairs; i += kThreads) {
+            uint32_t m = runs[chunk * most * 4 + i];  // up to the last chunk's end
+            if (moved) {
+                m = 0;
+                for (int w = 0; w < kWarps; w++) m = __vmaxu2(m, parts_top[w * most * 4 + i]);
+            }
+            runs[i] = m;
+            const uint32_t *tops = reinterpret_cast<const uint32_t *>(c.top + (size_t)cur.slot(i >> 2) * 4) + (i & 3);
+            uint32_t w[kChunk][4];
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                // (what lies behind the last position that is seen may hold anything)
-                p[i] = i < left ? exps[min(max(s[i] - m, -2048), 0)] : 0;
-                sum += p[i];
-            }
-            const uint32_t w0 = (uint32_t)p[0] | (uint32_t)p[1] << 16, w1 = (uint32_t)p[2] | (uint32_t)p[3] << 16;
-            uint32_t *dst = reinterpret_cast<uint32_t *>(prob + nb * 64 + (warp >> 1) * 32 + g * 4 + 2 * (warp & 1) + (t4 >> 1)) + (t4 & 1);
-            dst[0] = low4(w0, w1);
-            dst[2] = high4(w0, w1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (t4 == 0) {
-                psum[warp * most * 8 + col] = sum;
-                before[col] = m;
-                if (warp == 0) factor[col] = exps[max(was - m, -2048)];
-            }
+            for (int k = 0; k < kChunk; k++)
+                if (k < n)
+                    for (int b = 0; b < 4; b++) w[k][b] = tops[(k * 4 + b) * 4];
+#pragma unroll
+            for (int k = 0; k < kChunk; k++)
+                if (k < n) {
+                    m = __vmaxu2(m, __vmaxu2(__vmaxu2(w[k][0], w[k][1]), __vmaxu2(w[k][2], w[k][3])));
+                    runs[(k + 1) * most * 4 + i] = m;
+                }
+            runs[chunk * most * 4 + i] = m;  // (where n is less, nobody else reads it)
         }
         __syncthreads();
-        for (int col = threadIdx.x; col < blocks * 8; col += kThreads) {
-            const int *ps = psum + col;
-            c.fsum[(size_t)cur.slot(col >> 3) * 8 + (col & 7)] = make_int2(factor[col], ps[0] + ps[most * 8] + ps[2 * most * 8] + ps[3 * most * 8]);
+        // probabilities: a warp has block `warp` of 16 positions of every tile
+        const int cp = lane & 3, pos = warp * 16 + 8 * (lane >> 4) + 2 * (lane >> 2 & 3);
+        const int before = z.length - z.rows + 1;
+        for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+            const uint32_t *score = c.score + (size_t)cur.slot(nb) * 256 + pos * 4 + cp;
+            const int seen0 = seen[nb * 8 + 2 * cp], seen1 = seen[nb * 8 + 2 * cp + 1];
+            const bool full = nb * 8 + 8 <= z.rows * c.group;
+            uint32_t w[kChunk][2];
+#pragma unroll
+            for (int k = 0; k < kChunk; k++)
+                if (k < n) {
+                    w[k][0] = score[k * 256];
+                    w[k][1] = score[k * 256 + 4];
+                }
+#pragma unroll
+            for (int k = 0; k < kChunk; k++)
+                if (k < n) {
+                    const int p = (cur.t + k) * kTile;
+                    probabilities(exps, w[k][0], w[k][1], runs[(k + 1) * most * 4 + nb * 4 + cp], full && p + kTile <= before, p + pos, seen0, seen1, warp,
+                                  prob + (k * most + nb) * 64);
+                }
         }
-        if (turn < turns && turn < blocks) {
-            // byte planes of the values: [step][element pair][row or row + 8, positions 0-3 or 4-7]
-            uint32_t vh[2][2][4], vl[2][2][4];
-            unsigned char *v = here + 8 * t4 * kRowBytes + ((part * 4 + (g >> 1)) ^ (2 * t4)) * 16 + (g & 1) * 8;
-            bool limit = false;
+        __syncthreads();
 #pragma unroll 1
-            for (;;) {
-                uint32_t out = 0;
+        for (int k = share.first, i = 0; k < n; k += share.step, i ^= 1) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+            __syncwarp();
+            uint32_t vl[2][2][4], vh[2][2][4];
+            const bool limit = value_planes(ring + i * kSlice, vl, vh);
+            __syncwarp();
+            fetch(i);
+            for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+                uint32_t y[4];
+                int sum[2];
+                weigh(vl, vh, limit, prob + (k * most + nb) * 64, y, share.part == 0, sum);
+                const size_t slot = (size_t)cur.slot(nb) + k;
+                uint32_t *dst = reinterpret_cast<uint32_t *>(c.tv + (slot * 8 + g) * c.dim + share.part * 32 + 2 * t4);
 #pragma unroll
-                for (int s = 0; s < 2; s++)
-#pragma unroll
-                    for (int half = 0; half < 2; half++) {
-                        uint2 w[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const uint2 *>(v + (32 * s + 4 * half + i) * kRowBytes);
-#pragma unroll
-                        for (int mb = 0; mb < 2; mb++) {
-                            const uint32_t w0 = mb ? w[0].y : w[0].x, w1 = mb ? w[1].y : w[1].x, w2 = mb ? w[2].y : w[2].x, w3 = mb ? w[3].y : w[3].x;
-                            const uint32_t a = __byte_perm(w0, w1, 0x5140), b = __byte_perm(w2, w3, 0x5140);
-                            const uint32_t d = __byte_perm(w0, w1, 0x7362), e = __byte_perm(w2, w3, 0x7362);
-                            vl[s][mb][2 * half] = __byte_perm(a, b, 0x5410);
-                            vh[s][mb][2 * half] = __byte_perm(a, b, 0x7632);
-                            vl[s][mb][2 * half + 1] = __byte_perm(d, e, 0x5410);
-                            vh[s][mb][2 * half + 1] = __byte_perm(d, e, 0x7632);
-                            out |= (vh[s][mb][2 * half] ^ (vh[s][mb][2 * half] << 1)) | (vh[s][mb][2 * half + 1] ^ (vh[s][mb][2 * half + 1] << 1));
-                        }
-                    }
-                // some high byte is not in [-8, 7] (its bits 3 to 7 differ): limited where they lie, and once more
-                if (limit || !__any_sync(0xffffffffu, mine && (out & 0xf0f0f0f0u) != 0)) break;
-                limit = true;
-#pragma unroll 1
-                for (int i = 0; i < 16; i++) {
-                    uint2 *w = reinterpret_cast<uint2 *>(v + ((i & 8) * 4 + (i & 7)) * kRowBytes);
-                    *w = make_uint2(limit2(w->x), limit2(w->y));
-                }
-            }
-            for (int nb = turn; nb < blocks; nb += turns) {
-                const uint4 b0 = prob[nb * 64 + lane], b1 = prob[nb * 64 + 32 + lane];
-                uint32_t tv[2][2];  // [column 2 t4 + j][elements e0, e0 + 1 and e0 + 2, e0 + 3]
-#pragma unroll
-                for (int mb = 0; mb < 2; mb++) {
-                    int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {0, 0, 0, 0};
-#pragma unroll
-                    for (int s = 0; s < 2; s++) {
-                        const uint4 b = s ? b1 : b0;
-                        const uint32_t(&h)[4] = vh[s][mb], (&l)[4] = vl[s][mb];
-                        mma_su(hh, h[0], h[1], h[2], h[3], b.z, b.w);
-                        mma_su(mid, h[0], h[1], h[2], h[3], b.x, b.y);
-                        mma_uu(ll, l[0], l[1], l[2], l[3], b.x, b.y);
-                        mma_uu(mid, l[0], l[1], l[2], l[3], b.z, b.w);
-                        if (limit) {
-                            const uint32_t r0 = rest2(__byte_perm(b.x, b.z, 0x5140)), r1 = rest2(__byte_perm(b.x, b.z, 0x7362));
-                            const uint32_t r2 = rest2(__byte_perm(b.y, b.w, 0x5140)), r3 = rest2(__byte_perm(b.y, b.w, 0x7362));
-                            uint32_t m[4];
-#pragma unroll
-                            for (int i = 0; i < 4; i++) m[i] = at_limit(h[i]);
-                            mma_us(mid, m[0], m[1], m[2], m[3], high4(r0, r1), high4(r2, r3));
-                            mma_uu(ll, m[0], m[1], m[2], m[3], low4(r0, r1), low4(r2, r3));
-                        }
-                    }
-                    int y[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int ts = (int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]);
-                        y[i] = ((ts >> 5) + 257) >> 9;  // rnd8 of rnd6: (ts + 2^5 + 2^13) / 2^14, within 32 bits
-                    }
-                    tv[0][mb] = pack_sat16(y[0], y[2]);
-                    tv[1][mb] = pack_sat16(y[1], y[3]);
-                }
-                if (mine) {
-                    int16_t *dst = c.tv + ((size_t)cur.slot(nb) * 8 + 2 * t4) * c.dim + e0;
-                    *reinterpret_cast<uint2 *>(dst) = make_uint2(tv[0][0], tv[0][1]);
-                    *reinterpret_cast<uint2 *>(dst + c.dim) = make_uint2(tv[1][0], tv[1][1]);
+                for (int o = 0; o < 4; o++)
+                    if (share.part * 32 + 8 * o < c.dim) dst[4 * o] = y[o];
+                if (share.part == 0 && lane < 4) {
+                    const uint32_t was = runs[k * most * 4 + nb * 4 + lane], m = runs[(k + 1) * most * 4 + nb * 4 + lane];
+                    const uint32_t d = m - __vmaxu2(was, __vmaxu2(m, 0x08000800u) - 0x08000800u);
+                    *reinterpret_cast<int4 *>(c.fsum + slot * 8 + 2 * lane) = make_int4(exps[d & 0xffffu], sum[0], exps[d >> 16], sum[1]);
                 }
             }
         }
-        stage = stage + 1 == stages ? 0 : stage + 1;
-        moved = item + 1 < end && cur.next(c, meta);
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        item += n;
+        moved = false;
+        if (item < end) {
+            cur.t += n - 1;
+            moved = cur.next(c, meta);
+        }
     }
+    report(c, worst);
 }
 
 // ---- join ---------------------------------------------------------------------------
@@ -737,34 +833,6 @@ static __device__ __forceinline__ uint32_t request_of(const uint32_t *offsets, u
     before = __ballot_sync(0xffffffffu, lane < step && at < requests && offsets[at] <= r);
     return before ? block + 31 - __clz(before) : block;
 }
-
-// What a stretch of tiles makes of a value x that comes in: x + s, limited to [lo, hi] (sums that
-// saturate at every step combine to that).  Without kLong no sum can reach the limits.
-template <bool kLong>
-struct Stretch;
-template <>
-struct Stretch<false> {
-    int s;
-    __device__ void start() { s = 0; }
-    __device__ void add(int v) { s += v; }
-    __device__ int of(int x) const { return x + s; }
-};
-template <>
-struct Stretch<true> {
-    long long s;
-    int lo, hi;
-    __device__ void start() {
-        s = 0;
-        lo = INT_MIN;
-        hi = INT_MAX;
-    }
-    __device__ void add(int v) {
-        s += v;
-        lo = llmx::add_sat(lo, v);
-        hi = llmx::add_sat(hi, v);
-    }
-    __device__ int of(int x) const { return (int)min(max(x + s, (long long)lo), (long long)hi); }
-};
 
 constexpr int kShortTiles = 255;  // tiles whose sums stay below 2^31: of values 2^23 each, of probabilities 2^22
 constexpr int kMaxStretches = 3;  // per warp
@@ -784,23 +852,52 @@ static __device__ __forceinline__ int add_high(uint32_t w, int x) {
     asm("dp2a.lo.s32.s32 %0, %1, %2, %3;" : "=r"(r) : "r"(w), "r"(0x0100), "r"(x));
     return r;
 }
+// Four elements of a row over its sum, as two words
+static __device__ __forceinline__ uint2 quotient(const int (&x)[4], int sum) {
+    const long long inv = sat16(rnd((long long)llmx::recip_q16(sum < 16 ? 16 : sum), 8));
+    auto one = [&](int y) { return (int)(((long long)y * inv + 32768) >> 16); };
+    return make_uint2(pack_sat16(one(x[0]), one(x[1])), pack_sat16(one(x[2]), one(x[3])));
+}
+
+// What tiles without a factor do to a row's four elements: their sums, and (of a long text) the least and
+// the largest value, from which it is seen that nothing on the way saturates.
+struct Stretch {
+    int s[4];
+    uint32_t lo, hi;  // of pairs of elements
+    int start, tiles, psum;
+    __device__ void clear(int t) {
+        s[0] = s[1] = s[2] = s[3] = 0;
+        lo = hi = 0;
+        start = t;
+        tiles = psum = 0;
+    }
+    template <bool kLong>
+    __device__ void add(uint2 v, int p) {
+        s[0] = add_low(v.x, s[0]);
+        s[1] = add_high(v.x, s[1]);
+        s[2] = add_low(v.y, s[2]);
+        s[3] = add_high(v.y, s[3]);
+        psum += p;
+        tiles++;
+        if constexpr (kLong) {
+            lo = __vmins2(lo, __vmins2(v.x, v.y));
+            hi = __vmaxs2(hi, __vmaxs2(v.x, v.y));
+        }
+    }
+};
 
 // One query head's row per CTA.  A lane has four elements, a warp an equal part of the tiles.  Between
 // tiles that raise the maximum (whose factor is not 1: few in a long text) the recurrence only adds,
-// so a warp gives what its tiles do to any value that comes in as a few stretches (a factor, then a
-// sum), and the first warp, which starts from 0, puts them together; tiles beyond a warp's
-// kMaxStretches it goes through itself.
+// so a warp gives what its tiles do to any value that comes in as a few stretches (a factor, then
+// sums), and the first warp, which starts from 0, puts them together; tiles beyond a warp's
+// kMaxStretches, and a stretch on which something might saturate, it goes through itself, one by one.
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    struct Four {
-        Stretch<kLong> e[4];
-    };
-    __shared__ Stretch<kLong> norms[kMaxJoinWarps][kMaxStretches];
     __shared__ int factors[kMaxJoinWarps][kMaxStretches], counts[kMaxJoinWarps], rest[kMaxJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     const int quads = c.dim >> 2;
-    Four *stretches = reinterpret_cast<Four *>(dynamic);  // [warps - 1][kMaxStretches][quads]
+    Stretch *stretches = reinterpret_cast<Stretch *>(dynamic);  // [warps - 1][kMaxStretches][32]
     pdl_wait();
     pdl_trigger();
     const uint32_t row = blockIdx.x / c.heads;
@@ -814,61 +911,36 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     const size_t at = ((size_t)m.slot + (size_t)(h * blocks + (col >> 3)) * m.tiles) * 8 + (col & 7);
     const uint2 *tv = reinterpret_cast<const uint2 *>(c.tv + at * c.dim) + min(lane, quads - 1);
     const int2 *fsum = c.fsum + at;
-    const int step = 8 * quads;  // from a tile to the next
-    const int first = (int)((long long)m.tiles * warp / warps), end = (int)((long long)m.tiles * (warp + 1) / warps);
+    const uint32_t step = 8 * quads;  // from a tile to the next
+    auto begin_of = [&](int w) { return (int)((long long)m.tiles * w / warps); };
 
     int sum = 0, x[4] = {0, 0, 0, 0};
     uint2 v[kAhead];
     int2 f[kAhead];
     auto load = [&](int t0, int t1) {  // what lies behind t1 changes nothing
+        if (t0 + kAhead <= t1) {
+#pragma unroll
+            for (int i = 0; i < kAhead; i++) {
+                v[i] = tv[(size_t)(t0 + i) * step];
+                f[i] = fsum[(t0 + i) * 8];
+            }
+            return;
+        }
 #pragma unroll
         for (int i = 0; i < kAhead; i++) {
             v[i] = make_uint2(0, 0);
             f[i] = make_int2(16384, 0);
             if (t0 + i < t1) {
                 v[i] = tv[(size_t)(t0 + i) * step];
-                f[i] = fsum[(size_t)(t0 + i) * 8];
+                f[i] = fsum[(t0 + i) * 8];
             }
         }
     };
-    // (one of a warp's lanes' factors stands for all of them)
-    auto plain = [&]() {
+    auto plain = [&]() {  // no factor among them (factors are at most 16384: one below has no bit 14)
         int all = 16384;
 #pragma unroll
-        for (int i = 0; i < kAhead; i++) all &= f[i].x;  // at most 16384: a factor below it has no bit 14
-        return __any_sync(0xffffffffu, all == 16384) != 0;
-    };
-    auto add_all = [&](Stretch<kLong> &n, Four &p) {
-        if constexpr (kLong) {
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                n.add(4 * f[i].y);
-                p.e[0].add(add_low(v[i].x, 0) * 256);
-                p.e[1].add(add_high(v[i].x, 0) * 256);
-                p.e[2].add(add_low(v[i].y, 0) * 256);
-                p.e[3].add(add_high(v[i].y, 0) * 256);
-            }
-        } else {
-            int s = 0, y[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                s += f[i].y;
-                y[0] = add_low(v[i].x, y[0]);
-                y[1] = add_high(v[i].x, y[1]);
-                y[2] = add_low(v[i].y, y[2]);
-                y[3] = add_high(v[i].y, y[3]);
-            }
-            n.add(4 * s);
-#pragma unroll
-            for (int k = 0; k < 4; k++) p.e[k].add(256 * y[k]);
-        }
-    };
-    auto add_one = [&](Stretch<kLong> &n, Four &p, uint2 w, int s) {
-        n.add(4 * s);
-        p.e[0].add(llmx::lo16(w.x) * 256);
-        p.e[1].add(llmx::hi16(w.x) * 256);
-        p.e[2].add(llmx::lo16(w.y) * 256);
-        p.e[3].add(llmx::hi16(w.y) * 256);
+        for (int i = 0; i < kAhead; i++) all &= f[i].x;
+        return __shfl_sync(0xffffffffu, all, 0) == 16384;
     };
     auto factor = [&](int by) {  // a factor of 1 leaves everything as it is
         if (by == 16384) return;
@@ -876,62 +948,89 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = times(x[k], by);
     };
-    auto apply = [&](const Stretch<kLong> &n, const Four &p) {
-        sum = n.of(sum);
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = p.e[k].of(x[k]);
+    auto one = [&](uint2 w, int p) {  // a tile on top of (sum, x)
+        if constexpr (kLong) {
+            sum = llmx::add_sat(sum, 4 * p);
+            x[0] = llmx::add_sat(x[0], llmx::lo16(w.x) * 256);
+            x[1] = llmx::add_sat(x[1], llmx::hi16(w.x) * 256);
+            x[2] = llmx::add_sat(x[2], llmx::lo16(w.y) * 256);
+            x[3] = llmx::add_sat(x[3], llmx::hi16(w.y) * 256);
+        } else {
+            sum += 4 * p;
+            x[0] += llmx::lo16(w.x) * 256;
+            x[1] += llmx::hi16(w.x) * 256;
+            x[2] += llmx::lo16(w.y) * 256;
+            x[3] += llmx::hi16(w.y) * 256;
+        }
     };
-    auto clear = [&](Stretch<kLong> &n, Four &p) {
-        n.start();
-#pragma unroll
-        for (int k = 0; k < 4; k++) p.e[k].start();
-    };
-    // tiles t0 .. t1 - 1 on top of (sum, x)
-    auto replay = [&](int t0, int t1) {
+    auto replay = [&](int t0, int t1) {  // tiles t0 .. t1 - 1 on top of (sum, x), one by one
+#pragma unroll 1
         for (; t0 < t1; t0 += kAhead) {
             load(t0, t1);
-            Stretch<kLong> n;
-            Four p;
-            clear(n, p);
-            if (plain()) {
-                add_all(n, p);
-                apply(n, p);
-                continue;
-            }
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
                 factor(f[i].x);
-                clear(n, p);
-                add_one(n, p, v[i], f[i].y);
-                apply(n, p);
+                one(v[i], f[i].y);
             }
         }
     };
-    if (warp == 0) {
-        replay(first, end);
-    } else {
-        Stretch<kLong> n;
-        Four p;
-        clear(n, p);
-        int f0 = 16384, count = 0, left = end;
-        Four *mine = stretches + (size_t)(warp - 1) * kMaxStretches * quads + lane;
-        auto close = [&]() {
-            if (lane < quads) mine[count * quads] = p;
-            if (lane == 0) {
-                norms[warp][count] = n;
-                factors[warp][count] = f0;
+    auto apply = [&](const Stretch &p) {
+        if constexpr (kLong) {
+            // the furthest that any of its sums can be from what comes in
+            const long long up = 256ll * p.tiles * max(llmx::lo16(p.hi), llmx::hi16(p.hi)), down = 256ll * p.tiles * min(llmx::lo16(p.lo), llmx::hi16(p.lo));
+            const bool far = max(max(x[0], x[1]), max(x[2], x[3])) + up > INT_MAX || min(min(x[0], x[1]), min(x[2], x[3])) + down < INT_MIN ||
+                             sum + 4ll * p.psum > INT_MAX;
+            if (__any_sync(0xffffffffu, far)) {
+                replay(p.start, p.start + p.tiles);  // (their factors, but for the first one, which is used, are 1)
+                return;
             }
+        }
+        sum += 4 * p.psum;
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = (int)((uint32_t)x[k] + 256u * (uint32_t)p.s[k]);
+    };
+    if (warp == 0) {
+        const int end = begin_of(1);
+#pragma unroll 1
+        for (int t0 = 0; t0 < end; t0 += kAhead) {
+            load(t0, end);
+            if (plain()) {
+                Stretch p;
+                p.clear(t0);
+#pragma unroll
+                for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i], f[i].y);
+                p.tiles = min(kAhead, end - t0);
+                apply(p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kAhead; i++) {
+                    factor(f[i].x);
+                    one(v[i], f[i].y);
+                }
+            }
+        }
+    } else {
+        const int first = begin_of(warp), end = begin_of(warp + 1);
+        Stretch p;
+        p.clear(first);
+        int f0 = 16384, count = 0, left = end;
+        Stretch *mine = stretches + (warp - 1) * kMaxStretches * 32 + lane;
+        auto close = [&]() {
+            mine[count * 32] = p;
+            if (lane == 0) factors[warp][count] = f0;
             count++;
         };
+#pragma unroll 1
         for (int t0 = first; t0 < end && left == end; t0 += kAhead) {
             load(t0, end);
             if (plain()) {
-                add_all(n, p);
+#pragma unroll
+                for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i], f[i].y);
                 continue;
             }
 #pragma unroll
             for (int i = 0; i < kAhead; i++) {
-                if (left != end) continue;
+                if (left != end || t0 + i >= end) continue;
                 if (f[i].x != 16384) {
                     if (t0 + i > first) {  // the stretch ends here
                         if (count + 1 == kMaxStretches) {
@@ -939,13 +1038,15 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
                             continue;
                         }
                         close();
-                        clear(n, p);
+                        p.clear(t0 + i);
                     }
                     f0 = f[i].x;
                 }
-                add_one(n, p, v[i], f[i].y);
+                p.add<kLong>(v[i], f[i].y);
             }
         }
+        // (of the last stretch, places behind the end may have been counted)
+        p.tiles = min(p.tiles, left - p.start);
         if (first < end) close();
         if (lane == 0) {
             counts[warp] = count;
@@ -955,19 +1056,267 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     if (warps > 1) {
         __syncthreads();
         if (warp != 0) return;
+#pragma unroll 1
         for (int w = 1; w < warps; w++) {
+#pragma unroll 1
             for (int k = 0; k < counts[w]; k++) {
                 factor(factors[w][k]);
-                apply(norms[w][k], stretches[((size_t)(w - 1) * kMaxStretches + k) * quads + min(lane, quads - 1)]);
+                apply(stretches[((w - 1) * kMaxStretches + k) * 32 + lane]);
             }
-            replay(rest[w], (int)((long long)m.tiles * (w + 1) / warps));
+            replay(rest[w], begin_of(w + 1));
         }
     }
-    if (lane >= quads) return;
-    const long long inv = sat16(rnd((long long)llmx::recip_q16(sum < 16 ? 16 : sum), 8));
-    auto last = [&](int y) { return (int)(((long long)y * inv + 32768) >> 16); };
-    *reinterpret_cast<uint2 *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 4 * lane) =
-        make_uint2(pack_sat16(last(x[0]), last(x[1])), pack_sat16(last(x[2]), last(x[3])));
+    if (lane < quads) *reinterpret_cast<uint2 *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 4 * lane) = quotient(x, sum);
+}
+
+// ---- all at once --------------------------------------------------------------------
+// A cluster of CTAs per (request, key head), each with an equal part of its tiles, goes through the
+// three steps with everything in shared memory: scores, the maxima of the CTAs before from these,
+// probabilities (in place of the scores), values, which go to the CTA that has their column, and the
+// recurrence there.
+struct Places {  // in dynamic shared memory, in bytes
+    int prob, exps, runs, tops, base, maxima, tv, fsum, column, queries, size;
+    __host__ __device__ Places(int tiles, int cluster, int most, int dim) {
+        int at = kRing;
+        auto place = [&](int n) {
+            const int was = at;
+            at += (n + 15) / 16 * 16;
+            return was;
+        };
+        const int own = (most * 8 + cluster - 1) / cluster;  // columns of a CTA
+        prob = place(tiles * most * 1024);
+        exps = place(kExpWords * 4);
+        runs = place((tiles + 1) * most * 16);
+        tops = place(tiles * most * 64);
+        base = place(most * 16);
+        maxima = place(cluster * most * 16);
+        tv = place(own * tiles * cluster * dim * 2);
+        fsum = place(own * tiles * cluster * 8);
+        column = place((int)sizeof(Column));
+        queries = place(2 * most * ((dim + 31) / 32) * 512);
+        size = at;
+    }
+};
+constexpr int kAttendBlocks = 8;  // column blocks that k_attend takes: their queries fit the ring
+
+static __device__ __forceinline__ void put(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+static __device__ __forceinline__ void cluster_meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int KS, bool kOne>
+__global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;
+    const int log = c.cluster_log, cluster = 1 << log;
+    const Places at(c.tiles, cluster, most, c.dim);
+    unsigned char *ring = dynamic + warp * kDepth * kSlice;
+    uint4 *queries = reinterpret_cast<uint4 *>(dynamic + at.queries), *rests = queries + most * KS * 32;
+    uint32_t *score = reinterpret_cast<uint32_t *>(dynamic + at.prob);  // [tiles][most][64 positions][4 pairs], then the probabilities
+    const int16_t *exps = reinterpret_cast<const int16_t *>(dynamic + at.exps);
+    uint32_t *runs = reinterpret_cast<uint32_t *>(dynamic + at.runs);      // [tiles + 1][most * 4] maxima up to a tile of this CTA's
+    uint32_t *tops = reinterpret_cast<uint32_t *>(dynamic + at.tops);      // [tiles][most][4 blocks][4 pairs]
+    uint32_t *base = reinterpret_cast<uint32_t *>(dynamic + at.base);      // [most * 4] maxima of the CTAs before
+    uint32_t *maxima = reinterpret_cast<uint32_t *>(dynamic + at.maxima);  // [cluster][most * 4]
+    Column &column = *reinterpret_cast<Column *>(dynamic + at.column);
+    for (int i = threadIdx.x; i < kExpWords; i += kThreads)
+        reinterpret_cast<uint32_t *>(dynamic + at.exps)[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
+    pdl_wait();
+    pdl_trigger();
+    __shared__ int all_tiles[kWarps];
+    const int strip = (int)(blockIdx.x >> log), rank = (int)(blockIdx.x & (unsigned)(cluster - 1));
+    const int b = strip / c.kv, h = strip - b * c.kv;
+    const uint32_t o0 = c.offsets[b], o1 = c.offsets[b + 1], len = c.lengths[b];
+    if (o0 > o1 || o1 > c.rows || o1 - o0 > (uint32_t)c.max_block || len > c.longest) {
+        if (threadIdx.x == 0) atomicOr(c.error, kErrRequest);
+        return;  // (the whole cluster)
+    }
+    if (o0 == o1) return;
+    llmx::cluster_arrive();
+    const Strip z{c.table + (size_t)b * c.ld_table, h, (int)(o1 - o0), (int)len, ((int)(o1 - o0) * c.group + 7) >> 3, o0};
+    const int n = (z.length + kTile - 1) / kTile, t0 = n * rank >> log, own = (n * (rank + 1) >> log) - t0;
+    const int columns = z.rows * c.group, pairs = z.blocks * 4;
+    uint32_t worst = 0;
+
+    // ---- scores
+    const Share share(c.dim, warp);
+    int fetched = share.first;
+    auto fetch = [&](int slot) {
+        if (fetched < own) {
+            fetch_values(c, z, t0 + fetched, share.part, ring + slot * kSlice, worst);
+            fetched += share.step;
+        }
+        commit();
+    };
+    {
+        uint4 raw[2][KS];
+        KeyPages pages;
+        int p0 = t0 * kTile + warp * 16;
+        if (own > 0) {
+            pages.load(c, z, p0, worst);
+            load_keys<KS>(c, z, pages, p0, raw);
+        }
+        if (own > 1) pages.load(c, z, p0 + kTile, worst);
+        stage_queries<KS>(c, z, warp, kWarps, queries, rests, column);
+#pragma unroll
+        for (int i = 0; i < kDepth; i++) fetch(i);
+        // whether the whole call is within what the handle was made for
+        int sum = 0;
+        for (uint32_t i = threadIdx.x; i < c.requests; i += kThreads) {
+            int rows, tiles;
+            if (request(c, i, rows, tiles)) sum += tiles;
+        }
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        if (lane == 0) all_tiles[warp] = sum;
+        __syncthreads();
+#pragma unroll 1
+        for (int k = 0; k < own; k++, p0 += kTile) {
+            uint32_t kh[KS][4], kl[KS][4];
+            const bool some = key_planes<KS>(raw, kl, kh);
+            if (k + 1 < own) {
+                load_keys<KS>(c, z, pages, p0 + kTile, raw);
+                if (k + 2 < own) pages.load(c, z, p0 + 2 * kTile, worst);
+            }
+            for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+                const int block = (k * most + nb) * 4 + warp;
+                uint32_t top = 0;
+                if (p0 < z.length) {
+                    uint32_t w[2];
+                    top = score_block<KS>(c, z, kl, kh, some, nb, p0, queries, rests, column, w);
+                    score[block * 64 + lane] = w[0];
+                    score[block * 64 + 32 + lane] = w[1];
+                }
+                if (lane < 4) tops[block * 4 + lane] = top;
+            }
+        }
+    }
+    __syncthreads();
+    llmx::cluster_wait();  // every CTA of the cluster is there
+    // ---- maxima
+    for (int i = threadIdx.x; i < pairs; i += kThreads) {
+        uint32_t m = 0;
+        const uint32_t *top = tops + (i >> 2) * 16 + (i & 3);
+        for (int k = 0; k < own; k++, top += most * 16) {
+            runs[k * most * 4 + i] = m;
+            m = __vmaxu2(m, __vmaxu2(__vmaxu2(top[0], top[4]), __vmaxu2(top[8], top[12])));
+        }
+        runs[own * most * 4 + i] = m;
+        for (int r = rank + 1; r < cluster; r++) put(llmx::remote(maxima + rank * most * 4 + i, (uint32_t)r), m);
+    }
+    cluster_meet();
+    for (int i = threadIdx.x; i < pairs; i += kThreads) {
+        uint32_t m = 0;
+        for (int r = 0; r < rank; r++) m = __vmaxu2(m, maxima[r * most * 4 + i]);
+        base[i] = m;
+    }
+    __syncthreads();
+    // ---- probabilities: a tile against 8 columns a warp, in place
+    // Column nb * 8 + i belongs to CTA i mod cluster (at most 8), which holds `stride` tiles of each of its columns.
+    const int stride = c.tiles << log, of_block = 8 >> log;
+    auto owner = [&](int offset, int i) { return llmx::remote(dynamic + offset, (uint32_t)(i & (cluster - 1))); };
+    const int cp = lane & 3, pos = 8 * (lane >> 4) + 2 * (lane >> 2 & 3);
+    const uint32_t factor0 = owner(at.fsum, 2 * cp), factor1 = owner(at.fsum, 2 * cp + 1);
+    for (int k = 0, nb = warp; k < own;) {
+        if (!kOne && nb >= z.blocks) {
+            nb -= z.blocks;
+            k++;
+            continue;
+        }
+        if (kOne) {  // (one block: the warps take the tiles in turn)
+            k = nb;
+            if (k >= own) break;
+        }
+        const int block = kOne ? 0 : nb, col = block * 8 + 2 * cp;
+        uint32_t *here = score + (k * most + block) * 256;
+        uint32_t w[4][2];
+#pragma unroll
+        for (int blk = 0; blk < 4; blk++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) w[blk][i] = here[blk * 64 + (pos + i) * 4 + cp];
+        const uint32_t before = base[block * 4 + cp], was = __vmaxu2(before, runs[k * most * 4 + block * 4 + cp]),
+                       m = __vmaxu2(before, runs[(k + 1) * most * 4 + block * 4 + cp]);
+        const int2 seen = *reinterpret_cast<const int2 *>(&column.seen[col]);
+        const int p = (t0 + k) * kTile;
+        const bool whole = block * 8 + 8 <= columns && p + kTile <= z.length - z.rows + 1;
+        __syncwarp();
+#pragma unroll
+        for (int blk = 0; blk < 4; blk++)
+            probabilities(exps, w[blk][0], w[blk][1], m, whole, p + pos + 16 * blk, seen.x, seen.y, blk, reinterpret_cast<uint4 *>(here));
+        if (lane < 4) {
+            const uint32_t d = m - __vmaxu2(was, __vmaxu2(m, 0x08000800u) - 0x08000800u);
+            const uint32_t f0 = (uint32_t)(((block * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
+            const uint32_t f1 = (uint32_t)(((block * of_block + (2 * cp + 1 >> log)) * stride + t0 + k) * 8);
+            if (col < columns) put(factor0 + f0, (uint32_t)exps[d & 0xffffu]);
+            if (col + 1 < columns) put(factor1 + f1, (uint32_t)exps[d >> 16]);
+        }
+        nb += kWarps;
+    }
+    __syncthreads();
+    // ---- values
+    const uint32_t values = owner(at.tv, g) + (uint32_t)(share.part * 64 + 4 * t4);
+#pragma unroll 1
+    for (int k = share.first, i = 0; k < own; k += share.step, i ^= 1) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        __syncwarp();
+        uint32_t vl[2][2][4], vh[2][2][4];
+        const bool limit = value_planes(ring + i * kSlice, vl, vh);
+        __syncwarp();
+        fetch(i);
+        for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+            uint32_t y[4];
+            int sum[2];
+            weigh(vl, vh, limit, reinterpret_cast<const uint4 *>(score) + (k * most + nb) * 64, y, share.part == 0, sum);
+            if (nb * 8 + g < columns) {
+                const uint32_t to = values + (uint32_t)(((nb * of_block + (g >> log)) * stride + t0 + k) * 2 * c.dim);
+#pragma unroll
+                for (int o = 0; o < 4; o++)
+                    if (share.part * 32 + 8 * o < c.dim) put(to + 16 * o, y[o]);
+            }
+            if (share.part == 0 && lane < 4) {
+                const uint32_t f0 = (uint32_t)(((nb * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
+                const uint32_t f1 = (uint32_t)(((nb * of_block + (2 * cp + 1 >> log)) * stride + t0 + k) * 8);
+                if (nb * 8 + 2 * cp < columns) put(factor0 + f0 + 4, (uint32_t)sum[0]);
+                if (nb * 8 + 2 * cp + 1 < columns) put(factor1 + f1 + 4, (uint32_t)sum[1]);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    report(c, worst);
+    cluster_meet();  // nothing is sent to another CTA from here on
+    long long total = 0;
+    for (int w = 0; w < kWarps; w++) total += all_tiles[w];
+    if (total * c.kv > c.capacity) {
+        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.error, kErrBudget);
+        return;
+    }
+    // ---- join: a column a warp, four elements a lane (too few tiles for anything to saturate)
+    const int quads = c.dim >> 2;
+    for (int idx = warp;; idx += kWarps) {
+        const int col = kOne || log == 3 ? (idx << log) + rank : (idx >> (3 - log)) * 8 + ((idx & (of_block - 1)) << log) + rank;
+        if (col >= columns) break;
+        const uint2 *tv = reinterpret_cast<const uint2 *>(dynamic + at.tv) + (size_t)idx * stride * quads + min(lane, quads - 1);
+        const int2 *fsum = reinterpret_cast<const int2 *>(dynamic + at.fsum) + idx * stride;
+        int sum = 0, x[4] = {0, 0, 0, 0};
+#pragma unroll 4
+        for (int t = 0; t < n; t++) {
+            const uint2 w = tv[t * quads];
+            const int2 f = fsum[t];
+            if (f.x != 16384) {
+                sum = times(sum, f.x);
+#pragma unroll
+                for (int k = 0; k < 4; k++) x[k] = times(x[k], f.x);
+            }
+            sum += 4 * f.y;
+            x[0] += llmx::lo16(w.x) * 256;
+            x[1] += llmx::hi16(w.x) * 256;
+            x[2] += llmx::lo16(w.y) * 256;
+            x[3] += llmx::hi16(w.y) * 256;
+        }
+        const int j = col / c.group, head = h * c.group + col - j * c.group;
+        if (lane < quads) *reinterpret_cast<uint2 *>(c.out + (size_t)(z.row0 + j) * c.ld_out + (size_t)head * c.dim + 4 * lane) = quotient(x, sum);
+    }
 }
 
 // ---- append -------------------------------------------------------------------------
@@ -1049,13 +1398,16 @@ __global__ void __launch_bounds__(256) k_append(const AppendCall c) {
 struct llmx_paged {
     int dev = 0, sms = 0;
     int heads = 0, kv = 0, dim = 0, page_len = 0;
+    bool one = false;  // one column block
     uint32_t max_requests = 0, max_block = 0, max_length = 0;
     long long capacity = 0;  // (key head, tile) items of a call
     size_t scores_smem = 0, values_smem = 0;
     int scores_ctas = 0, values_ctas = 0;  // that are on the device at once
     unsigned char *memory = nullptr;
     Meta *meta = nullptr;
-    int16_t *score = nullptr, *top = nullptr, *tv = nullptr, *exps = nullptr;
+    uint32_t *score = nullptr;
+    uint4 *top = nullptr;
+    int16_t *tv = nullptr, *exps = nullptr;
     int2 *fsum = nullptr;
     int *error = nullptr;
     uint64_t bytes = 0;
@@ -1086,17 +1438,27 @@ struct DeviceScope {
     }
 };
 
-const void *scores_kernel(int dim) {
+// The kernels for a head dimension, and for one column block or more.
+const void *attend_kernel(int dim, bool one) {
     switch ((dim + 31) / 32) {
-        case 1: return (const void *)k_scores<1>;
-        case 2: return (const void *)k_scores<2>;
-        case 3: return (const void *)k_scores<3>;
-        default: return (const void *)k_scores<4>;
+        case 1: return one ? (const void *)k_attend<1, true> : (const void *)k_attend<1, false>;
+        case 2: return one ? (const void *)k_attend<2, true> : (const void *)k_attend<2, false>;
+        case 3: return one ? (const void *)k_attend<3, true> : (const void *)k_attend<3, false>;
+        default: return one ? (const void *)k_attend<4, true> : (const void *)k_attend<4, false>;
     }
 }
+const void *scores_kernel(int dim, bool one) {
+    switch ((dim + 31) / 32) {
+        case 1: return one ? (const void *)k_scores<1, true> : (const void *)k_scores<1, false>;
+        case 2: return one ? (const void *)k_scores<2, true> : (const void *)k_scores<2, false>;
+        case 3: return one ? (const void *)k_scores<3, true> : (const void *)k_scores<3, false>;
+        default: return one ? (const void *)k_scores<4, true> : (const void *)k_scores<4, false>;
+    }
+}
+const void *values_kernel(bool one) { return one ? (const void *)k_values<true> : (const void *)k_values<false>; }
 
 template <class T>
-cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, const T &call, cudaStream_t s) {
+cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, const T &call, cudaStream_t s, int cluster = 0) {
     T copy = call;
     void *args[] = {&copy};
     cudaLaunchConfig_t cfg = {};
@@ -1104,11 +1466,14 @@ cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, cons
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster ? 2 : 1;
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
@@ -1178,6 +1543,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     p->max_requests = max_requests;
     p->max_block = max_block;
     p->max_length = max_length;
+    p->one = blocks == 1;
     p->capacity = (long long)(tiles * kv_heads);
     size_t at = 0;
     auto place = [&](size_t n) {
@@ -1186,19 +1552,22 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
         return was;
     };
     const size_t error_at = place(4), exps_at = place(kExpWords * 4), meta_at = place(max_requests * sizeof(Meta)),
-                 score_at = place(slots * 8 * kTile * 2), top_at = place(slots * 16), tv_at = place(slots * 8 * head_dim * 2),
+                 score_at = place(slots * 8 * kTile * 2), top_at = place(slots * 64), tv_at = place(slots * 8 * head_dim * 2),
                  fsum_at = place(slots * 64);
     p->bytes = at;
     p->scores_smem = 2 * blocks * ((head_dim + 31) / 32) * 512 + (size_t)max_requests * sizeof(Meta);
-    p->values_smem = (size_t)kStages * stage_bytes((int)blocks) + blocks * 1024 + kExpWords * 4 +
-                     (6 + kWarps) * blocks * 32 + (size_t)max_requests * sizeof(Meta);
+    const size_t chunk = std::max<size_t>(1, kChunk / blocks);
+    p->values_smem = kRing + chunk * blocks * 1024 + kExpWords * 4 + (chunk + 1 + kWarps + 2) * blocks * 16 + (size_t)max_requests * sizeof(Meta);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    int16_t e16[2049], host[kExpWords * 2] = {};
-    llmx::build_exp_tables(e16, host);
+    int16_t e16[2049], p18[2049], host[kExpWords * 2] = {};
+    llmx::build_exp_tables(e16, p18);
+    for (int i = 0; i <= 2048; i++) host[i] = p18[2048 - i];
     cudaError_t e;
     if ((e = cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(scores_kernel(p->dim), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute((const void *)k_values, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(scores_kernel(p->dim, p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(values_kernel(p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(attend_kernel(p->dim, p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute((const void *)k_join<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaFuncSetAttribute((const void *)k_join<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaMalloc(reinterpret_cast<void **>(&p->memory), at)) != cudaSuccess ||
         (e = cudaMemsetAsync(p->memory + error_at, 0, 4, s)) != cudaSuccess ||
@@ -1208,8 +1577,8 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
         return cuda_fail("create", e);
     }
     int per_sm[2] = {0, 0};
-    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[0], scores_kernel(p->dim), kThreads, p->scores_smem)) != cudaSuccess ||
-        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[1], (const void *)k_values, kThreads, p->values_smem)) != cudaSuccess) {
+    if ((e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[0], scores_kernel(p->dim, p->one), kThreads, p->scores_smem)) != cudaSuccess ||
+        (e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm[1], values_kernel(p->one), kThreads, p->values_smem)) != cudaSuccess) {
         release(p);
         return cuda_fail("create", e);
     }
@@ -1334,17 +1703,29 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.exps = p->exps;
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int all = (int)((longest + kTile - 1) / kTile), most = (c.max_block * c.group + 7) / 8;
+    static const int force = getenv("LLMX_C") ? atoi(getenv("LLMX_C")) : -1;
+    if (force > 0 && most <= kAttendBlocks && all <= 255) {
+        while (1 << c.cluster_log < force) c.cluster_log++;
+        const int cluster = 1 << c.cluster_log;
+        c.tiles = (all + cluster - 1) / cluster;
+        const Places at(c.tiles, cluster, most, c.dim);
+        if (at.size <= kMaxSmem) {
+            const cudaError_t e = launch(attend_kernel(p->dim, p->one), requests * (unsigned)(p->kv * cluster), kThreads, (size_t)at.size, c, s, cluster);
+            return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
+        }
+    }
     const uint64_t items = (uint64_t)requests * p->kv * ((longest + kTile - 1) / kTile);
     auto grid = [&](int ctas) { return (unsigned)std::min<uint64_t>(items, (uint64_t)ctas); };
-    cudaError_t e = launch(scores_kernel(p->dim), grid(p->scores_ctas), kThreads, p->scores_smem, c, s);
-    if (e == cudaSuccess) e = launch((const void *)k_values, grid(p->values_ctas), kThreads, p->values_smem, c, s);
+    cudaError_t e = launch(scores_kernel(p->dim, p->one), grid(p->scores_ctas), kThreads, p->scores_smem, c, s);
+    if (e == cudaSuccess) e = launch(values_kernel(p->one), grid(p->values_ctas), kThreads, p->values_smem, c, s);
     if (e == cudaSuccess) {
         const int tiles = (int)((longest + kTile - 1) / kTile);
         // few columns: a warp per kAhead tiles, for latency; many: no more warps than fill the SMs
         const uint64_t columns = (uint64_t)rows * p->heads;
         const int warps = (int)std::max<uint64_t>(1, std::min<uint64_t>({kMaxJoinWarps, (uint64_t)(tiles + kAhead - 1) / kAhead, (uint64_t)p->sms * 32 / columns}));
         const bool far = tiles > kShortTiles;
-        const size_t smem = (size_t)(warps - 1) * kMaxStretches * p->dim * (far ? sizeof(Stretch<true>) : sizeof(Stretch<false>));
+        const size_t smem = (size_t)(warps - 1) * kMaxStretches * 32 * sizeof(Stretch);
         e = launch(far ? (const void *)k_join<true> : (const void *)k_join<false>, rows * (unsigned)p->heads, 32 * warps, smem, c, s);
     }
     return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
