@@ -351,7 +351,8 @@ static __device__ __forceinline__ void stage_queries(const Call &c, const Strip 
 }
 
 // The pages of 16 positions' keys, and this lane's share of them: rows g and g + 8, dimensions 32 s + 8 t4
-// .. + 7; zeros for what is not there.
+// .. + 7.  What is not there is read from a place that is: scores of positions behind the last are
+// not looked at, and the queries' dimensions behind the last are 0.
 struct KeyPages {
     uint32_t page[2];
     __device__ __forceinline__ void load(const Call &c, const Strip &z, int p0, uint32_t &worst) {
@@ -360,75 +361,60 @@ struct KeyPages {
     }
 };
 template <int KS>
-static __device__ __forceinline__ void load_keys(const Call &c, const Strip &z, const KeyPages &pages, int p0, uint4 (&raw)[2][KS]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
+struct KeyRows {
     const char *row[2];
+    int last;  // bytes to the last step's dimensions
+    __device__ __forceinline__ void start(const Call &c, const Strip &z, const KeyPages &pages, int p0) {
+        const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
 #pragma unroll
-    for (int r = 0; r < 2; r++) row[r] = rows_of(c, c.k, pages.page[r], (uint32_t)(p0 >> 3) + r, z.h) + (g * c.row_bytes + 16 * t4);
-    if (p0 + 16 <= z.length && c.dim == 32 * KS) {
-#pragma unroll
-        for (int r = 0; r < 2; r++)
-#pragma unroll
-            for (int s = 0; s < KS; s++) raw[r][s] = ld16(row[r] + 64 * s);
-        return;
+        for (int r = 0; r < 2; r++) row[r] = rows_of(c, c.k, pages.page[r], (uint32_t)(p0 >> 3) + r, z.h) + (g * c.row_bytes + 16 * t4);
+        last = 32 * (KS - 1) + 8 * t4 < c.dim ? 64 * (KS - 1) : -16 * t4;
     }
+    __device__ __forceinline__ void load(int s, uint4 (&raw)[2][KS]) const {
 #pragma unroll
-    for (int r = 0; r < 2; r++)
-#pragma unroll
-        for (int s = 0; s < KS; s++) raw[r][s] = p0 + 8 * r + g < z.length && 32 * s + 8 * t4 < c.dim ? ld16(row[r] + 64 * s) : make_uint4(0, 0, 0, 0);
-}
-// Their byte planes, limited and from 0 to 4096: min(k, 2048), then max(k + 2048, 0).  Returns whether some
-// value of the warp's is at the upper limit (its high byte is 16).
+        for (int r = 0; r < 2; r++) raw[r][s] = ld16(row[r] + (s == KS - 1 ? last : 64 * s));
+    }
+};
 template <int KS>
-static __device__ __forceinline__ bool key_planes(const uint4 (&raw)[2][KS], uint32_t (&kl)[KS][4], uint32_t (&kh)[KS][4]) {
-    uint32_t limit = 0;
+static __device__ __forceinline__ void load_keys(const Call &c, const Strip &z, const KeyPages &pages, int p0, uint4 (&raw)[2][KS]) {
+    KeyRows<KS> rows;
+    rows.start(c, z, pages, p0);
 #pragma unroll
-    for (int s = 0; s < KS; s++)
-#pragma unroll
-        for (int r = 0; r < 2; r++) {
-            auto shift = [](uint32_t w) { return __viaddmax_s16x2(__vmins2(w, 0x08000800u), 0x08000800u, 0u); };
-            const uint4 w = make_uint4(shift(raw[r][s].x), shift(raw[r][s].y), shift(raw[r][s].z), shift(raw[r][s].w));
-            kl[s][r] = low4(w.x, w.y);
-            kl[s][r + 2] = low4(w.z, w.w);
-            kh[s][r] = high4(w.x, w.y);
-            kh[s][r + 2] = high4(w.z, w.w);
-            limit |= kh[s][r] | kh[s][r + 2];
-        }
-    return __any_sync(0xffffffffu, (limit & 0x10101010u) != 0);
+    for (int s = 0; s < KS; s++) rows.load(s, raw);
 }
 
-// A warp scores 16 positions (the rows of A, a lane's 16-byte loads of key rows split into bytes)
-// against the 8 columns (query rows) of block nb: w[0] position p0 + g, w[1] p0 + 8 + g, columns
-// 2 t4 and 2 t4 + 1, biased.  Returns their columns' maxima over the positions that they see, in
-// lanes 0 to 3 (of column pair t4).
-template <int KS>
-static __device__ __forceinline__ uint32_t score_block(const Call &c, const Strip &z, const uint32_t (&kl)[KS][4], const uint32_t (&kh)[KS][4], bool some,
-                                                       int nb, int p0, const uint4 *queries, const uint4 *rests, const Column &column, uint32_t (&w)[2]) {
-    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int2 bias = *reinterpret_cast<const int2 *>(&column.bias[nb * 8 + 2 * t4]);
-    int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {-bias.x, -bias.y, -bias.x, -bias.y};
+// What scores 16 positions (the rows of A) against 8 columns (query rows): the sums of the byte products.
+struct Sums {
+    int hh[4], mid[4], ll[4];
+    __device__ __forceinline__ void start(const Column &column, int nb) {
+        const int2 bias = *reinterpret_cast<const int2 *>(&column.bias[nb * 8 + 2 * (threadIdx.x & 3)]);
 #pragma unroll
-    for (int s = 0; s < KS; s++) {
-        const uint4 q = queries[(nb * KS + s) * 32 + lane];
-        mma_us(hh, kh[s], q.z, q.w, hh);
-        mma_uu(mid, kh[s], q.x, q.y, mid);
-        mma_uu(ll, kl[s], q.x, q.y, ll);
-        mma_us(mid, kl[s], q.z, q.w, mid);
-    }
-    if (some) {
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const uint4 r = rests[(nb * KS + s) * 32 + lane];
-            uint32_t m[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) m[i] = kh[s][i] >> 4 & 0x01010101u;
-            mma_us(mid, m, r.z, r.w, mid);
-            mma_uu(ll, m, r.x, r.y, ll);
+        for (int i = 0; i < 4; i++) {
+            hh[i] = mid[i] = 0;
+            ll[i] = i & 1 ? -bias.y : -bias.x;
         }
     }
+    __device__ __forceinline__ void add(const uint32_t (&kl)[4], const uint32_t (&kh)[4], uint4 q) {
+        mma_us(hh, kh, q.z, q.w, hh);
+        mma_uu(mid, kh, q.x, q.y, mid);
+        mma_uu(ll, kl, q.x, q.y, ll);
+        mma_us(mid, kl, q.z, q.w, mid);
+    }
+    __device__ __forceinline__ void add_rest(const uint32_t (&kh)[4], uint4 r) {
+        uint32_t m[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) m[i] = kh[i] >> 4 & 0x01010101u;
+        mma_us(mid, m, r.z, r.w, mid);
+        mma_uu(ll, m, r.x, r.y, ll);
+    }
+};
+// The scores from them: w[0] position p0 + g, w[1] p0 + 8 + g, columns 2 t4 and 2 t4 + 1 of block nb, biased.
+// Returns their columns' maxima over the positions that they see, in lanes 0 to 3 (of column pair t4).
+static __device__ __forceinline__ uint32_t finish_scores(const Call &c, const Strip &z, const Sums &u, int nb, int p0, const Column &column, uint32_t (&w)[2]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     int sc[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++) sc[i] = score_of((int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]), c.scale8);
+    for (int i = 0; i < 4; i++) sc[i] = score_of((int)(((uint32_t)u.hh[i] << 16) + ((uint32_t)u.mid[i] << 8) + (uint32_t)u.ll[i]), c.scale8);
     const int2 wide = *reinterpret_cast<const int2 *>(&column.wide[nb * 8 + 2 * t4]);
     if (__any_sync(0xffffffffu, (wide.x | wide.y) != 0)) {
 #pragma unroll 1
@@ -459,10 +445,56 @@ static __device__ __forceinline__ uint32_t score_block(const Call &c, const Stri
     return top;
 }
 
+// The byte planes of one step of 32 dimensions, limited and from 0 to 4096: min(k, 2048), then max(k + 2048, 0).
+// Returns the high ones together.
+static __device__ __forceinline__ uint32_t step_planes(const uint4 a, const uint4 b, uint32_t (&kl)[4], uint32_t (&kh)[4]) {
+    auto shift = [](uint32_t w) { return __viaddmax_s16x2(__vmins2(w, 0x08000800u), 0x08000800u, 0u); };
+    const uint4 x = make_uint4(shift(a.x), shift(a.y), shift(a.z), shift(a.w)), y = make_uint4(shift(b.x), shift(b.y), shift(b.z), shift(b.w));
+    kl[0] = low4(x.x, x.y);
+    kl[1] = low4(y.x, y.y);
+    kl[2] = low4(x.z, x.w);
+    kl[3] = low4(y.z, y.w);
+    kh[0] = high4(x.x, x.y);
+    kh[1] = high4(y.x, y.y);
+    kh[2] = high4(x.z, x.w);
+    kh[3] = high4(y.z, y.w);
+    return kh[0] | kh[1] | kh[2] | kh[3];
+}
+// Scores a warp's 16 positions against all column blocks and loads the next ones' keys, at pn, meanwhile;
+// store(nb, maxima, scores).
+template <int KS, bool kOne, class Store>
+static __device__ __forceinline__ void score_tile(const Call &c, const Strip &z, int p0, uint4 (&raw)[2][KS], const Strip &zn, const KeyPages &pages, int pn,
+                                                  const uint4 *queries, const uint4 *rests, const Column &column, Store store) {
+    const int lane = threadIdx.x & 31;
+    KeyRows<KS> next;
+    next.start(c, zn, pages, pn);
+    uint32_t kl[KS][4], kh[KS][4], limit = 0;
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+        limit |= step_planes(raw[0][s], raw[1][s], kl[s], kh[s]);
+        next.load(s, raw);
+    }
+    // some value is at the upper limit (its high byte is 16)
+    const bool some = __any_sync(0xffffffffu, (limit & 0x10101010u) != 0);
+#pragma unroll 1
+    for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+        Sums u;
+        u.start(column, nb);
+#pragma unroll
+        for (int s = 0; s < KS; s++) u.add(kl[s], kh[s], queries[(nb * KS + s) * 32 + lane]);
+        if (some)
+#pragma unroll
+            for (int s = 0; s < KS; s++) u.add_rest(kh[s], rests[(nb * KS + s) * 32 + lane]);
+        uint32_t w[2];
+        const uint32_t top = finish_scores(c, z, u, nb, p0, column, w);
+        store(nb, top, w);
+    }
+}
+
 // One CTA's run of tiles, a warp per 16 positions.
 template <int KS, bool kOne>  // steps of 32 dimensions; one column block
 __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    extern __shared__ __align__(1024) unsigned char dynamic[];
     __shared__ __align__(16) Column column;
     const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;  // column blocks
     uint4 *queries = reinterpret_cast<uint4 *>(dynamic);          // [most][KS][32]
@@ -483,7 +515,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
     KeyPages pages;
     pages.load(c, z, cur.t * kTile + warp * 16, worst);
     load_keys<KS>(c, z, pages, cur.t * kTile + warp * 16, raw);
-    if (cur.t + 1 < cur.tiles) pages.load(c, z, (cur.t + 1) * kTile + warp * 16, worst);
+    pages.load(c, z, (cur.t + 1) * kTile + warp * 16, worst);
     for (int item = first; item < end;) {  // a (request, key head)
         __syncthreads();                   // the last one's columns are done with
         stage_queries<KS>(c, z, warp, kWarps, queries, rests, column);
@@ -494,31 +526,22 @@ __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
         int p0 = cur.t * kTile + warp * 16;
         const Strip here = z;
         for (int k = 0; k < n; k++, p0 += kTile, at += 4) {
-            uint32_t kh[KS][4], kl[KS][4];
-            const bool some = key_planes<KS>(raw, kl, kh);
             // the next tile's keys are on their way while this one's are used, the next one's page numbers too
-            if (k + 1 < n) {
-                load_keys<KS>(c, z, pages, p0 + kTile, raw);
-                if (k + 2 < n) pages.load(c, z, p0 + 2 * kTile, worst);
-            } else if (item + n < end) {
+            const bool inside = k + 1 < n, more = inside || item + n < end;
+            if (!inside && more) {
                 cur.t += n - 1;
                 cur.next(c, meta);
                 z = cur.strip();
                 pages.load(c, z, warp * 16, worst);
-                load_keys<KS>(c, z, pages, warp * 16, raw);
-                if (cur.tiles > 1) pages.load(c, z, kTile + warp * 16, worst);
             }
-            for (int nb = 0; nb < (kOne ? 1 : here.blocks); nb++) {
+            const int pn = inside ? p0 + kTile : warp * 16;
+            score_tile<KS, kOne>(c, here, p0, raw, z, pages, pn, queries, rests, column, [&](int nb, uint32_t top, const uint32_t(&w)[2]) {
                 const size_t block = at + nb * step;
-                uint32_t top = 0;  // (-32768)
-                if (p0 < here.length) {
-                    uint32_t w[2];
-                    top = score_block<KS>(c, here, kl, kh, some, nb, p0, queries, rests, column, w);
-                    c.score[block * 64 + lane] = w[0];
-                    c.score[block * 64 + 32 + lane] = w[1];
-                }
+                c.score[block * 64 + lane] = w[0];
+                c.score[block * 64 + 32 + lane] = w[1];
                 if (lane < 4) reinterpret_cast<uint32_t *>(c.top)[block * 4 + lane] = top;
-            }
+            });
+            pages.load(c, z, pn + kTile, worst);
         }
         item += n;
     }
@@ -531,26 +554,22 @@ constexpr int kDepth = 2;                       // tiles of a warp's ring
 constexpr int kSlice = kTile * 64;              // bytes of a tile's share: 64 positions, 32 elements
 constexpr int kRing = kWarps * kDepth * kSlice;
 
-static __device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+static __device__ __forceinline__ void copy16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
 // A tile's values of 32 elements into a warp's ring: a position's 64 bytes in a row, its 16-byte units
 // turned by row / 2 mod 4, so that the 8 rows that a matrix load takes, and those that a copy writes, lie in
-// different banks.  A lane copies one unit of 8 positions, from one page.
+// different banks.  A lane copies one unit of 8 positions, from one page, in an order of its own.  What
+// is not there comes from a place that is: its probabilities are 0, its elements not stored.
 static __device__ __forceinline__ void fetch_values(const Call &c, const Strip &z, int t, int part, unsigned char *ring, uint32_t &worst) {
     const int lane = threadIdx.x & 31, unit = lane & 3, j = lane >> 2;
-    const int left = z.length - t * kTile - 8 * j;  // positions from this lane's first on
-    const uint32_t p8 = (uint32_t)(t * 8 + j);
-    // (what is not there may hold anything: the probabilities there are 0)
-    if (left <= 0 || part * 32 + unit * 8 >= c.dim) return;
-    const char *rows = rows_of(c, c.v, page_of(c, z.table, p8, worst), p8, z.h) + (part * 64 + unit * 16);
-    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring) + j * 512;
+    const uint32_t p8 = min((uint32_t)(t * 8 + j), (uint32_t)(z.length - 1) >> 3);
+    const char *rows = rows_of(c, c.v, page_of(c, z.table, p8, worst), p8, z.h) + (part * 32 + unit * 8 < c.dim ? part * 64 + unit * 16 : 0);
+    // row i ^ j goes to j * 512 + (i ^ j) * 64 + (unit ^ (i ^ j) / 2 mod 4) * 16 (a slice starts at a multiple of 512)
+    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring) + j * 512 + j * 64 + ((unit ^ (j >> 1)) & 3) * 16;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t r = (i + j) & 7;  // (rows in another order for each lane: in different banks)
-        copy16(dst + r * 64 + ((unit ^ (r >> 1)) & 3) * 16, rows + r * c.row_bytes, (int)r < left);
-    }
+    for (int i = 0; i < 8; i++) copy16(dst ^ (uint32_t)(i * 64 + (i >> 1 & 3) * 16), rows + (uint32_t)(i ^ j) * c.row_bytes);
 }
 static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 
@@ -562,8 +581,8 @@ static __device__ __forceinline__ void load_octet(uint32_t at, uint32_t (&r)[4])
 // are those of 8 j + 2 t4 and the next, j = 0, 1 (first words) and j = 2, 3.  Returns whether values were limited.
 static __device__ __forceinline__ bool value_planes(const unsigned char *ring, uint32_t (&vl)[2][2][4], uint32_t (&vh)[2][2][4]) {
     const int lane = threadIdx.x & 31;
-    const uint32_t row = (uint32_t)__cvta_generic_to_shared(ring) + lane * 64;
-    const int turn = lane >> 1 & 3;
+    // octet o of a row is its unit o ^ row / 2 mod 4
+    const uint32_t row = (uint32_t)__cvta_generic_to_shared(ring) + lane * 64 + (lane >> 1 & 3) * 16;
     bool limit = false;
 #pragma unroll 1
     for (;;) {
@@ -573,7 +592,7 @@ static __device__ __forceinline__ bool value_planes(const unsigned char *ring, u
 #pragma unroll
             for (int o = 0; o < 4; o++) {
                 uint32_t r[4];
-                load_octet(row + s * 2048 + ((o ^ turn) * 16), r);
+                load_octet((row ^ (uint32_t)(o * 16)) + s * 2048, r);
                 if (limit)
 #pragma unroll
                     for (int i = 0; i < 4; i++) r[i] = limit2(r[i]);
@@ -620,29 +639,52 @@ static __device__ __forceinline__ void weigh(const uint32_t (&vl)[2][2][4], cons
                                              bool with_sum, int (&sum)[2]) {
     const int lane = threadIdx.x & 31;
     const uint4 b[2] = {prob[lane], prob[32 + lane]};
-#pragma unroll
-    for (int mb = 0; mb < 2; mb++) {
-        // rnd8 of rnd6 of the sum is (sum + 2^5 + 2^13) >> 14; the sum is below 2^31 - 2^16
-        int hh[4] = {0, 0, 0, 0}, mid[4] = {0, 0, 0, 0}, ll[4] = {8224, 8224, 8224, 8224};
+    uint4 rest[2];  // of the probabilities, for values at the upper limit
+    if (limit)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            mma_su(hh, vh[s][mb], b[s].z, b[s].w, hh);
-            mma_su(mid, vh[s][mb], b[s].x, b[s].y, mid);
-            mma_uu(ll, vl[s][mb], b[s].x, b[s].y, ll);
-            mma_uu(mid, vl[s][mb], b[s].z, b[s].w, mid);
-            if (limit) {
-                const uint32_t r0 = rest2(__byte_perm(b[s].x, b[s].z, 0x5140)), r1 = rest2(__byte_perm(b[s].x, b[s].z, 0x7362));
-                const uint32_t r2 = rest2(__byte_perm(b[s].y, b[s].w, 0x5140)), r3 = rest2(__byte_perm(b[s].y, b[s].w, 0x7362));
+            const uint32_t r0 = rest2(__byte_perm(b[s].x, b[s].z, 0x5140)), r1 = rest2(__byte_perm(b[s].x, b[s].z, 0x7362));
+            const uint32_t r2 = rest2(__byte_perm(b[s].y, b[s].w, 0x5140)), r3 = rest2(__byte_perm(b[s].y, b[s].w, 0x7362));
+            rest[s] = make_uint4(low4(r0, r1), low4(r2, r3), high4(r0, r1), high4(r2, r3));
+        }
+#pragma unroll
+    for (int mb = 0; mb < 2; mb++) {
+        // The high products' sums become a part of the middle ones' and these of the low ones'; and rnd8 of rnd6 of
+        // the sum is (sum + 2^5 + 2^13) >> 14; the sum is below 2^31 - 2^16.
+        int d[4] = {0, 0, 0, 0}, v[4];
+        mma_su(d, vh[0][mb], b[0].z, b[0].w, d);
+        mma_su(d, vh[1][mb], b[1].z, b[1].w, d);
+#pragma unroll
+        for (int i = 0; i < 4; i++) d[i] *= 256;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            mma_su(d, vh[s][mb], b[s].x, b[s].y, d);
+            mma_uu(d, vl[s][mb], b[s].z, b[s].w, d);
+        }
+        if (limit) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
                 uint32_t m[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) m[i] = at_limit(vh[s][mb][i]);
-                mma_us(mid, m, high4(r0, r1), high4(r2, r3), mid);
-                mma_uu(ll, m, low4(r0, r1), low4(r2, r3), ll);
+                mma_us(d, m, rest[s].z, rest[s].w, d);
             }
         }
-        int v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (int)(((uint32_t)hh[i] << 16) + ((uint32_t)mid[i] << 8) + (uint32_t)ll[i]) >> 14;
+        for (int i = 0; i < 4; i++) d[i] = (int)((uint32_t)d[i] * 256u + 8224u);
+        mma_uu(d, vl[0][mb], b[0].x, b[0].y, d);
+        mma_uu(d, vl[1][mb], b[1].x, b[1].y, d);
+        if (limit) {
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                uint32_t m[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) m[i] = at_limit(vh[s][mb][i]);
+                mma_uu(d, m, rest[s].x, rest[s].y, d);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] = d[i] >> 14;
         y[2 * mb] = transpose8(pack_sat16(v[0], v[1]));
         y[2 * mb + 1] = transpose8(pack_sat16(v[2], v[3]));
     }
@@ -663,31 +705,32 @@ constexpr int kChunk = 4;  // tiles of a (request, key head) whose probabilities
 
 // The warps' shares of a tile's elements: `part` of 32, and with fewer parts than warps every `step`-th tile.
 struct Share {
-    int part, first, step;
+    int part, first, step, octets;  // (octets of elements)
     __device__ __forceinline__ Share(int dim, int warp) {
         const int log = dim > 64 ? 2 : dim > 32 ? 1 : 0;  // 4, 2 or 1 (of three parts the fourth warp has none)
         part = warp & ((1 << log) - 1);
         first = part * 32 < dim ? warp >> log : INT_MAX;
         step = kWarps >> log;
+        octets = min((dim - part * 32) >> 3, 4);
     }
 };
 
 // One CTA's run of tiles, in chunks of up to kChunk: their probabilities, by all warps, through shared
-// memory; then every warp weighs its 32 elements of every tile, for itself.
+// memory (two buffers in turn, so one barrier a chunk does); then every warp weighs its 32 elements
+// of every tile, for itself.
 template <bool kOne>
 __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
+    extern __shared__ __align__(1024) unsigned char dynamic[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3, cp = t4;
     const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;  // column blocks
     const int chunk = kOne ? kChunk : max(1, kChunk / most);
     unsigned char *ring = dynamic + warp * kDepth * kSlice;
-    uint4 *prob = reinterpret_cast<uint4 *>(dynamic + kRing);                    // [chunk][most][64]
-    uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + chunk * most * 64);
+    uint4 *prob = reinterpret_cast<uint4 *>(dynamic + kRing);  // [2][chunk][most][64]
+    uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + 2 * chunk * most * 64);
     const int16_t *exps = reinterpret_cast<const int16_t *>(exps_w);
-    uint32_t *runs = exps_w + kExpWords;         // [chunk + 1][most * 4] maxima of column pairs up to a tile
-    uint32_t *parts_top = runs + (chunk + 1) * most * 4;  // [kWarps][most * 4]
-    int *seen = reinterpret_cast<int *>(parts_top + kWarps * most * 4);  // [most * 8]
-    Meta *meta = reinterpret_cast<Meta *>(seen + most * 8);
+    uint32_t *before = exps_w + kExpWords + warp * most * 4;  // the warp's own: maxima of column pairs up to the chunk
+    int *seen = reinterpret_cast<int *>(exps_w + kExpWords + kWarps * most * 4);  // [2][most * 8]
+    Meta *meta = reinterpret_cast<Meta *>(seen + 2 * most * 8);
     for (int i = threadIdx.x; i < kExpWords; i += kThreads) exps_w[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
     pdl_wait();
     pdl_trigger();
@@ -701,29 +744,47 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     if (first >= end) return;
     uint32_t worst = 0;
     const Share share(c.dim, warp);
+    const int pos = warp * 16 + 8 * (lane >> 4) + 2 * (lane >> 2 & 3);  // of a tile: this lane's first of two
     Cursor cur;
     cur.start(c, meta, first);
     bool moved = true;
+    int turn = 0, buffer = 0;
+    // of a chunk's tiles: scores of this lane's two positions and column pair; maxima of 16 positions, 16 words of
+    // two tiles a load
+    uint32_t score[kChunk][2], top[kChunk / 2];
+    auto load_scores = [&](int slot, int n) {
+        const uint32_t *s = c.score + (size_t)slot * 256 + pos * 4 + cp;
+        const uint32_t *t = reinterpret_cast<const uint32_t *>(c.top) + (size_t)slot * 16 + lane;
+#pragma unroll
+        for (int k = 0; k < kChunk; k++) {
+            const int at = min(k, n - 1) * 256;
+            score[k][0] = s[at];
+            score[k][1] = s[at + 4];
+        }
+#pragma unroll
+        for (int k = 0; k < kChunk / 2; k++) top[k] = 32 * k + lane < 16 * n ? t[32 * k] : 0;
+    };
+    auto length_of = [&](int item) { return min(min(chunk, cur.tiles - cur.t), end - item); };
+    if constexpr (kOne) load_scores(cur.slot(0), length_of(first));
     for (int item = first; item < end;) {
         const Strip z = cur.strip();
-        const int n = min(min(chunk, cur.tiles - cur.t), end - item);  // tiles of this chunk
-        const int pairs = z.blocks * 4;
+        const int n = length_of(item), t0 = cur.t, slot0 = cur.slot(0), tiles = cur.tiles;
         int fetched = share.first;
         auto fetch = [&](int slot) {
             if (fetched < n) {
-                fetch_values(c, z, cur.t + fetched, share.part, ring + slot * kSlice, worst);
+                fetch_values(c, z, t0 + fetched, share.part, ring + slot * kSlice, worst);
                 fetched += share.step;
             }
             commit();
         };
 #pragma unroll
         for (int i = 0; i < kDepth; i++) fetch(i);
-        __syncthreads();  // the last chunk is done with
-        if (moved) {      // the maxima of the tiles before
+        if (moved) {  // the maxima of the tiles before, by every warp for itself
+            turn ^= 1;
             for (int nb = 0; nb < z.blocks; nb++) {
-                const uint4 *tops = c.top + (size_t)(cur.slot(nb) - cur.t) * 4;
+                const uint4 *tops = c.top + (size_t)(slot0 + nb * tiles - t0) * 4;
                 uint4 m = make_uint4(0, 0, 0, 0);
-                for (int i = threadIdx.x; i < cur.t * 4; i += kThreads) {
+                for (int i = lane; i < t0 * 4; i += 32) {
                     const uint4 w = tops[i];
                     m = make_uint4(__vmaxu2(m.x, w.x), __vmaxu2(m.y, w.y), __vmaxu2(m.z, w.z), __vmaxu2(m.w, w.w));
                 }
@@ -734,55 +795,55 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
                     m.z = __vmaxu2(m.z, __shfl_xor_sync(0xffffffffu, m.z, o));
                     m.w = __vmaxu2(m.w, __shfl_xor_sync(0xffffffffu, m.w, o));
                 }
-                if (lane == 0) *reinterpret_cast<uint4 *>(parts_top + (warp * most + nb) * 4) = m;
+                if (lane == 0) *reinterpret_cast<uint4 *>(before + nb * 4) = m;
             }
+            // (two buffers: warps may still be at the last one's)
             for (int col = threadIdx.x; col < z.blocks * 8; col += kThreads)
-                seen[col] = col < z.rows * c.group ? z.length - z.rows + 1 + col / c.group : 0;
+                seen[turn * most * 8 + col] = col < z.rows * c.group ? z.length - z.rows + 1 + col / c.group : 0;
             __syncthreads();
         }
-        for (int i = threadIdx.x; i < pairs; i += kThreads) {
-            uint32_t m = runs[chunk * most * 4 + i];  // up to the last chunk's end
-            if (moved) {
-                m = 0;
-                for (int w = 0; w < kWarps; w++) m = __vmaxu2(m, parts_top[w * most * 4 + i]);
-            }
-            runs[i] = m;
-            const uint32_t *tops = reinterpret_cast<const uint32_t *>(c.top + (size_t)cur.slot(i >> 2) * 4) + (i & 3);
-            uint32_t w[kChunk][4];
-#pragma unroll
-            for (int k = 0; k < kChunk; k++)
-                if (k < n)
-                    for (int b = 0; b < 4; b++) w[k][b] = tops[(k * 4 + b) * 4];
-#pragma unroll
-            for (int k = 0; k < kChunk; k++)
-                if (k < n) {
-                    m = __vmaxu2(m, __vmaxu2(__vmaxu2(w[k][0], w[k][1]), __vmaxu2(w[k][2], w[k][3])));
-                    runs[(k + 1) * most * 4 + i] = m;
-                }
-            runs[chunk * most * 4 + i] = m;  // (where n is less, nobody else reads it)
-        }
-        __syncthreads();
-        // probabilities: a warp has block `warp` of 16 positions of every tile
-        const int cp = lane & 3, pos = warp * 16 + 8 * (lane >> 4) + 2 * (lane >> 2 & 3);
-        const int before = z.length - z.rows + 1;
+        uint4 *pb = prob + (buffer ? chunk * most * 64 : 0);
+        buffer ^= 1;
+        const int whole = z.length - z.rows + 1;  // positions that every row sees
         for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
-            const uint32_t *score = c.score + (size_t)cur.slot(nb) * 256 + pos * 4 + cp;
-            const int seen0 = seen[nb * 8 + 2 * cp], seen1 = seen[nb * 8 + 2 * cp + 1];
+            const int slot = slot0 + nb * tiles;
+            if constexpr (!kOne) load_scores(slot, n);
+            // maxima of this lane's column pair up to each tile
+            uint32_t m[kChunk];
+#pragma unroll
+            for (int k = 0; k < kChunk / 2; k++) {
+                uint32_t w = top[k];
+                w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, 4));
+                w = __vmaxu2(w, __shfl_xor_sync(0xffffffffu, w, 8));
+                m[2 * k] = __shfl_sync(0xffffffffu, w, cp);
+                m[2 * k + 1] = __shfl_sync(0xffffffffu, w, 16 + cp);
+            }
+            uint32_t was = before[nb * 4 + cp];
+            const int seen0 = seen[turn * most * 8 + nb * 8 + 2 * cp], seen1 = seen[turn * most * 8 + nb * 8 + 2 * cp + 1];
             const bool full = nb * 8 + 8 <= z.rows * c.group;
-            uint32_t w[kChunk][2];
 #pragma unroll
             for (int k = 0; k < kChunk; k++)
                 if (k < n) {
-                    w[k][0] = score[k * 256];
-                    w[k][1] = score[k * 256 + 4];
+                    const int p = (t0 + k) * kTile;
+                    m[k] = __vmaxu2(m[k], was);
+                    probabilities(exps, score[k][0], score[k][1], m[k], full && p + kTile <= whole, p + pos, seen0, seen1, warp, pb + (k * most + nb) * 64);
+                    if (warp == 0 && lane < 4) {
+                        const uint32_t d = m[k] - __vmaxu2(was, __vmaxu2(m[k], 0x08000800u) - 0x08000800u);
+                        int2 *f = c.fsum + (size_t)(slot + k) * 8 + 2 * lane;
+                        f[0].x = exps[d & 0xffffu];
+                        f[1].x = exps[d >> 16];
+                    }
+                    was = m[k];
                 }
-#pragma unroll
-            for (int k = 0; k < kChunk; k++)
-                if (k < n) {
-                    const int p = (cur.t + k) * kTile;
-                    probabilities(exps, w[k][0], w[k][1], runs[(k + 1) * most * 4 + nb * 4 + cp], full && p + kTile <= before, p + pos, seen0, seen1, warp,
-                                  prob + (k * most + nb) * 64);
-                }
+            __syncwarp();
+            if (lane < 4) before[nb * 4 + lane] = was;
+            __syncwarp();
+        }
+        item += n;
+        if (item < end) {
+            cur.t += n - 1;
+            moved = cur.next(c, meta);
+            if constexpr (kOne) load_scores(cur.slot(0), length_of(item));  // on their way while the values are weighed
         }
         __syncthreads();
 #pragma unroll 1
@@ -796,26 +857,20 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
             for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
                 uint32_t y[4];
                 int sum[2];
-                weigh(vl, vh, limit, prob + (k * most + nb) * 64, y, share.part == 0, sum);
-                const size_t slot = (size_t)cur.slot(nb) + k;
+                weigh(vl, vh, limit, pb + (k * most + nb) * 64, y, share.part == 0, sum);
+                const size_t slot = (size_t)(slot0 + nb * tiles + k);
                 uint32_t *dst = reinterpret_cast<uint32_t *>(c.tv + (slot * 8 + g) * c.dim + share.part * 32 + 2 * t4);
 #pragma unroll
                 for (int o = 0; o < 4; o++)
-                    if (share.part * 32 + 8 * o < c.dim) dst[4 * o] = y[o];
+                    if (o < share.octets) dst[4 * o] = y[o];
                 if (share.part == 0 && lane < 4) {
-                    const uint32_t was = runs[k * most * 4 + nb * 4 + lane], m = runs[(k + 1) * most * 4 + nb * 4 + lane];
-                    const uint32_t d = m - __vmaxu2(was, __vmaxu2(m, 0x08000800u) - 0x08000800u);
-                    *reinterpret_cast<int4 *>(c.fsum + slot * 8 + 2 * lane) = make_int4(exps[d & 0xffffu], sum[0], exps[d >> 16], sum[1]);
+                    int2 *f = c.fsum + slot * 8 + 2 * lane;
+                    f[0].y = sum[0];
+                    f[1].y = sum[1];
                 }
             }
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-        item += n;
-        moved = false;
-        if (item < end) {
-            cur.t += n - 1;
-            moved = cur.next(c, meta);
-        }
     }
     report(c, worst);
 }
@@ -893,7 +948,7 @@ struct Stretch {
 // kMaxStretches, and a stretch on which something might saturate, it goes through itself, one by one.
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    extern __shared__ __align__(1024) unsigned char dynamic[];
     __shared__ int factors[kMaxJoinWarps][kMaxStretches], counts[kMaxJoinWarps], rest[kMaxJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     const int quads = c.dim >> 2;
@@ -1107,7 +1162,7 @@ static __device__ __forceinline__ void cluster_meet() {
 
 template <int KS, bool kOne>
 __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
-    extern __shared__ __align__(16) unsigned char dynamic[];
+    extern __shared__ __align__(1024) unsigned char dynamic[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
     const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;
     const int log = c.cluster_log, cluster = 1 << log;
@@ -1158,7 +1213,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
             pages.load(c, z, p0, worst);
             load_keys<KS>(c, z, pages, p0, raw);
         }
-        if (own > 1) pages.load(c, z, p0 + kTile, worst);
+        pages.load(c, z, p0 + kTile, worst);
         stage_queries<KS>(c, z, warp, kWarps, queries, rests, column);
 #pragma unroll
         for (int i = 0; i < kDepth; i++) fetch(i);
@@ -1173,23 +1228,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
         __syncthreads();
 #pragma unroll 1
         for (int k = 0; k < own; k++, p0 += kTile) {
-            uint32_t kh[KS][4], kl[KS][4];
-            const bool some = key_planes<KS>(raw, kl, kh);
-            if (k + 1 < own) {
-                load_keys<KS>(c, z, pages, p0 + kTile, raw);
-                if (k + 2 < own) pages.load(c, z, p0 + 2 * kTile, worst);
-            }
-            for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+            score_tile<KS, kOne>(c, z, p0, raw, z, pages, p0 + kTile, queries, rests, column, [&](int nb, uint32_t top, const uint32_t(&w)[2]) {
                 const int block = (k * most + nb) * 4 + warp;
-                uint32_t top = 0;
-                if (p0 < z.length) {
-                    uint32_t w[2];
-                    top = score_block<KS>(c, z, kl, kh, some, nb, p0, queries, rests, column, w);
-                    score[block * 64 + lane] = w[0];
-                    score[block * 64 + 32 + lane] = w[1];
-                }
+                score[block * 64 + lane] = w[0];
+                score[block * 64 + 32 + lane] = w[1];
                 if (lane < 4) tops[block * 4 + lane] = top;
-            }
+            });
+            pages.load(c, z, p0 + 2 * kTile, worst);
         }
     }
     __syncthreads();
@@ -1272,7 +1317,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
                 const uint32_t to = values + (uint32_t)(((nb * of_block + (g >> log)) * stride + t0 + k) * 2 * c.dim);
 #pragma unroll
                 for (int o = 0; o < 4; o++)
-                    if (share.part * 32 + 8 * o < c.dim) put(to + 16 * o, y[o]);
+                    if (o < share.octets) put(to + 16 * o, y[o]);
             }
             if (share.part == 0 && lane < 4) {
                 const uint32_t f0 = (uint32_t)(((nb * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
@@ -1557,7 +1602,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     p->bytes = at;
     p->scores_smem = 2 * blocks * ((head_dim + 31) / 32) * 512 + (size_t)max_requests * sizeof(Meta);
     const size_t chunk = std::max<size_t>(1, kChunk / blocks);
-    p->values_smem = kRing + chunk * blocks * 1024 + kExpWords * 4 + (chunk + 1 + kWarps + 2) * blocks * 16 + (size_t)max_requests * sizeof(Meta);
+    p->values_smem = kRing + 2 * chunk * blocks * 1024 + kExpWords * 4 + (kWarps + 4) * blocks * 16 + (size_t)max_requests * sizeof(Meta);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int16_t e16[2049], p18[2049], host[kExpWords * 2] = {};
     llmx::build_exp_tables(e16, p18);
