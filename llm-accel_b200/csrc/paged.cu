@@ -89,6 +89,7 @@ struct Call {
     int2 *fsum;          // [slot][8]: P(m_before - m), the sum of P
     const int16_t *exps; // [2049] of differences 0, -1, ... -2048
     int *error;
+    int blocks;              // k_attend: column blocks of a cluster at most
     int tiles, cluster_log;  // k_attend: of a CTA at most; CTAs of a (request, key head): up to 8, a power of 2
 };
 
@@ -244,6 +245,7 @@ struct Strip {
     const int32_t *table;
     int h, rows, length, blocks;
     uint32_t row0;
+    int col0;  // first of the columns at hand (k_attend may have a part of them), `blocks` blocks of 8
 };
 // One (request, key head, tile) after another.
 struct Cursor {
@@ -293,7 +295,7 @@ struct Cursor {
     }
     // Slot of this tile in column block nb.
     __device__ int slot(int nb) const { return slot0 + nb * tiles + t; }
-    __device__ Strip strip() const { return Strip{table, h, rows, length, blocks, row0}; }
+    __device__ Strip strip() const { return Strip{table, h, rows, length, blocks, row0, 0}; }
 };
 
 static __device__ __forceinline__ void range_of(int items, int &first, int &end) {
@@ -318,10 +320,10 @@ struct Column {
 template <int KS>
 static __device__ __forceinline__ void stage_queries(const Call &c, const Strip &z, int warp, int warps, uint4 *queries, uint4 *rests, Column &column) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
-    const int columns = z.rows * c.group;
+    const int columns = z.rows * c.group - z.col0;
     for (int nb = warp; nb < z.blocks; nb += warps) {
-        const int col = nb * 8 + g, j = col / c.group;
-        const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + col - j * c.group) * c.dim + 8 * t4;
+        const int col = nb * 8 + g, j = (z.col0 + col) / c.group;
+        const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + z.col0 + col - j * c.group) * c.dim + 8 * t4;
         uint32_t big = 0;
         int sum = 0;
 #pragma unroll
@@ -422,8 +424,8 @@ static __device__ __forceinline__ uint32_t finish_scores(const Call &c, const St
             const int col = nb * 8 + 2 * t4 + (i & 1), p = p0 + g + (i >> 1) * 8;
             if (!column.wide[col] || p >= z.length) continue;
             uint32_t none = 0;
-            const int j = col / c.group;
-            const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + col - j * c.group) * c.dim;
+            const int j = (z.col0 + col) / c.group;
+            const int16_t *q = c.q + (size_t)(z.row0 + j) * c.ld_q + (size_t)(z.h * c.group + z.col0 + col - j * c.group) * c.dim;
             const int16_t *k = reinterpret_cast<const int16_t *>(rows_of(c, c.k, page_of(c, z.table, (uint32_t)p >> 3, none), (uint32_t)p >> 3, z.h) + (p & 7) * c.row_bytes);
             const int y = score_exact(q, k, c.dim, c.scale8);
             if (i == 0) sc[0] = y;
@@ -578,14 +580,15 @@ static __device__ __forceinline__ void load_octet(uint32_t at, uint32_t (&r)[4])
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 // Byte planes of a tile's 32 elements as A: [step of 32 positions][16 elements].  A lane's bytes of positions
-// are those of 8 j + 2 t4 and the next, j = 0, 1 (first words) and j = 2, 3.  Returns whether values were limited.
-static __device__ __forceinline__ bool value_planes(const unsigned char *ring, uint32_t (&vl)[2][2][4], uint32_t (&vh)[2][2][4]) {
-    const int lane = threadIdx.x & 31;
-    // octet o of a row is its unit o ^ row / 2 mod 4
-    const uint32_t row = (uint32_t)__cvta_generic_to_shared(ring) + lane * 64 + (lane >> 1 & 3) * 16;
-    bool limit = false;
-#pragma unroll 1
-    for (;;) {
+// are those of 8 j + 2 t4 and the next, j = 0, 1 (first words) and j = 2, 3.
+struct Planes {
+    uint32_t l[2][2][4], h[2][2][4];
+    // Returns whether some value is not within [-2048, 2047] (the high byte's bits 3 to 7 differ).
+    template <bool kLimit>
+    __device__ __forceinline__ bool load(const unsigned char *ring) {
+        const int lane = threadIdx.x & 31;
+        // octet o of a row is its unit o ^ row / 2 mod 4
+        const uint32_t row = (uint32_t)__cvta_generic_to_shared(ring) + lane * 64 + (lane >> 1 & 3) * 16;
         uint32_t out = 0;
 #pragma unroll
         for (int s = 0; s < 2; s++)
@@ -593,54 +596,55 @@ static __device__ __forceinline__ bool value_planes(const unsigned char *ring, u
             for (int o = 0; o < 4; o++) {
                 uint32_t r[4];
                 load_octet((row ^ (uint32_t)(o * 16)) + s * 2048, r);
-                if (limit)
+                if (kLimit)
 #pragma unroll
                     for (int i = 0; i < 4; i++) r[i] = limit2(r[i]);
-                vl[s][o >> 1][o & 1] = low4(r[0], r[1]);
-                vl[s][o >> 1][2 + (o & 1)] = low4(r[2], r[3]);
-                vh[s][o >> 1][o & 1] = high4(r[0], r[1]);
-                vh[s][o >> 1][2 + (o & 1)] = high4(r[2], r[3]);
+                l[s][o >> 1][o & 1] = low4(r[0], r[1]);
+                l[s][o >> 1][2 + (o & 1)] = low4(r[2], r[3]);
+                h[s][o >> 1][o & 1] = high4(r[0], r[1]);
+                h[s][o >> 1][2 + (o & 1)] = high4(r[2], r[3]);
+                if (!kLimit)
 #pragma unroll
-                for (int i = 0; i < 2; i++) out |= vh[s][o >> 1][2 * i + (o & 1)] ^ (vh[s][o >> 1][2 * i + (o & 1)] << 1);
+                    for (int i = 0; i < 2; i++) out |= h[s][o >> 1][2 * i + (o & 1)] ^ (h[s][o >> 1][2 * i + (o & 1)] << 1);
             }
-        // some high byte is not in [-8, 7] (its bits 3 to 7 differ): limited, once more
-        if (limit || !__any_sync(0xffffffffu, (out & 0xf0f0f0f0u) != 0)) return limit;
-        limit = true;
+        return !kLimit && __any_sync(0xffffffffu, (out & 0xf0f0f0f0u) != 0);
     }
-}
+};
+
+// Place of lane u's 16 bytes of B among 32: turned, so that the bytes of a column pair's two positions, which 16 lanes
+// store, lie in as many banks as they can.
+static __device__ __forceinline__ int place_of(int u) { return u ^ (u >> 3 << 1); }
 
 // Probabilities of 16 positions (block blk of a tile) against 8 columns, as bytes in the order of B.
 // Lane: column pair lane & 3, positions 8 r + 2 t and the next; s: their scores, biased; m: the pair's
 // maxima; prob: [2 steps][32 lanes] {low, low, high, high}.
-static __device__ __forceinline__ void probabilities(const int16_t *exps, uint32_t s0, uint32_t s1, uint32_t m, bool whole, int p, int seen0, int seen1, int blk,
+static __device__ __forceinline__ void probabilities(const int16_t *exps, uint32_t s0, uint32_t s1, uint32_t m, int p, int seen0, int seen1, int blk,
                                                      uint4 *prob) {
     const int lane = threadIdx.x & 31, cp = lane & 3, t = lane >> 2 & 3, r = lane >> 4;
     const uint32_t floor = __vmaxu2(m, 0x08000800u) - 0x08000800u;
     // differences to the maximum, 0 to 2048 (what is not seen may hold anything)
     const uint32_t d0 = m - __vminu2(__vmaxu2(s0, floor), m), d1 = m - __vminu2(__vmaxu2(s1, floor), m);
     uint32_t a0 = (uint16_t)exps[d0 & 0xffffu], b0 = (uint16_t)exps[d0 >> 16], a1 = (uint16_t)exps[d1 & 0xffffu], b1 = (uint16_t)exps[d1 >> 16];
-    if (!whole) {
-        if (p >= seen0) a0 = 0;
-        if (p >= seen1) b0 = 0;
-        if (p + 1 >= seen0) a1 = 0;
-        if (p + 1 >= seen1) b1 = 0;
-    }
+    a0 = p < seen0 ? a0 : 0;
+    b0 = p < seen1 ? b0 : 0;
+    a1 = p + 1 < seen0 ? a1 : 0;
+    b1 = p + 1 < seen1 ? b1 : 0;
     const uint32_t a = __byte_perm(a0, a1, 0x5140), b = __byte_perm(b0, b1, 0x5140);  // {low, low, high, high}
-    uint16_t *dst = reinterpret_cast<uint16_t *>(prob + (blk >> 1) * 32 + cp * 8 + t) + 2 * (blk & 1) + r;
-    dst[0] = (uint16_t)a;
-    dst[4] = (uint16_t)(a >> 16);
-    dst[32] = (uint16_t)b;
-    dst[36] = (uint16_t)(b >> 16);
+    // (place_of(cp * 8 + t), and of the next column's, 4 further)
+    const int at = cp * 8 + (t ^ 2 * cp);
+    uint16_t *dst = reinterpret_cast<uint16_t *>(prob + (blk >> 1) * 32) + 2 * (blk & 1) + r;
+    dst[8 * at] = (uint16_t)a;
+    dst[8 * at + 4] = (uint16_t)(a >> 16);
+    dst[8 * (at ^ 4)] = (uint16_t)b;
+    dst[8 * (at ^ 4) + 4] = (uint16_t)(b >> 16);
 }
 
 // A tile's values against 8 columns: y[o] is the word of column g, elements 8 o + 2 t4 and the next, of
-// the part's 32.  sum: lanes 0 to 3 get the columns' sums of P (2 t4 and 2 t4 + 1).
-static __device__ __forceinline__ void weigh(const uint32_t (&vl)[2][2][4], const uint32_t (&vh)[2][2][4], bool limit, const uint4 *prob, uint32_t (&y)[4],
-                                             bool with_sum, int (&sum)[2]) {
-    const int lane = threadIdx.x & 31;
-    const uint4 b[2] = {prob[lane], prob[32 + lane]};
-    uint4 rest[2];  // of the probabilities, for values at the upper limit
-    if (limit)
+// the part's 32.  kLimit: values were limited, and some may be at the upper limit.
+template <bool kLimit>
+static __device__ __forceinline__ void weigh(const Planes &v, const uint4 (&b)[2], uint32_t (&y)[4]) {
+    uint4 rest[2];  // of the probabilities
+    if (kLimit)
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const uint32_t r0 = rest2(__byte_perm(b[s].x, b[s].z, 0x5140)), r1 = rest2(__byte_perm(b[s].x, b[s].z, 0x7362));
@@ -651,68 +655,62 @@ static __device__ __forceinline__ void weigh(const uint32_t (&vl)[2][2][4], cons
     for (int mb = 0; mb < 2; mb++) {
         // The high products' sums become a part of the middle ones' and these of the low ones'; and rnd8 of rnd6 of
         // the sum is (sum + 2^5 + 2^13) >> 14; the sum is below 2^31 - 2^16.
-        int d[4] = {0, 0, 0, 0}, v[4];
-        mma_su(d, vh[0][mb], b[0].z, b[0].w, d);
-        mma_su(d, vh[1][mb], b[1].z, b[1].w, d);
+        int d[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int s = 0; s < 2; s++) mma_su(d, v.h[s][mb], b[s].z, b[s].w, d);
 #pragma unroll
         for (int i = 0; i < 4; i++) d[i] *= 256;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            mma_su(d, vh[s][mb], b[s].x, b[s].y, d);
-            mma_uu(d, vl[s][mb], b[s].z, b[s].w, d);
+            mma_su(d, v.h[s][mb], b[s].x, b[s].y, d);
+            mma_uu(d, v.l[s][mb], b[s].z, b[s].w, d);
         }
-        if (limit) {
+        uint32_t m[2][4];
+        if (kLimit)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                uint32_t m[4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) m[i] = at_limit(vh[s][mb][i]);
-                mma_us(d, m, rest[s].z, rest[s].w, d);
+                for (int i = 0; i < 4; i++) m[s][i] = at_limit(v.h[s][mb][i]);
+                mma_us(d, m[s], rest[s].z, rest[s].w, d);
             }
-        }
 #pragma unroll
         for (int i = 0; i < 4; i++) d[i] = (int)((uint32_t)d[i] * 256u + 8224u);
-        mma_uu(d, vl[0][mb], b[0].x, b[0].y, d);
-        mma_uu(d, vl[1][mb], b[1].x, b[1].y, d);
-        if (limit) {
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                uint32_t m[4];
+        for (int s = 0; s < 2; s++) mma_uu(d, v.l[s][mb], b[s].x, b[s].y, d);
+        if (kLimit)
 #pragma unroll
-                for (int i = 0; i < 4; i++) m[i] = at_limit(vh[s][mb][i]);
-                mma_uu(d, m, rest[s].x, rest[s].y, d);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = d[i] >> 14;
-        y[2 * mb] = transpose8(pack_sat16(v[0], v[1]));
-        y[2 * mb + 1] = transpose8(pack_sat16(v[2], v[3]));
+            for (int s = 0; s < 2; s++) mma_uu(d, m[s], rest[s].x, rest[s].y, d);
+        y[2 * mb] = transpose8(pack_sat16(d[0] >> 14, d[1] >> 14));
+        y[2 * mb + 1] = transpose8(pack_sat16(d[2] >> 14, d[3] >> 14));
     }
-    if (with_sum) {
-        const uint32_t one[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
-        int low[4] = {0, 0, 0, 0}, high[4] = {0, 0, 0, 0};
+}
+// The columns' sums of P: lanes 0 to 3 get those of 2 t4 and 2 t4 + 1.
+static __device__ __forceinline__ int2 sum_of(const uint4 (&b)[2]) {
+    const uint32_t one[4] = {0x01010101u, 0x01010101u, 0x01010101u, 0x01010101u};
+    int d[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int s = 0; s < 2; s++) {
-            mma_uu(low, one, b[s].x, b[s].y, low);
-            mma_uu(high, one, b[s].z, b[s].w, high);
-        }
-        sum[0] = low[0] + 256 * high[0];
-        sum[1] = low[1] + 256 * high[1];
-    }
+    for (int s = 0; s < 2; s++) mma_uu(d, one, b[s].z, b[s].w, d);
+    d[0] *= 256;
+    d[1] *= 256;
+#pragma unroll
+    for (int s = 0; s < 2; s++) mma_uu(d, one, b[s].x, b[s].y, d);
+    return make_int2(d[0], d[1]);
 }
 
 constexpr int kChunk = 4;  // tiles of a (request, key head) whose probabilities k_values forms at once
 
 // The warps' shares of a tile's elements: `part` of 32, and with fewer parts than warps every `step`-th tile.
 struct Share {
-    int part, first, step, octets;  // (octets of elements)
+    int part, first, step, shift, octets;  // (octets of elements)
     __device__ __forceinline__ Share(int dim, int warp) {
         const int log = dim > 64 ? 2 : dim > 32 ? 1 : 0;  // 4, 2 or 1 (of three parts the fourth warp has none)
         part = warp & ((1 << log) - 1);
         first = part * 32 < dim ? warp >> log : INT_MAX;
         step = kWarps >> log;
+        shift = 2 - log;
         octets = min((dim - part * 32) >> 3, 4);
     }
+    __device__ __forceinline__ int count(int n) const { return n > first ? (n - first + step - 1) >> shift : 0; }
 };
 
 // One CTA's run of tiles, in chunks of up to kChunk: their probabilities, by all warps, through shared
@@ -749,6 +747,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     cur.start(c, meta, first);
     bool moved = true;
     int turn = 0, buffer = 0;
+    int from = 0, into = 0, flying = 0, ahead = 0;  // the ring: next slot to use and to fill, tiles in it, of the next chunk
     // of a chunk's tiles: scores of this lane's two positions and column pair; maxima of 16 positions, 16 words of
     // two tiles a load
     uint32_t score[kChunk][2], top[kChunk / 2];
@@ -769,16 +768,16 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     for (int item = first; item < end;) {
         const Strip z = cur.strip();
         const int n = length_of(item), t0 = cur.t, slot0 = cur.slot(0), tiles = cur.tiles;
-        int fetched = share.first;
-        auto fetch = [&](int slot) {
-            if (fetched < n) {
-                fetch_values(c, z, t0 + fetched, share.part, ring + slot * kSlice, worst);
-                fetched += share.step;
-            }
+        // tiles of this chunk that are this warp's; those that the last chunk's loop has fetched already
+        const int mine = share.count(n);
+        int fetched = ahead;
+        auto fetch = [&](const Strip &of, int t) {
+            fetch_values(c, of, t, share.part, ring + into * kSlice, worst);
             commit();
+            into ^= 1;
+            flying++;
         };
-#pragma unroll
-        for (int i = 0; i < kDepth; i++) fetch(i);
+        for (; flying < kDepth && fetched < mine; fetched++) fetch(z, t0 + share.first + fetched * share.step);
         if (moved) {  // the maxima of the tiles before, by every warp for itself
             turn ^= 1;
             for (int nb = 0; nb < z.blocks; nb++) {
@@ -804,7 +803,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
         }
         uint4 *pb = prob + (buffer ? chunk * most * 64 : 0);
         buffer ^= 1;
-        const int whole = z.length - z.rows + 1;  // positions that every row sees
         for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
             const int slot = slot0 + nb * tiles;
             if constexpr (!kOne) load_scores(slot, n);
@@ -820,14 +818,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
             }
             uint32_t was = before[nb * 4 + cp];
             const int seen0 = seen[turn * most * 8 + nb * 8 + 2 * cp], seen1 = seen[turn * most * 8 + nb * 8 + 2 * cp + 1];
-            const bool full = nb * 8 + 8 <= z.rows * c.group;
 #pragma unroll
             for (int k = 0; k < kChunk; k++)
-                if (k < n) {
-                    const int p = (t0 + k) * kTile;
+                if (kOne || k < n) {  // (the last tile again behind it)
+                    const int p = (t0 + min(k, n - 1)) * kTile;
                     m[k] = __vmaxu2(m[k], was);
-                    probabilities(exps, score[k][0], score[k][1], m[k], full && p + kTile <= whole, p + pos, seen0, seen1, warp, pb + (k * most + nb) * 64);
-                    if (warp == 0 && lane < 4) {
+                    probabilities(exps, score[k][0], score[k][1], m[k], p + pos, seen0, seen1, warp, pb + (k * most + nb) * 64);
+                    if (warp == 0 && lane < 4 && k < n) {
                         const uint32_t d = m[k] - __vmaxu2(was, __vmaxu2(m[k], 0x08000800u) - 0x08000800u);
                         int2 *f = c.fsum + (size_t)(slot + k) * 8 + 2 * lane;
                         f[0].x = exps[d & 0xffffu];
@@ -840,37 +837,49 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
             __syncwarp();
         }
         item += n;
+        int coming = 0;  // tiles of the next chunk that are this warp's
+        ahead = 0;
         if (item < end) {
             cur.t += n - 1;
             moved = cur.next(c, meta);
             if constexpr (kOne) load_scores(cur.slot(0), length_of(item));  // on their way while the values are weighed
+            coming = share.count(length_of(item));
         }
+        const Strip zn = cur.strip();
         __syncthreads();
 #pragma unroll 1
-        for (int k = share.first, i = 0; k < n; k += share.step, i ^= 1) {
-            asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+        for (int k = share.first; k < n; k += share.step) {
+            if (flying == kDepth) asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+            else asm volatile("cp.async.wait_group 0;" ::: "memory");
             __syncwarp();
-            uint32_t vl[2][2][4], vh[2][2][4];
-            const bool limit = value_planes(ring + i * kSlice, vl, vh);
+            Planes v;
+            const bool limit = v.load<false>(ring + from * kSlice);
+            if (limit) v.load<true>(ring + from * kSlice);
+            from ^= 1;
+            flying--;
             __syncwarp();
-            fetch(i);
+            if (fetched < mine) fetch(z, t0 + share.first + fetched++ * share.step);
+            else if (ahead < coming) fetch(zn, cur.t + share.first + ahead++ * share.step);
             for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+                const uint4 *p = pb + (k * most + nb) * 64 + place_of(lane), b2[2] = {p[0], p[32]};
                 uint32_t y[4];
-                int sum[2];
-                weigh(vl, vh, limit, pb + (k * most + nb) * 64, y, share.part == 0, sum);
+                if (limit) weigh<true>(v, b2, y);
+                else weigh<false>(v, b2, y);
                 const size_t slot = (size_t)(slot0 + nb * tiles + k);
                 uint32_t *dst = reinterpret_cast<uint32_t *>(c.tv + (slot * 8 + g) * c.dim + share.part * 32 + 2 * t4);
 #pragma unroll
                 for (int o = 0; o < 4; o++)
                     if (o < share.octets) dst[4 * o] = y[o];
-                if (share.part == 0 && lane < 4) {
-                    int2 *f = c.fsum + slot * 8 + 2 * lane;
-                    f[0].y = sum[0];
-                    f[1].y = sum[1];
+                if (share.part == 0) {
+                    const int2 sum = sum_of(b2);
+                    int2 *f = c.fsum + slot * 8 + 2 * t4;
+                    if (g == 0) {
+                        f[0].y = sum.x;
+                        f[1].y = sum.y;
+                    }
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     report(c, worst);
 }
@@ -881,17 +890,17 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
 static __device__ __forceinline__ uint32_t request_of(const uint32_t *offsets, uint32_t requests, uint32_t r) {
     const uint32_t lane = threadIdx.x & 31, step = (requests + 31) / 32;
     uint32_t at = lane * step;
-    uint32_t before = __ballot_sync(0xffffffffu, at < requests && offsets[at] <= r);
+    uint32_t before = __ballot_sync(0xffffffffu, at < requests && __ldcg(offsets + min(at, requests - 1)) <= r);
     const uint32_t block = before ? (31 - __clz(before)) * step : 0;
     if (step == 1) return block;
     at = block + lane;
-    before = __ballot_sync(0xffffffffu, lane < step && at < requests && offsets[at] <= r);
+    before = __ballot_sync(0xffffffffu, lane < step && at < requests && __ldcg(offsets + min(at, requests - 1)) <= r);
     return before ? block + 31 - __clz(before) : block;
 }
 
 constexpr int kShortTiles = 255;  // tiles whose sums stay below 2^31: of values 2^23 each, of probabilities 2^22
 constexpr int kMaxStretches = 3;  // per warp
-constexpr int kAhead = 8;         // tiles loaded at once
+constexpr int kAhead = 16;        // tiles loaded at once
 constexpr int kMaxJoinWarps = 16;
 
 // x times a factor f < 1 (Q2.14), rounded
@@ -914,26 +923,34 @@ static __device__ __forceinline__ uint2 quotient(const int (&x)[4], int sum) {
     return make_uint2(pack_sat16(one(x[0]), one(x[1])), pack_sat16(one(x[2]), one(x[3])));
 }
 
-// What tiles without a factor do to a row's four elements: their sums, and (of a long text) the least and
-// the largest value, from which it is seen that nothing on the way saturates.
+// What tiles without a factor, but for the first one's, do to a row's four elements: their sums, and (of a
+// long text) how far from what comes in they can get on the way, by the least and the largest value.
 struct Stretch {
     int s[4];
-    uint32_t lo, hi;  // of pairs of elements
-    int start, tiles, psum;
-    __device__ void clear(int t) {
+    uint32_t lo, hi;  // of pairs of elements; once closed, the furthest down and up
+    int factor, start, tiles, psum;
+    template <bool kLong>
+    __device__ __forceinline__ void close(int end, int p) {
+        tiles = end - start;
+        psum += p;
+        if constexpr (kLong) {
+            lo = (uint32_t)(int)max(256ll * tiles * min(llmx::lo16(lo), llmx::hi16(lo)), (long long)INT_MIN);
+            hi = (uint32_t)(int)min(256ll * tiles * max(llmx::lo16(hi), llmx::hi16(hi)), (long long)INT_MAX);
+        }
+    }
+    __device__ __forceinline__ void clear(int f, int t) {
         s[0] = s[1] = s[2] = s[3] = 0;
         lo = hi = 0;
+        factor = f;
         start = t;
-        tiles = psum = 0;
+        psum = 0;
     }
     template <bool kLong>
-    __device__ void add(uint2 v, int p) {
+    __device__ __forceinline__ void add(uint2 v) {
         s[0] = add_low(v.x, s[0]);
         s[1] = add_high(v.x, s[1]);
         s[2] = add_low(v.y, s[2]);
         s[3] = add_high(v.y, s[3]);
-        psum += p;
-        tiles++;
         if constexpr (kLong) {
             lo = __vmins2(lo, __vmins2(v.x, v.y));
             hi = __vmaxs2(hi, __vmaxs2(v.x, v.y));
@@ -943,23 +960,26 @@ struct Stretch {
 
 // One query head's row per CTA.  A lane has four elements, a warp an equal part of the tiles.  Between
 // tiles that raise the maximum (whose factor is not 1: few in a long text) the recurrence only adds,
-// so a warp gives what its tiles do to any value that comes in as a few stretches (a factor, then
-// sums), and the first warp, which starts from 0, puts them together; tiles beyond a warp's
-// kMaxStretches, and a stretch on which something might saturate, it goes through itself, one by one.
+// so a warp gives what its tiles do to any value that comes in as a few stretches, and the first
+// warp, which starts from 0, puts them together; tiles beyond a warp's kMaxStretches it goes
+// through itself, and a stretch on which something might saturate tile by tile.
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
-    __shared__ int factors[kMaxJoinWarps][kMaxStretches], counts[kMaxJoinWarps], rest[kMaxJoinWarps];
+    __shared__ int counts[kMaxJoinWarps], rest[kMaxJoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = (int)blockDim.x >> 5;
     const int quads = c.dim >> 2;
     Stretch *stretches = reinterpret_cast<Stretch *>(dynamic);  // [warps - 1][kMaxStretches][32]
-    pdl_wait();
-    pdl_trigger();
+    // This launch starts once every CTA of k_values has waited for k_scores, so that what came before k_scores'
+    // end (the requests, and what k_scores made of them) can be read, through the L2, before its own wait.
     const uint32_t row = blockIdx.x / c.heads;
     const int head = (int)(blockIdx.x - row * c.heads);
     const uint32_t b = request_of(c.offsets, c.requests, row);
-    const uint32_t begin = c.offsets[b], behind = c.offsets[b + 1];
-    const Meta m = c.meta[b];
+    const uint32_t begin = __ldcg(c.offsets + b), behind = __ldcg(c.offsets + b + 1);
+    const int4 m4 = __ldcg(reinterpret_cast<const int4 *>(c.meta + b));
+    const Meta m{m4.x, m4.y, m4.z, m4.w};
+    pdl_wait();
+    pdl_trigger();
     if (row < begin || row >= behind || m.rows < 0) return;  // of no request, or of a void one
     const int h = head / c.group, col = (int)(row - begin) * c.group + head - h * c.group;
     const int blocks = (m.rows * c.group + 7) / 8;
@@ -967,76 +987,29 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     const uint2 *tv = reinterpret_cast<const uint2 *>(c.tv + at * c.dim) + min(lane, quads - 1);
     const int2 *fsum = c.fsum + at;
     const uint32_t step = 8 * quads;  // from a tile to the next
-    auto begin_of = [&](int w) { return (int)((long long)m.tiles * w / warps); };
+    auto begin_of = [&](int w) { return m.tiles * w / warps; };
 
     int sum = 0, x[4] = {0, 0, 0, 0};
-    uint2 v[kAhead];
-    int2 f[kAhead];
-    auto load = [&](int t0, int t1) {  // what lies behind t1 changes nothing
-        if (t0 + kAhead <= t1) {
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                v[i] = tv[(size_t)(t0 + i) * step];
-                f[i] = fsum[(t0 + i) * 8];
-            }
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) {
-            v[i] = make_uint2(0, 0);
-            f[i] = make_int2(16384, 0);
-            if (t0 + i < t1) {
-                v[i] = tv[(size_t)(t0 + i) * step];
-                f[i] = fsum[(t0 + i) * 8];
-            }
-        }
-    };
-    auto plain = [&]() {  // no factor among them (factors are at most 16384: one below has no bit 14)
-        int all = 16384;
-#pragma unroll
-        for (int i = 0; i < kAhead; i++) all &= f[i].x;
-        return __shfl_sync(0xffffffffu, all, 0) == 16384;
-    };
-    auto factor = [&](int by) {  // a factor of 1 leaves everything as it is
-        if (by == 16384) return;
-        sum = times(sum, by);
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = times(x[k], by);
-    };
-    auto one = [&](uint2 w, int p) {  // a tile on top of (sum, x)
-        if constexpr (kLong) {
-            sum = llmx::add_sat(sum, 4 * p);
-            x[0] = llmx::add_sat(x[0], llmx::lo16(w.x) * 256);
-            x[1] = llmx::add_sat(x[1], llmx::hi16(w.x) * 256);
-            x[2] = llmx::add_sat(x[2], llmx::lo16(w.y) * 256);
-            x[3] = llmx::add_sat(x[3], llmx::hi16(w.y) * 256);
-        } else {
-            sum += 4 * p;
-            x[0] += llmx::lo16(w.x) * 256;
-            x[1] += llmx::hi16(w.x) * 256;
-            x[2] += llmx::lo16(w.y) * 256;
-            x[3] += llmx::hi16(w.y) * 256;
-        }
-    };
-    auto replay = [&](int t0, int t1) {  // tiles t0 .. t1 - 1 on top of (sum, x), one by one
-#pragma unroll 1
-        for (; t0 < t1; t0 += kAhead) {
-            load(t0, t1);
-#pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                factor(f[i].x);
-                one(v[i], f[i].y);
-            }
-        }
-    };
     auto apply = [&](const Stretch &p) {
+        if (p.factor != 16384) {  // a factor of 1 leaves everything as it is
+            sum = times(sum, p.factor);
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = times(x[k], p.factor);
+        }
         if constexpr (kLong) {
-            // the furthest that any of its sums can be from what comes in
-            const long long up = 256ll * p.tiles * max(llmx::lo16(p.hi), llmx::hi16(p.hi)), down = 256ll * p.tiles * min(llmx::lo16(p.lo), llmx::hi16(p.lo));
-            const bool far = max(max(x[0], x[1]), max(x[2], x[3])) + up > INT_MAX || min(min(x[0], x[1]), min(x[2], x[3])) + down < INT_MIN ||
-                             sum + 4ll * p.psum > INT_MAX;
+            // (hi is at least 0, lo at most 0)
+            const bool far = max(max(x[0], x[1]), max(x[2], x[3])) > INT_MAX - (int)p.hi || min(min(x[0], x[1]), min(x[2], x[3])) < INT_MIN - (int)p.lo ||
+                             sum > INT_MAX - 4 * p.psum;
             if (__any_sync(0xffffffffu, far)) {
-                replay(p.start, p.start + p.tiles);  // (their factors, but for the first one, which is used, are 1)
+#pragma unroll 1
+                for (int t = p.start; t < p.start + p.tiles; t++) {
+                    const uint2 v = tv[(size_t)t * step];
+                    sum = llmx::add_sat(sum, 4 * fsum[t * 8].y);
+                    x[0] = llmx::add_sat(x[0], llmx::lo16(v.x) * 256);
+                    x[1] = llmx::add_sat(x[1], llmx::hi16(v.x) * 256);
+                    x[2] = llmx::add_sat(x[2], llmx::lo16(v.y) * 256);
+                    x[3] = llmx::add_sat(x[3], llmx::hi16(v.y) * 256);
+                }
                 return;
             }
         }
@@ -1044,81 +1017,74 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = (int)((uint32_t)x[k] + 256u * (uint32_t)p.s[k]);
     };
-    if (warp == 0) {
-        const int end = begin_of(1);
+    // Tiles t0 .. t1 - 1 as stretches, which are applied or kept in mine[]; returns where the place for them ran out.
+    auto walk = [&](int t0, int t1, bool use, Stretch *mine, int &count) {
+        Stretch p;
+        bool open = false;
+        for (int w0 = t0; w0 < t1; w0 += 32) {
+            const int n = min(32, t1 - w0);
+            const int2 f = lane < n ? fsum[(w0 + lane) * 8] : make_int2(16384, 0);
+            uint32_t turns = __ballot_sync(0xffffffffu, f.x != 16384);
+            if (!open) {
+                p.clear(__shfl_sync(0xffffffffu, f.x, 0), w0);
+                turns &= ~1u;
+                open = true;
+            }
+            int from = 0;  // of this window's tiles, the first whose P is not in the stretch
+            uint2 v[kAhead];
 #pragma unroll 1
-        for (int t0 = 0; t0 < end; t0 += kAhead) {
-            load(t0, end);
-            if (plain()) {
-                Stretch p;
-                p.clear(t0);
-#pragma unroll
-                for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i], f[i].y);
-                p.tiles = min(kAhead, end - t0);
-                apply(p);
-            } else {
+            for (int b0 = 0; b0 < n; b0 += kAhead) {
 #pragma unroll
                 for (int i = 0; i < kAhead; i++) {
-                    factor(f[i].x);
-                    one(v[i], f[i].y);
+                    v[i] = make_uint2(0, 0);
+                    if (b0 + i < n) v[i] = tv[(size_t)(w0 + b0 + i) * step];
                 }
-            }
-        }
-    } else {
-        const int first = begin_of(warp), end = begin_of(warp + 1);
-        Stretch p;
-        p.clear(first);
-        int f0 = 16384, count = 0, left = end;
-        Stretch *mine = stretches + (warp - 1) * kMaxStretches * 32 + lane;
-        auto close = [&]() {
-            mine[count * 32] = p;
-            if (lane == 0) factors[warp][count] = f0;
-            count++;
-        };
-#pragma unroll 1
-        for (int t0 = first; t0 < end && left == end; t0 += kAhead) {
-            load(t0, end);
-            if (plain()) {
+                if ((turns >> b0 & ((1u << kAhead) - 1)) == 0) {
 #pragma unroll
-                for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i], f[i].y);
-                continue;
-            }
+                    for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i]);
+                    continue;
+                }
 #pragma unroll
-            for (int i = 0; i < kAhead; i++) {
-                if (left != end || t0 + i >= end) continue;
-                if (f[i].x != 16384) {
-                    if (t0 + i > first) {  // the stretch ends here
-                        if (count + 1 == kMaxStretches) {
-                            left = t0 + i;
-                            continue;
+                for (int i = 0; i < kAhead; i++) {
+                    const int t = b0 + i;
+                    if (turns >> t & 1u) {  // the stretch ends here
+                        if (!use && count + 1 == kMaxStretches) {
+                            p.close<kLong>(w0 + t, __reduce_add_sync(0xffffffffu, lane >= from && lane < t ? f.y : 0));
+                            mine[count++ * 32] = p;
+                            return w0 + t;
                         }
-                        close();
-                        p.clear(t0 + i);
+                        p.close<kLong>(w0 + t, __reduce_add_sync(0xffffffffu, lane >= from && lane < t ? f.y : 0));
+                        from = t;
+                        if (use) apply(p);
+                        else mine[count++ * 32] = p;
+                        p.clear(__shfl_sync(0xffffffffu, f.x, t), w0 + t);
                     }
-                    f0 = f[i].x;
+                    p.add<kLong>(v[i]);
                 }
-                p.add<kLong>(v[i], f[i].y);
             }
+            p.psum += __reduce_add_sync(0xffffffffu, lane >= from ? f.y : 0);
         }
-        // (of the last stretch, places behind the end may have been counted)
-        p.tiles = min(p.tiles, left - p.start);
-        if (first < end) close();
+        if (open) {
+            p.close<kLong>(t1, 0);
+            if (use) apply(p);
+            else mine[count++ * 32] = p;
+        }
+        return t1;
+    };
+    int count = 0;
+    const int left = walk(begin_of(warp), begin_of(warp + 1), warp == 0, stretches + (warp - 1) * kMaxStretches * 32 + lane, count);
+    if (warps > 1) {
         if (lane == 0) {
             counts[warp] = count;
             rest[warp] = left;
         }
-    }
-    if (warps > 1) {
         __syncthreads();
         if (warp != 0) return;
 #pragma unroll 1
         for (int w = 1; w < warps; w++) {
 #pragma unroll 1
-            for (int k = 0; k < counts[w]; k++) {
-                factor(factors[w][k]);
-                apply(stretches[((w - 1) * kMaxStretches + k) * 32 + lane]);
-            }
-            replay(rest[w], begin_of(w + 1));
+            for (int k = 0; k < counts[w]; k++) apply(stretches[((w - 1) * kMaxStretches + k) * 32 + lane]);
+            if (rest[w] < begin_of(w + 1)) walk(rest[w], begin_of(w + 1), true, nullptr, count);
         }
     }
     if (lane < quads) *reinterpret_cast<uint2 *>(c.out + (size_t)row * c.ld_out + (size_t)head * c.dim + 4 * lane) = quotient(x, sum);
@@ -1152,8 +1118,6 @@ struct Places {  // in dynamic shared memory, in bytes
         size = at;
     }
 };
-constexpr int kAttendBlocks = 8;  // column blocks that k_attend takes: their queries fit the ring
-
 static __device__ __forceinline__ void put(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 static __device__ __forceinline__ void cluster_meet() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -1164,7 +1128,7 @@ template <int KS, bool kOne>
 __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
-    const int most = kOne ? 1 : (c.max_block * c.group + 7) / 8;
+    const int most = kOne ? 1 : c.blocks;
     const int log = c.cluster_log, cluster = 1 << log;
     const Places at(c.tiles, cluster, most, c.dim);
     unsigned char *ring = dynamic + warp * kDepth * kSlice;
@@ -1182,17 +1146,18 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     pdl_trigger();
     __shared__ int all_tiles[kWarps];
     const int strip = (int)(blockIdx.x >> log), rank = (int)(blockIdx.x & (unsigned)(cluster - 1));
-    const int b = strip / c.kv, h = strip - b * c.kv;
+    const int b = strip / c.kv, h = strip - b * c.kv, nb0 = (int)blockIdx.y * most;
     const uint32_t o0 = c.offsets[b], o1 = c.offsets[b + 1], len = c.lengths[b];
     if (o0 > o1 || o1 > c.rows || o1 - o0 > (uint32_t)c.max_block || len > c.longest) {
         if (threadIdx.x == 0) atomicOr(c.error, kErrRequest);
         return;  // (the whole cluster)
     }
-    if (o0 == o1) return;
+    const int rows = (int)(o1 - o0), columns = min(rows * c.group - nb0 * 8, most * 8);
+    if (columns <= 0) return;
     llmx::cluster_arrive();
-    const Strip z{c.table + (size_t)b * c.ld_table, h, (int)(o1 - o0), (int)len, ((int)(o1 - o0) * c.group + 7) >> 3, o0};
+    const Strip z{c.table + (size_t)b * c.ld_table, h, rows, (int)len, (columns + 7) >> 3, o0, nb0 * 8};
     const int n = (z.length + kTile - 1) / kTile, t0 = n * rank >> log, own = (n * (rank + 1) >> log) - t0;
-    const int columns = z.rows * c.group, pairs = z.blocks * 4;
+    const int pairs = z.blocks * 4;
     uint32_t worst = 0;
 
     // ---- scores
@@ -1284,11 +1249,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
                        m = __vmaxu2(before, runs[(k + 1) * most * 4 + block * 4 + cp]);
         const int2 seen = *reinterpret_cast<const int2 *>(&column.seen[col]);
         const int p = (t0 + k) * kTile;
-        const bool whole = block * 8 + 8 <= columns && p + kTile <= z.length - z.rows + 1;
         __syncwarp();
 #pragma unroll
         for (int blk = 0; blk < 4; blk++)
-            probabilities(exps, w[blk][0], w[blk][1], m, whole, p + pos + 16 * blk, seen.x, seen.y, blk, reinterpret_cast<uint4 *>(here));
+            probabilities(exps, w[blk][0], w[blk][1], m, p + pos + 16 * blk, seen.x, seen.y, blk, reinterpret_cast<uint4 *>(here));
         if (lane < 4) {
             const uint32_t d = m - __vmaxu2(was, __vmaxu2(m, 0x08000800u) - 0x08000800u);
             const uint32_t f0 = (uint32_t)(((block * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
@@ -1305,25 +1269,28 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     for (int k = share.first, i = 0; k < own; k += share.step, i ^= 1) {
         asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
         __syncwarp();
-        uint32_t vl[2][2][4], vh[2][2][4];
-        const bool limit = value_planes(ring + i * kSlice, vl, vh);
+        Planes v;
+        const bool limit = v.load<false>(ring + i * kSlice);
+        if (limit) v.load<true>(ring + i * kSlice);
         __syncwarp();
         fetch(i);
         for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
+            const uint4 *p = reinterpret_cast<const uint4 *>(score) + (k * most + nb) * 64 + place_of(lane), b2[2] = {p[0], p[32]};
             uint32_t y[4];
-            int sum[2];
-            weigh(vl, vh, limit, reinterpret_cast<const uint4 *>(score) + (k * most + nb) * 64, y, share.part == 0, sum);
+            if (limit) weigh<true>(v, b2, y);
+            else weigh<false>(v, b2, y);
             if (nb * 8 + g < columns) {
                 const uint32_t to = values + (uint32_t)(((nb * of_block + (g >> log)) * stride + t0 + k) * 2 * c.dim);
 #pragma unroll
                 for (int o = 0; o < 4; o++)
                     if (o < share.octets) put(to + 16 * o, y[o]);
             }
-            if (share.part == 0 && lane < 4) {
+            if (share.part == 0) {
+                const int2 sum = sum_of(b2);
                 const uint32_t f0 = (uint32_t)(((nb * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
                 const uint32_t f1 = (uint32_t)(((nb * of_block + (2 * cp + 1 >> log)) * stride + t0 + k) * 8);
-                if (nb * 8 + 2 * cp < columns) put(factor0 + f0 + 4, (uint32_t)sum[0]);
-                if (nb * 8 + 2 * cp + 1 < columns) put(factor1 + f1 + 4, (uint32_t)sum[1]);
+                if (g == 0 && nb * 8 + 2 * cp < columns) put(factor0 + f0 + 4, (uint32_t)sum.x);
+                if (g == 0 && nb * 8 + 2 * cp + 1 < columns) put(factor1 + f1 + 4, (uint32_t)sum.y);
             }
         }
     }
@@ -1333,7 +1300,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     long long total = 0;
     for (int w = 0; w < kWarps; w++) total += all_tiles[w];
     if (total * c.kv > c.capacity) {
-        if (blockIdx.x == 0 && threadIdx.x == 0) atomicOr(c.error, kErrBudget);
+        if (threadIdx.x == 0) atomicOr(c.error, kErrBudget);
         return;
     }
     // ---- join: a column a warp, four elements a lane (too few tiles for anything to saturate)
@@ -1359,7 +1326,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
             x[2] += llmx::lo16(w.y) * 256;
             x[3] += llmx::hi16(w.y) * 256;
         }
-        const int j = col / c.group, head = h * c.group + col - j * c.group;
+        const int j = (z.col0 + col) / c.group, head = h * c.group + z.col0 + col - j * c.group;
         if (lane < quads) *reinterpret_cast<uint2 *>(c.out + (size_t)(z.row0 + j) * c.ld_out + (size_t)head * c.dim + 4 * lane) = quotient(x, sum);
     }
 }
@@ -1503,11 +1470,12 @@ const void *scores_kernel(int dim, bool one) {
 const void *values_kernel(bool one) { return one ? (const void *)k_values<true> : (const void *)k_values<false>; }
 
 template <class T>
-cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, const T &call, cudaStream_t s, int cluster = 0) {
+cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, const T &call, cudaStream_t s, int cluster = 0,
+                   unsigned grid_y = 1) {
     T copy = call;
     void *args[] = {&copy};
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = dim3(grid, grid_y);
     cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -1611,7 +1579,8 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     if ((e = cudaDeviceGetAttribute(&p->sms, cudaDevAttrMultiProcessorCount, device)) != cudaSuccess ||
         (e = cudaFuncSetAttribute(scores_kernel(p->dim, p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaFuncSetAttribute(values_kernel(p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
-        (e = cudaFuncSetAttribute(attend_kernel(p->dim, p->one), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(attend_kernel(p->dim, true), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
+        (e = cudaFuncSetAttribute(attend_kernel(p->dim, false), cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaFuncSetAttribute((const void *)k_join<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaFuncSetAttribute((const void *)k_join<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem)) != cudaSuccess ||
         (e = cudaMalloc(reinterpret_cast<void **>(&p->memory), at)) != cudaSuccess ||
@@ -1748,15 +1717,31 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.exps = p->exps;
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // All at once where the clusters, of 8 CTAs, fit the device together; with room left, a request's column blocks
+    // are shared out over several clusters.
     const int all = (int)((longest + kTile - 1) / kTile), most = (c.max_block * c.group + 7) / 8;
+    const uint64_t clusters = (uint64_t)requests * p->kv;
     static const int force = getenv("LLMX_C") ? atoi(getenv("LLMX_C")) : -1;
-    if (force > 0 && most <= kAttendBlocks && all <= 255) {
-        while (1 << c.cluster_log < force) c.cluster_log++;
+    static const int fg = getenv("LLMX_G") ? atoi(getenv("LLMX_G")) : 0;
+    if (force != 0) {
+        c.cluster_log = 3;
+        while (c.cluster_log > 0 && (force > 0 ? 1 << c.cluster_log > force : 1 << c.cluster_log > all)) c.cluster_log--;
         const int cluster = 1 << c.cluster_log;
         c.tiles = (all + cluster - 1) / cluster;
-        const Places at(c.tiles, cluster, most, c.dim);
-        if (at.size <= kMaxSmem) {
-            const cudaError_t e = launch(attend_kernel(p->dim, p->one), requests * (unsigned)(p->kv * cluster), kThreads, (size_t)at.size, c, s, cluster);
+        int best = 0;
+        for (int groups = 1; groups <= most; groups++) {
+            const int blocks = (most + groups - 1) / groups;
+            if (fg ? groups != fg : (groups > 1 && (most + blocks - 1) / blocks != groups)) continue;
+            const Places at(c.tiles, cluster, blocks, c.dim);
+            if (at.size > kMaxSmem || all > kShortTiles) continue;
+            const uint64_t room = (uint64_t)p->sms * std::min<uint64_t>(4, (227 * 1024) / (at.size + 2048));
+            if (force > 0 || clusters * cluster * groups <= (groups > 1 ? 2 : 1) * room) best = blocks;
+        }
+        if (best) {
+            c.blocks = best;
+            const Places at(c.tiles, cluster, best, c.dim);
+            const cudaError_t e = launch(attend_kernel(p->dim, best == 1), (unsigned)(clusters * cluster), kThreads, (size_t)at.size, c, s, cluster,
+                                         (unsigned)((most + best - 1) / best));
             return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
         }
     }
