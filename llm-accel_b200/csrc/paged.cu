@@ -28,7 +28,7 @@
 
 #include <algorithm>
 #include <climits>
-#include <cstdlib>
+#include <cmath>
 #include <cstdint>
 #include <new>
 #include <string>
@@ -53,6 +53,7 @@ using llmx::sat32;
 constexpr uint32_t kMaxRequests = 1024, kMaxHeads = 1024, kMaxLength = 1u << 20, kMaxColumns = 128, kMaxPageLen = 65536;
 constexpr uint32_t kMaxAppendRows = 1u << 20;
 constexpr int kThreads = 128, kWarps = kThreads / 32;
+constexpr int kSmemOfSm = 227 * 1024;
 constexpr int kMaxSmem = 160 * 1024;  // what any call of k_scores, k_values or k_join asks for
 constexpr int kErrRequest = 1;    // offsets or length of a request out of range
 constexpr int kErrPage = 2;       // a page number out of range
@@ -727,7 +728,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     uint32_t *exps_w = reinterpret_cast<uint32_t *>(prob + 2 * chunk * most * 64);
     const int16_t *exps = reinterpret_cast<const int16_t *>(exps_w);
     uint32_t *before = exps_w + kExpWords + warp * most * 4;  // the warp's own: maxima of column pairs up to the chunk
-    int *seen = reinterpret_cast<int *>(exps_w + kExpWords + kWarps * most * 4);  // [2][most * 8]
+    uint32_t *tops_of = exps_w + kExpWords + kWarps * most * 4;                  // [2][kWarps][most * 4]
+    int *seen = reinterpret_cast<int *>(tops_of + 2 * kWarps * most * 4);         // [2][most * 8]
     Meta *meta = reinterpret_cast<Meta *>(seen + 2 * most * 8);
     for (int i = threadIdx.x; i < kExpWords; i += kThreads) exps_w[i] = reinterpret_cast<const uint32_t *>(c.exps)[i];
     pdl_wait();
@@ -778,12 +780,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
             flying++;
         };
         for (; flying < kDepth && fetched < mine; fetched++) fetch(z, t0 + share.first + fetched * share.step);
-        if (moved) {  // the maxima of the tiles before, by every warp for itself
+        if (moved) {  // the maxima of the tiles before
             turn ^= 1;
             for (int nb = 0; nb < z.blocks; nb++) {
                 const uint4 *tops = c.top + (size_t)(slot0 + nb * tiles - t0) * 4;
                 uint4 m = make_uint4(0, 0, 0, 0);
-                for (int i = lane; i < t0 * 4; i += 32) {
+#pragma unroll 4
+                for (int i = threadIdx.x; i < t0 * 4; i += kThreads) {
                     const uint4 w = tops[i];
                     m = make_uint4(__vmaxu2(m.x, w.x), __vmaxu2(m.y, w.y), __vmaxu2(m.z, w.z), __vmaxu2(m.w, w.w));
                 }
@@ -794,12 +797,19 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
                     m.z = __vmaxu2(m.z, __shfl_xor_sync(0xffffffffu, m.z, o));
                     m.w = __vmaxu2(m.w, __shfl_xor_sync(0xffffffffu, m.w, o));
                 }
-                if (lane == 0) *reinterpret_cast<uint4 *>(before + nb * 4) = m;
+                if (lane == 0) *reinterpret_cast<uint4 *>(tops_of + (turn * kWarps + warp) * most * 4 + nb * 4) = m;
             }
             // (two buffers: warps may still be at the last one's)
             for (int col = threadIdx.x; col < z.blocks * 8; col += kThreads)
                 seen[turn * most * 8 + col] = col < z.rows * c.group ? z.length - z.rows + 1 + col / c.group : 0;
             __syncthreads();
+            for (int i = lane; i < z.blocks * 4; i += 32) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int w = 0; w < kWarps; w++) m = __vmaxu2(m, tops_of[(turn * kWarps + w) * most * 4 + i]);
+                before[i] = m;
+            }
+            __syncwarp();
         }
         uint4 *pb = prob + (buffer ? chunk * most * 64 : 0);
         buffer ^= 1;
@@ -1490,6 +1500,45 @@ cudaError_t launch(const void *fn, unsigned grid, int threads, size_t smem, cons
     return cudaLaunchKernelExC(&cfg, fn, args);
 }
 
+// How k_attend takes a call, or ctas = 0 where the three launches are faster.
+struct Clusters {
+    uint64_t ctas = 0;
+    int log = 0, tiles = 0, blocks = 0, smem = 0;
+};
+// Microseconds as measured (16 query heads, 2 key heads of 128; 1 to 64 requests of 64 to 16000 positions): a
+// cluster's turn takes 5.3 and 1.5 per tile of a CTA, more by 0.34 of it for each further column block and
+// by 0.6 of it for each CTA an SM has (0.9 with several blocks); the three launches 11.5, 1.1 per further block and 1.15 per
+// tile an SM has (more by 0.5 of it per further block).  Requests are taken to be 0.6 as long as the
+// longest, on average.  64 x 1024: 23.7 by clusters of 4, 31.4 of 8, 27.5 by three launches; one of
+// 2048: 11.4 and 12.3, of 4096 17.7 and 14.5; 64 x 2048 50.5 and 45.0.
+Clusters choose(const llmx_paged *p, uint64_t strips, int all, int most) {
+    constexpr double kLoad = 0.6;
+    Clusters best;
+    double least = 11.5 + 1.1 * (most - 1) + 1.15 * kLoad * (double)strips * all / p->sms * (1 + 0.5 * (most - 1));
+    if (all > kShortTiles) return best;
+    for (int log = 0; log <= 3; log++) {
+        const int cluster = 1 << log, tiles = (all + cluster - 1) / cluster;
+        if (log && cluster > all) break;
+        for (int blocks = 1; blocks <= most; blocks++) {
+            const int groups = (most + blocks - 1) / blocks;
+            if (blocks > 1 && (most + blocks - 2) / (blocks - 1) == groups) continue;  // no fewer groups for more blocks
+            const Places at(tiles, cluster, blocks, p->dim);
+            if (at.size > kMaxSmem) continue;
+            const double ctas = kLoad * (double)strips * cluster * groups, room = (double)p->sms * std::min(4, kSmemOfSm / (at.size + 2048));
+            const double us = 5.3 * std::ceil(ctas / room) + 1.5 * tiles * (1 + 0.34 * (blocks - 1)) * (1 + (blocks > 1 ? 0.9 : 0.6) * ctas / p->sms);
+            if (us < least) {
+                least = us;
+                best.ctas = strips * cluster;
+                best.log = log;
+                best.tiles = tiles;
+                best.blocks = blocks;
+                best.smem = at.size;
+            }
+        }
+    }
+    return best;
+}
+
 void release(llmx_paged *p) {
     cudaFree(p->memory);
     delete p;
@@ -1570,7 +1619,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     p->bytes = at;
     p->scores_smem = 2 * blocks * ((head_dim + 31) / 32) * 512 + (size_t)max_requests * sizeof(Meta);
     const size_t chunk = std::max<size_t>(1, kChunk / blocks);
-    p->values_smem = kRing + 2 * chunk * blocks * 1024 + kExpWords * 4 + (kWarps + 4) * blocks * 16 + (size_t)max_requests * sizeof(Meta);
+    p->values_smem = kRing + 2 * chunk * blocks * 1024 + kExpWords * 4 + (3 * kWarps + 4) * blocks * 16 + (size_t)max_requests * sizeof(Meta);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     int16_t e16[2049], p18[2049], host[kExpWords * 2] = {};
     llmx::build_exp_tables(e16, p18);
@@ -1717,33 +1766,15 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.exps = p->exps;
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // All at once where the clusters, of 8 CTAs, fit the device together; with room left, a request's column blocks
-    // are shared out over several clusters.
     const int all = (int)((longest + kTile - 1) / kTile), most = (c.max_block * c.group + 7) / 8;
-    const uint64_t clusters = (uint64_t)requests * p->kv;
-    static const int force = getenv("LLMX_C") ? atoi(getenv("LLMX_C")) : -1;
-    static const int fg = getenv("LLMX_G") ? atoi(getenv("LLMX_G")) : 0;
-    if (force != 0) {
-        c.cluster_log = 3;
-        while (c.cluster_log > 0 && (force > 0 ? 1 << c.cluster_log > force : 1 << c.cluster_log > all)) c.cluster_log--;
-        const int cluster = 1 << c.cluster_log;
-        c.tiles = (all + cluster - 1) / cluster;
-        int best = 0;
-        for (int groups = 1; groups <= most; groups++) {
-            const int blocks = (most + groups - 1) / groups;
-            if (fg ? groups != fg : (groups > 1 && (most + blocks - 1) / blocks != groups)) continue;
-            const Places at(c.tiles, cluster, blocks, c.dim);
-            if (at.size > kMaxSmem || all > kShortTiles) continue;
-            const uint64_t room = (uint64_t)p->sms * std::min<uint64_t>(4, (227 * 1024) / (at.size + 2048));
-            if (force > 0 || clusters * cluster * groups <= (groups > 1 ? 2 : 1) * room) best = blocks;
-        }
-        if (best) {
-            c.blocks = best;
-            const Places at(c.tiles, cluster, best, c.dim);
-            const cudaError_t e = launch(attend_kernel(p->dim, best == 1), (unsigned)(clusters * cluster), kThreads, (size_t)at.size, c, s, cluster,
-                                         (unsigned)((most + best - 1) / best));
-            return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
-        }
+    const Clusters how = choose(p, (uint64_t)requests * p->kv, all, most);
+    if (how.ctas) {
+        c.cluster_log = how.log;
+        c.tiles = how.tiles;
+        c.blocks = how.blocks;
+        const cudaError_t e = launch(attend_kernel(p->dim, how.blocks == 1), (unsigned)how.ctas, kThreads, (size_t)how.smem, c, s, 1 << how.log,
+                                     (unsigned)((most + how.blocks - 1) / how.blocks));
+        return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
     }
     const uint64_t items = (uint64_t)requests * p->kv * ((longest + kTile - 1) / kTile);
     auto grid = [&](int ctas) { return (unsigned)std::min<uint64_t>(items, (uint64_t)ctas); };
