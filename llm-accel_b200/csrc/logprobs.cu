@@ -11,14 +11,15 @@
 //
 // Two launches.  k_rows reads the logits once.  All rows are one line of chunks of 512 logits, cut
 // into equal runs, a run per warp; for every row that its run touches a warp leaves a
-// part: the maximum, both sums relative to it (binary32, of 16 terms at a time), the tokens
-// ahead of the given one and its best tokens in order.  k_rows_join adds up a row's parts, in
+// part: the maximum, both sums relative to it (binary32, of 16 terms at a time) and the tokens
+// ahead of the given one; and every chunk's maximum.  k_rows_join adds up a row's parts, in
 // binary64 and in order, so a result depends on no timing.
 //
-// The best tokens: a warp holds them in order, one a lane, as 64-bit keys (logit, then the
-// lower index), and passes over chunks whose maximum does not exceed the least of them.
-// Others' logits above that go to a buffer in shared memory; 32 of them are sorted over the lanes and
-// merged at a time, so that even rising logits cost a few instructions each.
+// The most likely tokens need no more of the first launch than the chunks' maxima: the k best tokens
+// lie in the k best chunks (by maximum, then by index: every chunk has a token that is ahead of
+// whatever lies in a chunk behind it), which k_rows_join reads again.  A warp holds the best 64-bit keys
+// (logit, then the lower index) in order, one a lane; keys above the least of them go to a buffer in
+// shared memory, of which 32 at a time are sorted over the lanes and merged.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -44,8 +45,8 @@ constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kChunk = 512;               // logits: four 16-byte loads a lane
 constexpr uint32_t kMaxCtas = 592;        // of k_rows: four on each of 148 SMs
 
-// What a warp leaves of a row; its best tokens follow.
-struct Part {
+// What a warp leaves of a row.
+struct __align__(16) Part {
     int32_t top;      // maximum; kExcluded: nothing but excluded tokens
     uint32_t ahead;   // tokens ahead of the given one
     float rest, sum;  // of exp(-d) and of log2(e) d exp(-d), without one maximum
@@ -62,15 +63,13 @@ struct Call {
     float *entropy;
     uint32_t *top_tokens;
     float *top_logprobs;
-    unsigned char *parts;  // [slots] of part_bytes
-    uint32_t part_bytes;
+    // Parts of a warp's rows lie one after another, and those of a row's warps too: warp w's part of row r is
+    // number w + r, and on the way from one to the next either w or r grows by one.
+    Part *parts;
+    int32_t *maxima;       // [rows][chunks]
     uint32_t chunks;       // of a row
     uint32_t per;          // chunks a warp
 };
-
-// Parts of a warp's rows lie one after another, and those of a row's warps too: warp w's part
-// of row r is slot w + r, and on the way from one to the next either w or r grows by one.
-static __device__ __forceinline__ unsigned char *part_at(const Call &c, unsigned long long slot) { return c.parts + slot * c.part_bytes; }
 
 static __device__ __forceinline__ bool is_greedy(float t) { return !(t > kMinTemperature); }
 
@@ -145,28 +144,56 @@ struct Best {
 };
 
 // Logits i0 + 128 j + 4 lane .. + 3 of a row, excluded ones in place of those that are not there;
-// wide: the row's elements with an index that is 0 mod 4 are 16-byte aligned.
-static __device__ __forceinline__ void load(const int32_t *row, uint32_t vocab, uint32_t i0, bool wide, int (&z)[16]) {
+// aligned: those with an index that is 0 mod 4 are 16-byte aligned.
+static __device__ __forceinline__ void load(const int32_t *row, uint32_t vocab, uint32_t i0, bool aligned, int (&z)[16]) {
+    const uint32_t first = i0 + 4 * (threadIdx.x & 31);
+    if (aligned && i0 + kChunk <= vocab) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-        const uint32_t i = i0 + 128 * j + 4 * (threadIdx.x & 31);
-        if (wide && i + 3 < vocab) {
+        for (int j = 0; j < 4; j++)
             asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
                          : "=r"(z[4 * j]), "=r"(z[4 * j + 1]), "=r"(z[4 * j + 2]), "=r"(z[4 * j + 3])
-                         : "l"(row + i)
+                         : "l"(row + first + 128 * j)
                          : "memory");
-        } else {
+    } else {
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                z[4 * j + k] = kExcluded;
-                if (i + k < vocab) z[4 * j + k] = __ldcg(row + i + k);
-            }
+        for (int i = 0; i < 16; i++) {
+            const uint32_t v = first + 128 * (i / 4) + i % 4;
+            z[i] = kExcluded;
+            if (v < vocab) z[i] = __ldcg(row + v);
         }
     }
 }
 
+// Pairs of binary32 numbers.
+using f32x2 = unsigned long long;
+static __device__ __forceinline__ f32x2 pack2(float a, float b) {
+    f32x2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+static __device__ __forceinline__ void unpack2(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+static __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+static __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+static __device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+static __device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
-    __shared__ unsigned long long buffers[kWarps][64];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     pdl_wait();
     pdl_trigger();
@@ -174,96 +201,98 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
     const unsigned long long all = (unsigned long long)c.chunks * c.rows;
     const unsigned long long begin = w * c.per, end = min(begin + c.per, all);
     if (begin >= all) return;
-    Best best;
     uint32_t r = (uint32_t)(begin / c.chunks), chunk = (uint32_t)(begin - (unsigned long long)r * c.chunks);
+    const bool aligned = (((uintptr_t)c.logits | (c.ld * 4)) & 15u) == 0;
+    const int32_t *row = c.logits + (size_t)r * c.ld;
     int next[16];
-    auto fetch = [&](uint32_t row, uint32_t at) {
-        const int32_t *p = c.logits + (size_t)row * c.ld;
-        load(p, c.vocab, at * kChunk, ((uintptr_t)p & 15u) == 0, next);
-    };
-    fetch(r, chunk);
+    load(row, c.vocab, chunk * kChunk, aligned, next);
     for (unsigned long long at = begin; at < end;) {
         // one row's share of the run
         const uint32_t share = (uint32_t)min((unsigned long long)(c.chunks - chunk), end - at);
         const float temperature = c.temperature ? c.temperature[r] : 1.0f;
         const bool greedy = is_greedy(temperature);
-        // log2(e) / 2^16 / T in two parts: a rounded one alone would turn all terms the same way
-        const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
+        // -log2(e) / 2^16 / T in two parts: a rounded one alone would turn all terms the same way
+        const double scale = greedy ? 0.0 : -1.4426950408889634 / 65536.0 / (double)temperature;
         const float s_hi = (float)scale, s_lo = (float)(scale - (double)s_hi);
+        const f32x2 hi2 = pack2(s_hi, s_hi), lo2 = pack2(s_lo, s_lo);
         const uint32_t token = c.tokens ? c.tokens[r] : kNone;
-        const int mine = token < c.vocab ? __ldcg(c.logits + (size_t)r * c.ld + token) : kExcluded;
-        int m = kExcluded;  // of the warp
-        int least = kExcluded;
+        const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
+        int m = kExcluded;   // of the warp
+        bool far = false;    // an excluded token's term is 0 by itself, so far away is it
         float rest = 0, sum = 0;
         uint32_t ahead = 0;
-        best.start(buffers[warp], c.top);
-        for (uint32_t n = 0; n < share; n++, at++) {
+        for (uint32_t n = 0; n < share; n++) {
             int z[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) z[i] = next[i];
-            const uint32_t i0 = chunk * kChunk + 4 * lane;
-            if (++chunk == c.chunks) {
-                chunk = 0;
-                r++;
-            }
-            if (at + 1 < end) fetch(r, chunk);
+            const uint32_t i0 = (chunk + n) * kChunk;
+            if (n + 1 < share) load(row, c.vocab, i0 + kChunk, aligned, next);
+            else if (at + share < end) load(row + c.ld, c.vocab, 0, aligned, next);
             int most = z[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) most = max(most, z[i]);
             const int top = __reduce_max_sync(0xffffffffu, most);
+            if (lane == 0) c.maxima[(size_t)r * c.chunks + chunk + n] = top;
             if (top == kExcluded) continue;
-            int skip = -1;  // the maximum that is left out of the sums
-            if (top > m) {
-                if (!greedy && m != kExcluded) {  // the old maximum becomes an ordinary token
-                    const float d = (float)((uint32_t)top - (uint32_t)m);
-                    const float e = fmaf(d, s_hi, d * s_lo);
-                    const float f = exp2f(-e);
-                    if (lane == 0) rest += 1.0f;  // (it is 0 away from itself)
-                    sum = f * fmaf(rest, e, sum);
-                    rest *= f;
-                }
-                m = top;
-                const uint32_t who = __ballot_sync(0xffffffffu, most == top);
-                if (lane == __ffs(who) - 1) {
+            if (top > m || !far) {
+                int skip = -1;  // the maximum that is left out of the sums
+                if (top > m) {
+                    if (!greedy && m != kExcluded) {  // the old maximum becomes an ordinary token
+                        const float d = (float)((uint32_t)top - (uint32_t)m);
+                        const float e = fmaf(d, s_hi, d * s_lo), f = exp2f(e);
+                        if (lane == 0) rest += 1.0f;  // (it is 0 away from itself)
+                        sum = f * fmaf(rest, e, sum);
+                        rest *= f;
+                    }
+                    m = top;
+                    far = (float)((uint32_t)m ^ 0x80000000u) * s_hi < -150.0f;
+                    const uint32_t who = __ballot_sync(0xffffffffu, most == top);
+                    if (lane == __ffs(who) - 1) {
 #pragma unroll
-                    for (int i = 15; i >= 0; i--)
-                        if (z[i] == top) skip = i;
+                        for (int i = 15; i >= 0; i--)
+                            if (z[i] == top) skip = i;
+                    }
                 }
+                if (!greedy) {
+                    float r16 = 0, s16 = 0;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        const float d = (float)((uint32_t)m - (uint32_t)z[i]), e = fmaf(d, s_hi, d * s_lo);
+                        const float x = z[i] == kExcluded || i == skip ? 0.0f : exp2_fast(e);
+                        r16 += x;
+                        s16 = fmaf(x, e, s16);
+                    }
+                    rest += r16;
+                    sum += s16;
+                }
+            } else {
+                f32x2 r2 = 0, s2 = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i += 2) {
+                    const f32x2 d = pack2((float)((uint32_t)m - (uint32_t)z[i]), (float)((uint32_t)m - (uint32_t)z[i + 1]));
+                    const f32x2 e = fma2(d, hi2, mul2(d, lo2));
+                    float e0, e1;
+                    unpack2(e, e0, e1);
+                    const f32x2 x = pack2(exp2_fast(e0), exp2_fast(e1));
+                    r2 = add2(r2, x);
+                    s2 = fma2(x, e, s2);
+                }
+                float a, b;
+                unpack2(r2, a, b);
+                rest += a + b;
+                unpack2(s2, a, b);
+                sum += a + b;
             }
-            if (!greedy) {
-                float r16 = 0, s16 = 0;
+            if (top >= mine && mine != kExcluded) {
+                const uint32_t first = i0 + 4 * lane;
+                if (token - i0 < (uint32_t)kChunk) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float d = (float)((uint32_t)m - (uint32_t)z[i]);
-                    const float e = fmaf(d, s_hi, d * s_lo);
-                    float x;
-                    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(x) : "f"(-e));
-                    if (z[i] == kExcluded || i == skip) x = 0;
-                    r16 += x;
-                    s16 = fmaf(x, e, s16);
-                }
-                rest += r16;
-                sum += s16;
-            }
-            if (mine != kExcluded && top >= mine) {
+                    for (int i = 0; i < 16; i++) ahead += z[i] > mine || (z[i] == mine && first + 128 * (i / 4) + i % 4 < token);
+                } else {
+                    const int over = token < i0 ? mine : mine - 1;  // in front of the token equal ones are ahead
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const uint32_t v = i0 + 128 * (i / 4) + i % 4;
-                    ahead += z[i] > mine || (z[i] == mine && v < token);
+                    for (int i = 0; i < 16; i++) ahead += z[i] > over;
                 }
-            }
-            if (c.top && top > least) {
-                int bound = least;
-                if (least == kExcluded) {  // the first chunk: the top-th of the lanes' maxima bounds from below
-                    const unsigned long long k = sort64(key_of(most, 0));
-                    const int t = logit_of(__shfl_sync(0xffffffffu, k, (int)c.top - 1));
-                    bound = t == kExcluded ? t : t - 1;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) best.push(z[i] > bound, key_of(z[i], i0 + 128 * (i / 4) + i % 4));
-                best.finish();
-                const unsigned long long k = best.least();
-                least = k ? logit_of(k) : kExcluded;
             }
         }
         ahead = __reduce_add_sync(0xffffffffu, ahead);
@@ -272,16 +301,33 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
             rest += __shfl_xor_sync(0xffffffffu, rest, o);
             sum += __shfl_xor_sync(0xffffffffu, sum, o);
         }
-        const uint32_t row = chunk == 0 ? r - 1 : r;
-        unsigned char *part = part_at(c, w + row);
-        if (lane == 0) *reinterpret_cast<Part *>(part) = Part{m, ahead, rest, sum};
-        if (lane < (int)c.top) reinterpret_cast<unsigned long long *>(part + sizeof(Part))[lane] = best.list;
+        if (lane == 0) c.parts[w + r] = Part{m, ahead, rest, -sum};
+        at += share;
+        chunk += share;
+        if (chunk == c.chunks) {
+            chunk = 0;
+            r++;
+            row += c.ld;
+        }
     }
+}
+
+// The warps' lists put together, in the first warp.
+static __device__ __forceinline__ unsigned long long gather(unsigned long long list, unsigned long long (&lists)[kWarps][32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int half = kWarps / 2; half; half /= 2) {
+        if (warp >= half && warp < 2 * half) lists[warp][lane] = list;
+        __syncthreads();
+        if (warp < half) list = merge64(list, lists[warp + half][lane]);
+    }
+    return list;
 }
 
 __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     __shared__ unsigned long long buffers[kWarps][64];
     __shared__ unsigned long long lists[kWarps][32];
+    __shared__ unsigned long long chosen[32];
     __shared__ int tops[kWarps], holders[kWarps];
     __shared__ double rests[kWarps], sums[kWarps];
     __shared__ uint32_t aheads[kWarps];
@@ -289,23 +335,36 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     pdl_wait();
     pdl_trigger();
     const uint32_t r = blockIdx.x;
+    const int32_t *row = c.logits + (size_t)r * c.ld;
     // the warps of k_rows that had a share of this row
     const unsigned long long first = (unsigned long long)r * c.chunks / c.per, last = ((unsigned long long)(r + 1) * c.chunks - 1) / c.per;
     const int parts = (int)(last - first + 1);
+    const Part *part = c.parts + first + r;
     const float temperature = c.temperature ? c.temperature[r] : 1.0f;
     const bool greedy = is_greedy(temperature);
     const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
-
-    int m = kExcluded;
-    for (int i = threadIdx.x; i < parts; i += kThreads) m = max(m, reinterpret_cast<const Part *>(part_at(c, first + i + r))->top);
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) tops[warp] = m;
+    const uint32_t token = c.tokens ? c.tokens[r] : kNone;
+    const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
+    // The best chunks.  (Where there are fewer than 32 a warp they are one sort.)
+    Best best;
+    best.start(buffers[warp], max(c.top, 1u));
+    unsigned long long bound = 0;
+    const int32_t *maxima = c.maxima + (size_t)r * c.chunks;
+    for (uint32_t i = warp * 32; i < c.chunks; i += kThreads) {
+        const int z = i + lane < c.chunks ? maxima[i + lane] : kExcluded;
+        const unsigned long long key = z == kExcluded ? 0 : key_of(z, i + lane);
+        best.push(key > bound, key);
+        bound = max(bound, best.least());
+    }
+    best.finish();
+    unsigned long long list = gather(best.list, lists);
+    if (warp == 0) chosen[lane] = list;
     __syncthreads();
-    for (int i = 0; i < kWarps; i++) m = max(m, tops[i]);
+    const int m = chosen[0] ? logit_of(chosen[0]) : kExcluded;
     // one maximum stays out of the sums: that of the first part which holds it
     int holder = INT_MAX;
     for (int i = threadIdx.x; i < parts && holder == INT_MAX; i += kThreads)
-        if (reinterpret_cast<const Part *>(part_at(c, first + i + r))->top == m) holder = i;
+        if (part[i].top == m) holder = i;
     holder = __reduce_min_sync(0xffffffffu, holder);
     if (lane == 0) holders[warp] = holder;
     __syncthreads();
@@ -313,7 +372,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     double rest = 0, sum = 0;
     uint32_t ahead = 0;
     for (int i = threadIdx.x; i < parts; i += kThreads) {
-        const Part p = *reinterpret_cast<const Part *>(part_at(c, first + i + r));
+        const Part p = part[i];
         ahead += p.ahead;
         if (p.top == kExcluded || greedy) continue;
         if (i == holder) {
@@ -325,36 +384,41 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
             sum += f * ((double)p.sum + with * e);
         }
     }
-    Best best;
-    best.start(buffers[warp], c.top);
-    if (c.top) {
-        // this warp's parts: warp, warp + kWarps, ...; their best tokens bound the list from below
-        unsigned long long k = 0;
-        if (warp + kWarps * lane < parts)
-            k = reinterpret_cast<const unsigned long long *>(part_at(c, first + warp + kWarps * lane + r) + sizeof(Part))[0];
-        k = __shfl_sync(0xffffffffu, sort64(k), (int)c.top - 1);
-        unsigned long long bound = k ? k - 1 : 0;
-        for (int i = warp; i < parts; i += kWarps) {
-            const unsigned long long *list = reinterpret_cast<const unsigned long long *>(part_at(c, first + i + r) + sizeof(Part));
-            const unsigned long long key = lane < (int)c.top ? list[lane] : 0;
-            best.push(key > bound, key);
-            bound = max(bound, best.least());
-        }
-        best.finish();
-    }
 #pragma unroll
     for (int o = 16; o; o /= 2) {
         rest += __shfl_xor_sync(0xffffffffu, rest, o);
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     ahead = __reduce_add_sync(0xffffffffu, ahead);
-    lists[warp][lane] = best.list;
     if (lane == 0) {
         rests[warp] = rest;
         sums[warp] = sum;
         aheads[warp] = ahead;
     }
-    __syncthreads();
+    // The best tokens, in the best chunks: the maximum of the last of these bounds them from below.
+    list = 0;
+    if (c.top) {
+        const unsigned long long least = chosen[c.top - 1];
+        bound = least ? (least >> 32 << 32) - 1 : 0;  // (any token with that logit may be one)
+        best.start(buffers[warp], c.top);
+        const bool aligned = ((uintptr_t)row & 15u) == 0;
+        for (uint32_t i = warp; i < c.top; i += kWarps) {
+            if (chosen[i] == 0) break;
+            const uint32_t i0 = (kNone - (uint32_t)chosen[i]) * kChunk;
+            int z[16];
+            load(row, c.vocab, i0, aligned, z);
+#pragma unroll
+            for (int k = 0; k < 16; k++) {
+                const unsigned long long key = z[k] == kExcluded ? 0 : key_of(z[k], i0 + 4 * lane + 128 * (k / 4) + k % 4);
+                best.push(key > bound, key);
+            }
+            bound = max(bound, best.least());
+        }
+        best.finish();
+        list = gather(best.list, lists);
+    } else {
+        __syncthreads();
+    }
     if (warp != 0) return;
     rest = sum = 0;
     ahead = 0;
@@ -363,9 +427,6 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
         sum += sums[i];
         ahead += aheads[i];
     }
-    unsigned long long list = best.list;
-    if (c.top)
-        for (int i = 1; i < kWarps; i++) list = merge64(list, lists[i][lane]);
     const double log_sum = log1p(rest), step = greedy ? 0.0 : 1.0 / (65536.0 * (double)temperature);
     // of a token that is not excluded
     auto logprob = [&](int z, bool ahead_of_all) -> float {
@@ -374,10 +435,8 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     };
     if (lane == 0) {
         if (c.tokens) {
-            const uint32_t token = c.tokens[r];
-            const int z = token < c.vocab ? __ldcg(c.logits + (size_t)r * c.ld + token) : kExcluded;
-            c.logprob[r] = z == kExcluded ? -INFINITY : logprob(z, ahead == 0);
-            c.rank[r] = z == kExcluded ? kNone : ahead;
+            c.logprob[r] = mine == kExcluded ? -INFINITY : logprob(mine, ahead == 0);
+            c.rank[r] = mine == kExcluded ? kNone : ahead;
         }
         c.entropy[r] = greedy || m == kExcluded ? 0.0f : (float)(log_sum + 0.6931471805599453 * sum / (1.0 + rest));
     }
@@ -387,8 +446,13 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     }
 }
 
-uint32_t part_bytes(uint32_t top) { return (uint32_t)sizeof(Part) + 8 * ((top + 1) / 2 * 2); }
 uint64_t chunks_of(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + kChunk - 1) / kChunk); }
+
+// Bytes of the workspace in front of the chunks' maxima: the parts.
+size_t maxima_at(uint32_t rows, uint32_t vocab) {
+    const uint64_t warps = std::min<uint64_t>(chunks_of(rows, vocab), (uint64_t)kMaxCtas * kWarps);
+    return ((warps + rows) * sizeof(Part) + 255) / 256 * 256;
+}
 
 int fail(int code, const std::string &msg) {
     llmx::set_last_error("token_logprobs: " + msg);
@@ -417,8 +481,8 @@ cudaError_t launch(const void *fn, unsigned grid, const Call &call, cudaStream_t
 }  // namespace
 
 extern "C" size_t llmx_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top) {
-    const uint64_t warps = std::min<uint64_t>(chunks_of(rows, vocab), (uint64_t)kMaxCtas * kWarps);
-    return ((warps + rows) * part_bytes(std::min(top, kMaxTop)) + 255) / 256 * 256;
+    (void)top;  // the best tokens pass through no memory
+    return maxima_at(rows, vocab) + (chunks_of(rows, vocab) * sizeof(int32_t) + 255) / 256 * 256;
 }
 
 extern "C" int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vocab, uint32_t rows, const uint32_t *tokens,
@@ -457,8 +521,8 @@ extern "C" int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vo
     c.entropy = entropy;
     c.top_tokens = top_tokens;
     c.top_logprobs = top_logprobs;
-    c.parts = static_cast<unsigned char *>(workspace);
-    c.part_bytes = part_bytes(top);
+    c.parts = static_cast<Part *>(workspace);
+    c.maxima = reinterpret_cast<int32_t *>(static_cast<unsigned char *>(workspace) + maxima_at(rows, vocab));
     c.chunks = (vocab + kChunk - 1) / kChunk;
     const uint64_t all = chunks_of(rows, vocab), most = std::min<uint64_t>((uint64_t)sms * 3, kMaxCtas) * kWarps;
     c.per = (uint32_t)((all + most - 1) / most);
