@@ -143,23 +143,25 @@ struct Best {
     }
 };
 
-// Logits i0 + 128 j + 4 lane .. + 3 of a row, excluded ones in place of those that are not there;
-// aligned: those with an index that is 0 mod 4 are 16-byte aligned.
-static __device__ __forceinline__ void load(const int32_t *row, uint32_t vocab, uint32_t i0, bool aligned, int (&z)[16]) {
-    const uint32_t first = i0 + 4 * (threadIdx.x & 31);
-    if (aligned && i0 + kChunk <= vocab) {
+// Rows are taken from the 16-byte boundary at or before their start on, so that a chunk is read by four
+// 16-byte loads a lane wherever the row starts: token v of a row is place v + shift.
+static __device__ __forceinline__ uint32_t shift_of(const int32_t *row) { return (uint32_t)((uintptr_t)row >> 2) & 3u; }
+// Places i0 + 128 j + 4 lane .. + 3 of a row, excluded tokens in place of those that are not there.
+static __device__ __forceinline__ void load(const int32_t *row, uint32_t vocab, uint32_t i0, int (&z)[16]) {
+    const uint32_t shift = shift_of(row), first = i0 + 4 * (threadIdx.x & 31);
+    if (i0 >= shift && i0 + kChunk - shift <= vocab) {
 #pragma unroll
         for (int j = 0; j < 4; j++)
             asm volatile("ld.global.L1::no_allocate.v4.s32 {%0,%1,%2,%3}, [%4];"
                          : "=r"(z[4 * j]), "=r"(z[4 * j + 1]), "=r"(z[4 * j + 2]), "=r"(z[4 * j + 3])
-                         : "l"(row + first + 128 * j)
+                         : "l"(row - shift + first + 128 * j)
                          : "memory");
     } else {
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            const uint32_t v = first + 128 * (i / 4) + i % 4;
+            const uint32_t v = first + 128 * (i / 4) + i % 4 - shift;
             z[i] = kExcluded;
-            if (v < vocab) z[i] = __ldcg(row + v);
+            if (v < vocab) z[i] = __ldcg(row + v);  // (one in front of the row is far beyond it)
         }
     }
 }
@@ -202,10 +204,9 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
     const unsigned long long begin = w * c.per, end = min(begin + c.per, all);
     if (begin >= all) return;
     uint32_t r = (uint32_t)(begin / c.chunks), chunk = (uint32_t)(begin - (unsigned long long)r * c.chunks);
-    const bool aligned = (((uintptr_t)c.logits | (c.ld * 4)) & 15u) == 0;
     const int32_t *row = c.logits + (size_t)r * c.ld;
     int next[16];
-    load(row, c.vocab, chunk * kChunk, aligned, next);
+    load(row, c.vocab, chunk * kChunk, next);
     for (unsigned long long at = begin; at < end;) {
         // one row's share of the run
         const uint32_t share = (uint32_t)min((unsigned long long)(c.chunks - chunk), end - at);
@@ -217,6 +218,7 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
         const f32x2 hi2 = pack2(s_hi, s_hi), lo2 = pack2(s_lo, s_lo);
         const uint32_t token = c.tokens ? c.tokens[r] : kNone;
         const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
+        const uint32_t place = token + shift_of(row);
         int m = kExcluded;   // of the warp
         bool far = false;    // an excluded token's term is 0 by itself, so far away is it
         float rest = 0, sum = 0;
@@ -226,8 +228,8 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
 #pragma unroll
             for (int i = 0; i < 16; i++) z[i] = next[i];
             const uint32_t i0 = (chunk + n) * kChunk;
-            if (n + 1 < share) load(row, c.vocab, i0 + kChunk, aligned, next);
-            else if (at + share < end) load(row + c.ld, c.vocab, 0, aligned, next);
+            if (n + 1 < share) load(row, c.vocab, i0 + kChunk, next);
+            else if (at + share < end) load(row + c.ld, c.vocab, 0, next);
             int most = z[0];
 #pragma unroll
             for (int i = 1; i < 16; i++) most = max(most, z[i]);
@@ -285,11 +287,11 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
             }
             if (top >= mine && mine != kExcluded) {
                 const uint32_t first = i0 + 4 * lane;
-                if (token - i0 < (uint32_t)kChunk) {
+                if (place - i0 < (uint32_t)kChunk) {
 #pragma unroll
-                    for (int i = 0; i < 16; i++) ahead += z[i] > mine || (z[i] == mine && first + 128 * (i / 4) + i % 4 < token);
+                    for (int i = 0; i < 16; i++) ahead += z[i] > mine || (z[i] == mine && first + 128 * (i / 4) + i % 4 < place);
                 } else {
-                    const int over = token < i0 ? mine : mine - 1;  // in front of the token equal ones are ahead
+                    const int over = place < i0 ? mine : mine - 1;  // in front of the token equal ones are ahead
 #pragma unroll
                     for (int i = 0; i < 16; i++) ahead += z[i] > over;
                 }
@@ -324,14 +326,16 @@ static __device__ __forceinline__ unsigned long long gather(unsigned long long l
     return list;
 }
 
+constexpr int kCandidates = 256;  // tokens whose places are found by comparing all with all
+
 __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     __shared__ unsigned long long buffers[kWarps][64];
     __shared__ unsigned long long lists[kWarps][32];
-    __shared__ unsigned long long chosen[32];
-    __shared__ int tops[kWarps], holders[kWarps];
+    __shared__ unsigned long long chosen[32], candidates[kCandidates];
     __shared__ double rests[kWarps], sums[kWarps];
-    __shared__ uint32_t aheads[kWarps];
+    __shared__ uint32_t aheads[kWarps], found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) found = 0;
     pdl_wait();
     pdl_trigger();
     const uint32_t r = blockIdx.x;
@@ -340,113 +344,165 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     const unsigned long long first = (unsigned long long)r * c.chunks / c.per, last = ((unsigned long long)(r + 1) * c.chunks - 1) / c.per;
     const int parts = (int)(last - first + 1);
     const Part *part = c.parts + first + r;
+    const int32_t *maxima = c.maxima + (size_t)r * c.chunks;
+    // (all loads are on their way before the first is used)
+    const Part mine_part = (int)threadIdx.x < parts ? part[threadIdx.x] : Part{kExcluded, 0, 0, 0};
+    auto key_at = [&](uint32_t i) -> unsigned long long {
+        const int z = i < c.chunks ? maxima[i] : kExcluded;
+        return z == kExcluded ? 0 : key_of(z, i);
+    };
+    const unsigned long long key0 = key_at(threadIdx.x), key1 = key_at(kThreads + threadIdx.x);
     const float temperature = c.temperature ? c.temperature[r] : 1.0f;
-    const bool greedy = is_greedy(temperature);
-    const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
     const uint32_t token = c.tokens ? c.tokens[r] : kNone;
     const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
-    // The best chunks.  (Where there are fewer than 32 a warp they are one sort.)
-    Best best;
-    best.start(buffers[warp], max(c.top, 1u));
-    unsigned long long bound = 0;
-    const int32_t *maxima = c.maxima + (size_t)r * c.chunks;
-    for (uint32_t i = warp * 32; i < c.chunks; i += kThreads) {
-        const int z = i + lane < c.chunks ? maxima[i + lane] : kExcluded;
-        const unsigned long long key = z == kExcluded ? 0 : key_of(z, i + lane);
-        best.push(key > bound, key);
-        bound = max(bound, best.least());
+    const bool greedy = is_greedy(temperature);
+    const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
+    // The best chunks.
+    unsigned long long list;
+    if (c.top <= 1) {  // the best one: maxima of keys
+        unsigned long long k = key0 > key1 ? key0 : key1;
+        for (uint32_t i = 2 * kThreads + threadIdx.x; i < c.chunks; i += kThreads) k = max(k, key_at(i));
+        const uint32_t hi = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32));
+        const uint32_t lo = __reduce_max_sync(0xffffffffu, (uint32_t)(k >> 32) == hi ? (uint32_t)k : 0u);
+        if (lane == 0) lists[warp][0] = (unsigned long long)hi << 32 | lo;
+        __syncthreads();
+        list = 0;
+        for (int w = 0; w < kWarps; w++) list = max(list, lists[w][0]);
+        if (threadIdx.x == 0) chosen[0] = list;
+    } else {
+        Best best;
+        best.start(buffers[warp], c.top);
+        best.list = sort64(key0);
+        unsigned long long bound = best.least();
+        best.push(key1 > bound, key1);
+        for (uint32_t i = 2 * kThreads + warp * 32; i < c.chunks; i += kThreads) {
+            const unsigned long long key = key_at(i + lane);
+            best.push(key > bound, key);
+            bound = max(bound, best.least());
+        }
+        best.finish();
+        list = gather(best.list, lists);
+        if (warp == 0) chosen[lane] = list;
     }
-    best.finish();
-    unsigned long long list = gather(best.list, lists);
-    if (warp == 0) chosen[lane] = list;
     __syncthreads();
-    const int m = chosen[0] ? logit_of(chosen[0]) : kExcluded;
-    // one maximum stays out of the sums: that of the first part which holds it
-    int holder = INT_MAX;
-    for (int i = threadIdx.x; i < parts && holder == INT_MAX; i += kThreads)
-        if (part[i].top == m) holder = i;
-    holder = __reduce_min_sync(0xffffffffu, holder);
-    if (lane == 0) holders[warp] = holder;
-    __syncthreads();
-    for (int i = 0; i < kWarps; i++) holder = min(holder, holders[i]);
+    // Their logits, on their way while the parts are added up; four chunks a warp at most.
+    const unsigned long long most = chosen[0], least = c.top ? chosen[c.top - 1] : 0;
+    int z[16];
+    const bool any = (uint32_t)warp < c.top && chosen[min(warp, 31)] != 0;
+    if (any) load(row, c.vocab, (kNone - (uint32_t)chosen[warp]) * kChunk, z);
+    const int m = most ? logit_of(most) : kExcluded;
+    // One maximum stays out of the sums: the parts that have it count one less.
     double rest = 0, sum = 0;
     uint32_t ahead = 0;
-    for (int i = threadIdx.x; i < parts; i += kThreads) {
-        const Part p = part[i];
+    int with = 0;
+    auto add = [&](const Part &p) {
         ahead += p.ahead;
-        if (p.top == kExcluded || greedy) continue;
-        if (i == holder) {
+        if (p.top == kExcluded || greedy) return;
+        if (p.top == m) {
+            with++;
             rest += (double)p.rest;
             sum += (double)p.sum;
         } else {
-            const double e = (double)((uint32_t)m - (uint32_t)p.top) * scale, f = exp2(-e), with = (double)p.rest + 1.0;
-            rest += f * with;
-            sum += f * ((double)p.sum + with * e);
+            const double e = (double)((uint32_t)m - (uint32_t)p.top) * scale, f = exp2(-e), all = (double)p.rest + 1.0;
+            rest += f * all;
+            sum += f * ((double)p.sum + all * e);
         }
-    }
+    };
+    add(mine_part);
+    for (int i = kThreads + threadIdx.x; i < parts; i += kThreads) add(part[i]);
 #pragma unroll
     for (int o = 16; o; o /= 2) {
         rest += __shfl_xor_sync(0xffffffffu, rest, o);
         sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     ahead = __reduce_add_sync(0xffffffffu, ahead);
+    with = __reduce_add_sync(0xffffffffu, with);
     if (lane == 0) {
         rests[warp] = rest;
         sums[warp] = sum;
         aheads[warp] = ahead;
+        lists[warp][1] = (unsigned long long)with;
     }
-    // The best tokens, in the best chunks: the maximum of the last of these bounds them from below.
-    list = 0;
-    if (c.top) {
-        const unsigned long long least = chosen[c.top - 1];
-        bound = least ? (least >> 32 << 32) - 1 : 0;  // (any token with that logit may be one)
-        best.start(buffers[warp], c.top);
-        const bool aligned = ((uintptr_t)row & 15u) == 0;
-        for (uint32_t i = warp; i < c.top; i += kWarps) {
-            if (chosen[i] == 0) break;
-            const uint32_t i0 = (kNone - (uint32_t)chosen[i]) * kChunk;
-            int z[16];
-            load(row, c.vocab, i0, aligned, z);
+    // The best tokens: the maximum of the last of the best chunks bounds them from below (any token with that
+    // logit may be one).
+    const unsigned long long bound = least ? (least >> 32 << 32) - 1 : 0;
+    auto chunk_keys = [&](uint32_t i, auto use) {
+        const uint32_t i0 = (kNone - (uint32_t)chosen[i]) * kChunk + 4 * lane - shift_of(row);
 #pragma unroll
-            for (int k = 0; k < 16; k++) {
-                const unsigned long long key = z[k] == kExcluded ? 0 : key_of(z[k], i0 + 4 * lane + 128 * (k / 4) + k % 4);
-                best.push(key > bound, key);
-            }
-            bound = max(bound, best.least());
+        for (int k = 0; k < 16; k++) {
+            const unsigned long long key = z[k] == kExcluded ? 0 : key_of(z[k], i0 + 128 * (k / 4) + k % 4);
+            use(key > bound, key);
         }
-        best.finish();
-        list = gather(best.list, lists);
-    } else {
-        __syncthreads();
+    };
+    for (uint32_t i = warp; i < c.top && chosen[i] != 0; i += kWarps) {
+        if (i >= (uint32_t)kWarps) load(row, c.vocab, (kNone - (uint32_t)chosen[i]) * kChunk, z);
+        chunk_keys(i, [&](bool in, unsigned long long key) {
+            if (in) {
+                const uint32_t at = atomicAdd(&found, 1u);
+                if (at < (uint32_t)kCandidates) candidates[at] = key;
+            }
+        });
     }
-    if (warp != 0) return;
-    rest = sum = 0;
+    __syncthreads();
+    double all_rest = 0, all_sum = 0;
+    long long all_with = -1;
     ahead = 0;
     for (int i = 0; i < kWarps; i++) {
-        rest += rests[i];
-        sum += sums[i];
+        all_rest += rests[i];
+        all_sum += sums[i];
         ahead += aheads[i];
+        all_with += (long long)lists[i][1];
     }
+    if (greedy || m == kExcluded) all_with = 0;
+    rest = all_rest + (double)all_with;
+    sum = all_sum;
     const double log_sum = log1p(rest), step = greedy ? 0.0 : 1.0 / (65536.0 * (double)temperature);
     // of a token that is not excluded
     auto logprob = [&](int z, bool ahead_of_all) -> float {
         if (greedy) return ahead_of_all ? 0.0f : -INFINITY;
         return (float)(-(double)((uint32_t)m - (uint32_t)z) * step - log_sum);
     };
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         if (c.tokens) {
             c.logprob[r] = mine == kExcluded ? -INFINITY : logprob(mine, ahead == 0);
             c.rank[r] = mine == kExcluded ? kNone : ahead;
         }
         c.entropy[r] = greedy || m == kExcluded ? 0.0f : (float)(log_sum + 0.6931471805599453 * sum / (1.0 + rest));
     }
-    if (lane < (int)c.top) {
-        c.top_tokens[(size_t)r * c.top + lane] = list ? kNone - (uint32_t)list : kNone;
-        c.top_logprobs[(size_t)r * c.top + lane] = list ? logprob(logit_of(list), lane == 0) : -INFINITY;
+    if (c.top == 0) return;
+    auto put = [&](uint32_t place, unsigned long long key) {
+        c.top_tokens[(size_t)r * c.top + place] = key ? kNone - (uint32_t)key : kNone;
+        c.top_logprobs[(size_t)r * c.top + place] = key ? logprob(logit_of(key), place == 0) : -INFINITY;
+    };
+    const uint32_t n = found;
+    if (n <= (uint32_t)kCandidates) {
+        if (threadIdx.x < n) {
+            const unsigned long long key = candidates[threadIdx.x];
+            uint32_t place = 0;
+            for (uint32_t i = 0; i < n; i++) place += candidates[i] > key;
+            if (place < c.top) put(place, key);
+        }
+        if (threadIdx.x >= n && threadIdx.x < c.top) put(threadIdx.x, 0);  // fewer than asked for
+        return;
     }
+    // many equal ones: in order, by warps
+    Best best;
+    best.start(buffers[warp], c.top);
+    for (uint32_t i = warp; i < c.top && chosen[i] != 0; i += kWarps) {
+        load(row, c.vocab, (kNone - (uint32_t)chosen[i]) * kChunk, z);
+        unsigned long long most_key = 0;
+        chunk_keys(i, [&](bool, unsigned long long key) { most_key = max(most_key, key); });
+        // the top-th of the lanes' best bounds from below as well
+        const unsigned long long t = __shfl_sync(0xffffffffu, sort64(most_key), (int)c.top - 1), floor = max(best.least(), t ? t - 1 : 0);
+        chunk_keys(i, [&](bool in, unsigned long long key) { best.push(in && key > floor, key); });
+    }
+    best.finish();
+    list = gather(best.list, lists);
+    if (warp == 0 && lane < (int)c.top) put((uint32_t)lane, list);
 }
 
-uint64_t chunks_of(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + kChunk - 1) / kChunk); }
+// (of rows that may start anywhere)
+uint64_t chunks_of(uint32_t rows, uint32_t vocab) { return (uint64_t)rows * ((vocab + 3 + kChunk - 1) / kChunk); }
 
 // Bytes of the workspace in front of the chunks' maxima: the parts.
 size_t maxima_at(uint32_t rows, uint32_t vocab) {
@@ -523,8 +579,9 @@ extern "C" int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vo
     c.top_logprobs = top_logprobs;
     c.parts = static_cast<Part *>(workspace);
     c.maxima = reinterpret_cast<int32_t *>(static_cast<unsigned char *>(workspace) + maxima_at(rows, vocab));
-    c.chunks = (vocab + kChunk - 1) / kChunk;
-    const uint64_t all = chunks_of(rows, vocab), most = std::min<uint64_t>((uint64_t)sms * 3, kMaxCtas) * kWarps;
+    const bool aligned = (((uintptr_t)logits | (ld * 4)) & 15u) == 0;
+    c.chunks = (vocab + (aligned ? 0 : 3) + kChunk - 1) / kChunk;
+    const uint64_t all = (uint64_t)rows * c.chunks, most = std::min<uint64_t>((uint64_t)sms * 3, kMaxCtas) * kWarps;
     c.per = (uint32_t)((all + most - 1) / most);
     const uint64_t warps = (all + c.per - 1) / c.per;
     cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -1355,63 +1355,81 @@ struct AppendCall {
     const uint32_t *offsets, *lengths;
     uint32_t rows, requests, pages;
     int heads, kv, dim, page_len;
+    uint32_t parts_magic;  // for dividing by dim / 16
     int *error;
 };
 
+// Two pairs.  A table may hold any 16-bit values: x0 c - x1 s stays within 2^31 - 2^15 even so, and x1 c + x0 s
+// leaves 32 bits in one case only, as 2^31, where the wrapped sum is one that nothing else gives.
 static __device__ __forceinline__ void turn2(uint32_t x0, uint32_t x1, uint32_t c, uint32_t s, uint32_t &y0, uint32_t &y1) {
-    // products of 16-bit values, their sums in 64 bits: a table may hold any value
-    auto one = [](long long a, int ca, long long b, int cb) { return sat16(rnd(a * ca + b * cb, 8)); };
+    auto minus = [](int a, int ca, int b, int cb) { return (a * ca + 128 - b * cb) >> 8; };
+    auto plus = [](int a, int ca, int b, int cb) {
+        const int w = (int)((uint32_t)(a * ca) + (uint32_t)(b * cb) + 128u);
+        return (w == INT_MIN + 128 ? INT_MAX : w) >> 8;
+    };
     const int c0 = llmx::lo16(c), c1 = llmx::hi16(c), s0 = llmx::lo16(s), s1 = llmx::hi16(s);
     const int a0 = llmx::lo16(x0), a1 = llmx::hi16(x0), b0 = llmx::lo16(x1), b1 = llmx::hi16(x1);
-    y0 = (uint32_t)(one(a0, c0, b0, -s0) & 0xffff) | (uint32_t)one(a1, c1, b1, -s1) << 16;
-    y1 = (uint32_t)(one(b0, c0, a0, s0) & 0xffff) | (uint32_t)one(b1, c1, a1, s1) << 16;
+    y0 = pack_sat16(minus(a0, c0, b0, s0), minus(a1, c1, b1, s1));
+    y1 = pack_sat16(plus(b0, c0, a0, s0), plus(b1, c1, a1, s1));
 }
 
-// A CTA per row; a thread turns 8 pairs (i, i + dim/2) of a head, or copies 16 values.
+// A CTA per row; a thread turns 8 pairs (i, i + dim/2) of a head, or copies 16 values.  The row's own values are on
+// their way while its request, its position, and by that its page and its turn are looked up, one after
+// another: that is what a row takes.
 __global__ void __launch_bounds__(256) k_append(const AppendCall c) {
     pdl_wait();
     pdl_trigger();
     const uint32_t r = blockIdx.x;
+    const int parts = c.dim >> 4, half = c.dim >> 1, items = (c.heads + 2 * c.kv) * parts;  // 16 values each
+    auto load = [&](int i, int &head, int &part, uint4 &x0, uint4 &x1) {
+        head = parts == 1 ? i : (int)__umulhi((uint32_t)i, c.parts_magic);
+        part = i - head * parts;
+        const int16_t *src = c.qkv + (size_t)r * c.ld_qkv + (size_t)head * c.dim;
+        const bool turned = head < c.heads + c.kv;
+        x0 = *reinterpret_cast<const uint4 *>(src + (turned ? 8 : 16) * part);
+        x1 = *reinterpret_cast<const uint4 *>(src + (turned ? half + 8 * part : 16 * part + 8));
+    };
+    int head = 0, part = 0;
+    uint4 x0, x1;
+    if ((int)threadIdx.x < items) load((int)threadIdx.x, head, part, x0, x1);
     const uint32_t b = request_of(c.offsets, c.requests, r);
     const uint32_t first = c.offsets[b], last = c.offsets[b + 1];
     if (r < first || r >= last) return;  // of no request
     const long long position = (long long)c.lengths[b] - (long long)(last - first) + (r - first);
     if (position < 0) return;  // in front of the sequence
-    const long long at = position / c.page_len;
-    if (position >= c.positions || at >= (long long)c.ld_table) {
+    const uint32_t at = (uint32_t)position / (uint32_t)c.page_len;
+    if (position >= c.positions || at >= c.ld_table) {
         if (threadIdx.x == 0) atomicOr(c.error, kErrRequest);
         return;
     }
     const uint32_t page = (uint32_t)c.table[(size_t)b * c.ld_table + at];
-    if (page >= c.pages) {
-        if (threadIdx.x == 0) atomicOr(c.error, kErrPage);
-        return;
-    }
-    const size_t inside = (size_t)(position - at * c.page_len);
-    const int parts = c.dim >> 4, half = c.dim >> 1;  // 16 values each
     const int16_t *turn = c.rope + (size_t)position * c.dim;
-    for (int i = threadIdx.x; i < (c.heads + 2 * c.kv) * parts; i += blockDim.x) {
-        const int head = i / parts, part = i - head * parts;
-        const int16_t *src = c.qkv + (size_t)r * c.ld_qkv + (size_t)head * c.dim;
+    const size_t inside = (size_t)((uint32_t)position - at * (uint32_t)c.page_len);
+    for (int i = threadIdx.x; i < items; i += blockDim.x) {
+        if (i != (int)threadIdx.x) load(i, head, part, x0, x1);
+        uint4 y0 = x0, y1 = x1;
+        int16_t *dst;
+        int at0 = 16 * part, at1 = 16 * part + 8;
         if (head < c.heads + c.kv) {
-            const uint4 x0 = *reinterpret_cast<const uint4 *>(src + 8 * part), x1 = *reinterpret_cast<const uint4 *>(src + half + 8 * part);
             const uint4 cs = *reinterpret_cast<const uint4 *>(turn + 8 * part), sn = *reinterpret_cast<const uint4 *>(turn + half + 8 * part);
-            uint4 y0, y1;
             turn2(x0.x, x1.x, cs.x, sn.x, y0.x, y1.x);
             turn2(x0.y, x1.y, cs.y, sn.y, y0.y, y1.y);
             turn2(x0.z, x1.z, cs.z, sn.z, y0.z, y1.z);
             turn2(x0.w, x1.w, cs.w, sn.w, y0.w, y1.w);
-            int16_t *dst = head < c.heads ? c.q + (size_t)r * c.ld_q + (size_t)head * c.dim
-                                          : c.k + (((size_t)page * c.kv + (head - c.heads)) * c.page_len + inside) * c.dim;
-            *reinterpret_cast<uint4 *>(dst + 8 * part) = y0;
-            *reinterpret_cast<uint4 *>(dst + half + 8 * part) = y1;
-        } else {
-            const uint4 *from = reinterpret_cast<const uint4 *>(src) + 2 * part;
-            uint4 *to = reinterpret_cast<uint4 *>(c.v + (((size_t)page * c.kv + (head - c.heads - c.kv)) * c.page_len + inside) * c.dim) + 2 * part;
-            const uint4 a = from[0], d = from[1];
-            to[0] = a;
-            to[1] = d;
+            at0 = 8 * part;
+            at1 = half + 8 * part;
         }
+        if (page >= c.pages) {
+            if (i == 0) atomicOr(c.error, kErrPage);
+            return;
+        }
+        if (head < c.heads) dst = c.q + (size_t)r * c.ld_q + (size_t)head * c.dim;
+        else {
+            const bool key = head < c.heads + c.kv;
+            dst = (key ? c.k : c.v) + (((size_t)page * c.kv + (head - c.heads - (key ? 0 : c.kv))) * c.page_len + inside) * c.dim;
+        }
+        *reinterpret_cast<uint4 *>(dst + at0) = y0;
+        *reinterpret_cast<uint4 *>(dst + at1) = y1;
     }
 }
 
@@ -1704,6 +1722,7 @@ extern "C" int llmx_paged_append(llmx_paged *p, const int16_t *qkv, uint32_t row
     c.dim = p->dim;
     c.page_len = p->page_len;
     c.error = p->error;
+    c.parts_magic = (uint32_t)(((1ull << 32) + p->dim / 16 - 1) / (p->dim / 16));
     const int work = (p->heads + 2 * p->kv) * (p->dim / 16);
     const cudaError_t e = launch((const void *)k_append, rows, std::min(256, (work + 31) / 32 * 32), 0, c, static_cast<cudaStream_t>(stream));
     return e == cudaSuccess ? LLMX_OK : cuda_fail("append", e);
