@@ -14,6 +14,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -66,11 +67,24 @@ def _compile(src, force, build_dir, defines):
     return obj
 
 
+def _build_calls(force):
+    """The Python module of csrc/pycalls.c, next to the library; without Python's
+    headers it is left out, and llmx.py makes all its calls through ctypes."""
+    src, out = os.path.join(CSRC, "pycalls.c"), os.path.join(HERE, "_llmxcalls.so")
+    inc = sysconfig.get_paths()["include"]
+    if not os.path.exists(os.path.join(inc, "Python.h")):
+        return
+    if force or _newer(out, [src, os.path.join(ROOT, "include", "llmx.h")]):
+        subprocess.run([os.environ.get("CC", "gcc"), "-O2", "-Wall", "-shared", "-fPIC", "-I", inc, "-I", os.path.join(ROOT, "include"),
+                        src, "-o", out], check=True)
+
+
 def build(force: bool = False, timeline: bool = False) -> str:
     build_dir = BUILD + "_timeline" if timeline else BUILD
     lib = os.path.join(HERE, "libllmx_timeline.so") if timeline else LIB
     defines = ["-DLLMX_TIMELINE"] if timeline else []
     os.makedirs(build_dir, exist_ok=True)
+    _build_calls(force)
     with cf.ThreadPoolExecutor(len(SOURCES)) as ex:
         objs = list(ex.map(lambda s: _compile(s, force, build_dir, defines), SOURCES))
     if force or _newer(lib, objs):

@@ -1392,19 +1392,39 @@ __global__ void __launch_bounds__(256) k_append(const AppendCall c) {
     int head = 0, part = 0;
     uint4 x0, x1;
     if ((int)threadIdx.x < items) load((int)threadIdx.x, head, part, x0, x1);
-    const uint32_t b = request_of(c.offsets, c.requests, r);
-    const uint32_t first = c.offsets[b], last = c.offsets[b + 1];
-    if (r < first || r >= last) return;  // of no request
-    const long long position = (long long)c.lengths[b] - (long long)(last - first) + (r - first);
-    if (position < 0) return;  // in front of the sequence
-    const uint32_t at = (uint32_t)position / (uint32_t)c.page_len;
-    if (position >= c.positions || at >= c.ld_table) {
-        if (threadIdx.x == 0) atomicOr(c.error, kErrRequest);
-        return;
+    // the first warp looks the row's place up
+    __shared__ uint32_t where[3];  // page (kNowhere: the row is left out), position, and that within the page
+    constexpr uint32_t kNowhere = 0xffffffffu;
+    if (threadIdx.x < 32) {
+        const uint32_t b = request_of(c.offsets, c.requests, r);
+        const uint32_t first = __ldcg(c.offsets + b), last = __ldcg(c.offsets + b + 1), length = __ldcg(c.lengths + b);
+        const long long position = (long long)length - (long long)(last - first) + (r - first);
+        const uint32_t at = (uint32_t)position / (uint32_t)c.page_len;
+        uint32_t page = kNowhere;
+        if (r >= first && r < last && position >= 0) {  // of a request, and not in front of the sequence
+            int bad = 0;
+            if (position >= c.positions || at >= c.ld_table) {
+                bad = kErrRequest;
+            } else {
+                page = (uint32_t)__ldcg(c.table + (size_t)b * c.ld_table + at);
+                if (page >= c.pages) {
+                    page = kNowhere;
+                    bad = kErrPage;
+                }
+            }
+            if (bad && threadIdx.x == 0) atomicOr(c.error, bad);
+        }
+        if (threadIdx.x == 0) {
+            where[0] = page;
+            where[1] = (uint32_t)position;
+            where[2] = (uint32_t)position - at * (uint32_t)c.page_len;
+        }
     }
-    const uint32_t page = (uint32_t)c.table[(size_t)b * c.ld_table + at];
+    __syncthreads();
+    const uint32_t page = where[0], position = where[1];
+    const size_t inside = where[2];
+    if (page == kNowhere) return;
     const int16_t *turn = c.rope + (size_t)position * c.dim;
-    const size_t inside = (size_t)((uint32_t)position - at * (uint32_t)c.page_len);
     for (int i = threadIdx.x; i < items; i += blockDim.x) {
         if (i != (int)threadIdx.x) load(i, head, part, x0, x1);
         uint4 y0 = x0, y1 = x1;
@@ -1418,10 +1438,6 @@ __global__ void __launch_bounds__(256) k_append(const AppendCall c) {
             turn2(x0.w, x1.w, cs.w, sn.w, y0.w, y1.w);
             at0 = 8 * part;
             at1 = half + 8 * part;
-        }
-        if (page >= c.pages) {
-            if (i == 0) atomicOr(c.error, kErrPage);
-            return;
         }
         if (head < c.heads) dst = c.q + (size_t)r * c.ld_q + (size_t)head * c.dim;
         else {

@@ -14,6 +14,7 @@ GPU is an error.
 from __future__ import annotations
 
 import ctypes as C
+import importlib.util
 import os
 
 import numpy as np
@@ -75,6 +76,27 @@ class Status(C.Structure):
 
 
 _lib = None
+# What a serving loop calls at every step, by name: the functions of the module that build.py makes of
+# csrc/pycalls.c, or the library's own through ctypes.
+_calls = {}
+STEP_CALLS = ("llmx_adapters_project", "llmx_verify_drafts", "llmx_token_logprobs", "llmx_paged_append", "llmx_paged_attention")
+
+
+def _bind_calls(L):
+    path = os.path.join(HERE, "_llmxcalls.so")
+    module = None
+    if os.path.exists(path):
+        spec = importlib.util.spec_from_file_location("_llmxcalls", path)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError:  # built for another interpreter
+            module = None
+    for name in STEP_CALLS:
+        _calls[name] = getattr(L, name)
+        if module is not None:
+            module.bind(name, C.cast(getattr(L, name), C.c_void_p).value, getattr(L, name))
+            _calls[name] = getattr(module, name)
 
 
 def lib():
@@ -181,6 +203,7 @@ def lib():
             f = getattr(L, name)
             f.restype = res
             f.argtypes = args
+        _bind_calls(L)
         _lib = L
     return _lib
 
@@ -358,7 +381,7 @@ class Adapters:
         check(lib().llmx_adapters_set(self.h, slot, rank, scale, down_ptr, up_ptr, stream), "adapters_set")
 
     def project(self, x_ptr, rows, slot_ptr, out_ptr, out_format=OUT_Q8_8, ld_x=0, ld_out=0, stream=None):
-        check(lib().llmx_adapters_project(self.h, x_ptr, rows, ld_x, slot_ptr, out_ptr, out_format, ld_out, stream),
+        check(_calls["llmx_adapters_project"](self.h.value, x_ptr, rows, ld_x, slot_ptr, out_ptr, out_format, ld_out, stream),
               "adapters_project")
 
     def error(self, stream=None):
@@ -394,13 +417,13 @@ class Paged:
     def append(self, qkv_ptr, rows, offsets_ptr, lengths_ptr, requests, rope_ptr, positions, table_ptr, ld_table, k_ptr,
                v_ptr, pages, q_ptr, ld_qkv=0, ld_q=0, stream=None):
         """Rotates queries and keys of rows [q | k | v] and puts keys and values into the pages."""
-        check(lib().llmx_paged_append(self.h, qkv_ptr, rows, ld_qkv, offsets_ptr, lengths_ptr, requests, rope_ptr, positions,
+        check(_calls["llmx_paged_append"](self.h.value, qkv_ptr, rows, ld_qkv, offsets_ptr, lengths_ptr, requests, rope_ptr, positions,
                                       table_ptr, ld_table, k_ptr, v_ptr, pages, q_ptr, ld_q, stream), "paged_append")
 
     def attention(self, q_ptr, rows, offsets_ptr, lengths_ptr, requests, table_ptr, ld_table, k_ptr, v_ptr, pages, out_ptr,
                   longest=0, ld_q=0, ld_out=0, stream=None):
         """Attention of every request's rows over its pages (Task 18's arithmetic)."""
-        check(lib().llmx_paged_attention(self.h, q_ptr, rows, ld_q, offsets_ptr, lengths_ptr, requests, longest, table_ptr,
+        check(_calls["llmx_paged_attention"](self.h.value, q_ptr, rows, ld_q, offsets_ptr, lengths_ptr, requests, longest, table_ptr,
                                          ld_table, k_ptr, v_ptr, pages, out_ptr, ld_out, stream), "paged_attention")
 
     def error(self, stream=None):
@@ -420,7 +443,8 @@ def verify_drafts(target_ptr, draft_ptr, vocab, draft_tokens_ptr, offsets_ptr, r
                   temperature_ptr, accept_u_ptr, sample_u_ptr, tokens_ptr, accepted_ptr, probs_ptr, workspace_ptr,
                   workspace_bytes, ld_target=0, ld_draft=0, stream=None):
     """llmx_verify_drafts on device pointers (ints); allocates nothing."""
-    check(lib().llmx_verify_drafts(target_ptr, ld_target, draft_ptr, ld_draft, vocab, draft_tokens_ptr, offsets_ptr,
+    lib()
+    check(_calls["llmx_verify_drafts"](target_ptr, ld_target, draft_ptr, ld_draft, vocab, draft_tokens_ptr, offsets_ptr,
                                    requests, drafts, max_drafts, temperature_ptr, accept_u_ptr, sample_u_ptr,
                                    tokens_ptr, accepted_ptr, probs_ptr, workspace_ptr, workspace_bytes, stream),
           "verify_drafts")
@@ -433,7 +457,8 @@ def logprobs_workspace_bytes(rows, vocab, top):
 def token_logprobs(logits_ptr, rows, vocab, tokens_ptr, temperature_ptr, top, logprob_ptr, rank_ptr, entropy_ptr,
                    top_tokens_ptr, top_logprobs_ptr, workspace_ptr, workspace_bytes, ld=0, stream=None):
     """llmx_token_logprobs on device pointers (ints); allocates nothing."""
-    check(lib().llmx_token_logprobs(logits_ptr, ld, vocab, rows, tokens_ptr, temperature_ptr, top, logprob_ptr, rank_ptr,
+    lib()
+    check(_calls["llmx_token_logprobs"](logits_ptr, ld, vocab, rows, tokens_ptr, temperature_ptr, top, logprob_ptr, rank_ptr,
                                     entropy_ptr, top_tokens_ptr, top_logprobs_ptr, workspace_ptr, workspace_bytes, stream),
           "token_logprobs")
 

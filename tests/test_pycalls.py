@@ -1,0 +1,63 @@
+"""Calls of a serving step from Python: the module of csrc/pycalls.c beside ctypes.  No GPU needed: the
+calls are refused, by the library itself."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+COUNTS = {"llmx_adapters_project": 9, "llmx_verify_drafts": 19, "llmx_token_logprobs": 15, "llmx_paged_append": 17, "llmx_paged_attention": 16}
+
+
+@pytest.fixture(scope="module")
+def calls(llmx):
+    llmx.lib()
+    return llmx._calls
+
+
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_same_answers_as_ctypes(llmx, calls, name):
+    """None, numbers, numpy's numbers, numbers wider than their parameter, ctypes' own pointers."""
+    slow, n = getattr(llmx.lib(), name), COUNTS[name]
+    for args in ([None if t in (C.c_void_p,) else 0 for t in slow.argtypes], [0] * n):
+        assert slow(*args) == calls[name](*args)
+        detail = llmx.last_error()
+        slow(*args)
+        assert llmx.last_error() == detail
+    null = [C.c_void_p(0) if t is C.c_void_p else 0 for t in slow.argtypes]
+    assert calls[name](*null) == slow(*null)
+    assert calls[name](*[np.int64(0)] * n) == slow(*[0] * n)
+    assert calls[name](*[0 if t is C.c_void_p else 1 << 40 for t in slow.argtypes]) == slow(*[0 if t is C.c_void_p else 1 << 40 for t in slow.argtypes])
+
+
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_wrong_arguments(llmx, calls, name):
+    n = COUNTS[name]
+    with pytest.raises((TypeError, C.ArgumentError)):
+        calls[name](*[0] * (n - 1))
+    with pytest.raises((TypeError, C.ArgumentError)):
+        calls[name](*["a"] * n)
+    with pytest.raises((TypeError, C.ArgumentError)):
+        calls[name](*[1.5] * n)
+
+
+def test_arguments_arrive_in_their_places(llmx, calls):
+    """What the library says of each argument in turn."""
+    def said(name, args):
+        assert calls[name](*args) == llmx.ERR_ARG
+        return llmx.last_error()
+
+    good = [256, 0, 100, 2, 256, 256, 3, 256, 256, 256, 256, 256, 256, llmx.logprobs_workspace_bytes(2, 100, 3), None]
+    for at, value, text in ((1, 99, "stride"), (2, 0, "vocab must"), (3, 1 << 21, "rows must"), (6, 33, "top must"), (0, None, "null"),
+                            (7, None, "null pointer with tokens"), (10, None, "null pointer with top"), (12, 128, "256-byte"),
+                            (13, 1, "too small")):
+        bad = list(good)
+        bad[at] = value
+        assert text in said("llmx_token_logprobs", bad), at
+    good = [256, 0, 256, 0, 1000, 256, 256, 2, 4, 3, 256, 256, 256, 256, 256, 256, 256, 1 << 20, None]
+    for at, value, text in ((1, 999, "stride"), (3, 999, "stride"), (4, 0, "vocab must"), (7, 0, "requests must"), (8, 7, "exceeds"),
+                            (9, 1024, "max_drafts must"), (16, 128, "256-byte"), (17, 1, "too small"), (12, None, "null"), (15, 252, "aligned")):
+        bad = list(good)
+        bad[at] = value
+        assert text in said("llmx_verify_drafts", bad), at
+    for name in ("llmx_paged_append", "llmx_paged_attention", "llmx_adapters_project"):
+        assert "null handle" in said(name, [None] + [1] * (COUNTS[name] - 1))
