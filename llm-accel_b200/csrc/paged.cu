@@ -1108,7 +1108,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
 struct Places {  // in dynamic shared memory, in bytes
     int prob, exps, runs, tops, base, maxima, tv, fsum, column, queries, size;
     __host__ __device__ Places(int tiles, int cluster, int most, int dim) {
-        int at = kRing;
+        int at = kWarps * kSlice;  // (a tile a warp)
         auto place = [&](int n) {
             const int was = at;
             at += (n + 15) / 16 * 16;
@@ -1141,7 +1141,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     const int most = kOne ? 1 : c.blocks;
     const int log = c.cluster_log, cluster = 1 << log;
     const Places at(c.tiles, cluster, most, c.dim);
-    unsigned char *ring = dynamic + warp * kDepth * kSlice;
+    unsigned char *ring = dynamic + warp * kSlice;
     uint4 *queries = reinterpret_cast<uint4 *>(dynamic + at.queries), *rests = queries + most * KS * 32;
     uint32_t *score = reinterpret_cast<uint32_t *>(dynamic + at.prob);  // [tiles][most][64 positions][4 pairs], then the probabilities
     const int16_t *exps = reinterpret_cast<const int16_t *>(dynamic + at.exps);
@@ -1173,9 +1173,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     // ---- scores
     const Share share(c.dim, warp);
     int fetched = share.first;
-    auto fetch = [&](int slot) {
+    auto fetch = [&]() {
         if (fetched < own) {
-            fetch_values(c, z, t0 + fetched, share.part, ring + slot * kSlice, worst);
+            fetch_values(c, z, t0 + fetched, share.part, ring, worst);
             fetched += share.step;
         }
         commit();
@@ -1190,8 +1190,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
         }
         pages.load(c, z, p0 + kTile, worst);
         stage_queries<KS>(c, z, warp, kWarps, queries, rests, column);
-#pragma unroll
-        for (int i = 0; i < kDepth; i++) fetch(i);
+        fetch();
         // whether the whole call is within what the handle was made for
         int sum = 0;
         for (uint32_t i = threadIdx.x; i < c.requests; i += kThreads) {
@@ -1276,14 +1275,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     // ---- values
     const uint32_t values = owner(at.tv, g) + (uint32_t)(share.part * 64 + 4 * t4);
 #pragma unroll 1
-    for (int k = share.first, i = 0; k < own; k += share.step, i ^= 1) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    for (int k = share.first; k < own; k += share.step) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
         __syncwarp();
         Planes v;
-        const bool limit = v.load<false>(ring + i * kSlice);
-        if (limit) v.load<true>(ring + i * kSlice);
+        const bool limit = v.load<false>(ring);
+        if (limit) v.load<true>(ring);
         __syncwarp();
-        fetch(i);
+        fetch();
         for (int nb = 0; nb < (kOne ? 1 : z.blocks); nb++) {
             const uint4 *p = reinterpret_cast<const uint4 *>(score) + (k * most + nb) * 64 + place_of(lane), b2[2] = {p[0], p[32]};
             uint32_t y[4];
