@@ -1538,16 +1538,17 @@ struct Clusters {
     uint64_t ctas = 0;
     int log = 0, tiles = 0, blocks = 0, smem = 0;
 };
-// Microseconds as measured (16 query heads, 2 key heads of 128; 1 to 64 requests of 64 to 16000 positions): a
-// cluster's turn takes 5.3 and 1.5 per tile of a CTA, more by 0.34 of it for each further column block and
-// by 0.6 of it for each CTA an SM has (0.9 with several blocks); the three launches 11.5, 1.1 per further block and 1.15 per
-// tile an SM has (more by 0.5 of it per further block).  Requests are taken to be 0.6 as long as the
-// longest, on average.  64 x 1024: 23.7 by clusters of 4, 31.4 of 8, 27.5 by three launches; one of
-// 2048: 11.4 and 12.3, of 4096 17.7 and 14.5; 64 x 2048 50.5 and 45.0.
+// Microseconds as measured (16 query heads, 2 key heads of 128; 1 to 64 requests of 64 to 8192 positions, even
+// and ragged, 1 and 4 rows).  A turn of clusters takes 5.2 and 1.45 per tile of a CTA, and 0.72 more per tile for
+// each CTA that shares its SM (0.55 with its request's columns in several clusters, 0.43 with several column
+// blocks a cluster), all of the latter more by 0.68 for each further block.  There are as many turns as it takes SMs that hold 4 CTAs, or what their memory
+// allows; the later ones are taken to be half as long.  The three launches take 11.5, 1.3 per further
+// block and 1.15 per tile an SM has (more by 0.52 of it per further block), with requests 0.8 as long
+// as the longest.  64 x 1024: 19.7 by clusters of 4, 26.6 of 8, 27.6 by three launches; 64 up to 2048:
+// 35.3, 26.1 and 30.6; one of 2048 11.0 (of 8) and 12.2, of 4096 17.5 and 14.5; 64 x 4096 85 and 76.5.
 Clusters choose(const llmx_paged *p, uint64_t strips, int all, int most) {
-    constexpr double kLoad = 0.6;
     Clusters best;
-    double least = 11.5 + 1.1 * (most - 1) + 1.15 * kLoad * (double)strips * all / p->sms * (1 + 0.5 * (most - 1));
+    double least = 11.5 + 1.3 * (most - 1) + 1.15 * 0.8 * (double)strips * all / p->sms * (1 + 0.52 * (most - 1));
     if (all > kShortTiles) return best;
     for (int log = 0; log <= 3; log++) {
         const int cluster = 1 << log, tiles = (all + cluster - 1) / cluster;
@@ -1557,8 +1558,11 @@ Clusters choose(const llmx_paged *p, uint64_t strips, int all, int most) {
             if (blocks > 1 && (most + blocks - 2) / (blocks - 1) == groups) continue;  // no fewer groups for more blocks
             const Places at(tiles, cluster, blocks, p->dim);
             if (at.size > kMaxSmem) continue;
-            const double ctas = kLoad * (double)strips * cluster * groups, room = (double)p->sms * std::min(4, kSmemOfSm / (at.size + 2048));
-            const double us = 5.3 * std::ceil(ctas / room) + 1.5 * tiles * (1 + 0.34 * (blocks - 1)) * (1 + (blocks > 1 ? 0.9 : 0.6) * ctas / p->sms);
+            const double each = (double)strips * cluster * groups / p->sms, room = std::min(4, kSmemOfSm / (at.size + 2048));
+            const double work = std::max(1.0, (double)all / cluster) * (1 + 0.68 * (blocks - 1));
+            const double turn = work * (1.45 + (blocks > 1 ? 0.43 : groups > 1 ? 0.55 : 0.72) * std::min(each, room));
+            const double turns = blocks == 1 && groups > 1 ? each / room : std::ceil(each / room);
+            const double us = 5.2 + turn + (std::max(1.0, turns) - 1) * (5.2 + turn / 2);
             if (us < least) {
                 least = us;
                 best.ctas = strips * cluster;
