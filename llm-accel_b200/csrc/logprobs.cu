@@ -236,38 +236,44 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
             const int top = __reduce_max_sync(0xffffffffu, most);
             if (lane == 0) c.maxima[(size_t)r * c.chunks + chunk + n] = top;
             if (top == kExcluded) continue;
-            if (top > m || !far) {
-                int skip = -1;  // the maximum that is left out of the sums
-                if (top > m) {
-                    if (!greedy && m != kExcluded) {  // the old maximum becomes an ordinary token
-                        const float d = (float)((uint32_t)top - (uint32_t)m);
-                        const float e = fmaf(d, s_hi, d * s_lo), f = exp2f(e);
-                        if (lane == 0) rest += 1.0f;  // (it is 0 away from itself)
-                        sum = f * fmaf(rest, e, sum);
-                        rest *= f;
-                    }
-                    m = top;
-                    far = (float)((uint32_t)m ^ 0x80000000u) * s_hi < -150.0f;
-                    const uint32_t who = __ballot_sync(0xffffffffu, most == top);
-                    if (lane == __ffs(who) - 1) {
+            if (top >= mine && mine != kExcluded) {
+                const uint32_t first = i0 + 4 * lane;
+                if (place - i0 < (uint32_t)kChunk) {
 #pragma unroll
-                        for (int i = 15; i >= 0; i--)
-                            if (z[i] == top) skip = i;
-                    }
-                }
-                if (!greedy) {
-                    float r16 = 0, s16 = 0;
+                    for (int i = 0; i < 16; i++) ahead += z[i] > mine || (z[i] == mine && first + 128 * (i / 4) + i % 4 < place);
+                } else {
+                    const int over = place < i0 ? mine : mine - 1;  // in front of the token equal ones are ahead
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const float d = (float)((uint32_t)m - (uint32_t)z[i]), e = fmaf(d, s_hi, d * s_lo);
-                        const float x = z[i] == kExcluded || i == skip ? 0.0f : exp2_fast(e);
-                        r16 += x;
-                        s16 = fmaf(x, e, s16);
-                    }
-                    rest += r16;
-                    sum += s16;
+                    for (int i = 0; i < 16; i++) ahead += z[i] > over;
                 }
-            } else {
+            }
+            if (greedy) {
+                m = max(m, top);
+                continue;
+            }
+            if (top > m) {
+                if (m != kExcluded) {  // the old maximum becomes an ordinary token
+                    const float d = (float)((uint32_t)top - (uint32_t)m);
+                    const float e = fmaf(d, s_hi, d * s_lo), f = exp2f(e);
+                    if (lane == 0) rest += 1.0f;  // (it is 0 away from itself)
+                    sum = f * fmaf(rest, e, sum);
+                    rest *= f;
+                }
+                m = top;
+                far = (float)((uint32_t)m ^ 0x80000000u) * s_hi < -150.0f;
+                // The new one stays out: one lane takes those that it has for excluded and counts all but one.
+                const uint32_t who = __ballot_sync(0xffffffffu, most == top);
+                const bool here = lane == __ffs(who) - 1;
+                const int gone = here ? top : kExcluded;
+                int count = 0;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    count += z[i] == gone;
+                    z[i] = z[i] == gone ? kExcluded : z[i];
+                }
+                if (here) rest += (float)(count - 1);
+            }
+            if (far) {
                 f32x2 r2 = 0, s2 = 0;
 #pragma unroll
                 for (int i = 0; i < 16; i += 2) {
@@ -284,17 +290,17 @@ __global__ void __launch_bounds__(kThreads, 3) k_rows(const Call c) {
                 rest += a + b;
                 unpack2(s2, a, b);
                 sum += a + b;
-            }
-            if (top >= mine && mine != kExcluded) {
-                const uint32_t first = i0 + 4 * lane;
-                if (place - i0 < (uint32_t)kChunk) {
+            } else {
+                float r16 = 0, s16 = 0;
 #pragma unroll
-                    for (int i = 0; i < 16; i++) ahead += z[i] > mine || (z[i] == mine && first + 128 * (i / 4) + i % 4 < place);
-                } else {
-                    const int over = place < i0 ? mine : mine - 1;  // in front of the token equal ones are ahead
-#pragma unroll
-                    for (int i = 0; i < 16; i++) ahead += z[i] > over;
+                for (int i = 0; i < 16; i++) {
+                    const float d = (float)((uint32_t)m - (uint32_t)z[i]), e = fmaf(d, s_hi, d * s_lo);
+                    const float x = z[i] == kExcluded ? 0.0f : exp2_fast(e);
+                    r16 += x;
+                    s16 = fmaf(x, e, s16);
                 }
+                rest += r16;
+                sum += s16;
             }
         }
         ahead = __reduce_add_sync(0xffffffffu, ahead);
