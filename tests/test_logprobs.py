@@ -277,3 +277,63 @@ def test_graph_streams_and_repeats(llmx, torch):
         b.call(s2.cuda_stream)
     a.check()
     b.check()
+
+
+@gpu
+def test_offsets_beyond_32_bits(llmx, torch):
+    """Rows that lie 2^27 elements apart, the last ones behind 2^31."""
+    rng = np.random.default_rng(8)
+    ld, rows, vocab = 2**27 + 1, 19, 700
+    z = logits(rng, rows, vocab)
+    tokens = draw_tokens(rng, z)
+    d = Device(llmx, torch, z, tokens, None, 5)
+    big = torch.empty((rows - 1) * ld + vocab, dtype=torch.int32, device="cuda")
+    for r in range(rows):
+        big[r * ld:r * ld + vocab] = torch.from_numpy(z[r]).cuda()
+    d.logits, d.at, d.ld = big, big.data_ptr(), ld
+    d.call()
+    d.check()
+
+
+@gpu
+@pytest.mark.parametrize("vocab,rows", [(2**22, 3), (1, 2000), (5, 20000)])
+def test_largest(llmx, torch, vocab, rows):
+    rng = np.random.default_rng(9)
+    z = rng.integers(-(2**19), 2**19, (rows, vocab)).astype(np.int32)
+    check(llmx, torch, z, rng.integers(0, vocab, rows).astype(np.uint32), None, 3)
+
+
+@gpu
+def test_of_verified_tokens(llmx, torch):
+    """What the verification of drafts leaves, asked for at once: the rows' tokens go from one call to the
+    next on the device, in one graph."""
+    import test_verify as V
+    rng = np.random.default_rng(10)
+    counts, vocab = [3, 0, 4, 1], 20011
+    for temperature in (0.0, 1.0):
+        c = V.make(rng, counts, vocab, temperature=[temperature] * 4)
+        v = V.Device(llmx, torch, c)
+        most, rows = c["most"], len(c["target"])
+        where = torch.tensor([r * (most + 1) + j for r, k in enumerate(counts) for j in range(k + 1)], device="cuda")
+        d = Device(llmx, torch, c["target"], np.zeros(rows, np.uint32), None, 4)
+
+        def step():
+            v.call()
+            d.d_tokens.copy_(v.out[where])
+            d.call()
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        for _ in range(2):
+            d.d_tokens.fill_(1)
+            graph.replay()
+            tokens = v.check()[0]  # (requests, most + 1), 0xffffffff behind the drawn one
+            d.tokens = tokens.reshape(-1)[where.cpu().numpy()]
+            got, _ = d.check()
+            drawn = d.tokens != NO_TOKEN
+            assert drawn.sum() >= len(counts) and (got["rank"][~drawn] == NO_TOKEN).all()
+            if temperature == 0:  # an accepted draft and a drawn token are the rows' maxima
+                assert (got["rank"][drawn] == 0).all()

@@ -591,3 +591,127 @@ def test_attention_sublayer_of_many_requests(llmx, torch, shape):
             assert np.array_equal(pool.cpu().numpy()[table[r][pos // page], :, pos % page].transpose(1, 0, 2), cache)
     for h in (a, o, p, *contexts):
         h.close()
+
+
+@gpu
+def test_rows_in_front_of_the_first_request(llmx, torch, oracle):
+    """offsets[0] above 0: rows in front of the first request's are left as they are, as those behind the last."""
+    rng = np.random.default_rng(19)
+    c = Case(rng, [(2, 100), (0, 5), (3, 77)], 8, 2, 32, pad=9)
+    want = c.want(oracle)
+    d = Device(llmx, torch, c)
+    d.offsets += 4
+    d.q = torch.roll(d.q, 4, 0)
+    d.call()
+    got = d.result()
+    assert (got[:4] == FILL).all() and np.array_equal(got[4:], want[:-4])
+    rope = llmx.rope_table(32, 100)
+    x = rng.integers(-32768, 32767, (c.rows, 12 * 32)).astype(np.int16)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    dx, dr, dk, dv = dev(x), dev(rope), dev(c.k), dev(c.v)
+    q = torch.full((c.rows, 256), FILL, dtype=torch.int16, device="cuda")
+    d.p.append(dx.data_ptr(), c.rows, d.offsets.data_ptr(), d.lengths.data_ptr(), 3, dr.data_ptr(), 100, d.table.data_ptr(), c.table.shape[1],
+               dk.data_ptr(), dv.data_ptr(), c.pages, q.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    d.p.error()
+    k, v = c.k.copy(), c.v.copy()
+    out = np.full((c.rows, 256), FILL, np.int16)
+    for b, (rows, length) in enumerate(c.plan):
+        for j in range(rows):
+            r, p = 4 + int(c.offsets[b]) + j, length - rows + j
+            turned = rotate(x[r].reshape(12, 32)[:10], rope[p])
+            out[r] = turned[:8].reshape(-1)
+            k[c.table[b, p // 16], :, p % 16] = turned[8:]
+            v[c.table[b, p // 16], :, p % 16] = x[r].reshape(12, 32)[10:]
+    assert np.array_equal(q.cpu().numpy(), out) and np.array_equal(dk.cpu().numpy(), k) and np.array_equal(dv.cpu().numpy(), v)
+
+
+@gpu
+def test_append_beyond_32_bits(llmx, torch):
+    """Pages whose first element lies beyond 2^31 elements."""
+    page, kv, hd = 64, 2, 128
+    per = kv * page * hd
+    pages = 2**31 // per + 20
+    rng = np.random.default_rng(20)
+    c = Case(rng, [(5, 200), (100, 130)], 4, kv, hd, page)
+    rope = llmx.rope_table(hd, 200)
+    x = rng.integers(-32768, 32767, (c.rows, 8 * hd)).astype(np.int16)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    where = pages - c.pages + np.arange(c.pages)
+    table = c.table.copy()
+    table[:, :-1] = np.where(table[:, :-1] >= 0, table[:, :-1] + pages - c.pages, -1)
+    big = [torch.zeros((pages, kv, page, hd), dtype=torch.int16, device="cuda") for _ in range(2)]
+    dx, dr, dt = dev(x), dev(rope), dev(table)
+    do, dl = dev(c.offsets.view(np.int32)), dev(c.lengths.view(np.int32))
+    q = torch.empty((c.rows, 4 * hd), dtype=torch.int16, device="cuda")
+    p = llmx.Paged(4, kv, hd, page, 2, 1, 200, 400)
+    p.append(dx.data_ptr(), c.rows, do.data_ptr(), dl.data_ptr(), 2, dr.data_ptr(), 200, dt.data_ptr(), table.shape[1], big[0].data_ptr(),
+             big[1].data_ptr(), pages, q.data_ptr(), stream=torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    p.error()
+    k, v = np.zeros_like(c.k), np.zeros_like(c.v)
+    for b, (rows, length) in enumerate(c.plan):
+        for j in range(rows):
+            r, at = int(c.offsets[b]) + j, length - rows + j
+            row = x[r].reshape(8, hd)
+            k[c.table[b, at // page], :, at % page] = rotate(row[4:6], rope[at])
+            v[c.table[b, at // page], :, at % page] = row[6:]
+    for got, want in zip(big, (k, v)):
+        assert np.array_equal(got[torch.from_numpy(where).cuda()].cpu().numpy(), want)
+        assert not got[:pages - c.pages].any()
+
+
+@gpu
+def test_decoding_in_one_graph(llmx, torch, oracle):
+    """Append and attention captured together and replayed token by token, the lengths counted on the device:
+    every request's rows are those of the oracle on the cache so far."""
+    rng = np.random.default_rng(21)
+    heads, kv, hd, page, steps, most = 8, 2, 64, 16, 40, 130
+    start = np.array([0, 1, 15, 60, 90], np.int32)
+    b = len(start)
+    width = -(-most // page)
+    table = rng.permutation(b * width).astype(np.int32).reshape(b, width)
+    dev = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    pools = [rng.integers(-600, 600, (b * width, kv, page, hd)).astype(np.int16) for _ in range(2)]
+    dk, dv, dt, dl = dev(pools[0]), dev(pools[1]), dev(table), dev(start)
+    do = torch.arange(b + 1, dtype=torch.int32, device="cuda")
+    rope = llmx.rope_table(hd, most)
+    dr = dev(rope)
+    qkv = torch.zeros((b, (heads + 2 * kv) * hd), dtype=torch.int16, device="cuda")
+    out = torch.zeros((b, heads * hd), dtype=torch.int16, device="cuda")
+    p = llmx.Paged(heads, kv, hd, page, b, 1, most, b * most)
+
+    def step():
+        s = torch.cuda.current_stream().cuda_stream
+        dl.add_(1)
+        p.append(qkv.data_ptr(), b, do.data_ptr(), dl.data_ptr(), b, dr.data_ptr(), most, dt.data_ptr(), width, dk.data_ptr(), dv.data_ptr(),
+                 b * width, qkv.data_ptr(), ld_q=qkv.shape[1], stream=s)
+        p.attention(qkv.data_ptr(), b, do.data_ptr(), dl.data_ptr(), b, dt.data_ptr(), width, dk.data_ptr(), dv.data_ptr(), b * width,
+                    out.data_ptr(), ld_q=qkv.shape[1], stream=s)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    dl.copy_(dev(start))
+    dk.copy_(dev(pools[0]))
+    dv.copy_(dev(pools[1]))
+    for n in range(steps):
+        x = np.clip(np.rint(rng.normal(0, 500, qkv.shape)), -32768, 32767).astype(np.int16)
+        qkv.copy_(dev(x))
+        graph.replay()
+        got = out.cpu().numpy().reshape(b, heads, hd)
+        for r in range(b):
+            at = int(start[r]) + n
+            row = x[r].reshape(-1, hd)
+            turned = rotate(row[:heads + kv], rope[at])
+            page_at = table[r, at // page]
+            pools[0][page_at, :, at % page], pools[1][page_at, :, at % page] = turned[heads:], row[heads + kv:]
+            pos = np.arange(at + 1)
+            k, v = (pool[table[r][pos // page], :, pos % page] for pool in pools)
+            for h in range(kv):
+                g = heads // kv
+                want = oracle.attention_group(turned[h * g:(h + 1) * g], k[:, h], v[:, h])
+                assert np.array_equal(got[r, h * g:(h + 1) * g], want), (n, r, h)
+    p.error()
