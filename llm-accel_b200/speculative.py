@@ -8,7 +8,8 @@ its request's adapter (llmx_adapters_project, Q16.16 logits), and the drafts are
 verified and a next token drawn for all of them (llmx_verify_drafts).  Drafts are
 copied from the request's own text: what followed the last two tokens
 when they last occurred.  Rows of rejected drafts leave nothing behind: the next block
-starts at the first position that was not accepted and overwrites their K/V.
+starts at the first position that was not accepted and overwrites their K/V.  Where they
+are asked for, the tokens' log probabilities come from the same logits (llmx_token_logprobs).
 
 Every request has a context, so a K/V cache, of its own; the contexts hold
 the same weights.  Needs torch for the device arrays.
@@ -74,6 +75,7 @@ class Server:
         self.tokens, self.accepted = new((requests, drafts + 1), torch.int32), new((requests,), torch.int32)
         size = llmx.verify_workspace_bytes(requests, requests * drafts, self.s.vocab)
         self.work = new((size,), torch.uint8)
+        self.report = None  # of the log probabilities, once they are asked for
         torch.cuda.synchronize(self.dev)
 
     def close(self):
@@ -106,8 +108,32 @@ class Server:
         here.wait_stream(self.torch.cuda.ExternalStream(c.stream, device=self.dev))
         self.x[row:row + n].view(-1).copy_(_view(self.torch, c.hidden_ptr(0), n * self.s.hidden, self.dev))
 
-    def generate(self, prompts, slots, max_new, temperature=0.0, seed=0):
-        """New tokens of every request, and (drafted, accepted) over all of them."""
+    def _logprobs(self, offsets, top):
+        """Of the tokens that verify_drafts just left, at temperature 1: arrays logprob, rank and entropy of every
+        row of the logits, and the `top` most likely tokens with theirs; also each request's first row."""
+        t, rows = self.torch, offsets[-1] + len(offsets) - 1
+        if self.report is None or self.report[0].numel() < llmx.logprobs_workspace_bytes(self.rows, self.s.vocab, top):
+            new = lambda shape, kind: t.zeros(shape, dtype=kind, device=self.dev)  # noqa: E731
+            self.report = (new((llmx.logprobs_workspace_bytes(self.rows, self.s.vocab, top),), t.uint8),
+                           t.full((self.rows,), 1 / self.logit_step, device=self.dev))
+        work, temperature = self.report
+        # token j of request r was drawn from row offsets[r] + r + j
+        first = [o + r for r, o in enumerate(offsets)]
+        where = [r * (self.drafts + 1) + j for r in range(len(offsets) - 1) for j in range(first[r + 1] - first[r])]
+        drawn = self.tokens.view(-1)[t.tensor(where, device=self.dev)]
+        out = [t.empty(n, dtype=kind, device=self.dev) for n, kind in
+               ((rows, t.float32), (rows, t.int32), (rows, t.float32), ((rows, top), t.int32), ((rows, top), t.float32))]
+        p = lambda a: a.data_ptr() if a.numel() else None  # noqa: E731
+        llmx.token_logprobs(self.logits.data_ptr(), rows, self.s.vocab, drawn.data_ptr(), temperature.data_ptr(), top, *map(p, out),
+                            work.data_ptr(), work.numel(), stream=self.stream())
+        return [a.cpu().numpy() for a in out], first
+
+    def generate(self, prompts, slots, max_new, temperature=0.0, seed=0, logprobs=None):
+        """New tokens of every request, and (drafted, accepted) over all of them.  With logprobs = n (0 to 32)
+        also, for every new token, (log probability, rank, entropy of its row, the n most likely
+        tokens as (token, log probability)): of the logits at temperature 1, whatever the tokens are drawn at."""
+        if logprobs is not None and not 0 <= logprobs <= 32:
+            raise ValueError("logprobs must be 0..32 (the most likely tokens beside each), or None")
         t, count = self.torch, len(prompts)
         if count != len(self.contexts):
             raise ValueError(f"{count} prompts for {len(self.contexts)} requests")
@@ -125,6 +151,7 @@ class Server:
         dev = lambda a: t.from_numpy(np.ascontiguousarray(a).view(np.int32)).to(self.dev)  # noqa: E731
         temperatures = t.full((count,), float(temperature) / self.logit_step, device=self.dev)
         drafted = taken = 0
+        told = [[] for _ in texts]
         while any(len(x) < g for x, g in zip(texts, goal)):
             guesses, offsets, row, owners = [], [0], 0, []
             for r, text in enumerate(texts):
@@ -143,13 +170,22 @@ class Server:
             llmx.verify_drafts(self.logits.data_ptr(), None, self.s.vocab, p(d_guess), p(d_offsets), count, len(guesses), self.drafts,
                                p(temperatures), p(d_accept), p(d_sample), p(self.tokens), p(self.accepted), None, p(self.work),
                                self.work.numel(), stream=self.stream())
+            if logprobs is not None:
+                (lp, rank, entropy, ids, others), first = self._logprobs(offsets, logprobs)
             # nothing is made of rows or logits that a kernel gave up
             self.head.error(self.stream())
             for c in self.contexts:
                 c.synchronize()
             drafted += sum(offsets[r + 1] - offsets[r] for r, text in enumerate(texts) if len(text) < goal[r])
+            was = [len(text) for text in texts]
             taken += append_tokens(texts, goal, self.tokens.cpu().numpy(), self.accepted.cpu().numpy())
-        return [text[len(q):] for text, q in zip(texts, prompts)], (drafted, taken)
+            if logprobs is not None:
+                for r, text in enumerate(texts):
+                    for row in range(first[r], first[r] + len(text) - was[r]):
+                        told[r].append((float(lp[row]), int(rank[row]), float(entropy[row]),
+                                        list(zip(ids[row].tolist(), others[row].tolist()))))
+        out = [text[len(q):] for text, q in zip(texts, prompts)]
+        return (out, (drafted, taken)) if logprobs is None else (out, (drafted, taken), told)
 
 
 def _view(torch, pointer, count, device):

@@ -165,3 +165,40 @@ def test_each_request_gets_its_own_adapter(llmx):
             assert out == want
             assert (taken > 0) == (drafts > 0)
         sv.close()
+
+
+@pytest.mark.parametrize("untied", [False, True])
+def test_log_probabilities(llmx, untied):
+    """The tokens' log probabilities: those of the logits that they were drawn from, the same ones with and
+    without drafts, and the tokens those of a call that does not ask for them."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    import test_logprobs as T
+    model = llmx.Model(llmx.shape("small")).init_gaussian(11, lm_head=untied)
+    told = []
+    for drafts in (0, 4):
+        sv = server(spec, model, drafts)
+        plain = sv.generate(PROMPTS, [0, -1, 1], 9)
+        out, counts, report = sv.generate(PROMPTS, [0, -1, 1], 9, logprobs=3)
+        assert (out, counts) == plain
+        assert [len(r) for r in report] == [9, 9, 9]
+        for text, mine in zip(out, report):
+            for token, (logprob, rank, entropy, best) in zip(text, mine):
+                assert rank == 0 and best[0] == (token, logprob) and len(best) == 3 and entropy >= 0
+        told.append([x for r in report for x in r])
+        # one step, whose logits are still there
+        out, _, report = sv.generate(PROMPTS, [0, -1, 1], 1, temperature=1.0, seed=3, logprobs=2)
+        z = sv.logits[:3].cpu().numpy()
+        tokens = np.array([o[0] for o in out], np.uint32)
+        want = T.oracle(z, tokens, np.full(3, 1 / sv.logit_step, np.float32), 2)
+        for r in range(3):
+            logprob, rank, entropy, best = report[r][0]
+            log, total = T.bounds(want["terms"][r], 1)
+            near = lambda got, w, room: abs(got - w) <= room + abs(w) * 2.0**-24  # noqa: E731
+            assert rank == want["rank"][r] and near(logprob, want["logprob"][r], log) and near(entropy, want["entropy"][r], total)
+            assert [t for t, _ in best] == want["top_tokens"][r].tolist()
+        with pytest.raises(ValueError):
+            sv.generate(PROMPTS, [0, -1, 1], 1, logprobs=33)
+        sv.close()
+    assert model.shape.vocab <= 509  # a row is one warp's, whatever rows there are: the same bits
+    assert told[0] == told[1]
