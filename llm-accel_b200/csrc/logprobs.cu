@@ -342,15 +342,22 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     __shared__ uint32_t aheads[kWarps], found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) found = 0;
-    pdl_wait();
-    pdl_trigger();
     const uint32_t r = blockIdx.x;
     const int32_t *row = c.logits + (size_t)r * c.ld;
+    // This launch starts once every CTA of k_rows has waited for what is before it, so that the call's arguments can be
+    // read, through the L2, before its own wait.
+    const float temperature = c.temperature ? __ldcg(c.temperature + r) : 1.0f;
+    const uint32_t token = c.tokens ? __ldcg(c.tokens + r) : kNone;
+    const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
+    const bool greedy = is_greedy(temperature);
+    const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature, step = greedy ? 0.0 : 1.0 / (65536.0 * (double)temperature);
     // the warps of k_rows that had a share of this row
     const unsigned long long first = (unsigned long long)r * c.chunks / c.per, last = ((unsigned long long)(r + 1) * c.chunks - 1) / c.per;
     const int parts = (int)(last - first + 1);
     const Part *part = c.parts + first + r;
     const int32_t *maxima = c.maxima + (size_t)r * c.chunks;
+    pdl_wait();
+    pdl_trigger();
     // (all loads are on their way before the first is used)
     const Part mine_part = (int)threadIdx.x < parts ? part[threadIdx.x] : Part{kExcluded, 0, 0, 0};
     auto key_at = [&](uint32_t i) -> unsigned long long {
@@ -358,11 +365,6 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
         return z == kExcluded ? 0 : key_of(z, i);
     };
     const unsigned long long key0 = key_at(threadIdx.x), key1 = key_at(kThreads + threadIdx.x);
-    const float temperature = c.temperature ? c.temperature[r] : 1.0f;
-    const uint32_t token = c.tokens ? c.tokens[r] : kNone;
-    const int mine = token < c.vocab ? __ldcg(row + token) : kExcluded;
-    const bool greedy = is_greedy(temperature);
-    const double scale = greedy ? 0.0 : 1.4426950408889634 / 65536.0 / (double)temperature;
     // The best chunks.
     unsigned long long list;
     if (c.top <= 1) {  // the best one: maxima of keys
@@ -462,7 +464,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     if (greedy || m == kExcluded) all_with = 0;
     rest = all_rest + (double)all_with;
     sum = all_sum;
-    const double log_sum = log1p(rest), step = greedy ? 0.0 : 1.0 / (65536.0 * (double)temperature);
+    const double log_sum = log1p(rest);
     // of a token that is not excluded
     auto logprob = [&](int z, bool ahead_of_all) -> float {
         if (greedy) return ahead_of_all ? 0.0f : -INFINITY;
