@@ -462,10 +462,12 @@ int llmx_verify_drafts(const int32_t *target, size_t ld_target, const int32_t *d
  *   entropy    = log1p(rest) + sum of d_v exp(-d_v) / (1 + rest)            nats
  *   rank(v)    = the number of tokens ahead of v in the order (logit down, index up)
  * INT32_MIN excludes a token; T <= 1e-6 (or NaN) leaves the first maximum alone (its log probability
- * is 0, all others' -infinity, the entropy 0).  Terms are binary32 with whole-number
- * differences, added in a fixed order (16 at a time, a lane's and a warp's sums in binary32, those
- * of a row in binary64), the formulas binary64: results are within 4e-7 of the
- * entropy and max(1, |logprob|), and do not depend on the rows beside them in more than that.
+ * is 0, all others' -infinity, the entropy 0).  Terms are binary32 with whole-number differences (each within
+ * 2^-22 + 2^-23 d of itself; below 2^-126 it is 0), added in a fixed order: 16 at a time, a lane's and a
+ * warp's sums in binary32, those of a row in binary64, as are the formulas.  Measured at vocabularies of
+ * 32003 to 2^22 and temperatures of 0.3 to 3 against binary64: log probabilities are off by up to 6e-8 of themselves
+ * or of 1, entropies by up to 1.4e-7.  A row's last bits may depend on how many rows the call has and
+ * how they are aligned, on nothing else.
  * ------------------------------------------------------------------------- */
 /* Bytes of workspace for a call of these sizes. */
 size_t llmx_logprobs_workspace_bytes(uint32_t rows, uint32_t vocab, uint32_t top);

@@ -6,15 +6,21 @@
 // host/host_qwen_8x64.cpp:3610-3739, rotation rotate_fix16_pair_with_quantized_rope
 // host:4765-4788.  The reference has one sequence with one contiguous cache.
 //
-// Attention is three launches over the requests' 64-position tiles.
-//   k_scores  QK: scores (int16) and each tile's maximum;
-//   k_values  the running maximum is the prefix maximum of the tiles' maxima, so a
-//             tile's probabilities and its values tv (int16) need nothing else of the
-//             tiles before it;
-//   k_join    replays the recurrence of (sum, acc), which rounds at every tile, in
-//             order, and divides.
-// So the cache's length is split over as many CTAs as there are tiles, and nothing
-// waits for anything but a launch.
+// Attention takes a request's 64-position tiles through three steps, of which only the last goes tile by tile.
+//   scores  QK: scores (int16) and each tile's maximum;
+//   values  the running maximum is the prefix maximum of the tiles' maxima, so a tile's probabilities
+//           and its values tv (int16) need nothing else of the tiles before it;
+//   join    replays the recurrence of (sum, acc), which rounds at every tile, in order, and
+//           divides.  Between tiles that raise the maximum it only adds.
+// So a request's length is split over as many warps as it has tiles.  There are two ways, between which
+// choose() decides by what both were measured to take:
+//   k_attend                     one launch, a cluster of up to 8 CTAs per (request, key head), everything
+//                                in shared memory.  For few or short texts, which latency bounds: one request
+//                                of 513 positions 7.7 us (three launches 11.1), 64 of up to 2304 29.8 (34).
+//   k_scores, k_values, k_join   one launch each over all tiles, scores and tv through the L2.  For many long
+//                                texts, which HBM and instructions bound, and for one that is longer
+//                                than a cluster can hold: 64 requests of 8192 positions 133 us for 537 MB of
+//                                keys and values (4.0 TB/s; a copy alone would take 82), one of 32768 28.5.
 //
 // Products are formed by int8 matrix instructions, exactly.  A product is
 // rnd4(x sat16(16 y)) with y the cached value: with c = y limited to [-2048, 2048]
@@ -494,7 +500,10 @@ static __device__ __forceinline__ void score_tile(const Call &c, const Strip &z,
     }
 }
 
-// One CTA's run of tiles, a warp per 16 positions.
+// One CTA's run of tiles, a warp per 16 positions: the 16 rows of A, loaded straight from HBM as its lanes
+// hold them, two tiles ahead in registers; the queries are B.  Four CTAs an SM by registers.  64 x 8192:
+// 54 us, 278 MB at 5.1 TB/s (78 % of a copy), 50 % of the issue slots and 53 % of the ALU (splitting keys into
+// bytes); five CTAs with the planes formed step by step 55.6.
 template <int KS, bool kOne>  // steps of 32 dimensions; one column block
 __global__ void __launch_bounds__(kThreads, 4) k_scores(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -716,7 +725,9 @@ struct Share {
 
 // One CTA's run of tiles, in chunks of up to kChunk: their probabilities, by all warps, through shared
 // memory (two buffers in turn, so one barrier a chunk does); then every warp weighs its 32 elements
-// of every tile, for itself.
+// of every tile, for itself, from a ring of two tiles that cp.async fills.  64 x 8192: 65 us at 4.4 TB/s, 41 %
+// of the issue slots: latency (loads, barriers, shared memory) with the 16 warps an SM that registers leave;
+// five CTAs with one buffer of probabilities 27 us more, starting before k_scores' end no less.
 template <bool kOne>
 __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -972,7 +983,8 @@ struct Stretch {
 // tiles that raise the maximum (whose factor is not 1: few in a long text) the recurrence only adds,
 // so a warp gives what its tiles do to any value that comes in as a few stretches, and the first
 // warp, which starts from 0, puts them together; tiles beyond a warp's kMaxStretches it goes
-// through itself, and a stretch on which something might saturate tile by tile.
+// through itself, and a stretch on which something might saturate tile by tile.  Tile by tile throughout
+// it took 224 us of a request of 32768 positions, so 10; 64 x 8192: 66 before, 13 now, 34 MB from the L2.
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -1104,7 +1116,8 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
 // A cluster of CTAs per (request, key head), each with an equal part of its tiles, goes through the
 // three steps with everything in shared memory: scores, the maxima of the CTAs before from these,
 // probabilities (in place of the scores), values, which go to the CTA that has their column, and the
-// recurrence there.
+// recurrence there.  Latency bounds it (issue slots 25 to 29 %): two meetings of the cluster, keys before values,
+// and at 64 requests of up to 2304 positions 1024 CTAs in two turns, 29.8 us for 71 MB.
 struct Places {  // in dynamic shared memory, in bytes
     int prob, exps, runs, tops, base, maxima, tv, fsum, column, queries, size;
     __host__ __device__ Places(int tiles, int cluster, int most, int dim) {
@@ -1374,7 +1387,8 @@ static __device__ __forceinline__ void turn2(uint32_t x0, uint32_t x1, uint32_t 
 
 // A CTA per row; a thread turns 8 pairs (i, i + dim/2) of a head, or copies 16 values.  The row's own values are on
 // their way while its request, its position, and by that its page and its turn are looked up, one after
-// another: that is what a row takes.
+// another: that is what a row takes.  8192 rows of 16 + 2 + 2 heads of 128: 21.2 us for 85 MB, 53 % of the issue slots; with
+// 2, 3, 4 or 6 rows a CTA 21.4 to 24.5, and 64 rows 2.9 to 5.1 for 2.6.
 __global__ void __launch_bounds__(256) k_append(const AppendCall c) {
     pdl_wait();
     pdl_trigger();
