@@ -715,3 +715,15 @@ def test_decoding_in_one_graph(llmx, torch, oracle):
                 want = oracle.attention_group(turned[h * g:(h + 1) * g], k[:, h], v[:, h])
                 assert np.array_equal(got[r, h * g:(h + 1) * g], want), (n, r, h)
     p.error()
+
+
+@gpu
+@pytest.mark.parametrize("rows,before,longest", [(200, 37, 0), (77, 0, 0), (77, 0, 17000)])
+def test_prompt_as_blocks(llmx, torch, oracle, rows, before, longest):
+    """A prompt's rows in one call: blocks of 8 as requests of their own, with one table."""
+    rng = np.random.default_rng(rows)
+    ends = list(range(8, rows, 8)) + [rows]
+    c = Case(rng, [(n - m, before + n) for m, n in zip([0] + ends, ends)], 16, 2, 64)
+    c.table[:] = c.table[-1]
+    c.table = np.pad(c.table, ((0, 0), (0, longest // 16 + 1)), constant_values=-1)
+    check(llmx, torch, oracle, c, longest=longest)
