@@ -1470,6 +1470,7 @@ struct llmx_paged {
     bool one = false;  // one column block
     uint32_t max_requests = 0, max_block = 0, max_length = 0;
     long long capacity = 0;  // (key head, tile) items of a call
+    uint64_t positions = 0;  // of all requests of a call
     size_t scores_smem = 0, values_smem = 0;
     int scores_ctas = 0, values_ctas = 0;  // that are on the device at once
     unsigned char *memory = nullptr;
@@ -1552,17 +1553,24 @@ struct Clusters {
     uint64_t ctas = 0;
     int log = 0, tiles = 0, blocks = 0, smem = 0;
 };
-// Microseconds as measured (16 query heads, 2 key heads of 128; 1 to 64 requests of 64 to 8192 positions, even
-// and ragged, 1 and 4 rows).  A turn of clusters takes 5.2 and 1.45 per tile of a CTA, and 0.72 more per tile for
-// each CTA that shares its SM (0.55 with its request's columns in several clusters, 0.43 with several column
-// blocks a cluster), all of the latter more by 0.68 for each further block.  There are as many turns as it takes SMs that hold 4 CTAs, or what their memory
-// allows; the later ones are taken to be half as long.  The three launches take 11.5, 1.3 per further
-// block and 1.15 per tile an SM has (more by 0.52 of it per further block), with requests 0.8 as long
-// as the longest.  64 x 1024: 19.7 by clusters of 4, 26.6 of 8, 27.6 by three launches; 64 up to 2048:
-// 35.3, 26.1 and 30.6; one of 2048 11.0 (of 8) and 12.2, of 4096 17.5 and 14.5; 64 x 4096 85 and 76.5.
-Clusters choose(const llmx_paged *p, uint64_t strips, int all, int most) {
+// Estimates whose order was fitted to measurements of every way (2090 calls: 1 to 64 query heads of 16 to 128, 1 to 128
+// requests of up to 20 to 16000 positions, all as long and of any length, 1 to 8 rows; caches in HBM and in the L2): what is picked
+// was 1.8 % slower than the best way on average (4.9 % by the estimate before, which knew 16 heads of 128 only), 56 % at
+// most (13 requests of 3000, 3 rows: three launches 39, 30 by clusters of 8 that hold all columns).
+//   Three launches: a start, more per further column block, and the tiles that an SM has.
+//   Clusters: a CTA's tiles, slower for each CTA that shares its SM and each further block; CTAs beyond those that the
+// SMs hold at once (4, or what their memory allows, and a little less for larger clusters) come in later turns, which a
+// part of one costs like most of a whole one.
+// Lengths are on the device: requests count as long as the longest, as far as the handle's room for all allows. The shorter
+// they are on average, the fewer tiles three launches have and the cheaper are the later turns.
+// 16 heads of 128, 1 row: 64 of 1024 19.7 us by clusters of 4, 26.6 of 8, 27.6 by three launches; one of 2048 11.0 (of 8) and
+// 12.2, of 4096 17.5 and 14.5; 64 of 4096 85 and 76.
+Clusters choose(const llmx_paged *p, uint64_t requests, int all, int most) {
     Clusters best;
-    double least = 11.5 + 1.3 * (most - 1) + 1.15 * 0.8 * (double)strips * all / p->sms * (1 + 0.52 * (most - 1));
+    const uint64_t strips = requests * (uint64_t)p->kv;
+    const double fill = std::min(1.0, ((double)p->positions / kTile + 0.5 * (double)requests) / ((double)requests * all));
+    const double per_tile = 0.2 + 0.2 * ((p->dim + 31) / 32), shorter = std::pow(fill, 2.5), fewer = std::pow(fill, 0.3);
+    double least = 18.2 + 1.06 * (most - 1) + 0.56 * per_tile * fill * (double)strips * all / p->sms * (1 + 0.87 * (most - 1));
     if (all > kShortTiles) return best;
     for (int log = 0; log <= 3; log++) {
         const int cluster = 1 << log, tiles = (all + cluster - 1) / cluster;
@@ -1572,11 +1580,11 @@ Clusters choose(const llmx_paged *p, uint64_t strips, int all, int most) {
             if (blocks > 1 && (most + blocks - 2) / (blocks - 1) == groups) continue;  // no fewer groups for more blocks
             const Places at(tiles, cluster, blocks, p->dim);
             if (at.size > kMaxSmem) continue;
-            const double each = (double)strips * cluster * groups / p->sms, room = std::min(4, kSmemOfSm / (at.size + 2048));
-            const double work = std::max(1.0, (double)all / cluster) * (1 + 0.68 * (blocks - 1));
-            const double turn = work * (1.45 + (blocks > 1 ? 0.43 : groups > 1 ? 0.55 : 0.72) * std::min(each, room));
-            const double turns = blocks == 1 && groups > 1 ? each / room : std::ceil(each / room);
-            const double us = 5.2 + turn + (std::max(1.0, turns) - 1) * (5.2 + turn / 2);
+            const double room = std::min(4, kSmemOfSm / (at.size + 2048)), load = fewer * (double)strips * cluster * groups / p->sms;
+            const double work = tiles * per_tile * (1 + 0.4 * (blocks - 1));
+            const double turn = work * (2.16 + (blocks > 1 ? 0.17 : groups > 1 ? 0.22 : 0.12) * std::min(load, room));
+            const double turns = std::max(1.0, load / (room * (1 - 0.027 * log)));
+            const double us = 4.3 + turn + (turns - 1 + 0.39 * (std::ceil(turns - 1e-9) - turns)) * (8.9 + 0.9 * turn * shorter);
             if (us < least) {
                 least = us;
                 best.ctas = strips * cluster;
@@ -1658,6 +1666,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
     p->max_length = max_length;
     p->one = blocks == 1;
     p->capacity = (long long)(tiles * kv_heads);
+    p->positions = positions;
     size_t at = 0;
     auto place = [&](size_t n) {
         const size_t was = at;
@@ -1819,7 +1828,7 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
     c.error = p->error;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int all = (int)((longest + kTile - 1) / kTile), most = (c.max_block * c.group + 7) / 8;
-    const Clusters how = choose(p, (uint64_t)requests * p->kv, all, most);
+    const Clusters how = choose(p, requests, all, most);
     if (how.ctas) {
         c.cluster_log = how.log;
         c.tiles = how.tiles;
