@@ -507,7 +507,8 @@ typedef struct llmx_paged llmx_paged;
 /* Reserves the workspace of attention calls: heads (1 to 1024, a multiple of kv_heads), head_dim
  * (a multiple of 16 up to 128), page_len (a multiple of 8 up to 65536, fewer than 2^31 values a page); at most max_requests
  * (1 to 1024) requests of max_block (1 to 8) rows, max_length (1 to 2^20) positions each
- * and max_positions together.  heads / kv_heads * max_block is at most 128.  One handle
+ * and max_positions together (which also tells how long requests are on average: the closer, the better the
+ * way that a call's tiles are divided up).  heads / kv_heads * max_block is at most 128.  One handle
  * serves every layer of these sizes. */
 int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_len,
                       uint32_t max_requests, uint32_t max_block, uint32_t max_length, uint64_t max_positions,
