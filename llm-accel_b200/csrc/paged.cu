@@ -984,7 +984,7 @@ struct Stretch {
 // so a warp gives what its tiles do to any value that comes in as a few stretches, and the first
 // warp, which starts from 0, puts them together; tiles beyond a warp's kMaxStretches it goes
 // through itself, and a stretch on which something might saturate tile by tile.  Tile by tile throughout
-// it took 224 us of a request of 32768 positions, so 10; 64 x 8192: 66 before, 13 now, 34 MB from the L2.
+// it took 224 us of a request of 32768 positions with cold caches, so 18; 64 x 8192: 66, so 21 (34 MB).
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
