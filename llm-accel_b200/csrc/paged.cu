@@ -19,8 +19,8 @@
 //                                of 513 positions 7.7 us (three launches 11.1), 64 of up to 2304 29.8 (34).
 //   k_scores, k_values, k_join   one launch each over all tiles, scores and tv through the L2.  For many long
 //                                texts, which HBM and instructions bound, and for one that is longer
-//                                than a cluster can hold: 64 requests of 8192 positions 133 us for 537 MB of
-//                                keys and values (4.0 TB/s; a copy alone would take 82), one of 32768 28.5.
+//                                than a cluster can hold: 64 requests of 8192 positions 131 us for 537 MB of
+//                                keys and values (4.1 TB/s; a copy alone would take 82), one of 32768 28.4.
 //
 // Products are formed by int8 matrix instructions, exactly.  A product is
 // rnd4(x sat16(16 y)) with y the cached value: with c = y limited to [-2048, 2048]
@@ -1046,6 +1046,16 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
         for (int w0 = t0; w0 < t1; w0 += 32) {
             const int n = min(32, t1 - w0);
             const int2 f = lane < n ? fsum[(w0 + lane) * 8] : make_int2(16384, 0);
+            uint2 v[kAhead];
+            auto load = [&](int b0) {
+#pragma unroll
+                for (int i = 0; i < kAhead; i++) {
+                    v[i] = make_uint2(0, 0);
+                    if (b0 + i < n) v[i] = tv[(size_t)(w0 + b0 + i) * step];
+                }
+            };
+            // with the factors, not after them: 64 x 8192 132.6 -> 131.2 in all; a text of 32768 positions 28.5 -> 29.2
+            if constexpr (!kLong) load(0);
             uint32_t turns = __ballot_sync(0xffffffffu, f.x != 16384);
             if (!open) {
                 p.clear(__shfl_sync(0xffffffffu, f.x, 0), w0);
@@ -1053,14 +1063,9 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
                 open = true;
             }
             int from = 0;  // of this window's tiles, the first whose P is not in the stretch
-            uint2 v[kAhead];
 #pragma unroll 1
             for (int b0 = 0; b0 < n; b0 += kAhead) {
-#pragma unroll
-                for (int i = 0; i < kAhead; i++) {
-                    v[i] = make_uint2(0, 0);
-                    if (b0 + i < n) v[i] = tv[(size_t)(w0 + b0 + i) * step];
-                }
+                if (kLong || b0) load(b0);
                 if ((turns >> b0 & ((1u << kAhead) - 1)) == 0) {
 #pragma unroll
                     for (int i = 0; i < kAhead; i++) p.add<kLong>(v[i]);
