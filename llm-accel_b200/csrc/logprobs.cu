@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     __shared__ unsigned long long lists[kWarps][32];
     __shared__ unsigned long long chosen[32], candidates[kCandidates];
     __shared__ double rests[kWarps], sums[kWarps];
-    __shared__ uint32_t aheads[kWarps], found;
+    __shared__ uint32_t aheads[kWarps], withs[kWarps], found;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) found = 0;
     const uint32_t r = blockIdx.x;
@@ -410,7 +410,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
     // One maximum stays out of the sums: the parts that have it count one less.
     double rest = 0, sum = 0;
     uint32_t ahead = 0;
-    int with = 0;
+    uint32_t with = 0;
     auto add = [&](const Part &p) {
         ahead += p.ahead;
         if (p.top == kExcluded || greedy) return;
@@ -437,7 +437,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
         rests[warp] = rest;
         sums[warp] = sum;
         aheads[warp] = ahead;
-        lists[warp][1] = (unsigned long long)with;
+        withs[warp] = with;  // (not in lists: gather writes there, below, while others may still add these up)
     }
     // The best tokens: the maximum of the last of the best chunks bounds them from below (any token with that
     // logit may be one).
@@ -467,7 +467,7 @@ __global__ void __launch_bounds__(kThreads) k_rows_join(const Call c) {
         all_rest += rests[i];
         all_sum += sums[i];
         ahead += aheads[i];
-        all_with += (long long)lists[i][1];
+        all_with += withs[i];
     }
     if (greedy || m == kExcluded) all_with = 0;
     rest = all_rest + (double)all_with;

@@ -337,3 +337,27 @@ def test_of_verified_tokens(llmx, torch):
             assert drawn.sum() >= len(counts) and (got["rank"][~drawn] == NO_TOKEN).all()
             if temperature == 0:  # an accepted draft and a drawn token are the rows' maxima
                 assert (got["rank"][drawn] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("top", [1, 2, 3, 4, 5, 9])
+def test_many_equal_many_rows(llmx, torch, top):
+    """More equal tokens than are compared all with all, in many rows at once: warps that have none of the best chunks to
+    look through (top below 8) are at the lists' end long before the others.  The same bits in every row and every call."""
+    rng = np.random.default_rng(top)
+    rows, vocab = 600, 2048
+    z = np.tile(rng.integers(-9, 1, vocab) // 2 * 65536, (rows, 1)).astype(np.int32)  # some 200 of each value
+    z[:, rng.random(vocab) < 0.3] = 65536
+    tokens = np.full(rows, 1500, np.uint32)
+    d = Device(llmx, torch, z, tokens, None, top)
+    want = oracle(z[:1], tokens[:1], np.ones(1, np.float32), top)
+    log, ent = bounds(want["terms"][0], vocab // 512 + 1)
+    for _ in range(20):
+        d.call()
+        got = d.result()
+        for f in ("logprob", "rank", "entropy", "top_tokens", "top_logprobs"):
+            assert (got[f] == got[f][:1]).all(), f
+        assert np.array_equal(got["top_tokens"][0], want["top_tokens"][0]) and got["rank"][0] == want["rank"][0]
+        assert abs(got["entropy"][0] - want["entropy"][0]) <= ent + want["entropy"][0] * 2.0**-24
+        for g, w in ((got["logprob"][0], want["logprob"][0]), (got["top_logprobs"][0], want["top_logprobs"][0])):
+            assert (np.abs(g - w) <= log + np.abs(w) * 2.0**-24).all()
