@@ -497,6 +497,7 @@ static __device__ __forceinline__ void score_tile(const Call &c, const Strip &z,
         uint32_t w[2];
         const uint32_t top = finish_scores(c, z, u, nb, p0, column, w);
         store(nb, top, w);
+        __syncwarp();  // (lanes 0 to 3 stored more)
     }
 }
 
@@ -898,6 +899,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_values(const Call c) {
                         f[0].y = sum.x;
                         f[1].y = sum.y;
                     }
+                    __syncwarp();
                 }
             }
         }
@@ -1147,7 +1149,10 @@ struct Places {  // in dynamic shared memory, in bytes
     }
 };
 static __device__ __forceinline__ void put(uint32_t at, uint32_t v) { asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
+// (aligned: a warp's lanes meet first, here and before the arrival and the matrix instructions that follow
+// what only some of them did)
 static __device__ __forceinline__ void cluster_meet() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -1182,6 +1187,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
     }
     const int rows = (int)(o1 - o0), columns = min(rows * c.group - nb0 * 8, most * 8);
     if (columns <= 0) return;
+    __syncwarp();
     llmx::cluster_arrive();
     const Strip z{c.table + (size_t)b * c.ld_table, h, rows, (int)len, (columns + 7) >> 3, o0, nb0 * 8};
     const int n = (z.length + kTile - 1) / kTile, t0 = n * rank >> log, own = (n * (rank + 1) >> log) - t0;
@@ -1312,12 +1318,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_attend(const Call c) {
                 for (int o = 0; o < 4; o++)
                     if (o < share.octets) put(to + 16 * o, y[o]);
             }
+            __syncwarp();
             if (share.part == 0) {
                 const int2 sum = sum_of(b2);
                 const uint32_t f0 = (uint32_t)(((nb * of_block + (2 * cp >> log)) * stride + t0 + k) * 8);
                 const uint32_t f1 = (uint32_t)(((nb * of_block + (2 * cp + 1 >> log)) * stride + t0 + k) * 8);
                 if (g == 0 && nb * 8 + 2 * cp < columns) put(factor0 + f0 + 4, (uint32_t)sum.x);
                 if (g == 0 && nb * 8 + 2 * cp + 1 < columns) put(factor1 + f1 + 4, (uint32_t)sum.y);
+                __syncwarp();
             }
         }
     }

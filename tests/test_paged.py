@@ -727,3 +727,21 @@ def test_prompt_as_blocks(llmx, torch, oracle, rows, before, longest):
     c.table[:] = c.table[-1]
     c.table = np.pad(c.table, ((0, 0), (0, longest // 16 + 1)), constant_values=-1)
     check(llmx, torch, oracle, c, longest=longest)
+
+
+@gpu
+@pytest.mark.parametrize("heads,block,hd", [(5, 5, 80), (9, 7, 48), (7, 8, 128), (3, 3, 16)])
+@pytest.mark.parametrize("longest", [0, 20000])
+def test_partly_filled_column_blocks(llmx, torch, oracle, heads, block, hd, longest):
+    """Query rows that do not fill their blocks of 8, so that some lanes store and others do not between one block's
+    matrix instructions and the next one's; requests that leave CTAs of a cluster without a tile.  The same every time."""
+    rng = np.random.default_rng(heads)
+    c = Case(rng, [(block, 700), (1, 65), (block - 1, 130), (2, 64), (block, 1)], heads, 1, hd)
+    c.table = np.pad(c.table, ((0, 0), (0, longest // 16 + 1)), constant_values=-1)
+    d, want = Device(llmx, torch, c, longest=longest), c.want(oracle)
+    for _ in range(10):
+        d.out.fill_(FILL)
+        d.call()
+        got = d.result()
+        assert np.array_equal(got, want), report(got, want)
+    d.p.error()
