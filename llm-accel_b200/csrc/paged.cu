@@ -952,10 +952,19 @@ struct Stretch {
     int s[4];
     uint32_t lo, hi;  // of pairs of elements; once closed, the furthest down and up
     int factor, start, tiles, psum;
+    // A tile's P add up to 2^20 at most, those of a long stretch to more than 32 bits hold.  From kFull on four times the sum
+    // are 2^31 or more, and what they are added to is not negative: the sum saturates, by how much need not be known.
+    static constexpr int kFull = 1 << 29;
+    // p: of 32 tiles at most
+    template <bool kLong>
+    __device__ __forceinline__ void add_psum(int p) {
+        psum += p;
+        if constexpr (kLong) psum = min(psum, kFull);
+    }
     template <bool kLong>
     __device__ __forceinline__ void close(int end, int p) {
         tiles = end - start;
-        psum += p;
+        add_psum<kLong>(p);
         if constexpr (kLong) {
             lo = (uint32_t)(int)max(256ll * tiles * min(llmx::lo16(lo), llmx::hi16(lo)), (long long)INT_MIN);
             hi = (uint32_t)(int)min(256ll * tiles * max(llmx::lo16(hi), llmx::hi16(hi)), (long long)INT_MAX);
@@ -1023,7 +1032,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
         if constexpr (kLong) {
             // (hi is at least 0, lo at most 0)
             const bool far = max(max(x[0], x[1]), max(x[2], x[3])) > INT_MAX - (int)p.hi || min(min(x[0], x[1]), min(x[2], x[3])) < INT_MIN - (int)p.lo ||
-                             sum > INT_MAX - 4 * p.psum;
+                             sum + 4ll * p.psum > INT_MAX;
             if (__any_sync(0xffffffffu, far)) {
 #pragma unroll 1
                 for (int t = p.start; t < p.start + p.tiles; t++) {
@@ -1091,7 +1100,7 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
                     p.add<kLong>(v[i]);
                 }
             }
-            p.psum += __reduce_add_sync(0xffffffffu, lane >= from ? f.y : 0);
+            p.add_psum<kLong>(__reduce_add_sync(0xffffffffu, lane >= from ? f.y : 0));
         }
         if (open) {
             p.close<kLong>(t1, 0);
