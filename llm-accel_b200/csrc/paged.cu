@@ -950,7 +950,7 @@ static __device__ __forceinline__ uint2 quotient(const int (&x)[4], int sum) {
 // long text) how far from what comes in they can get on the way, by the least and the largest value.
 struct Stretch {
     int s[4];
-    uint32_t lo, hi;  // of pairs of elements; once closed, the furthest down and up
+    uint32_t lo, hi;  // of pairs of elements; once closed, the furthest down and up, over 256 (2^14 tiles of 2^15 at most)
     int factor, start, tiles, psum;
     // A tile's P add up to 2^20 at most, those of a long stretch to more than 32 bits hold.  From kFull on four times the sum
     // are 2^31 or more, and what they are added to is not negative: the sum saturates, by how much need not be known.
@@ -966,8 +966,8 @@ struct Stretch {
         tiles = end - start;
         add_psum<kLong>(p);
         if constexpr (kLong) {
-            lo = (uint32_t)(int)max(256ll * tiles * min(llmx::lo16(lo), llmx::hi16(lo)), (long long)INT_MIN);
-            hi = (uint32_t)(int)min(256ll * tiles * max(llmx::lo16(hi), llmx::hi16(hi)), (long long)INT_MAX);
+            lo = (uint32_t)(tiles * min(llmx::lo16(lo), llmx::hi16(lo)));
+            hi = (uint32_t)(tiles * max(llmx::lo16(hi), llmx::hi16(hi)));
         }
     }
     __device__ __forceinline__ void clear(int f, int t) {
@@ -1030,9 +1030,10 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
             for (int k = 0; k < 4; k++) x[k] = times(x[k], p.factor);
         }
         if constexpr (kLong) {
-            // (hi is at least 0, lo at most 0)
-            const bool far = max(max(x[0], x[1]), max(x[2], x[3])) > INT_MAX - (int)p.hi || min(min(x[0], x[1]), min(x[2], x[3])) < INT_MIN - (int)p.lo ||
-                             sum + 4ll * p.psum > INT_MAX;
+            // x + 256 h is above 2^31 - 1 just where floor(x / 256) + h is above 2^23 - 1, below -2^31 where that is below
+            // -2^23; likewise of sum + 4 psum: nothing here leaves 32 bits.
+            const bool far = (max(max(x[0], x[1]), max(x[2], x[3])) >> 8) + (int)p.hi > INT_MAX >> 8 ||
+                             (min(min(x[0], x[1]), min(x[2], x[3])) >> 8) + (int)p.lo < INT_MIN >> 8 || (sum >> 2) + p.psum > INT_MAX >> 2;
             if (__any_sync(0xffffffffu, far)) {
 #pragma unroll 1
                 for (int t = p.start; t < p.start + p.tiles; t++) {

@@ -75,3 +75,40 @@ def test_flat_stretches(llmx, torch, oracle, scores):
         raise_from(c, position, score)
     out = check(llmx, torch, oracle, c)
     assert (out != 0).any() == (scores[-1] == 1800)
+
+
+# a tile's values saturate from 512 on (64 * 512 = 2^15)
+LARGE = [700, -700, 511, -511, 512, -512, 600, -600, 32767, -32768, 300, -300, 0, 1, -1, 450]
+
+
+@pytest.mark.parametrize("length", [16384, 16448, 16512, 24000, 32704, 40000])
+@pytest.mark.parametrize("score", [None, 1000, 2000])
+def test_large_values_by_one_warp(llmx, torch, oracle, length, score):
+    """From 257 tiles in a stretch on the values' sums pass 2^31, from nothing up or down."""
+    c = flat(np.random.default_rng(4), length, 8, ONE_WARP, LARGE)
+    if score:
+        raise_from(c, length - 1, score)
+    out = check(llmx, torch, oracle, c)
+    assert (out != 0).any() or score != 2000
+
+
+@pytest.mark.parametrize("then,rise,last", [(500, 1024, 1000), (450, 600, 1440)])
+@pytest.mark.parametrize("first", [10, 260, 300])
+@pytest.mark.parametrize("values", [LARGE, [700] * 16, [-700] * 16])
+def test_values_that_turn(llmx, torch, oracle, values, first, then, rise, last):
+    """Sums below 0 that a stretch takes beyond 2^31, and the other way round."""
+    c = flat(np.random.default_rng(5), (first + then) * 64, 8, ONE_WARP, values)
+    p = np.arange(first * 64)
+    c.v[c.table[0][p // 64], :, p % 64] = -np.clip(np.array(values, np.int32), -32767, 32767).astype(np.int16)
+    raise_from(c, first * 64, rise)
+    raise_from(c, (first + then) * 64 - 1, last)
+    out = check(llmx, torch, oracle, c)
+    assert (out != 0).any() or last == 1000
+
+
+@pytest.mark.parametrize("heads,pad", [(1, 0), (8, ONE_WARP)])
+def test_longest_with_large_values(llmx, torch, oracle, heads, pad):
+    c = flat(np.random.default_rng(6), 2**20, heads, pad, LARGE)
+    check(llmx, torch, oracle, c)
+    raise_from(c, 2**20 - 1, 2000)
+    check(llmx, torch, oracle, c)
