@@ -3,9 +3,9 @@
  * launches; here it costs a tenth of that.  llmx.py binds the addresses of the library that it
  * has loaded and uses ctypes for all else, and for these too where this module was not built.
  *
- * Arguments are whole numbers (pointers too) or None for NULL, longer ones cut to the parameter's size; a call
- * with anything else (a ctypes pointer, say) goes through ctypes after all.  The result is the
- * status code. */
+ * Arguments are whole numbers (pointers too), longer ones cut to the parameter's size, and None for a NULL
+ * pointer; a call with anything else (a ctypes pointer, say, or None in a number's place) goes through ctypes
+ * after all, which takes it or says what is wrong.  The result is the status code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -13,13 +13,14 @@
 
 #include "llmx.h"
 
-static int arguments(const char *name, PyObject *const *args, Py_ssize_t got, Py_ssize_t want, unsigned long long *out) {
+/* kinds: a letter per argument, P where it is a pointer. */
+static int arguments(const char *name, const char *kinds, PyObject *const *args, Py_ssize_t got, Py_ssize_t want, unsigned long long *out) {
     if (got != want) {
         PyErr_Format(PyExc_TypeError, "%s takes %zd arguments, got %zd", name, want, got);
         return 0;
     }
     for (Py_ssize_t i = 0; i < want; i++) {
-        if (args[i] == Py_None) {
+        if (args[i] == Py_None && kinds[i] == 'P') {
             out[i] = 0;
             continue;
         }
@@ -32,19 +33,20 @@ static int arguments(const char *name, PyObject *const *args, Py_ssize_t got, Py
 #define P(type, i) ((type)(uintptr_t)a[i])
 #define U(i) ((uint32_t)a[i])
 #define Z(i) ((size_t)a[i])
-/* A function of this module: the bound address, and the call with its arguments a[0] .. a[n - 1]. */
-#define CALL(fn, n, ...)                                                              \
+/* A function of this module: the bound address, and the call with its arguments a[0], a[1] and on, one for each letter
+ * of kinds (P, U and Z, as below; I: int). */
+#define CALL(fn, kinds, ...)                                                          \
     static __typeof__(&fn) p_##fn;                                                    \
     static PyObject *o_##fn; /* the same function through ctypes */                   \
     static PyObject *c_##fn(PyObject *self, PyObject *const *args, Py_ssize_t got) {  \
-        unsigned long long a[n];                                                      \
+        unsigned long long a[sizeof(kinds) - 1];                                      \
         int rc;                                                                       \
         (void)self;                                                                   \
         if (!p_##fn) {                                                                \
             PyErr_SetString(PyExc_RuntimeError, #fn " is not bound");                 \
             return NULL;                                                              \
         }                                                                             \
-        if (!arguments(#fn, args, got, n, a)) {                                       \
+        if (!arguments(#fn, kinds, args, got, (Py_ssize_t)sizeof(kinds) - 1, a)) {    \
             if (!PyErr_ExceptionMatches(PyExc_TypeError)) return NULL;                \
             PyErr_Clear();                                                            \
             return PyObject_Vectorcall(o_##fn, args, (size_t)got, NULL);              \
@@ -53,16 +55,16 @@ static int arguments(const char *name, PyObject *const *args, Py_ssize_t got, Py
         Py_END_ALLOW_THREADS return PyLong_FromLong(rc);                              \
     }
 
-CALL(llmx_adapters_project, 9, P(llmx_adapters *, 0), P(const int16_t *, 1), U(2), Z(3), P(const int32_t *, 4), P(void *, 5), (int)a[6], Z(7),
+CALL(llmx_adapters_project, "PPUZPPIZP", P(llmx_adapters *, 0), P(const int16_t *, 1), U(2), Z(3), P(const int32_t *, 4), P(void *, 5), (int)a[6], Z(7),
      P(void *, 8))
-CALL(llmx_verify_drafts, 19, P(const int32_t *, 0), Z(1), P(const int32_t *, 2), Z(3), U(4), P(const uint32_t *, 5), P(const uint32_t *, 6), U(7),
+CALL(llmx_verify_drafts, "PZPZUPPUUUPPPPPPPZP", P(const int32_t *, 0), Z(1), P(const int32_t *, 2), Z(3), U(4), P(const uint32_t *, 5), P(const uint32_t *, 6), U(7),
      U(8), U(9), P(const float *, 10), P(const uint32_t *, 11), P(const uint32_t *, 12), P(uint32_t *, 13), P(uint32_t *, 14), P(uint64_t *, 15),
      P(void *, 16), Z(17), P(void *, 18))
-CALL(llmx_token_logprobs, 15, P(const int32_t *, 0), Z(1), U(2), U(3), P(const uint32_t *, 4), P(const float *, 5), U(6), P(float *, 7),
+CALL(llmx_token_logprobs, "PZUUPPUPPPPPPZP", P(const int32_t *, 0), Z(1), U(2), U(3), P(const uint32_t *, 4), P(const float *, 5), U(6), P(float *, 7),
      P(uint32_t *, 8), P(float *, 9), P(uint32_t *, 10), P(float *, 11), P(void *, 12), Z(13), P(void *, 14))
-CALL(llmx_paged_append, 17, P(llmx_paged *, 0), P(const int16_t *, 1), U(2), Z(3), P(const uint32_t *, 4), P(const uint32_t *, 5), U(6),
+CALL(llmx_paged_append, "PPUZPPUPUPZPPUPZP", P(llmx_paged *, 0), P(const int16_t *, 1), U(2), Z(3), P(const uint32_t *, 4), P(const uint32_t *, 5), U(6),
      P(const int16_t *, 7), U(8), P(const int32_t *, 9), Z(10), P(int16_t *, 11), P(int16_t *, 12), U(13), P(int16_t *, 14), Z(15), P(void *, 16))
-CALL(llmx_paged_attention, 16, P(llmx_paged *, 0), P(const int16_t *, 1), U(2), Z(3), P(const uint32_t *, 4), P(const uint32_t *, 5), U(6), U(7),
+CALL(llmx_paged_attention, "PPUZPPUUPZPPUPZP", P(llmx_paged *, 0), P(const int16_t *, 1), U(2), Z(3), P(const uint32_t *, 4), P(const uint32_t *, 5), U(6), U(7),
      P(const int32_t *, 8), Z(9), P(const int16_t *, 10), P(const int16_t *, 11), U(12), P(int16_t *, 13), Z(14), P(void *, 15))
 
 /* bind(name, address, function): where the library's function of that name is, and the same through ctypes. */

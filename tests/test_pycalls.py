@@ -61,3 +61,19 @@ def test_arguments_arrive_in_their_places(llmx, calls):
         assert text in said("llmx_verify_drafts", bad), at
     for name in ("llmx_paged_append", "llmx_paged_attention", "llmx_adapters_project"):
         assert "null handle" in said(name, [None] + [1] * (COUNTS[name] - 1))
+
+
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_none_is_no_number(llmx, calls, name):
+    """None is a NULL pointer, and an error in the place of a number (where it would be 0: no rows, say, and a call that
+    does nothing)."""
+    slow = getattr(llmx.lib(), name)
+    good = [None if t is C.c_void_p else 0 for t in slow.argtypes]
+    for i, t in enumerate(slow.argtypes):
+        args = list(good)
+        args[i] = None
+        if t is C.c_void_p:
+            assert calls[name](*args) == slow(*args)
+        else:
+            with pytest.raises((TypeError, C.ArgumentError)):
+                calls[name](*args)
