@@ -3,15 +3,18 @@
  * launches; here it costs a tenth of that.  llmx.py binds the addresses of the library that it
  * has loaded and uses ctypes for all else, and for these too where this module was not built.
  *
- * Arguments are whole numbers (pointers too), longer ones cut to the parameter's size, and None for a NULL
- * pointer; a call with anything else (a ctypes pointer, say, or None in a number's place) goes through ctypes
- * after all, which takes it or says what is wrong.  The result is the status code. */
+ * Arguments are whole numbers, longer ones cut to the parameter's size.  Pointers are too, or None for NULL, but nothing
+ * that merely has an __index__: a tensor of one element has, and its value is not its address.  A call with anything
+ * else (a ctypes pointer, say, or None in a number's place) goes through ctypes after all, which takes it or says
+ * what is wrong.  The result is the status code. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <stdint.h>
 
 #include "llmx.h"
+
+static PyObject *integral; /* numbers.Integral */
 
 /* kinds: a letter per argument, P where it is a pointer. */
 static int arguments(const char *name, const char *kinds, PyObject *const *args, Py_ssize_t got, Py_ssize_t want, unsigned long long *out) {
@@ -23,6 +26,11 @@ static int arguments(const char *name, const char *kinds, PyObject *const *args,
         if (args[i] == Py_None && kinds[i] == 'P') {
             out[i] = 0;
             continue;
+        }
+        if (kinds[i] == 'P' && !PyLong_Check(args[i])) {
+            const int is = PyObject_IsInstance(args[i], integral);
+            if (is == 0) PyErr_Format(PyExc_TypeError, "%s: argument %zd is not an address", name, i + 1);
+            if (is <= 0) return 0;
         }
         out[i] = PyLong_AsUnsignedLongLongMask(args[i]);
         if (out[i] == (unsigned long long)-1 && PyErr_Occurred()) return 0;
@@ -96,4 +104,10 @@ static PyMethodDef methods[] = {ENTRY(llmx_adapters_project), ENTRY(llmx_verify_
                                 ENTRY(llmx_paged_attention),  {"bind", bind, METH_VARARGS, NULL}, {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_llmxcalls", NULL, -1, methods, NULL, NULL, NULL, NULL};
 
-PyMODINIT_FUNC PyInit__llmxcalls(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__llmxcalls(void) {
+    PyObject *numbers = PyImport_ImportModule("numbers");
+    if (!numbers) return NULL;
+    Py_XSETREF(integral, PyObject_GetAttrString(numbers, "Integral"));
+    Py_DECREF(numbers);
+    return integral ? PyModule_Create(&module) : NULL;
+}

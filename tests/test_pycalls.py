@@ -77,3 +77,33 @@ def test_none_is_no_number(llmx, calls, name):
         else:
             with pytest.raises((TypeError, C.ArgumentError)):
                 calls[name](*args)
+
+
+class Index:
+    """Something that can stand for a whole number without being one, as a tensor of one element can."""
+
+    def __index__(self):
+        return 0
+
+
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_arrays_are_no_addresses(llmx, calls, name):
+    """An array of one element in the place of its address: its value is not taken for that.  In a number's place it is
+    one, as for ctypes."""
+    slow = getattr(llmx.lib(), name)
+    good = [None if t is C.c_void_p else 0 for t in slow.argtypes]
+    wrong = [Index(), np.array(0), np.zeros(1, np.int32)]
+    try:
+        import torch
+        wrong += [torch.zeros(1, dtype=torch.int32), torch.tensor(0)]
+    except ImportError:
+        pass
+    for i, t in enumerate(slow.argtypes):
+        for x in wrong:
+            args = [*good[:i], x, *good[i + 1:]]
+            if t is C.c_void_p or getattr(x, "ndim", 0) == 1 and isinstance(x, np.ndarray):
+                with pytest.raises((TypeError, C.ArgumentError)):
+                    calls[name](*args)
+            else:
+                assert calls[name](*args) == slow(*args)
+        calls[name](*good[:i], np.int32(0), *good[i + 1:])  # (a whole number)
