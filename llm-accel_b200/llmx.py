@@ -94,7 +94,7 @@ def _bind_calls(L):
             module = None
     for name in STEP_CALLS:
         _calls[name] = getattr(L, name)
-        if module is not None:
+        if hasattr(module, name):  # (one built from an older source may lack some)
             module.bind(name, C.cast(getattr(L, name), C.c_void_p).value, getattr(L, name))
             _calls[name] = getattr(module, name)
 

@@ -107,3 +107,50 @@ def test_arrays_are_no_addresses(llmx, calls, name):
             else:
                 assert calls[name](*args) == slow(*args)
         calls[name](*good[:i], np.int32(0), *good[i + 1:])  # (a whole number)
+
+
+def compiled(folder, source, names):
+    """The module made of `source`, under each of the names in `folder`."""
+    import os
+    import shutil
+    import subprocess
+    import sysconfig
+    inc = sysconfig.get_paths()["include"]
+    gcc = os.environ.get("CC", "gcc")
+    if not os.path.exists(os.path.join(inc, "Python.h")) or shutil.which(gcc) is None:
+        pytest.skip("no headers of Python, or no compiler")
+    (folder / "calls.c").write_text(source)
+    include = os.path.join(os.path.dirname(__file__), "..", "include")
+    for name in names:
+        subprocess.run([gcc, "-O1", "-shared", "-fPIC", "-I", inc, "-I", include, str(folder / "calls.c"), "-o", str(folder / name)], check=True)
+
+
+def source_of_calls():
+    import os
+    with open(os.path.join(os.path.dirname(__file__), "..", "llm-accel_b200", "csrc", "pycalls.c")) as f:
+        return f.read()
+
+
+@pytest.fixture
+def elsewhere(llmx, tmp_path, monkeypatch):
+    """The binding as it looks for its module in an empty folder; afterwards as it was."""
+    L = llmx.lib()
+    monkeypatch.setattr(llmx, "HERE", str(tmp_path))
+    yield lambda: llmx._bind_calls(L)
+    monkeypatch.undo()
+    llmx._bind_calls(L)
+
+
+def test_module_of_an_older_source(llmx, elsewhere, tmp_path):
+    """A module that lacks a function: that one goes through ctypes, the others through the module."""
+    import re
+    import sysconfig
+    source = source_of_calls()
+    source = re.sub(r"\n    BIND\(llmx_paged_attention\)", "", source)
+    source = re.sub(r"ENTRY\(llmx_paged_attention\),", "", source)
+    compiled(tmp_path, source, ["_llmxcalls.so", "_llmxcalls" + sysconfig.get_config_var("EXT_SUFFIX")])
+    elsewhere()
+    for name in COUNTS:
+        through_ctypes = llmx._calls[name] is getattr(llmx.lib(), name)
+        assert through_ctypes == (name == "llmx_paged_attention")
+        assert llmx._calls[name](*[None if t is C.c_void_p else 0 for t in getattr(llmx.lib(), name).argtypes]) == llmx.ERR_ARG
