@@ -68,9 +68,10 @@ def _compile(src, force, build_dir, defines):
 
 
 def _build_calls(force):
-    """The Python module of csrc/pycalls.c, next to the library; without Python's
-    headers it is left out, and llmx.py makes all its calls through ctypes."""
-    src, out = os.path.join(CSRC, "pycalls.c"), os.path.join(HERE, "_llmxcalls.so")
+    """The Python module of csrc/pycalls.c, next to the library, for this interpreter
+    alone; without Python's headers it is left out, and llmx.py makes all its calls
+    through ctypes."""
+    src, out = os.path.join(CSRC, "pycalls.c"), os.path.join(HERE, "_llmxcalls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
     inc = sysconfig.get_paths()["include"]
     if not os.path.exists(os.path.join(inc, "Python.h")):
         return

@@ -16,6 +16,7 @@ from __future__ import annotations
 import ctypes as C
 import importlib.util
 import os
+import sysconfig
 
 import numpy as np
 
@@ -83,14 +84,15 @@ STEP_CALLS = ("llmx_adapters_project", "llmx_verify_drafts", "llmx_token_logprob
 
 
 def _bind_calls(L):
-    path = os.path.join(HERE, "_llmxcalls.so")
+    # (its name says for which interpreter it was built: one built for another may load, and go wrong)
+    path = os.path.join(HERE, "_llmxcalls" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
     module = None
     if os.path.exists(path):
         spec = importlib.util.spec_from_file_location("_llmxcalls", path)
         try:
             module = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(module)
-        except ImportError:  # built for another interpreter
+        except ImportError:
             module = None
     for name in STEP_CALLS:
         _calls[name] = getattr(L, name)

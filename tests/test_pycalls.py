@@ -154,3 +154,17 @@ def test_module_of_an_older_source(llmx, elsewhere, tmp_path):
         through_ctypes = llmx._calls[name] is getattr(llmx.lib(), name)
         assert through_ctypes == (name == "llmx_paged_attention")
         assert llmx._calls[name](*[None if t is C.c_void_p else 0 for t in getattr(llmx.lib(), name).argtypes]) == llmx.ERR_ARG
+
+
+def test_module_of_another_interpreter(llmx, elsewhere, tmp_path):
+    """Only a module whose file name says that it is for this interpreter is loaded: one for another may load as well, and
+    run with that one's reference counting."""
+    import sysconfig
+    compiled(tmp_path, source_of_calls(), ["_llmxcalls.so", "_llmxcalls.cpython-3999-x86_64-linux-gnu.so"])
+    elsewhere()
+    assert all(llmx._calls[name] is getattr(llmx.lib(), name) for name in COUNTS)
+    suffix = sysconfig.get_config_var("EXT_SUFFIX")
+    assert suffix not in (None, ".so")
+    (tmp_path / "_llmxcalls.so").rename(tmp_path / ("_llmxcalls" + suffix))
+    elsewhere()
+    assert all(llmx._calls[name] is not getattr(llmx.lib(), name) for name in COUNTS)
