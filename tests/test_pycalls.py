@@ -168,3 +168,35 @@ def test_module_of_another_interpreter(llmx, elsewhere, tmp_path):
     (tmp_path / "_llmxcalls.so").rename(tmp_path / ("_llmxcalls" + suffix))
     elsewhere()
     assert all(llmx._calls[name] is not getattr(llmx.lib(), name) for name in COUNTS)
+
+
+@pytest.fixture
+def module(llmx, calls):
+    """The module itself; afterwards bound to the library again.  Without it the tests above compare ctypes with itself."""
+    import os
+    import sysconfig
+    import types
+    if not os.path.exists(os.path.join(sysconfig.get_paths()["include"], "Python.h")):
+        pytest.skip("no headers of Python: the module is not built")
+    assert all(isinstance(calls[name], types.BuiltinFunctionType) for name in COUNTS)
+    yield calls["llmx_paged_append"].__self__
+    llmx._bind_calls(llmx.lib())
+
+
+@pytest.mark.parametrize("name", list(COUNTS))
+def test_every_argument_in_its_place(llmx, module, name):
+    """A function that writes down what it gets, in the library's place: other values in every place, as wide as
+    the parameters are, and wider ones."""
+    slow, got = getattr(llmx.lib(), name), []
+    fake = C.CFUNCTYPE(C.c_int, *slow.argtypes)(lambda *a: got.append(a) or 42)
+    module.bind(name, C.cast(fake, C.c_void_p).value, slow)
+    width = [8 * C.sizeof(t) for t in slow.argtypes]
+    assert len(width) == COUNTS[name]
+    for values in ([3 + i for i in range(len(width))], [(0x7123456789abcdef - (i << 33) - (i << 3)) % 2**(w - 1) for i, w in enumerate(width)],
+                   [(0xfedcba9876543210 + (i << 32) + i) for i in range(len(width))]):
+        assert getattr(module, name)(*values) == 42
+        kept = [v % 2**w for v, w in zip(values, width)]
+        kept = [v - 2**w if t is C.c_int and v >= 2**(w - 1) else v for v, w, t in zip(kept, width, slow.argtypes)]
+        assert list(got.pop()) == kept and not got
+    nothing = [None if t is C.c_void_p else 0 for t in slow.argtypes]
+    assert getattr(module, name)(*nothing) == 42 and list(got.pop()) == nothing
