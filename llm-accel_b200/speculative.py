@@ -130,8 +130,9 @@ class Server:
 
     def generate(self, prompts, slots, max_new, temperature=0.0, seed=0, logprobs=None):
         """New tokens of every request, and (drafted, accepted) over all of them.  With logprobs = n (0 to 32)
-        also, for every new token, (log probability, rank, entropy of its row, the n most likely
-        tokens as (token, log probability)): of the logits at temperature 1, whatever the tokens are drawn at."""
+        also, for every new token, (log probability, rank, entropy of its row, the n most likely tokens, or
+        all where there are fewer, as (token, log probability)): of the logits at temperature 1, whatever the tokens are
+        drawn at."""
         if logprobs is not None and not 0 <= logprobs <= 32:
             raise ValueError("logprobs must be 0..32 (the most likely tokens beside each), or None")
         t, count = self.torch, len(prompts)
@@ -182,8 +183,9 @@ class Server:
             if logprobs is not None:
                 for r, text in enumerate(texts):
                     for row in range(first[r], first[r] + len(text) - was[r]):
-                        told[r].append((float(lp[row]), int(rank[row]), float(entropy[row]),
-                                        list(zip(ids[row].tolist(), others[row].tolist()))))
+                        # (behind the last token that is not excluded the lists hold NO_TOKEN)
+                        best = [(t, x) for t, x in zip(ids[row].tolist(), others[row].tolist()) if t >= 0]
+                        told[r].append((float(lp[row]), int(rank[row]), float(entropy[row]), best))
         out = [text[len(q):] for text, q in zip(texts, prompts)]
         return (out, (drafted, taken)) if logprobs is None else (out, (drafted, taken), told)
 

@@ -202,3 +202,20 @@ def test_log_probabilities(llmx, untied):
         sv.close()
     assert model.shape.vocab <= 509  # a row is one warp's, whatever rows there are: the same bits
     assert told[0] == told[1]
+
+
+def test_more_log_probabilities_than_tokens(llmx):
+    """A vocabulary of fewer tokens than were asked for: all of them are told, and nothing else."""
+    pytest.importorskip("torch")
+    import speculative as spec
+    s = llmx.shape("small")
+    s.vocab = 20
+    model = llmx.Model(s).init_reference_random(7)
+    for drafts in (0, 4):
+        sv = server(spec, model, drafts)
+        out, _, report = sv.generate(PROMPTS, [0, -1, 1], 5, logprobs=32)
+        for text, mine in zip(out, report):
+            for token, (logprob, rank, entropy, best) in zip(text, mine):
+                assert rank == 0 and best[0] == (token, logprob)
+                assert sorted(t for t, _ in best) == list(range(20)) and all(np.isfinite(x) for _, x in best)
+        sv.close()
