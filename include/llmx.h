@@ -553,6 +553,10 @@ int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t rows, size_t 
 int llmx_paged_error(llmx_paged *p, void *stream);
 /* Bytes of device memory the handle holds. */
 uint64_t llmx_paged_device_bytes(const llmx_paged *p);
+/* For tests: the way that this handle's attention calls take from now on.  -1: by an estimate of the time (the default);
+ * 0: three launches; 16 i + b, b from 1 to 16: one, by clusters of 2^i CTAs (i from 0 to 3) with b blocks of 8 query rows each, or
+ * three where a call does not fit that.  taken (host): the way of a call of these sizes.  Results are the same by every way. */
+int llmx_selftest_paged_way(llmx_paged *p, int way, uint32_t requests, uint32_t longest, int *taken);
 
 /* ---------------------------------------------------------------------------
  * Host runtime: qwen_executor_t host:7607-8161

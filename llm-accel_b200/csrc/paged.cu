@@ -1496,6 +1496,7 @@ struct llmx_paged {
     uint64_t positions = 0;  // of all requests of a call
     size_t scores_smem = 0, values_smem = 0;
     int scores_ctas = 0, values_ctas = 0;  // that are on the device at once
+    int way = -1;  // of attention calls, for tests: see way_of; -1: as choose() estimates
     unsigned char *memory = nullptr;
     Meta *meta = nullptr;
     uint32_t *score = nullptr;
@@ -1576,6 +1577,8 @@ struct Clusters {
     uint64_t ctas = 0;
     int log = 0, tiles = 0, blocks = 0, smem = 0;
 };
+// As one number: 0 for three launches, else 16 log + blocks (1 to 16).
+int way_of(int log, int blocks) { return 16 * log + blocks; }
 // Estimates whose order was fitted to measurements of every way (2090 calls: 1 to 64 query heads of 16 to 128, 1 to 128
 // requests of up to 20 to 16000 positions, all as long and of any length, 1 to 8 rows; caches in HBM and in the L2): what is picked
 // was 1.8 % slower than the best way on average (4.9 % by the estimate before, which knew 16 heads of 128 only), 56 % at
@@ -1594,7 +1597,8 @@ Clusters choose(const llmx_paged *p, uint64_t requests, int all, int most) {
     const double fill = std::min(1.0, ((double)p->positions / kTile + 0.5 * (double)requests) / ((double)requests * all));
     const double per_tile = 0.2 + 0.2 * ((p->dim + 31) / 32), shorter = std::pow(fill, 2.5), fewer = std::pow(fill, 0.3);
     double least = 18.2 + 1.06 * (most - 1) + 0.56 * per_tile * fill * (double)strips * all / p->sms * (1 + 0.87 * (most - 1));
-    if (all > kShortTiles) return best;
+    if (p->way > 0) least = HUGE_VAL;
+    if (all > kShortTiles || p->way == 0) return best;
     for (int log = 0; log <= 3; log++) {
         const int cluster = 1 << log, tiles = (all + cluster - 1) / cluster;
         if (log && cluster > all) break;
@@ -1608,7 +1612,7 @@ Clusters choose(const llmx_paged *p, uint64_t requests, int all, int most) {
             const double turn = work * (2.16 + (blocks > 1 ? 0.17 : groups > 1 ? 0.22 : 0.12) * std::min(load, room));
             const double turns = std::max(1.0, load / (room * (1 - 0.027 * log)));
             const double us = 4.3 + turn + (turns - 1 + 0.39 * (std::ceil(turns - 1e-9) - turns)) * (8.9 + 0.9 * turn * shorter);
-            if (us < least) {
+            if (us < least && (p->way < 0 || p->way == way_of(log, blocks))) {
                 least = us;
                 best.ctas = strips * cluster;
                 best.log = log;
@@ -1874,6 +1878,17 @@ extern "C" int llmx_paged_attention(llmx_paged *p, const int16_t *q, uint32_t ro
         e = launch(far ? (const void *)k_join<true> : (const void *)k_join<false>, rows * (unsigned)p->heads, 32 * warps, smem, c, s);
     }
     return e == cudaSuccess ? LLMX_OK : cuda_fail("attention", e);
+}
+
+extern "C" int llmx_selftest_paged_way(llmx_paged *p, int way, uint32_t requests, uint32_t longest, int *taken) {
+    if (!p || !taken) return fail(LLMX_ERR_ARG, "null pointer");
+    if (way < -1 || way > way_of(3, 16)) return fail(LLMX_ERR_ARG, "way must be -1..64, got " + std::to_string(way));
+    if (requests == 0 || requests > p->max_requests || longest == 0 || longest > p->max_length)
+        return fail(LLMX_ERR_ARG, "sizes that the handle is not for");
+    p->way = way;
+    const Clusters how = choose(p, requests, (int)((longest + kTile - 1) / kTile), ((int)p->max_block * (p->heads / p->kv) + 7) / 8);
+    *taken = how.ctas ? way_of(how.log, how.blocks) : 0;
+    return LLMX_OK;
 }
 
 extern "C" int llmx_paged_error(llmx_paged *p, void *stream) {

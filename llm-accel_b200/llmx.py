@@ -186,6 +186,7 @@ def lib():
                                                C.c_size_t, vp, vp, C.c_uint32, vp, C.c_size_t, vp]),
             "llmx_paged_error": (C.c_int, [vp, vp]),
             "llmx_paged_device_bytes": (C.c_uint64, [vp]),
+            "llmx_selftest_paged_way": (C.c_int, [vp, C.c_int, C.c_uint32, C.c_uint32, C.POINTER(C.c_int)]),
             "llmx_upload_vocab": (C.c_int, [vp, vp]),
             "llmx_allreduce_kind": (C.c_int, [vp]),
             "llmx_decode_fuses_o": (C.c_int, [vp]),
@@ -427,6 +428,13 @@ class Paged:
         """Attention of every request's rows over its pages (Task 18's arithmetic)."""
         check(_calls["llmx_paged_attention"](self.h.value, q_ptr, rows, ld_q, offsets_ptr, lengths_ptr, requests, longest, table_ptr,
                                          ld_table, k_ptr, v_ptr, pages, out_ptr, ld_out, stream), "paged_attention")
+
+    def selftest_way(self, way, requests, longest):
+        """For tests: makes attention take a way (-1: by estimate; 0: three launches; 16 i + b: clusters of 2^i CTAs with b
+        column blocks each) and says which one a call of these sizes takes."""
+        taken = C.c_int()
+        check(lib().llmx_selftest_paged_way(self.h, way, requests, longest, C.byref(taken)), "selftest_paged_way")
+        return taken.value
 
     def error(self, stream=None):
         """Waits for the stream; raises when a call met something out of range."""
