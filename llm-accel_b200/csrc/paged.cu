@@ -89,7 +89,7 @@ struct Call {
     int scale8;                   // fm(1/sqrt(dim)), Q8.8
     long long capacity;           // (key head, tile) items
     // workspace
-    Meta *meta;          // [requests]
+    Meta *meta;          // [requests + 1]: the last one's rows say whether some request is void
     uint32_t *score;     // [slot][64 positions][4 column pairs], biased
     uint4 *top;          // [slot][4 blocks of 16 positions]: the maxima of 4 column pairs, biased
     int16_t *tv;         // [slot][8][dim]
@@ -189,6 +189,7 @@ static __device__ int plan(const Call &c, Meta *meta) {
     __shared__ long long part[2][kWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     long long slots = 0, items = 0;  // of the requests before this round's
+    bool some_void = false;
     for (uint32_t first = 0; first < c.requests; first += kThreads) {
         const uint32_t b = first + threadIdx.x;
         Meta m{0, 0, 0, -1};
@@ -200,8 +201,9 @@ static __device__ int plan(const Call &c, Meta *meta) {
                 m.tiles = tiles;
                 i = (long long)c.kv * m.tiles;
                 s = i * ((m.rows * c.group + 7) / 8);
-            } else if (blockIdx.x == 0) {
-                atomicOr(c.error, kErrRequest);
+            } else {
+                some_void = true;
+                if (blockIdx.x == 0) atomicOr(c.error, kErrRequest);
             }
         }
         long long ss = s, ii = i;
@@ -236,11 +238,12 @@ static __device__ int plan(const Call &c, Meta *meta) {
         }
     }
     const bool fits = items <= c.capacity;  // (an item has a slot per column block: they fit as well)
-    __syncthreads();
+    some_void = __syncthreads_or(some_void);
     if (!fits)
         for (uint32_t b = threadIdx.x; b < c.requests; b += kThreads) meta[b] = Meta{0, 0, 0, -1};
     if (blockIdx.x == 0) {
         if (!fits && threadIdx.x == 0) atomicOr(c.error, kErrBudget);
+        if (threadIdx.x == 0) c.meta[c.requests] = Meta{0, 0, 0, some_void};
         for (uint32_t b = threadIdx.x; b < c.requests; b += kThreads) c.meta[b] = meta[b];
     }
     __syncthreads();
@@ -921,6 +924,22 @@ static __device__ __forceinline__ uint32_t request_of(const uint32_t *offsets, u
     return before ? block + 31 - __clz(before) : block;
 }
 
+// The same where offsets may be out of order, which misleads a search: the first request whose row it is, of those that
+// are not void; the number of requests where there is none.  By a whole warp.
+static __device__ __noinline__ uint32_t claimant_of(const uint32_t *offsets, const Meta *meta, uint32_t requests, uint32_t r) {
+    for (uint32_t first = 0; first < requests; first += 32) {
+        const uint32_t b = first + (threadIdx.x & 31);
+        bool mine = false;
+        if (b < requests) {  // (a row in front of the request's is far behind it in 32 bits)
+            const int rows = __ldcg(&meta[b].rows);
+            mine = rows > 0 && r - __ldcg(offsets + b) < (uint32_t)rows;
+        }
+        const uint32_t who = __ballot_sync(0xffffffffu, mine);
+        if (who) return first + (uint32_t)__ffs(who) - 1;
+    }
+    return requests;
+}
+
 constexpr int kShortTiles = 255;  // tiles whose sums stay below 2^31: of values 2^23 each, of probabilities 2^22
 constexpr int kMaxStretches = 3;  // per warp
 constexpr int kAhead = 16;        // tiles loaded at once
@@ -1008,12 +1027,22 @@ __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     const uint32_t row = blockIdx.x / c.heads;
     const int head = (int)(blockIdx.x - row * c.heads);
     const uint32_t b = request_of(c.offsets, c.requests, row);
-    const uint32_t begin = __ldcg(c.offsets + b), behind = __ldcg(c.offsets + b + 1);
-    const int4 m4 = __ldcg(reinterpret_cast<const int4 *>(c.meta + b));
-    const Meta m{m4.x, m4.y, m4.z, m4.w};
+    uint32_t begin = __ldcg(c.offsets + b);
+    const uint32_t behind = __ldcg(c.offsets + b + 1);
+    auto meta_of = [&](uint32_t b) {
+        const int4 m4 = __ldcg(reinterpret_cast<const int4 *>(c.meta + b));
+        return Meta{m4.x, m4.y, m4.z, m4.w};
+    };
+    Meta m = meta_of(b);
     pdl_wait();
     pdl_trigger();
-    if (row < begin || row >= behind || m.rows < 0) return;  // of no request, or of a void one
+    if (row < begin || row >= behind || m.rows < 0) {  // of no request, or of a void one, or not found
+        if (__ldcg(&c.meta[c.requests].rows) == 0) return;
+        const uint32_t other = claimant_of(c.offsets, c.meta, c.requests, row);
+        if (other == c.requests) return;
+        begin = __ldcg(c.offsets + other);
+        m = meta_of(other);
+    }
     const int h = head / c.group, col = (int)(row - begin) * c.group + head - h * c.group;
     const int blocks = (m.rows * c.group + 7) / 8;
     const size_t at = ((size_t)m.slot + (size_t)(h * blocks + (col >> 3)) * m.tiles) * 8 + (col & 7);
@@ -1700,7 +1729,7 @@ extern "C" int llmx_paged_create(int device, uint32_t heads, uint32_t kv_heads, 
         at += (n + 255) / 256 * 256;
         return was;
     };
-    const size_t error_at = place(4), exps_at = place(kExpWords * 4), meta_at = place(max_requests * sizeof(Meta)),
+    const size_t error_at = place(4), exps_at = place(kExpWords * 4), meta_at = place((max_requests + 1) * sizeof(Meta)),
                  score_at = place(slots * 8 * kTile * 2), top_at = place(slots * 64), tv_at = place(slots * 8 * head_dim * 2),
                  fsum_at = place(slots * 64);
     p->bytes = at;

@@ -202,3 +202,30 @@ def test_large_bounds_take_three_launches(llmx, bound):
         p = llmx.Paged(heads, kv, hd, 16, requests, block, bound, 3000)
         assert p.selftest_way(-1, requests, bound) == 0, (heads, kv, hd, requests, block)
         p.close()
+
+
+@gpu
+@pytest.mark.parametrize("requests,split", [(4, 1), (20, 7), (70, 33), (300, 150), (1024, 1000)])
+def test_offsets_out_of_order(llmx, torch, oracle, requests, split):
+    """Two ascending runs of offsets: the request between them, which ends before it starts, is left out and reported, and
+    every other one, whose rows nobody else claims, is served."""
+    rng = np.random.default_rng(requests)
+    plan = [(int(rng.integers(0, 4)), int(rng.integers(1, 90))) for _ in range(requests)]
+    plan[0], plan[split], plan[-1] = (3, 200), (0, 50), (2, 150)
+    c = Case(rng, plan, 4, 2, 16, 8)
+    first, total = int(c.offsets[split]), c.total
+    want = np.concatenate([np.roll(c.want(oracle)[:total], total - first, 0), np.full((2, 4, 16), FILL, np.int16)])
+    d = Device(llmx, torch, c, block=3)
+    d.q[:total] = torch.roll(d.q[:total], total - first, 0)
+    # requests up to split take the rows behind the others'
+    offsets = np.where(np.arange(requests + 1) <= split, c.offsets.astype(np.int64) + total - first, c.offsets.astype(np.int64) - first)
+    assert offsets[split] == total and offsets[split + 1] == 0
+    d.offsets.copy_(torch.from_numpy(offsets.astype(np.int32)))
+    for way in every_way(d):
+        d.out.fill_(FILL)
+        d.call()
+        got = d.result()
+        assert np.array_equal(got, want), (way, report(got, want))
+        with pytest.raises(llmx.LlmxError) as e:
+            d.p.error()
+        assert e.value.code == llmx.ERR_RANGE
