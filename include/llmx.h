@@ -524,7 +524,8 @@ int llmx_paged_destroy(llmx_paged *p);
  *         16-byte aligned
  *   q     device, the rotated queries, rows ld_q elements apart (0 = heads * head_dim, else a
  *         multiple of 8), 16-byte aligned; may be qkv itself with the same stride
- * A row in front of its sequence is left out.  A row whose position has no table entry or rope
+ * A row in front of its sequence is left out, and so may be rows where offsets are out of order (attention reports
+ * those).  A row whose position has no table entry or rope
  * row, or whose page number is outside [0, pages), is left out and reported by
  * llmx_paged_error.  Two rows of a call must not have the same place in the pages. */
 int llmx_paged_append(llmx_paged *p, const int16_t *qkv, uint32_t rows, size_t ld_qkv, const uint32_t *offsets,

@@ -599,8 +599,10 @@ extern "C" int llmx_token_logprobs(const int32_t *logits, size_t ld, uint32_t vo
     c.chunks = (vocab + (aligned ? 0 : 3) + kChunk - 1) / kChunk;
     const uint64_t all = (uint64_t)rows * c.chunks, most = std::min<uint64_t>((uint64_t)sms * 3, kMaxCtas) * kWarps;
     // All warps that there can be at once share the chunks, unless runs of one length leave few of them idle: those make
-    // fewer parts.  (64 rows of 151936: runs of 5 and 6 chunks 16.9 us, of 6 by 11 % fewer warps 18.2; 77 rows of 32003: of
-    // 1 and 2 chunks 9.8 us, of 2 9.2.)
+    // fewer parts.  Measured both ways at 2 to 1000 rows of 32003 to 256000, 5 best (122 calls): the 35 where all share take up to 1.9 us
+    // less that way, all but one (64 rows of 151936 14.8 for 16.0, 128 of 50257 12.2 for 13.2, 64 of 256000 18.4 for 20.2; 77 of 50257
+    // 10.8 for 10.7).  Of the others, those with runs of 2 may be ahead either way by 0.6 us (64 of 32003 9.0 and 9.5 if all shared,
+    // 64 of 50257 10.5 and 9.9); where less than 1/16 is idle, all sharing would be from 1.4 us less to 1.0 more, mostly 0.4 less.
     const uint64_t per = (all + most - 1) / most, even = (all + per - 1) / per;
     c.warps = (uint32_t)(per > 2 && even * 16 < most * 15 ? most : even);
     cudaStream_t s = static_cast<cudaStream_t>(stream);

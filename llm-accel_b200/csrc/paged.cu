@@ -166,7 +166,8 @@ static __device__ __forceinline__ uint32_t pack_sat16(int lo, int hi) {
 static __device__ __forceinline__ int score_of(int total, int scale8) {
     return (int)(((long long)total * scale8 + (128 + (128 << 8))) >> 16);
 }
-// A score with its four saturating banks.
+// A score with its four saturating banks, by one lane: a decode step of 64 requests of up to 2304 positions takes 30 us, 106 where
+// one of 16 query heads has an element of 32.0 or more, 277 where all have.
 static __device__ __noinline__ int score_exact(const int16_t *q, const int16_t *k, int dim, int scale8) {
     long long bank[4] = {0, 0, 0, 0};
     for (int e = 0; e < dim; e++) bank[e & 3] += llmx::qk_prod(q[e], llmx::q412(k[e]));
@@ -1014,7 +1015,8 @@ struct Stretch {
 // so a warp gives what its tiles do to any value that comes in as a few stretches, and the first
 // warp, which starts from 0, puts them together; tiles beyond a warp's kMaxStretches it goes
 // through itself, and a stretch on which something might saturate tile by tile.  Tile by tile throughout
-// it took 224 us of a request of 32768 positions with cold caches, so 18; 64 x 8192: 66, so 21 (34 MB).
+// it took 224 us of a request of 32768 positions with cold caches, so 18; 64 x 8192: 66, so 21 (34 MB).  A text whose positions
+// all weigh the same goes tile by tile: all three launches 44 us for 28 at 32768 positions, 3.7 ms for 0.44 at 2^20.
 template <bool kLong>
 __global__ void __launch_bounds__(32 * kMaxJoinWarps) k_join(const Call c) {
     extern __shared__ __align__(1024) unsigned char dynamic[];
@@ -1610,8 +1612,10 @@ struct Clusters {
 int way_of(int log, int blocks) { return 16 * log + blocks; }
 // Estimates whose order was fitted to measurements of every way (2090 calls: 1 to 64 query heads of 16 to 128, 1 to 128
 // requests of up to 20 to 16000 positions, all as long and of any length, 1 to 8 rows; caches in HBM and in the L2): what is picked
-// was 1.8 % slower than the best way on average (4.9 % by the estimate before, which knew 16 heads of 128 only), 56 % at
-// most (13 requests of 3000, 3 rows: three launches 39, 30 by clusters of 8 that hold all columns).
+// was 1.8 % slower than the best way on average (4.9 % by the estimate before, which knew 16 heads of 128 only), more than
+// 20 % in 45 of them, 56 % at most (24 requests of up to 320, 3 rows: 15.9 us by clusters of 4, 10.2 of 2). 420 of the calls
+// were drawn, from about what perf/more_operators.py draws, and each counted as 4 to 12 of the 1670 of a grid, those of
+// requests of any length least: ragged blocks of 2 to 5 rows are where it picks worst.
 //   Three launches: a start, more per further column block, and the tiles that an SM has.
 //   Clusters: a CTA's tiles, slower for each CTA that shares its SM and each further block; CTAs beyond those that the
 // SMs hold at once (4, or what their memory allows, and a little less for larger clusters) come in later turns, which a
